@@ -53,7 +53,8 @@ constexpr int EPI_WARPS = 4;
 constexpr int STG_BYTES = 4096;   // one epilogue staging buffer (32 rows x 128 bytes)
 constexpr int NUM_THREADS = 192;  // warp 0 TMA, warp 1 MMA + TMEM allocation, warps 2-5 epilogue
 
-enum Kind : int { KIND_BF16 = 0, KIND_MXFP8 = 1, KIND_FP8 = 2 };   // FP8: e4m3 / e5m2 codes, one factor per tensor
+// FP8: e4m3 / e5m2 codes, one factor per tensor.  MXFP4: packed e2m1 codes, one UE8M0 scale per 32 elements.
+enum Kind : int { KIND_BF16 = 0, KIND_MXFP8 = 1, KIND_FP8 = 2, KIND_MXFP4 = 3 };
 
 struct EpiArgs {
   int M, N;
@@ -314,30 +315,40 @@ inline int make_out_tmap(CUtensorMap* tmD, CUtensorMap* tmTail, void* d, int M, 
 // ----------------------------------------------------------------------------------
 // CTA-pair mainloop
 // ----------------------------------------------------------------------------------
-template <int KIND, int BN, int KSUB>
+// GATE (bf16): what becomes of the accumulators besides the plain epilogue.
+//   1  the tile's halves are the gate and the up projection of the same BN / 2 output columns
+//   2  the tile is the gradient of a gated activation
+template <int KIND, int BN, int KSUB, int GATE = 0>
 struct PairCfg {
-  static constexpr bool MX = (KIND == KIND_MXFP8);
+  static constexpr bool F4 = (KIND == KIND_MXFP4);
+  static constexpr bool MX = (KIND == KIND_MXFP8) || F4;
+  static constexpr int KG = F4 ? 2 : 1;           // 128-element scale groups per 128-byte sub-block
+  static constexpr int OUT_N = GATE == 1 ? BN / 2 : BN;        // output columns of a tile
   static constexpr int THREADS = MX ? NUM_THREADS + 128 : NUM_THREADS;   // + 4 scale-forwarding warps
   static constexpr int BNH = BN / 2;              // B rows staged by each CTA
   static constexpr int A_SUB = 128 * 128;         // 128 rows x 128 bytes of K
   static constexpr int B_SUB = BNH * 128;
   static constexpr int B_ATOMS = (BN + 127) / 128;
-  static constexpr int SFA_SUB = MX ? 512 : 0;
-  static constexpr int SFB_SUB = MX ? 512 * B_ATOMS : 0;
+  static constexpr int SFA_SUB = MX ? 512 * KG : 0;
+  static constexpr int SFB_SUB = MX ? 512 * KG * B_ATOMS : 0;
   static constexpr int AB_STAGE = KSUB * (A_SUB + B_SUB);      // operand bytes landed per CTA per stage
   static constexpr int SF_STAGE = KSUB * (SFA_SUB + SFB_SUB);  // scale bytes landed per CTA per stage
   static constexpr int STAGE = AB_STAGE + SF_STAGE;
-  static constexpr int EPI_BYTES = EPI_WARPS * 2 * STG_BYTES;
+  static constexpr int STG_BUFS = GATE != 0 ? 3 : 2;           // staging buffers per epilogue warp
+  static constexpr int EPI_BYTES = EPI_WARPS * STG_BUFS * STG_BYTES;
+  static constexpr int SF_SET_COLS = F4 ? 24 : 16;             // per 128-element group: 4 columns of A scales, 4 per 128 rows of B; padding
   static constexpr int SMEM_BUDGET = 232448 - 1024 - 1024 - 512 - EPI_BYTES;
-  static constexpr int STAGES = SMEM_BUDGET / STAGE;
+  // (MXFP4: the scale sets in tensor memory, one per stage, run out before shared memory does)
+  static constexpr int STAGES = F4 && SMEM_BUDGET / STAGE > (512 - 2 * BN) / (KSUB * SF_SET_COLS) ? (512 - 2 * BN) / (KSUB * SF_SET_COLS)
+                                                                                                  : SMEM_BUDGET / STAGE;
   static constexpr int SMEM = STAGES * STAGE + 1024 + 1024 + 512 + EPI_BYTES;
   static constexpr int SF_COL = 2 * BN;           // first TMEM column of the scale area
-  static constexpr int SF_SET_COLS = 16;          // 4 columns of A scales, 4 per 128 rows of B, padding
   static constexpr int SF_SETS = STAGES * KSUB;   // one scale set per staged k block
   static constexpr int USED_COLS = 2 * BN + (MX ? SF_SETS * SF_SET_COLS : 0);
   static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
   static constexpr int NUM_BARS = 2 * STAGES + 4 + (MX ? 2 * STAGES : 0);
-  static_assert(4 + 4 * B_ATOMS <= SF_SET_COLS, "scale set too narrow");
+  static_assert(!MX || KG * (4 + 4 * B_ATOMS) <= SF_SET_COLS, "scale set too narrow");
+  static_assert(GATE == 0 || KIND == KIND_BF16, "gated epilogues belong to the bf16 kind");
   static_assert(USED_COLS <= 512, "accumulators and scale sets exceed tensor memory");
   static_assert(B_SUB % 1024 == 0, "B half tile must be whole swizzle atoms");
   static_assert(STAGES >= 2, "not enough shared memory for two stages");
@@ -452,6 +463,16 @@ struct TpReduce {
 template <int NOWN>
 struct OwnerMaps { CUtensorMap m[NOWN]; };
 
+// Gated activation in the epilogue (GATE 1: forward, GATE 2: its gradient).
+struct GateArgs {
+  int act;                        // 0: SiLU, 1: GELU (tanh form)
+  int F;                          // GATE 1: rows of the gate half of the stacked weight
+  int want_gu;                    // GATE 1: gate and up go to memory too
+  int want_a;                     // GATE 2: the activation's product is written again
+  const __nv_bfloat16* gu;        // GATE 2: [M, 2F], gate columns first
+  long long ldgu;
+};
+
 struct PairParams {
   GroupArgs grp;
   SplitArgs split;
@@ -463,6 +484,7 @@ struct PairParams {
   int* status;
   TpGather tp;
   TpReduce rs;
+  GateArgs gate;
 };
 
 // Tile t of the launch: its row / column tile, expert and range of k stages (kb_elems = contraction
@@ -511,18 +533,116 @@ B200_DEVICE TileInfo tile_info(int t, int num_m, int num_n, int num_kb, int kb_e
   return ti;
 }
 
-template <int KIND, int BN, int KSUB, int NOWN = 1>
-__global__ void __launch_bounds__(PairCfg<KIND, BN, KSUB>::THREADS, 1)
+// Gated activation of one value, and its slope.  act 0: SiLU; 1: GELU in its tanh form, as a sigmoid: 0.5 x (1 + tanh z) = x sigmoid(2 z).
+B200_DEVICE float gate_act(float g, int act) {
+  return g * sigmoid(act == 0 ? g : 1.5957691216f * g * fmaf(0.044715f * g, g, 1.f));
+}
+B200_DEVICE void gate_act_grad(float g, int act, float& value, float& slope) {
+  if (act == 0) {
+    const float s = sigmoid(g);
+    value = g * s;
+    slope = s * (1.f + g * (1.f - s));
+  } else {
+    const float z = 1.5957691216f * g * fmaf(0.044715f * g, g, 1.f), s = sigmoid(z);
+    value = g * s;
+    // (s (1 - s) vanishes long before the cubic's slope overflows; inf * 0 is kept out)
+    const float t = s * (1.f - s);
+    slope = s + (t > 0.f ? g * t * 1.5957691216f * fmaf(3.f * 0.044715f * g, g, 1.f) : 0.f);
+  }
+}
+
+// 32 rows x 32 bf16 columns from registers to a 2 KB staging buffer (64-byte swizzle: chunk ^= (row / 2) % 4).
+B200_DEVICE void stage_32x32(uint8_t* buf, int lane, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+
+// Epilogue of the gated kernels: this warp's 32 rows, 32 output columns at a time.
+//   GATE 1  gate = columns [0, BN / 2) of the accumulator, up = [BN / 2, BN); a = act(gate) * up, made in fp32 and rounded once, leaves
+//           through tmA, gate and up (bf16: what the backward keeps) through tmG and tmU
+//   GATE 2  da = the accumulator, not rounded; d gate and d up leave through tmG and tmU, the product a of the kept projections (which the
+//           gradient of the down projection needs) through tmA
+// The three maps have 32 x 32 boxes with the 64-byte swizzle; each clips at its own M x F.  Two sets of three 2 KB buffers per warp.
+template <int BN, int GATE>
+B200_DEVICE void gate_drain(const CUtensorMap* tmA, const CUtensorMap* tmG, const CUtensorMap* tmU, const PairParams& p, uint32_t t_row,
+                            int row0, int n0, uint8_t* stg, int lane) {
+  constexpr int OUT_N = GATE == 1 ? BN / 2 : BN;
+  const bool w_gu = GATE == 2 || p.gate.want_gu, w_a = GATE == 1 || p.gate.want_a;
+  const int act = p.gate.act, row = row0 + lane;
+#pragma unroll 1
+  for (int c = 0; c < OUT_N / 32; ++c) {
+    const int col0 = n0 + c * 32;
+    uint8_t* buf = stg + (c & 1) * 6144;
+    uint32_t wa[16], wg[16], wu[16];
+    if constexpr (GATE == 1) {
+      uint32_t g[32], u[32];
+      tmem_ld_32x32b_x32(t_row + c * 32, g);
+      tmem_ld_32x32b_x32(t_row + OUT_N + c * 32, u);
+      tc_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        wg[i] = pack_bf16x2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+        wu[i] = pack_bf16x2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+        wa[i] = pack_bf16x2(gate_act(__uint_as_float(g[2 * i]), act) * __uint_as_float(u[2 * i]),
+                            gate_act(__uint_as_float(g[2 * i + 1]), act) * __uint_as_float(u[2 * i + 1]));
+      }
+    } else {
+      // (F is a multiple of 8: a 16-byte vector is in range or past the end as a whole)
+      const bool live = row < p.M;
+      const __nv_bfloat16* src = p.gate.gu + (long long)row * p.gate.ldgu + col0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = live && col0 + j * 8 < p.N;
+        const uint4 a = in ? *reinterpret_cast<const uint4*>(src + j * 8) : make_uint4(0u, 0u, 0u, 0u);
+        const uint4 b = in ? *reinterpret_cast<const uint4*>(src + p.N + j * 8) : make_uint4(0u, 0u, 0u, 0u);
+        wg[4 * j] = a.x; wg[4 * j + 1] = a.y; wg[4 * j + 2] = a.z; wg[4 * j + 3] = a.w;
+        wu[4 * j] = b.x; wu[4 * j + 1] = b.y; wu[4 * j + 2] = b.z; wu[4 * j + 3] = b.w;
+      }
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(t_row + c * 32, r);
+      tc_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 gf = unpack_bf16x2(wg[i]), uf = unpack_bf16x2(wu[i]);
+        const float2 d = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        float v0, s0, v1, s1;
+        gate_act_grad(gf.x, act, v0, s0);
+        gate_act_grad(gf.y, act, v1, s1);
+        wg[i] = pack_bf16x2(d.x * uf.x * s0, d.y * uf.y * s1);
+        wu[i] = pack_bf16x2(d.x * v0, d.y * v1);
+        wa[i] = pack_bf16x2(v0 * uf.x, v1 * uf.y);
+      }
+    }
+    if (lane == 0) tma_store_wait_read<1>();        // the stores of the chunk before last have left this set
+    __syncwarp();
+    if (w_a) stage_32x32(buf, lane, wa);
+    if (w_gu) { stage_32x32(buf + 2048, lane, wg); stage_32x32(buf + 4096, lane, wu); }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (col0 < p.N && row0 < p.M) {
+        if (w_a) tma_store_2d(tmA, buf, col0, row0);
+        if (w_gu) { tma_store_2d(tmG, buf + 2048, col0, row0); tma_store_2d(tmU, buf + 4096, col0, row0); }
+      }
+      tma_store_commit();
+    }
+  }
+}
+
+template <int KIND, int BN, int KSUB, int NOWN = 1, int GATE = 0>
+__global__ void __launch_bounds__(PairCfg<KIND, BN, KSUB, GATE>::THREADS, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmSFA, const __grid_constant__ CUtensorMap tmSFB,
                  const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmDt,
                  const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmWt,
                  const __grid_constant__ PairParams p, const __grid_constant__ OwnerMaps<NOWN> om) {
   b200::begin_kernel();
-  using C = PairCfg<KIND, BN, KSUB>;
+  using C = PairCfg<KIND, BN, KSUB, GATE>;
   constexpr bool MX = C::MX;
   constexpr bool F8 = (KIND == KIND_FP8);
-  constexpr int KB_ELEMS = (MX || F8) ? 128 : 64; // contraction elements per 128-byte sub-block
+  constexpr bool F4 = C::F4;
+  constexpr int KB_ELEMS = F4 ? 256 : (MX || F8) ? 128 : 64; // contraction elements per 128-byte sub-block
   constexpr int UMMA_K_BYTES = 32;                // one MMA consumes 32 bytes of K per row
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -552,12 +672,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   const int pair_id = (int)(blockIdx.x >> 1) - n_aux;
   const int num_pairs = (int)(gridDim.x >> 1) - n_aux;
   const int num_m = (p.M + 255) / 256;
-  const int num_n = (p.N + BN - 1) / BN;
+  const int num_n = (p.N + C::OUT_N - 1) / C::OUT_N;
   // work units: whole tiles, then the slices of the split tiles
   const int num_tiles = p.split.rem > 0 ? p.split.first + p.split.rem * p.split.S
                                         : (p.grp.mode == 2 ? p.grp.E : 1) * num_m * num_n;
   const int num_kb = (p.K + KB_ELEMS * KSUB - 1) / (KB_ELEMS * KSUB);
-  const int num_kb128 = (p.K + KB_ELEMS - 1) / KB_ELEMS;   // 128-byte K blocks (scale groups of the MX layout)
+  const int num_kb128 = F4 ? (p.K + 127) / 128 : (p.K + KB_ELEMS - 1) / KB_ELEMS;   // 128-byte K blocks (scale groups of the MX layout)
 
   if (threadIdx.x == 0) {
     if (!is_aux) {                                // a copy CTA sets up its own barriers in the same words
@@ -582,7 +702,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 
   if (is_aux) {
     // ------------------------------ copy CTAs of the all-gather ------------------------------
-    if constexpr (!MX) {                          // (the gathering launchers use the bf16 and per-tensor FP8 kinds)
+    if constexpr (!MX && GATE == 0) {             // (the gathering launchers use the bf16 and per-tensor FP8 kinds)
       static_assert(tpcopy::COPY_STAGES * tpcopy::COPY_PIECE <= C::STAGES * C::STAGE, "copy ring must fit the operand stages");
       if (p.rs.on) tpreduce::reduce_cta(p.rs, num_n, smem, bars, C::THREADS);
       else if (p.tp.copy_mode == 1) tpcopy::copy_cta_push(p.tp, (int)blockIdx.x, 2 * n_aux, C::THREADS);
@@ -604,7 +724,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int m0 = mb * 256 + (int)rank * 128;          // this CTA's rows of A
         const bool b_mn = !MX && !F8 && p.b_mn_major;
         // this CTA's rows of B, and where the expert's contraction starts in an MN-major stack
-        const int n0 = ti.nb * BN + (int)rank * C::BNH + (p.grp.mode == 1 && !b_mn ? ti.e * p.N : 0);
+        // (gated forward: the leader stages gate rows, its partner the up rows of the same output columns)
+        const int n0 = GATE == 1 ? ti.nb * C::BNH + (int)rank * p.gate.F
+                                 : ti.nb * BN + (int)rank * C::BNH + (p.grp.mode == 1 && !b_mn ? ti.e * p.N : 0);
         const int kb_off = (p.grp.mode == 1 && b_mn) ? ti.e * p.K : 0;
         if (p.tp.on) {
           const int c = (mb * 256) / p.tp.rows_per;             // rank block that holds this tile's rows of A
@@ -628,7 +750,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             // (consecutive k groups of a tile are adjacent in the atom layout): A's atoms of this CTA's 128
             // rows, B's atoms of the whole N tile (each CTA's tensor core scales all N columns of its rows)
             mbar_expect_tx(&sffull[stage], C::SF_STAGE);
-            const int kg = kb * KSUB;
+            const int kg = kb * KSUB * C::KG;
             tma_load_2d(sSFA + stage * KSUB * C::SFA_SUB, &tmSFA, &sffull[stage], 0, (mb * 2 + (int)rank) * num_kb128 + kg);
             tma_load_2d(sSFB + stage * KSUB * C::SFB_SUB, &tmSFB, &sffull[stage], 0, (nb * num_kb128 + kg) * C::B_ATOMS);
           }
@@ -636,7 +758,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           for (int s = 0; s < KSUB; ++s) {
             uint8_t* a_dst = sA + (stage * KSUB + s) * C::A_SUB;
             uint8_t* b_dst = sB + (stage * KSUB + s) * C::B_SUB;
-            const int k0 = (kb * KSUB + s) * KB_ELEMS;
+            const int k0 = (kb * KSUB + s) * (F4 ? KB_ELEMS / 2 : KB_ELEMS);   // (MXFP4: in bytes, two elements each)
             if (MX || F8 || !p.a_mn_major) {
               tma_load_2d_pair(a_dst, &tmA, bar, k0, m0);
             } else {
@@ -660,7 +782,8 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     // uniform registers and the descriptors advance by an addition.  (One lane of a divergent warp that rebuilt them
     // needed more cycles per instruction than a block-scaled one runs.)
     if (rank == 0) {
-      const uint32_t idesc0 = MX ? umma_idesc_mx(0, 0, 0, 0, 256, BN)
+      const uint32_t idesc0 = F4 ? umma_idesc_mx(1, 1, 0, 0, 256, BN)     // e2m1 has format code 1 in kind::mxf4
+                              : MX ? umma_idesc_mx(0, 0, 0, 0, 256, BN)
                               : F8 ? umma_idesc(p.a_fmt, p.b_fmt, 0, 0, 256, BN)
                                    : umma_idesc(1, 1, p.a_mn_major, p.b_mn_major, 256, BN);
       const bool a_mn = !MX && !F8 && p.a_mn_major, b_mn = !MX && !F8 && p.b_mn_major;
@@ -672,7 +795,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       // An odd number of 128-byte blocks leaves nothing but padding in the second half of the last stage of two (a contraction of
       // 2880 block-scaled elements is 22.5 blocks: 23 are multiplied, not 24).  Its operands arrive as zeros, but its scales are
       // whatever follows in the buffer, and zero times a NaN scale is NaN: it must not be multiplied.
-      const bool odd_tail = KSUB == 2 && p.grp.mode != 2 && (num_kb128 & 1);
+      const bool odd_tail = !F4 && KSUB == 2 && p.grp.mode != 2 && (num_kb128 & 1);
       int stage = 0; uint32_t phase = 0;
       int it = 0;
       bool ok = true;
@@ -699,7 +822,15 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) {
                 const uint32_t accum = (kb > 0 || s > 0 || kk > 0) ? 1u : 0u;
-                if (MX) {
+                if constexpr (F4) {
+                  // 64 elements an instruction, two scale bytes of a 32-bit scale column each: ids 0 and 2.  What starts past K is
+                  // left out, for the reason given at odd_tail (inside the last 64 elements the scale bytes past K are zero).
+                  if (((ti.kb0 + kb) * KSUB + s) * KB_ELEMS + kk * 64 < p.K) {
+                    const uint32_t id = (uint32_t)(kk & 1) * 2;
+                    tc_mma_mxf4_ss_pair(d_tmem, ad + kk * a_kstep, bd + kk * b_kstep, idesc0 | (id << 29) | (id << 4), accum,
+                                        t_sfa + 4 * (kk >> 1), t_sfa + 8 + 8 * (kk >> 1));
+                  }
+                } else if (MX) {
                   // scale byte kk of every 32-bit scale column: a_sf_id bits [29,31), b_sf_id bits [4,6)
                   tc_mma_mxf8_ss_pair(d_tmem, ad + kk * a_kstep, bd + kk * b_kstep, idesc0 | ((uint32_t)kk << 29) | ((uint32_t)kk << 4),
                                       accum, t_sfa, t_sfa + 4);
@@ -721,7 +852,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   } else if (warp < 2 + EPI_WARPS) {
     // ------------------------------ epilogue (both CTAs) ------------------------------
     const int q = warp & 3;                       // TMEM lane quarter owned by this warp
-    uint8_t* stg = sE + (warp - 2) * 2 * STG_BYTES;
+    uint8_t* stg = sE + (warp - 2) * C::STG_BUFS * STG_BYTES;
     const uint32_t tempty_leader0 = mapa_u32(smem_u32(&tempty[0]), 0);
     const uint32_t tempty_leader1 = mapa_u32(smem_u32(&tempty[1]), 0);
     int buf = 0;
@@ -742,7 +873,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       if (!warp_wait(&tfull[acc], acc_phase, abort_flag, p.status, 330)) { ok = false; break; }
       tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t(q * 32) << 16) + acc * BN;
-      if (p.rs.on) {
+      if constexpr (GATE != 0) {
+        gate_drain<BN, GATE>(&tmD, &tmSFA, &tmSFB, p, t_row, ti.mb * 256 + (int)rank * 128 + q * 32, ti.nb * C::OUT_N, stg, lane);
+      } else if (p.rs.on) {
         // the tile goes into the owner's staging slot of this rank, through the owner's tensor map; then the owner's
         // counter of these 128 rows learns that this warp's part has landed
         const int m0 = ti.mb * 256 + (int)rank * 128;
@@ -796,6 +929,27 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         tc_fence_after();
 #pragma unroll
         for (int s = 0; s < KSUB; ++s) {
+          if constexpr (F4) {
+            // both 128-element groups of the sub-block: A's four columns each, then up to eight columns of B's each
+            uint32_t r[16], rb[8];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const uint4 a4 = *reinterpret_cast<const uint4*>(sSFA + (stage * KSUB + s) * C::SFA_SUB + g * 512 + lane * 16);
+              r[4 * g] = a4.x; r[4 * g + 1] = a4.y; r[4 * g + 2] = a4.z; r[4 * g + 3] = a4.w;
+#pragma unroll
+              for (int a = 0; a < 2; ++a) {
+                uint4 b4 = make_uint4(0u, 0u, 0u, 0u);
+                if (a < C::B_ATOMS)
+                  b4 = *reinterpret_cast<const uint4*>(sSFB + (stage * KSUB + s) * C::SFB_SUB + (g * C::B_ATOMS + a) * 512 + lane * 16);
+                uint32_t* to = g == 0 ? r + 8 + 4 * a : rb + 4 * a;
+                to[0] = b4.x; to[1] = b4.y; to[2] = b4.z; to[3] = b4.w;
+              }
+            }
+            const uint32_t set = lane_base + (uint32_t)(stage * KSUB + s) * C::SF_SET_COLS;
+            tmem_st_32x32b_x16(set, r);
+            tmem_st_32x32b_x8(set + 16, rb);
+            continue;
+          }
           uint32_t r[16];
           const uint4 a4 = *reinterpret_cast<const uint4*>(sSFA + (stage * KSUB + s) * C::SFA_SUB + lane * 16);
           r[0] = a4.x; r[1] = a4.y; r[2] = a4.z; r[3] = a4.w;
@@ -897,9 +1051,9 @@ split_finish_kernel(const float* __restrict__ ws, SplitArgs sp, int num_m, int n
   }
 }
 
-template <int KIND, int BN, int KSUB>
+template <int KIND, int BN, int KSUB, int GATE = 0>
 void pair_launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, cudaStream_t stream) {
-  using C = PairCfg<KIND, BN, KSUB>;
+  using C = PairCfg<KIND, BN, KSUB, GATE>;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.blockDim = dim3(C::THREADS, 1, 1);
@@ -910,19 +1064,19 @@ void pair_launch_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attr, cuda
 }
 
 // CTA pairs of this kernel that can be resident at once on the current device (cached); 0 or a failure code in `rc`.
-template <int KIND, int BN, int KSUB, int NOWN = 1>
+template <int KIND, int BN, int KSUB, int NOWN = 1, int GATE = 0>
 int pair_capacity(const char* what, int& rc) {
-  using C = PairCfg<KIND, BN, KSUB>;
+  using C = PairCfg<KIND, BN, KSUB, GATE>;
   static int max_pairs[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
   dev &= 63;
   rc = 0;
   if (max_pairs[dev] == 0) {
-    auto kern = gemm_pair_kernel<KIND, BN, KSUB, NOWN>;
+    auto kern = gemm_pair_kernel<KIND, BN, KSUB, NOWN, GATE>;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
-    pair_launch_config<KIND, BN, KSUB>(cfg, attr, nullptr);
+    pair_launch_config<KIND, BN, KSUB, GATE>(cfg, attr, nullptr);
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) {
       cudaGetLastError();
@@ -949,9 +1103,9 @@ template <int KIND, int BN, int KSUB>
 SplitArgs pair_split(int M, int N, int K, int& rc) {
   const int P = pair_capacity<KIND, BN, KSUB>("split", rc);
   const int tiles = ((M + 255) / 256) * ((N + BN - 1) / BN);
-  const int kb = (KIND == KIND_BF16 ? 64 : 128) * KSUB, num_kb = (K + kb - 1) / kb;
+  const int kb = (KIND == KIND_BF16 ? 64 : KIND == KIND_MXFP4 ? 256 : 128) * KSUB, num_kb = (K + kb - 1) / kb;
   if (rc || P <= 0) return {tiles, 0, 1, num_kb};
-  const double stage_us = 256.0 * BN * kb * 2 / (KIND == KIND_BF16 ? 19.0e6 : 34.0e6);
+  const double stage_us = 256.0 * BN * kb * 2 / (KIND == KIND_BF16 ? 19.0e6 : KIND == KIND_MXFP4 ? 54.0e6 : 34.0e6);
   return split_plan(tiles, num_kb, stage_us, 256.0 * BN * 4, P);
 }
 template <int BN>
@@ -961,23 +1115,24 @@ long long split_bytes(const SplitArgs& s) { return (long long)s.rem * (s.rem > 0
 // not exceed that: a pair that waits for SMs would start only after a resident pair finished all its
 // tiles).  With a workspace that is large enough (pair_split, split_bytes) the last wave is split along K; `d`, `ldd`:
 // the output the second launch finishes.  Returns 0, or a failure code with message.
-template <int KIND, int BN, int KSUB, int NOWN = 1>
+template <int KIND, int BN, int KSUB, int NOWN = 1, int GATE = 0>
 int launch_pair(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmSFA, const CUtensorMap& tmSFB,
                 const CUtensorMap& tmD, const CUtensorMap& tmDt, const PairParams& p_in, cudaStream_t stream,
                 const char* what, const OwnerMaps<NOWN>* owners = nullptr, float* ws = nullptr, long long ws_bytes = 0,
                 void* d = nullptr, long long ldd = 0) {
   PairParams p = p_in;
-  auto kern = gemm_pair_kernel<KIND, BN, KSUB, NOWN>;
+  auto kern = gemm_pair_kernel<KIND, BN, KSUB, NOWN, GATE>;
   static const OwnerMaps<NOWN> no_owners = {};
   const OwnerMaps<NOWN>& om = owners != nullptr ? *owners : no_owners;
   int rc = 0;
-  const int max_pairs = pair_capacity<KIND, BN, KSUB, NOWN>(what, rc);
+  const int max_pairs = pair_capacity<KIND, BN, KSUB, NOWN, GATE>(what, rc);
   if (rc) return rc;
-  const int num_m = (p.M + 255) / 256, num_n = (p.N + BN - 1) / BN;
+  constexpr int OUT_N = PairCfg<KIND, BN, KSUB, GATE>::OUT_N;
+  const int num_m = (p.M + 255) / 256, num_n = (p.N + OUT_N - 1) / OUT_N;
   const int tiles = (p.grp.mode == 2 ? p.grp.E : 1) * num_m * num_n;
   p.split = SplitArgs{tiles, 0, 1, 0};
   CUtensorMap tmW = tmD, tmWt = tmDt;
-  if (ws != nullptr && d != nullptr && p.grp.mode == 0 && !p.tp.on && !p.rs.on) {
+  if (GATE == 0 && ws != nullptr && d != nullptr && p.grp.mode == 0 && !p.tp.on && !p.rs.on) {
     const SplitArgs sp = pair_split<KIND, BN, KSUB>(p.M, p.N, p.K, rc);
     if (rc) return rc;
     if (sp.rem > 0 && ws_bytes >= split_bytes<BN>(sp)) {
@@ -993,7 +1148,7 @@ int launch_pair(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMa
   const int pairs = (units < room ? units : room) + n_aux;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  pair_launch_config<KIND, BN, KSUB>(cfg, attr, stream);
+  pair_launch_config<KIND, BN, KSUB, GATE>(cfg, attr, stream);
   cfg.gridDim = dim3(2 * pairs, 1, 1);
   if (!p.tp.on && !p.rs.on) {     // a launch that waits for other GPUs is ordered as before
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;

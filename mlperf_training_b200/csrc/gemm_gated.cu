@@ -1,0 +1,72 @@
+// Gated feed-forward block in bf16, on the CTA-pair mainloop of gemm_core.cuh:
+//
+//   b200_gemm_gated       a = act(x Wg^T) * (x Wu^T), optionally with the projections themselves (gu, kept for the backward), in one launch
+//   b200_gemm_gated_grad  da = dy Wd, then d gate = da u act'(g), d up = da act(g) and a again, in one launch
+//
+// W = [Wg; Wu] is the stacked [2F, D] weight of the two projections as the model keeps it.  A 256-row tile of 128 output columns runs as one
+// 256 x 256 tile: the leader CTA stages the 128 gate rows, its partner the 128 up rows of the same columns, so that the gate lands in the
+// accumulator's first half and the up projection in its second, and an epilogue warp has both at hand.  Against a GEMM and a SwiGLU kernel the
+// projections are not read again: 4 bytes of T F less each way, and forward without a backward writes 2 bytes instead of 6.
+#include "common.cuh"
+#include "gemm_core.cuh"
+#include "runtime.h"
+
+namespace {
+int check(const char* what, const void* p, long long ld) {
+  return (((uintptr_t)p & 15) != 0 || ld % 8 != 0) ? b200::fail(861, "%s: operands must be 16-byte aligned, pitches multiples of 8", what) : 0;
+}
+}  // namespace
+
+// x [M, K], w [2F, K], a [M, F], gu [M, 2F] or null; pitches in elements, multiples of 8; F and K multiples of 8.  act: 0 SiLU, 1 GELU (tanh).
+B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, int M, int F, int K, long long ldx, long long ldw,
+                             long long lda, long long ldgu, int act, void* stream) {
+  using namespace gemmcore;
+  if (M <= 0 || F <= 0 || K <= 0) return b200::fail(860, "gemm_gated: empty problem %d x 2 x %d x %d", M, F, K);
+  if (F % 8 != 0 || K % 8 != 0) return b200::fail(862, "gemm_gated: F=%d and K=%d must be multiples of 8", F, K);
+  int r;
+  if ((r = check("gemm_gated", x, ldx)) || (r = check("gemm_gated", w, ldw)) || (r = check("gemm_gated", a, lda)) ||
+      (gu != nullptr && (r = check("gemm_gated", gu, ldgu))))
+    return r;
+  CUtensorMap tmX, tmW, tmA, tmG, tmU;
+  if ((r = b200::make_tmap_2d(&tmX, b200::DT_BF16, x, K, M, ldx * 2, 64, 128, b200::SWZ_128))) return r;
+  if ((r = b200::make_tmap_2d(&tmW, b200::DT_BF16, w, K, 2LL * F, ldw * 2, 64, 128, b200::SWZ_128))) return r;
+  if ((r = b200::make_tmap_2d(&tmA, b200::DT_BF16, a, F, M, lda * 2, 32, 32, b200::SWZ_64))) return r;
+  tmG = tmU = tmA;
+  if (gu != nullptr) {
+    if ((r = b200::make_tmap_2d(&tmG, b200::DT_BF16, gu, F, M, ldgu * 2, 32, 32, b200::SWZ_64))) return r;
+    if ((r = b200::make_tmap_2d(&tmU, b200::DT_BF16, (uint8_t*)gu + 2LL * F, F, M, ldgu * 2, 32, 32, b200::SWZ_64))) return r;
+  }
+  PairParams p = {};
+  p.M = M; p.N = F; p.K = K;
+  p.group_m = raster_group_m() > 1 ? raster_group_m() / 2 : 1;
+  p.gate.act = act; p.gate.F = F; p.gate.want_gu = gu != nullptr;
+  p.status = b200::status_ptr();
+  return launch_pair<KIND_BF16, 256, 1, 1, 1>(tmX, tmW, tmG, tmU, tmA, tmA, p, (cudaStream_t)stream, "gemm_gated");
+}
+
+// dy [M, K], wd [K, F] (the down projection's weight as it is), gu [M, 2F]; dgu [M, 2F], a [M, F] or null.
+B200_API int b200_gemm_gated_grad(const void* dy, const void* wd, const void* gu, void* dgu, void* a, int M, int F, int K, long long lddy,
+                                  long long ldwd, long long ldgu, long long lddgu, long long lda, int act, void* stream) {
+  using namespace gemmcore;
+  if (M <= 0 || F <= 0 || K <= 0) return b200::fail(863, "gemm_gated_grad: empty problem %d x %d x %d", M, F, K);
+  if (F % 8 != 0 || K % 8 != 0) return b200::fail(864, "gemm_gated_grad: F=%d and K=%d must be multiples of 8", F, K);
+  int r;
+  if ((r = check("gemm_gated_grad", dy, lddy)) || (r = check("gemm_gated_grad", wd, ldwd)) || (r = check("gemm_gated_grad", gu, ldgu)) ||
+      (r = check("gemm_gated_grad", dgu, lddgu)) || (a != nullptr && (r = check("gemm_gated_grad", a, lda))))
+    return r;
+  CUtensorMap tmY, tmW, tmA, tmG, tmU;
+  if ((r = b200::make_tmap_2d(&tmY, b200::DT_BF16, dy, K, M, lddy * 2, 64, 128, b200::SWZ_128))) return r;
+  if ((r = b200::make_tmap_2d(&tmW, b200::DT_BF16, wd, F, K, ldwd * 2, 64, 64, b200::SWZ_128))) return r;
+  if ((r = b200::make_tmap_2d(&tmG, b200::DT_BF16, dgu, F, M, lddgu * 2, 32, 32, b200::SWZ_64))) return r;
+  if ((r = b200::make_tmap_2d(&tmU, b200::DT_BF16, (uint8_t*)dgu + 2LL * F, F, M, lddgu * 2, 32, 32, b200::SWZ_64))) return r;
+  tmA = tmG;
+  if (a != nullptr && (r = b200::make_tmap_2d(&tmA, b200::DT_BF16, a, F, M, lda * 2, 32, 32, b200::SWZ_64))) return r;
+  PairParams p = {};
+  p.M = M; p.N = F; p.K = K;
+  p.b_mn_major = 1;
+  p.group_m = raster_group_m() > 1 ? raster_group_m() / 2 : 1;
+  p.gate.act = act; p.gate.F = F; p.gate.want_a = a != nullptr;
+  p.gate.gu = (const __nv_bfloat16*)gu; p.gate.ldgu = ldgu;
+  p.status = b200::status_ptr();
+  return launch_pair<KIND_BF16, 256, 1, 1, 2>(tmY, tmW, tmG, tmU, tmA, tmA, p, (cudaStream_t)stream, "gemm_gated_grad");
+}

@@ -1,0 +1,281 @@
+// Micro-scaled quantisation of values in registers: blocks of 32 values with one UE8M0 scale, elements e4m3 (8 bits) or e2m1 (4 bits,
+// two per byte, the even element in the low half).
+//
+// Scale: the smallest power of two s with amax / s <= vmax (448 = 1.75 * 2^8, 6 = 1.5 * 2^2), biased by 127; at least 1 (2^-126) where amax
+// is not zero, 0 where it is.  255 (NaN) for a block that holds an infinity or a NaN: e2m1 has neither, and with any other scale the value
+// would come back as an ordinary number.  No element saturates: amax / s <= vmax.
+// Magnitudes are compared as integers (their fp32 bits less the sign), in which a NaN is above infinity and both above every number.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace mxq {
+
+enum Fmt : int { E4M3 = 0, E2M1 = 1 };
+
+template <int FMT>
+B200_DEVICE uint32_t e8m0(uint32_t amax_bits) {
+  // exponent of amax less that of vmax, one more where the fraction exceeds vmax's (the addition carries)
+  const int e = (int)((amax_bits + (FMT == E2M1 ? 0x3fffffu : 0x1fffffu)) >> 23) - (FMT == E2M1 ? 2 : 8);
+  return amax_bits >= 0x7f800000u ? 255u : amax_bits == 0u ? 0u : (uint32_t)max(e, 1);
+}
+// 2^(127 - e) for e <= 253 (no finite block has more)
+B200_DEVICE float inv_scale(uint32_t e) { return __uint_as_float((254u - min(e, 254u)) << 23); }
+B200_DEVICE uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+B200_DEVICE uint32_t pack4_e4m3(float a, float b, float c, float d) {
+  const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+// eight values to eight e2m1 codes, round to nearest even
+B200_DEVICE uint32_t pack8_e2m1(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+// y (|y| <= 6) to a value of e2m1: |y| / quantum + (u + 1/2) / 256 rounded down, u a random byte.  The expectation over u is y to within
+// 1/512 of a quantum, and a value of the format stays as it is.
+B200_DEVICE float round_stochastic(float y, uint32_t u) {
+  const uint32_t q = max(abs_bits(y) & 0x7f800000u, 0x3f800000u) - 0x00800000u;    // quantum: 0.5 below 2, 1 below 4, 2
+  const float t = floorf(fabsf(y) * __uint_as_float(0x7f000000u - q) + ((float)u + 0.5f) * 0.00390625f);
+  return copysignf(fminf(t * __uint_as_float(q), 6.f), y);
+}
+
+// byte offset of scale (row r of the operand, scale column kc) in the atom layout the block-scaled GEMMs read (quant_mxfp8.cu)
+B200_DEVICE long long sf_offset(long long r, int kc, int tile_rows, int atoms_per_tile, long long k_groups) {
+  const long long tile = r / tile_rows;
+  const int rr = (int)(r - tile * tile_rows);
+  const int atom = rr >> 7, ra = rr & 127;
+  return ((tile * k_groups + (kc >> 2)) * atoms_per_tile + atom) * 512 + (ra & 31) * 16 + (ra >> 5) * 4 + (kc & 3);
+}
+
+// Eight values of a 32-block whose other values are in the three neighbouring lanes (lane / 4 is the block): codes in q (e2m1: q.x),
+// returns the scale byte.  noise: eight random bytes, null for round to nearest.
+template <int FMT>
+B200_DEVICE uint32_t quant_row8(const float (&v)[8], const uint2* noise, uint2& q) {
+  uint32_t m = abs_bits(v[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = max(m, abs_bits(v[i]));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const uint32_t e = e8m0<FMT>(m);
+  const float inv = inv_scale(e);
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = v[i] * inv;
+  if constexpr (FMT == E4M3) {
+    q = make_uint2(pack4_e4m3(y[0], y[1], y[2], y[3]), pack4_e4m3(y[4], y[5], y[6], y[7]));
+  } else {
+    if (noise != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = round_stochastic(y[i], ((i < 4 ? noise->x : noise->y) >> (8 * (i & 3))) & 0xffu);
+    }
+    q = make_uint2(pack8_e2m1(y), 0u);
+  }
+  return e;
+}
+
+// Sixteen rows of one column; the other half of the 32-block is in the neighbouring lane.  Codes in q (e4m3: 16 bytes, e2m1: q.x, q.y).
+template <int FMT>
+B200_DEVICE uint32_t quant_col16(float (&v)[16], const uint32_t* noise4, uint4& q) {
+  uint32_t m = abs_bits(v[0]);
+#pragma unroll
+  for (int i = 1; i < 16; ++i) m = max(m, abs_bits(v[i]));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  const uint32_t e = e8m0<FMT>(m);
+  const float inv = inv_scale(e);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] *= inv;
+  if constexpr (FMT == E4M3) {
+    q = make_uint4(pack4_e4m3(v[0], v[1], v[2], v[3]), pack4_e4m3(v[4], v[5], v[6], v[7]), pack4_e4m3(v[8], v[9], v[10], v[11]),
+                   pack4_e4m3(v[12], v[13], v[14], v[15]));
+  } else {
+    if (noise4 != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = round_stochastic(v[i], (noise4[i >> 2] >> (8 * (i & 3))) & 0xffu);
+    }
+    const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+    const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
+    q = make_uint4(pack8_e2m1(lo), pack8_e2m1(hi), 0u, 0u);
+  }
+  return e;
+}
+
+// v <- H v / 4, H[i][j] = (-1)^popcount(i & j): four steps of sums and differences in fp32
+B200_DEVICE void hadamard16(float (&v)[16]) {
+#pragma unroll
+  for (int s = 1; s < 16; s <<= 1)
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((i & s) == 0) {
+        const float a = v[i], b = v[i | s];
+        v[i] = a + b;
+        v[i | s] = a - b;
+      }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] *= 0.25f;
+}
+
+// ----------------------------------------------------------------------------------
+// 128 x 128 tile: rows pass and columns pass (used by quant_mxfp4.cu and norm_mx.cu)
+// ----------------------------------------------------------------------------------
+struct TileArgs {
+  const __nv_bfloat16* x;         // [R, C], pitch ldx
+  long long ldx;
+  int R, C;
+  const uint8_t* noise;           // [R, C] dense, or null
+  const float* rstd;              // SCALED: [R], x is multiplied by rstd[row] * w[column] first
+  const __nv_bfloat16* w;
+  int hadamard;                   // column copy: groups of 16 rows are transformed first
+  uint8_t* q_row; uint8_t* sf_row; int row_tile;
+  uint8_t* q_col; uint8_t* sf_col; int col_tile;
+  int Rp;                         // rows of the column copy's contraction: R filled up with zeros
+};
+
+constexpr int TILE = 128;
+// Shared tile of bf16 pairs: rows at a pitch of 68 words, 4 words more every 16 rows, so that the eight lanes of a column, 16 rows apart, lie
+// 4 banks apart (quant_mxfp8.cu).  Bytes of noise: rows at a pitch of 34 words, 2 more every 16 rows.
+constexpr int PITCH_W = 68, TILE_WORDS = TILE * PITCH_W + 8 * 4;
+constexpr int NPITCH_W = 34, NOISE_WORDS = TILE * NPITCH_W + 8 * 2;
+B200_DEVICE int tile_off(int r) { return r * PITCH_W + (r >> 4) * 4; }
+B200_DEVICE int noise_off(int r) { return r * NPITCH_W + (r >> 4) * 2; }
+
+// grid (ceil(C / 128), ceil(R / 128)), 256 threads.  C is a multiple of 32; rows past R and columns past C read as zero and are not written,
+// but for the zero codes and scale bytes that fill the copies' last 32 rows and last scale word: an operand read by a GEMM holds no byte
+// inside its contraction that was not written here.
+template <int FMT, bool SCALED, bool NOISE>
+__global__ void __launch_bounds__(256)
+mx_tile_kernel(const TileArgs p) {
+  b200::begin_kernel();
+  __shared__ __align__(16) uint32_t tile[TILE_WORDS];
+  extern __shared__ __align__(16) uint32_t noise_s[];     // NOISE: NOISE_WORDS
+  __shared__ __align__(4) uint8_t sfs[2][TILE][4];
+  __shared__ float rstd_s[SCALED ? TILE : 1];
+  const int c0 = blockIdx.x * TILE;
+  const long long r0 = (long long)blockIdx.y * TILE;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int sub_row = lane >> 4, chunk = lane & 15;
+  const bool col_live = c0 + chunk * 8 < p.C;
+  const bool rows = p.q_row != nullptr, cols = p.q_col != nullptr;
+  if constexpr (SCALED) {
+    if (tid < TILE) rstd_s[tid] = r0 + tid < p.R ? p.rstd[r0 + tid] : 0.f;
+    __syncthreads();
+  }
+  float w8[8];
+  if constexpr (SCALED) {
+    const uint4 u = col_live ? *reinterpret_cast<const uint4*>(p.w + c0 + chunk * 8) : make_uint4(0u, 0u, 0u, 0u);
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+    w8[0] = a.x; w8[1] = a.y; w8[2] = b.x; w8[3] = b.y; w8[4] = c.x; w8[5] = c.y; w8[6] = d.x; w8[7] = d.y;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint4 xv[4];
+    uint2 nv[NOISE ? 4 : 1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long r = r0 + (h * 4 + i) * 16 + warp * 2 + sub_row;
+      const bool live = col_live && r < p.R;
+      xv[i] = live ? *reinterpret_cast<const uint4*>(p.x + r * p.ldx + c0 + chunk * 8) : make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (NOISE)
+        nv[i] = live ? *reinterpret_cast<const uint2*>(p.noise + r * p.C + c0 + chunk * 8) : make_uint2(0x80808080u, 0x80808080u);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (h * 4 + i) * 16 + warp * 2 + sub_row;
+      if (rows) {
+        const float2 a = unpack_bf16x2(xv[i].x), b = unpack_bf16x2(xv[i].y), c = unpack_bf16x2(xv[i].z), d = unpack_bf16x2(xv[i].w);
+        float v[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+        if constexpr (SCALED) {
+          const float s = rstd_s[r];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = v[j] * s * w8[j];
+        }
+        uint2 q;
+        const uint32_t e = quant_row8<FMT>(v, NOISE ? &nv[NOISE ? i : 0] : nullptr, q);
+        if (col_live && r0 + r < p.R) {
+          if constexpr (FMT == E4M3) *reinterpret_cast<uint2*>(p.q_row + (r0 + r) * p.C + c0 + chunk * 8) = q;
+          else *reinterpret_cast<uint32_t*>(p.q_row + (((r0 + r) * p.C + c0) >> 1) + chunk * 4) = q.x;
+        }
+        if ((chunk & 3) == 0) sfs[0][r][chunk >> 2] = (uint8_t)e;
+      }
+      if (cols) {
+        *reinterpret_cast<uint4*>(tile + tile_off(r) + chunk * 4) = xv[i];
+        if constexpr (NOISE) *reinterpret_cast<uint2*>(noise_s + noise_off(r) + chunk * 2) = nv[i];
+      }
+    }
+  }
+  __syncthreads();
+  if (rows && tid < TILE && r0 + tid < p.R) {
+    const long long o = sf_offset(r0 + tid, c0 >> 5, p.row_tile, (p.row_tile + 127) >> 7, (p.C + 127) >> 7);
+    *reinterpret_cast<uint32_t*>(p.sf_row + o) = *reinterpret_cast<const uint32_t*>(&sfs[0][tid][0]);
+  }
+  if (!cols) return;
+  const int sub = lane & 7;                      // rows sub * 16 .. + 15 of two columns
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const int cw = pass * 32 + warp * 4 + (lane >> 3), c = 2 * cw;
+    float va[16], vb[16];
+    uint32_t na[NOISE ? 4 : 1], nb[NOISE ? 4 : 1];
+    const uint32_t* t = tile + tile_off(sub * 16) + cw;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 f = unpack_bf16x2(t[i * PITCH_W]);
+      va[i] = f.x;
+      vb[i] = f.y;
+    }
+    if constexpr (NOISE) {
+      const uint16_t* n = reinterpret_cast<const uint16_t*>(noise_s + noise_off(sub * 16)) + cw;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = n[(4 * i + j) * NPITCH_W * 2];
+        na[i] = (u[0] & 0xffu) | (u[1] & 0xffu) << 8 | (u[2] & 0xffu) << 16 | u[3] << 24;
+        nb[i] = u[0] >> 8 | (u[1] >> 8) << 8 | (u[2] >> 8) << 16 | (u[3] >> 8) << 24;
+      }
+    }
+    if constexpr (SCALED) {
+      const float2 w = c0 + c < p.C ? unpack_bf16x2(*reinterpret_cast<const uint32_t*>(p.w + c0 + c)) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float s = rstd_s[sub * 16 + i];
+        va[i] = va[i] * s * w.x;
+        vb[i] = vb[i] * s * w.y;
+      }
+    }
+    if (p.hadamard) {
+      hadamard16(va);
+      hadamard16(vb);
+    }
+    uint4 qa, qb;
+    const uint32_t ea = quant_col16<FMT>(va, NOISE ? na : nullptr, qa), eb = quant_col16<FMT>(vb, NOISE ? nb : nullptr, qb);
+    if (c0 + c < p.C && r0 + sub * 16 < p.Rp) {
+      if constexpr (FMT == E4M3) {
+        uint8_t* dst = p.q_col + (long long)(c0 + c) * p.Rp + r0 + sub * 16;
+        *reinterpret_cast<uint4*>(dst) = qa;
+        *reinterpret_cast<uint4*>(dst + p.Rp) = qb;
+      } else {
+        uint8_t* dst = p.q_col + (((long long)(c0 + c) * p.Rp + r0) >> 1) + sub * 8;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(qa.x, qa.y);
+        *reinterpret_cast<uint2*>(dst + (p.Rp >> 1)) = make_uint2(qb.x, qb.y);
+      }
+    }
+    if ((sub & 1) == 0) { sfs[1][c][sub >> 1] = (uint8_t)ea; sfs[1][c + 1][sub >> 1] = (uint8_t)eb; }
+  }
+  __syncthreads();
+  if (tid < TILE && c0 + tid < p.C) {
+    const long long o = sf_offset(c0 + tid, (int)(r0 >> 5), p.col_tile, (p.col_tile + 127) >> 7, (p.Rp + 127) >> 7);
+    *reinterpret_cast<uint32_t*>(p.sf_col + o) = *reinterpret_cast<const uint32_t*>(&sfs[1][tid][0]);
+  }
+}
+
+}  // namespace mxq

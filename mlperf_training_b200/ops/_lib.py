@@ -83,6 +83,12 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_attn_fwd": [P, P, P, P, P, P, I, I, I, I, I, I, L, L, L, L, L, L, L, L, F, I, I, P],
         "b200_quant_mxfp8": [P, L, I, I, P, P, I, P, P, I, P, P],
         "b200_gemm_mxfp8": [P, P, P, P, P, I, I, I, L, L, L, I, I, P, P, L, F, P, L, P],
+        "b200_quant_mxfp4": [P, L, I, I, P, I, P, P, I, P, P, I, P],
+        "b200_dequant_mx": [P, P, P, L, I, I, I, I, P],
+        "b200_gemm_mxfp4": [P, P, P, P, P, I, I, I, L, L, L, I, I, P, P, L, F, P, L, P],
+        "b200_norm_mx": [P, P, P, P, P, I, I, F, P, P, I, P, P, I, P],
+        "b200_gemm_gated": [P, P, P, P, I, I, I, L, L, L, L, I, P],
+        "b200_gemm_gated_grad": [P, P, P, P, P, I, I, I, L, L, L, L, L, I, P],
         "b200_router_topk": [P, I, I, I, P, P, P, P],
         "b200_router_plan": [P, P, I, I, I, P, P, I, P, P],
         "b200_permute_rows": [P, P, I, I, I, P, P, P, P, P, I, P],
@@ -172,7 +178,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     if hasattr(lib, "b200_qk_norm_rope_scratch_elems"):
         lib.b200_qk_norm_rope_scratch_elems.argtypes = [I, I, I, I]
         lib.b200_qk_norm_rope_scratch_elems.restype = c_ll
-    for name in ("b200_gemm_bf16_workspace", "b200_gemm_mxfp8_workspace"):
+    for name in ("b200_gemm_bf16_workspace", "b200_gemm_mxfp8_workspace", "b200_gemm_mxfp4_workspace"):
         if hasattr(lib, name):
             getattr(lib, name).argtypes = [I, I, I]
             getattr(lib, name).restype = c_ll

@@ -96,6 +96,49 @@ def linear(x, weight, bias=None, residual=None, precision="bf16"):
     return _apply(LinearFn, x, weight, bias, residual, precision, torch.is_grad_enabled())
 
 
+class MXFP4LinearFn(Function):
+    """Linear layer on MXFP4 operands, forward and backward (``ops.linear.fp4_forward`` / ``fp4_backward``)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, noise, grad=True):
+        y, saved = L.fp4_forward(x, weight, bias=bias, residual=residual, need_wgrad=grad and weight.requires_grad,
+                                 need_dgrad=grad and ctx.needs_input_grad[0])
+        tensors, ctx.meta = L.Saved.pack(saved) if saved is not None else ([], None)
+        ctx.save_for_backward(weight, noise, *tensors)
+        ctx.has_res = residual is not None
+        ctx.bias_ref = bias
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        weight, noise, *tensors = ctx.saved_tensors
+        saved = L.Saved.unpack(tensors, ctx.meta) if ctx.meta is not None else None
+        dx, dw = L.fp4_backward(dy, saved, weight, noise=noise, need_dx=ctx.needs_input_grad[0],
+                                need_dw=ctx.needs_input_grad[1] and saved is not None)
+        db = _vec_grad(ctx.bias_ref, dy.sum(0, dtype=torch.float32)) if ctx.bias_ref is not None else None
+        return dx, dw, db, dy if ctx.has_res and ctx.needs_input_grad[3] else None, None, None
+
+
+def mxfp4_linear(x, weight, bias=None, residual=None, noise=None):
+    """``y = Q(x) Q(W)^T (+ bias) (+ residual)`` with MXFP4 operands; backward ``dx = Qs(dy) Q(W^T)^T``, ``dW = Qs(H dy)^T Q(H x)``.  ``x [T, K]``,
+    ``weight [N, K]``, K a multiple of 32, N too where a gradient of ``x`` is wanted.  ``noise [T, N]`` (uint8): the bytes with which the
+    output gradient is rounded stochastically; None: drawn in the backward.  The weight's 4-bit copies are kept on the weight until it
+    changes."""
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise ValueError(f"mxfp4_linear: input {tuple(x.shape)} for a weight {tuple(weight.shape)}")
+    T, N = x.shape[0], weight.shape[0]
+    if x.shape[1] == 0 or x.shape[1] % 32:
+        raise ValueError(f"mxfp4_linear: {x.shape[1]} input features are not a positive multiple of 32")
+    grad = torch.is_grad_enabled()
+    if grad and x.requires_grad and N % 32:
+        raise ValueError(f"mxfp4_linear: {N} output features are not a multiple of 32, as the gradient of the input needs")
+    if grad and weight.requires_grad and N % 32:
+        raise ValueError(f"mxfp4_linear: {N} output features are not a multiple of 32, as the gradient of the weight needs")
+    if noise is not None and (noise.shape != (T, N) or noise.dtype != torch.uint8):
+        raise ValueError(f"mxfp4_linear: noise {tuple(noise.shape)} {noise.dtype} for an output {T}x{N}")
+    return _apply(MXFP4LinearFn, x, weight, bias, residual, noise, grad)
+
+
 class NormFn(Function):
     """RMSNorm / LayerNorm / SwishLayerNorm on rows."""
 
@@ -171,8 +214,112 @@ class NormLinearFn(Function):
 
 def norm_linear(x, norm_w, weight, *, norm_b=None, bias=None, eps=1e-5, layer_norm=False, precision="bf16", pass_x=False):
     """``pass_x``: returns ``(y, x)``; the gradient of the second output (x taken past the norm by a residual connection) is added
-    where the norm's backward writes dx, not by a pass of its own (46000 x 512: 52 us, norm and addition 71)."""
+    where the norm's backward writes dx, not by a pass of its own (46000 x 512: 52 us, norm and addition 71).  ``precision="fp4"``: the linear
+    behind an RMS norm reads the norm's own 8-bit output (``add_norm_linear``) where its sizes allow; elsewhere its operands have 4 bits."""
+    if precision == "fp4" and not layer_norm and norm_b is None and bias is None and add_norm_linear_eligible(x, weight):
+        y, h = add_norm_linear(x, None, norm_w, weight, eps)
+        return (y, h) if pass_x else y
     return _apply(NormLinearFn, x, norm_w, norm_b, weight, bias, eps, layer_norm, precision, torch.is_grad_enabled(), pass_x)
+
+
+class AddNormLinearFn(Function):
+    """``h = x + residual``, ``y = Q(norm(h)) Q(W)^T`` with MXFP8 operands that come straight from the norm: the operand of the forward
+    product and, for the weight gradient, its transposed copy.  Returns ``(y, h)``; the gradient of ``h`` joins where the norm's backward
+    writes dx."""
+
+    @staticmethod
+    def forward(ctx, x, residual, norm_w, weight, eps, grad=True):
+        from . import mxfp8 as MX
+        from .norm_mx import rms_norm_quantize
+        grad = grad and any(ctx.needs_input_grad)
+        w_row, _ = L.weight_operands(weight, need_col=grad)
+        need_dw = grad and weight.requires_grad
+        row, col, h, rstd = rms_norm_quantize(x, norm_w, eps, residual=residual, row_tile=MX.A_TILE,
+                                              col_tile=MX.b_tile(x.shape[1]) if need_dw else None)
+        y = MX.gemm(row, w_row, out_dtype=x.dtype)
+        tensors, ctx.meta = L.Saved.pack(col) if col is not None else ([], None)
+        ctx.save_for_backward(h, norm_w, weight, rstd, *tensors)
+        ctx.refs = (norm_w, weight)
+        ctx.has_res = residual is not None
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    def backward(ctx, dy, dh):
+        from . import mxfp8 as MX
+        if dy is None:
+            return dh, dh if ctx.has_res else None, None, None, None, None
+        h, norm_w, weight, rstd, *tensors = ctx.saved_tensors
+        need_dw = ctx.meta is not None
+        dy_row, dy_col = MX.quantize(dy.contiguous(), row_tile=MX.A_TILE, col_tile=MX.A_TILE if need_dw else None)
+        _, w_col = L.weight_operands(weight, need_col=True)
+        dn = MX.gemm(dy_row, w_col, out_dtype=dy.dtype)
+        dw = _mx_wgrad(ctx.refs[1], dy_col, L.Saved.unpack(tensors, ctx.meta)) if need_dw else None
+        dx, dnw, _ = K.norm_bwd(dn, h, norm_w, None, None, rstd, dres=None if dh is None else dh.to(h.dtype))
+        return dx, dx if ctx.has_res else None, _vec_grad(ctx.refs[0], dnw), dw, None, None
+
+
+def add_norm_linear_eligible(x, weight) -> bool:
+    from .norm_mx import MAX_WIDTH
+    return L.mx_eligible(x.shape[0], weight.shape[0], weight.shape[1]) and x.shape[1] <= MAX_WIDTH
+
+
+def add_norm_linear(x, residual, norm_w, weight, eps=1e-5):
+    """``(y, h)``: ``h = x + residual`` (``x`` where that is None), ``y = rms_norm(h) W^T`` with MXFP8 operands from the norm itself.  Tokens,
+    input and output features are multiples of 128 (as every MXFP8 linear in training), at most 8192 input features."""
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise ValueError(f"add_norm_linear: input {tuple(x.shape)} for a weight {tuple(weight.shape)}")
+    if not add_norm_linear_eligible(x, weight):
+        raise ValueError(f"add_norm_linear: {tuple(x.shape)} x {tuple(weight.shape)}: sizes must be multiples of 128, at most 8192 input features")
+    return _apply(AddNormLinearFn, x, residual, norm_w, weight, eps, torch.is_grad_enabled())
+
+
+class GatedMLPFn(Function):
+    """``y = (act(x Wg^T) * (x Wu^T)) Wd^T (+ residual)`` in bf16: the projections, the activation and the product in one kernel, the down
+    projection in another; backward: the gradient of the activation in the epilogue of the down projection's dgrad.  Kept for
+    backward: ``x`` and the projections (the activation's product is made again where they are read)."""
+
+    @staticmethod
+    def forward(ctx, x, w_gate_up, w_down, residual, act, grad=True):
+        grad = grad and any(ctx.needs_input_grad)
+        a, gu = K.gated_fwd(x, w_gate_up, act, want_gu=grad)
+        if a.shape[0]:
+            y = K.gemm(a, w_down, residual=residual)
+        else:
+            y = x.new_empty((0, w_down.shape[0]))
+        ctx.save_for_backward(x, w_gate_up, w_down, gu)
+        ctx.act, ctx.has_res = act, residual is not None
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w_gate_up, w_down, gu = ctx.saved_tensors
+        need_x, need_gu, need_down, need_res = (ctx.needs_input_grad[i] for i in range(4))
+        dres = dy if ctx.has_res and need_res else None
+        if dy.shape[0] == 0:
+            zero = lambda t: None if getattr(t, "main_grad", None) is not None else torch.zeros_like(t)
+            return x.new_empty(x.shape), zero(w_gate_up), zero(w_down), dres, None, None
+        dx = dw_gu = dw_down = None
+        if need_x or need_gu or need_down:
+            dgu, a = K.gated_bwd(dy, w_down, gu, ctx.act, want_a=need_down)
+            if need_down:
+                dw_down = _wgrad(dy, a, w_down)
+            del a
+            if need_x:
+                dx = K.gemm(dgu, w_gate_up, b_mn_major=True)
+            if need_gu:
+                dw_gu = _wgrad(dgu, x, w_gate_up)
+        return dx, dw_gu, dw_down, dres, None, None
+
+
+def gated_mlp(x, w_gate_up, w_down, residual=None, act="silu"):
+    """Gated feed-forward block of ``x [T, D]`` with the stacked ``w_gate_up [2F, D]`` (gate rows first) and ``w_down [D_out, F]``; ``act``
+    "silu" or "gelu" (tanh form).  Widths are multiples of 8, operands bf16 on the GPU."""
+    if x.dim() != 2 or w_gate_up.dim() != 2 or w_down.dim() != 2 or 2 * w_down.shape[1] != w_gate_up.shape[0] or w_gate_up.shape[1] != x.shape[1]:
+        raise ValueError(f"gated_mlp: input {tuple(x.shape)}, weights {tuple(w_gate_up.shape)} and {tuple(w_down.shape)}")
+    if residual is not None and residual.shape != (x.shape[0], w_down.shape[0]):
+        raise ValueError(f"gated_mlp: residual {tuple(residual.shape)} for an output {x.shape[0]}x{w_down.shape[0]}")
+    return _apply(GatedMLPFn, x, w_gate_up, w_down, residual, act, torch.is_grad_enabled())
 
 
 class SwiGLULinearFn(Function):

@@ -284,6 +284,77 @@ def swiglu_bwd(da: torch.Tensor, gu: torch.Tensor) -> torch.Tensor:
     return out
 
 
+GATE_ACTS = {"silu": 0, "gelu": 1}       # gelu: the tanh form
+
+
+def _gate_check(what: str, x: torch.Tensor, w: torch.Tensor, act: str, Fh: int, D: int) -> None:
+    if act not in GATE_ACTS:
+        raise ValueError(f"{what}: unknown activation '{act}' (known: {sorted(GATE_ACTS)})")
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"{what}: expected 2-D tensors, got {tuple(x.shape)} and {tuple(w.shape)}")
+    if x.device != w.device:
+        raise ValueError(f"{what}: operands on {x.device} and {w.device}")
+    if use_kernels(x):
+        if x.dtype != BF16 or w.dtype != BF16:
+            raise TypeError(f"{what}: operands must be bf16")
+        if Fh % 8 or D % 8 or not Fh or not D:
+            raise ValueError(f"{what}: widths {D} and {Fh} must be positive multiples of 8")
+
+
+def _gate_value(g: torch.Tensor, act: str) -> torch.Tensor:
+    return F.silu(g) if act == "silu" else F.gelu(g, approximate="tanh")
+
+
+def gated_fwd(x: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu", *, want_gu: bool = True):
+    """``a = act(x Wg^T) * (x Wu^T)`` of ``x [T, D]`` and the stacked ``w_gate_up [2F, D]`` (gate rows first) in one launch.  Returns
+    ``(a [T, F], gu [T, 2F])``; ``gu`` (the projections, for the backward) is None without
+    ``want_gu``."""
+    T, D = x.shape
+    Fh = w_gate_up.shape[0] // 2
+    _gate_check("gated_fwd", x, w_gate_up, act, Fh, D)
+    if w_gate_up.shape[1] != D or w_gate_up.shape[0] % 2:
+        raise ValueError(f"gated_fwd: weight {tuple(w_gate_up.shape)} for {D} columns and two stacked projections")
+    if not use_kernels(x):
+        gu = x.float() @ w_gate_up.float().t()
+        a = (_gate_value(gu[:, :Fh], act) * gu[:, Fh:]).to(x.dtype)
+        return a, gu.to(x.dtype) if want_gu else None
+    a = torch.empty((T, Fh), dtype=x.dtype, device=x.device)
+    gu = torch.empty((T, 2 * Fh), dtype=x.dtype, device=x.device) if want_gu else None
+    if T:
+        x, w = _row_major(x), _row_major(w_gate_up)
+        call("b200_gemm_gated", ptr(x), ptr(w), ptr(a), ptr(gu), T, Fh, D, x.stride(0), w.stride(0), a.stride(0), 2 * Fh, GATE_ACTS[act],
+             stream_ptr())
+    return a, gu
+
+
+def gated_bwd(dy: torch.Tensor, w_down: torch.Tensor, gu: torch.Tensor, act: str = "silu", *, want_a: bool = True):
+    """Gradient of ``gu [T, 2F]`` from that of ``a W_down^T``, ``dy [T, D]``, ``w_down [D, F]``, in one launch: ``da = dy W_down``, ``d gate = da
+    * up * act'(gate)``, ``d up = da * act(gate)``.  Returns ``(dgu [T, 2F], a [T, F])``; ``a`` (made again from ``gu``, for the gradient of
+    ``w_down``) is None without ``want_a``."""
+    T, F2 = gu.shape
+    D, Fh = w_down.shape
+    _gate_check("gated_bwd", dy, w_down, act, Fh, D)
+    if dy.shape != (T, D) or F2 != 2 * Fh or gu.dtype != dy.dtype or gu.device != dy.device:
+        raise ValueError(f"gated_bwd: gradient {tuple(dy.shape)}, weight {tuple(w_down.shape)}, projections {tuple(gu.shape)} {gu.dtype}")
+    if not use_kernels(dy):
+        da = dy.float() @ w_down.float()
+        g = gu[:, :Fh].float().detach().requires_grad_(True)
+        u = gu[:, Fh:].float()
+        with torch.enable_grad():
+            v = _gate_value(g, act)
+        (dg,) = torch.autograd.grad(v, g, da * u)
+        v = v.detach()
+        return torch.cat([dg, da * v], 1).to(dy.dtype), (v * u).to(dy.dtype) if want_a else None
+    gu = _row_major(gu)
+    dgu = torch.empty((T, F2), dtype=dy.dtype, device=dy.device)
+    a = torch.empty((T, Fh), dtype=dy.dtype, device=dy.device) if want_a else None
+    if T:
+        dy, w = _row_major(dy), _row_major(w_down)
+        call("b200_gemm_gated_grad", ptr(dy), ptr(w), ptr(gu), ptr(dgu), ptr(a), T, Fh, D, dy.stride(0), w.stride(0), gu.stride(0), F2, Fh,
+             GATE_ACTS[act], stream_ptr())
+    return dgu, a
+
+
 def gelu_fwd(x: torch.Tensor) -> torch.Tensor:
     if not use_kernels(x):
         return F.gelu(x.float(), approximate="tanh").to(x.dtype)

@@ -13,6 +13,9 @@ operands whose elements were rounded to the 6- or 4-bit format first - every suc
 the product is the narrow format's, bit for bit, at the 8-bit operand rate; gradients of the 4-bit recipes are
 rounded stochastically and their weight-gradient operands pass a block Hadamard transform along the tokens.
 
+``precision="fp4"`` runs the product itself on 4-bit operands (``ops.mxfp4``): activations and weights rounded to nearest, output
+gradients stochastically, both operands of the weight gradient behind a 16-row Hadamard transform.
+
 What is saved for backward is the return value of ``forward`` (a bf16 tensor or the fp8 operand);
 ``Saved.pack`` / ``Saved.unpack`` move it through ``ctx.save_for_backward``.
 
@@ -26,6 +29,7 @@ import torch
 
 from . import fp8 as F8
 from . import kernels as K
+from . import mxfp4 as M4
 from . import mxfp8 as MX
 
 # bumped by the optimizer engine after every parameter update: invalidates cached weight copies
@@ -135,6 +139,67 @@ def fp8_weight_operands(weight: torch.Tensor, need_col: bool = True):
     return row, col
 
 
+def fp4_eligible(rows: int, n_out: int, n_in: int) -> bool:
+    """The 4-bit product contracts over whole blocks of 32: output features in dgrad, input features in forward (tokens are filled up)."""
+    return rows > 0 and n_out > 0 and n_in > 0 and n_out % 32 == 0 and n_in % 32 == 0
+
+
+def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
+    """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, cached on the tensor until it changes: through torch (its
+    version counter) or through an optimizer step."""
+    cacheable = not weight.is_inference()
+    key = (_WEIGHT_EPOCH if weight.requires_grad else -1, weight._version if cacheable else -1)
+    cache = getattr(weight, "_mx4_cache", None)
+    row = None
+    if cacheable and cache is not None and cache[0] == key:
+        if cache[2] is not None or not need_col:
+            return cache[1], cache[2]
+        row = cache[1]
+    N, Kd = weight.shape
+    w = weight.detach()
+    if w.dtype != torch.bfloat16 and w.is_cuda:
+        w = w.to(torch.bfloat16)
+    new_row, col = M4.quantize(w, row_tile=M4.b_tile(N) if row is None else None, col_tile=M4.b_tile(Kd) if need_col else None)
+    row = new_row if row is None else row
+    if cacheable:
+        weight._mx4_cache = (key, row, col)
+    return row, col
+
+
+def fp4_forward(x: torch.Tensor, weight: torch.Tensor, *, bias=None, residual=None, need_wgrad: bool = True, need_dgrad: bool = False):
+    """``y = Q(x) Q(W)^T (+ bias) (+ residual)``; returns ``(y, saved)``, ``saved`` the column-wise copy of the Hadamard transform of ``x``."""
+    w_row, _ = fp4_weight_operands(weight, need_col=need_dgrad)
+    xq = x if x.dtype == torch.bfloat16 or not x.is_cuda else x.to(torch.bfloat16)
+    x_row, x_col = M4.quantize(xq, row_tile=M4.A_TILE, col_tile=M4.b_tile(x.shape[1]) if need_wgrad else None, hadamard=True)
+    return M4.gemm(x_row, w_row, bias=bias, residual=residual, out_dtype=x.dtype), x_col
+
+
+def fp4_backward(dy: torch.Tensor, saved, weight: torch.Tensor, *, noise: torch.Tensor | None = None, need_dx: bool = True,
+                 need_dw: bool = True):
+    """``(dx, dw)``: ``dx = Qs(dy) Q(W^T)^T``, ``dw = Qs(H dy)^T Q(H x)`` (None when it went into ``weight.main_grad``).  ``noise``: the bytes of
+    the stochastic rounding, one per element of ``dy``; None: drawn here."""
+    dx = dw = None
+    if not (need_dx or need_dw):
+        return dx, dw
+    dyq = dy if dy.dtype == torch.bfloat16 or not dy.is_cuda else dy.to(torch.bfloat16)
+    if noise is None:
+        noise = torch.randint(0, 256, dy.shape, dtype=torch.uint8, device=dy.device)
+    dy_row, dy_col = M4.quantize(dyq, row_tile=M4.A_TILE if need_dx else None, col_tile=M4.A_TILE if need_dw else None, noise=noise,
+                                 hadamard=True)
+    if need_dx:
+        _, w_col = fp4_weight_operands(weight, need_col=True)
+        dx = M4.gemm(dy_row, w_col, out_dtype=dy.dtype)
+    if need_dw:
+        if not isinstance(saved, M4.MX4Operand):         # (a forward of another precision left its activation as it was)
+            _, saved = M4.quantize(saved, col_tile=M4.b_tile(weight.shape[1]), hadamard=True)
+        mg = getattr(weight, "main_grad", None)
+        if mg is not None:
+            M4.gemm(dy_col, saved, out=mg, accumulate=True)
+        else:
+            dw = M4.gemm(dy_col, saved, out_dtype=weight.dtype)
+    return dx, dw
+
+
 class Saved:
     """The activation copy kept for the weight-gradient GEMM."""
 
@@ -142,6 +207,8 @@ class Saved:
     def pack(obj):
         if isinstance(obj, MX.MXOperand):
             return [obj.q, obj.sf], ("mx", obj.rows, obj.k, obj.tile_rows)
+        if isinstance(obj, M4.MX4Operand):
+            return [obj.q, obj.sf], ("mx4", obj.rows, obj.k, obj.tile_rows)
         if isinstance(obj, F8.FP8Operand):
             return [obj.q, obj.inv_scale], ("f8", obj.rows, obj.k, obj.fmt)
         return [obj], ("t",)
@@ -150,6 +217,8 @@ class Saved:
     def unpack(tensors, meta):
         if meta[0] == "mx":
             return MX.MXOperand(tensors[0], tensors[1], meta[1], meta[2], meta[3])
+        if meta[0] == "mx4":
+            return M4.MX4Operand(tensors[0], tensors[1], meta[1], meta[2], meta[3])
         if meta[0] == "f8":
             return F8.FP8Operand(tensors[0], tensors[1], meta[1], meta[2], meta[3])
         return tensors[0]
@@ -157,6 +226,8 @@ class Saved:
 
 def low_precision(precision: str, rows: int, n_out: int, n_in: int) -> bool:
     """The call runs a quantised GEMM (and saves a quantised activation copy for backward)."""
+    if precision == "fp4":
+        return fp4_eligible(rows, n_out, n_in)
     # (the per-tensor FP8 GEMM has CTA-pair tiles only: its M - the tokens in forward and dgrad, the output
     # features in wgrad - must exceed one 128-row tile)
     return (is_mx(precision) or precision == "fp8") and mx_eligible(rows, n_out, n_in) and (is_mx(precision) or (rows > 128 and n_out > 128))
@@ -182,6 +253,8 @@ def forward(x: torch.Tensor, weight: torch.Tensor, precision: str, *, bias=None,
                                        col_fmt=b_act)
         y = MX.gemm(x_row, w_row, bias=bias, residual=residual, out_dtype=x.dtype)
         return y, x_col
+    if precision == "fp4" and fp4_eligible(M, N, Kd):
+        return fp4_forward(x, weight, bias=bias, residual=residual, need_wgrad=need_wgrad, need_dgrad=need_dgrad)
     if precision == "fp8" and low_precision(precision, M, N, Kd):
         w_row, _ = fp8_weight_operands(weight, need_col=False)
         st = _site(weight, "x", "e4m3")
@@ -224,6 +297,8 @@ def backward(dy: torch.Tensor, saved, weight: torch.Tensor, precision: str, *, n
             else:
                 dw = MX.gemm(dy_col, saved, out_dtype=weight.dtype if weight.dtype != torch.float32 else torch.float32)
         return dx, dw
+    if precision == "fp4" and fp4_eligible(M, N, Kd):
+        return fp4_backward(dy, saved, weight, need_dx=need_dx, need_dw=need_dw)
     if precision == "fp8" and low_precision(precision, M, N, Kd):
         if need_dw and not isinstance(saved, F8.FP8Operand):
             st = _site(weight, "x", "e4m3")

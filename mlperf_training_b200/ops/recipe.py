@@ -10,7 +10,7 @@ The reference trains with micro-scaled low-precision linears and changes the rec
 * GPT-OSS / FLUX: weight de-oscillation for MXFP4 (start step 768, period 100, ratio 4.0;
   small_llm_moe_pretraining/primus/conf/gpt_oss_20B-MXFP4-deosc-mlperf-pretrain.yaml:197-204).
 
-This framework implements two low-precision recipe families with different numerics:
+This framework implements low-precision recipe families with different numerics:
 
 * the micro-scaled family - one UE8M0 scale per 32 contraction elements
   (``tcgen05.mma.kind::mxf8f6f4.block_scale``; ``ops.mxfp8``, ``ops.linear.MX_RECIPES``): ``mxfp8`` (e4m3
@@ -19,6 +19,8 @@ This framework implements two low-precision recipe families with different numer
   weights forward, MXFP4 backward).  The narrow members round their operands to the 6- / 4-bit element format
   and carry them as e4m3 codes - every such value is an e4m3 value - so the GEMM result is the narrow
   format's bit for bit, at the 8-bit operand rate (not the 4-bit rate);
+* ``fp4``    MXFP4 operands multiplied at the 4-bit rate (``tcgen05.mma.kind::mxf4``; ``ops.mxfp4``), gradients as in
+  ``mxfp4``; a linear behind an RMS norm takes the norm's own MXFP8 output instead (``ops.norm_mx``);
 * ``fp8``    per-tensor e4m3 forward operands and e5m2 gradients with delayed scaling
   (``tcgen05.mma.kind::f8f6f4``; ``ops.fp8``) - what the reference calls fp8 / hybrid / delayed.
 
@@ -49,6 +51,7 @@ from .linear import bump_weight_epoch
 FORMAT_MAP = {
     "bf16": "bf16", "none": "bf16",
     "mxfp8": "mxfp8", "mxfp6": "mxfp6", "mxfp4": "mxfp4", "e2m1": "mxfp4", "nvfp4": "mxfp4", "a4w4": "mxfp4", "a6w4": "a6w4",
+    "fp4": "fp4",
     "mxfp8_fwd_mxfp4_bwd": "mxfp8_fwd_mxfp4_bwd", "fp8_fwd_mxfp4_bwd": "mxfp8_fwd_mxfp4_bwd",
     "fp8": "fp8", "fp8_hybrid": "fp8", "hybrid": "fp8", "e4m3": "fp8", "delayed": "fp8", "tensorwise": "fp8",
 }
