@@ -60,7 +60,9 @@ class GPTConfig:
     recompute_layers: int = 0
     swiglu_store: str = "bf16"          # "fp8": the fused MXFP8 MLP keeps its gate | up activation for backward as e4m3 codes
     dtype: str = "bf16"
-    precision: str = "bf16"         # GEMM precision of the linears: "bf16" | "mxfp8"
+    # GEMM precision of the linears: "bf16" | "mxfp8" | ... | "fp4" (linears behind a norm read its 8-bit output, the others multiply 4-bit
+    # operands; dense MLPs of layers kept in bf16 run as one gated block)
+    precision: str = "bf16"
     # the first / last N transformer layers keep bf16 linears whatever ``precision`` says (Megatron's
     # first_last_layers_bf16 with num_layers_at_start_in_bf16 / num_layers_at_end_in_bf16, an option of the
     # low-precision recipes: small_llm_moe_pretraining/primus/conf/gpt_oss_20B-MXFP4-deosc-mlperf-pretrain.yaml:55-57)
@@ -192,6 +194,8 @@ class DenseMLP(nn.Module):
         pr = "bf16" if self.force_bf16 else self.precision
         if pr == "mxfp8" and self.fused and F.fused_mlp_eligible(h, self.w_gate_up, self.w_down):
             return F.fused_mlp(h, norm_w, self.w_gate_up, self.w_down, eps, self.store_fp8)
+        if self.force_bf16 and self.precision == "fp4":
+            return F.gated_mlp(F.rms_norm(h, norm_w, eps), self.w_gate_up, self.w_down, residual=h)
         gu = F.norm_linear(h, norm_w, self.w_gate_up, eps=eps, precision=pr)
         return F.swiglu_linear(gu, self.w_down, residual=h, precision=pr)
 
