@@ -4,7 +4,8 @@
 // Scale: the smallest power of two s with amax / s <= vmax (448 = 1.75 * 2^8, 6 = 1.5 * 2^2), biased by 127; at least 1 (2^-126) where amax
 // is not zero, 0 where it is.  255 (NaN) for a block that holds an infinity or a NaN: e2m1 has neither, and with any other scale the value
 // would come back as an ordinary number.  No element saturates: amax / s <= vmax.
-// Magnitudes are compared as integers (their fp32 bits less the sign), in which a NaN is above infinity and both above every number.
+// Magnitudes are compared so that a NaN is kept: as integers (their bits less the sign: a NaN is above infinity, both above every number),
+// or by the maximum that hands a NaN on.
 #pragma once
 #include <cuda_fp8.h>
 
@@ -43,11 +44,14 @@ B200_DEVICE uint32_t pack8_e2m1(const float (&v)[8]) {
   return r;
 }
 // y (|y| <= 6) to a value of e2m1: |y| / quantum + (u + 1/2) / 256 rounded down, u a random byte.  The expectation over u is y to within
-// 1/512 of a quantum, and a value of the format stays as it is.
-B200_DEVICE float round_stochastic(float y, uint32_t u) {
-  const uint32_t q = max(abs_bits(y) & 0x7f800000u, 0x3f800000u) - 0x00800000u;    // quantum: 0.5 below 2, 1 below 4, 2
-  const float t = floorf(fabsf(y) * __uint_as_float(0x7f000000u - q) + ((float)u + 0.5f) * 0.00390625f);
-  return copysignf(fminf(t * __uint_as_float(q), 6.f), y);
+// 1/512 of a quantum, and a value of the format stays as it is.  The quantum is the upper bit of the fraction, so this is an integer addition
+// to the bits below it and a mask (a carry out of the fraction is the next power of two); below 1, where the quantum stays 0.5, one is added
+// first and taken off after.  No conversions: floor and int-to-float run at a quarter of the rate of these.
+// `u` is the word that holds the byte, `at` the byte's place in it.
+B200_DEVICE float round_stochastic(float y, uint32_t u, int at) {
+  const float a = fabsf(y), one = a < 1.f ? 1.f : 0.f;
+  const uint32_t z = (__float_as_uint(a + one) + (((u >> (8 * at)) & 0xffu) << 14) + 0x2000u) & 0xffc00000u;
+  return __uint_as_float(__float_as_uint(__uint_as_float(z) - one) | (__float_as_uint(y) & 0x80000000u));
 }
 
 // byte offset of scale (row r of the operand, scale column kc) in the atom layout the block-scaled GEMMs read (quant_mxfp8.cu)
@@ -58,71 +62,111 @@ B200_DEVICE long long sf_offset(long long r, int kc, int tile_rows, int atoms_pe
   return ((tile * k_groups + (kc >> 2)) * atoms_per_tile + atom) * 512 + (ra & 31) * 16 + (ra >> 5) * 4 + (kc & 3);
 }
 
-// Eight values of a 32-block whose other values are in the three neighbouring lanes (lane / 4 is the block): codes in q (e2m1: q.x),
-// returns the scale byte.  noise: eight random bytes, null for round to nearest.
+// Largest magnitude of bf16 pairs, halves by themselves, as integers.
+B200_DEVICE uint32_t amax2(uint32_t m, uint32_t pair) { return __vmaxu2(m, pair & 0x7fff7fffu); }
+
+// Eight scaled values (eight elements of a 32-block, |y| <= vmax) to codes; noise: eight random bytes or null (e2m1: codes in q.x).
+template <int FMT>
+B200_DEVICE uint2 codes8(float (&y)[8], const uint2* noise) {
+  if constexpr (FMT == E4M3) {
+    return make_uint2(pack4_e4m3(y[0], y[1], y[2], y[3]), pack4_e4m3(y[4], y[5], y[6], y[7]));
+  } else {
+    if (noise != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = round_stochastic(y[i], i < 4 ? noise->x : noise->y, i & 3);
+    }
+    return make_uint2(pack8_e2m1(y), 0u);
+  }
+}
+
+// Eight values of a 32-block whose other values are in the three neighbouring lanes (lane / 4 is the block): codes in q, returns the scale
+// byte.  From fp32 values, and from bf16 as they are (magnitudes compared in pairs, scaled in pairs).
 template <int FMT>
 B200_DEVICE uint32_t quant_row8(const float (&v)[8], const uint2* noise, uint2& q) {
-  uint32_t m = abs_bits(v[0]);
+  float m = fabsf(v[0]);
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = max(m, abs_bits(v[i]));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const uint32_t e = e8m0<FMT>(m);
+  for (int i = 1; i < 8; ++i) m = fmax_nan(m, fabsf(v[i]));
+  m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const uint32_t e = e8m0<FMT>(abs_bits(m));
   const float inv = inv_scale(e);
   float y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = v[i] * inv;
-  if constexpr (FMT == E4M3) {
-    q = make_uint2(pack4_e4m3(y[0], y[1], y[2], y[3]), pack4_e4m3(y[4], y[5], y[6], y[7]));
-  } else {
-    if (noise != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = round_stochastic(y[i], ((i < 4 ? noise->x : noise->y) >> (8 * (i & 3))) & 0xffu);
-    }
-    q = make_uint2(pack8_e2m1(y), 0u);
-  }
+  q = codes8<FMT>(y, noise);
   return e;
 }
-
-// Sixteen rows of one column; the other half of the 32-block is in the neighbouring lane.  Codes in q (e4m3: 16 bytes, e2m1: q.x, q.y).
 template <int FMT>
-B200_DEVICE uint32_t quant_col16(float (&v)[16], const uint32_t* noise4, uint4& q) {
-  uint32_t m = abs_bits(v[0]);
-#pragma unroll
-  for (int i = 1; i < 16; ++i) m = max(m, abs_bits(v[i]));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  const uint32_t e = e8m0<FMT>(m);
+B200_DEVICE uint32_t quant_row8(const uint4& v, const uint2* noise, uint2& q) {
+  uint32_t m = amax2(amax2(amax2(v.x & 0x7fff7fffu, v.y), v.z), v.w);
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const uint32_t e = e8m0<FMT>(max(m << 16, m & 0xffff0000u));
   const float inv = inv_scale(e);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] *= inv;
-  if constexpr (FMT == E4M3) {
-    q = make_uint4(pack4_e4m3(v[0], v[1], v[2], v[3]), pack4_e4m3(v[4], v[5], v[6], v[7]), pack4_e4m3(v[8], v[9], v[10], v[11]),
-                   pack4_e4m3(v[12], v[13], v[14], v[15]));
-  } else {
-    if (noise4 != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = round_stochastic(v[i], (noise4[i >> 2] >> (8 * (i & 3))) & 0xffu);
-    }
-    const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-    const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
-    q = make_uint4(pack8_e2m1(lo), pack8_e2m1(hi), 0u, 0u);
-  }
+  const float2 i2 = make_float2(inv, inv);
+  const float2 a = fmul2(unpack_bf16x2(v.x), i2), b = fmul2(unpack_bf16x2(v.y), i2);
+  const float2 c = fmul2(unpack_bf16x2(v.z), i2), d = fmul2(unpack_bf16x2(v.w), i2);
+  float y[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+  q = codes8<FMT>(y, noise);
   return e;
 }
 
-// v <- H v / 4, H[i][j] = (-1)^popcount(i & j): four steps of sums and differences in fp32
-B200_DEVICE void hadamard16(float (&v)[16]) {
+// v <- H v / 4, H[i][j] = (-1)^popcount(i & j), of two columns at a time: four steps of sums and differences in fp32 (divided first, so that
+// no sum overflows that would not in the end).
+B200_DEVICE void hadamard16(float2 (&v)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = fmul2(v[i], make_float2(0.25f, 0.25f));
 #pragma unroll
   for (int s = 1; s < 16; s <<= 1)
 #pragma unroll
     for (int i = 0; i < 16; ++i)
       if ((i & s) == 0) {
-        const float a = v[i], b = v[i | s];
-        v[i] = a + b;
-        v[i | s] = a - b;
+        const float2 a = v[i], b = v[i | s];
+        v[i] = fadd2(a, b);
+        v[i | s] = ffma2(b, make_float2(-1.f, -1.f), a);
       }
+}
+
+// Sixteen rows of two columns; the other halves of the 32-blocks are in the neighbouring lane.  `m`: the bits of the largest magnitudes of the
+// two (this lane's rows).  noise: word i holds the bytes of rows 4 i .. 4 i + 3 (na: first column, nb: second), null for nearest.  Codes in
+// qa, qb (e4m3: 16 bytes, e2m1: two words), scale bytes in ea, eb.
+template <int FMT>
+B200_DEVICE void quant_col16(float2 (&v)[16], uint32_t ma, uint32_t mb, const uint32_t* na, const uint32_t* nb, uint4& qa, uint4& qb,
+                             uint32_t& ea, uint32_t& eb) {
+  ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
+  mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+  ea = e8m0<FMT>(ma);
+  eb = e8m0<FMT>(mb);
+  const float2 inv = make_float2(inv_scale(ea), inv_scale(eb));
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] *= 0.25f;
+  for (int i = 0; i < 16; ++i) v[i] = fmul2(v[i], inv);
+  uint32_t a[4], b[4];
+  if constexpr (FMT == E4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = pack4_e4m3(v[4 * i].x, v[4 * i + 1].x, v[4 * i + 2].x, v[4 * i + 3].x);
+      b[i] = pack4_e4m3(v[4 * i].y, v[4 * i + 1].y, v[4 * i + 2].y, v[4 * i + 3].y);
+    }
+  } else {
+    a[2] = a[3] = b[2] = b[3] = 0u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x[8], y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = v[8 * h + i].x;
+        y[i] = v[8 * h + i].y;
+        if (na != nullptr) {
+          x[i] = round_stochastic(x[i], na[2 * h + (i >> 2)], i & 3);
+          y[i] = round_stochastic(y[i], nb[2 * h + (i >> 2)], i & 3);
+        }
+      }
+      a[h] = pack8_e2m1(x);
+      b[h] = pack8_e2m1(y);
+    }
+  }
+  qa = make_uint4(a[0], a[1], a[2], a[3]);
+  qb = make_uint4(b[0], b[1], b[2], b[3]);
 }
 
 // ----------------------------------------------------------------------------------
@@ -135,7 +179,6 @@ struct TileArgs {
   const uint8_t* noise;           // [R, C] dense, or null
   const float* rstd;              // SCALED: [R], x is multiplied by rstd[row] * w[column] first
   const __nv_bfloat16* w;
-  int hadamard;                   // column copy: groups of 16 rows are transformed first
   uint8_t* q_row; uint8_t* sf_row; int row_tile;
   uint8_t* q_col; uint8_t* sf_col; int col_tile;
   int Rp;                         // rows of the column copy's contraction: R filled up with zeros
@@ -152,7 +195,7 @@ B200_DEVICE int noise_off(int r) { return r * NPITCH_W + (r >> 4) * 2; }
 // grid (ceil(C / 128), ceil(R / 128)), 256 threads.  C is a multiple of 32; rows past R and columns past C read as zero and are not written,
 // but for the zero codes and scale bytes that fill the copies' last 32 rows and last scale word: an operand read by a GEMM holds no byte
 // inside its contraction that was not written here.
-template <int FMT, bool SCALED, bool NOISE>
+template <int FMT, bool SCALED, bool NOISE, bool HAD>
 __global__ void __launch_bounds__(256)
 mx_tile_kernel(const TileArgs p) {
   b200::begin_kernel();
@@ -192,15 +235,19 @@ mx_tile_kernel(const TileArgs p) {
     for (int i = 0; i < 4; ++i) {
       const int r = (h * 4 + i) * 16 + warp * 2 + sub_row;
       if (rows) {
-        const float2 a = unpack_bf16x2(xv[i].x), b = unpack_bf16x2(xv[i].y), c = unpack_bf16x2(xv[i].z), d = unpack_bf16x2(xv[i].w);
-        float v[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+        uint2 q;
+        uint32_t e;
+        const uint2* noise = NOISE ? &nv[NOISE ? i : 0] : nullptr;
         if constexpr (SCALED) {
+          const float2 a = unpack_bf16x2(xv[i].x), b = unpack_bf16x2(xv[i].y), c = unpack_bf16x2(xv[i].z), d = unpack_bf16x2(xv[i].w);
+          float v[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
           const float s = rstd_s[r];
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = v[j] * s * w8[j];
+          e = quant_row8<FMT>(v, noise, q);
+        } else {
+          e = quant_row8<FMT>(xv[i], noise, q);
         }
-        uint2 q;
-        const uint32_t e = quant_row8<FMT>(v, NOISE ? &nv[NOISE ? i : 0] : nullptr, q);
         if (col_live && r0 + r < p.R) {
           if constexpr (FMT == E4M3) *reinterpret_cast<uint2*>(p.q_row + (r0 + r) * p.C + c0 + chunk * 8) = q;
           else *reinterpret_cast<uint32_t*>(p.q_row + (((r0 + r) * p.C + c0) >> 1) + chunk * 4) = q.x;
@@ -223,41 +270,55 @@ mx_tile_kernel(const TileArgs p) {
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     const int cw = pass * 32 + warp * 4 + (lane >> 3), c = 2 * cw;
-    float va[16], vb[16];
     uint32_t na[NOISE ? 4 : 1], nb[NOISE ? 4 : 1];
-    const uint32_t* t = tile + tile_off(sub * 16) + cw;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 f = unpack_bf16x2(t[i * PITCH_W]);
-      va[i] = f.x;
-      vb[i] = f.y;
-    }
     if constexpr (NOISE) {
+      // bytes of the two columns, row by row, turned into words of four rows each
       const uint16_t* n = reinterpret_cast<const uint16_t*>(noise_s + noise_off(sub * 16)) + cw;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t u[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = n[(4 * i + j) * NPITCH_W * 2];
-        na[i] = (u[0] & 0xffu) | (u[1] & 0xffu) << 8 | (u[2] & 0xffu) << 16 | u[3] << 24;
-        nb[i] = u[0] >> 8 | (u[1] >> 8) << 8 | (u[2] >> 8) << 16 | (u[3] >> 8) << 24;
+        const uint32_t u01 = __byte_perm(n[(4 * i) * NPITCH_W * 2], n[(4 * i + 1) * NPITCH_W * 2], 0x5140);
+        const uint32_t u23 = __byte_perm(n[(4 * i + 2) * NPITCH_W * 2], n[(4 * i + 3) * NPITCH_W * 2], 0x5140);
+        na[i] = __byte_perm(u01, u23, 0x5410);
+        nb[i] = __byte_perm(u01, u23, 0x7632);
       }
     }
-    if constexpr (SCALED) {
-      const float2 w = c0 + c < p.C ? unpack_bf16x2(*reinterpret_cast<const uint32_t*>(p.w + c0 + c)) : make_float2(0.f, 0.f);
+    float2 v[16];
+    uint32_t ma = 0u, mb = 0u;
+    const uint32_t* t = tile + tile_off(sub * 16) + cw;
+    if constexpr (!SCALED && !HAD) {
+      uint32_t m = 0u;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float s = rstd_s[sub * 16 + i];
-        va[i] = va[i] * s * w.x;
-        vb[i] = vb[i] * s * w.y;
+        const uint32_t u = t[i * PITCH_W];
+        m = amax2(m, u);
+        v[i] = unpack_bf16x2(u);
       }
-    }
-    if (p.hadamard) {
-      hadamard16(va);
-      hadamard16(vb);
+      ma = m << 16;
+      mb = m & 0xffff0000u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = unpack_bf16x2(t[i * PITCH_W]);
+      if constexpr (SCALED) {
+        const float2 w = c0 + c < p.C ? unpack_bf16x2(*reinterpret_cast<const uint32_t*>(p.w + c0 + c)) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float s = rstd_s[sub * 16 + i];
+          v[i] = fmul2(fmul2(v[i], make_float2(s, s)), w);
+        }
+      }
+      if constexpr (HAD) hadamard16(v);
+      float fa = 0.f, fb = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        fa = fmax_nan(fa, fabsf(v[i].x));
+        fb = fmax_nan(fb, fabsf(v[i].y));
+      }
+      ma = abs_bits(fa);
+      mb = abs_bits(fb);
     }
     uint4 qa, qb;
-    const uint32_t ea = quant_col16<FMT>(va, NOISE ? na : nullptr, qa), eb = quant_col16<FMT>(vb, NOISE ? nb : nullptr, qb);
+    uint32_t ea, eb;
+    quant_col16<FMT>(v, ma, mb, NOISE ? na : nullptr, NOISE ? nb : nullptr, qa, qb, ea, eb);
     if (c0 + c < p.C && r0 + sub * 16 < p.Rp) {
       if constexpr (FMT == E4M3) {
         uint8_t* dst = p.q_col + (long long)(c0 + c) * p.Rp + r0 + sub * 16;

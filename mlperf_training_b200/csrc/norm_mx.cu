@@ -128,7 +128,7 @@ B200_API int b200_norm_mx(const void* x, const void* residual, const void* w, vo
   q.rstd = (const float*)rstd; q.w = (const __nv_bfloat16*)w;
   q.q_col = (uint8_t*)q_col; q.sf_col = (uint8_t*)sf_col; q.col_tile = col_tile;
   q.Rp = (T + 127) / 128 * 128;
-  b200::launch(mxq::mx_tile_kernel<mxq::E4M3, true, false>, dim3((D + 127) / 128, (T + 127) / 128), 256, 0, st, q);
+  b200::launch(mxq::mx_tile_kernel<mxq::E4M3, true, false, false>, dim3((D + 127) / 128, (T + 127) / 128), 256, 0, st, q);
   b200::count_launch();
   return b200::check_launch("norm_mx(columns)");
 }

@@ -12,47 +12,114 @@
 
 namespace {
 
-// Codes to values: a thread holds eight neighbouring elements.  out_f32: 0 bf16, 1 fp32.
-template <int FMT>
+// Codes to values, written to bf16 or fp32.  A lane has eight neighbouring elements, a warp eight consecutive rows: their scale bytes are 16
+// bytes apart in one atom (tile rows are multiples of 16), so one division places all of them, and eight loads of each kind are in flight.
+// An e2m1 code becomes a bf16 by two table look-ups of its bytes (prmt) and its sign; the product with the scale, a power of two, is exact.
+constexpr int DQ_ROWS = 8;
+
+B200_DEVICE uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
+// elements 0, 1 and 2, 3 of four codes in the low half of c, as bf16 pairs
+B200_DEVICE void e2m1x4_bf16(uint32_t c, uint32_t& w01, uint32_t& w23) {
+  const uint32_t m = c & 0x7777u;
+  const uint32_t lo = prmt(0xc0800000u, 0xc0804000u, m), hi = prmt(0x3f3f3f00u, 0x40404040u, m);   // 0 .5 1 1.5 | 2 3 4 6
+  w01 = prmt(lo, hi, 0x5140u) | (c << 12 & 0x8000u) | (c << 24 & 0x80000000u);
+  w23 = prmt(lo, hi, 0x7362u) | (c << 4 & 0x8000u) | (c << 16 & 0x80000000u);
+}
+B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int FMT, bool F32>
 __global__ void __launch_bounds__(256)
-mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, void* __restrict__ out, long long R, int K, int tile_rows,
-                  int out_f32) {
+mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, void* __restrict__ out, int R, int K, int tile_rows) {
   b200::begin_kernel();
   const int vecs = K >> 3;
-  const long long n = R * vecs;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const long long r = i / vecs;
-    const int v = (int)(i - r * vecs);
-    const uint32_t e = sf[mxq::sf_offset(r, v >> 2, tile_rows, (tile_rows + 127) >> 7, (K + 127) >> 7)];
-    const float s = e == 255u ? __uint_as_float(0x7fffffffu) : e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23);
-    float f[8];
-    if constexpr (FMT == mxq::E4M3) {
-      const uint2 c = *reinterpret_cast<const uint2*>(q + i * 8);
+  const int v = blockIdx.x * 32 + (threadIdx.x & 31);
+  if (v >= vecs) return;
+  for (long long r0 = ((long long)blockIdx.y * 8 + (threadIdx.x >> 5)) * DQ_ROWS; r0 < R; r0 += (long long)gridDim.y * 8 * DQ_ROWS) {
+    const uint8_t* s0 = sf + mxq::sf_offset(r0, v >> 2, tile_rows, (tile_rows + 127) >> 7, (K + 127) >> 7);
+    uint32_t e[DQ_ROWS];
+    uint2 c[DQ_ROWS];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? c.x : c.y) >> (16 * (j & 1))), __NV_E4M3);
-        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        f[2 * j] = g.x * s;
-        f[2 * j + 1] = g.y * s;
-      }
-    } else {
-      const uint32_t c = *reinterpret_cast<const uint32_t*>(q + i * 4);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6: code m >= 2 is (1 + (m & 1) / 2) * 2^(m / 2 - 1)
-        const uint32_t m = (c >> (4 * j)) & 7u, sign = ((c >> (4 * j)) & 8u) << 28;
-        const uint32_t b = m >= 2u ? ((126u + (m >> 1)) << 23 | (m & 1u) << 22) : m * 0x3f000000u;
-        f[j] = __uint_as_float(b | sign) * s;
+    for (int i = 0; i < DQ_ROWS; ++i) {
+      const bool in = r0 + i < R;
+      e[i] = in ? s0[i * 16] : 0u;
+      c[i] = make_uint2(0u, 0u);
+      if (in) {
+        if constexpr (FMT == mxq::E4M3) c[i] = *reinterpret_cast<const uint2*>(q + (r0 + i) * K + v * 8);
+        else c[i].x = *reinterpret_cast<const uint32_t*>(q + (((r0 + i) * K) >> 1) + v * 4);
       }
     }
-    if (out_f32) {
-      float4* o = reinterpret_cast<float4*>((float*)out + i * 8);
-      o[0] = make_float4(f[0], f[1], f[2], f[3]);
-      o[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-      reinterpret_cast<uint4*>(out)[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+#pragma unroll
+    for (int i = 0; i < DQ_ROWS; ++i) {
+      if (r0 + i >= R) break;
+      // 2^(e - 127) as bf16: 0 is 2^-127, below the normal numbers; 255 is a NaN
+      const uint32_t sb = e[i] == 255u ? 0x7fc0u : e[i] == 0u ? 0x0040u : e[i] << 7;
+      const float s = __uint_as_float(sb << 16);
+      const long long at = (r0 + i) * K + v * 8;
+      float f[8];
+      uint32_t w[4];
+      if constexpr (FMT == mxq::E4M3) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? c[i].x : c[i].y) >> (16 * (j & 1))), __NV_E4M3);
+          const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          f[2 * j] = g.x * s;
+          f[2 * j + 1] = g.y * s;
+          if constexpr (!F32) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+        }
+      } else {
+        e2m1x4_bf16(c[i].x, w[0], w[1]);
+        e2m1x4_bf16(c[i].x >> 16, w[2], w[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (F32) {
+            const float2 g = unpack_bf16x2(w[j]);
+            f[2 * j] = g.x * s;
+            f[2 * j + 1] = g.y * s;
+          } else {
+            w[j] = mul_bf16x2(w[j], sb | sb << 16);
+          }
+        }
+      }
+      if constexpr (F32) {
+        float4* o = reinterpret_cast<float4*>((float*)out + at);
+        o[0] = make_float4(f[0], f[1], f[2], f[3]);
+        o[1] = make_float4(f[4], f[5], f[6], f[7]);
+      } else {
+        *reinterpret_cast<uint4*>((__nv_bfloat16*)out + at) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
   }
+}
+
+template <int FMT>
+void launch_dequant(dim3 grid, cudaStream_t st, const void* q, const void* sf, void* out, int R, int K, int tile_rows, int out_f32) {
+  if (out_f32) b200::launch(mx_dequant_kernel<FMT, true>, grid, 256, 0, st, (const uint8_t*)q, (const uint8_t*)sf, out, R, K, tile_rows);
+  else b200::launch(mx_dequant_kernel<FMT, false>, grid, 256, 0, st, (const uint8_t*)q, (const uint8_t*)sf, out, R, K, tile_rows);
+}
+
+template <bool NOISE, bool HAD>
+int launch_tile(dim3 grid, cudaStream_t st, const mxq::TileArgs& p) {
+  const auto kern = mxq::mx_tile_kernel<mxq::E2M1, false, NOISE, HAD>;
+  const int dyn = NOISE ? mxq::NOISE_WORDS * 4 : 0;
+  if (NOISE) {
+    // (the tile of bytes comes on top of 36 KB of static shared memory: more than a launch gets unasked)
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dyn);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return b200::fail(728, "quant_mxfp4: cannot set %d bytes of shared memory: %s", dyn, cudaGetErrorString(e));
+      }
+      configured[dev & 63] = true;
+    }
+  }
+  b200::launch(kern, grid, 256, dyn, st, p);
+  return 0;
 }
 
 }  // namespace
@@ -69,40 +136,28 @@ B200_API int b200_quant_mxfp4(const void* x, long long ldx, int R, int C, const 
   if (R > 65535 * mxq::TILE) return b200::fail(724, "quant_mxfp4: R=%d rows are more than a launch covers", R);
   mxq::TileArgs p = {};
   p.x = (const __nv_bfloat16*)x; p.ldx = ldx; p.R = R; p.C = C;
-  p.noise = (const uint8_t*)noise; p.hadamard = hadamard;
+  p.noise = (const uint8_t*)noise;
   p.q_row = (uint8_t*)q_row; p.sf_row = (uint8_t*)sf_row; p.row_tile = row_tile;
   p.q_col = (uint8_t*)q_col; p.sf_col = (uint8_t*)sf_col; p.col_tile = col_tile;
   p.Rp = (R + 31) / 32 * 32;
   const dim3 grid((C + mxq::TILE - 1) / mxq::TILE, (R + mxq::TILE - 1) / mxq::TILE);
-  if (noise != nullptr) {
-    // (the tile of bytes comes on top of 36 KB of static shared memory: more than a launch gets unasked)
-    static bool configured[64] = {false};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!configured[dev & 63]) {
-      const cudaError_t e = cudaFuncSetAttribute(mxq::mx_tile_kernel<mxq::E2M1, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, mxq::NOISE_WORDS * 4);
-      if (e != cudaSuccess) {
-        cudaGetLastError();
-        return b200::fail(728, "quant_mxfp4: cannot set %d bytes of shared memory: %s", mxq::NOISE_WORDS * 4, cudaGetErrorString(e));
-      }
-      configured[dev & 63] = true;
-    }
-    b200::launch(mxq::mx_tile_kernel<mxq::E2M1, false, true>, grid, 256, mxq::NOISE_WORDS * 4, (cudaStream_t)stream, p);
-  }
-  else b200::launch(mxq::mx_tile_kernel<mxq::E2M1, false, false>, grid, 256, 0, (cudaStream_t)stream, p);
+  int r;
+  if (noise != nullptr) r = hadamard ? launch_tile<true, true>(grid, (cudaStream_t)stream, p) : launch_tile<true, false>(grid, (cudaStream_t)stream, p);
+  else r = hadamard && q_col != nullptr ? launch_tile<false, true>(grid, (cudaStream_t)stream, p) : launch_tile<false, false>(grid, (cudaStream_t)stream, p);
+  if (r) return r;
   b200::count_launch();
   return b200::check_launch("quant_mxfp4");
 }
 
 // Values of an operand: q [R, K] e4m3 (fmt 0) or [R, K / 2] e2m1 (fmt 1) codes, dense; out [R, K] bf16 or fp32, dense.
-B200_API int b200_dequant_mx(const void* q, const void* sf, void* out, long long R, int K, int tile_rows, int fmt, int out_f32, void* stream) {
-  if (R <= 0 || K <= 0 || K % 32 != 0) return b200::fail(725, "dequant_mx: R=%lld must be positive and K=%d a positive multiple of 32", R, K);
+B200_API int b200_dequant_mx(const void* q, const void* sf, void* out, int R, int K, int tile_rows, int fmt, int out_f32, void* stream) {
+  if (R <= 0 || K <= 0 || K % 32 != 0) return b200::fail(725, "dequant_mx: R=%d must be positive and K=%d a positive multiple of 32", R, K);
   if (tile_rows <= 0 || tile_rows % 16 != 0) return b200::fail(726, "dequant_mx: tile rows must be positive multiples of 16");
   if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0) return b200::fail(727, "dequant_mx: codes and output must be 16-byte aligned");
-  const long long blocks = (R * (K / 8) + 255) / 256, most = b200::sm_count() * 32ll;
-  const dim3 grid((unsigned)(blocks < most ? blocks : most));
-  if (fmt == mxq::E4M3) b200::launch(mx_dequant_kernel<mxq::E4M3>, grid, 256, 0, (cudaStream_t)stream, (const uint8_t*)q, (const uint8_t*)sf, out, R, K, tile_rows, out_f32);
-  else b200::launch(mx_dequant_kernel<mxq::E2M1>, grid, 256, 0, (cudaStream_t)stream, (const uint8_t*)q, (const uint8_t*)sf, out, R, K, tile_rows, out_f32);
+  const int rows = (R - 1) / (8 * DQ_ROWS) + 1;
+  const dim3 grid((K / 8 + 31) / 32, rows < 65535 ? rows : 65535);
+  if (fmt == mxq::E4M3) launch_dequant<mxq::E4M3>(grid, (cudaStream_t)stream, q, sf, out, R, K, tile_rows, out_f32);
+  else launch_dequant<mxq::E2M1>(grid, (cudaStream_t)stream, q, sf, out, R, K, tile_rows, out_f32);
   b200::count_launch();
   return b200::check_launch("dequant_mx");
 }

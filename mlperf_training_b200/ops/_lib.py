@@ -84,7 +84,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_quant_mxfp8": [P, L, I, I, P, P, I, P, P, I, P, P],
         "b200_gemm_mxfp8": [P, P, P, P, P, I, I, I, L, L, L, I, I, P, P, L, F, P, L, P],
         "b200_quant_mxfp4": [P, L, I, I, P, I, P, P, I, P, P, I, P],
-        "b200_dequant_mx": [P, P, P, L, I, I, I, I, P],
+        "b200_dequant_mx": [P, P, P, I, I, I, I, I, P],
         "b200_gemm_mxfp4": [P, P, P, P, P, I, I, I, L, L, L, I, I, P, P, L, F, P, L, P],
         "b200_norm_mx": [P, P, P, P, P, I, I, F, P, P, I, P, P, I, P],
         "b200_gemm_gated": [P, P, P, P, I, I, I, L, L, L, L, I, P],
