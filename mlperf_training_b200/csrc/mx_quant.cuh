@@ -4,8 +4,7 @@
 // Scale: the smallest power of two s with amax / s <= vmax (448 = 1.75 * 2^8, 6 = 1.5 * 2^2), biased by 127; at least 1 (2^-126) where amax
 // is not zero, 0 where it is.  255 (NaN) for a block that holds an infinity or a NaN: e2m1 has neither, and with any other scale the value
 // would come back as an ordinary number.  No element saturates: amax / s <= vmax.
-// Magnitudes are compared so that a NaN is kept: as integers (their bits less the sign: a NaN is above infinity, both above every number),
-// or by the maximum that hands a NaN on.
+// Magnitudes are compared by the maximum that hands a NaN on, and as integers (a NaN's bits are above infinity's, both above every number's).
 #pragma once
 #include <cuda_fp8.h>
 
@@ -44,14 +43,29 @@ B200_DEVICE uint32_t pack8_e2m1(const float (&v)[8]) {
   return r;
 }
 // y (|y| <= 6) to a value of e2m1: |y| / quantum + (u + 1/2) / 256 rounded down, u a random byte.  The expectation over u is y to within
-// 1/512 of a quantum, and a value of the format stays as it is.  The quantum is the upper bit of the fraction, so this is an integer addition
-// to the bits below it and a mask (a carry out of the fraction is the next power of two); below 1, where the quantum stays 0.5, one is added
-// first and taken off after.  No conversions: floor and int-to-float run at a quarter of the rate of these.
-// `u` is the word that holds the byte, `at` the byte's place in it.
+// 1/512 of a quantum, and a value of the format stays as it is.
+// y comes times 2^-126, which puts the smallest normal number of the format, 1, on the smallest one of fp32: e2m1's quantum is then the upper
+// bit of the fraction in both formats' normal and subnormal numbers alike, and the rounding is an integer addition below that bit and a mask (a
+// carry out of the fraction is the next power of two).  Seven instructions an element less than with floor, whose conversions run at a
+// quarter of the rate.  Returns the value times 2^-126.  `u` is the word that holds the byte, `at` the byte's place in it.
+constexpr float STOCH_DOWN = 1.17549435e-38f, STOCH_UP = 8.50705917e37f;      // 2^-126, 2^126
 B200_DEVICE float round_stochastic(float y, uint32_t u, int at) {
-  const float a = fabsf(y), one = a < 1.f ? 1.f : 0.f;
-  const uint32_t z = (__float_as_uint(a + one) + (((u >> (8 * at)) & 0xffu) << 14) + 0x2000u) & 0xffc00000u;
-  return __uint_as_float(__float_as_uint(__uint_as_float(z) - one) | (__float_as_uint(y) & 0x80000000u));
+  const uint32_t n = __byte_perm(u, 0x80u, 0x5504 | at << 4);                  // 256 u + 128
+  return __uint_as_float((__float_as_uint(y) + n * 64u) & 0x81c00000u);
+}
+// eight of them to codes
+B200_DEVICE uint32_t pack8_e2m1_stochastic(const float2 (&y)[4], uint32_t u0, uint32_t u1) {
+  const float2 dn = make_float2(STOCH_DOWN, STOCH_DOWN), up = make_float2(STOCH_UP, STOCH_UP);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 d = fmul2(y[i], dn);
+    const uint32_t u = i < 2 ? u0 : u1;
+    const float2 r = fmul2(make_float2(round_stochastic(d.x, u, 2 * (i & 1)), round_stochastic(d.y, u, 2 * (i & 1) + 1)), up);
+    v[2 * i] = r.x;
+    v[2 * i + 1] = r.y;
+  }
+  return pack8_e2m1(v);
 }
 
 // byte offset of scale (row r of the operand, scale column kc) in the atom layout the block-scaled GEMMs read (quant_mxfp8.cu)
@@ -62,51 +76,47 @@ B200_DEVICE long long sf_offset(long long r, int kc, int tile_rows, int atoms_pe
   return ((tile * k_groups + (kc >> 2)) * atoms_per_tile + atom) * 512 + (ra & 31) * 16 + (ra >> 5) * 4 + (kc & 3);
 }
 
-// Largest magnitude of bf16 pairs, halves by themselves, as integers.
-B200_DEVICE uint32_t amax2(uint32_t m, uint32_t pair) { return __vmaxu2(m, pair & 0x7fff7fffu); }
+// Largest magnitude of bf16 pairs, halves by themselves; a NaN is handed on.
+B200_DEVICE uint32_t amax2(uint32_t m, uint32_t pair) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&m), __habs2(*reinterpret_cast<__nv_bfloat162*>(&pair)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 // Eight scaled values (eight elements of a 32-block, |y| <= vmax) to codes; noise: eight random bytes or null (e2m1: codes in q.x).
 template <int FMT>
-B200_DEVICE uint2 codes8(float (&y)[8], const uint2* noise) {
-  if constexpr (FMT == E4M3) {
-    return make_uint2(pack4_e4m3(y[0], y[1], y[2], y[3]), pack4_e4m3(y[4], y[5], y[6], y[7]));
-  } else {
-    if (noise != nullptr) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = round_stochastic(y[i], i < 4 ? noise->x : noise->y, i & 3);
-    }
-    return make_uint2(pack8_e2m1(y), 0u);
-  }
+B200_DEVICE uint2 codes8(const float2 (&y)[4], const uint2* noise) {
+  if constexpr (FMT == E4M3) return make_uint2(pack4_e4m3(y[0].x, y[0].y, y[1].x, y[1].y), pack4_e4m3(y[2].x, y[2].y, y[3].x, y[3].y));
+  if (noise != nullptr) return make_uint2(pack8_e2m1_stochastic(y, noise->x, noise->y), 0u);
+  const float v[8] = {y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
+  return make_uint2(pack8_e2m1(v), 0u);
 }
 
 // Eight values of a 32-block whose other values are in the three neighbouring lanes (lane / 4 is the block): codes in q, returns the scale
 // byte.  From fp32 values, and from bf16 as they are (magnitudes compared in pairs, scaled in pairs).
 template <int FMT>
 B200_DEVICE uint32_t quant_row8(const float (&v)[8], const uint2* noise, uint2& q) {
-  float m = fabsf(v[0]);
+  float m = 0.f;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmax_nan(m, fabsf(v[i]));
+  for (int i = 0; i < 8; ++i) m = fmax_nan(m, fabsf(v[i]));
   m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const uint32_t e = e8m0<FMT>(abs_bits(m));
   const float inv = inv_scale(e);
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = v[i] * inv;
+  const float2 y[4] = {make_float2(v[0] * inv, v[1] * inv), make_float2(v[2] * inv, v[3] * inv), make_float2(v[4] * inv, v[5] * inv),
+                       make_float2(v[6] * inv, v[7] * inv)};
   q = codes8<FMT>(y, noise);
   return e;
 }
 template <int FMT>
 B200_DEVICE uint32_t quant_row8(const uint4& v, const uint2* noise, uint2& q) {
-  uint32_t m = amax2(amax2(amax2(v.x & 0x7fff7fffu, v.y), v.z), v.w);
-  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  uint32_t m = amax2(amax2(amax2(amax2(0u, v.x), v.y), v.z), v.w);
+  m = amax2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = amax2(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const uint32_t e = e8m0<FMT>(max(m << 16, m & 0xffff0000u));
   const float inv = inv_scale(e);
   const float2 i2 = make_float2(inv, inv);
-  const float2 a = fmul2(unpack_bf16x2(v.x), i2), b = fmul2(unpack_bf16x2(v.y), i2);
-  const float2 c = fmul2(unpack_bf16x2(v.z), i2), d = fmul2(unpack_bf16x2(v.w), i2);
-  float y[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+  const float2 y[4] = {fmul2(unpack_bf16x2(v.x), i2), fmul2(unpack_bf16x2(v.y), i2), fmul2(unpack_bf16x2(v.z), i2),
+                       fmul2(unpack_bf16x2(v.w), i2)};
   q = codes8<FMT>(y, noise);
   return e;
 }
@@ -151,18 +161,18 @@ B200_DEVICE void quant_col16(float2 (&v)[16], uint32_t ma, uint32_t mb, const ui
     a[2] = a[3] = b[2] = b[3] = 0u;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float x[8], y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = v[8 * h + i].x;
-        y[i] = v[8 * h + i].y;
-        if (na != nullptr) {
-          x[i] = round_stochastic(x[i], na[2 * h + (i >> 2)], i & 3);
-          y[i] = round_stochastic(y[i], nb[2 * h + (i >> 2)], i & 3);
-        }
+      const float2* w = v + 8 * h;
+      if (na != nullptr) {
+        const float2 x[4] = {make_float2(w[0].x, w[1].x), make_float2(w[2].x, w[3].x), make_float2(w[4].x, w[5].x), make_float2(w[6].x, w[7].x)};
+        const float2 y[4] = {make_float2(w[0].y, w[1].y), make_float2(w[2].y, w[3].y), make_float2(w[4].y, w[5].y), make_float2(w[6].y, w[7].y)};
+        a[h] = pack8_e2m1_stochastic(x, na[2 * h], na[2 * h + 1]);
+        b[h] = pack8_e2m1_stochastic(y, nb[2 * h], nb[2 * h + 1]);
+      } else {
+        const float x[8] = {w[0].x, w[1].x, w[2].x, w[3].x, w[4].x, w[5].x, w[6].x, w[7].x};
+        const float y[8] = {w[0].y, w[1].y, w[2].y, w[3].y, w[4].y, w[5].y, w[6].y, w[7].y};
+        a[h] = pack8_e2m1(x);
+        b[h] = pack8_e2m1(y);
       }
-      a[h] = pack8_e2m1(x);
-      b[h] = pack8_e2m1(y);
     }
   }
   qa = make_uint4(a[0], a[1], a[2], a[3]);
@@ -209,8 +219,9 @@ mx_tile_kernel(const TileArgs p) {
   const int sub_row = lane >> 4, chunk = lane & 15;
   const bool col_live = c0 + chunk * 8 < p.C;
   const bool rows = p.q_row != nullptr, cols = p.q_col != nullptr;
+  const int row_lim = (int)min((long long)TILE, p.R - r0);            // rows of this tile
   if constexpr (SCALED) {
-    if (tid < TILE) rstd_s[tid] = r0 + tid < p.R ? p.rstd[r0 + tid] : 0.f;
+    if (tid < TILE) rstd_s[tid] = tid < row_lim ? p.rstd[r0 + tid] : 0.f;
     __syncthreads();
   }
   float w8[8];
@@ -219,17 +230,25 @@ mx_tile_kernel(const TileArgs p) {
     const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
     w8[0] = a.x; w8[1] = a.y; w8[2] = b.x; w8[3] = b.y; w8[4] = c.x; w8[5] = c.y; w8[6] = d.x; w8[7] = d.y;
   }
+  // (addresses advance by sixteen rows; a multiplication and a 64-bit comparison a vector were a fifth of the instructions)
+  const int t0 = warp * 2 + sub_row;
+  const __nv_bfloat16* src = p.x + (r0 + t0) * p.ldx + c0 + chunk * 8;
+  const uint8_t* nsrc = NOISE ? p.noise + (r0 + t0) * p.C + c0 + chunk * 8 : nullptr;
+  uint8_t* qdst = rows ? p.q_row + (FMT == E4M3 ? (r0 + t0) * p.C + c0 + chunk * 8 : (((r0 + t0) * p.C + c0) >> 1) + chunk * 4) : nullptr;
+  const long long step = 16 * p.ldx, nstep = 16ll * p.C, qstep = FMT == E4M3 ? 16ll * p.C : 8ll * p.C;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint4 xv[4];
     uint2 nv[NOISE ? 4 : 1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const long long r = r0 + (h * 4 + i) * 16 + warp * 2 + sub_row;
-      const bool live = col_live && r < p.R;
-      xv[i] = live ? *reinterpret_cast<const uint4*>(p.x + r * p.ldx + c0 + chunk * 8) : make_uint4(0u, 0u, 0u, 0u);
-      if constexpr (NOISE)
-        nv[i] = live ? *reinterpret_cast<const uint2*>(p.noise + r * p.C + c0 + chunk * 8) : make_uint2(0x80808080u, 0x80808080u);
+      const bool live = col_live && (h * 4 + i) * 16 + t0 < row_lim;
+      xv[i] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+      src += step;
+      if constexpr (NOISE) {
+        nv[i] = live ? *reinterpret_cast<const uint2*>(nsrc) : make_uint2(0x80808080u, 0x80808080u);
+        nsrc += nstep;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -248,10 +267,11 @@ mx_tile_kernel(const TileArgs p) {
         } else {
           e = quant_row8<FMT>(xv[i], noise, q);
         }
-        if (col_live && r0 + r < p.R) {
-          if constexpr (FMT == E4M3) *reinterpret_cast<uint2*>(p.q_row + (r0 + r) * p.C + c0 + chunk * 8) = q;
-          else *reinterpret_cast<uint32_t*>(p.q_row + (((r0 + r) * p.C + c0) >> 1) + chunk * 4) = q.x;
+        if (col_live && r < row_lim) {
+          if constexpr (FMT == E4M3) *reinterpret_cast<uint2*>(qdst) = q;
+          else *reinterpret_cast<uint32_t*>(qdst) = q.x;
         }
+        qdst += qstep;
         if ((chunk & 3) == 0) sfs[0][r][chunk >> 2] = (uint8_t)e;
       }
       if (cols) {
@@ -261,7 +281,7 @@ mx_tile_kernel(const TileArgs p) {
     }
   }
   __syncthreads();
-  if (rows && tid < TILE && r0 + tid < p.R) {
+  if (rows && tid < row_lim) {
     const long long o = sf_offset(r0 + tid, c0 >> 5, p.row_tile, (p.row_tile + 127) >> 7, (p.C + 127) >> 7);
     *reinterpret_cast<uint32_t*>(p.sf_row + o) = *reinterpret_cast<const uint32_t*>(&sfs[0][tid][0]);
   }
