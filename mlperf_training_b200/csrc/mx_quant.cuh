@@ -76,48 +76,50 @@ B200_DEVICE long long sf_offset(long long r, int kc, int tile_rows, int atoms_pe
   return ((tile * k_groups + (kc >> 2)) * atoms_per_tile + atom) * 512 + (ra & 31) * 16 + (ra >> 5) * 4 + (kc & 3);
 }
 
+// max(m, |a|, |b|), a NaN handed on
+B200_DEVICE float fmax3_nan(float m, float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+  return y;
+}
 // Largest magnitude of bf16 pairs, halves by themselves; a NaN is handed on.
 B200_DEVICE uint32_t amax2(uint32_t m, uint32_t pair) {
   const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&m), __habs2(*reinterpret_cast<__nv_bfloat162*>(&pair)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Eight scaled values (eight elements of a 32-block, |y| <= vmax) to codes; noise: eight random bytes or null (e2m1: codes in q.x).
-template <int FMT>
-B200_DEVICE uint2 codes8(const float2 (&y)[4], const uint2* noise) {
-  if constexpr (FMT == E4M3) return make_uint2(pack4_e4m3(y[0].x, y[0].y, y[1].x, y[1].y), pack4_e4m3(y[2].x, y[2].y, y[3].x, y[3].y));
-  if (noise != nullptr) return make_uint2(pack8_e2m1_stochastic(y, noise->x, noise->y), 0u);
-  const float v[8] = {y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
-  return make_uint2(pack8_e2m1(v), 0u);
-}
-
 // Eight values of a 32-block whose other values are in the three neighbouring lanes (lane / 4 is the block): codes in q, returns the scale
-// byte.  From fp32 values, and from bf16 as they are (magnitudes compared in pairs, scaled in pairs).
-template <int FMT>
-B200_DEVICE uint32_t quant_row8(const float (&v)[8], const uint2* noise, uint2& q) {
+// byte.  From fp32 values to e4m3, and from bf16 as they are (magnitudes compared and values scaled in pairs) to e2m1; noise: eight random
+// bytes, null for round to nearest.
+// (e4m3: the values are z * s, s the same for the block.  s and the scale are not multiplied into one factor: that overflows for small blocks.)
+B200_DEVICE uint32_t quant_row8_e4m3(const float2 (&z)[4], float s, uint2& q) {
   float m = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmax_nan(m, fabsf(v[i]));
+  for (int i = 0; i < 4; ++i) m = fmax3_nan(m, z[i].x, z[i].y);
   m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const uint32_t e = e8m0<FMT>(abs_bits(m));
+  const uint32_t e = e8m0<E4M3>(abs_bits(m * s));
   const float inv = inv_scale(e);
-  const float2 y[4] = {make_float2(v[0] * inv, v[1] * inv), make_float2(v[2] * inv, v[3] * inv), make_float2(v[4] * inv, v[5] * inv),
-                       make_float2(v[6] * inv, v[7] * inv)};
-  q = codes8<FMT>(y, noise);
+  const float2 s2 = make_float2(s, s), i2 = make_float2(inv, inv);
+  const float2 a = fmul2(fmul2(z[0], s2), i2), b = fmul2(fmul2(z[1], s2), i2), c = fmul2(fmul2(z[2], s2), i2), d = fmul2(fmul2(z[3], s2), i2);
+  q = make_uint2(pack4_e4m3(a.x, a.y, b.x, b.y), pack4_e4m3(c.x, c.y, d.x, d.y));
   return e;
 }
-template <int FMT>
-B200_DEVICE uint32_t quant_row8(const uint4& v, const uint2* noise, uint2& q) {
+B200_DEVICE uint32_t quant_row8_e2m1(const uint4& v, const uint2* noise, uint32_t& q) {
   uint32_t m = amax2(amax2(amax2(amax2(0u, v.x), v.y), v.z), v.w);
   m = amax2(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = amax2(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const uint32_t e = e8m0<FMT>(max(m << 16, m & 0xffff0000u));
+  const uint32_t e = e8m0<E2M1>(max(m << 16, m & 0xffff0000u));
   const float inv = inv_scale(e);
   const float2 i2 = make_float2(inv, inv);
   const float2 y[4] = {fmul2(unpack_bf16x2(v.x), i2), fmul2(unpack_bf16x2(v.y), i2), fmul2(unpack_bf16x2(v.z), i2),
                        fmul2(unpack_bf16x2(v.w), i2)};
-  q = codes8<FMT>(y, noise);
+  if (noise != nullptr) {
+    q = pack8_e2m1_stochastic(y, noise->x, noise->y);
+  } else {
+    const float f[8] = {y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
+    q = pack8_e2m1(f);
+  }
   return e;
 }
 
@@ -139,9 +141,9 @@ B200_DEVICE void hadamard16(float2 (&v)[16]) {
 
 // Sixteen rows of two columns; the other halves of the 32-blocks are in the neighbouring lane.  `m`: the bits of the largest magnitudes of the
 // two (this lane's rows).  noise: word i holds the bytes of rows 4 i .. 4 i + 3 (na: first column, nb: second), null for nearest.  Codes in
-// qa, qb (e4m3: 16 bytes, e2m1: two words), scale bytes in ea, eb.
+// qa, qb (e4m3: 16 bytes, e2m1: two words), scale bytes in ea, eb.  e4m3: the values are v * w (w: one factor per column).
 template <int FMT>
-B200_DEVICE void quant_col16(float2 (&v)[16], uint32_t ma, uint32_t mb, const uint32_t* na, const uint32_t* nb, uint4& qa, uint4& qb,
+B200_DEVICE void quant_col16(float2 (&v)[16], float2 w, uint32_t ma, uint32_t mb, const uint32_t* na, const uint32_t* nb, uint4& qa, uint4& qb,
                              uint32_t& ea, uint32_t& eb) {
   ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
   mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
@@ -149,7 +151,7 @@ B200_DEVICE void quant_col16(float2 (&v)[16], uint32_t ma, uint32_t mb, const ui
   eb = e8m0<FMT>(mb);
   const float2 inv = make_float2(inv_scale(ea), inv_scale(eb));
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = fmul2(v[i], inv);
+  for (int i = 0; i < 16; ++i) v[i] = fmul2(FMT == E4M3 ? fmul2(v[i], w) : v[i], inv);
   uint32_t a[4], b[4];
   if constexpr (FMT == E4M3) {
 #pragma unroll
@@ -180,15 +182,13 @@ B200_DEVICE void quant_col16(float2 (&v)[16], uint32_t ma, uint32_t mb, const ui
 }
 
 // ----------------------------------------------------------------------------------
-// 128 x 128 tile: rows pass and columns pass (used by quant_mxfp4.cu and norm_mx.cu)
+// 128 x 128 tile to e2m1: rows pass and columns pass
 // ----------------------------------------------------------------------------------
 struct TileArgs {
   const __nv_bfloat16* x;         // [R, C], pitch ldx
   long long ldx;
   int R, C;
   const uint8_t* noise;           // [R, C] dense, or null
-  const float* rstd;              // SCALED: [R], x is multiplied by rstd[row] * w[column] first
-  const __nv_bfloat16* w;
   uint8_t* q_row; uint8_t* sf_row; int row_tile;
   uint8_t* q_col; uint8_t* sf_col; int col_tile;
   int Rp;                         // rows of the column copy's contraction: R filled up with zeros
@@ -205,14 +205,13 @@ B200_DEVICE int noise_off(int r) { return r * NPITCH_W + (r >> 4) * 2; }
 // grid (ceil(C / 128), ceil(R / 128)), 256 threads.  C is a multiple of 32; rows past R and columns past C read as zero and are not written,
 // but for the zero codes and scale bytes that fill the copies' last 32 rows and last scale word: an operand read by a GEMM holds no byte
 // inside its contraction that was not written here.
-template <int FMT, bool SCALED, bool NOISE, bool HAD>
+template <bool NOISE, bool HAD>
 __global__ void __launch_bounds__(256)
 mx_tile_kernel(const TileArgs p) {
   b200::begin_kernel();
   __shared__ __align__(16) uint32_t tile[TILE_WORDS];
   extern __shared__ __align__(16) uint32_t noise_s[];     // NOISE: NOISE_WORDS
   __shared__ __align__(4) uint8_t sfs[2][TILE][4];
-  __shared__ float rstd_s[SCALED ? TILE : 1];
   const int c0 = blockIdx.x * TILE;
   const long long r0 = (long long)blockIdx.y * TILE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -220,22 +219,12 @@ mx_tile_kernel(const TileArgs p) {
   const bool col_live = c0 + chunk * 8 < p.C;
   const bool rows = p.q_row != nullptr, cols = p.q_col != nullptr;
   const int row_lim = (int)min((long long)TILE, p.R - r0);            // rows of this tile
-  if constexpr (SCALED) {
-    if (tid < TILE) rstd_s[tid] = tid < row_lim ? p.rstd[r0 + tid] : 0.f;
-    __syncthreads();
-  }
-  float w8[8];
-  if constexpr (SCALED) {
-    const uint4 u = col_live ? *reinterpret_cast<const uint4*>(p.w + c0 + chunk * 8) : make_uint4(0u, 0u, 0u, 0u);
-    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-    w8[0] = a.x; w8[1] = a.y; w8[2] = b.x; w8[3] = b.y; w8[4] = c.x; w8[5] = c.y; w8[6] = d.x; w8[7] = d.y;
-  }
   // (addresses advance by sixteen rows; a multiplication and a 64-bit comparison a vector were a fifth of the instructions)
   const int t0 = warp * 2 + sub_row;
   const __nv_bfloat16* src = p.x + (r0 + t0) * p.ldx + c0 + chunk * 8;
   const uint8_t* nsrc = NOISE ? p.noise + (r0 + t0) * p.C + c0 + chunk * 8 : nullptr;
-  uint8_t* qdst = rows ? p.q_row + (FMT == E4M3 ? (r0 + t0) * p.C + c0 + chunk * 8 : (((r0 + t0) * p.C + c0) >> 1) + chunk * 4) : nullptr;
-  const long long step = 16 * p.ldx, nstep = 16ll * p.C, qstep = FMT == E4M3 ? 16ll * p.C : 8ll * p.C;
+  uint8_t* qdst = rows ? p.q_row + (((r0 + t0) * p.C + c0) >> 1) + chunk * 4 : nullptr;
+  const long long step = 16 * p.ldx, nstep = 16ll * p.C, qstep = 8ll * p.C;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint4 xv[4];
@@ -254,23 +243,9 @@ mx_tile_kernel(const TileArgs p) {
     for (int i = 0; i < 4; ++i) {
       const int r = (h * 4 + i) * 16 + warp * 2 + sub_row;
       if (rows) {
-        uint2 q;
-        uint32_t e;
-        const uint2* noise = NOISE ? &nv[NOISE ? i : 0] : nullptr;
-        if constexpr (SCALED) {
-          const float2 a = unpack_bf16x2(xv[i].x), b = unpack_bf16x2(xv[i].y), c = unpack_bf16x2(xv[i].z), d = unpack_bf16x2(xv[i].w);
-          float v[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-          const float s = rstd_s[r];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = v[j] * s * w8[j];
-          e = quant_row8<FMT>(v, noise, q);
-        } else {
-          e = quant_row8<FMT>(xv[i], noise, q);
-        }
-        if (col_live && r < row_lim) {
-          if constexpr (FMT == E4M3) *reinterpret_cast<uint2*>(qdst) = q;
-          else *reinterpret_cast<uint32_t*>(qdst) = q.x;
-        }
+        uint32_t q;
+        const uint32_t e = quant_row8_e2m1(xv[i], NOISE ? &nv[NOISE ? i : 0] : nullptr, q);
+        if (col_live && r < row_lim) *reinterpret_cast<uint32_t*>(qdst) = q;
         qdst += qstep;
         if ((chunk & 3) == 0) sfs[0][r][chunk >> 2] = (uint8_t)e;
       }
@@ -305,7 +280,7 @@ mx_tile_kernel(const TileArgs p) {
     float2 v[16];
     uint32_t ma = 0u, mb = 0u;
     const uint32_t* t = tile + tile_off(sub * 16) + cw;
-    if constexpr (!SCALED && !HAD) {
+    if constexpr (!HAD) {
       uint32_t m = 0u;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -318,37 +293,23 @@ mx_tile_kernel(const TileArgs p) {
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = unpack_bf16x2(t[i * PITCH_W]);
-      if constexpr (SCALED) {
-        const float2 w = c0 + c < p.C ? unpack_bf16x2(*reinterpret_cast<const uint32_t*>(p.w + c0 + c)) : make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float s = rstd_s[sub * 16 + i];
-          v[i] = fmul2(fmul2(v[i], make_float2(s, s)), w);
-        }
-      }
-      if constexpr (HAD) hadamard16(v);
+      hadamard16(v);
       float fa = 0.f, fb = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        fa = fmax_nan(fa, fabsf(v[i].x));
-        fb = fmax_nan(fb, fabsf(v[i].y));
+      for (int i = 0; i < 16; i += 2) {
+        fa = fmax3_nan(fa, v[i].x, v[i + 1].x);
+        fb = fmax3_nan(fb, v[i].y, v[i + 1].y);
       }
       ma = abs_bits(fa);
       mb = abs_bits(fb);
     }
     uint4 qa, qb;
     uint32_t ea, eb;
-    quant_col16<FMT>(v, ma, mb, NOISE ? na : nullptr, NOISE ? nb : nullptr, qa, qb, ea, eb);
+    quant_col16<E2M1>(v, make_float2(1.f, 1.f), ma, mb, NOISE ? na : nullptr, NOISE ? nb : nullptr, qa, qb, ea, eb);
     if (c0 + c < p.C && r0 + sub * 16 < p.Rp) {
-      if constexpr (FMT == E4M3) {
-        uint8_t* dst = p.q_col + (long long)(c0 + c) * p.Rp + r0 + sub * 16;
-        *reinterpret_cast<uint4*>(dst) = qa;
-        *reinterpret_cast<uint4*>(dst + p.Rp) = qb;
-      } else {
-        uint8_t* dst = p.q_col + (((long long)(c0 + c) * p.Rp + r0) >> 1) + sub * 8;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(qa.x, qa.y);
-        *reinterpret_cast<uint2*>(dst + (p.Rp >> 1)) = make_uint2(qb.x, qb.y);
-      }
+      uint8_t* dst = p.q_col + (((long long)(c0 + c) * p.Rp + r0) >> 1) + sub * 8;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(qa.x, qa.y);
+      *reinterpret_cast<uint2*>(dst + (p.Rp >> 1)) = make_uint2(qb.x, qb.y);
     }
     if ((sub & 1) == 0) { sfs[1][c][sub >> 1] = (uint8_t)ea; sfs[1][c + 1][sub >> 1] = (uint8_t)eb; }
   }

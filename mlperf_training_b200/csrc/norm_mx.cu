@@ -23,78 +23,283 @@ struct NormMxArgs {
   uint8_t* q_row; uint8_t* sf_row; int row_tile;      // or null
 };
 
-// NT threads hold a row, four 16-byte vectors each; a CTA of 256 threads has 256 / NT rows.
+// Sums of bf16 pairs, rounded once; what is normalised is the stored (rounded) sum.
+B200_DEVICE uint32_t add2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+B200_DEVICE uint4 add8(const uint4& a, const uint4& b) { return make_uint4(add2(a.x, b.x), add2(a.y, b.y), add2(a.z, b.z), add2(a.w, b.w)); }
+B200_DEVICE float2 sumsq8(const uint4& u, float2 s) {
+  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+  return ffma2(d, d, ffma2(c, c, ffma2(b, b, ffma2(a, a, s))));
+}
+// h * w of eight values: exact in fp32 (two factors of eight bits), so n = (h w) rstd is rounded once
+B200_DEVICE void mul8(const uint4& h, const uint4& w, float2 (&z)[4]) {
+  z[0] = fmul2(unpack_bf16x2(h.x), unpack_bf16x2(w.x));
+  z[1] = fmul2(unpack_bf16x2(h.y), unpack_bf16x2(w.y));
+  z[2] = fmul2(unpack_bf16x2(h.z), unpack_bf16x2(w.z));
+  z[3] = fmul2(unpack_bf16x2(h.w), unpack_bf16x2(w.w));
+}
+
+// The row copy alone.  A warp holds 512 columns of a row, two 16-byte vectors a lane: NT = 32, 64, .. 512 threads a row, 256 / NT rows a CTA.
+// The squares are added up in the order of the kernel below (lane, warp, then 512-column pieces in order), so a row has the same codes
+// whether the column copy is made with it or not.
 template <int NT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(NT > 256 ? NT : 256)
 norm_mx_rows_kernel(const NormMxArgs p) {
   b200::begin_kernel();
-  __shared__ float red[8];
-  const int t = threadIdx.x % NT, team = threadIdx.x / NT, warp = threadIdx.x >> 5;
-  const long long row = (long long)blockIdx.x * (256 / NT) + team;
+  constexpr int CTA = NT > 256 ? NT : 256;
+  __shared__ float red[CTA / 32];
+  const int t = threadIdx.x % NT, team = threadIdx.x / NT, lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * (CTA / NT) + team;
   const bool live = row < p.T;
-  uint4 v[4];
-  float ss = 0.f;
+  const int c0 = (t >> 5) * 512 + lane * 8;
+  const long long at = row * p.D + c0;
+  const bool in[2] = {c0 < p.D, c0 + 256 < p.D};
+  uint4 v[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int c = (t + i * NT) * 8;
-    v[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (live && c < p.D) v[i] = *reinterpret_cast<const uint4*>(p.x + row * p.D + c);
-  }
+  for (int j = 0; j < 2; ++j) v[j] = live && in[j] ? *reinterpret_cast<const uint4*>(p.x + at + j * 256) : make_uint4(0u, 0u, 0u, 0u);
   if (p.res != nullptr) {
+    uint4 u[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = (t + i * NT) * 8;
-      if (live && c < p.D) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p.res + row * p.D + c);
-        const float2 a0 = unpack_bf16x2(v[i].x), a1 = unpack_bf16x2(v[i].y), a2 = unpack_bf16x2(v[i].z), a3 = unpack_bf16x2(v[i].w);
-        const float2 b0 = unpack_bf16x2(u.x), b1 = unpack_bf16x2(u.y), b2 = unpack_bf16x2(u.z), b3 = unpack_bf16x2(u.w);
-        v[i] = make_uint4(pack_bf16x2(a0.x + b0.x, a0.y + b0.y), pack_bf16x2(a1.x + b1.x, a1.y + b1.y),
-                          pack_bf16x2(a2.x + b2.x, a2.y + b2.y), pack_bf16x2(a3.x + b3.x, a3.y + b3.y));
-        *reinterpret_cast<uint4*>(p.h + row * p.D + c) = v[i];      // what is normalised is the stored (rounded) sum
-      }
+    for (int j = 0; j < 2; ++j) u[j] = live && in[j] ? *reinterpret_cast<const uint4*>(p.res + at + j * 256) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      v[j] = add8(v[j], u[j]);
+      if (live && in[j]) *reinterpret_cast<uint4*>(p.h + at + j * 256) = v[j];
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 a0 = unpack_bf16x2(v[i].x), a1 = unpack_bf16x2(v[i].y), a2 = unpack_bf16x2(v[i].z), a3 = unpack_bf16x2(v[i].w);
-    ss += a0.x * a0.x + a0.y * a0.y + a1.x * a1.x + a1.y * a1.y + a2.x * a2.x + a2.y * a2.y + a3.x * a3.x + a3.y * a3.y;
-  }
-  ss = warp_sum(ss);
+  const float2 s2 = sumsq8(v[1], sumsq8(v[0], make_float2(0.f, 0.f)));
+  float ss = warp_sum(s2.x + s2.y);
   if constexpr (NT > 32) {
-    if ((threadIdx.x & 31) == 0) red[warp] = ss;
+    if (lane == 0) red[threadIdx.x >> 5] = ss;
     __syncthreads();
     ss = 0.f;
 #pragma unroll
     for (int i = 0; i < NT / 32; ++i) ss += red[team * (NT / 32) + i];
   }
-  const float rstd = rsqrtf(ss / p.D + p.eps);
+  const float rstd = __frsqrt_rn(ss / p.D + p.eps);
   if (t == 0 && live) p.rstd[row] = rstd;
   if (p.q_row == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int vi = t + i * NT, c = vi * 8;
-    const uint4 u = c < p.D ? *reinterpret_cast<const uint4*>(p.w + c) : make_uint4(0u, 0u, 0u, 0u);
-    const float2 a0 = unpack_bf16x2(v[i].x), a1 = unpack_bf16x2(v[i].y), a2 = unpack_bf16x2(v[i].z), a3 = unpack_bf16x2(v[i].w);
-    const float2 b0 = unpack_bf16x2(u.x), b1 = unpack_bf16x2(u.y), b2 = unpack_bf16x2(u.z), b3 = unpack_bf16x2(u.w);
-    float n[8] = {a0.x * rstd * b0.x, a0.y * rstd * b0.y, a1.x * rstd * b1.x, a1.y * rstd * b1.y,
-                  a2.x * rstd * b2.x, a2.y * rstd * b2.y, a3.x * rstd * b3.x, a3.y * rstd * b3.y};
-    if (c >= p.D) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) n[j] = 0.f;        // (an infinite rstd does not reach the padding)
-    }
+  for (int j = 0; j < 2; ++j) {
+    const int c = c0 + j * 256;
+    float2 z[4];
+    mul8(v[j], in[j] ? *reinterpret_cast<const uint4*>(p.w + c) : make_uint4(0u, 0u, 0u, 0u), z);
     uint2 q;
-    uint32_t e = mxq::quant_row8<mxq::E4M3>(n, nullptr, q);
-    if (live && c < p.D) *reinterpret_cast<uint2*>(p.q_row + row * p.D + c) = q;
+    uint32_t e = mxq::quant_row8_e4m3(z, rstd, q);
+    if (!in[j]) e = 0u;                              // (an infinite rstd does not reach the padding)
+    if (live && in[j]) *reinterpret_cast<uint2*>(p.q_row + at + j * 256) = q;
     // the four scale bytes of a 128-column group, from lanes 0, 4, 8, 12 of its sixteen
-    const int base = threadIdx.x & 16;
     uint32_t word = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) word |= __shfl_sync(0xffffffffu, e, base + 4 * j) << (8 * j);
-    if (live && (vi & 15) == 0 && c < p.D) {
-      const long long o = mxq::sf_offset(row, vi >> 2, p.row_tile, (p.row_tile + 127) >> 7, (p.D + 127) >> 7);
+    for (int k = 0; k < 4; ++k) word |= __shfl_sync(0xffffffffu, e, (lane & 16) + 4 * k) << (8 * k);
+    if (live && (lane & 15) == 0 && in[j]) {
+      const long long o = mxq::sf_offset(row, c >> 5, p.row_tile, (p.row_tile + 127) >> 7, (p.D + 127) >> 7);
       *reinterpret_cast<uint32_t*>(p.sf_row + o) = word;
     }
   }
+}
+
+// Both copies (or the column copy) in one pass over the input.  A cluster of CTAs owns 32 rows, each CTA COLS columns of them: 32 rows are one
+// block of the column copy's scales, and rows as wide as 8192 stay on chip as one piece.
+//   * a warp loads four rows x 512 columns, adds the residual, writes h, keeps the sums in registers (for the row copy) and puts them into
+//     shared memory (for the column copy);
+//   * the CTAs' partial sums of squares meet over distributed shared memory, in rank order: every CTA has the same rstd, and runs are
+//     bit-reproducible;
+//   * row copy from the registers, column copy from shared memory: two lanes walk two columns, 16 rows each, and write 16 codes of either.
+// 33 KB a CTA (512 columns), so that several CTAs of an SM cover one another's barrier.  With 128-row tiles the columns' codes would leave as
+// whole 128-byte lines, but a CTA would hold 130 KB and its load, barrier and compute phases would stand alone; the 32-byte pieces of four
+// neighbouring clusters meet in L2.
+struct NormMxCols {
+  uint8_t* q_col; uint8_t* sf_col; int col_tile;
+  int Tp;
+};
+
+template <int COLS>
+struct ClusterCfg {
+  static constexpr int PITCH_W = COLS / 2 + 4;                   // words; 16 more from row 16 on: the two lanes of a column lie 16 banks apart
+  static constexpr int SMEM = (32 * PITCH_W + 16) * 4;
+};
+B200_DEVICE float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int COLS>
+__global__ void __launch_bounds__(COLS / 2)
+norm_mx_cluster_kernel(const NormMxArgs p, const NormMxCols o) {
+  b200::begin_kernel();
+  using C = ClusterCfg<COLS>;
+  constexpr int HALVES = COLS / 512, MAX_CTAS = 8;
+  extern __shared__ __align__(16) uint32_t tile[];
+  __shared__ float part[HALVES][32];
+  __shared__ float rstd_s[32];
+  __shared__ __align__(4) uint8_t sfs[32][COLS / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = (int)cluster_ctarank(), ctas = gridDim.y;     // (the cluster spans the grid's y)
+  const long long r0 = (long long)blockIdx.x * 32;
+  const int c_cta = rank * COLS, rr0 = (warp & 7) * 4, cc = (warp >> 3) * 512 + lane * 8;
+  const int rows = (int)min(32ll, p.T - r0), live = rows - rr0;              // (a warp's rows past T: live <= 0)
+  const bool in0 = c_cta + cc < p.D, in1 = c_cta + cc + 256 < p.D;
+  const long long at = (r0 + rr0) * p.D + c_cta + cc;
+  uint4 v[4][2];
+  {
+    const __nv_bfloat16* src = p.x + at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i][0] = i < live && in0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+      v[i][1] = i < live && in1 ? *reinterpret_cast<const uint4*>(src + 256) : make_uint4(0u, 0u, 0u, 0u);
+      src += p.D;
+    }
+  }
+  if (p.res != nullptr) {
+    const __nv_bfloat16* src = p.res + at;
+    uint4 u[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i][0] = i < live && in0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+      u[i][1] = i < live && in1 ? *reinterpret_cast<const uint4*>(src + 256) : make_uint4(0u, 0u, 0u, 0u);
+      src += p.D;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i][0] = add8(v[i][0], u[i][0]); v[i][1] = add8(v[i][1], u[i][1]); }
+  }
+  {
+    uint32_t* dst = tile + rr0 * C::PITCH_W + (rr0 >> 4) * 16 + cc / 2;      // (a warp's four rows are on one side of row 16)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<uint4*>(dst + i * C::PITCH_W) = v[i][0];
+      *reinterpret_cast<uint4*>(dst + i * C::PITCH_W + 128) = v[i][1];
+      const float2 s2 = sumsq8(v[i][1], sumsq8(v[i][0], make_float2(0.f, 0.f)));
+      const float ss = warp_sum(s2.x + s2.y);
+      if (lane == 0) part[warp >> 3][rr0 + i] = ss;
+    }
+  }
+  cluster_sync_all();
+  if (tid < 32) {
+    float f[MAX_CTAS][HALVES];
+#pragma unroll
+    for (int q = 0; q < MAX_CTAS; ++q)
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) f[q][h] = q < ctas ? ld_cluster_f32(mapa_u32(smem_u32(&part[h][tid]), q)) : 0.f;
+    float ss = 0.f;
+#pragma unroll
+    for (int q = 0; q < MAX_CTAS; ++q)
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) ss += f[q][h];
+    const bool live = r0 + tid < p.T;
+    const float rstd = live ? __frsqrt_rn(ss / p.D + p.eps) : 0.f;
+    rstd_s[tid] = rstd;
+    if (live && rank == 0) p.rstd[r0 + tid] = rstd;
+  }
+  __syncthreads();
+  // (this CTA has read its peers' sums; they may leave once all have)
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // (h leaves only now: a release waits for the stores before it)
+  if (p.res != nullptr) {
+    __nv_bfloat16* dst = p.h + at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i < live && in0) *reinterpret_cast<uint4*>(dst) = v[i][0];
+      if (i < live && in1) *reinterpret_cast<uint4*>(dst + 256) = v[i][1];
+      dst += p.D;
+    }
+  }
+  if (p.q_row != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool in = j ? in1 : in0;
+      const uint4 w = in ? *reinterpret_cast<const uint4*>(p.w + c_cta + cc + j * 256) : make_uint4(0u, 0u, 0u, 0u);
+      uint8_t* dst = p.q_row + at + j * 256;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 z[4];
+        mul8(v[i][j], w, z);
+        uint2 q;
+        uint32_t e = mxq::quant_row8_e4m3(z, rstd_s[rr0 + i], q);
+        if (!in) e = 0u;                             // (an infinite rstd does not reach the padding)
+        if (i < live && in) *reinterpret_cast<uint2*>(dst) = q;
+        dst += p.D;
+        if ((lane & 3) == 0) sfs[rr0 + i][(cc + j * 256) >> 5] = (uint8_t)e;
+      }
+    }
+  }
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const int sub = lane & 1, cw = pass * (COLS / 4) + warp * 16 + (lane >> 1), c = c_cta + 2 * cw;
+    const bool in = c < p.D;
+    const uint32_t* t = tile + sub * (16 * C::PITCH_W + 16) + cw;
+    const float2 w = in ? unpack_bf16x2(*reinterpret_cast<const uint32_t*>(p.w + c)) : make_float2(0.f, 0.f);
+    float2 n[16];
+    float ma = 0.f, mb = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float s = rstd_s[sub * 16 + i];
+      n[i] = fmul2(unpack_bf16x2(t[i * C::PITCH_W]), make_float2(s, s));
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      ma = mxq::fmax3_nan(ma, n[i].x, n[i + 1].x);
+      mb = mxq::fmax3_nan(mb, n[i].y, n[i + 1].y);
+    }
+    uint4 qa, qb;
+    uint32_t ea, eb;
+    mxq::quant_col16<mxq::E4M3>(n, w, mxq::abs_bits(ma * w.x), mxq::abs_bits(mb * w.y), nullptr, nullptr, qa, qb, ea, eb);
+    if (in) {
+      uint8_t* dst = o.q_col + (long long)c * o.Tp + r0 + sub * 16;
+      *reinterpret_cast<uint4*>(dst) = qa;
+      *reinterpret_cast<uint4*>(dst + o.Tp) = qb;
+      o.sf_col[mxq::sf_offset(c + sub, (int)(r0 >> 5), o.col_tile, (o.col_tile + 127) >> 7, o.Tp >> 7)] = (uint8_t)(sub ? eb : ea);
+    }
+  }
+  if (p.q_row != nullptr) {
+    __syncthreads();
+    for (int i = tid; i < 32 * (COLS / 128); i += COLS / 2) {
+      const int r = i / (COLS / 128), g = i - r * (COLS / 128);
+      if (r < rows && c_cta + g * 128 < p.D) {
+        const long long to = mxq::sf_offset(r0 + r, (c_cta >> 5) + g * 4, p.row_tile, (p.row_tile + 127) >> 7, (p.D + 127) >> 7);
+        *reinterpret_cast<uint32_t*>(p.sf_row + to) = *reinterpret_cast<const uint32_t*>(&sfs[r][g * 4]);
+      }
+    }
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int COLS>
+int launch_cluster(const NormMxArgs& p, const NormMxCols& o, cudaStream_t stream) {
+  using C = ClusterCfg<COLS>;
+  const auto kern = norm_mx_cluster_kernel<COLS>;
+  if (C::SMEM > 40 * 1024) {
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return b200::fail(735, "norm_mx: cannot set %d bytes of shared memory: %s", C::SMEM, cudaGetErrorString(e));
+      }
+      configured[dev & 63] = true;
+    }
+  }
+  const int ctas = (p.D + COLS - 1) / COLS;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(o.Tp / 32, ctas, 1);
+  cfg.blockDim = dim3(COLS / 2, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1; attr[0].val.clusterDim.y = ctas; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, kern, p, o);
+  b200::count_launch();
+  return b200::check_launch("norm_mx(cluster)");
 }
 
 }  // namespace
@@ -111,24 +316,20 @@ B200_API int b200_norm_mx(const void* x, const void* residual, const void* w, vo
   if ((q_row && (row_tile <= 0 || row_tile % 16 != 0)) || (q_col && (col_tile <= 0 || col_tile % 16 != 0)))
     return b200::fail(732, "norm_mx: tile rows must be positive multiples of 16");
   if (residual != nullptr && h == nullptr) return b200::fail(733, "norm_mx: a residual needs a place for the sum");
-  if (T > 65535 * mxq::TILE) return b200::fail(734, "norm_mx: T=%d rows are more than a launch covers", T);
+  if (T > 0x7fffff00) return b200::fail(734, "norm_mx: T=%d rows cannot be filled up to a multiple of 128", T);
   NormMxArgs p = {(const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)w, (__nv_bfloat16*)h, (float*)rstd, T, D, eps,
                   (uint8_t*)q_row, (uint8_t*)sf_row, row_tile};
   cudaStream_t st = (cudaStream_t)stream;
-  if (D <= 1024) b200::launch(norm_mx_rows_kernel<32>, dim3((T + 7) / 8), 256, 0, st, p);
-  else if (D <= 2048) b200::launch(norm_mx_rows_kernel<64>, dim3((T + 3) / 4), 256, 0, st, p);
-  else if (D <= 4096) b200::launch(norm_mx_rows_kernel<128>, dim3((T + 1) / 2), 256, 0, st, p);
-  else b200::launch(norm_mx_rows_kernel<256>, dim3(T), 256, 0, st, p);
+  if (q_col != nullptr) {
+    const NormMxCols o = {(uint8_t*)q_col, (uint8_t*)sf_col, col_tile, (T + 127) / 128 * 128};
+    // (clusters of more than eight CTAs are not portable: wider rows take CTAs of 1024 columns)
+    return D <= 4096 ? launch_cluster<512>(p, o, st) : launch_cluster<1024>(p, o, st);
+  }
+  if (D <= 512) b200::launch(norm_mx_rows_kernel<32>, dim3((T + 7) / 8), 256, 0, st, p);
+  else if (D <= 1024) b200::launch(norm_mx_rows_kernel<64>, dim3((T + 3) / 4), 256, 0, st, p);
+  else if (D <= 2048) b200::launch(norm_mx_rows_kernel<128>, dim3((T + 1) / 2), 256, 0, st, p);
+  else if (D <= 4096) b200::launch(norm_mx_rows_kernel<256>, dim3(T), 256, 0, st, p);
+  else b200::launch(norm_mx_rows_kernel<512>, dim3(T), 512, 0, st, p);
   b200::count_launch();
-  int r = b200::check_launch("norm_mx");
-  if (r || q_col == nullptr) return r;
-  mxq::TileArgs q = {};
-  q.x = residual != nullptr ? (const __nv_bfloat16*)h : (const __nv_bfloat16*)x;
-  q.ldx = D; q.R = T; q.C = D;
-  q.rstd = (const float*)rstd; q.w = (const __nv_bfloat16*)w;
-  q.q_col = (uint8_t*)q_col; q.sf_col = (uint8_t*)sf_col; q.col_tile = col_tile;
-  q.Rp = (T + 127) / 128 * 128;
-  b200::launch(mxq::mx_tile_kernel<mxq::E4M3, true, false, false>, dim3((D + 127) / 128, (T + 127) / 128), 256, 0, st, q);
-  b200::count_launch();
-  return b200::check_launch("norm_mx(columns)");
+  return b200::check_launch("norm_mx");
 }

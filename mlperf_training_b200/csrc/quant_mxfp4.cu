@@ -102,7 +102,7 @@ void launch_dequant(dim3 grid, cudaStream_t st, const void* q, const void* sf, v
 
 template <bool NOISE, bool HAD>
 int launch_tile(dim3 grid, cudaStream_t st, const mxq::TileArgs& p) {
-  const auto kern = mxq::mx_tile_kernel<mxq::E2M1, false, NOISE, HAD>;
+  const auto kern = mxq::mx_tile_kernel<NOISE, HAD>;
   const int dyn = NOISE ? mxq::NOISE_WORDS * 4 : 0;
   if (NOISE) {
     // (the tile of bytes comes on top of 36 KB of static shared memory: more than a launch gets unasked)
