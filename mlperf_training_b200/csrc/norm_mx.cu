@@ -103,11 +103,11 @@ norm_mx_rows_kernel(const NormMxArgs p) {
 
 // Both copies (or the column copy) in one pass over the input.  A cluster of CTAs owns 32 rows, each CTA COLS columns of them: 32 rows are one
 // block of the column copy's scales, and rows as wide as 8192 stay on chip as one piece.
-//   * a warp loads four rows x 512 columns, adds the residual, writes h, keeps the sums in registers (for the row copy) and puts them into
-//     shared memory (for the column copy);
+//   * a warp loads four rows x 512 columns, two at a time, adds the residual and puts the sums into shared memory;
 //   * the CTAs' partial sums of squares meet over distributed shared memory, in rank order: every CTA has the same rstd, and runs are
 //     bit-reproducible;
-//   * row copy from the registers, column copy from shared memory: two lanes walk two columns, 16 rows each, and write 16 codes of either.
+//   * h and the row copy leave as the rows were loaded; for the column copy two lanes walk two columns, 16 rows each, and write 16 codes of
+//     either.
 // 33 KB a CTA (512 columns), so that several CTAs of an SM cover one another's barrier.  With 128-row tiles the columns' codes would leave as
 // whole 128-byte lines, but a CTA would hold 130 KB and its load, barrier and compute phases would stand alone; the 32-byte pieces of four
 // neighbouring clusters meet in L2.
@@ -128,7 +128,7 @@ B200_DEVICE float ld_cluster_f32(uint32_t addr) {
 }
 
 template <int COLS>
-__global__ void __launch_bounds__(COLS / 2)
+__global__ void __launch_bounds__(COLS / 2, 2048 / COLS)
 norm_mx_cluster_kernel(const NormMxArgs p, const NormMxCols o) {
   b200::begin_kernel();
   using C = ClusterCfg<COLS>;
@@ -144,37 +144,34 @@ norm_mx_cluster_kernel(const NormMxArgs p, const NormMxCols o) {
   const int rows = (int)min(32ll, p.T - r0), live = rows - rr0;              // (a warp's rows past T: live <= 0)
   const bool in0 = c_cta + cc < p.D, in1 = c_cta + cc + 256 < p.D;
   const long long at = (r0 + rr0) * p.D + c_cta + cc;
-  uint4 v[4][2];
-  {
-    const __nv_bfloat16* src = p.x + at;
+  uint32_t* const tw = tile + rr0 * C::PITCH_W + (rr0 >> 4) * 16 + cc / 2;      // (a warp's four rows are on one side of row 16)
+#pragma unroll 1
+  for (int i = 0; i < 4; i += 2) {
+    uint4 v[2][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i][0] = i < live && in0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-      v[i][1] = i < live && in1 ? *reinterpret_cast<const uint4*>(src + 256) : make_uint4(0u, 0u, 0u, 0u);
-      src += p.D;
+    for (int k = 0; k < 2; ++k) {
+      const __nv_bfloat16* src = p.x + at + (i + k) * (long long)p.D;
+      v[k][0] = i + k < live && in0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+      v[k][1] = i + k < live && in1 ? *reinterpret_cast<const uint4*>(src + 256) : make_uint4(0u, 0u, 0u, 0u);
     }
-  }
-  if (p.res != nullptr) {
-    const __nv_bfloat16* src = p.res + at;
-    uint4 u[4][2];
+    if (p.res != nullptr) {
+      uint4 u[2][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      u[i][0] = i < live && in0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-      u[i][1] = i < live && in1 ? *reinterpret_cast<const uint4*>(src + 256) : make_uint4(0u, 0u, 0u, 0u);
-      src += p.D;
+      for (int k = 0; k < 2; ++k) {
+        const __nv_bfloat16* src = p.res + at + (i + k) * (long long)p.D;
+        u[k][0] = i + k < live && in0 ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+        u[k][1] = i + k < live && in1 ? *reinterpret_cast<const uint4*>(src + 256) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) { v[k][0] = add8(v[k][0], u[k][0]); v[k][1] = add8(v[k][1], u[k][1]); }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i][0] = add8(v[i][0], u[i][0]); v[i][1] = add8(v[i][1], u[i][1]); }
-  }
-  {
-    uint32_t* dst = tile + rr0 * C::PITCH_W + (rr0 >> 4) * 16 + cc / 2;      // (a warp's four rows are on one side of row 16)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<uint4*>(dst + i * C::PITCH_W) = v[i][0];
-      *reinterpret_cast<uint4*>(dst + i * C::PITCH_W + 128) = v[i][1];
-      const float2 s2 = sumsq8(v[i][1], sumsq8(v[i][0], make_float2(0.f, 0.f)));
+    for (int k = 0; k < 2; ++k) {
+      *reinterpret_cast<uint4*>(tw + (i + k) * C::PITCH_W) = v[k][0];
+      *reinterpret_cast<uint4*>(tw + (i + k) * C::PITCH_W + 128) = v[k][1];
+      const float2 s2 = sumsq8(v[k][1], sumsq8(v[k][0], make_float2(0.f, 0.f)));
       const float ss = warp_sum(s2.x + s2.y);
-      if (lane == 0) part[warp >> 3][rr0 + i] = ss;
+      if (lane == 0) part[warp >> 3][rr0 + i + k] = ss;
     }
   }
   cluster_sync_all();
@@ -197,33 +194,24 @@ norm_mx_cluster_kernel(const NormMxArgs p, const NormMxCols o) {
   __syncthreads();
   // (this CTA has read its peers' sums; they may leave once all have)
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  // (h leaves only now: a release waits for the stores before it)
-  if (p.res != nullptr) {
-    __nv_bfloat16* dst = p.h + at;
+  // h and the row copy, from the warp's own part of the tile (h leaves only now: a release waits for the stores before it)
 #pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const bool in = j ? in1 : in0;
+    const uint4 w = in ? *reinterpret_cast<const uint4*>(p.w + c_cta + cc + j * 256) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 2
     for (int i = 0; i < 4; ++i) {
-      if (i < live && in0) *reinterpret_cast<uint4*>(dst) = v[i][0];
-      if (i < live && in1) *reinterpret_cast<uint4*>(dst + 256) = v[i][1];
-      dst += p.D;
-    }
-  }
-  if (p.q_row != nullptr) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const bool in = j ? in1 : in0;
-      const uint4 w = in ? *reinterpret_cast<const uint4*>(p.w + c_cta + cc + j * 256) : make_uint4(0u, 0u, 0u, 0u);
-      uint8_t* dst = p.q_row + at + j * 256;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float2 z[4];
-        mul8(v[i][j], w, z);
-        uint2 q;
-        uint32_t e = mxq::quant_row8_e4m3(z, rstd_s[rr0 + i], q);
-        if (!in) e = 0u;                             // (an infinite rstd does not reach the padding)
-        if (i < live && in) *reinterpret_cast<uint2*>(dst) = q;
-        dst += p.D;
-        if ((lane & 3) == 0) sfs[rr0 + i][(cc + j * 256) >> 5] = (uint8_t)e;
-      }
+      const uint4 v = *reinterpret_cast<const uint4*>(tw + i * C::PITCH_W + j * 128);
+      const long long to = at + i * (long long)p.D + j * 256;
+      if (p.res != nullptr && i < live && in) *reinterpret_cast<uint4*>(p.h + to) = v;
+      if (p.q_row == nullptr) continue;
+      float2 z[4];
+      mul8(v, w, z);
+      uint2 q;
+      uint32_t e = mxq::quant_row8_e4m3(z, rstd_s[rr0 + i], q);
+      if (!in) e = 0u;                               // (an infinite rstd does not reach the padding)
+      if (i < live && in) *reinterpret_cast<uint2*>(p.q_row + to) = q;
+      if ((lane & 3) == 0) sfs[rr0 + i][(cc + j * 256) >> 5] = (uint8_t)e;
     }
   }
 #pragma unroll 1
