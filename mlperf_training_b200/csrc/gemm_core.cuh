@@ -16,7 +16,7 @@
 //                         the completion bytes of both CTAs' TMA loads
 //   empty[s]  (each CTA)  released by the leader's tcgen05.commit to both CTAs
 //   tfull[a]  (each CTA)  accumulator a complete: leader's tcgen05.commit to both CTAs
-//   tempty[a] (leader's)  2 x 4 arrivals: the epilogue warps of both CTAs have drained accumulator a
+//   tempty[a] (leader's)  2 x 4 (8) arrivals: the epilogue warps of both CTAs have drained accumulator a
 // MXFP8 only - the UE8M0 scales reach TMEM through four extra warps per CTA (one per TMEM lane
 // quarter) that read the staged scale atoms from shared memory and write them with tcgen05.st, so
 // that the tensor pipe carries nothing but MMAs (a tcgen05.cp per atom stalls the in-order pipe for
@@ -98,9 +98,12 @@ inline int raster_group_m() {
 // bf16 output (BN a multiple of 64) leaves 64 columns per store (box 64 x 32, 128-byte swizzle).
 // A BN of 32 k + 16 ends with one 16-column store through tmTail (fp32: box 16 x 32 with 64-byte
 // swizzle; bf16: box 16 x 32, dense 32-byte rows).
-template <int BN, bool WIDE>
+// c_begin, c_end: the chunks of 32 columns this warp drains (all, unless two warps share a lane quarter).  EARLY: the residual's loads are issued
+// before the accumulator is read, so that one wait covers both (16 registers more).
+// NBUF: staging buffers of the warp.
+template <int BN, bool WIDE, bool EARLY = false, int NBUF = 2>
 B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTail, const EpiArgs& e, uint32_t t_row,
-                                int row0, int n0, uint8_t* stg, int& buf, int lane, int row_off = 0) {
+                                int row0, int n0, uint8_t* stg, int& buf, int lane, int row_off = 0, int c_begin = 0, int c_end = BN / 32) {
   static_assert(BN % 16 == 0, "accumulator width must be a multiple of 16 columns");
   static_assert(!WIDE || BN % 64 == 0, "64-column stores need BN to be a multiple of 64");
   const int row = row0 + lane;
@@ -110,11 +113,19 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
   const bool vec_res = e.residual != nullptr && (e.ldr % 8 == 0) && (e.N % 8 == 0) &&
                        ((reinterpret_cast<uintptr_t>(e.residual) & 15) == 0);
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {   // whole 32-column chunks
+  for (int c = c_begin; c < c_end; ++c) {   // whole 32-column chunks
+    const int col0 = n0 + c * 32;
+    uint4 early[EARLY ? 4 : 1];
+    const bool use_early = EARLY && vec_res && row < e.M;
+    if (use_early) {
+      const __nv_bfloat16* rp = e.residual + (long long)row * e.ldr + col0;
+#pragma unroll
+      for (int j = 0; j < (EARLY ? 4 : 1); ++j)
+        early[j] = col0 + j * 8 < e.N ? *reinterpret_cast<const uint4*>(rp + j * 8) : make_uint4(0u, 0u, 0u, 0u);
+    }
     uint32_t r[32];
     tmem_ld_32x32b_x32(t_row + c * 32, r);
     tc_wait_ld();
-    const int col0 = n0 + c * 32;
     float v[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * alpha;
@@ -129,7 +140,7 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (col0 + j * 8 < e.N) {
-            const uint4 u = *reinterpret_cast<const uint4*>(rp + j * 8);
+            const uint4 u = EARLY ? early[EARLY ? j : 0] : *reinterpret_cast<const uint4*>(rp + j * 8);
             const float2 f0 = unpack_bf16x2(u.x), f1 = unpack_bf16x2(u.y), f2 = unpack_bf16x2(u.z), f3 = unpack_bf16x2(u.w);
             v[j * 8 + 0] += f0.x; v[j * 8 + 1] += f0.y; v[j * 8 + 2] += f1.x; v[j * 8 + 3] += f1.y;
             v[j * 8 + 4] += f2.x; v[j * 8 + 5] += f2.y; v[j * 8 + 6] += f3.x; v[j * 8 + 7] += f3.y;
@@ -143,7 +154,7 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
     }
     if (e.out_f32) {
       // 32 rows x 32 fp32 (128 bytes per row), 128-byte swizzle
-      if (lane == 0) tma_store_wait_read<1>();
+      if (lane == 0) tma_store_wait_read<NBUF - 1>();
       __syncwarp();
       uint8_t* sb = stg + buf * STG_BYTES + lane * 128;
 #pragma unroll
@@ -160,10 +171,10 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
         }
         tma_store_commit();
       }
-      buf ^= 1;
+      buf ^= NBUF - 1;
     } else if (!WIDE) {
       // 32 rows x 32 bf16 = dense 64-byte rows, 64-byte swizzle (chunk ^= (row / 2) % 4)
-      if (lane == 0) tma_store_wait_read<1>();
+      if (lane == 0) tma_store_wait_read<NBUF - 1>();
       __syncwarp();
       uint8_t* sb = stg + buf * STG_BYTES + lane * 64;
 #pragma unroll
@@ -180,12 +191,12 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
         }
         tma_store_commit();
       }
-      buf ^= 1;
+      buf ^= NBUF - 1;
     } else {
       // 32 rows x 64 bf16 (128 bytes per row): two 32-column chunks fill one staging buffer
       const int half = c & 1;
       if (half == 0) {
-        if (lane == 0) tma_store_wait_read<1>();
+        if (lane == 0) tma_store_wait_read<NBUF - 1>();
         __syncwarp();
       }
       uint8_t* sb = stg + buf * STG_BYTES + lane * 128;
@@ -207,7 +218,7 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
           }
           tma_store_commit();
         }
-        buf ^= 1;
+        buf ^= NBUF - 1;
       }
     }
   }
@@ -243,7 +254,7 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
           if (col0 + i < e.N) v[i] += __bfloat162float(rp[i]);
       }
     }
-    if (lane == 0) tma_store_wait_read<1>();
+    if (lane == 0) tma_store_wait_read<NBUF - 1>();
     __syncwarp();
     if (e.out_f32) {
       // 32 rows x 16 fp32 = 64-byte rows, 64-byte swizzle
@@ -271,7 +282,7 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
       }
       tma_store_commit();
     }
-    buf ^= 1;
+    buf ^= NBUF - 1;
   }
 }
 
@@ -324,7 +335,9 @@ struct PairCfg {
   static constexpr bool MX = (KIND == KIND_MXFP8) || F4;
   static constexpr int KG = F4 ? 2 : 1;           // 128-element scale groups per 128-byte sub-block
   static constexpr int OUT_N = GATE == 1 ? BN / 2 : BN;        // output columns of a tile
-  static constexpr int THREADS = MX ? NUM_THREADS + 128 : NUM_THREADS;   // + 4 scale-forwarding warps
+  // Two epilogue warps per lane quarter where a tile's mainloop is short beside its epilogue: the 4-bit kind and the gated epilogues.
+  static constexpr int EPI_W = (F4 || GATE != 0) ? 2 * EPI_WARPS : EPI_WARPS;
+  static constexpr int THREADS = 64 + 32 * EPI_W + (MX ? 128 : 0);              // + 4 scale-forwarding warps
   static constexpr int BNH = BN / 2;              // B rows staged by each CTA
   static constexpr int A_SUB = 128 * 128;         // 128 rows x 128 bytes of K
   static constexpr int B_SUB = BNH * 128;
@@ -334,9 +347,13 @@ struct PairCfg {
   static constexpr int AB_STAGE = KSUB * (A_SUB + B_SUB);      // operand bytes landed per CTA per stage
   static constexpr int SF_STAGE = KSUB * (SFA_SUB + SFB_SUB);  // scale bytes landed per CTA per stage
   static constexpr int STAGE = AB_STAGE + SF_STAGE;
-  static constexpr int STG_BUFS = GATE != 0 ? 3 : 2;           // staging buffers per epilogue warp
-  static constexpr int EPI_BYTES = EPI_WARPS * STG_BUFS * STG_BYTES;
-  static constexpr int SF_SET_COLS = F4 ? 24 : 16;             // per 128-element group: 4 columns of A scales, 4 per 128 rows of B; padding
+  static constexpr int STG_BUFS = F4 ? 1 : 2;
+  static constexpr int STG_WARP = GATE != 0 ? 6144 : STG_BUFS * STG_BYTES;      // staging bytes per epilogue warp
+  static constexpr int EPI_BYTES = EPI_W * STG_WARP;
+  // Scale columns of a staged sub-block.  MXFP8: 4 of A, 4 per 128 rows of B, padding.  MXFP4: 4 of A and one per 32 rows of B, for each of
+  // the two groups.
+  static constexpr int SFB_COLS = F4 ? BN / 32 : 4 * B_ATOMS;
+  static constexpr int SF_SET_COLS = F4 ? 2 * (4 + SFB_COLS) : 16;
   static constexpr int SMEM_BUDGET = 232448 - 1024 - 1024 - 512 - EPI_BYTES;
   // (MXFP4: the scale sets in tensor memory, one per stage, run out before shared memory does)
   static constexpr int STAGES = F4 && SMEM_BUDGET / STAGE > (512 - 2 * BN) / (KSUB * SF_SET_COLS) ? (512 - 2 * BN) / (KSUB * SF_SET_COLS)
@@ -347,7 +364,8 @@ struct PairCfg {
   static constexpr int USED_COLS = 2 * BN + (MX ? SF_SETS * SF_SET_COLS : 0);
   static constexpr int TMEM_COLS = USED_COLS <= 256 ? 256 : 512;
   static constexpr int NUM_BARS = 2 * STAGES + 4 + (MX ? 2 * STAGES : 0);
-  static_assert(!MX || KG * (4 + 4 * B_ATOMS) <= SF_SET_COLS, "scale set too narrow");
+  static_assert(!MX || KG * (4 + SFB_COLS) <= SF_SET_COLS, "scale set too narrow");
+  static_assert(!F4 || SF_SET_COLS == 16 || SF_SET_COLS == 20, "the forwarders write 16 or 20 columns");
   static_assert(GATE == 0 || KIND == KIND_BF16, "gated epilogues belong to the bf16 kind");
   static_assert(USED_COLS <= 512, "accumulators and scale sets exceed tensor memory");
   static_assert(B_SUB % 1024 == 0, "B half tile must be whole swizzle atoms");
@@ -563,17 +581,17 @@ B200_DEVICE void stage_32x32(uint8_t* buf, int lane, const uint32_t (&w)[16]) {
 //           through tmA, gate and up (bf16: what the backward keeps) through tmG and tmU
 //   GATE 2  da = the accumulator, not rounded; d gate and d up leave through tmG and tmU, the product a of the kept projections (which the
 //           gradient of the down projection needs) through tmA
-// The three maps have 32 x 32 boxes with the 64-byte swizzle; each clips at its own M x F.  Two sets of three 2 KB buffers per warp.
+// The three maps have 32 x 32 boxes with the 64-byte swizzle; each clips at its own M x F.  Three 2 KB buffers per warp; the two warps of a
+// lane quarter take the chunks by turns.
 template <int BN, int GATE>
 B200_DEVICE void gate_drain(const CUtensorMap* tmA, const CUtensorMap* tmG, const CUtensorMap* tmU, const PairParams& p, uint32_t t_row,
-                            int row0, int n0, uint8_t* stg, int lane) {
+                            int row0, int n0, uint8_t* buf, int lane, int half) {
   constexpr int OUT_N = GATE == 1 ? BN / 2 : BN;
   const bool w_gu = GATE == 2 || p.gate.want_gu, w_a = GATE == 1 || p.gate.want_a;
   const int act = p.gate.act, row = row0 + lane;
 #pragma unroll 1
-  for (int c = 0; c < OUT_N / 32; ++c) {
+  for (int c = half; c < OUT_N / 32; c += 2) {
     const int col0 = n0 + c * 32;
-    uint8_t* buf = stg + (c & 1) * 6144;
     uint32_t wa[16], wg[16], wu[16];
     if constexpr (GATE == 1) {
       uint32_t g[32], u[32];
@@ -614,7 +632,7 @@ B200_DEVICE void gate_drain(const CUtensorMap* tmA, const CUtensorMap* tmG, cons
         wa[i] = pack_bf16x2(v0 * uf.x, v1 * uf.y);
       }
     }
-    if (lane == 0) tma_store_wait_read<1>();        // the stores of the chunk before last have left this set
+    if (lane == 0) tma_store_wait_read<0>();        // the stores of the chunk before have left the buffers
     __syncwarp();
     if (w_a) stage_32x32(buf, lane, wa);
     if (w_gu) { stage_32x32(buf + 2048, lane, wg); stage_32x32(buf + 4096, lane, wu); }
@@ -682,7 +700,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   if (threadIdx.x == 0) {
     if (!is_aux) {                                // a copy CTA sets up its own barriers in the same words
       for (int i = 0; i < C::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-      for (int i = 0; i < 2; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 2 * EPI_WARPS); }
+      for (int i = 0; i < 2; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 2 * C::EPI_W); }
       if (MX) {
         for (int i = 0; i < C::STAGES; ++i) { mbar_init(&sffull[i], 1); mbar_init(&sfrdy[i], 8); }
       }
@@ -828,7 +846,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                   if (((ti.kb0 + kb) * KSUB + s) * KB_ELEMS + kk * 64 < p.K) {
                     const uint32_t id = (uint32_t)(kk & 1) * 2;
                     tc_mma_mxf4_ss_pair(d_tmem, ad + kk * a_kstep, bd + kk * b_kstep, idesc0 | (id << 29) | (id << 4), accum,
-                                        t_sfa + 4 * (kk >> 1), t_sfa + 8 + 8 * (kk >> 1));
+                                        t_sfa + 4 * (kk >> 1), t_sfa + 8 + C::SFB_COLS * (kk >> 1));
                   }
                 } else if (MX) {
                   // scale byte kk of every 32-bit scale column: a_sf_id bits [29,31), b_sf_id bits [4,6)
@@ -849,10 +867,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
     }
-  } else if (warp < 2 + EPI_WARPS) {
+  } else if (warp < 2 + C::EPI_W) {
     // ------------------------------ epilogue (both CTAs) ------------------------------
     const int q = warp & 3;                       // TMEM lane quarter owned by this warp
-    uint8_t* stg = sE + (warp - 2) * C::STG_BUFS * STG_BYTES;
+    const int half = (warp - 2) / EPI_WARPS;      // which of the warps of this quarter
+    uint8_t* stg = sE + (warp - 2) * C::STG_WARP;
     const uint32_t tempty_leader0 = mapa_u32(smem_u32(&tempty[0]), 0);
     const uint32_t tempty_leader1 = mapa_u32(smem_u32(&tempty[1]), 0);
     int buf = 0;
@@ -874,7 +893,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       tc_fence_after();
       const uint32_t t_row = tmem_base + (uint32_t(q * 32) << 16) + acc * BN;
       if constexpr (GATE != 0) {
-        gate_drain<BN, GATE>(&tmD, &tmSFA, &tmSFB, p, t_row, ti.mb * 256 + (int)rank * 128 + q * 32, ti.nb * C::OUT_N, stg, lane);
+        gate_drain<BN, GATE>(&tmD, &tmSFA, &tmSFB, p, t_row, ti.mb * 256 + (int)rank * 128 + q * 32, ti.nb * C::OUT_N, stg, lane, half);
       } else if (p.rs.on) {
         // the tile goes into the owner's staging slot of this rank, through the owner's tensor map; then the owner's
         // counter of these 128 rows learns that this warp's part has landed
@@ -896,9 +915,17 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           e = EpiArgs{};
           e.M = 0x7fffffff; e.N = BN; e.out_f32 = 1; e.alpha = 1.f;
         }
-        epilogue_drain<BN, (BN % 64 == 0)>(part ? &tmW : &tmD, part ? &tmWt : &tmDt, e, t_row,
+        // two warps of a quarter: an odd number of 64-column stores (BN = 192) is shared 1 : 2 and 2 : 1 by turns
+        constexpr int CH = BN / 32;
+        int c0 = 0, c1 = CH;
+        if constexpr (C::EPI_W > EPI_WARPS) {
+          const int mid = ((CH / 2 + (it & 1)) / 2) * 2;
+          c0 = half ? mid : 0;
+          c1 = half ? CH : mid;
+        }
+        epilogue_drain<BN, (BN % 64 == 0), C::F4, C::STG_BUFS>(part ? &tmW : &tmD, part ? &tmWt : &tmDt, e, t_row,
                                            (part ? ti.part : ti.mb) * 256 + (int)rank * 128 + q * 32, part ? 0 : ti.nb * BN, stg, buf,
-                                           lane, p.grp.mode == 2 ? ti.e * p.M : 0);
+                                           lane, p.grp.mode == 2 ? ti.e * p.M : 0, c0, c1);
       }
       // all TMEM reads of this accumulator are complete (tcgen05.wait::ld inside): hand it back to the leader
       tc_fence_before();
@@ -930,24 +957,26 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 #pragma unroll
         for (int s = 0; s < KSUB; ++s) {
           if constexpr (F4) {
-            // both 128-element groups of the sub-block: A's four columns each, then up to eight columns of B's each
-            uint32_t r[16], rb[8];
+            // both 128-element groups of the sub-block: A's four columns each, then B's (a column holds 32 rows' scales)
+            uint32_t r[24];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const uint4 a4 = *reinterpret_cast<const uint4*>(sSFA + (stage * KSUB + s) * C::SFA_SUB + g * 512 + lane * 16);
               r[4 * g] = a4.x; r[4 * g + 1] = a4.y; r[4 * g + 2] = a4.z; r[4 * g + 3] = a4.w;
 #pragma unroll
-              for (int a = 0; a < 2; ++a) {
-                uint4 b4 = make_uint4(0u, 0u, 0u, 0u);
-                if (a < C::B_ATOMS)
-                  b4 = *reinterpret_cast<const uint4*>(sSFB + (stage * KSUB + s) * C::SFB_SUB + (g * C::B_ATOMS + a) * 512 + lane * 16);
-                uint32_t* to = g == 0 ? r + 8 + 4 * a : rb + 4 * a;
-                to[0] = b4.x; to[1] = b4.y; to[2] = b4.z; to[3] = b4.w;
+              for (int a = 0; a < C::B_ATOMS; ++a) {
+                const uint4 b4 = *reinterpret_cast<const uint4*>(sSFB + (stage * KSUB + s) * C::SFB_SUB + (g * C::B_ATOMS + a) * 512 + lane * 16);
+                uint32_t* to = r + 8 + C::SFB_COLS * g + 4 * a;
+                to[0] = b4.x; to[1] = b4.y;
+                if (4 * a + 2 < C::SFB_COLS) { to[2] = b4.z; to[3] = b4.w; }
               }
             }
             const uint32_t set = lane_base + (uint32_t)(stage * KSUB + s) * C::SF_SET_COLS;
-            tmem_st_32x32b_x16(set, r);
-            tmem_st_32x32b_x8(set + 16, rb);
+            uint32_t lo[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lo[i] = r[i];
+            tmem_st_32x32b_x16(set, lo);
+            if constexpr (C::SF_SET_COLS > 16) tmem_st_32x32b_x4(set + 16, make_uint4(r[16], r[17], r[18], r[19]));
             continue;
           }
           uint32_t r[16];
