@@ -491,6 +491,11 @@ struct GateArgs {
   long long ldgu;
 };
 
+// Rows of A's box for a problem of M rows.  Rows past M are filled with zeros on their way into shared memory at the price of real ones, and a
+// CTA's fill rate, not HBM, bounds problems of a few rows (7 x 2 x 14336 x 4096: 64 -> 47 us).  The rows of the tile that no box reaches hold
+// whatever was there; they are rows of D that nobody stores.
+inline int a_box_rows(int M) { return M >= 128 ? 128 : (M + 7) / 8 * 8; }
+
 struct PairParams {
   GroupArgs grp;
   SplitArgs split;
@@ -503,6 +508,7 @@ struct PairParams {
   TpGather tp;
   TpReduce rs;
   GateArgs gate;
+  int a_rows;                     // MXFP4 and gated kinds: rows of A's box (a_box_rows)
 };
 
 // Tile t of the launch: its row / column tile, expert and range of k stages (kb_elems = contraction
@@ -761,7 +767,10 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         for (int kb = ti.kb0; kb < ti.kb0 + ti.nkb; ++kb) {
           if (!mbar_wait_spin(&empty[stage], phase ^ 1, abort_flag, p.status, 310)) { ok = false; break; }
           const uint32_t bar = mapa_u32(smem_u32(&full[stage]), 0);
-          if (rank == 0) mbar_expect_tx(&full[stage], 2 * C::AB_STAGE);
+          if (rank == 0) {
+            if constexpr (F4 || GATE != 0) mbar_expect_tx(&full[stage], 2 * KSUB * (p.a_rows * 128 + C::B_SUB));
+            else mbar_expect_tx(&full[stage], 2 * C::AB_STAGE);
+          }
           if (MX) {
             // scale atoms first (the forwarding warps turn them into TMEM contents while the operand tiles
             // are still in flight), as rows of 128 int32, the stage's KSUB k groups in one box each

@@ -28,7 +28,7 @@ B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, in
       (gu != nullptr && (r = check("gemm_gated", gu, ldgu))))
     return r;
   CUtensorMap tmX, tmW, tmA, tmG, tmU;
-  if ((r = b200::make_tmap_2d(&tmX, b200::DT_BF16, x, K, M, ldx * 2, 64, 128, b200::SWZ_128))) return r;
+  if ((r = b200::make_tmap_2d(&tmX, b200::DT_BF16, x, K, M, ldx * 2, 64, a_box_rows(M), b200::SWZ_128))) return r;
   if ((r = b200::make_tmap_2d(&tmW, b200::DT_BF16, w, K, 2LL * F, ldw * 2, 64, 128, b200::SWZ_128))) return r;
   if ((r = b200::make_tmap_2d(&tmA, b200::DT_BF16, a, F, M, lda * 2, 32, 32, b200::SWZ_64))) return r;
   tmG = tmU = tmA;
@@ -40,6 +40,7 @@ B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, in
   p.M = M; p.N = F; p.K = K;
   p.group_m = raster_group_m() > 1 ? raster_group_m() / 2 : 1;
   p.gate.act = act; p.gate.F = F; p.gate.want_gu = gu != nullptr;
+  p.a_rows = a_box_rows(M);
   p.status = b200::status_ptr();
   return launch_pair<KIND_BF16, 256, 1, 1, 1>(tmX, tmW, tmG, tmU, tmA, tmA, p, (cudaStream_t)stream, "gemm_gated");
 }
@@ -55,7 +56,7 @@ B200_API int b200_gemm_gated_grad(const void* dy, const void* wd, const void* gu
       (r = check("gemm_gated_grad", dgu, lddgu)) || (a != nullptr && (r = check("gemm_gated_grad", a, lda))))
     return r;
   CUtensorMap tmY, tmW, tmA, tmG, tmU;
-  if ((r = b200::make_tmap_2d(&tmY, b200::DT_BF16, dy, K, M, lddy * 2, 64, 128, b200::SWZ_128))) return r;
+  if ((r = b200::make_tmap_2d(&tmY, b200::DT_BF16, dy, K, M, lddy * 2, 64, a_box_rows(M), b200::SWZ_128))) return r;
   if ((r = b200::make_tmap_2d(&tmW, b200::DT_BF16, wd, F, K, ldwd * 2, 64, 64, b200::SWZ_128))) return r;
   if ((r = b200::make_tmap_2d(&tmG, b200::DT_BF16, dgu, F, M, lddgu * 2, 32, 32, b200::SWZ_64))) return r;
   if ((r = b200::make_tmap_2d(&tmU, b200::DT_BF16, (uint8_t*)dgu + 2LL * F, F, M, lddgu * 2, 32, 32, b200::SWZ_64))) return r;
@@ -67,6 +68,7 @@ B200_API int b200_gemm_gated_grad(const void* dy, const void* wd, const void* gu
   p.group_m = raster_group_m() > 1 ? raster_group_m() / 2 : 1;
   p.gate.act = act; p.gate.F = F; p.gate.want_a = a != nullptr;
   p.gate.gu = (const __nv_bfloat16*)gu; p.gate.ldgu = ldgu;
+  p.a_rows = a_box_rows(M);
   p.status = b200::status_ptr();
   return launch_pair<KIND_BF16, 256, 1, 1, 2>(tmY, tmW, tmG, tmU, tmA, tmA, p, (cudaStream_t)stream, "gemm_gated_grad");
 }

@@ -30,7 +30,7 @@ int run(const void* a_q, const void* sfa, const void* b_q, const void* sfb, void
   CUtensorMap tmA, tmB, tmSFA, tmSFB, tmD, tmDt;
   int r;
   // (operands as bytes; what a box reaches past K, M or N arrives as zeros)
-  if ((r = b200::make_tmap_2d(&tmA, b200::DT_U8, a_q, K / 2, M, lda, 128, 128, b200::SWZ_128))) return r;
+  if ((r = b200::make_tmap_2d(&tmA, b200::DT_U8, a_q, K / 2, M, lda, 128, a_box_rows(M), b200::SWZ_128))) return r;
   if ((r = b200::make_tmap_2d(&tmB, b200::DT_U8, b_q, K / 2, N, ldb, 128, BN / 2, b200::SWZ_128))) return r;
   const int kg = (K + 127) / 128, atoms = (BN + 127) / 128;
   const long long a_rows = (long long)((M + 127) / 128) * kg, b_rows = (long long)((N + BN - 1) / BN) * kg * atoms;
@@ -41,6 +41,7 @@ int run(const void* a_q, const void* sfa, const void* b_q, const void* sfb, void
   p.M = M; p.N = N; p.K = K;
   p.group_m = raster_group_m();    // (rows of half the bytes: groups twice as tall as the 8-bit kernels', 16384 x 28672 x 4096 829 -> 815 us)
   p.epi = epi;
+  p.a_rows = a_box_rows(M);
   p.status = b200::status_ptr();
   return launch_pair<KIND_MXFP4, BN, KSUB, 1>(tmA, tmB, tmSFA, tmSFB, tmD, tmDt, p, stream, "gemm_mxfp4", nullptr, (float*)ws, ws_bytes, d, ldd);
 }

@@ -4,6 +4,7 @@
 //   call(name, *args)                   converts the arguments by their codes, calls the launcher with the GIL released and raises
 //                                       RuntimeError on a code other than 0
 //   gemm(...)                           ops.kernels.gemm for CUDA operands that need no copy: checks, output, split workspace, launch
+//   quant_mxfp4, dequant_mx, norm_mx, gemm_mxfp4   the same for ops.mxfp4 and ops.norm_mx
 //
 // ctypes converts twenty arguments through as many Python objects and calls: 5 of the 20 us a launch of a small model took.  With
 // it, the native GEMM operator and no autograd nodes where no gradient is wanted: a step of a two-layer model of width 512 2020 ->
@@ -100,6 +101,17 @@ PyObject* py_call(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_RETURN_NONE;
 }
 
+// the launchers of the micro-scaled operators, found by name when the table is bound
+using Quant4Fn = int (*)(const void*, long long, int, int, const void*, int, void*, void*, int, void*, void*, int, void*);
+using DequantFn = int (*)(const void*, const void*, void*, int, int, int, int, int, void*);
+using NormMxFn = int (*)(const void*, const void*, const void*, void*, void*, int, int, float, void*, void*, int, void*, void*, int, void*);
+using Gemm4Fn = int (*)(const void*, const void*, const void*, const void*, void*, int, int, int, long long, long long, long long, int, int,
+                        const void*, const void*, long long, float, void*, long long, void*);
+Quant4Fn g_quant4 = nullptr;
+DequantFn g_dequant = nullptr;
+NormMxFn g_norm_mx = nullptr;
+Gemm4Fn g_gemm4 = nullptr;
+
 // bind({name: (address, codes)}, address of b200_last_error, fallback)
 PyObject* py_bind(PyObject*, PyObject* args) {
   PyObject *table, *fallback;
@@ -118,6 +130,10 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     Py_INCREF(key);
     PyUnicode_InternInPlace(&key);
     t[key] = Entry{reinterpret_cast<void*>(addr), codes};
+    if (PyUnicode_CompareWithASCIIString(key, "b200_quant_mxfp4") == 0) g_quant4 = reinterpret_cast<Quant4Fn>(addr);
+    if (PyUnicode_CompareWithASCIIString(key, "b200_dequant_mx") == 0) g_dequant = reinterpret_cast<DequantFn>(addr);
+    if (PyUnicode_CompareWithASCIIString(key, "b200_norm_mx") == 0) g_norm_mx = reinterpret_cast<NormMxFn>(addr);
+    if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_mxfp4") == 0) g_gemm4 = reinterpret_cast<Gemm4Fn>(addr);
   }
   g_table = std::move(t);
   g_last_error = reinterpret_cast<const char* (*)()>(last);
@@ -132,7 +148,20 @@ using GemmFn = int (*)(const void*, const void*, void*, int, int, int, long long
 using WorkFn = long long (*)(int, int, int);
 GemmFn g_gemm = nullptr;
 WorkFn g_gemm_ws = nullptr;
-thread_local std::unordered_map<unsigned long long, long long> t_ws;   // (device, M, N, K) -> bytes; bounded below
+WorkFn g_gemm4_ws = nullptr;
+thread_local std::unordered_map<unsigned long long, long long> t_ws, t_ws4;   // (device, M, N, K) -> bytes; bounded below
+
+// bytes of the split workspace of a problem (the answer depends on the shape and the device alone)
+long long workspace_bytes(std::unordered_map<unsigned long long, long long>& known, WorkFn ask, int dev, int64_t M, int64_t N, int64_t K) {
+  if (M >= (1 << 20) || N >= (1 << 20) || K >= (1 << 20) || dev >= 16) return ask((int)M, (int)N, (int)K);
+  const unsigned long long key = ((unsigned long long)dev << 60) | ((unsigned long long)M << 40) | ((unsigned long long)N << 20) | (unsigned long long)K;
+  auto it = known.find(key);
+  if (it == known.end()) {
+    if (known.size() > 4096) known.clear();
+    it = known.emplace(key, ask((int)M, (int)N, (int)K)).first;
+  }
+  return it->second;
+}
 
 // rows that the GEMM's tensor maps take as they are
 bool plain(const at::Tensor& t) {
@@ -189,19 +218,7 @@ PyObject* py_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   const double alpha = PyFloat_AsDouble(args[9]);
   if (alpha == -1.0 && PyErr_Occurred()) return nullptr;
-  long long ws_bytes;
-  if (M < (1 << 20) && N < (1 << 20) && K < (1 << 20) && dev < 16) {
-    // (the answer depends on the shape and the device alone)
-    const unsigned long long key = ((unsigned long long)dev << 60) | ((unsigned long long)M << 40) | ((unsigned long long)N << 20) | (unsigned long long)K;
-    auto it = t_ws.find(key);
-    if (it == t_ws.end()) {
-      if (t_ws.size() > 4096) t_ws.clear();
-      it = t_ws.emplace(key, g_gemm_ws((int)M, (int)N, (int)K)).first;
-    }
-    ws_bytes = it->second;
-  } else {
-    ws_bytes = g_gemm_ws((int)M, (int)N, (int)K);
-  }
+  const long long ws_bytes = workspace_bytes(t_ws, g_gemm_ws, dev, M, N, K);
   int rc;
   {
     pybind11::gil_scoped_release nogil;
@@ -218,6 +235,206 @@ PyObject* py_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- micro-scaled operators: None where the general path has to look at the operands ----
+const at::Tensor* tensor_of(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+bool int_of(PyObject* o, long long& v) {
+  if (!PyLong_Check(o)) return false;
+  v = PyLong_AsLongLong(o);
+  return !(v == -1 && PyErr_Occurred());
+}
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool tile_ok(long long t) { return t >= 0 && t % 16 == 0 && t < (1 << 20); }
+int64_t sf_bytes(int64_t rows, int64_t k, int64_t tile) { return (rows + tile - 1) / tile * ((k + 127) / 128) * ((tile + 127) / 128) * 512; }
+PyObject* wrap_or_none(at::Tensor& t) {
+  if (t.defined()) return THPVariable_Wrap(std::move(t));
+  Py_RETURN_NONE;
+}
+PyObject* wrap_all(at::Tensor* t, int n) {
+  PyObject* out = PyTuple_New(n);
+  if (out == nullptr) return nullptr;
+  for (int i = 0; i < n; ++i) {
+    PyObject* o = wrap_or_none(t[i]);
+    if (o == nullptr) { Py_DECREF(out); return nullptr; }
+    PyTuple_SET_ITEM(out, i, o);
+  }
+  return out;
+}
+
+// quant_mxfp4(x, row_tile or 0, col_tile or 0, noise, hadamard): (q_row, sf_row, q_col, sf_col)
+PyObject* py_quant_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* x;
+  long long rt, ct;
+  if (nargs != 5 || g_quant4 == nullptr || (x = tensor_of(args[0])) == nullptr || !int_of(args[1], rt) || !int_of(args[2], ct)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const int had = PyObject_IsTrue(args[4]);
+  if (had < 0) return nullptr;
+  if (!x->is_cuda() || x->scalar_type() != at::kBFloat16 || !plain(*x) || x->size(0) <= 0 || x->size(1) <= 0 || x->size(1) % 32 != 0 ||
+      x->size(0) > 0x7fffffe0 || x->size(1) > 0x7fffffff || !tile_ok(rt) || !tile_ok(ct) || (rt == 0 && ct == 0))
+    Py_RETURN_NONE;
+  const int64_t R = x->size(0), C = x->size(1), Rp = (R + 31) / 32 * 32;
+  const int dev = x->device().index();
+  if (c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  const void* noise = nullptr;
+  if (args[3] != Py_None) {
+    const at::Tensor* n = tensor_of(args[3]);
+    if (n == nullptr || n->device() != x->device() || n->scalar_type() != at::kByte || n->sizes() != x->sizes() || !n->is_contiguous() ||
+        (reinterpret_cast<uintptr_t>(n->data_ptr()) & 7) != 0)
+      Py_RETURN_NONE;
+    noise = n->data_ptr();
+  }
+  at::Tensor t[4];
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    const auto o = x->options().dtype(at::kByte).requires_grad(false);
+    if (rt) { t[0] = at::empty({R, C / 2}, o); t[1] = at::empty({sf_bytes(R, C, rt)}, o); }
+    if (ct) { t[2] = at::empty({C, Rp / 2}, o); t[3] = at::empty({sf_bytes(C, Rp, ct)}, o); }
+    rc = g_quant4(x->data_ptr(), x->stride(0), (int)R, (int)C, noise, had, rt ? t[0].data_ptr() : nullptr, rt ? t[1].data_ptr() : nullptr,
+                  (int)rt, ct ? t[2].data_ptr() : nullptr, ct ? t[3].data_ptr() : nullptr, (int)ct,
+                  c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  if (rc != 0) return raise_code("b200_quant_mxfp4", rc);
+  return wrap_all(t, 4);
+  END_HANDLE_TH_ERRORS
+}
+
+// dequant_mx(q, sf, rows, k, tile_rows, e2m1, fp32): [rows, k]
+PyObject* py_dequant_mx(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *sf;
+  long long rows, k, tile;
+  if (nargs != 7 || g_dequant == nullptr || (q = tensor_of(args[0])) == nullptr || (sf = tensor_of(args[1])) == nullptr ||
+      !int_of(args[2], rows) || !int_of(args[3], k) || !int_of(args[4], tile)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const int four = PyObject_IsTrue(args[5]), f32 = PyObject_IsTrue(args[6]);
+  if (four < 0 || f32 < 0) return nullptr;
+  const int dev = q->is_cuda() ? q->device().index() : -1;
+  if (dev < 0 || sf->device() != q->device() || c10::cuda::current_device() != dev || rows <= 0 || k <= 0 || k % 32 != 0 || rows > 0x7fffffff ||
+      k > 0x7fffffff || tile <= 0 || !tile_ok(tile) || q->scalar_type() != at::kByte || sf->scalar_type() != at::kByte || !q->is_contiguous() ||
+      !sf->is_contiguous() || q->numel() != (four ? rows * (k / 2) : rows * k) || sf->numel() < sf_bytes(rows, k, tile) || !aligned16(q->data_ptr()))
+    Py_RETURN_NONE;
+  at::Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    out = at::empty({rows, k}, q->options().dtype(f32 ? at::kFloat : at::kBFloat16).requires_grad(false));
+    rc = g_dequant(q->data_ptr(), sf->data_ptr(), out.data_ptr(), (int)rows, (int)k, (int)tile, four, f32,
+                   c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  if (rc != 0) return raise_code("b200_dequant_mx", rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// norm_mx(x, weight, eps, residual, row_tile or 0, col_tile or 0): (q_row, sf_row, q_col, sf_col, h, rstd); h None without a residual
+PyObject* py_norm_mx(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *w, *res = nullptr;
+  long long rt, ct;
+  if (nargs != 6 || g_norm_mx == nullptr || (x = tensor_of(args[0])) == nullptr || (w = tensor_of(args[1])) == nullptr || !int_of(args[4], rt) ||
+      !int_of(args[5], ct) || (args[3] != Py_None && (res = tensor_of(args[3])) == nullptr)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const double eps = PyFloat_AsDouble(args[2]);
+  if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+  if (!x->is_cuda() || x->scalar_type() != at::kBFloat16 || x->dim() != 2 || !x->is_contiguous() || x->size(0) <= 0 || x->size(1) <= 0 ||
+      x->size(1) % 32 != 0 || x->size(1) > 8192 || x->size(0) > 0x7fffff00 || !aligned16(x->data_ptr()) || !tile_ok(rt) || !tile_ok(ct))
+    Py_RETURN_NONE;
+  const int64_t T = x->size(0), D = x->size(1), Tp = (T + 127) / 128 * 128;
+  if (w->device() != x->device() || w->scalar_type() != at::kBFloat16 || w->dim() != 1 || w->size(0) != D || !w->is_contiguous() || !aligned16(w->data_ptr()))
+    Py_RETURN_NONE;
+  if (res != nullptr && (res->device() != x->device() || res->scalar_type() != at::kBFloat16 || res->sizes() != x->sizes() ||
+                         !res->is_contiguous() || !aligned16(res->data_ptr())))
+    Py_RETURN_NONE;
+  const int dev = x->device().index();
+  if (c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  at::Tensor t[6];
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    const auto o = x->options().requires_grad(false), b = o.dtype(at::kByte);
+    if (rt) { t[0] = at::empty({T, D}, b); t[1] = at::empty({sf_bytes(T, D, rt)}, b); }
+    if (ct) { t[2] = at::empty({D, Tp}, b); t[3] = at::empty({sf_bytes(D, Tp, ct)}, b); }
+    if (res != nullptr) t[4] = at::empty({T, D}, o);
+    t[5] = at::empty({T}, o.dtype(at::kFloat));
+    rc = g_norm_mx(x->data_ptr(), res != nullptr ? res->data_ptr() : nullptr, w->data_ptr(), res != nullptr ? t[4].data_ptr() : nullptr,
+                   t[5].data_ptr(), (int)T, (int)D, (float)eps, rt ? t[0].data_ptr() : nullptr, rt ? t[1].data_ptr() : nullptr, (int)rt,
+                   ct ? t[2].data_ptr() : nullptr, ct ? t[3].data_ptr() : nullptr, (int)ct, c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  if (rc != 0) return raise_code("b200_norm_mx", rc);
+  return wrap_all(t, 6);
+  END_HANDLE_TH_ERRORS
+}
+
+// gemm_mxfp4(a_q, a_sf, b_q, b_sf, M, N, K, fp32, bias, residual, alpha): [M, N], a new tensor; the scales' tiles have been checked
+PyObject* py_gemm_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11 || g_gemm4 == nullptr || g_gemm4_ws == nullptr) Py_RETURN_NONE;
+  const at::Tensor* t[4];
+  for (int i = 0; i < 4; ++i)
+    if ((t[i] = tensor_of(args[i])) == nullptr || !t[i]->is_cuda() || t[i]->scalar_type() != at::kByte || !t[i]->is_contiguous() ||
+        t[i]->device() != t[0]->device() || !aligned16(t[i]->data_ptr()))
+      Py_RETURN_NONE;
+  long long M, N, K;
+  if (!int_of(args[4], M) || !int_of(args[5], N) || !int_of(args[6], K)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const int f32 = PyObject_IsTrue(args[7]);
+  if (f32 < 0) return nullptr;
+  const double alpha = PyFloat_AsDouble(args[10]);
+  if (alpha == -1.0 && PyErr_Occurred()) return nullptr;
+  const int dev = t[0]->device().index();
+  if (c10::cuda::current_device() != dev || M <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || M > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff ||
+      N * (f32 ? 4 : 2) % 16 != 0 || t[0]->numel() != M * (K / 2) || t[2]->numel() != N * (K / 2))
+    Py_RETURN_NONE;
+  const void *bias = nullptr, *res = nullptr;
+  long long ldr = 0;
+  if (args[8] != Py_None) {
+    const at::Tensor* b = tensor_of(args[8]);
+    if (b == nullptr || b->device() != t[0]->device() || b->scalar_type() != at::kBFloat16 || b->dim() != 1 || b->size(0) != N || !b->is_contiguous())
+      Py_RETURN_NONE;
+    bias = b->data_ptr();
+  }
+  if (args[9] != Py_None) {
+    const at::Tensor* r = tensor_of(args[9]);
+    if (r == nullptr || r->device() != t[0]->device() || r->scalar_type() != at::kBFloat16 || r->dim() != 2 || r->size(0) != M || r->size(1) != N ||
+        r->stride(1) != 1)
+      Py_RETURN_NONE;
+    res = r->data_ptr();
+    ldr = r->stride(0);
+  }
+  const long long ws_bytes = workspace_bytes(t_ws4, g_gemm4_ws, dev, M, N, K);
+  at::Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    const auto o = t[0]->options().requires_grad(false);
+    out = at::empty({M, N}, o.dtype(f32 ? at::kFloat : at::kBFloat16));
+    at::Tensor ws;
+    if (ws_bytes > 0) ws = at::empty({ws_bytes}, o);
+    rc = g_gemm4(t[0]->data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), t[3]->data_ptr(), out.data_ptr(), (int)M, (int)N, (int)K, K / 2, K / 2, N, f32, 0,
+                 bias, res, ldr, (float)alpha, ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  if (rc != 0) return raise_code("b200_gemm_mxfp4", rc);
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_mx(address of b200_gemm_mxfp4_workspace)
+PyObject* py_bind_mx(PyObject*, PyObject* args) {
+  unsigned long long w;
+  if (!PyArg_ParseTuple(args, "K", &w)) return nullptr;
+  g_gemm4_ws = reinterpret_cast<WorkFn>(w);
+  Py_RETURN_NONE;
+}
+
 // bind_gemm(address of b200_gemm_bf16, address of b200_gemm_bf16_workspace)
 PyObject* py_bind_gemm(PyObject*, PyObject* args) {
   unsigned long long g, w;
@@ -231,6 +448,11 @@ PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, nullptr},
     {"bind_gemm", py_bind_gemm, METH_VARARGS, nullptr},
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call)), METH_FASTCALL, nullptr},
+    {"bind_mx", py_bind_mx, METH_VARARGS, nullptr},
+    {"quant_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_quant_mxfp4)), METH_FASTCALL, nullptr},
+    {"dequant_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_dequant_mx)), METH_FASTCALL, nullptr},
+    {"norm_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_mx)), METH_FASTCALL, nullptr},
+    {"gemm_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gemm_mxfp4)), METH_FASTCALL, nullptr},
     {"gemm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gemm)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -161,6 +161,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         host.bind(table, ctypes.cast(lib.b200_last_error, c_void_p).value, _call_ctypes)
         if hasattr(lib, "b200_gemm_bf16_workspace"):
             host.bind_gemm(table["b200_gemm_bf16"][0], ctypes.cast(lib.b200_gemm_bf16_workspace, c_void_p).value)
+        if hasattr(lib, "b200_gemm_mxfp4_workspace"):
+            host.bind_mx(ctypes.cast(lib.b200_gemm_mxfp4_workspace, c_void_p).value)
     lib.b200_norm_bwd_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.restype = c_ll

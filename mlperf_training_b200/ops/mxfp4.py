@@ -13,6 +13,7 @@ A block that holds an infinity or a NaN gets the scale 255 (NaN): the format has
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -25,6 +26,7 @@ A_TILE = 128     # M tile of the GEMM: scale-atom grouping of A operands
 SF_NAN = 255
 
 
+@functools.lru_cache(maxsize=1024)
 def b_tile(n_rows: int) -> int:
     """N tile the GEMM uses for a B operand with ``n_rows`` rows (its scale-atom grouping)."""
     if _lib.LIB_PATH.exists():
@@ -145,6 +147,13 @@ def quantize(x: torch.Tensor, *, row_tile: int | None = None, col_tile: int | No
     for an A operand, ``b_tile(rows)`` for a B operand.  ``noise [R, C]`` (uint8, uniform): stochastic rounding of both copies,
     element (r, c) with the byte at (r, c), 128 for the filled up rows; None: to nearest even.  ``hadamard``: the column-wise copy is that
     of the 16-row Hadamard transform of the filled up ``x``."""
+    if x.is_cuda and use_kernels(x) and _lib.host is not None and row_tile != 0 and col_tile != 0:
+        # (operands for an input that is as the kernel reads it; None leaves copies and errors to the lines below)
+        r = _lib.host.quant_mxfp4(x, row_tile or 0, col_tile or 0, noise, hadamard)
+        if r is not None:
+            (R, C), (q_row, sf_row, q_col, sf_col) = x.shape, r
+            return (MX4Operand(q_row, sf_row, R, C, row_tile) if row_tile is not None else None,
+                    MX4Operand(q_col, sf_col, C, (R + 31) // 32 * 32, col_tile) if col_tile is not None else None)
     _check_matrix("mxfp4.quantize", x)
     _check_tile("mxfp4.quantize", row_tile)
     _check_tile("mxfp4.quantize", col_tile)
@@ -196,6 +205,10 @@ def dequantize(op, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     if not use_kernels(op.q):
         v = _unpack(op.q) if four else op.q.view(torch.float8_e4m3fn).float()
         return (v.view(op.rows, op.k // 32, 32) * _scale_values(op.sf)[..., None]).view(op.rows, op.k).to(dtype)
+    if _lib.host is not None:
+        out = _lib.host.dequant_mx(op.q, op.sf, op.rows, op.k, op.tile_rows, four, dtype == torch.float32)
+        if out is not None:
+            return out
     out = torch.empty((op.rows, op.k), dtype=dtype, device=op.q.device)
     if out.numel():
         call("b200_dequant_mx", ptr(op.q.contiguous()), ptr(op.sf), ptr(out), op.rows, op.k, op.tile_rows, int(four), int(dtype == torch.float32),
@@ -237,6 +250,10 @@ def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_d
         raise TypeError("mxfp4.gemm: output must be bf16 or fp32")
     if a.tile_rows != A_TILE or b.tile_rows != b_tile(N):
         raise ValueError(f"mxfp4.gemm: operand scale tiling ({a.tile_rows}, {b.tile_rows}) does not match the kernel tiles ({A_TILE}, {b_tile(N)})")
+    if out is None and _lib.host is not None:
+        d = _lib.host.gemm_mxfp4(a.q, a.sf, b.q, b.sf, M, N, Kd, out_dtype == torch.float32, bias, residual, alpha)
+        if d is not None:
+            return d
     if out is not None and (out.stride(1) != 1 or (N * out.element_size()) % 16 or (out.stride(0) * out.element_size()) % 16 or out.data_ptr() % 16 or out.stride(0) < N):
         if M and N:
             d = gemm(a, b, out_dtype=torch.float32 if accumulate else out_dtype, bias=bias, residual=residual, alpha=alpha)

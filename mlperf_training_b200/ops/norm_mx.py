@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib
 from . import mxfp4 as M4
 from . import mxfp8 as MX
 from ._lib import call, ptr, stream_ptr, use_kernels
@@ -30,6 +31,14 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, 
     ``h = x + residual`` rounded to bf16 (``x`` itself without a residual) is what is normalised; ``rstd [T]`` fp32.  ``row_op`` (when
     ``row_tile`` is given): rows T, contraction D.  ``col_op`` (when ``col_tile`` is given): rows D, contraction T filled up with zeros to a
     multiple of 128.  D is a multiple of 32 up to 8192; any T.  A block with an infinity or a NaN has the scale 255 (NaN)."""
+    if x.is_cuda and use_kernels(x) and _lib.host is not None and row_tile != 0 and col_tile != 0:
+        # (operands for inputs that are as the kernel reads them; None leaves copies and errors to the lines below)
+        r = _lib.host.norm_mx(x, weight, eps, residual, row_tile or 0, col_tile or 0)
+        if r is not None:
+            (T, D), (q_row, sf_row, q_col, sf_col, h, rstd) = x.shape, r
+            return (MX.MXOperand(q_row, sf_row, T, D, row_tile) if row_tile is not None else None,
+                    MX.MXOperand(q_col, sf_col, D, (T + 127) // 128 * 128, col_tile) if col_tile is not None else None,
+                    x if h is None else h, rstd)
     M4._check_matrix("rms_norm_quantize", x)
     M4._check_tile("rms_norm_quantize", row_tile)
     M4._check_tile("rms_norm_quantize", col_tile)
