@@ -9,6 +9,7 @@
 // projections are not read again: 4 bytes of T F less each way, and forward without a backward writes 2 bytes instead of 6.
 #include "common.cuh"
 #include "gemm_core.cuh"
+#include "gated_fewrows.cuh"
 #include "runtime.h"
 
 namespace {
@@ -27,6 +28,11 @@ B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, in
   if ((r = check("gemm_gated", x, ldx)) || (r = check("gemm_gated", w, ldw)) || (r = check("gemm_gated", a, lda)) ||
       (gu != nullptr && (r = check("gemm_gated", gu, ldgu))))
     return r;
+  if (M <= fewrows::MAX_ROWS) {
+    const fewrows::GatedArgs p = {(const __nv_bfloat16*)x, (const __nv_bfloat16*)w, (__nv_bfloat16*)a, (__nv_bfloat16*)gu, M, F, K, ldx, ldw, lda, ldgu,
+                                  act};
+    return fewrows::run_gated(p, (cudaStream_t)stream);
+  }
   CUtensorMap tmX, tmW, tmA, tmG, tmU;
   if ((r = b200::make_tmap_2d(&tmX, b200::DT_BF16, x, K, M, ldx * 2, 64, a_box_rows(M), b200::SWZ_128))) return r;
   if ((r = b200::make_tmap_2d(&tmW, b200::DT_BF16, w, K, 2LL * F, ldw * 2, 64, 128, b200::SWZ_128))) return r;
