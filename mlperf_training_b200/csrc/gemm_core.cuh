@@ -112,6 +112,7 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
   if (e.alpha_b != nullptr) alpha *= *e.alpha_b;
   const bool vec_res = e.residual != nullptr && (e.ldr % 8 == 0) && (e.N % 8 == 0) &&
                        ((reinterpret_cast<uintptr_t>(e.residual) & 15) == 0);
+  const bool vec_bias = EARLY && e.bias != nullptr && (e.N % 8 == 0) && ((reinterpret_cast<uintptr_t>(e.bias) & 15) == 0);
 #pragma unroll 1
   for (int c = c_begin; c < c_end; ++c) {   // whole 32-column chunks
     const int col0 = n0 + c * 32;
@@ -129,7 +130,18 @@ B200_DEVICE void epilogue_drain(const CUtensorMap* tmD, const CUtensorMap* tmTai
     float v[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * alpha;
-    if (e.bias != nullptr) {
+    if (EARLY && vec_bias) {
+      // (a load a column, as below, took longer than a 4-bit tile's mainloop has for a chunk)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (col0 + j * 8 < e.N) {
+          const uint4 u = *reinterpret_cast<const uint4*>(e.bias + col0 + j * 8);
+          const float2 f0 = unpack_bf16x2(u.x), f1 = unpack_bf16x2(u.y), f2 = unpack_bf16x2(u.z), f3 = unpack_bf16x2(u.w);
+          v[j * 8 + 0] += f0.x; v[j * 8 + 1] += f0.y; v[j * 8 + 2] += f1.x; v[j * 8 + 3] += f1.y;
+          v[j * 8 + 4] += f2.x; v[j * 8 + 5] += f2.y; v[j * 8 + 6] += f3.x; v[j * 8 + 7] += f3.y;
+        }
+      }
+    } else if (e.bias != nullptr) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (col0 + i < e.N) v[i] += __bfloat162float(e.bias[col0 + i]);
