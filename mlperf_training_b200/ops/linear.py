@@ -31,6 +31,7 @@ from . import fp8 as F8
 from . import kernels as K
 from . import mxfp4 as M4
 from . import mxfp8 as MX
+from ._lib import stream_ptr
 
 # bumped by the optimizer engine after every parameter update: invalidates cached weight copies
 _WEIGHT_EPOCH = 0
@@ -58,6 +59,11 @@ MX_RECIPES = {
     # the phase a FLUX run switches to: forward at 8 bits, backward still at 4
     "mxfp8_fwd_mxfp4_bwd": ("e4m3", "e4m3", "e2m1", "e2m1", "e2m1", True, 16),
 }
+
+
+def weight_format(precision: str) -> str:
+    """Element format of the forward weights of a micro-scaled recipe (e4m3 for every other precision); "fp4": of those it multiplies in 4 bits."""
+    return "e2m1" if precision == "fp4" else MX_RECIPES.get(precision, ("", "e4m3"))[1]
 
 
 def is_mx(precision: str) -> bool:
@@ -146,12 +152,14 @@ def fp4_eligible(rows: int, n_out: int, n_in: int) -> bool:
 
 def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
     """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, cached on the tensor until it changes: through torch (its
-    version counter) or through an optimizer step."""
+    version counter) or through an optimizer step.  A call on another stream than the one that made them waits for them there."""
     cacheable = not weight.is_inference()
     key = (_WEIGHT_EPOCH if weight.requires_grad else -1, weight._version if cacheable else -1)
     cache = getattr(weight, "_mx4_cache", None)
     row = None
     if cacheable and cache is not None and cache[0] == key:
+        if cache[3] is not None and cache[3] != stream_ptr():
+            _use_here(cache)
         if cache[2] is not None or not need_col:
             return cache[1], cache[2]
         row = cache[1]
@@ -162,8 +170,25 @@ def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
     new_row, col = M4.quantize(w, row_tile=M4.b_tile(N) if row is None else None, col_tile=M4.b_tile(Kd) if need_col else None)
     row = new_row if row is None else row
     if cacheable:
-        weight._mx4_cache = (key, row, col)
+        event = None
+        if w.is_cuda and not torch.cuda.is_current_stream_capturing():
+            event = torch.cuda.Event()
+            event.record()
+        weight._mx4_cache = (key, row, col, stream_ptr() if w.is_cuda else None, event)
     return row, col
+
+
+def _use_here(cache) -> None:
+    """Order the current stream behind the making of cached copies, and keep their memory until it is done with them.  (While a graph
+    is captured the caller has synchronised with what was made before, as for every tensor that a capture reads.)"""
+    if torch.cuda.is_current_stream_capturing() or cache[4] is None:
+        return
+    here = torch.cuda.current_stream()
+    here.wait_event(cache[4])
+    for op in cache[1:3]:
+        if op is not None:
+            op.q.record_stream(here)
+            op.sf.record_stream(here)
 
 
 def fp4_forward(x: torch.Tensor, weight: torch.Tensor, *, bias=None, residual=None, need_wgrad: bool = True, need_dgrad: bool = False):

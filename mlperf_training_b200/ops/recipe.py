@@ -74,8 +74,8 @@ class DeoscConfig:
     def status(self, precision: str) -> str:
         if not self.enabled:
             return "deosc: off"
-        from .linear import MX_RECIPES
-        fmt = MX_RECIPES.get(precision, ("", "e4m3"))[1]
+        from .linear import weight_format
+        fmt = weight_format(precision)
         if fmt != "e2m1":
             return (f"deosc: requested (start {self.start_step}, period {self.period}, ratio {self.ratio}) - idle: "
                     f"weights are {precision} ({fmt} elements), the oscillation it damps is a 4-bit-weight effect")
@@ -94,7 +94,7 @@ class Deoscillator:
         self.history: list = []              # (step, snapped at that period end)
         self._grid = None
 
-    def _keys(self, b):
+    def _keys(self, b, precision: str = "mxfp4"):
         """Per element of this rank's shard of bucket ``b``: (tracked?, scale-and-code key, code, grid value)."""
         from . import mxfp8 as MX
         dev = b.param_buf.device
@@ -109,7 +109,8 @@ class Deoscillator:
         v_max = MX.ELEMENT_FORMATS[self.fmt][2]
         for (name, p), o in zip(b.params, b.offsets):
             # only matrices that a micro-scaled linear, or stacks of them that the grouped expert MLP, has quantised
-            seen = getattr(p, "_mx_cache", None) is not None if p.dim() == 2 else getattr(p, "_mx_stack", None) is not None
+            # (in the fp4 recipe, those that it multiplies in 4 bits)
+            seen = getattr(p, "_mx4_cache" if precision == "fp4" else "_mx_cache", None) is not None if p.dim() == 2 else getattr(p, "_mx_stack", None) is not None
             if p.dim() not in (2, 3) or p.shape[-1] % 32 or not seen:
                 continue
             lo, hi = max(o, b.lo), min(o + p.numel(), b.hi)
@@ -145,15 +146,15 @@ class Deoscillator:
 
     def after_step(self, step: int, precision: str) -> int:
         """Returns the number of weights snapped at this step (non-zero only at a period end)."""
-        from .linear import MX_RECIPES
+        from .linear import weight_format
         cfg = self.cfg
-        if not cfg.enabled or step < cfg.start_step or MX_RECIPES.get(precision, ("", ""))[1] != self.fmt:
+        if not cfg.enabled or step < cfg.start_step or weight_format(precision) != self.fmt:
             return 0
         period_end = (step - cfg.start_step + 1) % max(cfg.period, 1) == 0
         n_snapped = 0
         with torch.no_grad():
             for b in self.engine.buckets:
-                tracked, key, code, value = self._keys(b)
+                tracked, key, code, value = self._keys(b, precision)
                 if not bool(tracked.any()):
                     continue
                 st = self.state.get(id(b))

@@ -174,6 +174,39 @@ def test_linear_on_another_stream_and_after_updates():
         assert torch.equal(F.mxfp4_linear(x, wi), -y0)
 
 
+def test_weight_copies_made_on_one_stream_and_used_on_others():
+    """The copies that a first call leaves on the weight are complete before another stream's call reads them."""
+    torch.manual_seed(0)
+    x, w = torch.randn(8, 4096, device="cuda").bfloat16(), torch.randn(16384, 4096, device="cuda").bfloat16()
+    want = F.mxfp4_linear(x, w.clone())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(5):
+        w = w.clone()
+        torch.cuda.synchronize()
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(F.mxfp4_linear(x, w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got)
+
+
+def test_linear_in_a_graph():
+    """Capture and replay of the layer: the copies of a frozen weight that a call made before are read, new inputs give new outputs."""
+    torch.manual_seed(0)
+    x, w = torch.randn(33, 256, device="cuda").bfloat16(), torch.randn(512, 256, device="cuda").bfloat16()
+    F.mxfp4_linear(x, w)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = F.mxfp4_linear(x, w)
+    for _ in range(2):
+        x.copy_(torch.randn_like(x))
+        g.replay()
+        assert torch.equal(y, F.mxfp4_linear(x, w))
+
+
 def test_drawn_noise_is_fresh_and_unbiased():
     """The backward draws its bytes itself when none are given: two backward passes differ, and their mean approaches the product with the
     unrounded gradient (256 draws: 1/16 of one draw's error)."""

@@ -152,6 +152,29 @@ def test_weight_copies_follow_the_optimizer_epoch():
     assert torch.equal(F.mxfp4_linear(x, w), -y0)
 
 
+def test_deoscillation_tracks_the_4_bit_weights():
+    """In the fp4 recipe the weights with 4-bit copies are tracked, and nothing else; one that flips between two codes is put on the grid."""
+    from mlperf_training_b200.ops.recipe import DeoscConfig, Deoscillator
+    from mlperf_training_b200.parallel.engine import OptimConfig, ZeroEngine
+    torch.manual_seed(0)
+    w4, w8 = torch.nn.Parameter(torch.randn(32, 64)), torch.nn.Parameter(torch.randn(32, 64))
+    engine = ZeroEngine(torch.nn.ParameterList([w4, w8]), OptimConfig())
+    d = Deoscillator(engine, DeoscConfig(enabled=True, start_step=0, period=8, ratio=2.0))
+    assert "on" in d.cfg.status("fp4") and "idle" in d.cfg.status("mxfp8")
+    with torch.no_grad():
+        w4[0, :32], w8[0, :32] = 6.0, 6.0
+        F.mxfp4_linear(torch.randn(1, 64), w4)
+        for step in range(8):
+            for b in engine.buckets:
+                for (name, p), o in zip(b.params, b.offsets):
+                    at = 1 if p is w4 or p is w8 else None
+                    if at is not None and b.master is not None:
+                        b.master[o - b.lo + at] = 2.5 + (0.1 if step % 2 else -0.1)
+                    p[0, 1] = 2.5 + (0.1 if step % 2 else -0.1)
+            n = d.after_step(step, "fp4")
+        assert n == 1 and float(w4[0, 1]) in (2.0, 3.0) and float(w8[0, 1]) not in (2.0, 3.0)
+
+
 def test_gemm_edges():
     a = M4.quantize(torch.randn(3, 32), row_tile=128)[0]
     b = M4.quantize(torch.randn(5, 32), row_tile=128)[0]
