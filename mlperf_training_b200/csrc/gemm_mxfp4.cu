@@ -50,8 +50,8 @@ int run(const void* a_q, const void* sfa, const void* b_q, const void* sfb, void
 // 74 CTA pairs).  Products of two e2m1 values are multiples of 1/4 up to 36: a sum of eight of them is exact in f16 (11 bits), so the codes
 // become f16 pairs, two HFMA2 chains of eight make a 32-block's sum, which goes on in fp32, scaled by both blocks' powers of two.
 // A warp owns the rows of B whose scales share 16 bytes of an atom (rows r, r + 32, r + 64, r + 96 of it), a lane a block of each at a time.
-// Measured (caches cold, tensor cores -> this): 4096 x 4096 13 -> 9 us, 4096 x 14336 20 -> 18.5, 28672 x 4096 28 -> 26; two rows take 34 us
-// there, so it is taken for one.  Bound by instructions: about three an element of B for conversion, product and scale.
+// Measured (caches cold, tensor cores -> this): 4096 x 4096 15 -> 8.5 us, 4096 x 14336 22 -> 16.5, 28672 x 4096 26 -> 23 (2.7 TB/s); two rows
+// took 34 us there, so it is taken for one.  Bound by instructions: about three an element of B for conversion, product and scale.
 struct GemvArgs {
   const uint8_t* a_q; const uint8_t* sfa;
   const uint8_t* b_q; const uint8_t* sfb;
@@ -73,7 +73,8 @@ B200_DEVICE void e2m1x8_f16(uint32_t c, __half2 (&h)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&r[i]);
 }
-B200_DEVICE float pow2_of(uint32_t e) { return __uint_as_float(e == 255u ? 0x7fffffffu : e == 0u ? 0x00400000u : e << 23); }
+// 2^(e - 127); 0 is 2^-127, below the normal numbers, 255 a NaN
+B200_DEVICE float pow2_of(uint32_t e) { return e == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(max(e << 23, 0x00400000u)); }
 
 // A step of a warp: a 32-block of each of its rows of B per lane, and the sixteen scale bytes with theirs among them, copied asynchronously into
 // the lane's own places of a ring in shared memory (so a lane waits for its own copies only).  Four steps a warp, 160 KB an SM, are in
@@ -160,7 +161,7 @@ gemv_mxfp4_kernel(const GemvArgs p) {
   uint4* xs = reinterpret_cast<uint4*>(smem + GEMV_RING);                              // [4][nb]: eight f16 each
   float* xf = reinterpret_cast<float*>(smem + GEMV_RING + (size_t)nb * 64);            // [nb] scales
   const int units = ((p.N + p.bn - 1) / p.bn) * 32 * atoms, stride = gridDim.x * GEMV_WARPS;
-  const long long row32 = 32 * p.ldb;
+  const uint32_t row32 = (uint32_t)(32 * p.ldb);       // (places inside a unit fit 32 bits: 96 rows' pitches of at most 28 KB)
   GemvWalk it;
   it.u = blockIdx.x * GEMV_WARPS + warp;
   it.step = 0;
@@ -172,8 +173,8 @@ gemv_mxfp4_kernel(const GemvArgs p) {
       uint4* dst = ring + slot * 160;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i < ahead.g.rows) copy16_async(dst + i * 32, ahead.g.src + i * row32 + kb * 16);
-      if (ahead.g.rows > 0) copy16_async(dst + 128, ahead.g.sf + (long long)(kb >> 2) * atoms * 512);
+        if (i < ahead.g.rows) copy16_async(dst + i * 32, ahead.g.src + (i * row32 + (uint32_t)kb * 16));
+      if (ahead.g.rows > 0) copy16_async(dst + 128, ahead.g.sf + (uint32_t)(kb >> 2) * (uint32_t)(atoms * 512));
     }
     copy_commit();
     ahead.next(p, units, stride, steps, kg, atoms);
@@ -248,7 +249,7 @@ int run_gemv(const GemvArgs& p, cudaStream_t stream) {
   return b200::check_launch("gemm_mxfp4(row)");
 }
 // Whether the kernel above is given the problem.
-bool one_row(int M, int K) { return M == 1 && K <= GEMV_ELEMS; }
+bool one_row(int M, int K, long long ldb) { return M == 1 && K <= GEMV_ELEMS && ldb <= GEMV_ELEMS; }
 
 }  // namespace
 
@@ -258,7 +259,7 @@ B200_API int b200_gemm_mxfp4_bn(int N) { return N <= 128 ? 128 : 192; }
 // Workspace (bytes, 16-byte aligned) with which b200_gemm_mxfp4 splits the last wave along K; 0 where that does not pay.
 B200_API long long b200_gemm_mxfp4_workspace(int M, int N, int K) {
   using namespace gemmcore;
-  if (M <= 0 || N <= 0 || K <= 0 || one_row(M, K)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || one_row(M, K, K / 2)) return 0;
   int rc = 0;
   return b200_gemm_mxfp4_bn(N) == 192 ? split_bytes<192>(pair_split<KIND_MXFP4, 192, KSUB>(M, N, K, rc))
                                       : split_bytes<128>(pair_split<KIND_MXFP4, 128, KSUB>(M, N, K, rc));
@@ -278,7 +279,7 @@ B200_API int b200_gemm_mxfp4(const void* a_q, const void* sfa, const void* b_q, 
   epi.residual = (const __nv_bfloat16*)residual;
   epi.ldr = ldr;
   epi.alpha = alpha;
-  if (one_row(M, K)) {
+  if (one_row(M, K, ldb)) {
     if ((((uintptr_t)a_q | (uintptr_t)b_q | (uintptr_t)sfb | (uintptr_t)ldb) & 15) != 0)
       return b200::fail(853, "gemm_mxfp4: operands and their row pitches must be 16-byte aligned");
     const GemvArgs p = {(const uint8_t*)a_q, (const uint8_t*)sfa, (const uint8_t*)b_q, (const uint8_t*)sfb, d, N, K, b200_gemm_mxfp4_bn(N), ldb, epi};
