@@ -4,7 +4,7 @@
 //   call(name, *args)                   converts the arguments by their codes, calls the launcher with the GIL released and raises
 //                                       RuntimeError on a code other than 0
 //   gemm(...)                           ops.kernels.gemm for CUDA operands that need no copy: checks, output, split workspace, launch
-//   quant_mxfp4, dequant_mx, norm_mx, gemm_mxfp4   the same for ops.mxfp4 and ops.norm_mx
+//   quant_mxfp4, dequant_mx, norm_mx, gemm_mxfp4, gated_fwd, gated_bwd   the same for ops.mxfp4, ops.norm_mx and the gated block
 //
 // ctypes converts twenty arguments through as many Python objects and calls: 5 of the 20 us a launch of a small model took.  With
 // it, the native GEMM operator and no autograd nodes where no gradient is wanted: a step of a two-layer model of width 512 2020 ->
@@ -107,7 +107,12 @@ using DequantFn = int (*)(const void*, const void*, void*, int, int, int, int, i
 using NormMxFn = int (*)(const void*, const void*, const void*, void*, void*, int, int, float, void*, void*, int, void*, void*, int, void*);
 using Gemm4Fn = int (*)(const void*, const void*, const void*, const void*, void*, int, int, int, long long, long long, long long, int, int,
                         const void*, const void*, long long, float, void*, long long, void*);
+using GatedFn = int (*)(const void*, const void*, void*, void*, int, int, int, long long, long long, long long, long long, int, void*);
+using GatedGradFn = int (*)(const void*, const void*, const void*, void*, void*, int, int, int, long long, long long, long long, long long, long long,
+                            int, void*);
 Quant4Fn g_quant4 = nullptr;
+GatedFn g_gated = nullptr;
+GatedGradFn g_gated_grad = nullptr;
 DequantFn g_dequant = nullptr;
 NormMxFn g_norm_mx = nullptr;
 Gemm4Fn g_gemm4 = nullptr;
@@ -131,6 +136,8 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     PyUnicode_InternInPlace(&key);
     t[key] = Entry{reinterpret_cast<void*>(addr), codes};
     if (PyUnicode_CompareWithASCIIString(key, "b200_quant_mxfp4") == 0) g_quant4 = reinterpret_cast<Quant4Fn>(addr);
+    if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_gated") == 0) g_gated = reinterpret_cast<GatedFn>(addr);
+    if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_gated_grad") == 0) g_gated_grad = reinterpret_cast<GatedGradFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_dequant_mx") == 0) g_dequant = reinterpret_cast<DequantFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_norm_mx") == 0) g_norm_mx = reinterpret_cast<NormMxFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_mxfp4") == 0) g_gemm4 = reinterpret_cast<Gemm4Fn>(addr);
@@ -427,6 +434,74 @@ PyObject* py_gemm_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+bool bf16_plain(const at::Tensor* t, c10::Device dev) {
+  return t != nullptr && t->is_cuda() && t->device() == dev && t->scalar_type() == at::kBFloat16 && plain(*t) && t->size(0) <= 0x7fffffff &&
+         t->size(1) <= 0x7fffffff;
+}
+
+// gated_fwd(x [T, D], w [2F, D], act, want_gu): (a [T, F], gu [T, 2F] or None)
+PyObject* py_gated_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *w;
+  long long act;
+  if (nargs != 4 || g_gated == nullptr || (x = tensor_of(args[0])) == nullptr || (w = tensor_of(args[1])) == nullptr || !int_of(args[2], act)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const int want = PyObject_IsTrue(args[3]);
+  if (want < 0) return nullptr;
+  if (!x->is_cuda() || !bf16_plain(x, x->device()) || !bf16_plain(w, x->device())) Py_RETURN_NONE;
+  const int64_t T = x->size(0), D = x->size(1), F = w->size(0) / 2;
+  const int dev = x->device().index();
+  if (c10::cuda::current_device() != dev || T <= 0 || D <= 0 || F <= 0 || D % 8 != 0 || F % 8 != 0 || w->size(0) != 2 * F || w->size(1) != D) Py_RETURN_NONE;
+  at::Tensor t[2];
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    const auto o = x->options().requires_grad(false);
+    t[0] = at::empty({T, F}, o);
+    if (want) t[1] = at::empty({T, 2 * F}, o);
+    rc = g_gated(x->data_ptr(), w->data_ptr(), t[0].data_ptr(), want ? t[1].data_ptr() : nullptr, (int)T, (int)F, (int)D, x->stride(0), w->stride(0),
+                 F, 2 * F, (int)act, c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  if (rc != 0) return raise_code("b200_gemm_gated", rc);
+  return wrap_all(t, 2);
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_bwd(dy [T, D], w_down [D, F], gu [T, 2F], act, want_a): (dgu [T, 2F], a [T, F] or None)
+PyObject* py_gated_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *dy, *w, *gu;
+  long long act;
+  if (nargs != 5 || g_gated_grad == nullptr || (dy = tensor_of(args[0])) == nullptr || (w = tensor_of(args[1])) == nullptr ||
+      (gu = tensor_of(args[2])) == nullptr || !int_of(args[3], act)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  const int want = PyObject_IsTrue(args[4]);
+  if (want < 0) return nullptr;
+  if (!dy->is_cuda() || !bf16_plain(dy, dy->device()) || !bf16_plain(w, dy->device()) || !bf16_plain(gu, dy->device())) Py_RETURN_NONE;
+  const int64_t T = dy->size(0), D = dy->size(1), F = w->size(1);
+  const int dev = dy->device().index();
+  if (c10::cuda::current_device() != dev || T <= 0 || D <= 0 || F <= 0 || D % 8 != 0 || F % 8 != 0 || w->size(0) != D || gu->size(0) != T ||
+      gu->size(1) != 2 * F)
+    Py_RETURN_NONE;
+  at::Tensor t[2];
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    const auto o = dy->options().requires_grad(false);
+    t[0] = at::empty({T, 2 * F}, o);
+    if (want) t[1] = at::empty({T, F}, o);
+    rc = g_gated_grad(dy->data_ptr(), w->data_ptr(), gu->data_ptr(), t[0].data_ptr(), want ? t[1].data_ptr() : nullptr, (int)T, (int)F, (int)D,
+                      dy->stride(0), w->stride(0), gu->stride(0), 2 * F, F, (int)act, c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  if (rc != 0) return raise_code("b200_gemm_gated_grad", rc);
+  return wrap_all(t, 2);
+  END_HANDLE_TH_ERRORS
+}
+
 // bind_mx(address of b200_gemm_mxfp4_workspace)
 PyObject* py_bind_mx(PyObject*, PyObject* args) {
   unsigned long long w;
@@ -450,6 +525,8 @@ PyMethodDef methods[] = {
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call)), METH_FASTCALL, nullptr},
     {"bind_mx", py_bind_mx, METH_VARARGS, nullptr},
     {"quant_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_quant_mxfp4)), METH_FASTCALL, nullptr},
+    {"gated_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gated_fwd)), METH_FASTCALL, nullptr},
+    {"gated_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gated_bwd)), METH_FASTCALL, nullptr},
     {"dequant_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_dequant_mx)), METH_FASTCALL, nullptr},
     {"norm_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_mx)), METH_FASTCALL, nullptr},
     {"gemm_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gemm_mxfp4)), METH_FASTCALL, nullptr},

@@ -9,16 +9,16 @@
 // sixteen values before they share a scale.
 //
 // Measured (caches cold): 14336 x 4096, both copies 38 us (181 MB: 4.8 TB/s), the row copy of 16384 x 4096 29 us (5.9 TB/s); 4011 x 14336, both
-// copies, with bytes and transform 68 us (236 MB).  Back to bf16: 58.7 M values of e2m1 31 us (4.8 TB/s), 67 M of e4m3 38 us (5.3 TB/s).
+// copies, with bytes and transform 68 us (236 MB).  Back to bf16: 58.7 M values of e2m1 31 us (4.8 TB/s), 67 M of e4m3 36 us (5.7 TB/s).
 #include "mx_quant.cuh"
 #include "runtime.h"
 
 namespace {
 
-// Codes to values, written to bf16 or fp32.  A lane has eight neighbouring elements, a warp eight consecutive rows: their scale bytes are 16
-// bytes apart in one atom (tile rows are multiples of 16), so one division places all of them, and eight loads of each kind are in flight.
+// Codes to values, written to bf16 or fp32.  A lane has eight neighbouring elements, a warp eight (e4m3: four) consecutive rows: their
+// scale bytes are 16 bytes apart in one atom (tile rows are multiples of 16), so one division places all of them, and as many loads of each
+// kind are in flight (e4m3 with eight 43 us for 67 M values, with four 39; e2m1 with four 37 for 59 M, with eight 35).
 // An e2m1 code becomes a bf16 by two table look-ups of its bytes (prmt) and its sign; the product with the scale, a power of two, is exact.
-constexpr int DQ_ROWS = 8;
 
 B200_DEVICE uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 // elements 0, 1 and 2, 3 of four codes in the low half of c, as bf16 pairs
@@ -33,19 +33,23 @@ B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+template <int FMT>
+constexpr int DQ_ROWS = FMT == mxq::E4M3 ? 4 : 8;
+
 template <int FMT, bool F32>
 __global__ void __launch_bounds__(256)
 mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, void* __restrict__ out, int R, int K, int tile_rows) {
   b200::begin_kernel();
+  constexpr int ROWS = DQ_ROWS<FMT>;
   const int vecs = K >> 3;
   const int v = blockIdx.x * 32 + (threadIdx.x & 31);
   if (v >= vecs) return;
-  for (long long r0 = ((long long)blockIdx.y * 8 + (threadIdx.x >> 5)) * DQ_ROWS; r0 < R; r0 += (long long)gridDim.y * 8 * DQ_ROWS) {
+  for (long long r0 = ((long long)blockIdx.y * 8 + (threadIdx.x >> 5)) * ROWS; r0 < R; r0 += (long long)gridDim.y * 8 * ROWS) {
     const uint8_t* s0 = sf + mxq::sf_offset(r0, v >> 2, tile_rows, (tile_rows + 127) >> 7, (K + 127) >> 7);
-    uint32_t e[DQ_ROWS];
-    uint2 c[DQ_ROWS];
+    uint32_t e[ROWS];
+    uint2 c[ROWS];
 #pragma unroll
-    for (int i = 0; i < DQ_ROWS; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       const bool in = r0 + i < R;
       e[i] = in ? s0[i * 16] : 0u;
       c[i] = make_uint2(0u, 0u);
@@ -55,7 +59,7 @@ mx_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf,
       }
     }
 #pragma unroll
-    for (int i = 0; i < DQ_ROWS; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       if (r0 + i >= R) break;
       // 2^(e - 127) as bf16: 0 is 2^-127, below the normal numbers; 255 is a NaN
       const uint32_t sb = e[i] == 255u ? 0x7fc0u : e[i] == 0u ? 0x0040u : e[i] << 7;
@@ -157,7 +161,7 @@ B200_API int b200_dequant_mx(const void* q, const void* sf, void* out, int R, in
   if (R <= 0 || K <= 0 || K % 32 != 0) return b200::fail(725, "dequant_mx: R=%d must be positive and K=%d a positive multiple of 32", R, K);
   if (tile_rows <= 0 || tile_rows % 16 != 0) return b200::fail(726, "dequant_mx: tile rows must be positive multiples of 16");
   if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0) return b200::fail(727, "dequant_mx: codes and output must be 16-byte aligned");
-  const int rows = (R - 1) / (8 * DQ_ROWS) + 1;
+  const int per = 8 * (fmt == mxq::E4M3 ? DQ_ROWS<mxq::E4M3> : DQ_ROWS<mxq::E2M1>), rows = (R - 1) / per + 1;
   const dim3 grid((K / 8 + 31) / 32, rows < 65535 ? rows : 65535);
   if (fmt == mxq::E4M3) launch_dequant<mxq::E4M3>(grid, (cudaStream_t)stream, q, sf, out, R, K, tile_rows, out_f32);
   else launch_dequant<mxq::E2M1>(grid, (cudaStream_t)stream, q, sf, out, R, K, tile_rows, out_f32);

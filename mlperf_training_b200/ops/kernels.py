@@ -309,6 +309,11 @@ def gated_fwd(x: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu", *, wa
     """``a = act(x Wg^T) * (x Wu^T)`` of ``x [T, D]`` and the stacked ``w_gate_up [2F, D]`` (gate rows first) in one launch.  Returns
     ``(a [T, F], gu [T, 2F])``; ``gu`` (the projections, for the backward) is None without
     ``want_gu``."""
+    if x.is_cuda and act in GATE_ACTS and use_kernels(x) and _lib.host is not None:
+        # (results for operands that are as the kernel reads them; None leaves copies and errors to the lines below)
+        r = _lib.host.gated_fwd(x, w_gate_up, GATE_ACTS[act], want_gu)
+        if r is not None:
+            return r
     T, D = x.shape
     Fh = w_gate_up.shape[0] // 2
     _gate_check("gated_fwd", x, w_gate_up, act, Fh, D)
@@ -331,6 +336,10 @@ def gated_bwd(dy: torch.Tensor, w_down: torch.Tensor, gu: torch.Tensor, act: str
     """Gradient of ``gu [T, 2F]`` from that of ``a W_down^T``, ``dy [T, D]``, ``w_down [D, F]``, in one launch: ``da = dy W_down``, ``d gate = da
     * up * act'(gate)``, ``d up = da * act(gate)``.  Returns ``(dgu [T, 2F], a [T, F])``; ``a`` (made again from ``gu``, for the gradient of
     ``w_down``) is None without ``want_a``."""
+    if dy.is_cuda and act in GATE_ACTS and use_kernels(dy) and _lib.host is not None:
+        r = _lib.host.gated_bwd(dy, w_down, gu, GATE_ACTS[act], want_a)
+        if r is not None:
+            return r
     T, F2 = gu.shape
     D, Fh = w_down.shape
     _gate_check("gated_bwd", dy, w_down, act, Fh, D)

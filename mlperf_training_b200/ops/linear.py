@@ -172,8 +172,10 @@ def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
     if cacheable:
         event = None
         if w.is_cuda and not torch.cuda.is_current_stream_capturing():
+            # (torch.cuda.current_stream(), which record() would call, takes several Python layers)
+            i, d, t = torch._C._cuda_getCurrentStream(torch._C._cuda_getDevice())
             event = torch.cuda.Event()
-            event.record()
+            event.record(torch.cuda.Stream(stream_id=i, device_index=d, device_type=t))
         weight._mx4_cache = (key, row, col, stream_ptr() if w.is_cuda else None, event)
     return row, col
 
