@@ -1,4 +1,4 @@
-// Gated projections of few activation rows (gated_fewrows.cu).
+// Gated projections, and the down projection behind them, of few activation rows (gated_fewrows.cu).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -15,5 +15,13 @@ struct GatedArgs {
   int act;
 };
 int run_gated(const GatedArgs& p, cudaStream_t stream);
+
+struct DownArgs {
+  const __nv_bfloat16* a; const __nv_bfloat16* w;     // [M, K], [N, K]
+  const __nv_bfloat16* res; __nv_bfloat16* y;         // [M, N] or null, [M, N]
+  int M, N, K;
+  long long lda, ldw, ldr, ldy;
+};
+int run_down(const DownArgs& p, cudaStream_t stream);
 
 }  // namespace fewrows

@@ -1,6 +1,7 @@
 // Gated feed-forward block in bf16, on the CTA-pair mainloop of gemm_core.cuh:
 //
 //   b200_gemm_gated       a = act(x Wg^T) * (x Wu^T), optionally with the projections themselves (gu, kept for the backward), in one launch
+//   b200_gated_down       y = a Wd^T (+ residual) of up to 64 rows (more are a plain GEMM)
 //   b200_gemm_gated_grad  da = dy Wd, then d gate = da u act'(g), d up = da act(g) and a again, in one launch
 //
 // W = [Wg; Wu] is the stacked [2F, D] weight of the two projections as the model keeps it.  A 256-row tile of 128 output columns runs as one
@@ -56,6 +57,17 @@ B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, in
   p.a_rows = a_box_rows(M);
   p.status = b200::status_ptr();
   return launch_pair<KIND_BF16, 256, 1, 1, 1>(tmX, tmW, tmG, tmU, tmA, tmA, p, (cudaStream_t)stream, "gemm_gated");
+}
+
+// a [M, K], w [N, K], res [M, N] or null, y [M, N]; M up to 64, N and K multiples of 8; pitches as above (any for res and y, which need 2-byte alignment).
+B200_API int b200_gated_down(const void* a, const void* w, const void* res, void* y, int M, int N, int K, long long lda, long long ldw,
+                             long long ldr, long long ldy, void* stream) {
+  if (M <= 0 || M > fewrows::MAX_ROWS || N <= 0 || K <= 0) return b200::fail(865, "gated_down: %d x %d x %d is not a product of 1 to 64 rows", M, N, K);
+  if (N % 8 != 0 || K % 8 != 0) return b200::fail(866, "gated_down: N=%d and K=%d must be multiples of 8", N, K);
+  int r;
+  if ((r = check("gated_down", a, lda)) || (r = check("gated_down", w, ldw))) return r;
+  const fewrows::DownArgs p = {(const __nv_bfloat16*)a, (const __nv_bfloat16*)w, (const __nv_bfloat16*)res, (__nv_bfloat16*)y, M, N, K, lda, ldw, ldr, ldy};
+  return fewrows::run_down(p, (cudaStream_t)stream);
 }
 
 // dy [M, K], wd [K, F] (the down projection's weight as it is), gu [M, 2F]; dgu [M, 2F], a [M, F] or null.

@@ -4,7 +4,7 @@
 //   call(name, *args)                   converts the arguments by their codes, calls the launcher with the GIL released and raises
 //                                       RuntimeError on a code other than 0
 //   gemm(...)                           ops.kernels.gemm for CUDA operands that need no copy: checks, output, split workspace, launch
-//   quant_mxfp4, dequant_mx, norm_mx, gemm_mxfp4, gated_fwd, gated_bwd   the same for ops.mxfp4, ops.norm_mx and the gated block
+//   quant_mxfp4, dequant_mx, norm_mx, gemm_mxfp4, gated_fwd, gated_down, gated_bwd   the same for ops.mxfp4, ops.norm_mx and the gated block
 //
 // ctypes converts twenty arguments through as many Python objects and calls: 5 of the 20 us a launch of a small model took.  With
 // it, the native GEMM operator and no autograd nodes where no gradient is wanted: a step of a two-layer model of width 512 2020 ->
@@ -110,8 +110,10 @@ using Gemm4Fn = int (*)(const void*, const void*, const void*, const void*, void
 using GatedFn = int (*)(const void*, const void*, void*, void*, int, int, int, long long, long long, long long, long long, int, void*);
 using GatedGradFn = int (*)(const void*, const void*, const void*, void*, void*, int, int, int, long long, long long, long long, long long, long long,
                             int, void*);
+using DownFn = int (*)(const void*, const void*, const void*, void*, int, int, int, long long, long long, long long, long long, void*);
 Quant4Fn g_quant4 = nullptr;
 GatedFn g_gated = nullptr;
+DownFn g_down = nullptr;
 GatedGradFn g_gated_grad = nullptr;
 DequantFn g_dequant = nullptr;
 NormMxFn g_norm_mx = nullptr;
@@ -137,6 +139,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     t[key] = Entry{reinterpret_cast<void*>(addr), codes};
     if (PyUnicode_CompareWithASCIIString(key, "b200_quant_mxfp4") == 0) g_quant4 = reinterpret_cast<Quant4Fn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_gated") == 0) g_gated = reinterpret_cast<GatedFn>(addr);
+    if (PyUnicode_CompareWithASCIIString(key, "b200_gated_down") == 0) g_down = reinterpret_cast<DownFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_gated_grad") == 0) g_gated_grad = reinterpret_cast<GatedGradFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_dequant_mx") == 0) g_dequant = reinterpret_cast<DequantFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_norm_mx") == 0) g_norm_mx = reinterpret_cast<NormMxFn>(addr);
@@ -469,6 +472,34 @@ PyObject* py_gated_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// gated_down(a [T, F], w [D, F], residual [T, D] or None): y [T, D], T up to 64
+PyObject* py_gated_down(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *a, *w, *res = nullptr;
+  if (nargs != 3 || g_down == nullptr || (a = tensor_of(args[0])) == nullptr || (w = tensor_of(args[1])) == nullptr ||
+      (args[2] != Py_None && (res = tensor_of(args[2])) == nullptr)) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
+  }
+  if (!a->is_cuda() || !bf16_plain(a, a->device()) || !bf16_plain(w, a->device()) || (res != nullptr && !bf16_plain(res, a->device()))) Py_RETURN_NONE;
+  const int64_t T = a->size(0), F = a->size(1), D = w->size(0);
+  const int dev = a->device().index();
+  if (c10::cuda::current_device() != dev || T <= 0 || T > 64 || D <= 0 || F <= 0 || D % 8 != 0 || F % 8 != 0 || w->size(1) != F ||
+      (res != nullptr && (res->size(0) != T || res->size(1) != D)))
+    Py_RETURN_NONE;
+  at::Tensor t[1];
+  int rc;
+  {
+    pybind11::gil_scoped_release nogil;
+    t[0] = at::empty({T, D}, a->options().requires_grad(false));
+    rc = g_down(a->data_ptr(), w->data_ptr(), res != nullptr ? res->data_ptr() : nullptr, t[0].data_ptr(), (int)T, (int)D, (int)F, a->stride(0), w->stride(0),
+                res != nullptr ? res->stride(0) : 0, D, c10::cuda::getCurrentCUDAStream(dev).stream());
+  }
+  if (rc != 0) return raise_code("b200_gated_down", rc);
+  return THPVariable_Wrap(t[0]);
+  END_HANDLE_TH_ERRORS
+}
+
 // gated_bwd(dy [T, D], w_down [D, F], gu [T, 2F], act, want_a): (dgu [T, 2F], a [T, F] or None)
 PyObject* py_gated_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -526,6 +557,7 @@ PyMethodDef methods[] = {
     {"bind_mx", py_bind_mx, METH_VARARGS, nullptr},
     {"quant_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_quant_mxfp4)), METH_FASTCALL, nullptr},
     {"gated_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gated_fwd)), METH_FASTCALL, nullptr},
+    {"gated_down", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gated_down)), METH_FASTCALL, nullptr},
     {"gated_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_gated_bwd)), METH_FASTCALL, nullptr},
     {"dequant_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_dequant_mx)), METH_FASTCALL, nullptr},
     {"norm_mx", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_mx)), METH_FASTCALL, nullptr},

@@ -88,6 +88,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_gemm_mxfp4": [P, P, P, P, P, I, I, I, L, L, L, I, I, P, P, L, F, P, L, P],
         "b200_norm_mx": [P, P, P, P, P, I, I, F, P, P, I, P, P, I, P],
         "b200_gemm_gated": [P, P, P, P, I, I, I, L, L, L, L, I, P],
+        "b200_gated_down": [P, P, P, P, I, I, I, L, L, L, L, P],
         "b200_gemm_gated_grad": [P, P, P, P, P, I, I, I, L, L, L, L, L, I, P],
         "b200_router_topk": [P, I, I, I, P, P, P, P],
         "b200_router_plan": [P, P, I, I, I, P, P, I, P, P],

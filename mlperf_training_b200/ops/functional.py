@@ -284,7 +284,7 @@ class GatedMLPFn(Function):
         grad = grad and any(ctx.needs_input_grad)
         a, gu = K.gated_fwd(x, w_gate_up, act, want_gu=grad)
         if a.shape[0]:
-            y = K.gemm(a, w_down, residual=residual)
+            y = K.gated_down(a, w_down, residual)
         else:
             y = x.new_empty((0, w_down.shape[0]))
         ctx.save_for_backward(x, w_gate_up, w_down, gu)

@@ -332,6 +332,39 @@ def gated_fwd(x: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu", *, wa
     return a, gu
 
 
+def _down_few_rows(T: int, D: int, Fh: int) -> bool:
+    """Whether the weight is to be the tile's rows in a down projection: up to 32 rows, up to 64 where the contraction is split over CTAs (each CTA then
+    finishes a part of the tokens).  Against ``gemm``, with a residual: 7 rows of 4096 x 14336 35 us for 44, 64 rows 37 for 44, but 64 rows
+    of 256 x 256 16 for 12 and of 16384 x 4096 47 for 43."""
+    return 1 <= T <= 32 or (T <= 64 and Fh >= 1024 and D <= 8192)
+
+
+def gated_down(a: torch.Tensor, w_down: torch.Tensor, residual: torch.Tensor | None = None):
+    """``y = a W_down^T (+ residual)`` of the gated block's ``a [T, F]`` and ``w_down [D, F]``.  A few rows read the weight split along F over
+    clusters of CTAs; more rows, and operands that are not bf16 on the GPU, are a ``gemm``."""
+    if not use_kernels(a) or a.dtype != BF16 or not _down_few_rows(a.shape[0], w_down.shape[0], a.shape[1]):
+        return gemm(a, w_down, residual=residual)
+    if _lib.host is not None:
+        r = _lib.host.gated_down(a, w_down, residual)
+        if r is not None:
+            return r
+    T, Fh = a.shape
+    D = w_down.shape[0]
+    _gate_check("gated_down", a, w_down, "silu", Fh, D)
+    if w_down.shape[1] != Fh:
+        raise ValueError(f"gated_down: weight {tuple(w_down.shape)} for {Fh} columns")
+    if residual is not None:
+        if residual.shape != (T, D) or residual.device != a.device:
+            raise ValueError(f"gated_down: residual {tuple(residual.shape)} on {residual.device} for an output {T}x{D} on {a.device}")
+        if residual.dtype != BF16 or residual.stride(1) != 1:
+            residual = residual.to(BF16).contiguous()
+    a, w = _row_major(a), _row_major(w_down)
+    y = torch.empty((T, D), dtype=BF16, device=a.device)
+    call("b200_gated_down", ptr(a), ptr(w), ptr(residual), ptr(y), T, D, Fh, a.stride(0), w.stride(0), 0 if residual is None else residual.stride(0),
+         y.stride(0), stream_ptr())
+    return y
+
+
 def gated_bwd(dy: torch.Tensor, w_down: torch.Tensor, gu: torch.Tensor, act: str = "silu", *, want_a: bool = True):
     """Gradient of ``gu [T, 2F]`` from that of ``a W_down^T``, ``dy [T, D]``, ``w_down [D, F]``, in one launch: ``da = dy W_down``, ``d gate = da
     * up * act'(gate)``, ``d up = da * act(gate)``.  Returns ``(dgu [T, 2F], a [T, F])``; ``a`` (made again from ``gu``, for the gradient of

@@ -129,3 +129,52 @@ def test_refusals():
         F.gated_mlp(x.cpu(), w, wd)
     with pytest.raises(RuntimeError, match="multiples of 8"):
         _lib.call("b200_gemm_gated", x.data_ptr(), w.data_ptr(), x.data_ptr(), None, 4, 12, 64, 64, 64, 16, 0, 0, _lib.stream_ptr())
+
+
+@pytest.mark.parametrize("T", [1, 7, 8, 16, 17, 33, 64])
+@pytest.mark.parametrize("N,Fh", [(8, 8), (136, 64), (128, 72), (264, 1000), (1000, 1032), (512, 2056), (4096, 14336), (19008, 512)])
+def test_down_projection_of_few_rows(T, N, Fh):
+    """Against 64 bits: the one rounding to bf16 (2^-9, doubled for a sum near a boundary), and 2^-23 of the running sum, taken as twice the
+    largest result, for each of the Fh / 16 steps of the accumulation.  The same result every time; strided and broadcast residuals."""
+    g = torch.Generator(device="cuda").manual_seed(T + N + Fh)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    a, w, r = n(T, Fh).bfloat16(), (n(N, Fh) * Fh ** -0.5).bfloat16(), n(T, N).bfloat16()
+    wide = torch.zeros(T, N + 16, device="cuda").bfloat16()
+    wide[:, 8:N + 8] = r
+    for res in (None, r, wide[:, 8:N + 8], r[:1].expand(T, N)):
+        y = K.gated_down(a, w, res)
+        want = a.double() @ w.double().t() + (0 if res is None else res.double())
+        assert bool(((y.double() - want).abs() <= want.abs() * 2 ** -8 + max(1, Fh / 16) * 2 ** -22 * want.abs().max()).all())
+        assert torch.equal(K.gated_down(a, w, res), y)
+    _lib.check_status("gated_down")
+
+
+def test_down_projection_keeps_rows_apart_and_leaves_neighbours_alone():
+    """A row with a NaN or an infinity stays apart; a weight row too; operands inside larger buffers filled with NaN."""
+    T, N, Fh = 9, 200, 1096
+    big_a = torch.full((T + 8, Fh + 64), float("nan"), device="cuda").bfloat16()
+    big_w = torch.full((N + 128, Fh + 64), float("nan"), device="cuda").bfloat16()
+    big_a[:T, :Fh] = torch.randn(T, Fh, device="cuda").bfloat16()
+    big_w[:N, :Fh] = torch.randn(N, Fh, device="cuda").bfloat16()
+    a, w = big_a[:T, :Fh], big_w[:N, :Fh]
+    y = K.gated_down(a, w)
+    assert bool(y.isfinite().all()) and torch.equal(y, K.gated_down(a.contiguous(), w.contiguous()))
+    a[3, 1095], w[150, 0] = float("nan"), float("inf")
+    z = K.gated_down(a, w)
+    keep = torch.ones(T, N, dtype=torch.bool, device="cuda")
+    keep[3], keep[:, 150] = False, False
+    assert torch.equal(z[keep], y[keep]) and bool(z[3].isnan().all()) and not bool(z[:, 150].isfinite().any())
+
+
+def test_down_projection_refusals_and_more_rows():
+    a, w = torch.randn(4, 64, device="cuda").bfloat16(), torch.randn(72, 64, device="cuda").bfloat16()
+    for bad in (lambda: K.gated_down(a, w[:, :56]), lambda: K.gated_down(a, w[:71]), lambda: K.gated_down(a, w.cpu()),
+                lambda: K.gated_down(a, w, torch.zeros(4, 64, device="cuda").bfloat16())):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        K.gated_down(a, w.float())
+    with pytest.raises(RuntimeError, match="1 to 64 rows"):
+        _lib.call("b200_gated_down", a.data_ptr(), w.data_ptr(), None, a.data_ptr(), 65, 72, 64, 64, 64, 0, 72, _lib.stream_ptr())
+    many = torch.randn(65, 64, device="cuda").bfloat16()
+    assert torch.equal(K.gated_down(many, w), K.gemm(many, w))
