@@ -172,7 +172,8 @@ gated_fewrows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
 // The weight is [N, K] with few rows and a long K, so that its 128-row tiles alone would leave most SMs idle (32 tiles of 4096 rows).  A cluster of
 // 1, 2, 4 or 8 CTAs owns a tile, each CTA a run of K; they put their fp32 sums into their own shared memory (the operands are done with it) and
 // each adds up every gridDim.y-th token of the tile, reading its neighbours' sums in the order of the ranks: one launch, no workspace, no atomics, the
-// same result every time.  A stage is 128 elements of K of 128 weight rows, four stages of 48 KB.  The residual is brought into L2 meanwhile, and the
+// same result every time.  A stage is 128 elements of K of 128 weight rows, four stages of 48 KB
+// (7 x 4096 x 14336: 24.5 us, 4.8 TB/s; the general GEMM and the sum of its parts 36).  The residual is brought into L2 meanwhile, and the
 // tokens are finished eight at a time: one after the other each waited 0.5 us for its own loads (64 rows of 4096 x 1024: 33 -> 16 us).
 constexpr int D_STAGES = 4;
 constexpr int DA_STAGE = 2 * 128 * 128, DB_STAGE = 2 * fewrows::MAX_ROWS * 128;
