@@ -169,9 +169,10 @@ def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
         w = w.to(torch.bfloat16)
     new_row, col = M4.quantize(w, row_tile=M4.b_tile(N) if row is None else None, col_tile=M4.b_tile(Kd) if need_col else None)
     row = new_row if row is None else row
-    if cacheable:
+    # (what a capture records has not been made when the call returns: such copies belong to that graph alone)
+    if cacheable and not (w.is_cuda and torch.cuda.is_current_stream_capturing()):
         event = None
-        if w.is_cuda and not torch.cuda.is_current_stream_capturing():
+        if w.is_cuda:
             # (torch.cuda.current_stream(), which record() would call, takes several Python layers)
             i, d, t = torch._C._cuda_getCurrentStream(torch._C._cuda_getDevice())
             event = torch.cuda.Event()
