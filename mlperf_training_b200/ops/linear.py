@@ -152,12 +152,14 @@ def fp4_eligible(rows: int, n_out: int, n_in: int) -> bool:
 
 def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
     """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, cached on the tensor until it changes: through torch (its
-    version counter) or through an optimizer step.  A call on another stream than the one that made them waits for them there."""
-    cacheable = not weight.is_inference()
-    key = (_WEIGHT_EPOCH if weight.requires_grad else -1, weight._version if cacheable else -1)
-    cache = getattr(weight, "_mx4_cache", None)
+    version counter) or through an optimizer step.  A call on another stream than the one that made them waits for them there.  A call under
+    graph capture makes its own, inside the graph: what it records is not made yet when it returns, copies made outside the graph may be gone
+    when it is replayed, and a replay follows the weight as it does with any tensor."""
+    keep = not weight.is_inference() and not (weight.is_cuda and torch.cuda.is_current_stream_capturing())
+    key = (_WEIGHT_EPOCH if weight.requires_grad else -1, weight._version if keep else -1)
+    cache = getattr(weight, "_mx4_cache", None) if keep else None
     row = None
-    if cacheable and cache is not None and cache[0] == key:
+    if cache is not None and cache[0] == key:
         if cache[3] is not None and cache[3] != stream_ptr():
             _use_here(cache)
         if cache[2] is not None or not need_col:
@@ -169,8 +171,7 @@ def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
         w = w.to(torch.bfloat16)
     new_row, col = M4.quantize(w, row_tile=M4.b_tile(N) if row is None else None, col_tile=M4.b_tile(Kd) if need_col else None)
     row = new_row if row is None else row
-    # (what a capture records has not been made when the call returns: such copies belong to that graph alone)
-    if cacheable and not (w.is_cuda and torch.cuda.is_current_stream_capturing()):
+    if keep:
         event = None
         if w.is_cuda:
             # (torch.cuda.current_stream(), which record() would call, takes several Python layers)
@@ -182,10 +183,7 @@ def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
 
 
 def _use_here(cache) -> None:
-    """Order the current stream behind the making of cached copies, and keep their memory until it is done with them.  (While a graph
-    is captured the caller has synchronised with what was made before, as for every tensor that a capture reads.)"""
-    if torch.cuda.is_current_stream_capturing() or cache[4] is None:
-        return
+    """Order the current stream behind the making of cached copies, and keep their memory until it is done with them."""
     here = torch.cuda.current_stream()
     here.wait_event(cache[4])
     for op in cache[1:3]:

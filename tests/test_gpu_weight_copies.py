@@ -56,3 +56,18 @@ def test_copies_recorded_by_a_capture_are_not_kept(layer, frozen):
         g.replay()
         assert torch.equal(y, want)
     _lib.check_status("capture")
+
+
+@pytest.mark.parametrize("layer", [fp4])
+def test_a_graph_does_not_read_copies_made_outside_it(layer):
+    """They may be gone when it is replayed, and a replay follows the weight as it does with any tensor."""
+    x, w = operands(128)
+    want = layer(x, w)
+    torch.cuda.synchronize()
+    g, y = capture(layer, x, w)
+    w.mul_(-1)
+    assert torch.equal(layer(x, w), -want)              # (the copies that the first call left are replaced)
+    junk = poison()
+    g.replay()
+    assert torch.equal(y, -want)
+    del junk
