@@ -26,6 +26,7 @@ llama2_sft/primus/src/llama2_custom.py:1904-1910 pre-quantises frozen base weigh
 from __future__ import annotations
 
 import torch
+from torch.multiprocessing.reductions import StorageWeakRef
 
 from . import fp8 as F8
 from . import kernels as K
@@ -150,13 +151,20 @@ def fp4_eligible(rows: int, n_out: int, n_in: int) -> bool:
     return rows > 0 and n_out > 0 and n_in > 0 and n_out % 32 == 0 and n_in % 32 == 0
 
 
+def _identity(weight: torch.Tensor):
+    """What a change of ``weight`` through torch alters: the version that in-place operations count up, storage, type, layout, device.
+    (The reference names the storage for good and does not keep its memory; an address may come back with another one.)"""
+    return (weight._version, StorageWeakRef(weight.untyped_storage()), weight.data_ptr(), weight.dtype, weight.shape, weight.stride(), weight.device)
+
+
 def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
-    """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, cached on the tensor until it changes: through torch (its
-    version counter) or through an optimizer step.  A call on another stream than the one that made them waits for them there.  A call under
+    """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, cached on the tensor until it changes: through torch
+    (in place, or with other storage) or through an optimizer step.  What torch does not see - writes through ``weight.data``, or by a kernel - has
+    to be followed by ``bump_weight_epoch()``.  A call on another stream than the one that made them waits for them there.  A call under
     graph capture makes its own, inside the graph: what it records is not made yet when it returns, copies made outside the graph may be gone
     when it is replayed, and a replay follows the weight as it does with any tensor."""
     keep = not weight.is_inference() and not (weight.is_cuda and torch.cuda.is_current_stream_capturing())
-    key = (_WEIGHT_EPOCH if weight.requires_grad else -1, weight._version if keep else -1)
+    key = (_WEIGHT_EPOCH if weight.requires_grad else -1, _identity(weight)) if keep else None
     cache = getattr(weight, "_mx4_cache", None) if keep else None
     row = None
     if cache is not None and cache[0] == key:

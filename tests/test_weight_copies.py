@@ -1,0 +1,49 @@
+"""Low-precision weight copies kept on a weight: what they follow (CPU)."""
+import pytest
+import torch
+
+from mlperf_training_b200.ops import functional as F
+from mlperf_training_b200.ops import linear as L
+
+
+def fp4(x, w):
+    return F.mxfp4_linear(x, w)
+
+
+def behind_norm(x, w):
+    return F.add_norm_linear(x, None, torch.ones(x.shape[1]), w)[0]
+
+
+def operands():
+    torch.manual_seed(0)
+    return torch.randn(128, 128), torch.nn.Parameter(torch.randn(256, 128))
+
+
+@pytest.mark.parametrize("layer", [fp4])
+def test_copies_follow_other_storage(layer):
+    """New storage under the same tensor (``.data``, ``Module.to`` and its relatives), another layout of the same storage."""
+    x, w = operands()
+    y = layer(x, w).detach()
+    w.data = -w.data
+    assert torch.equal(layer(x, w), -y)
+    m = torch.nn.Module()
+    m.w = w
+    m._apply(lambda t: -t)
+    assert torch.equal(layer(x, m.w), y)
+    square = torch.randn(128, 128)
+    v = square.clone()
+    layer(x, v)
+    v.data = v.data.t()                          # same pointer and shape, other strides
+    assert torch.equal(layer(x, v), layer(x, v.detach().clone()))
+
+
+@pytest.mark.parametrize("layer", [fp4])
+def test_an_address_that_comes_back_is_another_storage(layer):
+    x, w = operands()
+    y = layer(x, w).detach()
+    held = w.detach().numpy().copy()
+    w.data = torch.from_numpy(held)
+    layer(x, w)
+    held *= -1
+    w.data = torch.from_numpy(held)
+    assert torch.equal(layer(x, w), -y)
