@@ -94,28 +94,82 @@ def mx_eligible(rows: int, n_out: int, n_in: int) -> bool:
     return rows % 128 == 0 and n_out % 128 == 0 and n_in % 128 == 0
 
 
-def weight_operands(weight: torch.Tensor, need_col: bool = True, fmt: str = "e4m3", col_fmt: str | None = None):
-    """(w_row, w_col) micro-scaled copies of ``weight`` ``[N, K]``: ``w_row`` (rows N, contraction K) is
-    the B operand of forward, ``w_col`` (rows K, contraction N) the B operand of dgrad.  Cached on
-    the tensor until the next optimizer step (or forever for frozen weights); ``fmt`` / ``col_fmt``: their element
-    formats (part of the cache key)."""
-    cache = getattr(weight, "_mx_cache", None)
-    col_fmt = col_fmt or fmt
-    epoch = (_WEIGHT_EPOCH if weight.requires_grad else -1, fmt, col_fmt)
+def _identity(weight: torch.Tensor):
+    """What a change of ``weight`` through torch alters: the version that in-place operations count up, storage, type, layout, device.
+    (The reference names the storage for good and does not keep its memory; an address may come back with another one.)"""
+    return (weight._version, StorageWeakRef(weight.untyped_storage()), weight.data_ptr(), weight.dtype, weight.shape, weight.stride(), weight.device)
+
+
+def _epoch(weight: torch.Tensor) -> int:
+    return _WEIGHT_EPOCH if weight.requires_grad else -1
+
+
+def _kept_copies(weight: torch.Tensor, slot: str, formats: tuple, need_col: bool, make):
+    """(row, col) copies of ``weight [N, K]`` for forward and dgrad, kept on the tensor under ``slot`` until it changes: through torch (in
+    place, or with other storage) or through an optimizer step.  What torch does not see - writes through ``weight.data``, or by a kernel -
+    has to be followed by ``bump_weight_epoch()``.  ``make(w, need_row, need_col)``: the copies asked for; ``formats``: what besides the
+    weight they depend on.
+
+    A call on another stream than the one that made them waits for them there.  A call under graph capture makes its own, inside the
+    graph: what it records is not made yet when it returns, copies made outside the graph may be gone when it is replayed, and a replay
+    follows the weight as it does with any tensor.  Of tensors made in inference mode, whose updates torch does not count, none are kept.
+
+    An entry: ((epoch, *formats), row, col, identity of the weight, stream, event behind the making)."""
+    keep = not weight.is_inference() and not (weight.is_cuda and torch.cuda.is_current_stream_capturing())
     row = None
-    if cache is not None and cache[0] == epoch:
-        if cache[2] is not None or not need_col:
-            return cache[1], cache[2]
-        row = cache[1]                   # (a forward that expected no backward left it: only the other copy is missing)
-    N, Kd = weight.shape
+    if keep:
+        key, same = (_epoch(weight), *formats), _identity(weight)
+        cache = getattr(weight, slot, None)
+        if cache is not None and cache[0] == key and cache[3] == same:
+            if cache[4] is not None and cache[4] != stream_ptr():
+                _use_here(cache)
+            if cache[2] is not None or not need_col:
+                return cache[1], cache[2]
+            row = cache[1]               # (a forward that expected no backward left it: only the other copy is missing)
     w = weight.detach()
     if w.dtype != torch.bfloat16 and w.is_cuda:
         w = w.to(torch.bfloat16)
-    new_row, col = MX.quantize(w, row_tile=MX.b_tile(N) if row is None else None, col_tile=MX.b_tile(Kd) if need_col else None, fmt=fmt,
-                               col_fmt=col_fmt)
+    new_row, col = make(w, row is None, need_col)
     row = new_row if row is None else row
-    weight._mx_cache = (epoch, row, col)
+    if keep:
+        stream = event = None
+        if w.is_cuda:
+            # (torch.cuda.current_stream(), which record() would call, takes several Python layers)
+            i, d, t = torch._C._cuda_getCurrentStream(torch._C._cuda_getDevice())
+            stream, event = stream_ptr(), torch.cuda.Event()
+            event.record(torch.cuda.Stream(stream_id=i, device_index=d, device_type=t))
+        setattr(weight, slot, (key, row, col, same, stream, event))
     return row, col
+
+
+def _use_here(cache) -> None:
+    """Order the current stream behind the making of kept copies, and keep their memory until it is done with them."""
+    here = torch.cuda.current_stream()
+    here.wait_event(cache[5])
+    for op in cache[1:3]:
+        if op is not None:
+            op.q.record_stream(here)
+            op.sf.record_stream(here)
+
+
+def copies_kept(weight: torch.Tensor, slot: str, need_col: bool) -> bool:
+    """Whether the copies under ``slot`` are those of the weight as it is now (in whatever format they were made)."""
+    cache = getattr(weight, slot, None)
+    return (cache is not None and cache[0][0] == _epoch(weight) and (cache[2] is not None or not need_col)
+            and not weight.is_inference() and cache[3] == _identity(weight))
+
+
+def weight_operands(weight: torch.Tensor, need_col: bool = True, fmt: str = "e4m3", col_fmt: str | None = None):
+    """(w_row, w_col) micro-scaled copies of ``weight`` ``[N, K]``: ``w_row`` (rows N, contraction K) is
+    the B operand of forward, ``w_col`` (rows K, contraction N) the B operand of dgrad; ``fmt`` / ``col_fmt``: their element
+    formats.  Kept on the tensor by the rules of ``_kept_copies``."""
+    N, Kd = weight.shape
+    col_fmt = col_fmt or fmt
+
+    def make(w, need_row, need_col):
+        return MX.quantize(w, row_tile=MX.b_tile(N) if need_row else None, col_tile=MX.b_tile(Kd) if need_col else None, fmt=fmt, col_fmt=col_fmt)
+
+    return _kept_copies(weight, "_mx_cache", (fmt, col_fmt), need_col, make)
 
 
 def _site(weight: torch.Tensor, name: str, fmt: str) -> "F8.DelayedScale":
@@ -151,53 +205,14 @@ def fp4_eligible(rows: int, n_out: int, n_in: int) -> bool:
     return rows > 0 and n_out > 0 and n_in > 0 and n_out % 32 == 0 and n_in % 32 == 0
 
 
-def _identity(weight: torch.Tensor):
-    """What a change of ``weight`` through torch alters: the version that in-place operations count up, storage, type, layout, device.
-    (The reference names the storage for good and does not keep its memory; an address may come back with another one.)"""
-    return (weight._version, StorageWeakRef(weight.untyped_storage()), weight.data_ptr(), weight.dtype, weight.shape, weight.stride(), weight.device)
-
-
 def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
-    """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, cached on the tensor until it changes: through torch
-    (in place, or with other storage) or through an optimizer step.  What torch does not see - writes through ``weight.data``, or by a kernel - has
-    to be followed by ``bump_weight_epoch()``.  A call on another stream than the one that made them waits for them there.  A call under
-    graph capture makes its own, inside the graph: what it records is not made yet when it returns, copies made outside the graph may be gone
-    when it is replayed, and a replay follows the weight as it does with any tensor."""
-    keep = not weight.is_inference() and not (weight.is_cuda and torch.cuda.is_current_stream_capturing())
-    key = (_WEIGHT_EPOCH if weight.requires_grad else -1, _identity(weight)) if keep else None
-    cache = getattr(weight, "_mx4_cache", None) if keep else None
-    row = None
-    if cache is not None and cache[0] == key:
-        if cache[3] is not None and cache[3] != stream_ptr():
-            _use_here(cache)
-        if cache[2] is not None or not need_col:
-            return cache[1], cache[2]
-        row = cache[1]
+    """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, kept on the tensor by the rules of ``_kept_copies``."""
     N, Kd = weight.shape
-    w = weight.detach()
-    if w.dtype != torch.bfloat16 and w.is_cuda:
-        w = w.to(torch.bfloat16)
-    new_row, col = M4.quantize(w, row_tile=M4.b_tile(N) if row is None else None, col_tile=M4.b_tile(Kd) if need_col else None)
-    row = new_row if row is None else row
-    if keep:
-        event = None
-        if w.is_cuda:
-            # (torch.cuda.current_stream(), which record() would call, takes several Python layers)
-            i, d, t = torch._C._cuda_getCurrentStream(torch._C._cuda_getDevice())
-            event = torch.cuda.Event()
-            event.record(torch.cuda.Stream(stream_id=i, device_index=d, device_type=t))
-        weight._mx4_cache = (key, row, col, stream_ptr() if w.is_cuda else None, event)
-    return row, col
 
+    def make(w, need_row, need_col):
+        return M4.quantize(w, row_tile=M4.b_tile(N) if need_row else None, col_tile=M4.b_tile(Kd) if need_col else None)
 
-def _use_here(cache) -> None:
-    """Order the current stream behind the making of cached copies, and keep their memory until it is done with them."""
-    here = torch.cuda.current_stream()
-    here.wait_event(cache[4])
-    for op in cache[1:3]:
-        if op is not None:
-            op.q.record_stream(here)
-            op.sf.record_stream(here)
+    return _kept_copies(weight, "_mx4_cache", (), need_col, make)
 
 
 def fp4_forward(x: torch.Tensor, weight: torch.Tensor, *, bias=None, residual=None, need_wgrad: bool = True, need_dgrad: bool = False):

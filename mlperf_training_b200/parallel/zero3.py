@@ -180,12 +180,7 @@ class Zero3Engine(ZeroEngine):
     def _cached(self, b, need_col: bool) -> bool:
         if not self.skip_cached:
             return False
-        for _, p in b.params:
-            c = getattr(p, "_mx_cache", None)
-            epoch = L._WEIGHT_EPOCH if p.requires_grad else -1
-            if c is None or c[0][0] != epoch or (need_col and c[2] is None):      # key: (epoch, row format, column format)
-                return False
-        return True
+        return all(L.copies_kept(p, "_mx_cache", need_col) for _, p in b.params)
 
     def _ensure(self, idx: int, need_col: bool, prefetch: bool) -> None:
         b = self._by_block3.get(idx)

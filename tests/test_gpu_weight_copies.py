@@ -39,7 +39,7 @@ def capture(layer, x, w):
     return g, y
 
 
-@pytest.mark.parametrize("layer", [fp4])
+@pytest.mark.parametrize("layer", [fp4, behind_norm])
 @pytest.mark.parametrize("frozen", [True, False])
 def test_copies_recorded_by_a_capture_are_not_kept(layer, frozen):
     """An eager call and a second capture between a capture and its first replay make their own."""
@@ -58,7 +58,7 @@ def test_copies_recorded_by_a_capture_are_not_kept(layer, frozen):
     _lib.check_status("capture")
 
 
-@pytest.mark.parametrize("layer", [fp4])
+@pytest.mark.parametrize("layer", [fp4, behind_norm])
 def test_a_graph_does_not_read_copies_made_outside_it(layer):
     """They may be gone when it is replayed, and a replay follows the weight as it does with any tensor."""
     x, w = operands(128)
@@ -71,3 +71,20 @@ def test_a_graph_does_not_read_copies_made_outside_it(layer):
     g.replay()
     assert torch.equal(y, -want)
     del junk
+
+
+def test_copies_of_the_linear_behind_a_norm_made_on_one_stream_and_used_on_others():
+    torch.manual_seed(0)
+    x, w = torch.randn(128, 4096, device="cuda").bfloat16(), torch.randn(16384, 4096, device="cuda").bfloat16()
+    want = behind_norm(x, w.clone())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(5):
+        w = w.clone()
+        torch.cuda.synchronize()
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(behind_norm(x, w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got)

@@ -19,7 +19,7 @@ def operands():
     return torch.randn(128, 128), torch.nn.Parameter(torch.randn(256, 128))
 
 
-@pytest.mark.parametrize("layer", [fp4])
+@pytest.mark.parametrize("layer", [fp4, behind_norm])
 def test_copies_follow_other_storage(layer):
     """New storage under the same tensor (``.data``, ``Module.to`` and its relatives), another layout of the same storage."""
     x, w = operands()
@@ -37,7 +37,7 @@ def test_copies_follow_other_storage(layer):
     assert torch.equal(layer(x, v), layer(x, v.detach().clone()))
 
 
-@pytest.mark.parametrize("layer", [fp4])
+@pytest.mark.parametrize("layer", [fp4, behind_norm])
 def test_an_address_that_comes_back_is_another_storage(layer):
     x, w = operands()
     y = layer(x, w).detach()
@@ -47,3 +47,35 @@ def test_an_address_that_comes_back_is_another_storage(layer):
     held *= -1
     w.data = torch.from_numpy(held)
     assert torch.equal(layer(x, w), -y)
+
+
+@pytest.mark.parametrize("layer", [fp4, behind_norm])
+def test_copies_follow_updates_in_place(layer):
+    x, w = operands()
+    y = layer(x, w).detach()
+    for t in (w, torch.nn.Parameter(w.detach().clone(), requires_grad=False), w.detach().clone()):
+        assert torch.equal(layer(x, t), y)
+        with torch.no_grad():
+            t.mul_(-1)
+        assert torch.equal(layer(x, t), -y)
+    w = torch.nn.Parameter(w.detach().clone())
+    opt = torch.optim.SGD([w], lr=2.0)
+    layer(x, w)
+    w.grad = w.detach().clone()                  # a step of 2 w: the weight changes its sign
+    opt.step()
+    assert torch.equal(layer(x, w), y)           # (w was -w0)
+    with torch.inference_mode():
+        v = w.detach().clone()
+        assert torch.equal(layer(x, v), y)
+        v.mul_(-1)
+        assert torch.equal(layer(x, v), -y)
+
+
+def test_gradients_read_the_copies_of_the_updated_weight():
+    x, w = operands()
+    x.requires_grad_()
+    dy = torch.randn(128, 256)
+    (dx,) = torch.autograd.grad(behind_norm(x, w), x, dy)
+    with torch.no_grad():
+        w.mul_(-1)
+    assert torch.equal(torch.autograd.grad(behind_norm(x, w), x, dy)[0], -dx)
