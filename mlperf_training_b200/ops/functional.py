@@ -215,11 +215,39 @@ class NormLinearFn(Function):
 def norm_linear(x, norm_w, weight, *, norm_b=None, bias=None, eps=1e-5, layer_norm=False, precision="bf16", pass_x=False):
     """``pass_x``: returns ``(y, x)``; the gradient of the second output (x taken past the norm by a residual connection) is added
     where the norm's backward writes dx, not by a pass of its own (46000 x 512: 52 us, norm and addition 71).  ``precision="fp4"``: the linear
-    behind an RMS norm reads the norm's own 8-bit output (``add_norm_linear``) where its sizes allow; elsewhere its operands have 4 bits."""
+    behind an RMS norm without biases reads the norm's own 8-bit output (``add_norm_linear``) where its widths allow; elsewhere its operands
+    have 4 bits."""
     if precision == "fp4" and not layer_norm and norm_b is None and bias is None and add_norm_linear_eligible(x, weight):
         y, h = add_norm_linear(x, None, norm_w, weight, eps)
         return (y, h) if pass_x else y
     return _apply(NormLinearFn, x, norm_w, norm_b, weight, bias, eps, layer_norm, precision, torch.is_grad_enabled(), pass_x)
+
+
+def _norm_operand_linear(x, residual, norm_w, weight, eps, grad, need_dw):
+    """``y = Q(norm(h)) Q(W)^T`` of ``h = x + residual`` with MXFP8 operands that come straight from the norm: ``(y, h, rstd, col)``, ``col``
+    the transposed operand that the weight gradient reads (with ``need_dw``; its tokens filled up with zeros to a multiple of 128)."""
+    from . import mxfp8 as MX
+    from .norm_mx import rms_norm_quantize
+    w_row, _ = L.weight_operands(weight, need_col=grad)
+    row, col, h, rstd = rms_norm_quantize(x, norm_w, eps, residual=residual, row_tile=MX.A_TILE,
+                                          col_tile=MX.b_tile(x.shape[1]) if need_dw else None)
+    y = MX.gemm(row, w_row, out_dtype=x.dtype) if x.shape[0] else x.new_empty((0, weight.shape[0]))
+    return y, h, rstd, col
+
+
+def _norm_operand_linear_grad(dy, weight, ref, col):
+    """``(dn, dw)``: gradients of the norm's result and (with ``col``) of the weight, ``ref`` the parameter it is the value of."""
+    from . import mxfp8 as MX
+    from . import mxfp4 as M4
+    T = dy.shape[0]
+    if T == 0:
+        zero = col is not None and ref.requires_grad and getattr(ref, "main_grad", None) is None
+        return dy.new_empty((0, weight.shape[1])), torch.zeros_like(weight) if zero else None
+    # (the quantiser takes 128 rows at a time; rows of zeros add nothing to the weight gradient)
+    dy_row, dy_col = MX.quantize(M4.fill_rows(dy.contiguous(), 128), row_tile=MX.A_TILE, col_tile=MX.A_TILE if col is not None else None)
+    _, w_col = L.weight_operands(weight, need_col=True)
+    dn = MX.gemm(dy_row, w_col, out_dtype=dy.dtype)[:T]
+    return dn, _mx_wgrad(ref, dy_col, col) if col is not None else None
 
 
 class AddNormLinearFn(Function):
@@ -229,14 +257,8 @@ class AddNormLinearFn(Function):
 
     @staticmethod
     def forward(ctx, x, residual, norm_w, weight, eps, grad=True):
-        from . import mxfp8 as MX
-        from .norm_mx import rms_norm_quantize
         grad = grad and any(ctx.needs_input_grad)
-        w_row, _ = L.weight_operands(weight, need_col=grad)
-        need_dw = grad and weight.requires_grad
-        row, col, h, rstd = rms_norm_quantize(x, norm_w, eps, residual=residual, row_tile=MX.A_TILE,
-                                              col_tile=MX.b_tile(x.shape[1]) if need_dw else None)
-        y = MX.gemm(row, w_row, out_dtype=x.dtype)
+        y, h, rstd, col = _norm_operand_linear(x, residual, norm_w, weight, eps, grad, grad and weight.requires_grad)
         tensors, ctx.meta = L.Saved.pack(col) if col is not None else ([], None)
         ctx.save_for_backward(h, norm_w, weight, rstd, *tensors)
         ctx.refs = (norm_w, weight)
@@ -246,31 +268,29 @@ class AddNormLinearFn(Function):
 
     @staticmethod
     def backward(ctx, dy, dh):
-        from . import mxfp8 as MX
         if dy is None:
             return dh, dh if ctx.has_res else None, None, None, None, None
         h, norm_w, weight, rstd, *tensors = ctx.saved_tensors
-        need_dw = ctx.meta is not None
-        dy_row, dy_col = MX.quantize(dy.contiguous(), row_tile=MX.A_TILE, col_tile=MX.A_TILE if need_dw else None)
-        _, w_col = L.weight_operands(weight, need_col=True)
-        dn = MX.gemm(dy_row, w_col, out_dtype=dy.dtype)
-        dw = _mx_wgrad(ctx.refs[1], dy_col, L.Saved.unpack(tensors, ctx.meta)) if need_dw else None
+        dn, dw = _norm_operand_linear_grad(dy, weight, ctx.refs[1], L.Saved.unpack(tensors, ctx.meta) if ctx.meta is not None else None)
+        if dy.shape[0] == 0:
+            return torch.zeros_like(h), torch.zeros_like(h) if ctx.has_res else None, _vec_grad(ctx.refs[0], torch.zeros_like(norm_w)), dw, None, None
         dx, dnw, _ = K.norm_bwd(dn, h, norm_w, None, None, rstd, dres=None if dh is None else dh.to(h.dtype))
         return dx, dx if ctx.has_res else None, _vec_grad(ctx.refs[0], dnw), dw, None, None
 
 
 def add_norm_linear_eligible(x, weight) -> bool:
+    """By the widths alone: a weight is multiplied in the same format whatever the number of tokens is."""
     from .norm_mx import MAX_WIDTH
-    return L.mx_eligible(x.shape[0], weight.shape[0], weight.shape[1]) and x.shape[1] <= MAX_WIDTH
+    return weight.shape[0] % 128 == 0 and weight.shape[1] % 128 == 0 and 0 < weight.shape[1] <= MAX_WIDTH and weight.shape[0] > 0
 
 
 def add_norm_linear(x, residual, norm_w, weight, eps=1e-5):
-    """``(y, h)``: ``h = x + residual`` (``x`` where that is None), ``y = rms_norm(h) W^T`` with MXFP8 operands from the norm itself.  Tokens,
-    input and output features are multiples of 128 (as every MXFP8 linear in training), at most 8192 input features."""
+    """``(y, h)``: ``h = x + residual`` (``x`` where that is None), ``y = rms_norm(h) W^T`` with MXFP8 operands from the norm itself.  Any
+    number of tokens; input and output features are multiples of 128, at most 8192 input features."""
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"add_norm_linear: input {tuple(x.shape)} for a weight {tuple(weight.shape)}")
     if not add_norm_linear_eligible(x, weight):
-        raise ValueError(f"add_norm_linear: {tuple(x.shape)} x {tuple(weight.shape)}: sizes must be multiples of 128, at most 8192 input features")
+        raise ValueError(f"add_norm_linear: {tuple(x.shape)} x {tuple(weight.shape)}: widths must be multiples of 128, at most 8192 input features")
     return _apply(AddNormLinearFn, x, residual, norm_w, weight, eps, torch.is_grad_enabled())
 
 

@@ -1,0 +1,72 @@
+"""The fp4 recipe multiplies a weight in one format, whatever the number of tokens is."""
+import pytest
+import torch
+
+from mlperf_training_b200.ops import functional as F
+
+
+def devices():
+    return ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def operands(dev, T, D=256, N=384):
+    torch.manual_seed(T)
+    dtype = torch.bfloat16 if dev == "cuda" else torch.float32
+    x, nw, w = torch.randn(T, D), 1 + 0.1 * torch.randn(D), torch.randn(N, D) * D ** -0.5
+    return x.to(dev, dtype), nw.to(dev, dtype), w.to(dev, dtype)
+
+
+@pytest.mark.parametrize("dev", devices())
+@pytest.mark.parametrize("T", [1, 127, 129, 255, 300])
+def test_rows_do_not_depend_on_how_many_there_are(dev, T):
+    """The same operands: fp32 sums in another order, and at most a step of the result's type (2^-7) where that changes its rounding."""
+    x, nw, w = operands(dev, 384)
+    full = F.norm_linear(x, nw, w, precision="fp4").float()
+    part, h = F.norm_linear(x[:T], nw, w, precision="fp4", pass_x=True)
+    assert getattr(w, "_mx4_cache", None) is None and torch.equal(h, x[:T])
+    assert float((part.float() - full[:T]).norm()) <= 2 ** -7 * float(full[:T].norm())
+    alone, _ = F.add_norm_linear(x[:T], None, nw, w)
+    assert torch.equal(alone, part)
+
+
+@pytest.mark.parametrize("dev", devices())
+@pytest.mark.parametrize("T", [1, 100, 128, 131, 257])
+def test_gradients_of_any_number_of_tokens(dev, T):
+    """As for whole tiles of tokens: two operands of 8 bits in each product, 2^-5 of a value each at worst, a quarter of that in the mean."""
+    x, nw, w = operands(dev, T)
+    r = torch.randn_like(x)
+    t = [v.requires_grad_() for v in (x, r, nw, w)]
+    y, h = F.add_norm_linear(*t)
+    dy, dh = torch.randn_like(y), torch.randn_like(h)
+    dx, dr, dnw, dw = torch.autograd.grad([y, h], t, [dy, dh])
+    assert torch.equal(dx, dr) and dx.shape == x.shape and dw.shape == w.shape
+    hd, nd, wd = (v.detach().double().requires_grad_() for v in (h, nw.bfloat16(), w))
+    yd = (hd * (hd.square().mean(1, keepdim=True) + 1e-5).rsqrt() * nd) @ wd.t()
+    ref = torch.autograd.grad([yd, hd * 1.0], [hd, nd, wd], [dy.double(), dh.double()])
+    for got, want in ((y, yd), (dx, ref[0]), (dnw, ref[1]), (dw, ref[2])):
+        assert float((got.detach().double() - want.detach()).norm() / want.detach().norm()) < 2 ** -4
+
+
+@pytest.mark.parametrize("dev", devices())
+def test_no_tokens(dev):
+    x, nw, w = (v.requires_grad_() for v in operands(dev, 1))
+    e = x[:0].detach().requires_grad_()
+    y, h = F.add_norm_linear(e, None, nw, w)
+    assert y.shape == (0, 384) and h.shape == (0, 256)
+    dx, dnw, dw = torch.autograd.grad(y.sum() + h.sum(), [e, nw, w])
+    assert dx.shape == (0, 256) and not dnw.any() and not dw.any()
+    assert F.norm_linear(e, nw, w, precision="fp4").shape == (0, 384)
+
+
+@pytest.mark.parametrize("dev", devices())
+def test_a_ragged_evaluation_leaves_no_4_bit_copies_behind_a_norm(dev):
+    from mlperf_training_b200.models.gpt import GPT, GPTConfig
+    m = GPT(GPTConfig(n_layers=2, hidden=128, n_heads=2, n_kv_heads=2, head_dim=64, ffn_hidden=128, vocab_size=256, seq_len=128,
+                      dtype="bf16" if dev == "cuda" else "fp32", precision="fp4"), device=dev)
+    t = torch.randint(0, 256, (1, 101), generator=torch.Generator().manual_seed(0)).to(dev)
+    with torch.no_grad():
+        loss = m(t[:, :-1], t[:, 1:])
+    assert bool(loss.isfinite())
+    for b in m.blocks:
+        assert getattr(b.w_qkv, "_mx4_cache", None) is None and getattr(b.mlp.w_gate_up, "_mx4_cache", None) is None
+        assert b.w_qkv._mx_cache is not None and b.w_proj._mx4_cache is not None
