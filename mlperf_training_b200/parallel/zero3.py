@@ -22,7 +22,7 @@ Schedule (hooks called by the model around every block):
 * ``post_backward(i)`` reduce-scatters the gradient window into ``grad_buf`` (+=) on the
   communication stream and clears the window.
 
-With MXFP8 linears the quantised weight copies are cached on the parameters until the optimizer
+With micro-scaled linears the quantised weight copies are cached on the parameters until the optimizer
 step, so after the first micro-batch of a step a block's gather is skipped whenever every matrix
 of the block still has its cached copies (the gathered bf16 values would not be read).
 
@@ -180,7 +180,8 @@ class Zero3Engine(ZeroEngine):
     def _cached(self, b, need_col: bool) -> bool:
         if not self.skip_cached:
             return False
-        return all(L.copies_kept(p, "_mx_cache", need_col) for _, p in b.params)
+        # (a recipe multiplies a matrix in one format: 8-bit and 4-bit copies of one weight are not both valid and needed)
+        return all(L.copies_kept(p, "_mx_cache", need_col) or L.copies_kept(p, "_mx4_cache", need_col) for _, p in b.params)
 
     def _ensure(self, idx: int, need_col: bool, prefetch: bool) -> None:
         b = self._by_block3.get(idx)

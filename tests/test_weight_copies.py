@@ -79,3 +79,29 @@ def test_gradients_read_the_copies_of_the_updated_weight():
     with torch.no_grad():
         w.mul_(-1)
     assert torch.equal(torch.autograd.grad(behind_norm(x, w), x, dy)[0], -dx)
+
+
+def test_sharded_parameter_engine_knows_both_kinds_of_copies():
+    """A block whose matrices have their copies, 8-bit or 4-bit, is not gathered again; copies of an older weight do not count."""
+    from types import SimpleNamespace
+    from mlperf_training_b200.parallel.zero3 import Zero3Engine
+    x, w8 = operands()
+    w4 = torch.nn.Parameter(torch.randn(256, 128))
+    block = SimpleNamespace(params=[("w_qkv", w8), ("w_proj", w4)])
+    cached = lambda need_col: Zero3Engine._cached(SimpleNamespace(skip_cached=True), block, need_col)
+    assert not cached(False)
+    with torch.no_grad():
+        behind_norm(x, w8)
+        fp4(x, w4)
+    assert cached(False) and not cached(True)
+    x.requires_grad_()
+    behind_norm(x, w8)
+    fp4(x, w4)
+    assert cached(True)
+    with torch.no_grad():
+        w4.mul_(2)
+    assert not cached(False)
+    fp4(x, w4)
+    assert cached(True)
+    L.bump_weight_epoch()
+    assert not cached(False)
