@@ -664,21 +664,26 @@ def expand_rows(src, seq, offsets):
 class LMHeadLossFn(Function):
     """loss = mean CE(norm(x) W^T, labels): final norm, vocabulary GEMM and fused cross-entropy.
     The logits buffer is overwritten with its own gradient during forward, so backward starts
-    from dlogits without recomputing the softmax."""
+    from dlogits without recomputing the softmax.  ``precision="fp4"``: a linear behind a norm like every other
+    (``norm_linear``)."""
 
     @staticmethod
     def forward(ctx, x, norm_w, weight, labels, eps, loss_mask_count, precision, grad=True):
-        xn, _, _, rstd = K.norm_fwd(x, norm_w, None, eps)
         grad = grad and any(ctx.needs_input_grad)
-        keep = grad and L.low_precision(precision, x.shape[0], weight.shape[0], weight.shape[1])
-        logits, saved = L.forward(xn, weight, precision, need_wgrad=keep and weight.requires_grad, need_dgrad=grad)
-        del xn
+        ctx.norm_operand = precision == "fp4" and x.shape[0] > 0 and add_norm_linear_eligible(x, weight)
+        if ctx.norm_operand:
+            logits, x, rstd, saved = _norm_operand_linear(x, None, norm_w, weight, eps, grad, grad and weight.requires_grad)
+        else:
+            xn, _, _, rstd = K.norm_fwd(x, norm_w, None, eps)
+            keep = grad and L.low_precision(precision, x.shape[0], weight.shape[0], weight.shape[1])
+            logits, saved = L.forward(xn, weight, precision, need_wgrad=keep and weight.requires_grad, need_dgrad=grad)
+            del xn
         n_valid = loss_mask_count if loss_mask_count is not None else max(int(labels.numel()), 1)
         losses = K.cross_entropy_(logits, labels.view(-1), 1.0 / n_valid, write_grad=True)
         tensors, ctx.meta = L.Saved.pack(saved) if saved is not None else ([], None)
         ctx.save_for_backward(x, norm_w, weight, rstd, logits, *tensors)
         ctx.cfg = (eps, precision)
-        ctx.refs = (norm_w,)
+        ctx.refs = (norm_w, weight)
         return losses.sum() / n_valid
 
     @staticmethod
@@ -690,14 +695,14 @@ class LMHeadLossFn(Function):
         scale = dloss.reshape(())
         # upstream gradient other than 1 (loss scaling, grad accumulation weights) is applied to dlogits
         dl = dlogits if _is_one(scale) else (dlogits.float() * scale).to(dlogits.dtype)
-        if ctx.meta is not None:
-            saved = L.Saved.unpack(tensors, ctx.meta)
-        elif weight.requires_grad:
-            saved = K.norm_fwd(x, norm_w, None, eps)[0]
+        saved = L.Saved.unpack(tensors, ctx.meta) if ctx.meta is not None else None
+        if ctx.norm_operand:
+            dxn, dw = _norm_operand_linear_grad(dl, weight, ctx.refs[1], saved)
         else:
-            saved = None
-        dxn, dw = L.backward(dl, saved, weight, precision, need_dx=True,
-                             need_dw=weight.requires_grad and saved is not None)
+            if saved is None and weight.requires_grad:
+                saved = K.norm_fwd(x, norm_w, None, eps)[0]
+            dxn, dw = L.backward(dl, saved, weight, precision, need_dx=True,
+                                 need_dw=weight.requires_grad and saved is not None)
         del saved
         dx, dnw, _ = K.norm_bwd(dxn, x, norm_w, None, None, rstd)
         return dx, _vec_grad(ctx.refs[0], dnw), dw, None, None, None, None, None

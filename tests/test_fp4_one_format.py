@@ -70,3 +70,35 @@ def test_a_ragged_evaluation_leaves_no_4_bit_copies_behind_a_norm(dev):
     for b in m.blocks:
         assert getattr(b.w_qkv, "_mx4_cache", None) is None and getattr(b.mlp.w_gate_up, "_mx4_cache", None) is None
         assert b.w_qkv._mx_cache is not None and b.w_proj._mx4_cache is not None
+
+
+@pytest.mark.parametrize("dev", devices())
+@pytest.mark.parametrize("T", [1, 100, 256])
+def test_vocabulary_projection_is_a_linear_behind_a_norm(dev, T):
+    """Loss and gradients of the last norm and projection against 64 bits; the weight has 8-bit copies and no others.  (A logit is a sum
+    of products off by 2^-4 at worst; the softmax hands that on, so the gradients get twice the bound of a product.)"""
+    x, nw, w = operands(dev, T)
+    labels = torch.randint(0, w.shape[0], (T,), generator=torch.Generator().manual_seed(T)).to(dev)
+    t = [v.requires_grad_() for v in (x, nw, w)]
+    loss = F.lm_head_loss(*t, labels, precision="fp4")
+    got = torch.autograd.grad(loss, t)
+    assert getattr(w, "_mx4_cache", None) is None and getattr(w, "_mx_cache", None) is not None
+    td = [v.detach().double().requires_grad_() for v in (x, nw.bfloat16(), w)]
+    yd = (td[0] * (td[0].square().mean(1, keepdim=True) + 1e-5).rsqrt() * td[1]) @ td[2].t()
+    ref = torch.nn.functional.cross_entropy(yd, labels)
+    assert abs(float(loss.detach()) - float(ref.detach())) < 2 ** -4
+    for a, b in zip(got, torch.autograd.grad(ref, td)):
+        assert float((a.double() - b).norm() / b.norm()) < 2 ** -3
+
+
+@pytest.mark.parametrize("dev", devices())
+def test_a_model_step_leaves_8_bit_copies_behind_every_norm(dev):
+    from mlperf_training_b200.models.gpt import GPT, GPTConfig
+    m = GPT(GPTConfig(n_layers=2, hidden=128, n_heads=2, n_kv_heads=2, head_dim=64, ffn_hidden=128, vocab_size=256, seq_len=128,
+                      dtype="bf16" if dev == "cuda" else "fp32", precision="fp4"), device=dev)
+    t = torch.randint(0, 256, (1, 129), generator=torch.Generator().manual_seed(0)).to(dev)
+    m(t[:, :-1], t[:, 1:]).backward()
+    for w in [m.lm_head] + [w for b in m.blocks for w in (b.w_qkv, b.mlp.w_gate_up)]:
+        assert w._mx_cache is not None and getattr(w, "_mx4_cache", None) is None and bool(w.grad.isfinite().all())
+    for w in [w for b in m.blocks for w in (b.w_proj, b.mlp.w_down)]:
+        assert w._mx4_cache is not None and getattr(w, "_mx_cache", None) is None
