@@ -45,7 +45,7 @@ from dataclasses import dataclass, field
 
 import torch
 
-from .linear import bump_weight_epoch
+from .linear import bump_weight_epoch, weight_epoch, weight_format
 
 # reference recipe names -> precision implemented here
 FORMAT_MAP = {
@@ -74,7 +74,6 @@ class DeoscConfig:
     def status(self, precision: str) -> str:
         if not self.enabled:
             return "deosc: off"
-        from .linear import weight_format
         fmt = weight_format(precision)
         if fmt != "e2m1":
             return (f"deosc: requested (start {self.start_step}, period {self.period}, ratio {self.ratio}) - idle: "
@@ -93,6 +92,15 @@ class Deoscillator:
         self.snapped = 0                     # weights snapped so far (this rank's shards)
         self.history: list = []              # (step, snapped at that period end)
         self._grid = None
+        self._since = weight_epoch()         # weights multiplied since: those of the step that is looked at
+
+    def _seen(self, p, precision: str) -> bool:
+        """Whether a linear has quantised ``p`` to the format that is tracked.  In the fp4 recipe some matrices have 8 bits, so it goes by the
+        copies that the last step made: older ones may come from something else."""
+        if p.dim() == 2 and precision == "fp4":
+            c = getattr(p, "_mx4_cache", None)
+            return c is not None and c[0][0] >= self._since
+        return getattr(p, "_mx_cache" if p.dim() == 2 else "_mx_stack", None) is not None
 
     def _keys(self, b, precision: str = "mxfp4"):
         """Per element of this rank's shard of bucket ``b``: (tracked?, scale-and-code key, code, grid value)."""
@@ -109,9 +117,7 @@ class Deoscillator:
         v_max = MX.ELEMENT_FORMATS[self.fmt][2]
         for (name, p), o in zip(b.params, b.offsets):
             # only matrices that a micro-scaled linear, or stacks of them that the grouped expert MLP, has quantised
-            # (in the fp4 recipe, those that it multiplies in 4 bits)
-            seen = getattr(p, "_mx4_cache" if precision == "fp4" else "_mx_cache", None) is not None if p.dim() == 2 else getattr(p, "_mx_stack", None) is not None
-            if p.dim() not in (2, 3) or p.shape[-1] % 32 or not seen:
+            if p.dim() not in (2, 3) or p.shape[-1] % 32 or not self._seen(p, precision):
                 continue
             lo, hi = max(o, b.lo), min(o + p.numel(), b.hi)
             if lo >= hi:
@@ -146,7 +152,11 @@ class Deoscillator:
 
     def after_step(self, step: int, precision: str) -> int:
         """Returns the number of weights snapped at this step (non-zero only at a period end)."""
-        from .linear import weight_format
+        n_snapped = self._after_step(step, precision)
+        self._since = weight_epoch()
+        return n_snapped
+
+    def _after_step(self, step: int, precision: str) -> int:
         cfg = self.cfg
         if not cfg.enabled or step < cfg.start_step or weight_format(precision) != self.fmt:
             return 0

@@ -102,3 +102,24 @@ def test_a_model_step_leaves_8_bit_copies_behind_every_norm(dev):
         assert w._mx_cache is not None and getattr(w, "_mx4_cache", None) is None and bool(w.grad.isfinite().all())
     for w in [w for b in m.blocks for w in (b.w_proj, b.mlp.w_down)]:
         assert w._mx4_cache is not None and getattr(w, "_mx_cache", None) is None
+
+
+def test_deoscillation_goes_by_the_copies_of_the_last_step():
+    """4-bit copies that something made of a weight before the last step (an evaluation, an earlier recipe) do not put it on the grid."""
+    from mlperf_training_b200.ops import linear as L
+    from mlperf_training_b200.ops.recipe import DeoscConfig, Deoscillator
+    from mlperf_training_b200.parallel.engine import OptimConfig, ZeroEngine
+    torch.manual_seed(0)
+    w4, w8 = torch.nn.Parameter(torch.randn(32, 64)), torch.nn.Parameter(torch.randn(32, 64))
+    engine = ZeroEngine(torch.nn.ParameterList([w4, w8]), OptimConfig())
+    d = Deoscillator(engine, DeoscConfig(enabled=True, start_step=0, period=100, ratio=2.0))
+    tracked = lambda: {p.data_ptr(): bool(d._keys(b, "fp4")[0][o - b.lo]) for b in engine.buckets for (_, p), o in zip(b.params, b.offsets)}
+    x = torch.randn(1, 64)
+    with torch.no_grad():
+        F.mxfp4_linear(x, w8)
+        for step in range(3):
+            F.mxfp4_linear(x, w4)                # the forward of a step
+            L.bump_weight_epoch()                # and its update
+            t = tracked()
+            d.after_step(step, "fp4")
+    assert t[w4.data_ptr()] and not t[w8.data_ptr()]
