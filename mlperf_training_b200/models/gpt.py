@@ -60,8 +60,9 @@ class GPTConfig:
     recompute_layers: int = 0
     swiglu_store: str = "bf16"          # "fp8": the fused MXFP8 MLP keeps its gate | up activation for backward as e4m3 codes
     dtype: str = "bf16"
-    # GEMM precision of the linears: "bf16" | "mxfp8" | ... | "fp4" (linears behind a norm read its 8-bit output, the others multiply 4-bit
-    # operands; dense MLPs of layers kept in bf16 run as one gated block)
+    # GEMM precision of the linears: "bf16" | "mxfp8" | ... | "fp4" (linears behind an RMS norm, the vocabulary projection among them, read its
+    # 8-bit output where both widths are multiples of 128, the others multiply 4-bit operands; experts stay in bf16; dense MLPs of layers kept
+    # in bf16 run as one gated block)
     precision: str = "bf16"
     # the first / last N transformer layers keep bf16 linears whatever ``precision`` says (Megatron's
     # first_last_layers_bf16 with num_layers_at_start_in_bf16 / num_layers_at_end_in_bf16, an option of the

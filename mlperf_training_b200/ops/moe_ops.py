@@ -13,6 +13,9 @@ capacity / token dropping (small_llm_moe_pretraining/primus/conf/gpt_oss_20B-MXF
 """
 from __future__ import annotations
 
+import functools
+import warnings
+
 import torch
 from torch.autograd import Function
 
@@ -510,10 +513,18 @@ def _wgrad_into(param, dy, x, seg, E, pad=PAD, counts=None):
     return grouped_wgrad(dy, x, seg, E, out_dtype=param.dtype, pad=pad, counts=counts)
 
 
+@functools.lru_cache(maxsize=None)
+def _say_experts_in_bf16() -> None:
+    warnings.warn("precision 'fp4': the experts' products stay in bf16 (the grouped kernels have no packed 4-bit operands; "
+                  "'mxfp4' carries the same values at the 8-bit rate)", stacklevel=3)
+
+
 def expert_precision(precision: str, w1, w2) -> str:
     """Precision the expert GEMMs run at: the micro-scaled recipe asked for when the widths fit the block-scaled
-    grouped tiles, else bf16."""
+    grouped tiles, else bf16.  "fp4" has no grouped form: its experts are bf16, which a warning says once."""
     from .linear import is_mx
+    if precision == "fp4":
+        _say_experts_in_bf16()
     if is_mx(precision) and w1.dtype == torch.bfloat16 and mx_supported(w1, w2):
         return precision
     return "bf16"

@@ -123,3 +123,20 @@ def test_deoscillation_goes_by_the_copies_of_the_last_step():
             t = tracked()
             d.after_step(step, "fp4")
     assert t[w4.data_ptr()] and not t[w8.data_ptr()]
+
+
+def test_experts_stay_in_bf16_and_say_so():
+    """A mixture-of-experts decoder in the recipe: the experts are as the bf16 model has them, the attention's weights are not, and a warning
+    tells the two apart."""
+    from mlperf_training_b200.models.gpt import GPT, GPTConfig
+    from mlperf_training_b200.ops import moe_ops as M
+    cfg = dict(n_layers=1, hidden=128, n_heads=2, n_kv_heads=2, head_dim=64, ffn_hidden=128, vocab_size=256, seq_len=128, n_experts=4, top_k=2)
+    m = GPT(GPTConfig(**cfg, precision="fp4"))
+    moe = m.blocks[0].mlp
+    M._say_experts_in_bf16.cache_clear()
+    with pytest.warns(UserWarning, match="experts.*bf16"):
+        assert M.expert_precision("fp4", moe.w1, moe.w2) == "bf16"
+    t = torch.randint(0, 256, (1, 129), generator=torch.Generator().manual_seed(0))
+    m(t[:, :-1], t[:, 1:]).backward()
+    assert getattr(moe.w1, "_mx_stack", None) is None and getattr(m.blocks[0].w_proj, "_mx4_cache", None) is not None
+    assert bool(moe.w1.grad.isfinite().all())
