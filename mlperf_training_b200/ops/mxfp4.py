@@ -216,12 +216,19 @@ def dequantize(op, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
+def _aligned_result(M: int, N: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """``[M, N]`` with 16-byte aligned rows."""
+    per16 = 16 // dtype.itemsize
+    return torch.empty((M, (N + per16 - 1) // per16 * per16), dtype=dtype, device=device)[:, :N]
+
+
 def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_dtype=torch.bfloat16, accumulate: bool = False,
          bias: torch.Tensor | None = None, residual: torch.Tensor | None = None, alpha: float = 1.0) -> torch.Tensor:
     """``D[M,N] (+)= alpha * values(a) @ values(b)^T (+ bias[N]) (+ residual[M,N])``, bf16 or fp32.
 
     Any M and N.  Without ``out`` the result's rows are 16-byte aligned (for an N that is no multiple of 8 - 4 in fp32 - it is a view of
-    wider rows); an ``out`` with other rows, or of such an N (the kernel's stores end on 16 bytes), is filled through one like that.  An empty contraction gives the bias and the residual alone."""
+    wider rows); an ``out`` with other rows, or of such an N (the kernel's stores end on 16 bytes), is filled through one like that.  An empty
+    contraction gives the bias and the residual alone.  A bias or a residual with more bits than bf16 is added in fp32."""
     if not isinstance(a, MX4Operand) or not isinstance(b, MX4Operand):
         raise TypeError("mxfp4.gemm: both operands must be MXFP4")
     if a.k != b.k:
@@ -250,6 +257,16 @@ def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_d
         raise TypeError("mxfp4.gemm: output must be bf16 or fp32")
     if a.tile_rows != A_TILE or b.tile_rows != b_tile(N):
         raise ValueError(f"mxfp4.gemm: operand scale tiling ({a.tile_rows}, {b.tile_rows}) does not match the kernel tiles ({A_TILE}, {b_tile(N)})")
+    wide = [t for t in (bias, residual) if t is not None and t.dtype != torch.bfloat16]
+    if wide:
+        # (the kernel's epilogue adds bf16; what has more bits is added to the fp32 product here, and the sum rounded once)
+        d = gemm(a, b, out_dtype=torch.float32, bias=bias if bias is not None and bias.dtype == torch.bfloat16 else None,
+                 residual=residual if residual is not None and residual.dtype == torch.bfloat16 else None, alpha=alpha)
+        for t in wide:
+            d = d.add_(t.float())
+        if out is None:
+            return d if out_dtype == torch.float32 else _aligned_result(M, N, out_dtype, d.device).copy_(d)
+        return out.copy_(d.add_(out) if accumulate else d)
     if out is None and _lib.host is not None:
         d = _lib.host.gemm_mxfp4(a.q, a.sf, b.q, b.sf, M, N, Kd, out_dtype == torch.float32, bias, residual, alpha)
         if d is not None:
@@ -260,16 +277,15 @@ def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_d
             out.copy_(out.float().add_(d)) if accumulate else out.copy_(d)
         return out
     if out is None:
-        per16 = 8 if out_dtype == torch.bfloat16 else 4
-        out = torch.empty((M, (N + per16 - 1) // per16 * per16), dtype=out_dtype, device=a.q.device)[:, :N]
+        out = _aligned_result(M, N, out_dtype, a.q.device)
     if M == 0 or N == 0:
         return out
     if bias is not None:
-        bias = bias.to(torch.bfloat16).contiguous()
+        bias = bias.contiguous()
     ldr = 0
     if residual is not None:
-        if residual.dtype != torch.bfloat16 or residual.stride(1) != 1:
-            residual = residual.to(torch.bfloat16).contiguous()
+        if residual.stride(1) != 1:
+            residual = residual.contiguous()
         ldr = residual.stride(0)
     ws = _lib.gemm_workspace("b200_gemm_mxfp4_workspace", M, N, Kd, a.q.device)
     call("b200_gemm_mxfp4", ptr(a.q), ptr(a.sf), ptr(b.q), ptr(b.sf), ptr(out), M, N, Kd, a.q.stride(0), b.q.stride(0), out.stride(0),

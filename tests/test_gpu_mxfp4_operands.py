@@ -1,0 +1,39 @@
+"""MXFP4 product on the GPU: biases and residuals of other types, operands that are not what they say."""
+import pytest
+import torch
+
+from mlperf_training_b200.ops import _lib
+from mlperf_training_b200.ops import functional as F
+from mlperf_training_b200.ops import mxfp4 as M4
+
+pytestmark = pytest.mark.gpu
+
+
+def operands(M, N, K):
+    torch.manual_seed(M + N)
+    q = lambda r, tile: M4.quantize(torch.randn(r, K, device="cuda").bfloat16(), row_tile=tile)[0]
+    return q(M, M4.A_TILE), q(N, M4.b_tile(N))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 256, 128), (7, 100, 64), (300, 520, 160)])
+@pytest.mark.parametrize("which", ["bias", "residual", "both", "bf16 bias"])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+def test_bias_and_residual_keep_their_bits(M, N, K, which, out_dtype):
+    """Products of 4-bit values of one block are exact in fp32; the sums over blocks and the two additions are off by less than one part
+    in 2^20 of the magnitudes involved (rounded operands: one in 2^9), on top of the result's own rounding."""
+    a, b = operands(M, N, K)
+    bias = torch.randn(N, device="cuda") * 100
+    res = torch.randn(M, N, device="cuda") * 100
+    bias = None if which == "residual" else bias.bfloat16() if which == "bf16 bias" else bias
+    res = None if which == "bias" else res
+    got = M4.gemm(a, b, bias=bias, residual=res, out_dtype=out_dtype, alpha=0.5)
+    parts = [0.5 * M4.dequantize(a).double() @ M4.dequantize(b).double().t()] + [t.double().expand(M, N) for t in (bias, res) if t is not None]
+    want, size = sum(parts), 0.5 * M4.dequantize(a).double().abs() @ M4.dequantize(b).double().abs().t() + sum(p.abs() for p in parts[1:])
+    limit = size * 2 ** -20 + (want.abs() * 2 ** -8 if out_dtype == torch.bfloat16 else 0)
+    assert got.dtype == out_dtype and bool(((got.double() - want).abs() <= limit).all())
+    if out_dtype == torch.bfloat16:
+        assert torch.equal(got, M4.gemm(a, b, bias=bias, residual=res, out_dtype=torch.float32, alpha=0.5).bfloat16())
+    out = torch.full((M, N), 3.0, device="cuda", dtype=out_dtype)
+    M4.gemm(a, b, out=out, accumulate=True, bias=bias, residual=res, alpha=0.5)
+    assert bool(((out.double() - 3 - want).abs() <= (size + 3) * 2 ** -20 + ((want + 3).abs() * 2 ** -8 if out_dtype == torch.bfloat16 else 0)).all())
+    _lib.check_status("gemm")
