@@ -233,8 +233,9 @@ def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_d
         raise TypeError("mxfp4.gemm: both operands must be MXFP4")
     if a.k != b.k:
         raise ValueError(f"mxfp4.gemm: contraction mismatch {a.k} vs {b.k}")
-    if a.q.device != b.q.device:
-        raise ValueError(f"mxfp4.gemm: operands on {a.q.device} and {b.q.device}")
+    for t in (b.q, out, bias, residual):
+        if t is not None and t.device != a.q.device:
+            raise ValueError(f"mxfp4.gemm: operands on {a.q.device} and {t.device}")
     M, N, Kd = a.rows, b.rows, a.k
     if out is not None:
         if out.shape != (M, N):

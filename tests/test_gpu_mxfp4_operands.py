@@ -37,3 +37,15 @@ def test_bias_and_residual_keep_their_bits(M, N, K, which, out_dtype):
     M4.gemm(a, b, out=out, accumulate=True, bias=bias, residual=res, alpha=0.5)
     assert bool(((out.double() - 3 - want).abs() <= (size + 3) * 2 ** -20 + ((want + 3).abs() * 2 ** -8 if out_dtype == torch.bfloat16 else 0)).all())
     _lib.check_status("gemm")
+
+
+def test_vectors_of_another_device_are_refused():
+    a, b = operands(7, 256, 64)
+    x, w = torch.randn(7, 64, device="cuda").bfloat16(), torch.randn(256, 64, device="cuda").bfloat16()
+    for t in (dict(bias=torch.zeros(256)), dict(bias=torch.zeros(256).bfloat16()), dict(residual=torch.zeros(7, 256).bfloat16())):
+        with pytest.raises(ValueError):
+            M4.gemm(a, b, **t)
+        with pytest.raises(ValueError):
+            F.mxfp4_linear(x, w, **t)
+    with pytest.raises(ValueError):
+        M4.gemm(a, b, out=torch.zeros(7, 256).bfloat16())
