@@ -382,38 +382,40 @@ PyObject* py_norm_mx(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// gemm_mxfp4(a_q, a_sf, b_q, b_sf, M, N, K, fp32, bias, residual, alpha): [M, N], a new tensor; the scales' tiles have been checked
+// gemm_mxfp4(a_q, a_sf, a_tile, b_q, b_sf, b_tile, M, N, K, fp32, bias, residual, alpha): [M, N], a new tensor; the tiles have been checked to be
+// the kernel's
 PyObject* py_gemm_mxfp4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 11 || g_gemm4 == nullptr || g_gemm4_ws == nullptr) Py_RETURN_NONE;
+  if (nargs != 13 || g_gemm4 == nullptr || g_gemm4_ws == nullptr) Py_RETURN_NONE;
   const at::Tensor* t[4];
   for (int i = 0; i < 4; ++i)
-    if ((t[i] = tensor_of(args[i])) == nullptr || !t[i]->is_cuda() || t[i]->scalar_type() != at::kByte || !t[i]->is_contiguous() ||
+    if ((t[i] = tensor_of(args[i < 2 ? i : i + 1])) == nullptr || !t[i]->is_cuda() || t[i]->scalar_type() != at::kByte || !t[i]->is_contiguous() ||
         t[i]->device() != t[0]->device() || !aligned16(t[i]->data_ptr()))
       Py_RETURN_NONE;
-  long long M, N, K;
-  if (!int_of(args[4], M) || !int_of(args[5], N) || !int_of(args[6], K)) {
+  long long M, N, K, a_tile, b_tile;
+  if (!int_of(args[2], a_tile) || !int_of(args[5], b_tile) || !int_of(args[6], M) || !int_of(args[7], N) || !int_of(args[8], K)) {
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
   }
-  const int f32 = PyObject_IsTrue(args[7]);
+  const int f32 = PyObject_IsTrue(args[9]);
   if (f32 < 0) return nullptr;
-  const double alpha = PyFloat_AsDouble(args[10]);
+  const double alpha = PyFloat_AsDouble(args[12]);
   if (alpha == -1.0 && PyErr_Occurred()) return nullptr;
   const int dev = t[0]->device().index();
   if (c10::cuda::current_device() != dev || M <= 0 || N <= 0 || K <= 0 || K % 32 != 0 || M > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff ||
-      N * (f32 ? 4 : 2) % 16 != 0 || t[0]->numel() != M * (K / 2) || t[2]->numel() != N * (K / 2))
+      N * (f32 ? 4 : 2) % 16 != 0 || a_tile <= 0 || b_tile <= 0 || !tile_ok(a_tile) || !tile_ok(b_tile) ||
+      t[0]->numel() != M * (K / 2) || t[2]->numel() != N * (K / 2) || t[1]->numel() < sf_bytes(M, K, a_tile) || t[3]->numel() < sf_bytes(N, K, b_tile))
     Py_RETURN_NONE;
   const void *bias = nullptr, *res = nullptr;
   long long ldr = 0;
-  if (args[8] != Py_None) {
-    const at::Tensor* b = tensor_of(args[8]);
+  if (args[10] != Py_None) {
+    const at::Tensor* b = tensor_of(args[10]);
     if (b == nullptr || b->device() != t[0]->device() || b->scalar_type() != at::kBFloat16 || b->dim() != 1 || b->size(0) != N || !b->is_contiguous())
       Py_RETURN_NONE;
     bias = b->data_ptr();
   }
-  if (args[9] != Py_None) {
-    const at::Tensor* r = tensor_of(args[9]);
+  if (args[11] != Py_None) {
+    const at::Tensor* r = tensor_of(args[11]);
     if (r == nullptr || r->device() != t[0]->device() || r->scalar_type() != at::kBFloat16 || r->dim() != 2 || r->size(0) != M || r->size(1) != N ||
         r->stride(1) != 1)
       Py_RETURN_NONE;

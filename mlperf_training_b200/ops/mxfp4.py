@@ -192,6 +192,20 @@ def quantize(x: torch.Tensor, *, row_tile: int | None = None, col_tile: int | No
             MX4Operand(q_col, sf_col, C, Rp, col_tile) if col_tile is not None else None)
 
 
+def _check_operand(what: str, op) -> None:
+    """A kernel reads codes and scales by the sizes that an operand names: they have to be there."""
+    per_byte = 2 if isinstance(op, MX4Operand) else 1
+    if (op.rows < 0 or op.k < 0 or op.k % 32 or op.tile_rows <= 0 or op.tile_rows % 16 or op.q.dtype != torch.uint8
+            or op.q.shape != (op.rows, op.k // per_byte) or op.sf.dtype != torch.uint8 or op.sf.device != op.q.device
+            or not op.sf.is_contiguous() or op.sf.numel() < MX.sf_bytes(op.rows, op.k, op.tile_rows)):
+        raise ValueError(f"{what}: codes {tuple(op.q.shape)} {op.q.dtype} and scales {tuple(op.sf.shape)} {op.sf.dtype} on {op.sf.device} are not "
+                         f"those of {op.rows} rows of {op.k} values in tiles of {op.tile_rows} rows on {op.q.device}")
+
+
+def _aligned_codes(q: torch.Tensor) -> torch.Tensor:
+    return q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+
+
 def sf_plain(op) -> torch.Tensor:
     """Scales of an MXFP4 or MXFP8 operand as a plain ``[rows, k / 32]`` uint8 matrix."""
     return op.sf if not op.is_cuda else op.sf[MX.sf_index(op.rows, op.k, op.tile_rows, op.sf.device)]
@@ -209,9 +223,10 @@ def dequantize(op, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         out = _lib.host.dequant_mx(op.q, op.sf, op.rows, op.k, op.tile_rows, four, dtype == torch.float32)
         if out is not None:
             return out
+    _check_operand("mxfp4.dequantize", op)
     out = torch.empty((op.rows, op.k), dtype=dtype, device=op.q.device)
     if out.numel():
-        call("b200_dequant_mx", ptr(op.q.contiguous()), ptr(op.sf), ptr(out), op.rows, op.k, op.tile_rows, int(four), int(dtype == torch.float32),
+        call("b200_dequant_mx", ptr(_aligned_codes(op.q)), ptr(op.sf), ptr(out), op.rows, op.k, op.tile_rows, int(four), int(dtype == torch.float32),
              stream_ptr())
     return out
 
@@ -269,9 +284,11 @@ def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_d
             return d if out_dtype == torch.float32 else _aligned_result(M, N, out_dtype, d.device).copy_(d)
         return out.copy_(d.add_(out) if accumulate else d)
     if out is None and _lib.host is not None:
-        d = _lib.host.gemm_mxfp4(a.q, a.sf, b.q, b.sf, M, N, Kd, out_dtype == torch.float32, bias, residual, alpha)
+        d = _lib.host.gemm_mxfp4(a.q, a.sf, a.tile_rows, b.q, b.sf, b.tile_rows, M, N, Kd, out_dtype == torch.float32, bias, residual, alpha)
         if d is not None:
             return d
+    _check_operand("mxfp4.gemm", a)
+    _check_operand("mxfp4.gemm", b)
     if out is not None and (out.stride(1) != 1 or (N * out.element_size()) % 16 or (out.stride(0) * out.element_size()) % 16 or out.data_ptr() % 16 or out.stride(0) < N):
         if M and N:
             d = gemm(a, b, out_dtype=torch.float32 if accumulate else out_dtype, bias=bias, residual=residual, alpha=alpha)
@@ -289,7 +306,8 @@ def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_d
             residual = residual.contiguous()
         ldr = residual.stride(0)
     ws = _lib.gemm_workspace("b200_gemm_mxfp4_workspace", M, N, Kd, a.q.device)
-    call("b200_gemm_mxfp4", ptr(a.q), ptr(a.sf), ptr(b.q), ptr(b.sf), ptr(out), M, N, Kd, a.q.stride(0), b.q.stride(0), out.stride(0),
+    a_q, b_q = _aligned_codes(a.q), _aligned_codes(b.q)
+    call("b200_gemm_mxfp4", ptr(a_q), ptr(a.sf), ptr(b_q), ptr(b.sf), ptr(out), M, N, Kd, a_q.stride(0), b_q.stride(0), out.stride(0),
          int(out.dtype == torch.float32), int(accumulate), ptr(bias), ptr(residual), ldr, float(alpha), ptr(ws),
          0 if ws is None else ws.numel(), stream_ptr())
     return out

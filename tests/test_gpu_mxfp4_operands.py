@@ -49,3 +49,21 @@ def test_vectors_of_another_device_are_refused():
             F.mxfp4_linear(x, w, **t)
     with pytest.raises(ValueError):
         M4.gemm(a, b, out=torch.zeros(7, 256).bfloat16())
+
+
+def test_operands_that_do_not_hold_what_they_say_are_refused():
+    from dataclasses import replace
+    a, b = operands(7, 256, 64)
+    want = M4.gemm(a, b)
+    for bad in (lambda o: replace(o, rows=o.rows + 1), lambda o: replace(o, k=o.k + 128), lambda o: replace(o, sf=o.sf[:-1]),
+                lambda o: replace(o, sf=o.sf.cpu()), lambda o: replace(o, q=o.q[1:])):
+        for x, y in ((bad(a), b), (a, bad(b))):
+            with pytest.raises(ValueError):
+                M4.gemm(x, y)
+        with pytest.raises(ValueError):
+            M4.dequantize(bad(a))
+    held = torch.zeros(7, 100, dtype=torch.uint8, device="cuda")
+    held[:, 3:35] = a.q
+    assert torch.equal(M4.gemm(replace(a, q=held[:, 3:35]), b), want)
+    assert torch.equal(M4.dequantize(replace(a, q=held[:, 3:35])), M4.dequantize(a))
+    _lib.check_status("refusals")

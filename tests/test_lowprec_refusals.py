@@ -41,3 +41,37 @@ def test_product_refuses_vectors_of_another_device(launched, what):
     with pytest.raises(ValueError):
         M4.gemm(a, b, **{what: t})
     assert launched == []
+
+
+BAD = {
+    "short codes": lambda op: replace(op, q=op.q[:-1]),
+    "wide codes": lambda op: replace(op, q=op.q[:, ::2]),
+    "other codes": lambda op: replace(op, q=op.q.view(torch.int8)),
+    "short scales": lambda op: replace(op, sf=op.sf[:-1]),
+    "strided scales": lambda op: replace(op, sf=torch.zeros(2 * op.sf.numel(), dtype=torch.uint8)[::2]),
+    "other scales": lambda op: replace(op, sf=op.sf.to(torch.int16)),
+    "scales elsewhere": lambda op: replace(op, sf=op.sf.to("meta")),
+    "ragged contraction": lambda op: replace(op, k=op.k - 8),
+    "more rows": lambda op: replace(op, rows=op.rows + 1),
+}
+
+
+@pytest.mark.parametrize("why", sorted(BAD))
+def test_operands_that_do_not_hold_what_they_say(launched, why):
+    a, b = gpu_operand(5, 64, M4.A_TILE), gpu_operand(40, 64, M4.b_tile(40))
+    for x, y in ((BAD[why](a), b), (a, BAD[why](b))):
+        with pytest.raises(ValueError):
+            M4.gemm(x, y)
+    for op in (a, MX.MXOperand(torch.zeros(5, 64, dtype=torch.uint8), a.sf, 5, 64, 128)):
+        with pytest.raises(ValueError):
+            M4.dequantize(BAD[why](op))
+    assert launched == []
+
+
+def test_operands_of_other_layouts_are_copied(launched):
+    """Rows at a larger pitch, and an address that is not a multiple of 16."""
+    a, b = gpu_operand(5, 64, M4.A_TILE), gpu_operand(40, 64, M4.b_tile(40))
+    wide = replace(a, q=torch.zeros(5, 100, dtype=torch.uint8)[:, 3:35])
+    M4.gemm(wide, b)
+    M4.dequantize(wide)
+    assert launched == ["b200_gemm_mxfp4", "b200_dequant_mx"]
