@@ -342,22 +342,22 @@ def _down_few_rows(T: int, D: int, Fh: int) -> bool:
 def gated_down(a: torch.Tensor, w_down: torch.Tensor, residual: torch.Tensor | None = None):
     """``y = a W_down^T (+ residual)`` of the gated block's ``a [T, F]`` and ``w_down [D, F]``.  A few rows read the weight split along F over
     clusters of CTAs; more rows, and operands that are not bf16 on the GPU, are a ``gemm``."""
-    if not use_kernels(a) or a.dtype != BF16 or not _down_few_rows(a.shape[0], w_down.shape[0], a.shape[1]):
-        return gemm(a, w_down, residual=residual)
-    if _lib.host is not None:
+    few = use_kernels(a) and a.dtype == BF16 and a.dim() == 2 and w_down.dim() == 2 and _down_few_rows(a.shape[0], w_down.shape[0], a.shape[1])
+    if few and _lib.host is not None:
         r = _lib.host.gated_down(a, w_down, residual)
         if r is not None:
             return r
+    if a.dim() != 2 or w_down.dim() != 2 or w_down.shape[1] != a.shape[1] or w_down.device != a.device:
+        raise ValueError(f"gated_down: input {tuple(a.shape)} on {a.device}, weight {tuple(w_down.shape)} on {w_down.device}")
     T, Fh = a.shape
     D = w_down.shape[0]
+    if residual is not None and (residual.shape != (T, D) or residual.device != a.device):
+        raise ValueError(f"gated_down: residual {tuple(residual.shape)} on {residual.device} for an output {T}x{D} on {a.device}")
+    if not few:
+        return gemm(a, w_down, residual=residual)
     _gate_check("gated_down", a, w_down, "silu", Fh, D)
-    if w_down.shape[1] != Fh:
-        raise ValueError(f"gated_down: weight {tuple(w_down.shape)} for {Fh} columns")
-    if residual is not None:
-        if residual.shape != (T, D) or residual.device != a.device:
-            raise ValueError(f"gated_down: residual {tuple(residual.shape)} on {residual.device} for an output {T}x{D} on {a.device}")
-        if residual.dtype != BF16 or residual.stride(1) != 1:
-            residual = residual.to(BF16).contiguous()
+    if residual is not None and (residual.dtype != BF16 or residual.stride(1) != 1):
+        residual = residual.to(BF16).contiguous()
     a, w = _row_major(a), _row_major(w_down)
     y = torch.empty((T, D), dtype=BF16, device=a.device)
     call("b200_gated_down", ptr(a), ptr(w), ptr(residual), ptr(y), T, D, Fh, a.stride(0), w.stride(0), 0 if residual is None else residual.stride(0),

@@ -67,3 +67,12 @@ def test_operands_that_do_not_hold_what_they_say_are_refused():
     assert torch.equal(M4.gemm(replace(a, q=held[:, 3:35]), b), want)
     assert torch.equal(M4.dequantize(replace(a, q=held[:, 3:35])), M4.dequantize(a))
     _lib.check_status("refusals")
+
+
+@pytest.mark.parametrize("T", [7, 100])
+def test_gated_block_refuses_a_residual_or_weight_of_another_device(T):
+    x, wgu, wd, r = (torch.randn(*s, device="cuda").bfloat16() for s in ((T, 64), (256, 64), (64, 128), (T, 64)))
+    F.gated_mlp(x, wgu, wd, residual=r)
+    for bad in ((x, wgu, wd, r.cpu()), (x, wgu, wd.cpu(), r), (x, wgu.cpu(), wd, r), (x, wgu, wd, r[1:])):
+        with pytest.raises(ValueError):
+            F.gated_mlp(*bad[:3], residual=bad[3])

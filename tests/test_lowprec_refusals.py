@@ -75,3 +75,15 @@ def test_operands_of_other_layouts_are_copied(launched):
     M4.gemm(wide, b)
     M4.dequantize(wide)
     assert launched == ["b200_gemm_mxfp4", "b200_dequant_mx"]
+
+
+@pytest.mark.parametrize("T", [7, 100])
+@pytest.mark.parametrize("what", ["residual", "weight", "shape"])
+def test_down_projection_refuses_what_it_cannot_read(launched, T, what):
+    """By the few-row kernel and by the general product alike."""
+    a, w, r = (torch.zeros(*s, dtype=torch.bfloat16) for s in ((T, 64), (128, 64), (T, 128)))
+    w = w.to("meta") if what == "weight" else w
+    r = r.to("meta") if what == "residual" else r[:-1] if what == "shape" else r
+    with pytest.raises(ValueError):
+        K.gated_down(a, w, r)
+    assert launched == []
