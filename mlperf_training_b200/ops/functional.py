@@ -228,6 +228,8 @@ def _norm_operand_linear(x, residual, norm_w, weight, eps, grad, need_dw):
     the transposed operand that the weight gradient reads (with ``need_dw``; its tokens filled up with zeros to a multiple of 128)."""
     from . import mxfp8 as MX
     from .norm_mx import rms_norm_quantize
+    if weight.device != x.device:
+        raise ValueError(f"linear behind a norm: input on {x.device}, weight on {weight.device}")
     w_row, _ = L.weight_operands(weight, need_col=grad)
     row, col, h, rstd = rms_norm_quantize(x, norm_w, eps, residual=residual, row_tile=MX.A_TILE,
                                           col_tile=MX.b_tile(x.shape[1]) if need_dw else None)

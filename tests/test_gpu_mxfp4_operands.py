@@ -76,3 +76,12 @@ def test_gated_block_refuses_a_residual_or_weight_of_another_device(T):
     for bad in ((x, wgu, wd, r.cpu()), (x, wgu, wd.cpu(), r), (x, wgu.cpu(), wd, r), (x, wgu, wd, r[1:])):
         with pytest.raises(ValueError):
             F.gated_mlp(*bad[:3], residual=bad[3])
+
+
+def test_linear_behind_a_norm_refuses_operands_of_another_device():
+    x, nw, w = torch.randn(5, 128, device="cuda").bfloat16(), torch.ones(128, device="cuda").bfloat16(), torch.randn(256, 128, device="cuda").bfloat16()
+    for bad in ((x, None, nw, w.cpu()), (x, x.cpu(), nw, w), (x, None, nw.cpu(), w)):
+        with pytest.raises(ValueError):
+            F.add_norm_linear(*bad)
+    with pytest.raises(ValueError):
+        F.lm_head_loss(x, nw, w.cpu(), torch.zeros(5, dtype=torch.long, device="cuda"), precision="fp4")

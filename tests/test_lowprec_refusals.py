@@ -87,3 +87,13 @@ def test_down_projection_refuses_what_it_cannot_read(launched, T, what):
     with pytest.raises(ValueError):
         K.gated_down(a, w, r)
     assert launched == []
+
+
+def test_linear_behind_a_norm_refuses_a_weight_of_another_device(launched):
+    x, nw = torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(128, dtype=torch.bfloat16)
+    for w in (torch.zeros(256, 128, dtype=torch.bfloat16, device="meta"),):
+        with pytest.raises(ValueError):
+            F.add_norm_linear(x, None, nw, w)
+        with pytest.raises(ValueError):
+            F.lm_head_loss(x, nw, w, torch.zeros(4, dtype=torch.long), precision="fp4")
+    assert launched == []
