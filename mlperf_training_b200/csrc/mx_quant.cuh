@@ -141,9 +141,9 @@ B200_DEVICE void hadamard16(float2 (&v)[16]) {
 
 // Sixteen rows of two columns; the other halves of the 32-blocks are in the neighbouring lane.  `m`: the bits of the largest magnitudes of the
 // two (this lane's rows).  noise: word i holds the bytes of rows 4 i .. 4 i + 3 (na: first column, nb: second), null for nearest.  Codes in
-// qa, qb (e4m3: 16 bytes, e2m1: two words), scale bytes in ea, eb.  e4m3: the values are v * w (w: one factor per column).
+// qa, qb (e4m3: 16 bytes, e2m1: two words), scale bytes in ea, eb.
 template <int FMT>
-B200_DEVICE void quant_col16(float2 (&v)[16], float2 w, uint32_t ma, uint32_t mb, const uint32_t* na, const uint32_t* nb, uint4& qa, uint4& qb,
+B200_DEVICE void quant_col16(float2 (&v)[16], uint32_t ma, uint32_t mb, const uint32_t* na, const uint32_t* nb, uint4& qa, uint4& qb,
                              uint32_t& ea, uint32_t& eb) {
   ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
   mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
@@ -151,7 +151,7 @@ B200_DEVICE void quant_col16(float2 (&v)[16], float2 w, uint32_t ma, uint32_t mb
   eb = e8m0<FMT>(mb);
   const float2 inv = make_float2(inv_scale(ea), inv_scale(eb));
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = fmul2(FMT == E4M3 ? fmul2(v[i], w) : v[i], inv);
+  for (int i = 0; i < 16; ++i) v[i] = fmul2(v[i], inv);
   uint32_t a[4], b[4];
   if constexpr (FMT == E4M3) {
 #pragma unroll
@@ -308,7 +308,7 @@ mx_tile_kernel(const TileArgs p) {
     }
     uint4 qa, qb;
     uint32_t ea, eb;
-    quant_col16<E2M1>(v, make_float2(1.f, 1.f), ma, mb, NOISE ? na : nullptr, NOISE ? nb : nullptr, qa, qb, ea, eb);
+    quant_col16<E2M1>(v, ma, mb, NOISE ? na : nullptr, NOISE ? nb : nullptr, qa, qb, ea, eb);
     if (c0 + c < p.C && r0 + sub * 16 < p.Rp) {
       uint8_t* dst = p.q_col + (((long long)(c0 + c) * p.Rp + r0) >> 1) + sub * 8;
       *reinterpret_cast<uint2*>(dst) = make_uint2(qa.x, qa.y);

@@ -1,8 +1,8 @@
 """RMS norm of a residual sum with a micro-scaled output: what a block-scaled linear reads, straight from the norm.
 
-``n = h * rsqrt(mean(h^2) + eps) * weight`` with ``h = x + residual`` leaves as MXFP8 operands (``ops.mxfp8``); ``n`` itself is
-never written, and is not rounded before it is quantised.  The backward of the norm is ``ops.kernels.norm_bwd`` on the ``h`` and
-``rstd`` that are returned here.
+``n = (h * weight) * rsqrt(mean(h^2) + eps)`` with ``h = x + residual`` leaves as MXFP8 operands (``ops.mxfp8``); ``n`` itself is
+never written, and is rounded once, to fp32, before it is quantised (the product of two bf16 is exact there).  The backward of the norm
+is ``ops.kernels.norm_bwd`` on the ``h`` and ``rstd`` that are returned here.
 """
 from __future__ import annotations
 
@@ -56,7 +56,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, 
         h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
         hf = h.detach().float()
         rstd = torch.rsqrt((hf * hf).mean(-1) + eps)
-        n = hf * rstd[:, None] * weight.detach().to(torch.bfloat16).float()
+        n = (hf * weight.detach().to(torch.bfloat16).float()) * rstd[:, None]
         row_op = MX.MXOperand(*_e4m3_rows_cpu(n), T, D, row_tile) if row_tile is not None else None
         col_op = MX.MXOperand(*_e4m3_rows_cpu(M4.fill_rows(n, 128).t().contiguous()), D, Tp, col_tile) if col_tile is not None else None
         return row_op, col_op, h, rstd
