@@ -95,9 +95,15 @@ def mx_eligible(rows: int, n_out: int, n_in: int) -> bool:
 
 
 def _identity(weight: torch.Tensor):
-    """What a change of ``weight`` through torch alters: the version that in-place operations count up, storage, type, layout, device.
+    """What a change of ``weight`` through torch alters: the version that in-place operations count up, storage, address, type, layout.
     (The reference names the storage for good and does not keep its memory; an address may come back with another one.)"""
-    return (weight._version, StorageWeakRef(weight.untyped_storage()), weight.data_ptr(), weight.dtype, weight.shape, weight.stride(), weight.device)
+    return weight._version, StorageWeakRef(weight.untyped_storage()), weight.data_ptr(), weight.dtype, weight.shape, weight.stride()
+
+
+def _is_still(weight: torch.Tensor, identity) -> bool:
+    version, storage, address, dtype, shape, stride = identity
+    return (weight._version == version and weight.untyped_storage()._cdata == storage.cdata and weight.data_ptr() == address
+            and weight.dtype is dtype and weight.shape == shape and weight.stride() == stride)
 
 
 def _epoch(weight: torch.Tensor) -> int:
@@ -107,8 +113,8 @@ def _epoch(weight: torch.Tensor) -> int:
 def _kept_copies(weight: torch.Tensor, slot: str, formats: tuple, need_col: bool, make):
     """(row, col) copies of ``weight [N, K]`` for forward and dgrad, kept on the tensor under ``slot`` until it changes: through torch (in
     place, or with other storage) or through an optimizer step.  What torch does not see - writes through ``weight.data``, or by a kernel -
-    has to be followed by ``bump_weight_epoch()``.  ``make(w, need_row, need_col)``: the copies asked for; ``formats``: what besides the
-    weight they depend on.
+    has to be followed by ``bump_weight_epoch()``.  ``make(w, formats, need_row, need_col)``: the copies asked for;
+    ``formats``: what besides the weight they depend on.
 
     A call on another stream than the one that made them waits for them there.  A call under graph capture makes its own, inside the
     graph: what it records is not made yet when it returns, copies made outside the graph may be gone when it is replayed, and a replay
@@ -118,9 +124,9 @@ def _kept_copies(weight: torch.Tensor, slot: str, formats: tuple, need_col: bool
     keep = not weight.is_inference() and not (weight.is_cuda and torch.cuda.is_current_stream_capturing())
     row = None
     if keep:
-        key, same = (_epoch(weight), *formats), _identity(weight)
+        key = (_epoch(weight), *formats)
         cache = getattr(weight, slot, None)
-        if cache is not None and cache[0] == key and cache[3] == same:
+        if cache is not None and cache[0] == key and _is_still(weight, cache[3]):
             if cache[4] is not None and cache[4] != stream_ptr():
                 _use_here(cache)
             if cache[2] is not None or not need_col:
@@ -129,7 +135,7 @@ def _kept_copies(weight: torch.Tensor, slot: str, formats: tuple, need_col: bool
     w = weight.detach()
     if w.dtype != torch.bfloat16 and w.is_cuda:
         w = w.to(torch.bfloat16)
-    new_row, col = make(w, row is None, need_col)
+    new_row, col = make(w, formats, row is None, need_col)
     row = new_row if row is None else row
     if keep:
         stream = event = None
@@ -138,7 +144,7 @@ def _kept_copies(weight: torch.Tensor, slot: str, formats: tuple, need_col: bool
             i, d, t = torch._C._cuda_getCurrentStream(torch._C._cuda_getDevice())
             stream, event = stream_ptr(), torch.cuda.Event()
             event.record(torch.cuda.Stream(stream_id=i, device_index=d, device_type=t))
-        setattr(weight, slot, (key, row, col, same, stream, event))
+        setattr(weight, slot, (key, row, col, _identity(weight), stream, event))
     return row, col
 
 
@@ -156,20 +162,20 @@ def copies_kept(weight: torch.Tensor, slot: str, need_col: bool) -> bool:
     """Whether the copies under ``slot`` are those of the weight as it is now (in whatever format they were made)."""
     cache = getattr(weight, slot, None)
     return (cache is not None and cache[0][0] == _epoch(weight) and (cache[2] is not None or not need_col)
-            and not weight.is_inference() and cache[3] == _identity(weight))
+            and not weight.is_inference() and _is_still(weight, cache[3]))
+
+
+def _make_mx(w: torch.Tensor, formats: tuple, need_row: bool, need_col: bool):
+    N, Kd = w.shape
+    return MX.quantize(w, row_tile=MX.b_tile(N) if need_row else None, col_tile=MX.b_tile(Kd) if need_col else None, fmt=formats[0],
+                       col_fmt=formats[1])
 
 
 def weight_operands(weight: torch.Tensor, need_col: bool = True, fmt: str = "e4m3", col_fmt: str | None = None):
     """(w_row, w_col) micro-scaled copies of ``weight`` ``[N, K]``: ``w_row`` (rows N, contraction K) is
     the B operand of forward, ``w_col`` (rows K, contraction N) the B operand of dgrad; ``fmt`` / ``col_fmt``: their element
     formats.  Kept on the tensor by the rules of ``_kept_copies``."""
-    N, Kd = weight.shape
-    col_fmt = col_fmt or fmt
-
-    def make(w, need_row, need_col):
-        return MX.quantize(w, row_tile=MX.b_tile(N) if need_row else None, col_tile=MX.b_tile(Kd) if need_col else None, fmt=fmt, col_fmt=col_fmt)
-
-    return _kept_copies(weight, "_mx_cache", (fmt, col_fmt), need_col, make)
+    return _kept_copies(weight, "_mx_cache", (fmt, col_fmt or fmt), need_col, _make_mx)
 
 
 def _site(weight: torch.Tensor, name: str, fmt: str) -> "F8.DelayedScale":
@@ -205,14 +211,14 @@ def fp4_eligible(rows: int, n_out: int, n_in: int) -> bool:
     return rows > 0 and n_out > 0 and n_in > 0 and n_out % 32 == 0 and n_in % 32 == 0
 
 
+def _make_mx4(w: torch.Tensor, formats: tuple, need_row: bool, need_col: bool):
+    N, Kd = w.shape
+    return M4.quantize(w, row_tile=M4.b_tile(N) if need_row else None, col_tile=M4.b_tile(Kd) if need_col else None)
+
+
 def fp4_weight_operands(weight: torch.Tensor, need_col: bool = True):
     """(w_row, w_col) MXFP4 copies of ``weight [N, K]`` for forward and dgrad, kept on the tensor by the rules of ``_kept_copies``."""
-    N, Kd = weight.shape
-
-    def make(w, need_row, need_col):
-        return M4.quantize(w, row_tile=M4.b_tile(N) if need_row else None, col_tile=M4.b_tile(Kd) if need_col else None)
-
-    return _kept_copies(weight, "_mx4_cache", (), need_col, make)
+    return _kept_copies(weight, "_mx4_cache", (), need_col, _make_mx4)
 
 
 def fp4_forward(x: torch.Tensor, weight: torch.Tensor, *, bias=None, residual=None, need_wgrad: bool = True, need_dgrad: bool = False):

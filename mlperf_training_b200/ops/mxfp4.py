@@ -273,13 +273,13 @@ def gemm(a: MX4Operand, b: MX4Operand, *, out: torch.Tensor | None = None, out_d
         raise TypeError("mxfp4.gemm: output must be bf16 or fp32")
     if a.tile_rows != A_TILE or b.tile_rows != b_tile(N):
         raise ValueError(f"mxfp4.gemm: operand scale tiling ({a.tile_rows}, {b.tile_rows}) does not match the kernel tiles ({A_TILE}, {b_tile(N)})")
-    wide = [t for t in (bias, residual) if t is not None and t.dtype != torch.bfloat16]
-    if wide:
+    if (bias is not None and bias.dtype != torch.bfloat16) or (residual is not None and residual.dtype != torch.bfloat16):
         # (the kernel's epilogue adds bf16; what has more bits is added to the fp32 product here, and the sum rounded once)
         d = gemm(a, b, out_dtype=torch.float32, bias=bias if bias is not None and bias.dtype == torch.bfloat16 else None,
                  residual=residual if residual is not None and residual.dtype == torch.bfloat16 else None, alpha=alpha)
-        for t in wide:
-            d = d.add_(t.float())
+        for t in (bias, residual):
+            if t is not None and t.dtype != torch.bfloat16:
+                d = d.add_(t.float())
         if out is None:
             return d if out_dtype == torch.float32 else _aligned_result(M, N, out_dtype, d.device).copy_(d)
         return out.copy_(d.add_(out) if accumulate else d)
