@@ -10,9 +10,8 @@
 // projections are not read again: 4 bytes of T F less each way, and forward without a backward writes 2 bytes instead of 6.
 //
 // Roundings: a once from fp32, gate and up once where they are kept for the backward (at 2 bytes a value: fp32 would double what a block keeps),
-// da not at all.  What the backward makes of the kept projections (d gate, d up) so has two or three roundings of 2^-9 in it: the gradients of
-// x and W of 4096 x 4096 x 14336 are 0.0033 off in norm, 0.0017 of that the rounding of the results themselves.  The gradient of Wd reads the
-// forward's a (functional.py: GatedMLPFn); a made again from gate and up is for callers that keep less.
+// da not at all.  What the backward makes of the kept projections (d gate, d up, a) so has two or three roundings of 2^-9 in it: the gradients of
+// 4096 x 4096 x 14336 are 0.0035 off in norm, 0.0017 of that the rounding of the results themselves.
 // Measured (4096 tokens, 4096 x 2 x 14336, caches cold): forward 615 us (1.56 PFLOP/s), gradient 370 us (1.30 PFLOP/s; the GEMM of that size
 // alone 293): bound by the tensor pipe under the power cap, the gradient by its epilogue (two operands in, three results out) where a tile's
 // mainloop of 64 stages does not cover it.  Up to 64 rows: gated_fewrows.cu.

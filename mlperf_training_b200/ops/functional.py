@@ -299,8 +299,7 @@ def add_norm_linear(x, residual, norm_w, weight, eps=1e-5):
 class GatedMLPFn(Function):
     """``y = (act(x Wg^T) * (x Wu^T)) Wd^T (+ residual)`` in bf16: the projections, the activation and the product in one kernel, the down
     projection in another; backward: the gradient of the activation in the epilogue of the down projection's dgrad.  Kept for
-    backward: ``x``, the projections and, where ``w_down`` wants a gradient, the activation's product ``a``: 6 bytes of T F.  (``a`` could be
-    made again from the projections, but these were rounded to bf16: the gradient of ``w_down`` was 0.0038 off, half of that not its own.)"""
+    backward: ``x`` and the projections (the activation's product is made again where they are read)."""
 
     @staticmethod
     def forward(ctx, x, w_gate_up, w_down, residual, act, grad=True):
@@ -310,24 +309,24 @@ class GatedMLPFn(Function):
             y = K.gated_down(a, w_down, residual)
         else:
             y = x.new_empty((0, w_down.shape[0]))
-        ctx.save_for_backward(x, w_gate_up, w_down, gu, a if grad and ctx.needs_input_grad[2] else None)
+        ctx.save_for_backward(x, w_gate_up, w_down, gu)
         ctx.act, ctx.has_res = act, residual is not None
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, w_gate_up, w_down, gu, a = ctx.saved_tensors
+        x, w_gate_up, w_down, gu = ctx.saved_tensors
         need_x, need_gu, need_down, need_res = (ctx.needs_input_grad[i] for i in range(4))
         dres = dy if ctx.has_res and need_res else None
         if dy.shape[0] == 0:
             zero = lambda t: None if getattr(t, "main_grad", None) is not None else torch.zeros_like(t)
             return x.new_empty(x.shape), zero(w_gate_up), zero(w_down), dres, None, None
         dx = dw_gu = dw_down = None
-        if need_down:
-            dw_down = _wgrad(dy, a, w_down)
-        del a
-        if need_x or need_gu:
-            dgu, _ = K.gated_bwd(dy, w_down, gu, ctx.act, want_a=False)
+        if need_x or need_gu or need_down:
+            dgu, a = K.gated_bwd(dy, w_down, gu, ctx.act, want_a=need_down)
+            if need_down:
+                dw_down = _wgrad(dy, a, w_down)
+            del a
             if need_x:
                 dx = K.gemm(dgu, w_gate_up, b_mn_major=True)
             if need_gu:
