@@ -35,9 +35,10 @@ struct Params {
   int a_rows;                                         // rows of the activations' box
   __nv_bfloat16* a;
   long long lda;
-  __nv_bfloat16* gu;
+  void* gu;
   long long ldgu;
   int act;
+  int gu_f32;
   int* status;
 };
 
@@ -131,7 +132,8 @@ gated_fewrows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
       const int f = t * 128 + q * 32 + lane;
       const bool live = f < p.F;
       __nv_bfloat16* out = p.a + f;
-      __nv_bfloat16* gu = p.gu != nullptr ? p.gu + f : nullptr;
+      __nv_bfloat16* gu = p.gu != nullptr && !p.gu_f32 ? (__nv_bfloat16*)p.gu + f : nullptr;
+      float* gu32 = p.gu != nullptr && p.gu_f32 ? (float*)p.gu + f : nullptr;
       for (int c = 0; c < cols; c += 16) {
         uint32_t g[16], u[16];
         tmem_ld_32x32b_x16(row + c, g);
@@ -143,9 +145,11 @@ gated_fewrows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
             const float gv = __uint_as_float(g[i]), uv = __uint_as_float(u[i]);
             *out = __float2bfloat16_rn(gate_act(gv, p.act) * uv);
             if (gu != nullptr) { gu[0] = __float2bfloat16_rn(gv); gu[p.F] = __float2bfloat16_rn(uv); }
+            if (gu32 != nullptr) { gu32[0] = gv; gu32[p.F] = uv; }
           }
           out += p.lda;
           if (gu != nullptr) gu += p.ldgu;
+          if (gu32 != nullptr) gu32 += p.ldgu;
         }
       }
       tc_fence_before();
@@ -414,7 +418,7 @@ int run_gated(const GatedArgs& a, cudaStream_t stream) {
   CUtensorMap tmW, tmX;
   if ((r = b200::make_tmap_2d(&tmW, b200::DT_BF16, a.w, a.K, 2LL * a.F, a.ldw * 2, 64, 128, b200::SWZ_128))) return r;
   if ((r = b200::make_tmap_2d(&tmX, b200::DT_BF16, a.x, a.K, a.M, a.ldx * 2, 64, a_box_rows(a.M), b200::SWZ_128))) return r;
-  const Params p = {a.M, a.F, a.K, (a.F + 127) / 128, a_box_rows(a.M), a.a, a.lda, a.gu, a.ldgu, a.act, b200::status_ptr()};
+  const Params p = {a.M, a.F, a.K, (a.F + 127) / 128, a_box_rows(a.M), a.a, a.lda, a.gu, a.ldgu, a.act, a.gu_f32, b200::status_ptr()};
   b200::launch(gated_fewrows_kernel, dim3(p.tiles < b200::sm_count() ? p.tiles : b200::sm_count()), NUM_THREADS, SMEM, stream, tmW, tmX, p);
   b200::count_launch();
   return b200::check_launch("gemm_gated(few rows)");

@@ -9,10 +9,11 @@ constexpr int MAX_ROWS = 64;
 
 struct GatedArgs {
   const __nv_bfloat16* x; const __nv_bfloat16* w;     // [M, K], [2F, K]
-  __nv_bfloat16* a; __nv_bfloat16* gu;                // [M, F], [M, 2F] or null
+  __nv_bfloat16* a; void* gu;                         // [M, F], [M, 2F] (bf16 or fp32) or null
   int M, F, K;
   long long ldx, ldw, lda, ldgu;
   int act;
+  int gu_f32;
 };
 int run_gated(const GatedArgs& p, cudaStream_t stream);
 

@@ -499,8 +499,9 @@ struct GateArgs {
   int F;                          // GATE 1: rows of the gate half of the stacked weight
   int want_gu;                    // GATE 1: gate and up go to memory too
   int want_a;                     // GATE 2: the activation's product is written again
-  const __nv_bfloat16* gu;        // GATE 2: [M, 2F], gate columns first
+  const void* gu;                 // GATE 2: [M, 2F], gate columns first
   long long ldgu;
+  int gu_f32;                     // gate and up are fp32 in memory, else bf16
 };
 
 // Rows of A's box for a problem of M rows.  Rows past M are filled with zeros on their way into shared memory at the price of real ones, and a
@@ -594,13 +595,20 @@ B200_DEVICE void stage_32x32(uint8_t* buf, int lane, const uint32_t (&w)[16]) {
     *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
 
+// 32 rows x 32 fp32 columns to a 4 KB staging buffer (128-byte swizzle: chunk ^= row % 8).
+B200_DEVICE void stage_32x32_f32(uint8_t* buf, int lane, const uint32_t (&w)[32]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+
 // Epilogue of the gated kernels: this warp's 32 rows, 32 output columns at a time.
 //   GATE 1  gate = columns [0, BN / 2) of the accumulator, up = [BN / 2, BN); a = act(gate) * up, made in fp32 and rounded once, leaves
-//           through tmA, gate and up (bf16: what the backward keeps) through tmG and tmU
-//   GATE 2  da = the accumulator, not rounded; d gate and d up leave through tmG and tmU, the product a of the kept projections (which the
-//           gradient of the down projection needs) through tmA
-// The three maps have 32 x 32 boxes with the 64-byte swizzle; each clips at its own M x F.  Three 2 KB buffers per warp; the two warps of a
-// lane quarter take the chunks by turns.
+//           through tmA, gate and up (fp32 or bf16: what the backward keeps) through tmG and tmU
+//   GATE 2  da = the accumulator, not rounded; d gate and d up (bf16) leave through tmG and tmU, the product a of the kept projections (which
+//           the gradient of the down projection needs; of fp32 ones it is the forward's, bit for bit) through tmA
+// The three maps have 32 x 32 boxes, 64-byte swizzle in bf16, 128-byte in fp32; each clips at its own M x F.  6 KB of buffers per warp: three of
+// bf16, or one of fp32, which gate and up pass one after the other, and one of bf16.  The two warps of a lane quarter take the chunks by turns.
 template <int BN, int GATE>
 B200_DEVICE void gate_drain(const CUtensorMap* tmA, const CUtensorMap* tmG, const CUtensorMap* tmU, const PairParams& p, uint32_t t_row,
                             int row0, int n0, uint8_t* buf, int lane, int half) {
@@ -617,37 +625,80 @@ B200_DEVICE void gate_drain(const CUtensorMap* tmA, const CUtensorMap* tmG, cons
       tmem_ld_32x32b_x32(t_row + OUT_N + c * 32, u);
       tc_wait_ld();
 #pragma unroll
+      for (int i = 0; i < 16; ++i)
+        wa[i] = pack_bf16x2(gate_act(__uint_as_float(g[2 * i]), act) * __uint_as_float(u[2 * i]),
+                            gate_act(__uint_as_float(g[2 * i + 1]), act) * __uint_as_float(u[2 * i + 1]));
+      if (w_gu && p.gate.gu_f32) {
+        const bool in = col0 < p.N && row0 < p.M;
+        if (lane == 0) tma_store_wait_read<0>();    // the stores of the chunk before have left the buffers
+        __syncwarp();
+        stage_32x32_f32(buf, lane, g);
+        stage_32x32(buf + 4096, lane, wa);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (in) { tma_store_2d(tmG, buf, col0, row0); tma_store_2d(tmA, buf + 4096, col0, row0); }
+          tma_store_commit();
+          tma_store_wait_read<0>();
+        }
+        __syncwarp();
+        stage_32x32_f32(buf, lane, u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (in) tma_store_2d(tmU, buf, col0, row0);
+          tma_store_commit();
+        }
+        continue;
+      }
+#pragma unroll
       for (int i = 0; i < 16; ++i) {
         wg[i] = pack_bf16x2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
         wu[i] = pack_bf16x2(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
-        wa[i] = pack_bf16x2(gate_act(__uint_as_float(g[2 * i]), act) * __uint_as_float(u[2 * i]),
-                            gate_act(__uint_as_float(g[2 * i + 1]), act) * __uint_as_float(u[2 * i + 1]));
       }
     } else {
       // (F is a multiple of 8: a 16-byte vector is in range or past the end as a whole)
       const bool live = row < p.M;
-      const __nv_bfloat16* src = p.gate.gu + (long long)row * p.gate.ldgu + col0;
+      const long long at = (long long)row * p.gate.ldgu + col0;
+      float g[32], u[32];
+      if (p.gate.gu_f32) {
+        const float* src = (const float*)p.gate.gu + at;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = live && col0 + j * 8 < p.N;
-        const uint4 a = in ? *reinterpret_cast<const uint4*>(src + j * 8) : make_uint4(0u, 0u, 0u, 0u);
-        const uint4 b = in ? *reinterpret_cast<const uint4*>(src + p.N + j * 8) : make_uint4(0u, 0u, 0u, 0u);
-        wg[4 * j] = a.x; wg[4 * j + 1] = a.y; wg[4 * j + 2] = a.z; wg[4 * j + 3] = a.w;
-        wu[4 * j] = b.x; wu[4 * j + 1] = b.y; wu[4 * j + 2] = b.z; wu[4 * j + 3] = b.w;
+        for (int j = 0; j < 8; ++j) {
+          const bool in = live && col0 + j * 4 < p.N;
+          const float4 a = in ? *reinterpret_cast<const float4*>(src + j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 b = in ? *reinterpret_cast<const float4*>(src + p.N + j * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+          g[4 * j] = a.x; g[4 * j + 1] = a.y; g[4 * j + 2] = a.z; g[4 * j + 3] = a.w;
+          u[4 * j] = b.x; u[4 * j + 1] = b.y; u[4 * j + 2] = b.z; u[4 * j + 3] = b.w;
+        }
+      } else {
+        const __nv_bfloat16* src = (const __nv_bfloat16*)p.gate.gu + at;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = live && col0 + j * 8 < p.N;
+          const uint4 a = in ? *reinterpret_cast<const uint4*>(src + j * 8) : make_uint4(0u, 0u, 0u, 0u);
+          const uint4 b = in ? *reinterpret_cast<const uint4*>(src + p.N + j * 8) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 gf = unpack_bf16x2(aw[k]), uf = unpack_bf16x2(bw[k]);
+            g[8 * j + 2 * k] = gf.x; g[8 * j + 2 * k + 1] = gf.y;
+            u[8 * j + 2 * k] = uf.x; u[8 * j + 2 * k + 1] = uf.y;
+          }
+        }
       }
       uint32_t r[32];
       tmem_ld_32x32b_x32(t_row + c * 32, r);
       tc_wait_ld();
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float2 gf = unpack_bf16x2(wg[i]), uf = unpack_bf16x2(wu[i]);
         const float2 d = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
         float v0, s0, v1, s1;
-        gate_act_grad(gf.x, act, v0, s0);
-        gate_act_grad(gf.y, act, v1, s1);
-        wg[i] = pack_bf16x2(d.x * uf.x * s0, d.y * uf.y * s1);
+        gate_act_grad(g[2 * i], act, v0, s0);
+        gate_act_grad(g[2 * i + 1], act, v1, s1);
+        wg[i] = pack_bf16x2(d.x * u[2 * i] * s0, d.y * u[2 * i + 1] * s1);
         wu[i] = pack_bf16x2(d.x * v0, d.y * v1);
-        wa[i] = pack_bf16x2(v0 * uf.x, v1 * uf.y);
+        wa[i] = pack_bf16x2(v0 * u[2 * i], v1 * u[2 * i + 1]);
       }
     }
     if (lane == 0) tma_store_wait_read<0>();        // the stores of the chunk before have left the buffers

@@ -9,9 +9,9 @@
 // accumulator's first half and the up projection in its second, and an epilogue warp has both at hand.  Against a GEMM and a SwiGLU kernel the
 // projections are not read again: 4 bytes of T F less each way, and forward without a backward writes 2 bytes instead of 6.
 //
-// Roundings: a once from fp32, gate and up once where they are kept for the backward (at 2 bytes a value: fp32 would double what a block keeps),
-// da not at all.  What the backward makes of the kept projections (d gate, d up, a) so has two or three roundings of 2^-9 in it: the gradients of
-// 4096 x 4096 x 14336 are 0.0035 off in norm, 0.0017 of that the rounding of the results themselves.
+// Roundings: a once from fp32, da not at all.  gate and up are kept for the backward in fp32 where the caller asks for it (functional.py:
+// GatedMLPFn does), else rounded once to bf16, half the bytes; then d gate and d up have two or three roundings of 2^-9 in them and the gradients
+// of 4096 x 4096 x 14336 are 0.0033 off in norm, 0.0038 that of Wd, instead of 0.0024 (0.0017 the results' own rounding).
 // Measured (4096 tokens, 4096 x 2 x 14336, caches cold): forward 615 us (1.56 PFLOP/s), gradient 370 us (1.30 PFLOP/s; the GEMM of that size
 // alone 293): bound by the tensor pipe under the power cap, the gradient by its epilogue (two operands in, three results out) where a tile's
 // mainloop of 64 stages does not cover it.  Up to 64 rows: gated_fewrows.cu.
@@ -21,12 +21,14 @@
 #include "runtime.h"
 
 namespace {
+constexpr int GU_F32 = 2;
 int check(const char* what, const void* p, long long ld) {
   return (((uintptr_t)p & 15) != 0 || ld % 8 != 0) ? b200::fail(861, "%s: operands must be 16-byte aligned, pitches multiples of 8", what) : 0;
 }
 }  // namespace
 
-// x [M, K], w [2F, K], a [M, F], gu [M, 2F] or null; pitches in elements, multiples of 8; F and K multiples of 8.  act: 0 SiLU, 1 GELU (tanh).
+// x [M, K], w [2F, K], a [M, F], gu [M, 2F] or null; pitches in elements, multiples of 8; F and K multiples of 8.  act: 0 SiLU, 1 GELU (tanh),
+// + 2 (GU_F32) where gu is fp32, else bf16.
 B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, int M, int F, int K, long long ldx, long long ldw,
                              long long lda, long long ldgu, int act, void* stream) {
   using namespace gemmcore;
@@ -37,8 +39,8 @@ B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, in
       (gu != nullptr && (r = check("gemm_gated", gu, ldgu))))
     return r;
   if (M <= fewrows::MAX_ROWS) {
-    const fewrows::GatedArgs p = {(const __nv_bfloat16*)x, (const __nv_bfloat16*)w, (__nv_bfloat16*)a, (__nv_bfloat16*)gu, M, F, K, ldx, ldw, lda, ldgu,
-                                  act};
+    const fewrows::GatedArgs p = {(const __nv_bfloat16*)x, (const __nv_bfloat16*)w, (__nv_bfloat16*)a, gu, M, F, K, ldx, ldw, lda, ldgu,
+                                  act & 1, (act & GU_F32) != 0};
     return fewrows::run_gated(p, (cudaStream_t)stream);
   }
   CUtensorMap tmX, tmW, tmA, tmG, tmU;
@@ -47,13 +49,17 @@ B200_API int b200_gemm_gated(const void* x, const void* w, void* a, void* gu, in
   if ((r = b200::make_tmap_2d(&tmA, b200::DT_BF16, a, F, M, lda * 2, 32, 32, b200::SWZ_64))) return r;
   tmG = tmU = tmA;
   if (gu != nullptr) {
-    if ((r = b200::make_tmap_2d(&tmG, b200::DT_BF16, gu, F, M, ldgu * 2, 32, 32, b200::SWZ_64))) return r;
-    if ((r = b200::make_tmap_2d(&tmU, b200::DT_BF16, (uint8_t*)gu + 2LL * F, F, M, ldgu * 2, 32, 32, b200::SWZ_64))) return r;
+    const bool f32 = act & GU_F32;
+    const auto type = f32 ? b200::DT_F32 : b200::DT_BF16;
+    const auto swizzle = f32 ? b200::SWZ_128 : b200::SWZ_64;
+    const long long es = f32 ? 4 : 2;
+    if ((r = b200::make_tmap_2d(&tmG, type, gu, F, M, ldgu * es, 32, 32, swizzle))) return r;
+    if ((r = b200::make_tmap_2d(&tmU, type, (uint8_t*)gu + es * F, F, M, ldgu * es, 32, 32, swizzle))) return r;
   }
   PairParams p = {};
   p.M = M; p.N = F; p.K = K;
   p.group_m = raster_group_m() > 1 ? raster_group_m() / 2 : 1;
-  p.gate.act = act; p.gate.F = F; p.gate.want_gu = gu != nullptr;
+  p.gate.act = act & 1; p.gate.gu_f32 = (act & GU_F32) != 0; p.gate.F = F; p.gate.want_gu = gu != nullptr;
   p.a_rows = a_box_rows(M);
   p.status = b200::status_ptr();
   return launch_pair<KIND_BF16, 256, 1, 1, 1>(tmX, tmW, tmG, tmU, tmA, tmA, p, (cudaStream_t)stream, "gemm_gated");
@@ -70,7 +76,7 @@ B200_API int b200_gated_down(const void* a, const void* w, const void* res, void
   return fewrows::run_down(p, (cudaStream_t)stream);
 }
 
-// dy [M, K], wd [K, F] (the down projection's weight as it is), gu [M, 2F]; dgu [M, 2F], a [M, F] or null.
+// dy [M, K], wd [K, F] (the down projection's weight as it is), gu [M, 2F]; dgu [M, 2F] and a [M, F] (or null) bf16; act as above.
 B200_API int b200_gemm_gated_grad(const void* dy, const void* wd, const void* gu, void* dgu, void* a, int M, int F, int K, long long lddy,
                                   long long ldwd, long long ldgu, long long lddgu, long long lda, int act, void* stream) {
   using namespace gemmcore;
@@ -91,8 +97,8 @@ B200_API int b200_gemm_gated_grad(const void* dy, const void* wd, const void* gu
   p.M = M; p.N = F; p.K = K;
   p.b_mn_major = 1;
   p.group_m = raster_group_m() > 1 ? raster_group_m() / 2 : 1;
-  p.gate.act = act; p.gate.F = F; p.gate.want_a = a != nullptr;
-  p.gate.gu = (const __nv_bfloat16*)gu; p.gate.ldgu = ldgu;
+  p.gate.act = act & 1; p.gate.gu_f32 = (act & GU_F32) != 0; p.gate.F = F; p.gate.want_a = a != nullptr;
+  p.gate.gu = gu; p.gate.ldgu = ldgu;
   p.a_rows = a_box_rows(M);
   p.status = b200::status_ptr();
   return launch_pair<KIND_BF16, 256, 1, 1, 2>(tmY, tmW, tmG, tmU, tmA, tmA, p, (cudaStream_t)stream, "gemm_gated_grad");

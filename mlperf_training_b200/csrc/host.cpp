@@ -444,17 +444,16 @@ bool bf16_plain(const at::Tensor* t, c10::Device dev) {
          t->size(1) <= 0x7fffffff;
 }
 
-// gated_fwd(x [T, D], w [2F, D], act, want_gu): (a [T, F], gu [T, 2F] or None)
+// gated_fwd(x [T, D], w [2F, D], act, gu: 0 none, 1 bf16, 2 fp32): (a [T, F], gu [T, 2F] or None)
 PyObject* py_gated_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   const at::Tensor *x, *w;
-  long long act;
-  if (nargs != 4 || g_gated == nullptr || (x = tensor_of(args[0])) == nullptr || (w = tensor_of(args[1])) == nullptr || !int_of(args[2], act)) {
+  long long act, want;
+  if (nargs != 4 || g_gated == nullptr || (x = tensor_of(args[0])) == nullptr || (w = tensor_of(args[1])) == nullptr || !int_of(args[2], act) ||
+      !int_of(args[3], want)) {
     if (PyErr_Occurred()) return nullptr;
     Py_RETURN_NONE;
   }
-  const int want = PyObject_IsTrue(args[3]);
-  if (want < 0) return nullptr;
   if (!x->is_cuda() || !bf16_plain(x, x->device()) || !bf16_plain(w, x->device())) Py_RETURN_NONE;
   const int64_t T = x->size(0), D = x->size(1), F = w->size(0) / 2;
   const int dev = x->device().index();
@@ -465,9 +464,9 @@ PyObject* py_gated_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     pybind11::gil_scoped_release nogil;
     const auto o = x->options().requires_grad(false);
     t[0] = at::empty({T, F}, o);
-    if (want) t[1] = at::empty({T, 2 * F}, o);
+    if (want) t[1] = at::empty({T, 2 * F}, want == 2 ? o.dtype(at::kFloat) : o);
     rc = g_gated(x->data_ptr(), w->data_ptr(), t[0].data_ptr(), want ? t[1].data_ptr() : nullptr, (int)T, (int)F, (int)D, x->stride(0), w->stride(0),
-                 F, 2 * F, (int)act, c10::cuda::getCurrentCUDAStream(dev).stream());
+                 F, 2 * F, (int)act + (want == 2 ? 2 : 0), c10::cuda::getCurrentCUDAStream(dev).stream());
   }
   if (rc != 0) return raise_code("b200_gemm_gated", rc);
   return wrap_all(t, 2);
@@ -502,7 +501,7 @@ PyObject* py_gated_down(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// gated_bwd(dy [T, D], w_down [D, F], gu [T, 2F], act, want_a): (dgu [T, 2F], a [T, F] or None)
+// gated_bwd(dy [T, D], w_down [D, F], gu [T, 2F] (bf16 or fp32), act, want_a): (dgu [T, 2F], a [T, F] or None)
 PyObject* py_gated_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   const at::Tensor *dy, *w, *gu;
@@ -514,7 +513,9 @@ PyObject* py_gated_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   const int want = PyObject_IsTrue(args[4]);
   if (want < 0) return nullptr;
-  if (!dy->is_cuda() || !bf16_plain(dy, dy->device()) || !bf16_plain(w, dy->device()) || !bf16_plain(gu, dy->device())) Py_RETURN_NONE;
+  if (!dy->is_cuda() || !bf16_plain(dy, dy->device()) || !bf16_plain(w, dy->device())) Py_RETURN_NONE;
+  const bool f32 = gu->scalar_type() == at::kFloat;
+  if (f32 ? !(gu->device() == dy->device() && plain(*gu)) : !bf16_plain(gu, dy->device())) Py_RETURN_NONE;
   const int64_t T = dy->size(0), D = dy->size(1), F = w->size(1);
   const int dev = dy->device().index();
   if (c10::cuda::current_device() != dev || T <= 0 || D <= 0 || F <= 0 || D % 8 != 0 || F % 8 != 0 || w->size(0) != D || gu->size(0) != T ||
@@ -528,7 +529,7 @@ PyObject* py_gated_bwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     t[0] = at::empty({T, 2 * F}, o);
     if (want) t[1] = at::empty({T, F}, o);
     rc = g_gated_grad(dy->data_ptr(), w->data_ptr(), gu->data_ptr(), t[0].data_ptr(), want ? t[1].data_ptr() : nullptr, (int)T, (int)F, (int)D,
-                      dy->stride(0), w->stride(0), gu->stride(0), 2 * F, F, (int)act, c10::cuda::getCurrentCUDAStream(dev).stream());
+                      dy->stride(0), w->stride(0), gu->stride(0), 2 * F, F, (int)act + (f32 ? 2 : 0), c10::cuda::getCurrentCUDAStream(dev).stream());
   }
   if (rc != 0) return raise_code("b200_gemm_gated_grad", rc);
   return wrap_all(t, 2);

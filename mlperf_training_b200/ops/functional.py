@@ -299,12 +299,14 @@ def add_norm_linear(x, residual, norm_w, weight, eps=1e-5):
 class GatedMLPFn(Function):
     """``y = (act(x Wg^T) * (x Wu^T)) Wd^T (+ residual)`` in bf16: the projections, the activation and the product in one kernel, the down
     projection in another; backward: the gradient of the activation in the epilogue of the down projection's dgrad.  Kept for
-    backward: ``x`` and the projections (the activation's product is made again where they are read)."""
+    backward: ``x`` and the projections in fp32, 8 bytes of T F, from which the activation's product is made again as it was, bit for bit.
+    (Rounded to bf16 they cost the gradients as much as all the roundings behind them: 0.0033 off in norm, 0.0038 that of ``w_down``, against
+    0.0024 now.)"""
 
     @staticmethod
     def forward(ctx, x, w_gate_up, w_down, residual, act, grad=True):
         grad = grad and any(ctx.needs_input_grad)
-        a, gu = K.gated_fwd(x, w_gate_up, act, want_gu=grad)
+        a, gu = K.gated_fwd(x, w_gate_up, act, want_gu=grad, gu_dtype=torch.float32)
         if a.shape[0]:
             y = K.gated_down(a, w_down, residual)
         else:

@@ -285,6 +285,7 @@ def swiglu_bwd(da: torch.Tensor, gu: torch.Tensor) -> torch.Tensor:
 
 
 GATE_ACTS = {"silu": 0, "gelu": 1}       # gelu: the tanh form
+GU_F32 = 2                               # ... and fp32 projections
 
 
 def _gate_check(what: str, x: torch.Tensor, w: torch.Tensor, act: str, Fh: int, D: int) -> None:
@@ -305,13 +306,16 @@ def _gate_value(g: torch.Tensor, act: str) -> torch.Tensor:
     return F.silu(g) if act == "silu" else F.gelu(g, approximate="tanh")
 
 
-def gated_fwd(x: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu", *, want_gu: bool = True):
+def gated_fwd(x: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu", *, want_gu: bool = True, gu_dtype: torch.dtype | None = None):
     """``a = act(x Wg^T) * (x Wu^T)`` of ``x [T, D]`` and the stacked ``w_gate_up [2F, D]`` (gate rows first) in one launch.  Returns
-    ``(a [T, F], gu [T, 2F])``; ``gu`` (the projections, for the backward) is None without
-    ``want_gu``."""
+    ``(a [T, F], gu [T, 2F])``; ``gu`` (the projections, for the backward) in ``gu_dtype``, fp32 or that of ``x`` (None: that of ``x``), None
+    without ``want_gu``."""
+    if gu_dtype not in (None, x.dtype, torch.float32):
+        raise TypeError(f"gated_fwd: projections of {gu_dtype} for an input of {x.dtype}")
+    gu_dtype = gu_dtype or x.dtype
     if x.is_cuda and act in GATE_ACTS and use_kernels(x) and _lib.host is not None:
         # (results for operands that are as the kernel reads them; None leaves copies and errors to the lines below)
-        r = _lib.host.gated_fwd(x, w_gate_up, GATE_ACTS[act], want_gu)
+        r = _lib.host.gated_fwd(x, w_gate_up, GATE_ACTS[act], 0 if not want_gu else 2 if gu_dtype == torch.float32 else 1)
         if r is not None:
             return r
     T, D = x.shape
@@ -322,13 +326,13 @@ def gated_fwd(x: torch.Tensor, w_gate_up: torch.Tensor, act: str = "silu", *, wa
     if not use_kernels(x):
         gu = x.float() @ w_gate_up.float().t()
         a = (_gate_value(gu[:, :Fh], act) * gu[:, Fh:]).to(x.dtype)
-        return a, gu.to(x.dtype) if want_gu else None
+        return a, gu.to(gu_dtype) if want_gu else None
     a = torch.empty((T, Fh), dtype=x.dtype, device=x.device)
-    gu = torch.empty((T, 2 * Fh), dtype=x.dtype, device=x.device) if want_gu else None
+    gu = torch.empty((T, 2 * Fh), dtype=gu_dtype, device=x.device) if want_gu else None
     if T:
         x, w = _row_major(x), _row_major(w_gate_up)
-        call("b200_gemm_gated", ptr(x), ptr(w), ptr(a), ptr(gu), T, Fh, D, x.stride(0), w.stride(0), a.stride(0), 2 * Fh, GATE_ACTS[act],
-             stream_ptr())
+        call("b200_gemm_gated", ptr(x), ptr(w), ptr(a), ptr(gu), T, Fh, D, x.stride(0), w.stride(0), a.stride(0), 2 * Fh,
+             GATE_ACTS[act] + (GU_F32 if gu_dtype == torch.float32 else 0), stream_ptr())
     return a, gu
 
 
@@ -366,9 +370,9 @@ def gated_down(a: torch.Tensor, w_down: torch.Tensor, residual: torch.Tensor | N
 
 
 def gated_bwd(dy: torch.Tensor, w_down: torch.Tensor, gu: torch.Tensor, act: str = "silu", *, want_a: bool = True):
-    """Gradient of ``gu [T, 2F]`` from that of ``a W_down^T``, ``dy [T, D]``, ``w_down [D, F]``, in one launch: ``da = dy W_down``, ``d gate = da
-    * up * act'(gate)``, ``d up = da * act(gate)``.  Returns ``(dgu [T, 2F], a [T, F])``; ``a`` (made again from ``gu``, for the gradient of
-    ``w_down``) is None without ``want_a``."""
+    """Gradient of ``gu [T, 2F]`` (fp32 or the type of ``dy``) from that of ``a W_down^T``, ``dy [T, D]``, ``w_down [D, F]``, in one launch: ``da =
+    dy W_down``, ``d gate = da * up * act'(gate)``, ``d up = da * act(gate)``.  Returns ``(dgu [T, 2F], a [T, F])`` in the type of ``dy``; ``a``
+    (made again from ``gu``, for the gradient of ``w_down``; from fp32 it is the forward's) is None without ``want_a``."""
     if dy.is_cuda and act in GATE_ACTS and use_kernels(dy) and _lib.host is not None:
         r = _lib.host.gated_bwd(dy, w_down, gu, GATE_ACTS[act], want_a)
         if r is not None:
@@ -376,7 +380,7 @@ def gated_bwd(dy: torch.Tensor, w_down: torch.Tensor, gu: torch.Tensor, act: str
     T, F2 = gu.shape
     D, Fh = w_down.shape
     _gate_check("gated_bwd", dy, w_down, act, Fh, D)
-    if dy.shape != (T, D) or F2 != 2 * Fh or gu.dtype != dy.dtype or gu.device != dy.device:
+    if dy.shape != (T, D) or F2 != 2 * Fh or gu.dtype not in (dy.dtype, torch.float32) or gu.device != dy.device:
         raise ValueError(f"gated_bwd: gradient {tuple(dy.shape)}, weight {tuple(w_down.shape)}, projections {tuple(gu.shape)} {gu.dtype}")
     if not use_kernels(dy):
         da = dy.float() @ w_down.float()
@@ -388,12 +392,13 @@ def gated_bwd(dy: torch.Tensor, w_down: torch.Tensor, gu: torch.Tensor, act: str
         v = v.detach()
         return torch.cat([dg, da * v], 1).to(dy.dtype), (v * u).to(dy.dtype) if want_a else None
     gu = _row_major(gu)
+    gu = gu if gu.stride(0) % 8 == 0 else gu.clone(memory_format=torch.contiguous_format)
     dgu = torch.empty((T, F2), dtype=dy.dtype, device=dy.device)
     a = torch.empty((T, Fh), dtype=dy.dtype, device=dy.device) if want_a else None
     if T:
         dy, w = _row_major(dy), _row_major(w_down)
         call("b200_gemm_gated_grad", ptr(dy), ptr(w), ptr(gu), ptr(dgu), ptr(a), T, Fh, D, dy.stride(0), w.stride(0), gu.stride(0), F2, Fh,
-             GATE_ACTS[act], stream_ptr())
+             GATE_ACTS[act] + (GU_F32 if gu.dtype == torch.float32 else 0), stream_ptr())
     return dgu, a
 
 
