@@ -7,14 +7,15 @@
 // W = [Wg; Wu] is the stacked [2F, D] weight of the two projections as the model keeps it.  A 256-row tile of 128 output columns runs as one
 // 256 x 256 tile: the leader CTA stages the 128 gate rows, its partner the 128 up rows of the same columns, so that the gate lands in the
 // accumulator's first half and the up projection in its second, and an epilogue warp has both at hand.  Against a GEMM and a SwiGLU kernel the
-// projections are not read again: 4 bytes of T F less each way, and forward without a backward writes 2 bytes instead of 6.
+// projections are not read again by the forward, and one without a backward writes 2 bytes of T F instead of 6.
 //
 // Roundings: a once from fp32, da not at all.  gate and up are kept for the backward in fp32 where the caller asks for it (functional.py:
 // GatedMLPFn does), else rounded once to bf16, half the bytes; then d gate and d up have two or three roundings of 2^-9 in them and the gradients
-// of 4096 x 4096 x 14336 are 0.0033 off in norm, 0.0038 that of Wd, instead of 0.0024 (0.0017 the results' own rounding).
-// Measured (4096 tokens, 4096 x 2 x 14336, caches cold): forward 615 us (1.56 PFLOP/s), gradient 370 us (1.30 PFLOP/s; the GEMM of that size
-// alone 293): bound by the tensor pipe under the power cap, the gradient by its epilogue (two operands in, three results out) where a tile's
-// mainloop of 64 stages does not cover it.  Up to 64 rows: gated_fewrows.cu.
+// of 4096 x 4096 x 14336 are 0.0030 off in norm, 0.0034 that of Wd, instead of 0.0023 (0.0017 the results' own rounding).
+// Measured (4096 tokens, 4096 x 2 x 14336, caches cold): forward 648 us (1.48 PFLOP/s; 622 with projections in bf16, 600 without), gradient
+// 411 us (1.17 PFLOP/s; 378 from projections in bf16, the GEMM of that size alone 293): bound by the tensor pipe under the power cap, the
+// gradient by its epilogue (two operands in, three results out) where a tile's mainloop of 64 stages does not cover it.
+// Up to 64 rows: gated_fewrows.cu.
 #include "common.cuh"
 #include "gemm_core.cuh"
 #include "gated_fewrows.cuh"

@@ -51,7 +51,9 @@ int run(const void* a_q, const void* sfa, const void* b_q, const void* sfb, void
 // become f16 pairs, two HFMA2 chains of eight make a 32-block's sum, which goes on in fp32, scaled by both blocks' powers of two.
 // A warp owns the rows of B whose scales share 16 bytes of an atom (rows r, r + 32, r + 64, r + 96 of it), a lane a block of each at a time.
 // Measured (caches cold, tensor cores -> this): 4096 x 4096 15 -> 8.5 us, 4096 x 14336 22 -> 16.5, 28672 x 4096 26 -> 23 (2.7 TB/s); two rows
-// took 34 us there, so it is taken for one.  Bound by instructions: about three an element of B for conversion, product and scale.
+// took 34 us there, so it is taken for one.  Bound by how the rows lie on the SMs first, by instructions second (counted, caches cold): 3.4
+// instructions an element of B for conversion, product and scale keep the issue slots of a working SM 64 % busy, but 28672 rows are 9600 units on
+// 2368 warps, whose fifth round runs on a few SMs (an SM works 69 % of the time), and 4096 rows are 88 CTAs: 60 SMs have nothing to do (45 %).
 struct GemvArgs {
   const uint8_t* a_q; const uint8_t* sfa;
   const uint8_t* b_q; const uint8_t* sfb;
