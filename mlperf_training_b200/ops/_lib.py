@@ -11,6 +11,7 @@ loaded, so GPU runs never fall back silently to eager PyTorch.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -92,6 +93,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_gemm_gated_grad": [P, P, P, P, P, I, I, I, L, L, L, L, L, I, P],
         "b200_router_topk": [P, I, I, I, P, P, P, P],
         "b200_router_plan": [P, P, I, I, I, P, P, I, P, P],
+        "b200_route": [P, I, L, P, I, I, I, I, I, I, I, F, P, P, P, P],
+        "b200_route_bwd": [P, I, L, P, P, I, I, I, I, I, F, P, P],
+        "b200_balance_bias": [P, P, I, F, P, P],
         "b200_permute_rows": [P, P, I, I, I, P, P, P, P, P, I, P],
         "b200_unpermute_sum": [P, P, P, I, I, I, P, P, P],
         "b200_gemm_grouped_rows": [P, P, P, P, I, I, I, I, L, L, I, I, F, P],
@@ -169,6 +173,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.b200_hstu_gate_cat_scratch_elems.restype = c_ll
     lib.b200_norm_bwd_scratch_elems.restype = c_ll
     lib.b200_sumsq_scratch_elems.restype = c_int
+    if hasattr(lib, "b200_route_stores_counts"):
+        lib.b200_route_stores_counts.argtypes = [I]
+        lib.b200_route_stores_counts.restype = c_int
     if hasattr(lib, "b200_sort_scratch_bytes"):
         lib.b200_sort_scratch_bytes.argtypes = [L]
         lib.b200_sort_scratch_bytes.restype = c_ll
@@ -251,6 +258,16 @@ def stream_ptr() -> int:
     """Raw handle of the calling thread's current stream on its current device.  (``torch.cuda.current_stream()`` builds a
     Stream object through several Python layers: 4 us of each launch.)"""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def on_device_of(t: torch.Tensor):
+    """Makes the device of ``t`` the current one for a launch (nothing to do where it is: the usual case)."""
+    if t.device.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(t.device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -19,9 +19,10 @@ import warnings
 import torch
 from torch.autograd import Function
 
+from . import _lib
 from . import kernels as K
 from . import mxfp8
-from ._lib import call, ptr, stream_ptr, use_kernels
+from ._lib import call, on_device_of, ptr, stream_ptr, use_kernels
 
 PAD = 128        # row padding of an expert segment for the bf16 grouped kernels (one 128-row tile)
 PAD_MX = 256     # ... for the grouped kernels on CTA pairs (256 rows per pair): block-scaled, and bf16 where `pair_rows_ok`
@@ -42,7 +43,6 @@ def pair_rows_ok(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor) -> bool:
 
 def grouped_bn(n: int) -> int:
     """N tile of the block-scaled grouped GEMM for a per-expert output width ``n`` (0 = unsupported width)."""
-    from . import _lib
     if _lib.LIB_PATH.exists():
         return int(_lib.load().b200_gemm_grouped_mx_bn(int(n)))
     return 192 if n % 192 == 0 else (128 if n % 128 == 0 else 0)
@@ -77,6 +77,120 @@ def router_topk(logits: torch.Tensor, k: int):
     counts = torch.zeros(E, dtype=torch.int32, device=logits.device)
     call("b200_router_topk", ptr(logits), T, E, k, ptr(idx), ptr(w), ptr(counts), stream_ptr())
     return idx, w, counts
+
+
+ROUTE_EPS = 1e-20       # beside the sum that renormalised weights are divided by
+ROUTE_MAX_E, ROUTE_MAX_K, ROUTE_MAX_GROUPS = 256, 32, 32
+ROUTE_SCORES = ("softmax", "sigmoid")
+
+
+def _route_check(logits, k, score, bias, groups, top_groups) -> None:
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"route: logits [T, E] in fp32 or bf16, not {list(logits.shape)} in {logits.dtype}")
+    T, E = logits.shape
+    if score not in ROUTE_SCORES:
+        raise ValueError(f"route: score '{score}' (one of {', '.join(ROUTE_SCORES)})")
+    if not 1 <= E <= ROUTE_MAX_E or not 1 <= k <= min(E, ROUTE_MAX_K):
+        raise ValueError(f"route: k = {k} of {E} experts (at most {ROUTE_MAX_K} of {ROUTE_MAX_E})")
+    if not 1 <= groups <= ROUTE_MAX_GROUPS or E % groups or not 1 <= top_groups <= groups or top_groups * (E // groups) < k:
+        raise ValueError(f"route: {E} experts in {groups} groups (at most {ROUTE_MAX_GROUPS}) of which {top_groups} stay, for k = {k}")
+    if T > 2 ** 31 - 1:
+        raise ValueError(f"route: {T} tokens")
+    if bias is not None and (bias.shape != (E,) or bias.device != logits.device):
+        raise ValueError(f"route: bias [{E}] on {logits.device}, not {list(bias.shape)} on {bias.device}")
+
+
+def _route_scores(x: torch.Tensor, score: str) -> torch.Tensor:
+    if score == "sigmoid":
+        return torch.sigmoid(x)
+    return torch.where((x == float("-inf")).all(-1, keepdim=True), torch.zeros_like(x), torch.softmax(x, -1))
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def route_fwd(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1, top_groups: int = 1,
+              renormalize: bool = True, scale: float = 1.0):
+    """``(idx int32 [T, k], w fp32 [T, k], counts int32 [E])``: see ``route``."""
+    _route_check(logits, k, score, bias, groups, top_groups)
+    T, E = logits.shape
+    if not use_kernels(logits):
+        x = logits.double()
+        s = _route_scores(x, score)
+        lost = float("-inf")
+        by = x
+        if bias is not None or top_groups < groups:
+            by = s if bias is None else s + bias.double()
+            by = torch.where(by.isnan(), lost, by)
+        if top_groups < groups:
+            pair = by.unflatten(1, (groups, E // groups)).sort(-1, descending=True)[0][..., :2].sum(-1)
+            kept = torch.zeros(T, groups, dtype=torch.bool).scatter_(1, pair.sort(dim=-1, descending=True, stable=True)[1][:, :top_groups], True)
+            out = ~kept.repeat_interleave(E // groups, 1)
+        else:
+            out = torch.zeros_like(by, dtype=torch.bool)
+        # largest first, NaN behind -inf, experts of other groups last; ties to the lower index
+        order = torch.arange(E).expand(T, E)
+        for key in (torch.where(by.isnan(), lost, by).neg(), by.isnan().double(), out.double()):
+            order = order.gather(1, key.gather(1, order).sort(dim=-1, stable=True)[1])
+        idx = order[:, :k]
+        sj = s.gather(1, idx)
+        w = scale * sj / (sj.sum(-1, keepdim=True) + ROUTE_EPS) if renormalize else scale * sj
+        return idx.to(torch.int32), w.float(), torch.bincount(idx.reshape(-1), minlength=E).to(torch.int32)
+    logits = _rows_of(logits)
+    dev = logits.device
+    idx = torch.empty((T, k), dtype=torch.int32, device=dev)
+    w = torch.empty((T, k), dtype=torch.float32, device=dev)
+    counts = (torch.empty if _lib.load().b200_route_stores_counts(T) else torch.zeros)(E, dtype=torch.int32, device=dev)
+    b = None if bias is None else bias.detach().float().contiguous()
+    with on_device_of(logits):
+        call("b200_route", ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0), ptr(b), T, E, k, int(score == "sigmoid"), groups,
+             top_groups, int(renormalize), float(scale), ptr(idx), ptr(w), ptr(counts), stream_ptr())
+    return idx, w, counts
+
+
+def route_bwd(gw: torch.Tensor, logits: torch.Tensor, idx: torch.Tensor, *, score: str, renormalize: bool, scale: float) -> torch.Tensor:
+    """Gradient of the logits (their type) from that of the weights."""
+    T, E = logits.shape
+    if not use_kernels(logits):
+        s, at, g = _route_scores(logits.double(), score), idx.long(), scale * gw.double()
+        sj = s.gather(1, at)
+        if renormalize:
+            total = sj.sum(-1, keepdim=True) + ROUTE_EPS
+            g = (g - (g * sj).sum(-1, keepdim=True) / total) / total
+        if score == "sigmoid":
+            d = torch.zeros_like(s).scatter_(1, at, g * sj * torch.sigmoid(-logits.double().gather(1, at)))
+        else:
+            d = torch.zeros_like(s).scatter_(1, at, g)
+            d = s * (d - (g * sj).sum(-1, keepdim=True))
+        return d.to(logits.dtype)
+    logits = _rows_of(logits)
+    dx = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    gw = gw.float().contiguous()
+    with on_device_of(logits):
+        call("b200_route_bwd", ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0), ptr(idx), ptr(gw), T, E, idx.shape[1],
+             int(score == "sigmoid"), int(renormalize), float(scale), ptr(dx), stream_ptr())
+    return dx
+
+
+def balance_bias(bias: torch.Tensor, counts: torch.Tensor, rate: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``bias + rate * sign(mean(counts) - counts)``: one step of the bias that ``route`` selects by, towards experts with less than the mean
+    load (``counts`` of a step, summed over the ranks that share the router).  ``out`` may be ``bias``."""
+    E = bias.numel()
+    if bias.dtype != torch.float32 or bias.dim() != 1 or counts.shape != bias.shape or counts.dtype != torch.int32 or counts.device != bias.device:
+        raise ValueError(f"balance_bias: bias fp32 [E] and counts int32 [E] on one device, not {bias.dtype} {list(bias.shape)} and {counts.dtype} {list(counts.shape)}")
+    if out is not None and (out.dtype != torch.float32 or out.shape != bias.shape or out.device != bias.device or not out.is_contiguous()):
+        raise ValueError("balance_bias: out is a contiguous fp32 tensor like bias")
+    out = torch.empty_like(bias, memory_format=torch.contiguous_format) if out is None else out
+    if E == 0:
+        return out
+    if not use_kernels(bias):
+        n = counts.to(torch.int64)
+        return out.copy_(bias + rate * torch.sign(n.sum() - E * n).to(torch.float32))
+    bias, counts = bias.contiguous(), counts.contiguous()
+    with on_device_of(bias):
+        call("b200_balance_bias", ptr(bias), ptr(counts), E, float(rate), ptr(out), stream_ptr())
+    return out
 
 
 def plan(idx: torch.Tensor, counts: torch.Tensor, n_experts: int, pad: int = PAD):
@@ -236,6 +350,38 @@ class RouterFn(Function):
         out = torch.zeros(ctx.shape, dtype=gw.dtype, device=gw.device)
         out.scatter_(1, idx.long(), g)
         return out, None
+
+
+class RouteFn(Function):
+    @staticmethod
+    def forward(ctx, logits, bias, k, score, groups, top_groups, renormalize, scale):
+        idx, w, counts = route_fwd(logits, k, score=score, bias=bias, groups=groups, top_groups=top_groups, renormalize=renormalize, scale=scale)
+        ctx.save_for_backward(logits, idx)
+        ctx.cfg = (score, renormalize, scale)
+        ctx.mark_non_differentiable(idx, counts)
+        ctx.set_materialize_grads(False)
+        return idx, w, counts
+
+    @staticmethod
+    def backward(ctx, _gidx, gw, _gc):
+        if gw is None:
+            return (None,) * 8
+        logits, idx = ctx.saved_tensors
+        score, renormalize, scale = ctx.cfg
+        return (route_bwd(gw, logits, idx, score=score, renormalize=renormalize, scale=scale),) + (None,) * 7
+
+
+def route(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1, top_groups: int = 1,
+          renormalize: bool = True, scale: float = 1.0):
+    """Routing of tokens to experts: ``(idx int32 [T, k], w fp32 [T, k], counts int32 [E])`` from ``logits [T, E]`` (fp32 or bf16).
+
+    The scores are ``softmax`` over all experts or ``sigmoid``.  Experts are chosen by score + ``bias`` (fp32 ``[E]``, without a gradient: a
+    balance bias, or -inf for an expert that gets nothing), largest first, ties to the lower index.  With ``groups`` the experts lie in that
+    many equal groups and only the ``top_groups`` with the largest sum of their two best take part.  The weights are the scores of the chosen, without
+    the bias, divided by their sum (``renormalize``) and times ``scale``.  Comparisons hold in 64 bits; without a bias and groups it is the
+    logits that are compared.  ``idx``, ``w`` and ``counts`` go into ``moe_experts`` like those of ``router_topk``, which is
+    ``softmax`` with ``renormalize`` for few experts chosen by their logits."""
+    return RouteFn.apply(logits, bias, k, score, groups, top_groups, renormalize, scale)
 
 
 class PermuteFn(Function):
