@@ -78,6 +78,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_add_bf16": [P, P, P, L, P],
         "b200_accum_f32_bf16": [P, P, L, P],
         "b200_cross_entropy": [P, P, P, P, L, L, I, F, I, L, P],
+        "b200_distill_fwd": [P, I, L, P, P, I, P, I, I, I, I, I, F, F, L, P, P, P, P],
+        "b200_distill_bwd": [P, I, L, P, P, I, P, I, I, I, I, I, F, F, L, P, P, P, P, L, P],
         "b200_sumsq": [P, L, I, P, P, I, P],
         "b200_adamw": [P, I, P, P, I, P, P, L, F, F, F, F, F, I, F, P, F, I, P],
         "b200_adamw_bf16m": [P, I, P, P, I, P, P, L, F, F, F, F, F, I, F, P, F, I, P],

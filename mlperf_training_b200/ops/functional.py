@@ -723,6 +723,92 @@ def lm_head_loss(x, norm_w, weight, labels, *, eps=1e-5, n_valid=None, precision
     return LMHeadLossFn.apply(x, norm_w, weight, labels, eps, n_valid, precision, torch.is_grad_enabled())
 
 
+class DistillLossFn(Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ids, values, alpha, temperature, rest, ignore_index):
+        cfg = dict(alpha=alpha, temperature=temperature, rest=rest, ignore_index=ignore_index)
+        loss, saved = K.distill_fwd(logits, labels, ids, values, **cfg)
+        ctx.save_for_backward(logits, labels, ids, values, *(saved or ()))
+        ctx.cfg = cfg
+        return loss
+
+    @staticmethod
+    def backward(ctx, gy):
+        logits, labels, ids, values, *saved = ctx.saved_tensors
+        return (K.distill_bwd(gy, logits, labels, ids, values, saved, **ctx.cfg),) + (None,) * 7
+
+
+def distill_loss(logits, labels, ids, values, *, alpha=1.0, temperature=1.0, rest=False, ignore_index=-100):
+    """Distillation from a teacher's K largest logits mixed with cross-entropy: fp32 loss ``[T]`` of ``logits [T, V]`` (fp32 or bf16),
+
+        alpha * temperature^2 * KL(teacher || student, both at ``temperature``) + (1 - alpha) * cross-entropy(labels).
+
+    ``ids [T, K]`` (int32 or int64) and ``values [T, K]`` are the teacher's entries; one whose id is outside the vocabulary (-1, say) or whose
+    value is -inf is not there, so tokens may have fewer than K, or none (their KL is 0).  An id that is there twice counts twice.  ``values``
+    are logits, softmaxed over the entries at ``temperature``; or, with ``rest``, the teacher's log-probabilities over the whole vocabulary
+    at that temperature, and what they leave of 1 is one further event: any other id.  Tokens whose label is ``ignore_index`` have
+    loss and gradient 0; ``labels`` may be None where ``alpha`` is 1.  The gradient goes to the logits alone."""
+    return _apply(DistillLossFn, logits, labels, ids, values, alpha, temperature, rest, ignore_index)
+
+
+class LMHeadDistillFn(Function):
+    """Final norm, vocabulary GEMM and ``distill_loss``, summed over ``n_valid``.  The logits make room for their own gradient in backward,
+    which therefore runs once."""
+
+    @staticmethod
+    def forward(ctx, x, norm_w, weight, labels, ids, values, cfg, eps, n_valid, precision, grad=True):
+        grad = grad and any(ctx.needs_input_grad)
+        ctx.norm_operand = precision == "fp4" and x.shape[0] > 0 and add_norm_linear_eligible(x, weight)
+        if ctx.norm_operand:
+            logits, x, rstd, saved = _norm_operand_linear(x, None, norm_w, weight, eps, grad, grad and weight.requires_grad)
+        else:
+            xn, _, _, rstd = K.norm_fwd(x, norm_w, None, eps)
+            keep = grad and L.low_precision(precision, x.shape[0], weight.shape[0], weight.shape[1])
+            logits, saved = L.forward(xn, weight, precision, need_wgrad=keep and weight.requires_grad, need_dgrad=grad)
+            del xn
+        loss, stats = K.distill_fwd(logits, labels, ids, values, **cfg)
+        tensors, ctx.meta = L.Saved.pack(saved) if saved is not None else ([], None)
+        ctx.n_stats = len(stats or ())
+        ctx.save_for_backward(x, norm_w, weight, rstd, labels, ids, values, *(stats or ()), *tensors)
+        ctx.logits = logits if grad else None
+        ctx.args = (cfg, eps, n_valid, precision)
+        ctx.refs = (norm_w, weight)
+        return loss.sum() / n_valid
+
+    @staticmethod
+    def backward(ctx, dloss):
+        x, norm_w, weight, rstd, labels, ids, values, *more = ctx.saved_tensors
+        cfg, eps, n_valid, precision = ctx.args
+        if ctx.logits is None:
+            raise RuntimeError("lm_head_distill_loss: a second backward pass, after the gradient has taken the logits' place")
+        logits, ctx.logits = ctx.logits, None
+        stats, tensors = more[:ctx.n_stats], more[ctx.n_stats:]
+        gy = (dloss.reshape(1).float() / n_valid).expand(x.shape[0])
+        dl = K.distill_bwd(gy, logits, labels, ids, values, stats, out=logits, **cfg)
+        saved = L.Saved.unpack(tensors, ctx.meta) if ctx.meta is not None else None
+        if ctx.norm_operand:
+            dxn, dw = _norm_operand_linear_grad(dl, weight, ctx.refs[1], saved)
+        else:
+            if saved is None and weight.requires_grad:
+                saved = K.norm_fwd(x, norm_w, None, eps)[0]
+            dxn, dw = L.backward(dl, saved, weight, precision, need_dx=True, need_dw=weight.requires_grad and saved is not None)
+        del saved
+        dx, dnw, _ = K.norm_bwd(dxn, x, norm_w, None, None, rstd)
+        return (dx, _vec_grad(ctx.refs[0], dnw), dw) + (None,) * 8
+
+
+def lm_head_distill_loss(x, norm_w, weight, labels, ids, values, *, alpha=1.0, temperature=1.0, rest=False, ignore_index=-100, eps=1e-5,
+                         n_valid=None, precision="bf16"):
+    """``lm_head_loss`` with ``distill_loss`` (its arguments) in the place of the cross-entropy: the sum over the tokens divided by ``n_valid``
+    (all tokens where it is None).  Its backward pass runs once."""
+    cfg = dict(alpha=alpha, temperature=temperature, rest=rest, ignore_index=ignore_index)
+    K._distill_check(x.new_empty((x.shape[0], weight.shape[0]), device="meta"), None if labels is None else labels.to("meta"), ids.to("meta"),
+                     values.to("meta"), alpha, temperature, rest)
+    n_valid = n_valid if n_valid is not None else max(x.shape[0], 1)
+    return LMHeadDistillFn.apply(x, norm_w, weight, None if labels is None else labels.reshape(-1), ids, values, cfg, eps, n_valid, precision,
+                                 torch.is_grad_enabled())
+
+
 # --------------------------------------------------------------------------------------
 # MMDiT glue: AdaLN modulation, gated residual, rotary embedding on [B, S, H, D]
 # --------------------------------------------------------------------------------------

@@ -491,6 +491,127 @@ def cross_entropy_(logits: torch.Tensor, labels: torch.Tensor, grad_scale: float
 
 
 # --------------------------------------------------------------------------------------
+# distillation from a teacher's largest logits
+# --------------------------------------------------------------------------------------
+DISTILL_MAX_K = 1024
+DISTILL_MAX_REST_V = 1 << 20       # ids are marked in shared memory, a bit each
+
+
+def _distill_check(logits, labels, ids, values, alpha, temperature, rest) -> None:
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, BF16) or logits.shape[1] < 1:
+        raise ValueError(f"distill: logits [T, V] in fp32 or bf16, not {list(logits.shape)} in {logits.dtype}")
+    T, V = logits.shape
+    if ids.dim() != 2 or ids.shape != values.shape or ids.shape[0] != T or not 1 <= ids.shape[1] <= DISTILL_MAX_K:
+        raise ValueError(f"distill: ids and values [{T}, K], K at most {DISTILL_MAX_K}, not {list(ids.shape)} and {list(values.shape)}")
+    if ids.dtype not in (torch.int32, torch.int64) or values.dtype not in (torch.float32, BF16, torch.float16):
+        raise ValueError(f"distill: ids in int32 or int64 and values in a floating type of at most 32 bits, not {ids.dtype} and {values.dtype}")
+    if not 0.0 <= alpha <= 1.0 or not 0.0 < temperature < float("inf"):
+        raise ValueError(f"distill: alpha {alpha} (0 to 1), temperature {temperature} (above 0)")
+    if labels is None and alpha < 1.0:
+        raise ValueError("distill: the cross-entropy of alpha < 1 wants labels")
+    if labels is not None and (labels.shape != (T,) or labels.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"distill: labels [{T}] in int32 or int64, not {list(labels.shape)} in {labels.dtype}")
+    if rest and V > DISTILL_MAX_REST_V:
+        raise ValueError(f"distill: a vocabulary of {V} with rest (at most {DISTILL_MAX_REST_V})")
+    if any(t is not None and t.device != logits.device for t in (labels, ids, values)):
+        raise ValueError(f"distill: labels, ids and values on {logits.device}, where the logits are")
+
+
+def _distill_plain(logits, labels, ids, values, alpha, temperature, rest, ignore_index):
+    """Loss per token and what its gradient needs, in 64 bits."""
+    z, t = logits.double(), values.double()
+    T, V = z.shape
+    there = (ids >= 0) & (ids < V) & (t != float("-inf"))
+    at = torch.where(there, ids, 0).long()
+    live = torch.ones(T, dtype=torch.bool) if labels is None else labels != ignore_index
+    labelled = live & (alpha < 1) if labels is None else live & (alpha < 1) & (labels >= 0) & (labels < V)
+    label = torch.where(labelled, labels, 0).long() if labels is not None else torch.zeros(T, dtype=torch.long)
+    none = float("-inf")
+    if rest:
+        logp = t
+    else:
+        total = torch.logsumexp(torch.where(there, t / temperature, none), -1, keepdim=True)
+        logp = t / temperature - torch.where(total == none, 0.0, total)
+    p = torch.where(there, logp.exp(), 0.0)
+    logq, logq1 = torch.log_softmax(z / temperature, -1), torch.log_softmax(z, -1)
+    kl = torch.where(p != 0, p * (logp - logq.gather(1, at)), 0.0).sum(-1)
+    c, ratio = p.sum(-1), torch.zeros(T, dtype=torch.float64)
+    among = torch.zeros(T, V + 1, dtype=torch.bool).scatter_(1, torch.where(there, ids.long(), V), True)[:, :V]
+    if rest:
+        others, r = torch.logsumexp(torch.where(among, none, logq), -1), 1 - c
+        has = (r > 0) & (others > none)
+        kl = kl + torch.where(has, r * (r.clamp(min=1e-300).log() - others), 0.0)
+        ratio = torch.where(has, r / others.exp(), 0.0)
+        c = torch.where(has, c + r, c)
+    loss = alpha * temperature ** 2 * kl if alpha > 0 else torch.zeros_like(kl)
+    if alpha < 1:
+        loss = loss - (1 - alpha) * torch.where(labelled, logq1.gather(1, label[:, None])[:, 0], 0.0)
+    return torch.where(live, loss, 0.0), (logq, logq1, p, at, there, among, c, ratio, live, labelled, label)
+
+
+def _distill_plain_grad(gy, logits, labels, ids, values, alpha, temperature, rest, ignore_index):
+    _, (logq, logq1, p, at, there, among, c, ratio, live, labelled, label) = _distill_plain(logits, labels, ids, values, alpha, temperature, rest,
+                                                                                            ignore_index)
+    g = torch.zeros(logits.shape, dtype=torch.float64)
+    if alpha > 0:
+        g = logq.exp() * (c[:, None] - torch.where(among, 0.0, ratio[:, None]))
+        g.scatter_add_(1, at, torch.where(there, -p, 0.0))
+        g *= alpha * temperature
+    if alpha < 1:
+        g1 = logq1.exp()
+        g1[torch.arange(g.shape[0]), label] -= 1
+        g = g + (1 - alpha) * torch.where(labelled[:, None], g1, 0.0)
+    return torch.where(live[:, None], g * gy.double()[:, None], 0.0)
+
+
+def distill_fwd(logits: torch.Tensor, labels: torch.Tensor | None, ids: torch.Tensor, values: torch.Tensor, *, alpha: float = 1.0,
+                temperature: float = 1.0, rest: bool = False, ignore_index: int = -100):
+    """``(loss fp32 [T], saved)`` of ``functional.distill_loss``; ``saved`` goes into ``distill_bwd`` with the same arguments."""
+    _distill_check(logits, labels, ids, values, alpha, temperature, rest)
+    T, V = logits.shape
+    if not use_kernels(logits):
+        return _distill_plain(logits, labels, ids, values, alpha, temperature, rest, ignore_index)[0].float(), None
+    logits = logits if logits.stride(1) == 1 else logits.contiguous()
+    labels = None if labels is None else labels.to(torch.int64).contiguous()
+    ids, values = ids.contiguous(), (values.float() if values.dtype == torch.float16 else values).contiguous()
+    dev = logits.device
+    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    stats = torch.empty((T, 4), dtype=torch.float32, device=dev)
+    teacher = torch.empty(T, dtype=torch.float64, device=dev)
+    with _lib.on_device_of(logits):
+        call("b200_distill_fwd", ptr(logits), int(logits.dtype == BF16), logits.stride(0), ptr(labels), ptr(ids), int(ids.dtype == torch.int64),
+             ptr(values), int(values.dtype == BF16), T, ids.shape[1], V, int(rest), float(alpha), float(temperature), int(ignore_index), ptr(loss),
+             ptr(stats), ptr(teacher), stream_ptr())
+    return loss, (stats, teacher)
+
+
+def distill_bwd(gy: torch.Tensor, logits: torch.Tensor, labels: torch.Tensor | None, ids: torch.Tensor, values: torch.Tensor, saved, *,
+                alpha: float = 1.0, temperature: float = 1.0, rest: bool = False, ignore_index: int = -100, out: torch.Tensor | None = None):
+    """Gradient of the logits (their type) from that of the per-token losses ``gy [T]``; ``out`` may be the logits themselves."""
+    _distill_check(logits, labels, ids, values, alpha, temperature, rest)
+    T, V = logits.shape
+    if gy.shape != (T,) or gy.device != logits.device:
+        raise ValueError(f"distill: gradient [{T}] of the losses, not {list(gy.shape)} on {gy.device}")
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or out.stride(1) != 1):
+        raise ValueError("distill: out is like the logits, with contiguous rows")
+    if not use_kernels(logits):
+        g = _distill_plain_grad(gy, logits, labels, ids, values, alpha, temperature, rest, ignore_index).to(logits.dtype)
+        return g if out is None else out.copy_(g)
+    src = logits if logits.stride(1) == 1 else logits.contiguous()
+    if out is None:
+        out = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
+    labels = None if labels is None else labels.to(torch.int64).contiguous()
+    ids, values = ids.contiguous(), (values.float() if values.dtype == torch.float16 else values).contiguous()
+    gy = gy.float().contiguous()
+    stats, teacher = saved
+    with _lib.on_device_of(logits):
+        call("b200_distill_bwd", ptr(src), int(src.dtype == BF16), src.stride(0), ptr(labels), ptr(ids), int(ids.dtype == torch.int64), ptr(values),
+             int(values.dtype == BF16), T, ids.shape[1], V, int(rest), float(alpha), float(temperature), int(ignore_index), ptr(stats), ptr(teacher),
+             ptr(gy), ptr(out), out.stride(0), stream_ptr())
+    return out
+
+
+# --------------------------------------------------------------------------------------
 # optimizer
 # --------------------------------------------------------------------------------------
 def sumsq(g: torch.Tensor, out: torch.Tensor, accumulate: bool = False) -> torch.Tensor:
