@@ -154,6 +154,9 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_attn_delta": [P, P, P, I, I, I, I, L, L, L, L, P],
         "b200_attn_bwd": [P] * 9 + [I] * 6 + [L] * 12 + [F, I, I, I, P, L, P],
         "b200_attn_bwd_plan": [I] * 8 + [P],
+        "b200_attn_mask": [P, I, P, I, I, I, I, I, P, P],
+        "b200_attn_masked_fwd": [P] * 9 + [I] * 6 + [L] * 6 + [F, F, P],
+        "b200_attn_masked_bwd": [P] * 13 + [I] * 6 + [L] * 10 + [F, F, P, L, P],
     }
     codes = {P: "P", I: "I", L: "L", F: "F", ctypes.c_ulonglong: "U"}
     table = {}
@@ -175,6 +178,11 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.b200_hstu_gate_cat_scratch_elems.restype = c_ll
     lib.b200_norm_bwd_scratch_elems.restype = c_ll
     lib.b200_sumsq_scratch_elems.restype = c_int
+    if hasattr(lib, "b200_attn_mask_ints"):
+        lib.b200_attn_mask_ints.argtypes = [I, I, I]
+        lib.b200_attn_mask_ints.restype = c_ll
+        lib.b200_attn_masked_bwd_workspace.argtypes = [I, I, I, I]
+        lib.b200_attn_masked_bwd_workspace.restype = c_ll
     if hasattr(lib, "b200_route_stores_counts"):
         lib.b200_route_stores_counts.argtypes = [I]
         lib.b200_route_stores_counts.restype = c_int

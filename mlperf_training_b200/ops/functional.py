@@ -16,6 +16,8 @@ from torch.autograd import Function, forward_ad
 
 from . import kernels as K
 from . import linear as L
+from . import masked_attention as MA
+from .masked_attention import AttentionMask, attention_mask  # noqa: F401 - a mask is made once and used by masked_attention
 from ._lib import call, ptr, stream_ptr, use_kernels
 
 
@@ -600,6 +602,81 @@ def attention(q, k, v, *, causal=True, window=0, sink=None, scale=None):
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     return _apply(AttentionBSHDFn, q, k, v, sink, causal, window, scale)
+
+
+class MaskedAttentionFn(Function):
+    """Attention on ``[B, S, H, D]`` tensors under an ``AttentionMask``."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, sink, slopes, mask, softcap, scale):
+        out, lse, low = MA.masked_attention_fwd(q, k, v, mask, scale=scale, softcap=softcap, slopes=slopes, sink=sink,
+                                                for_backward=any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, out, lse, low, sink, slopes)
+        ctx.cfg = (mask, softcap, scale)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, low, sink, slopes = ctx.saved_tensors
+        mask, softcap, scale = ctx.cfg
+        dq, dk, dv, dsink = MA.masked_attention_bwd(dout, q, k, v, out, low, lse, mask, scale=scale, softcap=softcap, slopes=slopes, sink=sink)
+        return dq.to(q.dtype), dk, dv, (None if dsink is None else dsink.to(sink.dtype)), None, None, None, None
+
+
+def masked_attention(q, k, v, mask, *, softcap=0.0, slopes=None, sink=None, scale=None):
+    """Attention of ``q [B, Sq, Hq, D]`` over ``k``, ``v`` ``[B, Skv, Hkv, D]`` (bf16, D 64 or 128 on the GPU; any strides) under ``mask``, made by
+    ``attention_mask`` for (B, Sq, Skv).  A score is ``scale`` times the product; ``softcap`` makes it ``softcap * tanh(score / softcap)``;
+    ``slopes [Hq]`` (constants) take ``slope * |distance|`` from it; ``sink [Hq]`` adds a logit without a value to each row.  Rows that
+    see nothing give 0 and get no gradient.  Values of padding may be anything in the forward pass; the backward pass wants finite
+    inputs everywhere."""
+    MA.constant_slopes(slopes)
+    return _apply(MaskedAttentionFn, q, k, v, sink, slopes, mask, softcap, scale)
+
+
+class MaskedAttentionPackedFn(Function):
+    """Rotary embedding and masked attention on a packed ``[T, (Hq + 2 Hkv) * D]`` buffer, as ``AttentionFn`` has them."""
+
+    @staticmethod
+    def forward(ctx, qkv, sink, slopes, cos, sin, mask, Hq, Hkv, D, softcap, scale):
+        qkv = qkv.contiguous()
+        if cos is not None:
+            K.rope_(qkv, cos, sin, col0=0, n_heads=Hq + Hkv, head_dim=D, seq_len=mask.Sq)
+        q, k, v = _split_packed(qkv, mask, Hq, Hkv, D)
+        out, lse, low = MA.masked_attention_fwd(q, k, v, mask, scale=scale, softcap=softcap, slopes=slopes, sink=sink,
+                                                for_backward=any(ctx.needs_input_grad))
+        ctx.save_for_backward(qkv, out, lse, low, sink, slopes, cos, sin)
+        ctx.cfg = (mask, Hq, Hkv, D, softcap, scale)
+        return out.view(qkv.shape[0], Hq * D)
+
+    @staticmethod
+    def backward(ctx, dout):
+        qkv, out, lse, low, sink, slopes, cos, sin = ctx.saved_tensors
+        mask, Hq, Hkv, D, softcap, scale = ctx.cfg
+        q, k, v = _split_packed(qkv, mask, Hq, Hkv, D)
+        dqkv = torch.empty_like(qkv)
+        gq, gk, gv = _split_packed(dqkv, mask, Hq, Hkv, D)
+        dq, _, _, dsink = MA.masked_attention_bwd(dout.contiguous().view(out.shape), q, k, v, out, low, lse, mask, scale=scale, softcap=softcap,
+                                                  slopes=slopes, sink=sink, dk_out=gk, dv_out=gv)
+        if cos is not None:
+            K.rope_grad_(dq, dqkv, cos, sin, n_heads=Hq, n_kv_heads=Hkv, head_dim=D, seq_len=mask.Sq)
+        else:
+            gq.copy_(dq)
+        return (dqkv, None if dsink is None else dsink.to(sink.dtype)) + (None,) * 9
+
+
+def _split_packed(qkv, mask, Hq, Hkv, D):
+    v3 = qkv.view(mask.B, mask.Sq, -1)
+    q, k, v = v3.split([Hq * D, Hkv * D, Hkv * D], -1)
+    return q.unflatten(-1, (Hq, D)), k.unflatten(-1, (Hkv, D)), v.unflatten(-1, (Hkv, D))
+
+
+def masked_attention_packed(qkv, mask, *, Hq, Hkv, D, cos=None, sin=None, sink=None, softcap=0.0, slopes=None, scale=None):
+    """``attention_packed`` under an ``AttentionMask`` of ``Sq = Skv`` positions, with ``masked_attention``'s scores."""
+    if mask.Sq != mask.Skv or qkv.dim() != 2 or qkv.shape != (mask.B * mask.Sq, (Hq + 2 * Hkv) * D):
+        raise ValueError(f"masked_attention_packed: [{mask.B * mask.Sq}, {(Hq + 2 * Hkv) * D}] for a mask of {mask.B} x {mask.Sq} x {mask.Skv}, not "
+                         f"{list(qkv.shape)}")
+    MA.constant_slopes(slopes)
+    return _apply(MaskedAttentionPackedFn, qkv, sink, slopes, cos, sin, mask, Hq, Hkv, D, softcap, scale)
 
 
 class EmbeddingFn(Function):
