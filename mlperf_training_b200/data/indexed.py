@@ -154,6 +154,16 @@ class PackedSFTDataset:
         starts = np.asarray(row.get("seq_start_id", [0]), dtype=np.int64)
         return torch.from_numpy(tokens.copy()), torch.from_numpy(labels), torch.from_numpy(starts)
 
+    def documents(self, step: int, rank: int, world: int, local_batch: int) -> torch.Tensor:
+        """Ids ``[local_batch, seq_len]`` of the packed documents of ``batch``'s tokens, from ``seq_start_id``; -1 behind the last."""
+        base, out = (step * world + rank) * local_batch, torch.full((local_batch, self.seq_len), -1, dtype=torch.int64)
+        for k in range(local_batch):
+            row = self.rows[(base + k) % len(self.rows)]
+            n = min(len(row["input_ids"]), self.seq_len)
+            starts = np.sort(np.asarray(row.get("seq_start_id", [0]), dtype=np.int64))
+            out[k, :n] = torch.from_numpy(np.searchsorted(starts, np.arange(n), side="right"))
+        return out
+
     def batch(self, step: int, rank: int, world: int, local_batch: int):
         base = (step * world + rank) * local_batch
         items = [self[base + k] for k in range(local_batch)]

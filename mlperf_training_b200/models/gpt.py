@@ -41,11 +41,22 @@ class GPTConfig:
     window: int = 0                 # sliding-window length (0 = full attention)
     window_layers: str = "none"     # "none" | "even" | "all": which layers use the window
     sink: bool = False              # learned per-head sink logits
+    attn_softcap: float = 0.0       # scores become softcap * tanh(score / softcap) (0 = as they are)
+    attn_alibi: bool = False        # a bias of -2^(-8 h / n_heads) a position of distance, h = 1 .. n_heads, in the place of the rotary embedding
     # mixture of experts (0 experts = dense MLP)
     n_experts: int = 0
     top_k: int = 0
     moe_ffn_hidden: int = 0
     router_dtype: str = "fp32"
+    # routing (ops.moe_ops.route; as they stand: softmax over the top-k logits): scores "softmax" over all experts or "sigmoid", experts in
+    # groups of which the best router_top_groups take part (0 = all), weights divided by their sum, times router_scale; a rate above 0
+    # gives every router a balance bias that selects and moves by it after each optimizer step
+    router_score: str = "softmax"
+    router_groups: int = 1
+    router_top_groups: int = 0
+    router_renormalize: bool = True
+    router_scale: float = 1.0
+    router_bias_rate: float = 0.0
     ep_comm: str = "nccl"          # expert-parallel token movement: "nccl" all-to-all | "fused" peer-memory kernels
     # LoRA (rank 0 = off)
     lora_rank: int = 0
@@ -79,6 +90,16 @@ class GPTConfig:
         if self.window_layers == "all":
             return self.window
         return self.window if layer % 2 == 0 else 0
+
+    @property
+    def plain_router(self) -> bool:
+        """Softmax over the selected logits and nothing else (``ops.moe_ops.router_topk``)."""
+        return (self.router_score == "softmax" and self.router_top_groups in (0, self.router_groups) and self.router_renormalize
+                and self.router_scale == 1.0 and self.router_bias_rate <= 0.0)
+
+    @property
+    def plain_scores(self) -> bool:
+        return self.attn_softcap <= 0.0 and not self.attn_alibi
 
     def num_params(self) -> int:
         d, hd = self.hidden, self.head_dim
@@ -210,6 +231,8 @@ class Block(nn.Module):
         d, hd = cfg.hidden, cfg.head_dim
         self.tp = tp if (tp is not None and tp.world > 1) else None
         W = self.tp.world if self.tp is not None else 1
+        if self.tp is not None and not cfg.plain_scores:
+            raise NotImplementedError("tensor-parallel blocks do not carry capped scores or a distance bias")
         if cfg.n_heads % W or cfg.n_kv_heads % W:
             raise ValueError(f"heads {cfg.n_heads}/{cfg.n_kv_heads} are not divisible by the tensor-parallel size {W}")
         self.hq, self.hkv = cfg.n_heads // W, cfg.n_kv_heads // W
@@ -290,7 +313,18 @@ class Block(nn.Module):
             a = context_parallel_attention(q, k, v, group, window=window)
         return a.reshape(B * S, Hq * D)
 
-    def forward(self, x, cos, sin, B, S):
+    def _attention_masked(self, qkv, cos, sin, B, S, mask):
+        cfg = self.cfg
+        if mask is None:                 # (a pipeline stage's blocks: causal, with the layer's window)
+            mask = F.attention_mask(B, S, window=cfg.layer_window(self.layer), device=qkv.device)
+        slopes = None
+        if cfg.attn_alibi:
+            cos = sin = None
+            slopes = torch.exp2(-8.0 * torch.arange(1, cfg.n_heads + 1, dtype=torch.float32, device=qkv.device) / cfg.n_heads)
+        return F.masked_attention_packed(qkv, mask, Hq=cfg.n_heads, Hkv=cfg.n_kv_heads, D=cfg.head_dim, cos=cos, sin=sin, sink=self.sink,
+                                         softcap=cfg.attn_softcap, slopes=slopes)
+
+    def forward(self, x, cos, sin, B, S, mask=None):
         cfg = self.cfg
         if self.tp is not None:
             return self._forward_tp(x, cos, sin, B, S)
@@ -302,6 +336,8 @@ class Block(nn.Module):
             qkv = F.linear(xn, self.w_qkv, None, self.lora_qkv(xn), pr)      # adapter output joins in the GEMM epilogue
         if self.cp is not None:
             a = self._attention_cp(qkv, cos, sin, B, S)
+        elif mask is not None or not cfg.plain_scores:
+            a = self._attention_masked(qkv, cos, sin, B, S, mask)
         else:
             a = F.attention_packed(qkv, B=B, S=S, Hq=cfg.n_heads, Hkv=cfg.n_kv_heads, D=cfg.head_dim, cos=cos, sin=sin,
                                    sink=self.sink, causal=True, window=cfg.layer_window(self.layer))
@@ -313,7 +349,11 @@ class Block(nn.Module):
 
 
 class GPT(nn.Module):
-    """``forward(tokens [B,S], labels [B,S]) -> mean cross-entropy`` (labels -100 are ignored)."""
+    """``forward(tokens [B,S], labels [B,S]) -> mean cross-entropy`` (labels -100 are ignored).
+
+    ``documents [B,S]`` and ``prefix [B,S]`` (see ``ops.functional.attention_mask``) keep the attention of packed samples inside their documents
+    and let prompts see themselves both ways.  ``teacher = (ids, values)``, ``[B,S,K]`` each, puts ``ops.functional.distill_loss`` in the
+    place of the cross-entropy, with the arguments in ``distill`` (``alpha``, ``temperature``, ``rest``)."""
 
     def __init__(self, cfg: GPTConfig, device="cpu", seed: int = 0, ep_group=None, tp=None):
         super().__init__()
@@ -397,8 +437,8 @@ class GPT(nn.Module):
             for blk in self.blocks:
                 blk.cp = None
             return
-        if self.cfg.sink:
-            raise NotImplementedError("context parallelism does not carry attention sink logits")
+        if self.cfg.sink or not self.cfg.plain_scores:
+            raise NotImplementedError("context parallelism does not carry attention sink logits, capped scores or a distance bias")
         if mode not in ("allgather", "ulysses", "ring"):
             raise ValueError(f"unknown context-parallel mode '{mode}'")
         self.cp = (group, dist.get_world_size(group), dist.get_rank(group))
@@ -406,8 +446,54 @@ class GPT(nn.Module):
         for blk in self.blocks:
             blk.cp = (group, mode)
 
-    def forward(self, tokens: torch.Tensor, labels: torch.Tensor, n_valid: int | None = None) -> torch.Tensor:
+    def routers(self):
+        """MLPs with a balance bias, by block."""
+        return [blk.mlp for blk in self.blocks if getattr(blk.mlp, "router_bias", None) is not None]
+
+    @torch.no_grad()
+    def balance_routers(self, groups=()) -> None:
+        """One step of the routers' balance biases from the load since the last one, summed over the process ``groups`` that
+        share the routers.  Called after an optimizer step."""
+        import torch.distributed as dist
+        mlps = self.routers()
+        if not mlps:
+            return
+        load = torch.stack([m.router_load for m in mlps])
+        for g in groups:
+            dist.all_reduce(load, group=g)
+        for m, n in zip(mlps, load):
+            m.balance(n)
+
+    def router_state(self) -> list:
+        return [m.router_bias.detach().to("cpu", copy=True) for m in self.routers()]
+
+    @torch.no_grad()
+    def load_router_state(self, state: list) -> None:
+        mlps = self.routers()
+        if len(state) != len(mlps):
+            raise ValueError(f"{len(state)} balance biases for {len(mlps)} routers")
+        for m, b in zip(mlps, state):
+            m.router_bias.copy_(b.to(m.router_bias.device))
+            m.router_load.zero_()
+
+    def _masks(self, B, S, documents, prefix, device):
+        """The attention mask of each layer, or Nones: one is made for each window that the layers have."""
+        if documents is None and prefix is None and self.cfg.plain_scores:
+            return [None] * len(self.blocks)
+        if (documents is not None or prefix is not None) and (self.tp is not None or self.cp is not None):
+            raise NotImplementedError("document and prefix masks run without tensor or context parallelism")
+        if self.cp is not None or self.tp is not None:
+            return [None] * len(self.blocks)
+        windows = [self.cfg.layer_window(i) for i in range(len(self.blocks))]
+        made = {w: F.attention_mask(B, S, window=w, documents=documents, prefix=prefix, device=device) for w in sorted(set(windows))}
+        return [made[w] for w in windows]
+
+    def forward(self, tokens: torch.Tensor, labels: torch.Tensor, n_valid: int | None = None, documents: torch.Tensor | None = None,
+                prefix: torch.Tensor | None = None, teacher: tuple | None = None, distill: dict | None = None) -> torch.Tensor:
         B, S = tokens.shape
+        masks = self._masks(B, S, documents, prefix, tokens.device)
+        if teacher is not None and self.tp is not None:
+            raise NotImplementedError("distillation runs without tensor parallelism")
         cos, sin = self.rope(tokens.device)
         if self.cp is not None:
             _, W, r = self.cp
@@ -455,14 +541,18 @@ class GPT(nn.Module):
                 hooks.pre_forward(i)
             if ckpt and (self.cfg.recompute_layers <= 0 or i < self.cfg.recompute_layers):
                 from torch.utils.checkpoint import checkpoint
-                x = checkpoint(blk, x, cos, sin, B, S, use_reentrant=False)
+                x = checkpoint(blk, x, cos, sin, B, S, masks[i], use_reentrant=False)
             elif offload and (self.cfg.recompute_layers <= 0 or i < self.cfg.recompute_layers):
                 # keep what this block saves for backward in (pinned) host memory instead of on the device
                 with torch.autograd.graph.save_on_cpu(pin_memory=x.is_cuda):
-                    x = blk(x, cos, sin, B, S)
+                    x = blk(x, cos, sin, B, S, masks[i])
             else:
-                x = blk(x, cos, sin, B, S)
+                x = blk(x, cos, sin, B, S, masks[i])
         if hooks is not None and torch.is_grad_enabled() and x.requires_grad:
             x.register_hook(lambda g, h=hooks, i=n_blocks - 1: h.pre_backward(i))
+        if teacher is not None:
+            ids_t, values = (t.reshape(B * S, -1) for t in teacher)
+            return F.lm_head_distill_loss(x, self.final_norm, self.lm_head, tgt, ids_t, values, eps=self.cfg.norm_eps, n_valid=n_valid,
+                                          precision=self.cfg.precision, **(distill or {}))
         return F.lm_head_loss(x, self.final_norm, self.lm_head, tgt, eps=self.cfg.norm_eps,
                               n_valid=n_valid, precision=self.cfg.precision)

@@ -38,13 +38,24 @@ class MoEMLP(nn.Module):
             self.w1.expert_shard = self.w2.expert_shard = (self.ep, self.ep_rank)
         self.dispatcher = ExpertParallelDispatcher(ep_group, E) if self.ep > 1 else None
         self.ep_comm = ep_comm
+        # a balance bias selects experts beside their scores; the load since its last step is counted while gradients are on
+        balanced = cfg.router_bias_rate > 0
+        self.register_buffer("router_bias", torch.zeros(E, dtype=torch.float32, device=device) if balanced else None, persistent=False)
+        self.register_buffer("router_load", torch.zeros(E, dtype=torch.int32, device=device) if balanced else None, persistent=False)
         self._fused = None      # built on first use: its slab size depends on the number of tokens per step
 
     def forward(self, h, norm_w, eps):
         cfg = self.cfg
         hn = F.rms_norm(h, norm_w, eps)
         logits = F.router_logits(hn, self.router)          # fp32 logits on the tcgen05 GEMM (split-precision weight)
-        idx, w, counts = M.RouterFn.apply(logits, cfg.top_k)
+        if cfg.plain_router:
+            idx, w, counts = M.RouterFn.apply(logits, cfg.top_k)
+        else:
+            idx, w, counts = M.route(logits, cfg.top_k, score=cfg.router_score, bias=self.router_bias, groups=cfg.router_groups,
+                                     top_groups=cfg.router_top_groups or cfg.router_groups, renormalize=cfg.router_renormalize,
+                                     scale=cfg.router_scale)
+            if self.router_load is not None and torch.is_grad_enabled():
+                self.router_load += counts          # (twice where the block is recomputed, for every expert alike)
         prec = M.expert_precision(getattr(cfg, "precision", "bf16"), self.w1, self.w2)
         if self.dispatcher is None:
             return M.moe_experts(hn, idx, w, counts, self.w1, self.w2, prec, residual=h)
@@ -54,6 +65,11 @@ class MoEMLP(nn.Module):
         else:
             y = self.dispatcher(hn, idx, w, counts, self.w1, self.w2, prec)
         return h + y
+
+    def balance(self, load: torch.Tensor) -> None:
+        """One step of the balance bias from ``load`` (int32 ``[E]``), after which counting starts anew."""
+        M.balance_bias(self.router_bias, load.contiguous(), self.cfg.router_bias_rate, out=self.router_bias)
+        self.router_load.zero_()
 
     _shared: dict = {}
 

@@ -97,8 +97,8 @@ class GPTStage(nn.Module):
             for blk in self.blocks:
                 blk.cp = None
             return
-        if self.cfg.sink:
-            raise NotImplementedError("context parallelism does not carry attention sink logits")
+        if self.cfg.sink or not self.cfg.plain_scores:
+            raise NotImplementedError("context parallelism does not carry attention sink logits, capped scores or a distance bias")
         if mode not in ("allgather", "ulysses", "ring"):
             raise ValueError(f"unknown context-parallel mode '{mode}'")
         self.cp = (group, dist.get_world_size(group), dist.get_rank(group), mode)

@@ -85,6 +85,7 @@ class RunConfig:
     grad_reduce_in_bf16: bool = False                   # gradients cross the wire in bf16 (library-collective engine)
     eod_mask_loss: bool = False
     eod_token: int = 128001                              # <|end_of_text|> of the Llama-3 tokenizer
+    document_mask: bool = False                         # attention inside documents: of packed samples, else behind each eod_token
     precision_schedule: dict | str | None = None        # ops.recipe.PrecisionSchedule spec (phase switch at a step)
     vanish_at_step: int = 0                             # fault injection: rank ``vanish_rank`` leaves silently before this step
     vanish_rank: int = 1
@@ -142,6 +143,12 @@ def eod_masked(batch, eod_token: int):
         x, y = batch[:, :-1].contiguous(), batch[:, 1:].clone()
     y[x == eod_token] = -100
     return x, y
+
+
+def document_ids(tokens: torch.Tensor, eod_token: int) -> torch.Tensor:
+    """Number of end-of-document tokens before each position of ``tokens [b, S]``: an id for the document that it is in."""
+    ends = (tokens == eod_token).to(torch.int64)
+    return torch.cumsum(ends, dim=1) - ends
 
 
 def eval_spec(rc: "RunConfig") -> dict:
@@ -241,6 +248,8 @@ def run(exp: dict, device: str | None = None, stream=None) -> dict:
         dp_group = mesh.group("dp_shard") if replicate > 1 else mesh.group("dp")
         if cfg.precision != "bf16":
             cfg.precision = "bf16"       # everything outside the tensor-parallel linears stays bf16
+    if rc.document_mask and (pp_size > 1 or tp_size > 1 or cp_size > 1):
+        raise NotImplementedError("document_mask runs without pipeline, tensor or context parallelism")
     cp_group = ep_group = edp_group = None
     if ep_size > 1:
         others = (tp_size > 1) + (pp_size > 1) + (cp_size > 1)
@@ -320,10 +329,14 @@ def run(exp: dict, device: str | None = None, stream=None) -> dict:
     def host_batch(ds, i):
         """One step's batch for this data-parallel rank: tokens ``[b, S+1]``, or (tokens, labels)."""
         b = ds.batch(i, dp_rank, dp_world, local_batch)
+        packed = ds.documents(i, dp_rank, dp_world, local_batch) if rc.document_mask and hasattr(ds, "documents") else None
         if not isinstance(b, (tuple, list)) and getattr(ds, "loss_last", 0) > 0:
             b = (b[:, :-1].contiguous(), ds.labels(b))
         if rc.eod_mask_loss:
             b = eod_masked(b, int(rc.eod_token))
+        if rc.document_mask:
+            x, y = b if isinstance(b, (tuple, list)) else (b[:, :-1].contiguous(), b[:, 1:].contiguous())
+            b = (x, y, packed if packed is not None else document_ids(x, int(rc.eod_token)))
         return b
 
     # pipeline stages, expert shards and tensor-parallel slices differ per rank: those parameters travel
@@ -338,6 +351,8 @@ def run(exp: dict, device: str | None = None, stream=None) -> dict:
     if resuming:
         ck = resume_mgr.load()
         # pipeline stages and expert shards differ per rank: their parameters travel with the rank's optimizer shard
+        if ck["dense"] is not None and ck["dense"].get("router_bias"):
+            trainer.model.load_router_state(ck["dense"]["router_bias"])
         bufs = ck["optim"].get("stage_param_bufs") if (per_rank_params and ck["optim"] is not None) else ck["dense"]["param_bufs"]
         written_by = int(ck["meta"].get("world", world))
         if written_by != world and not per_rank_params:
@@ -476,7 +491,7 @@ def run(exp: dict, device: str | None = None, stream=None) -> dict:
                 for i in range(max(rc.eval_iters, 1)):
                     eb = host_batch(eval_data, i)
                     if isinstance(eb, tuple):
-                        sums += trainer.eval_sums(eb[0].to(trainer.device), eb[1].to(trainer.device))
+                        sums += trainer.eval_sums(*(t.to(trainer.device) for t in eb))
                     else:
                         sums += trainer.eval_sums(eb.to(trainer.device))
                 last_eval = float(sums[0] / sums[1].clamp(min=1))
@@ -496,7 +511,8 @@ def run(exp: dict, device: str | None = None, stream=None) -> dict:
                     else resume_mgr.save
                 saver(step + 1,
                                 dense={"param_bufs": [b.param_buf.detach().cpu() for b in trainer.engine.buckets],
-                                       "model_config": cfg.to_dict()},
+                                       "model_config": cfg.to_dict(),
+                                       "router_bias": trainer.model.router_state() if cfg.router_bias_rate > 0 else None},
                                 optim_shard=dict(_optim_shard(trainer, per_rank_params),
                                                  deosc=deosc.state_dict() if deosc is not None else None),
                                 meta={"samples": samples, "run_started": True, "window": 0, "batch_idx_in_window": -1,

@@ -35,6 +35,8 @@ def _chunk_bucket_of(name: str) -> str:
 class PipelineTrainer:
     def __init__(self, model_cfg: GPTConfig, opt: OptimConfig, train: TrainConfig, device, mesh, virtual_stages: int = 1,
                  freeze_base: bool = False, tp=None, ep_group=None, expert_dp_group=None, cp_group=None, cp_mode: str = "allgather"):
+        if model_cfg.router_bias_rate > 0:
+            raise NotImplementedError("pipeline stages do not move a router's balance bias")
         self.cfg, self.train_cfg = model_cfg, train
         self.device = torch.device(device)
         self.mesh = mesh

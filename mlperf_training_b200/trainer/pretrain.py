@@ -34,6 +34,7 @@ class TrainConfig:
     seed: int = 0
     comm: str = "nccl"
     zero_stage: int = 1             # 1: optimizer state sharded, parameters replicated; 3: block matrices sharded too
+    distill: dict | None = None     # alpha, temperature, rest of the loss of steps that are given a teacher's logits
 
 
 class PretrainTrainer:
@@ -102,7 +103,7 @@ class PretrainTrainer:
             return zigzag_chunk(t, self.cp_world, self.cp_rank, dim=1)
         return t[:, self.cp_rank * s:(self.cp_rank + 1) * s].contiguous()
 
-    def _loss(self, x: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
+    def _loss(self, x: torch.Tensor, y: torch.Tensor, documents=None, teacher=None) -> torch.Tensor:
         # explicit labels mask part of the positions (-100): the mean runs over the labelled ones.  With the
         # sequence sharded, every chunk divides by its share of the count, so that the average of the chunks'
         # losses (which is what the gradient reduction forms) is the mean over the whole sequence.
@@ -110,13 +111,31 @@ class PretrainTrainer:
         n_valid = max(int((y != -100).sum()), 1) / self.cp_world if masked else None
         if n_valid is not None and self.cp_group is None:
             n_valid = int(n_valid)
-        loss = self.model(self._chunk(x), self._chunk(y), n_valid=n_valid)
+        more = {}
+        if documents is not None:
+            more["documents"] = documents
+        if teacher is not None:
+            if self.cp_group is not None:
+                raise NotImplementedError("distillation runs without context parallelism")
+            more.update(teacher=teacher, distill=self.train_cfg.distill)
+        loss = self.model(self._chunk(x), self._chunk(y), n_valid=n_valid, **more)
         return loss
 
-    def train_step_device(self, tokens: torch.Tensor, labels: torch.Tensor | None = None) -> torch.Tensor:
+    def _router_groups(self) -> list:
+        """Process groups over which the load of a router is summed: all ranks that route tokens of their own through it."""
+        if not (dist.is_available() and dist.is_initialized()):
+            return []
+        groups = [self.dp_group if self.dp_group is not None else dist.group.WORLD] if (self.dp_group is not None or self.tp is None) else []
+        groups += [g for g in (self.replicate_group, self.tp.group if self.tp is not None else None) if g is not None]
+        return [g for g in groups if dist.get_world_size(g) > 1]
+
+    def train_step_device(self, tokens: torch.Tensor, labels: torch.Tensor | None = None, documents: torch.Tensor | None = None,
+                          teacher: tuple | None = None) -> torch.Tensor:
         """``tokens``: int64 ``[local_batch, seq_len + 1]`` on the device (or ``[local_batch, seq_len]``
         with explicit ``labels``, -100 = no loss).  Returns the mean loss over the step's micro-batches
-        as a 0-d device tensor (summed over the tensor-parallel group when there is one)."""
+        as a 0-d device tensor (summed over the tensor-parallel group when there is one).
+        ``documents [local_batch, seq_len]`` keeps the attention inside documents, ``teacher = (ids, values)``,
+        ``[local_batch, seq_len, K]`` each, distils (``TrainConfig.distill``): see ``models.gpt.GPT``."""
         mb = self.train_cfg.micro_batch
         self._masked = labels is not None
         x_all, y_all = self._split(tokens, labels)
@@ -127,12 +146,16 @@ class PretrainTrainer:
                 # reduce every block's gradients while the rest of this backward still runs
                 self.engine.begin_overlap()
                 self.model.grad_ready_hook = self.engine.on_block_grads_ready
-            loss = self._loss(x_all[i * mb:(i + 1) * mb], y_all[i * mb:(i + 1) * mb])
+            rows = slice(i * mb, (i + 1) * mb)
+            loss = self._loss(x_all[rows], y_all[rows], None if documents is None else documents[rows],
+                              None if teacher is None else tuple(t[rows] for t in teacher))
             loss.backward()
             self.model.grad_ready_hook = None
             d = loss.detach()
             total = d if total is None else total + d
         self.engine.step(self.lr(), grad_scale=1.0 / self.n_micro)
+        if self.cfg.router_bias_rate > 0:
+            self.model.balance_routers(self._router_groups())
         self.step_idx += 1
         total = total / self.n_micro
         if self.tp is not None:
@@ -155,15 +178,16 @@ class PretrainTrainer:
     def train_step(self, batch) -> float:
         """One optimizer step from host token ids ``[local_batch, seq_len + 1]`` (int64, ideally
         pinned), or a ``(tokens, labels)`` pair of ``[local_batch, seq_len]`` tensors for packed
-        fine-tuning data.  Host -> device copy, step, and a device -> host read of the loss."""
+        fine-tuning data, with the ids of its documents as a third where the attention is to stay inside them.  Host -> device copy, step, and a device -> host read of the loss."""
         if isinstance(batch, (tuple, list)):
-            loss = self.train_step_device(self._to_device(batch[0], 0), self._to_device(batch[1], 1))
+            documents = self._to_device(batch[2], 2) if len(batch) > 2 else None
+            loss = self.train_step_device(self._to_device(batch[0], 0), self._to_device(batch[1], 1), documents)
         else:
             loss = self.train_step_device(self._to_device(batch, 0))
         return float(loss.item())
 
     @torch.no_grad()
-    def eval_sums(self, tokens: torch.Tensor, labels: torch.Tensor | None = None) -> torch.Tensor:
+    def eval_sums(self, tokens: torch.Tensor, labels: torch.Tensor | None = None, documents: torch.Tensor | None = None) -> torch.Tensor:
         """Forward-only ``[sum of token losses, number of labelled tokens]`` on device tokens, summed
         over every rank: evaluation averages over tokens, not over micro-batches (the reference
         accumulates the same pair, llama2_sft/primus/src/llama2_custom.py:752-915)."""
@@ -173,7 +197,8 @@ class PretrainTrainer:
         for i in range(0, x_all.shape[0], mb):
             x, y = self._chunk(x_all[i:i + mb]), self._chunk(y_all[i:i + mb])
             n = (y != -100).sum()
-            l = self.model(x, y, n_valid=1)            # n_valid = 1: the plain sum of token losses
+            more = {} if documents is None else {"documents": documents[i:i + mb]}
+            l = self.model(x, y, n_valid=1, **more)    # n_valid = 1: the plain sum of token losses
             if self.tp is not None:
                 l = self.tp.all_reduce(l.float().clone())
             acc[0] += l.double()

@@ -49,6 +49,7 @@ def run_synthetic_warmup(trainer, train_steps: int = 2, eval_steps: int = 0, see
         return {"train_losses": [], "eval_losses": []}
     engine = trainer.engine
     snap = snapshot_engine(engine)
+    routers = trainer.model.router_state() if hasattr(trainer.model, "router_state") else []
     step_idx = trainer.step_idx
     dev = trainer.device
     gen = torch.Generator(device="cpu").manual_seed(seed)
@@ -63,6 +64,8 @@ def run_synthetic_warmup(trainer, train_steps: int = 2, eval_steps: int = 0, see
         toks = torch.randint(0, V, (trainer.train_cfg.micro_batch, S + 1), generator=gen).to(dev)
         report["eval_losses"].append(float(trainer.eval_loss(toks)))
     restore_engine(engine, snap)
+    if routers:
+        trainer.model.load_router_state(routers)
     trainer.step_idx = step_idx
     torch.set_rng_state(rng_state)
     if cuda_state is not None:
