@@ -1,9 +1,12 @@
 // Masks of attention as intervals (attn_mask.cuh) from document ids and prefix flags.
 //
-// A CTA per sequence scans its positions twice, 4096 at a time: from the end for the next start of a document and the next position without a
-// flag, then from the front for the start of the document, after which both intervals of a position are known.  Then a warp per tile of
-// 128 rows or keys gathers the range of tiles that it meets and the bounds within which all of it is visible.  A second launch
-// sorts the tiles of all sequences by that range, longest first, for the schedules of the attention kernels.
+// A CTA per sequence; a thread takes 16 neighbouring positions as bit masks (a document starts here, padding, flagged), so that the ends of
+// a document inside them are bit searches.  What lies outside comes from two scans over the threads: from the end, the next start and the next
+// position without a flag; from the front, the last start with the end of its prefix.  16384 positions go at a time; longer sequences are
+// walked once from the end before for what each such chunk has behind it.  Then the warps take tiles of 128 positions, write their
+// intervals and reduce the tables of the key tiles (and of the query tiles, where these lie on the same positions).  Then the tiles of all sequences
+// are sorted by their range, longest first, for the schedules of the attention kernels: by the same CTA for one sequence, else by a second launch.
+// 16384 positions: 32 us with a scan over 4096 positions at a time through global memory, now 9; 61 positions 5.
 #include "attn_mask.cuh"
 #include "runtime.h"
 
@@ -11,7 +14,7 @@ namespace {
 
 using b200::MaskLayout;
 
-constexpr int NT = 1024, PER = 4, CHUNK = NT * PER;
+constexpr int NT = 1024, PER = 16, CHUNK = NT * PER;
 constexpr int BINS = 2048;
 constexpr unsigned ALL = 0xffffffffu;
 
@@ -27,137 +30,154 @@ B200_DEVICE long long id_at(const MaskParams& p, long long i) {
   return p.ids64 ? reinterpret_cast<const long long*>(p.ids)[i] : (long long)reinterpret_cast<const int*>(p.ids)[i];
 }
 
-// Inclusive scan over the CTA's chunk (thread-major) in index order, from `carry`; MAXOP: running maximum, else running minimum from the end.
-template <bool MAXOP>
-B200_DEVICE void block_scan(int (&v)[PER], int carry, int* red) {
-  auto op = [](int a, int b) { return MAXOP ? max(a, b) : min(a, b); };
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (MAXOP) {
+// Bits of positions i0 + k: `start` of a document, `pad`, `flag`.  Positions that are not there: a start, padding, no flag.
+struct Bits { unsigned start, pad, flag; };
+B200_DEVICE Bits load_bits(const MaskParams& p, long long base, int i0, int S) {
+  Bits r = {0u, 0u, 0u};
+  const int n = max(min(S - i0, PER), 0);
+  if (p.ids != nullptr) {
+    long long id[PER];
+    const long long at = base + i0;
+    if (n == PER && !p.ids64 && ((uintptr_t)(reinterpret_cast<const int*>(p.ids) + at) & 15) == 0) {
 #pragma unroll
-    for (int i = 1; i < PER; ++i) v[i] = op(v[i], v[i - 1]);
-  } else {
+      for (int k = 0; k < PER; k += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(reinterpret_cast<const int*>(p.ids) + at + k);
+        id[k] = v.x; id[k + 1] = v.y; id[k + 2] = v.z; id[k + 3] = v.w;
+      }
+    } else {
 #pragma unroll
-    for (int i = PER - 2; i >= 0; --i) v[i] = op(v[i], v[i + 1]);
+      for (int k = 0; k < PER; ++k) id[k] = k < n ? id_at(p, at + k) : 0;
+    }
+    const int lane = threadIdx.x & 31;
+    long long before = __shfl_up_sync(ALL, id[PER - 1], 1);
+    if (lane == 0 && i0 > 0 && i0 <= S) before = id_at(p, at - 1);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if ((k == 0 ? before : id[k - 1]) != id[k]) r.start |= 1u << k;
+      if (id[k] < 0) r.pad |= 1u << k;
+    }
   }
-  int t = MAXOP ? v[PER - 1] : v[0];
-  const int none = MAXOP ? -1 : 0x7fffffff;
+  if (p.flags != nullptr) {
+    const uint8_t* f = p.flags + base + i0;
+    if (n == PER && ((uintptr_t)f & 15) == 0) {
+      const uint4 v = *reinterpret_cast<const uint4*>(f);
+      const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = MAXOP ? __shfl_up_sync(ALL, t, o) : __shfl_down_sync(ALL, t, o);
-    if (MAXOP ? lane >= o : lane + o < 32) t = op(t, u);
+      for (int k = 0; k < PER; ++k)
+        if ((w[k / 4] >> (k % 4 * 8)) & 0xffu) r.flag |= 1u << k;
+    } else {
+      for (int k = 0; k < n; ++k)
+        if (f[k]) r.flag |= 1u << k;
+    }
   }
-  __syncthreads();
-  if (lane == (MAXOP ? 31 : 0)) red[warp] = t;
-  __syncthreads();
-  int before = MAXOP ? __shfl_up_sync(ALL, t, 1) : __shfl_down_sync(ALL, t, 1);
-  if (lane == (MAXOP ? 0 : 31)) before = none;
-  before = op(before, carry);
-  if (MAXOP) { for (int w = 0; w < warp; ++w) before = op(before, red[w]); }
-  else { for (int w = warp + 1; w < NT / 32; ++w) before = op(before, red[w]); }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) v[i] = op(v[i], before);
+  if (i0 == 0) r.start |= 1u;
+  const unsigned gone = n < PER ? ~0u << n : 0u;               // positions behind the last
+  r.start |= gone;
+  r.pad |= gone;
+  r.flag &= ~gone;
+  return r;
 }
 
-__global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ MaskParams p) {
-  b200::begin_kernel();
-  __shared__ int red[NT / 32];
-  __shared__ int s_carry[2];
-  const MaskLayout& m = p.m;
-  const int b = blockIdx.x, S = m.Skv, off = m.Skv - m.Sq;
-  const long long base = (long long)b * S;
-  int2* q_iv = reinterpret_cast<int2*>(p.buf + m.q_iv) + (long long)b * m.Sp;
-  int2* k_iv = reinterpret_cast<int2*>(p.buf + m.k_iv) + (long long)b * m.Kp;
-  int2* next = reinterpret_cast<int2*>(p.buf + m.scratch) + base;     // (end of the document, next position without a flag)
-  auto starts = [&](int i) { return i == 0 || (p.ids != nullptr && id_at(p, base + i) != id_at(p, base + i - 1)); };
-  const int chunks = (S + CHUNK - 1) / CHUNK;
+// First position at or behind i0 + k that starts a document / that has no flag, within the thread's, else what lies behind.
+B200_DEVICE int next_start(const Bits& b, int i0, int k, int behind) {
+  const unsigned m = b.start & ((1u << PER) - 1u) & (~0u << k);
+  return k < PER && m ? i0 + __ffs(m) - 1 : behind;
+}
+B200_DEVICE int next_bare(const Bits& b, int i0, int k, int behind) {
+  const unsigned m = ~b.flag & ((1u << PER) - 1u) & (~0u << k);
+  return m ? i0 + __ffs(m) - 1 : behind;
+}
 
-  int end_carry = S, bare_carry = S;
-  for (int c = chunks - 1; c >= 0; --c) {
-    const int i0 = c * CHUNK + (int)threadIdx.x * PER;
-    int e[PER], f[PER];
+// (start << 32 | end of its prefix) for the start at i0 + k of a thread with `end` and `bare` behind it
+B200_DEVICE long long prefix_key(const Bits& b, int i0, int k, int end, int bare) {
+  return (long long)(i0 + k) << 32 | (long long)min(next_bare(b, i0, k, bare), next_start(b, i0, k + 1, end));
+}
+
+// Exclusive scans over the threads: running minimum from the end (two at once), running maximum from the front.  `carry` is what lies beyond
+// the chunk, and becomes what lies beyond the next one.
+B200_DEVICE void scan_back(int& a, int& b, int (&carry)[2], int (*red)[NT / 32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int v[2] = {a, b};
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int i = i0 + k;
-      e[k] = i + 1 < S && starts(i + 1) ? i + 1 : S;
-      f[k] = i < S && !(p.flags != nullptr && p.flags[base + i]) ? i : S;
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_down_sync(ALL, v[k], o);
+      if (lane + o < 32) v[k] = min(v[k], u);
     }
-    block_scan<false>(e, end_carry, red);
-    block_scan<false>(f, bare_carry, red);
+  __syncthreads();
+  if (lane == 0) { red[0][warp] = v[0]; red[1][warp] = v[1]; }
+  __syncthreads();
+  int out[2];
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
-      if (i0 + k < S) next[i0 + k] = make_int2(e[k], f[k]);
-    if (threadIdx.x == 0) { s_carry[0] = e[0]; s_carry[1] = f[0]; }
-    __syncthreads();
-    end_carry = s_carry[0];
-    bare_carry = s_carry[1];
+  for (int k = 0; k < 2; ++k) {
+    int w = red[k][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_down_sync(ALL, w, o);
+      if (lane + o < 32) w = min(w, u);
+    }
+    const int whole = __shfl_sync(ALL, w, 0);
+    int behind = __shfl_sync(ALL, w, min(warp + 1, 31));
+    if (warp == 31) behind = 0x7fffffff;
+    int mine = __shfl_down_sync(ALL, v[k], 1);
+    if (lane == 31) mine = 0x7fffffff;
+    out[k] = min(min(mine, behind), carry[k]);
+    carry[k] = min(whole, carry[k]);
+  }
+  a = out[0];
+  b = out[1];
+}
+B200_DEVICE long long scan_front(long long v, long long& carry, long long* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(ALL, v, o);
+    if (lane >= o) v = max(v, u);
   }
   __syncthreads();
-
-  int start_carry = 0;
-  for (int c = 0; c < chunks; ++c) {
-    const int i0 = c * CHUNK + (int)threadIdx.x * PER;
-    int s[PER];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) s[k] = i0 + k < S && starts(i0 + k) ? i0 + k : -1;
-    block_scan<true>(s, start_carry, red);
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int i = i0 + k;
-      if (i >= S) continue;
-      const int ds = s[k], de = next[i].x;
-      int lo = i, hi = i, first = i, end = i;                         // a negative id: nothing
-      if (p.ids == nullptr || id_at(p, base + i) >= 0) {
-        const int pe = p.flags != nullptr ? min(next[ds].y, de) : ds;
-        lo = p.window > 0 ? max(ds, i - p.window + 1) : ds;
-        hi = p.causal ? max(i + 1, pe) : de;
-        first = (!p.causal || i < pe) ? ds : i;
-        end = p.window > 0 && i < de - p.window ? i + p.window : de;
-      }
-      first = max(first - off, 0);                                    // as queries
-      end = max(end - off, 0);
-      k_iv[i] = first < end ? make_int2(first, end) : make_int2(max(i - off, 0), max(i - off, 0));
-      if (i >= off) q_iv[i - off] = make_int2(lo, hi);
-    }
-    if (threadIdx.x == NT - 1) s_carry[0] = s[PER - 1];
-    __syncthreads();
-    start_carry = s_carry[0];
-  }
-  for (int i = S + (int)threadIdx.x; i < m.Kp; i += NT) k_iv[i] = make_int2(0, 0);
-  for (int i = m.Sq + (int)threadIdx.x; i < m.Sp; i += NT) q_iv[i] = make_int2(0, 0);
+  if (lane == 31) red[warp] = v;
   __syncthreads();
+  long long w = red[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(ALL, w, o);
+    if (lane >= o) w = max(w, u);
+  }
+  const long long whole = __shfl_sync(ALL, w, 31);
+  long long before = __shfl_sync(ALL, w, max(warp - 1, 0));
+  if (warp == 0) before = -1;
+  long long mine = __shfl_up_sync(ALL, v, 1);
+  if (lane == 0) mine = -1;
+  const long long out = max(max(mine, before), carry);
+  carry = max(whole, carry);
+  return out;
+}
+static_assert(NT == 1024, "a lane for each warp");
 
-  // tiles: rows that are there, of either side
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nq = m.Sp / 128, nk = m.Kp / 128;
-  for (int t = warp; t < nq + nk; t += NT / 32) {
-    const bool of_q = t < nq;
-    const int tile = of_q ? t : t - nq, rows = of_q ? m.Sq : S;
-    const int2* iv = (of_q ? q_iv : k_iv) + tile * 128;
-    int lo_min = 0x7fffffff, hi_max = 0, lo_max = 0, hi_min = 0x7fffffff;
-    for (int r = lane; r < 128 && tile * 128 + r < rows; r += 32) {
-      const int2 v = iv[r];
-      if (v.x < v.y) { lo_min = min(lo_min, v.x); hi_max = max(hi_max, v.y); }
-      lo_max = max(lo_max, v.x);
-      hi_min = min(hi_min, v.x < v.y ? v.y : v.x);
-    }
+// What a tile of rows sees: of those that see something the first and last, and the bounds within which all see all.
+struct Tile {
+  int lo_min = 0x7fffffff, hi_max = 0, lo_max = 0, hi_min = 0x7fffffff;
+  B200_DEVICE void add(int lo, int hi) {
+    if (lo < hi) { lo_min = min(lo_min, lo); hi_max = max(hi_max, hi); }
+    lo_max = max(lo_max, lo);
+    hi_min = min(hi_min, lo < hi ? hi : lo);
+  }
+  B200_DEVICE void join() {                                   // over the warp
     lo_min = __reduce_min_sync(ALL, lo_min);
     hi_max = __reduce_max_sync(ALL, hi_max);
     lo_max = __reduce_max_sync(ALL, lo_max);
     hi_min = __reduce_min_sync(ALL, hi_min);
-    if (lane == 0) {
-      int4 o = make_int4(0, 0, lo_max, hi_min);
-      if (lo_min < hi_max) { o.x = lo_min / 128; o.y = (hi_max + 127) / 128; }
-      if (!of_q && tile * 128 + 128 > S) o.w = 0;                     // keys behind the last: always masked
-      (reinterpret_cast<int4*>(p.buf + (of_q ? m.qt : m.kt)) + (long long)b * (of_q ? nq : nk))[tile] = o;
-    }
   }
-}
+  B200_DEVICE int4 entry(bool cut) const {                     // cut: rows of the tile are not there (keys behind the last: always masked)
+    int4 o = make_int4(0, 0, lo_max, cut ? 0 : hi_min);
+    if (lo_min < hi_max) { o.x = lo_min / 128; o.y = (hi_max + 127) / 128; }
+    return o;
+  }
+};
 
-// CTA 0: pairs of query tiles, CTA 1: key tiles, by their number of tiles on the other side, most first (numbers above BINS - 1 alike).
-__global__ void __launch_bounds__(NT) attn_mask_order_kernel(const MaskLayout m, int* buf) {
-  b200::begin_kernel();
-  __shared__ int bins[BINS];
-  __shared__ int red[NT / 32];
-  const bool of_q = blockIdx.x == 0;
+// Pairs of query tiles or key tiles by their number of tiles on the other side, most first (numbers above BINS - 1 alike).
+B200_DEVICE void order_tiles(const MaskLayout& m, int* buf, bool of_q, int* bins, int* red) {
   const int n = of_q ? m.B * (m.Sp / 256) : m.B * (m.Kp / 128);
   const int4* t = reinterpret_cast<const int4*>(buf + (of_q ? m.qt : m.kt));
   int* out = buf + (of_q ? m.oq : m.ok);
@@ -179,14 +199,137 @@ __global__ void __launch_bounds__(NT) attn_mask_order_kernel(const MaskLayout m,
   }
   if (lane == 31) red[warp] = x;
   __syncthreads();
-  int at = x - a - c;
-  for (int w = 0; w < warp; ++w) at += red[w];
+  int w = red[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(ALL, w, o);
+    if (lane >= o) w += u;
+  }
+  const int before = __shfl_sync(ALL, w, max(warp - 1, 0));
+  const int at = x - a - c + (warp > 0 ? before : 0);
   bins[2 * threadIdx.x] = at;
   bins[2 * threadIdx.x + 1] = at + a;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += NT) out[atomicAdd(&bins[bin(i)], 1)] = i;      // (order within a bin: the schedule's alone)
+  __syncthreads();
 }
 static_assert(BINS == 2 * NT, "a thread scans two bins");
+
+__global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ MaskParams p) {
+  b200::begin_kernel();
+  __shared__ int red[2][NT / 32];
+  __shared__ long long red64[NT / 32];
+  __shared__ union {
+    int bins[BINS];
+    struct { long long cur[NT]; int2 behind[NT]; uint2 bits[NT]; } own;
+  } sh;
+  long long* s_cur = sh.own.cur;                                      // of each thread: start and prefix before it, what lies behind, its bits
+  int2* s_behind = sh.own.behind;
+  uint2* s_bits = sh.own.bits;
+  const MaskLayout& m = p.m;
+  const int b = blockIdx.x, S = m.Skv, off = m.Skv - m.Sq, nq = m.Sp / 128, nk = m.Kp / 128;
+  const long long base = (long long)b * S;
+  int2* q_iv = reinterpret_cast<int2*>(p.buf + m.q_iv) + (long long)b * m.Sp;
+  int2* k_iv = reinterpret_cast<int2*>(p.buf + m.k_iv) + (long long)b * m.Kp;
+  int4* qt = reinterpret_cast<int4*>(p.buf + m.qt) + (long long)b * nq;
+  int4* kt = reinterpret_cast<int4*>(p.buf + m.kt) + (long long)b * nk;
+  int2* behind = reinterpret_cast<int2*>(p.buf + m.scratch) + (long long)b * ((S + CHUNK - 1) / CHUNK);   // of chunk c: next start and next position without a flag
+  const int chunks = (S + CHUNK - 1) / CHUNK, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool same = off % 128 == 0;                                   // query tiles are key tiles
+
+  if (chunks > 1) {
+    int carry[2] = {S, S};
+    for (int c = chunks - 1; c >= 0; --c) {
+      if (threadIdx.x == 0) behind[c] = make_int2(carry[0], carry[1]);
+      const int i0 = c * CHUNK + (int)threadIdx.x * PER;
+      const Bits t = load_bits(p, base, i0, S);
+      int a = next_start(t, i0, 0, 0x7fffffff), e = next_bare(t, i0, 0, 0x7fffffff);
+      scan_back(a, e, carry, red);
+    }
+    __syncthreads();
+  }
+  long long front = 0;                                                // (start << 32 | end of its prefix)
+  for (int c = 0; c < chunks; ++c) {
+    const int i0 = c * CHUNK + (int)threadIdx.x * PER;
+    const Bits t = load_bits(p, base, i0, S);
+    int carry[2] = {S, S};
+    if (chunks > 1) { const int2 v = behind[c]; carry[0] = v.x; carry[1] = v.y; }
+    int end = next_start(t, i0, 0, 0x7fffffff), bare = next_bare(t, i0, 0, 0x7fffffff);
+    scan_back(end, bare, carry, red);                                 // behind this thread
+    end = min(end, S);
+    bare = min(bare, S);
+    const unsigned starts = t.start & (i0 < S ? (1u << PER) - 1u : 0u);
+    const int top = starts ? 31 - __clz(starts) : 0;
+    const long long cur = scan_front(starts ? prefix_key(t, i0, top, end, bare) : -1, front, red64);
+    // positions to warps: a tile of 128 at a time, so that neighbouring lanes write neighbouring intervals (each thread its own 16 would
+    // touch 32 lines a store, which took longer than all else: 16384 positions 16 us, now 9)
+    s_cur[threadIdx.x] = cur;
+    s_behind[threadIdx.x] = make_int2(end, bare);
+    s_bits[threadIdx.x] = make_uint2((t.start & 0xffffu) | t.pad << 16, t.flag);
+    __syncthreads();
+    for (int j = warp * 128; j < CHUNK && c * CHUNK + j < S; j += NT / 32 * 128) {
+      Tile tk, tq;
+#pragma unroll
+      for (int part = 0; part < 4; ++part) {
+        const int at = j + part * 32 + lane, i = c * CHUNK + at, owner = at / PER, k = at % PER, o0 = i - k;
+        if (i >= S) continue;
+        const uint2 w = s_bits[owner];
+        const int2 next = s_behind[owner];
+        const Bits u = {w.x & 0xffffu, w.x >> 16, w.y};
+        const unsigned mine = u.start & ((2u << k) - 1u);             // starts at or before this position
+        const long long key = mine ? prefix_key(u, o0, 31 - __clz(mine), next.x, next.y) : s_cur[owner];
+        const int ds = (int)(key >> 32), de = next_start(u, o0, k + 1, next.x);
+        int lo = i, hi = i, first = i, last = i;                      // padding: nothing
+        if (!(u.pad >> k & 1u)) {
+          const int pe = p.flags != nullptr ? (int)key : ds;
+          lo = p.window > 0 ? max(ds, i - p.window + 1) : ds;
+          hi = p.causal ? max(i + 1, pe) : de;
+          first = (!p.causal || i < pe) ? ds : i;
+          last = p.window > 0 && i < de - p.window ? i + p.window : de;
+        }
+        first = max(first - off, 0);                                  // as queries
+        last = max(last - off, 0);
+        if (first >= last) first = last = max(i - off, 0);
+        k_iv[i] = make_int2(first, last);
+        tk.add(first, last);
+        if (i >= off) {
+          q_iv[i - off] = make_int2(lo, hi);
+          tq.add(lo, hi);
+        }
+      }
+      tk.join();
+      if (same) tq.join();
+      const int i = c * CHUNK + j;
+      if (lane == 0) {
+        kt[i / 128] = tk.entry(i + 128 > S);
+        if (same && i >= off) qt[(i - off) / 128] = tq.entry(false);
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = S + (int)threadIdx.x; i < m.Kp; i += NT) k_iv[i] = make_int2(0, 0);
+  for (int i = m.Sq + (int)threadIdx.x; i < m.Sp; i += NT) q_iv[i] = make_int2(0, 0);
+  __syncthreads();
+  // query tiles on other positions than key tiles, and behind the last query
+  for (int t = (same ? (m.Sq + 127) / 128 : 0) + warp; t < nq; t += NT / 32) {
+    Tile v;
+    for (int r = t * 128 + lane; r < (t + 1) * 128 && r < m.Sq; r += 32) v.add(q_iv[r].x, q_iv[r].y);
+    v.join();
+    if (lane == 0) qt[t] = v.entry(false);
+  }
+  if (m.B == 1) {
+    __syncthreads();
+    order_tiles(m, p.buf, true, sh.bins, red[0]);
+    order_tiles(m, p.buf, false, sh.bins, red[0]);
+  }
+}
+
+__global__ void __launch_bounds__(NT) attn_mask_order_kernel(const __grid_constant__ MaskLayout m, int* buf) {
+  b200::begin_kernel();
+  __shared__ int bins[BINS];
+  __shared__ int red[NT / 32];
+  order_tiles(m, buf, blockIdx.x == 0, bins, red);
+}
 
 }  // namespace
 
@@ -203,7 +346,10 @@ B200_API int b200_attn_mask(const void* ids, int ids64, const uint8_t* flags, in
   MaskParams p = {MaskLayout::of(B, Sq, Skv), ids, flags, ids64, causal, window, buf};
   if ((long long)B * (p.m.Kp / 128) > 0x3fffffff) return b200::fail(942, "attn_mask: %d sequences of %d keys", B, Skv);
   b200::launch(attn_mask_kernel, B, NT, 0, (cudaStream_t)stream, p);
-  b200::launch(attn_mask_order_kernel, 2, NT, 0, (cudaStream_t)stream, p.m, buf);
-  b200::count_launch(2);
+  b200::count_launch();
+  if (B > 1) {
+    b200::launch(attn_mask_order_kernel, 2, NT, 0, (cudaStream_t)stream, p.m, buf);
+    b200::count_launch();
+  }
   return b200::check_launch("attn_mask");
 }

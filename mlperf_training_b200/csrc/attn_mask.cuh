@@ -26,8 +26,8 @@ struct MaskLayout {
     m.k_iv = m.q_iv + b * m.Sp * 2;        // int2 [B][Kp]; empty behind the last key
     m.oq = m.k_iv + b * m.Kp * 2;          // int [B * Sp / 256]: b * (Sp / 256) + pair of query tiles, most key tiles first
     m.ok = m.oq + b * (m.Sp / 256);        // int [B * Kp / 128]: b * (Kp / 128) + key tile, most query tiles first
-    m.scratch = (m.ok + b * (m.Kp / 128) + 1) / 2 * 2;   // int2 [B][Skv]
-    m.total = m.scratch + b * Skv * 2;
+    m.scratch = (m.ok + b * (m.Kp / 128) + 1) / 2 * 2;   // int2 [B][Skv / 16384]: what lies behind each chunk
+    m.total = m.scratch + b * ((Skv + 16383) / 16384) * 2;
     return m;
   }
 };

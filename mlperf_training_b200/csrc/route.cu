@@ -6,10 +6,14 @@
 //   idx = the k largest c among them, largest first, ties to the lower index         w_j = scale * s_j / (sum_j s_j + 1e-20)
 //
 // What is compared is c in 64 bits: two experts whose c differ by less than fp32 resolves would otherwise change places with the way
-// an exponential is rounded.  A warp takes a token in fp32 and keeps an eye on the gaps between neighbours (chosen experts, the best
-// one left out, groups kept and left out); a gap below the error bound of the fp32 values sends the token through the
-// same steps in fp64 (`choose_exact`; normal logits: 0.04 % of the tokens of 256 experts with sigmoid scores, 0.6 % with softmax).
-// Without a bias and without groups the order of c is that of the logits, which are compared as they are.
+// an exponential is rounded.  A warp takes a token.  A key of 32 bits holds c as 23 bits of fixed point between the smallest and largest
+// c that the biases allow, and the expert's index below, so that one warp-wide maximum gives the next expert; every lane keeps its
+// experts' keys sorted.  Where neighbours in the order (the best one left out and groups included) lie closer than the error
+// of what was compared, the token goes through the same steps in fp64 (`choose_exact`; normal logits: 0.1 % of the tokens of 256 experts with
+// sigmoid scores, 1 % with softmax).  Without a bias the order is that of the logits: their upper 24 bits are the key, exact for bf16,
+// and neighbours that agree in them but not in the rest go to `choose_exact`.
+// 65536 tokens, 256 experts in 8 groups, k 8, bf16: ROUTE_US us (33 MB in); with a scan for the maximum over unsorted fp32 values, an owner's
+// ballot and a shuffle a round 203.
 #include "common.cuh"
 #include "runtime.h"
 
@@ -40,17 +44,42 @@ B200_DEVICE void from_float(__nv_bfloat16& o, float v) { o = __float2bfloat16(v)
 template <typename TL, int N>
 struct alignas(N * sizeof(TL) < 16 ? N * sizeof(TL) : 16) Pack { TL v[N]; };
 
-// Order-preserving unsigned keys: 0 is nothing, NaN is below -inf.
+// Order-preserving unsigned key of a float; NaN is below -inf, and above 0 (nothing) in the upper 24 bits.
 B200_DEVICE unsigned key_of(float v) {
   const unsigned u = __float_as_uint(v);
-  if (v != v) return 1u;
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);        // -inf: 0x007fffff
+  return v != v ? 0x100u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);        // -inf: 0x007fffff
 }
-B200_DEVICE float value_of(unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); }
+// 1 / (1 + e^-x) to 3e-7
+B200_DEVICE float sigmoid_fast(float x) {
+  const float d = 1.f + ex2_approx(x * -1.4426950408889634f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
 
 // Above the error of the difference of two fp32 c, |c| <= 1 + b: 3e-7 a score (exponential by ex2.approx, reciprocal) and half a unit
 // of the sum each.  The values of two groups hold two c each and a sum's rounding: four times that.
 B200_DEVICE float gap_bound(float b) { return 1.5e-6f + 5e-7f * b; }
+
+// Descending order of a lane's keys.
+template <int N>
+B200_DEVICE void sort_down(unsigned (&k)[N]) {
+  auto ce = [&](int a, int b) {
+    const unsigned hi = max(k[a], k[b]), lo = min(k[a], k[b]);
+    k[a] = hi;
+    k[b] = lo;
+  };
+  if (N == 2) ce(0, 1);
+  if (N >= 4) {
+#pragma unroll
+    for (int h = 0; h < N; h += 4) { ce(h, h + 1); ce(h + 2, h + 3); ce(h, h + 2); ce(h + 1, h + 3); ce(h + 1, h + 2); }
+  }
+  if (N == 8) {                            // merge of the two sorted fours
+    ce(0, 4); ce(1, 5); ce(2, 6); ce(3, 7);
+    ce(2, 4); ce(3, 5);
+    ce(1, 2); ce(3, 4); ce(5, 6);
+  }
+}
 
 template <typename TL, int NPL>
 B200_DEVICE void load_row(const TL* row, int e0, int E, bool vec, float (&x)[NPL]) {
@@ -80,42 +109,50 @@ B200_DEVICE void softmax_stats(const float (&x)[NPL], float& m, float& inv) {
   inv = s > 0.f ? 1.f / s : (s != s ? s : 0.f);
 }
 
-// Two largest of a warp's share of a group, merged over its `sub` lanes; value of the group.
+// Two largest values so far.
 template <typename R>
-B200_DEVICE R group_value(const R* c, int n, int sub, int part, bool live) {
+struct Two {
   R a = -INFINITY, b = -INFINITY;
-  if (live)
-    for (int i = part; i < n; i += sub) {
-      const R v = c[i];
-      if (v > a) { b = a; a = v; } else if (v > b) b = v;
-    }
-  for (int o = sub / 2; o > 0; o >>= 1) {
-    const R a2 = __shfl_xor_sync(ALL, a, o), b2 = __shfl_xor_sync(ALL, b, o);
-    const R lo = a < a2 ? a : a2, hi = a < a2 ? a2 : a, m = b < b2 ? b2 : b;
-    a = hi;
-    b = lo < m ? m : lo;
+  B200_DEVICE void add(R v) {
+    const R lo = a < v ? a : v;
+    a = a < v ? v : a;
+    b = b < lo ? lo : b;
   }
-  return n > 1 ? a + b : a;
-}
+  B200_DEVICE void join(int o) {           // with another lane's, of other experts
+    const R a2 = __shfl_xor_sync(ALL, a, o), b2 = __shfl_xor_sync(ALL, b, o);
+    add(a2);
+    b = b < b2 ? b2 : b;
+  }
+  B200_DEVICE R value(int n) const { return n > 1 ? a + b : a; }
+};
 
-// Bit g * sub of the result: group g stays.  gap: between the worst that stays and the best that does not.
+// Whether this lane's group stays.  Groups are `sub` lanes each, in order; `v` is the group's value in all of them.  gap: between the worst that
+// stays and the best that does not.
+template <typename R>
+B200_DEVICE bool keep_group(R v, int G, int top, int sub, int lane, R& gap) {
+  const int g = lane / sub;
+  int rank = 0;
+  for (int h = 0; h < G; ++h) {
+    const R o = __shfl_sync(ALL, v, h * sub);
+    rank += (o > v || (o == v && h < g)) ? 1 : 0;
+  }
+  const R in = __shfl_sync(ALL, v, __ffs(__ballot_sync(ALL, g < G && rank == top - 1)) - 1);
+  const R out = __shfl_sync(ALL, v, __ffs(__ballot_sync(ALL, g < G && rank == top)) - 1);
+  gap = in - out;
+  return g < G && rank < top;
+}
+// The same from c in shared memory, for groups that are not whole lanes: bit g * sub of the result, group g stays.
 template <typename R>
 B200_DEVICE unsigned keep_groups(const R* c, int E, int G, int top, int lane, int& sub, R& gap) {
   int gp = 1;
   while (gp < G) gp *= 2;
   sub = 32 / gp;
   const int g = lane / sub, n = E / G;
-  const R v = group_value(c + g * n, n, sub, lane % sub, g < G);
-  int rank = 0;
-  for (int h = 0; h < G; ++h) {
-    const R o = __shfl_sync(ALL, v, h * sub);
-    rank += (o > v || (o == v && h < g)) ? 1 : 0;
-  }
-  const bool keep = g < G && rank < top;
-  // (the values at ranks top - 1 and top; lanes of one group agree)
-  R in = __shfl_sync(ALL, v, __ffs(__ballot_sync(ALL, g < G && rank == top - 1)) - 1);
-  R out = __shfl_sync(ALL, v, __ffs(__ballot_sync(ALL, g < G && rank == top)) - 1);
-  gap = in - out;
+  Two<R> t;
+  if (g < G)
+    for (int i = lane % sub; i < n; i += sub) t.add(c[g * n + i]);
+  for (int o = sub / 2; o > 0; o >>= 1) t.join(o);
+  const bool keep = keep_group<R>(t.value(n), G, top, sub, lane, gap);
   return __ballot_sync(ALL, keep && lane % sub == 0);
 }
 
@@ -140,6 +177,11 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
   int sub = 1;
   double gap;
   if (p.top < p.G) groups = keep_groups<double>(c, p.E, p.G, p.top, lane, sub, gap);
+  if (p.bias == nullptr) {                 // the order of the experts is that of the logits
+    __syncwarp();
+    for (int e = lane; e < p.E; e += 32) c[e] = (double)to_float(row[e]);
+    __syncwarp();
+  }
   const int n = p.E / p.G;
   unsigned taken = 0;                     // of this lane's experts lane + 32 i
   int mine = 0;
@@ -147,11 +189,16 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
     double best = -INFINITY;
     int at = MAX_E;                       // nothing yet: -inf at an index above all
     for (int i = 0, e = lane; e < p.E; ++i, e += 32)
-      if (!(taken >> i & 1) && (p.top == p.G || (groups >> (e / n * sub) & 1)) && (c[e] > best || at == MAX_E)) { best = c[e]; at = e; }
+      if (!(taken >> i & 1) && (p.top == p.G || (groups >> (e / n * sub) & 1)) && (c[e] > best || at == MAX_E || (best != best && c[e] == c[e]))) {
+        best = c[e];
+        at = e;
+      }
     for (int o = 16; o > 0; o >>= 1) {
       const double b = __shfl_xor_sync(ALL, best, o);
       const int a = __shfl_xor_sync(ALL, at, o);
-      if (a != MAX_E && (at == MAX_E || b > best || (b == best && a < at))) { best = b; at = a; }
+      // (NaN, of logits alone, is behind everything)
+      const bool same = b == best || (b != b && best != best);
+      if (a != MAX_E && (at == MAX_E || b > best || (best != best && b == b) || (same && a < at))) { best = b; at = a; }
     }
     if (at % 32 == lane) taken |= 1u << (at / 32);
     if (j == lane) mine = at;
@@ -161,22 +208,36 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
 
 // A warp takes a token; lane l holds experts l * NPL .. + NPL - 1.
 template <typename TL, int NPL>
-__global__ void __launch_bounds__(WARPS * 32) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams p) {
   b200::begin_kernel();
   __shared__ double s_c[WARPS][MAX_E];
   __shared__ int s_hist[MAX_E];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * NPL, n = p.E / p.G;
   for (int e = threadIdx.x; e < p.E; e += WARPS * 32) s_hist[e] = 0;
   __syncthreads();
-  const bool by_logit = p.bias == nullptr && p.top == p.G;
+  const bool biased = p.bias != nullptr, grouped = p.top < p.G;
+  // Groups of whole lanes, a power of two of them, are reduced in registers.
+  const int lanes = n / NPL;
+  const bool by_lanes = n % NPL == 0 && (lanes & (lanes - 1)) == 0;
+  // t = a c + b lies in [1 + 2^-22, 2): the fixed point is its mantissa
   float bias[NPL];
-  float largest = 0.f;                    // of the finite biases
+  float least = INFINITY, most = -INFINITY, largest = 0.f;       // of the finite biases
 #pragma unroll
   for (int i = 0; i < NPL; ++i) {
-    bias[i] = p.bias != nullptr && e0 + i < p.E ? p.bias[e0 + i] : 0.f;
-    if (fabsf(bias[i]) < INFINITY) largest = fmaxf(largest, fabsf(bias[i]));
+    bias[i] = biased && e0 + i < p.E ? p.bias[e0 + i] : 0.f;
+    if (fabsf(bias[i]) < INFINITY && e0 + i < p.E) {
+      least = fminf(least, bias[i]);
+      most = fmaxf(most, bias[i]);
+      largest = fmaxf(largest, fabsf(bias[i]));
+    }
   }
-  const float near = gap_bound(1.f + warp_max(largest));
+  least = -warp_max(-least);
+  most = warp_max(most);
+  if (!(least <= most)) least = most = 0.f;
+  const float a = (1.f - 0x1p-19f) / (1.f + most - least), base = 1.f + 0x1p-21f - a * least;
+  const float near = a * gap_bound(1.f + warp_max(largest)) + 0x1p-21f;      // in units of t
+#pragma unroll
+  for (int i = 0; i < NPL; ++i) bias[i] = fmaf(bias[i], a, base);
   float* sc = reinterpret_cast<float*>(s_c[warp]);
   for (long long t = (long long)blockIdx.x * WARPS + warp; t < p.T; t += (long long)gridDim.x * WARPS) {
     const TL* row = reinterpret_cast<const TL*>(p.logits) + t * p.ld;
@@ -185,75 +246,88 @@ __global__ void __launch_bounds__(WARPS * 32) route_kernel(const RouteParams p) 
     float m = 0.f, inv = 1.f;
     if (!p.sigmoid) softmax_stats<NPL>(x, m, inv);
     unsigned key[NPL];
-    unsigned groups = ALL;
-    int sub = 1;
     bool exact = false;
-    if (by_logit) {
-#pragma unroll
-      for (int i = 0; i < NPL; ++i) key[i] = e0 + i < p.E ? key_of(x[i]) : 0u;
-    } else {
-      float c[NPL];
+    float c[NPL];                                                // t of each expert
+    if (biased || grouped) {
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
-        c[i] = (p.sigmoid ? sigmoid(x[i]) : __expf(x[i] - m) * inv) + bias[i];
-        if (c[i] != c[i]) c[i] = -INFINITY;
-        key[i] = e0 + i < p.E ? key_of(c[i]) : 0u;
+        const float s = p.sigmoid ? sigmoid_fast(x[i]) : __expf(x[i] - m) * inv;
+        c[i] = fminf(fmaxf(fmaf(s, a, bias[i]), 1.f + 0x1p-23f), 2.f - 0x1p-23f);      // (NaN and -inf: the smallest)
       }
-      if (p.top < p.G) {
+    }
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const unsigned inverse = 255u - (unsigned)(e0 + i);
+      // (the exponent of t leaves the word at the top: 0x3f8 << 28 is 2^31, taken off again)
+      key[i] = biased ? (__float_as_uint(c[i]) << 8) - 0x80000000u + inverse : (key_of(x[i]) & 0xffffff00u) | inverse;
+      if (e0 + i >= p.E) key[i] = 0u;
+    }
+    if (grouped) {
+      float gap;
+      if (by_lanes) {
+        Two<float> two;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) two.add(c[i]);
+        for (int o = lanes / 2; o > 0; o >>= 1) two.join(o);
+        const bool keep = keep_group<float>(two.value(n), p.G, p.top, lanes, lane, gap);
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) key[i] = keep ? key[i] : 0u;
+      } else {
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
           if (e0 + i < p.E) sc[e0 + i] = c[i];
         __syncwarp();
-        float gap;
-        groups = keep_groups<float>(sc, p.E, p.G, p.top, lane, sub, gap);
+        int sub;
+        const unsigned groups = keep_groups<float>(sc, p.E, p.G, p.top, lane, sub, gap);
         __syncwarp();
-        exact = gap < 4.f * near;
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
           if (e0 + i < p.E && !(groups >> ((e0 + i) / n * sub) & 1)) key[i] = 0u;
       }
+      exact = gap < 4.f * near;
     }
-    // k rounds of: the largest key of the warp; one more for the gap to the best one left out
-    int mine = 0;
-    float before = INFINITY;
-    const int rounds = by_logit ? p.k : p.k + 1;
-    for (int j = 0; j < rounds; ++j) {
-      unsigned best = key[0];
+    sort_down<NPL>(key);
+    // the k largest keys of the warp, and the next one for the gap to it; lane j keeps the j-th
+    unsigned mine = 0u, top = 0u;
+    for (int j = 0; j <= p.k; ++j) {
+      top = __reduce_max_sync(ALL, key[0]);
+      if (lane == j) mine = top;
+      if (key[0] == top) {
 #pragma unroll
-      for (int i = 1; i < NPL; ++i) best = max(best, key[i]);
-      const unsigned top = __reduce_max_sync(ALL, best);
-      if (!by_logit) {
-        const float v = value_of(top);
-        exact |= top > 1u && before - v < near;
-        before = v;
-        if (j == p.k) break;
+        for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
+        key[NPL - 1] = 0u;
       }
-      const int owner = __ffs(__ballot_sync(ALL, best == top)) - 1;
-      int at = 0;
-      if (lane == owner) {
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < NPL; ++i)
-          if (!found && key[i] == top) { found = true; at = e0 + i; key[i] = 0u; }
+    }
+    int at = 255 - (int)(mine & 255u);
+    {
+      unsigned next = __shfl_down_sync(ALL, mine, 1);
+      if (lane == p.k - 1) next = top;                           // the best one left out
+      const bool pair = lane < p.k && (next >> 8) != 0u;
+      const unsigned units = (mine >> 8) - (next >> 8);
+      bool close = pair && (biased ? (float)units < near * 0x1p23f : units == 0u);
+      if (__any_sync(ALL, close) && !biased) {
+        // equal in 24 bits: equal logits are in order as they are
+        const float mv = to_float(row[min(at, p.E - 1)]), nv = to_float(row[min(255 - (int)(next & 255u), p.E - 1)]);
+        close = close && !(mv == nv || (mv != mv && nv != nv));
       }
-      at = __shfl_sync(ALL, at, owner);
-      if (lane == j) mine = at;
+      exact |= __any_sync(ALL, close);
     }
     if (exact) {
-      mine = choose_exact<TL>(row, p, s_c[warp], lane);
+      __syncwarp();
+      at = choose_exact<TL>(row, p, s_c[warp], lane);
       __syncwarp();
     }
     // weights of the chosen
     float s = 0.f;
     if (lane < p.k) {
-      const float xj = to_float(row[mine]);
+      const float xj = to_float(row[at]);
       s = p.sigmoid ? sigmoid(xj) : __expf(xj - m) * inv;
     }
     const float total = p.renorm ? warp_sum(s) + EPS : 1.f;
     if (lane < p.k) {
-      p.idx[t * p.k + lane] = mine;
+      p.idx[t * p.k + lane] = at;
       p.w[t * p.k + lane] = p.scale * (s / total);
-      atomicAdd(&s_hist[mine], 1);
+      atomicAdd(&s_hist[at], 1);
     }
   }
   __syncthreads();

@@ -156,6 +156,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_attn_bwd_plan": [I] * 8 + [P],
         "b200_attn_mask": [P, I, P, I, I, I, I, I, P, P],
         "b200_attn_masked_fwd": [P] * 9 + [I] * 6 + [L] * 6 + [F, F, P],
+        "b200_attn_masked_rows": [P] * 8 + [I] * 6 + [L] * 6 + [F, F, P, L, P],
         "b200_attn_masked_bwd": [P] * 13 + [I] * 6 + [L] * 10 + [F, F, P, L, P],
     }
     codes = {P: "P", I: "I", L: "L", F: "F", ctypes.c_ulonglong: "U"}
@@ -181,6 +182,10 @@ def _declare(lib: ctypes.CDLL) -> None:
     if hasattr(lib, "b200_attn_mask_ints"):
         lib.b200_attn_mask_ints.argtypes = [I, I, I]
         lib.b200_attn_mask_ints.restype = c_ll
+        lib.b200_attn_masked_few_rows.argtypes = [I, I, I, I]
+        lib.b200_attn_masked_few_rows.restype = c_int
+        lib.b200_attn_masked_rows_workspace.argtypes = [I, I, I, I, I, I]
+        lib.b200_attn_masked_rows_workspace.restype = c_ll
         lib.b200_attn_masked_bwd_workspace.argtypes = [I, I, I, I]
         lib.b200_attn_masked_bwd_workspace.restype = c_ll
     if hasattr(lib, "b200_route_stores_counts"):

@@ -183,7 +183,14 @@ def masked_attention_fwd(q, k, v, mask: AttentionMask, *, scale: float | None = 
     lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
     slopes = None if slopes is None else slopes.detach().float().contiguous()
     sink = None if sink is None else sink.detach().float().contiguous()
+    lib = _lib.load()
     with _lib.on_device_of(q):
+        if not for_backward and lib.b200_attn_masked_few_rows(B, Sq, Hq, Hkv):
+            n = int(lib.b200_attn_masked_rows_workspace(B, Sq, Skv, Hq, Hkv, D))
+            ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+            call("b200_attn_masked_rows", ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(sink), ptr(slopes), ptr(mask.buf), B, Sq, Skv, Hq, Hkv,
+                 D, q_row, k_row, v_row, q_batch, k_batch, v_batch, float(scale), float(softcap), ptr(ws), n, stream_ptr())
+            return out, lse, None
         call("b200_attn_masked_fwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(low), ptr(lse), ptr(sink), ptr(slopes), ptr(mask.buf), B, Sq, Skv, Hq,
              Hkv, D, q_row, k_row, v_row, q_batch, k_batch, v_batch, float(scale), float(softcap), stream_ptr())
     return out, lse, low

@@ -22,6 +22,7 @@ from torch.autograd import Function
 from . import _lib
 from . import kernels as K
 from . import mxfp8
+from .functional import _apply
 from ._lib import call, on_device_of, ptr, stream_ptr, use_kernels
 
 PAD = 128        # row padding of an expert segment for the bf16 grouped kernels (one 128-row tile)
@@ -358,7 +359,8 @@ class RouteFn(Function):
         idx, w, counts = route_fwd(logits, k, score=score, bias=bias, groups=groups, top_groups=top_groups, renormalize=renormalize, scale=scale)
         ctx.save_for_backward(logits, idx)
         ctx.cfg = (score, renormalize, scale)
-        ctx.mark_non_differentiable(idx, counts)
+        if any(ctx.needs_input_grad):
+            ctx.mark_non_differentiable(idx, counts)
         ctx.set_materialize_grads(False)
         return idx, w, counts
 
@@ -381,7 +383,7 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.T
     the bias, divided by their sum (``renormalize``) and times ``scale``.  Comparisons hold in 64 bits; without a bias and groups it is the
     logits that are compared.  ``idx``, ``w`` and ``counts`` go into ``moe_experts`` like those of ``router_topk``, which is
     ``softmax`` with ``renormalize`` for few experts chosen by their logits."""
-    return RouteFn.apply(logits, bias, k, score, groups, top_groups, renormalize, scale)
+    return _apply(RouteFn, logits, bias, k, score, groups, top_groups, renormalize, scale)
 
 
 class PermuteFn(Function):
