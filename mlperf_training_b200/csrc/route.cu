@@ -20,7 +20,7 @@
 namespace {
 
 constexpr int MAX_E = 256, MAX_K = 32, MAX_G = 32;
-constexpr int WARPS = 8;
+constexpr int WARPS = 8, WAIT = 32;
 constexpr float EPS = 1e-20f;
 constexpr unsigned ALL = 0xffffffffu;
 
@@ -44,10 +44,15 @@ B200_DEVICE void from_float(__nv_bfloat16& o, float v) { o = __float2bfloat16(v)
 template <typename TL, int N>
 struct alignas(N * sizeof(TL) < 16 ? N * sizeof(TL) : 16) Pack { TL v[N]; };
 
-// Order-preserving unsigned key of a float; NaN is below -inf, and above 0 (nothing) in the upper 24 bits.
+// Order-preserving unsigned key of a float (NaN: as -inf).
 B200_DEVICE unsigned key_of(float v) {
-  const unsigned u = __float_as_uint(v);
-  return v != v ? 0x100u : (u & 0x80000000u) ? ~u : (u | 0x80000000u);        // -inf: 0x007fffff
+  const int u = __float_as_int(fmaxf(v, -INFINITY));
+  return (unsigned)(u ^ ((u >> 31) | (int)0x80000000));          // -inf: 0x007fffff
+}
+B200_DEVICE float fma_sat(float a, float b, float c) {            // NaN: 0
+  float d;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 // 1 / (1 + e^-x) to 3e-7
 B200_DEVICE float sigmoid_fast(float x) {
@@ -81,16 +86,19 @@ B200_DEVICE void sort_down(unsigned (&k)[N]) {
   }
 }
 
+// A lane's experts of a row, as they are in memory (those that are not there: 0) and as numbers (-inf).
 template <typename TL, int NPL>
-B200_DEVICE void load_row(const TL* row, int e0, int E, bool vec, float (&x)[NPL]) {
-  if (vec && e0 + NPL <= E) {
-    const Pack<TL, NPL> p = *reinterpret_cast<const Pack<TL, NPL>*>(row + e0);
+B200_DEVICE Pack<TL, NPL> fetch_row(const TL* row, int e0, int E, bool vec) {
+  Pack<TL, NPL> r;
+  if (vec && e0 + NPL <= E) return *reinterpret_cast<const Pack<TL, NPL>*>(row + e0);
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) x[i] = to_float(p.v[i]);
-  } else {
+  for (int i = 0; i < NPL; ++i) r.v[i] = e0 + i < E ? row[e0 + i] : (TL)0.f;
+  return r;
+}
+template <typename TL, int NPL, bool FULL = false>
+B200_DEVICE void row_values(const Pack<TL, NPL>& r, int e0, int E, float (&x)[NPL]) {
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) x[i] = e0 + i < E ? to_float(row[e0 + i]) : -INFINITY;
-  }
+  for (int i = 0; i < NPL; ++i) x[i] = FULL || e0 + i < E ? to_float(r.v[i]) : -INFINITY;
 }
 
 // max and sum of a softmax over the row (sum 0: no finite logit)
@@ -141,6 +149,20 @@ B200_DEVICE bool keep_group(R v, int G, int top, int sub, int lane, R& gap) {
   gap = in - out;
   return g < G && rank < top;
 }
+// The same for positive fp32 values in `g` < G, by warp-wide maxima of keys that hold the group below 27 bits of its value (what they cut, 2^-19
+// of values below 4, is in the gap).
+B200_DEVICE bool keep_group(float v, int G, int top, int g, float& gap) {
+  unsigned key = g < G ? (__float_as_uint(v) & ~31u) | (31u - (unsigned)g) : 0u;
+  unsigned last = 0u;
+  bool keep = false;
+  for (int j = 0; j < top; ++j) {
+    last = __reduce_max_sync(ALL, key);
+    if (key == last) { keep = true; key = 0u; }
+  }
+  const unsigned next = __reduce_max_sync(ALL, key);
+  gap = __uint_as_float(last & ~31u) - __uint_as_float(next & ~31u) - 0x1p-18f;
+  return keep;
+}
 // The same from c in shared memory, for groups that are not whole lanes: bit g * sub of the result, group g stays.
 template <typename R>
 B200_DEVICE unsigned keep_groups(const R* c, int E, int G, int top, int lane, int& sub, R& gap) {
@@ -179,7 +201,10 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
   if (p.top < p.G) groups = keep_groups<double>(c, p.E, p.G, p.top, lane, sub, gap);
   if (p.bias == nullptr) {                 // the order of the experts is that of the logits
     __syncwarp();
-    for (int e = lane; e < p.E; e += 32) c[e] = (double)to_float(row[e]);
+    for (int e = lane; e < p.E; e += 32) {
+      const float x = to_float(row[e]);
+      c[e] = x == x ? (double)x : -INFINITY;
+    }
     __syncwarp();
   }
   const int n = p.E / p.G;
@@ -189,16 +214,11 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
     double best = -INFINITY;
     int at = MAX_E;                       // nothing yet: -inf at an index above all
     for (int i = 0, e = lane; e < p.E; ++i, e += 32)
-      if (!(taken >> i & 1) && (p.top == p.G || (groups >> (e / n * sub) & 1)) && (c[e] > best || at == MAX_E || (best != best && c[e] == c[e]))) {
-        best = c[e];
-        at = e;
-      }
+      if (!(taken >> i & 1) && (p.top == p.G || (groups >> (e / n * sub) & 1)) && (c[e] > best || at == MAX_E)) { best = c[e]; at = e; }
     for (int o = 16; o > 0; o >>= 1) {
       const double b = __shfl_xor_sync(ALL, best, o);
       const int a = __shfl_xor_sync(ALL, at, o);
-      // (NaN, of logits alone, is behind everything)
-      const bool same = b == best || (b != b && best != best);
-      if (a != MAX_E && (at == MAX_E || b > best || (best != best && b == b) || (same && a < at))) { best = b; at = a; }
+      if (a != MAX_E && (at == MAX_E || b > best || (b == best && a < at))) { best = b; at = a; }
     }
     if (at % 32 == lane) taken |= 1u << (at / 32);
     if (j == lane) mine = at;
@@ -206,12 +226,30 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
   return mine;
 }
 
+// Weights of the experts that lanes below k hold, and what the token adds to the counts.
+template <typename TL>
+B200_DEVICE void weigh(const TL* row, int t, int at, float m, float inv, const RouteParams& p, int* hist, int lane) {
+  float s = 0.f;
+  if (lane < p.k) {
+    const float x = to_float(row[at]);
+    s = p.sigmoid ? sigmoid(x) : __expf(x - m) * inv;
+  }
+  const float total = p.renorm ? warp_sum(s) + EPS : 1.f;
+  if (lane < p.k) {
+    p.idx[(long long)t * p.k + lane] = at;
+    p.w[(long long)t * p.k + lane] = p.scale * (s / total);
+    atomicAdd(&hist[at], 1);
+  }
+}
+
 // A warp takes a token; lane l holds experts l * NPL .. + NPL - 1.
-template <typename TL, int NPL>
-__global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams p) {
+// FULL: E is 32 * NPL.
+template <typename TL, int NPL, bool FULL>
+__global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const RouteParams p) {
   b200::begin_kernel();
   __shared__ double s_c[WARPS][MAX_E];
   __shared__ int s_hist[MAX_E];
+  __shared__ int s_wait[WARPS][WAIT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * NPL, n = p.E / p.G;
   for (int e = threadIdx.x; e < p.E; e += WARPS * 32) s_hist[e] = 0;
   __syncthreads();
@@ -219,7 +257,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams 
   // Groups of whole lanes, a power of two of them, are reduced in registers.
   const int lanes = n / NPL;
   const bool by_lanes = n % NPL == 0 && (lanes & (lanes - 1)) == 0;
-  // t = a c + b lies in [1 + 2^-22, 2): the fixed point is its mantissa
+  // u = a c + b lies in (0, 1); t = 1 + 2^-22 + u (1 - 2^-20) in [1, 2): the fixed point is its mantissa
   float bias[NPL];
   float least = INFINITY, most = -INFINITY, largest = 0.f;       // of the finite biases
 #pragma unroll
@@ -234,15 +272,27 @@ __global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams 
   least = -warp_max(-least);
   most = warp_max(most);
   if (!(least <= most)) least = most = 0.f;
-  const float a = (1.f - 0x1p-19f) / (1.f + most - least), base = 1.f + 0x1p-21f - a * least;
+  const float a = (1.f - 0x1p-19f) / (1.f + most - least), base = 0x1p-20f - a * least;
   const float near = a * gap_bound(1.f + warp_max(largest)) + 0x1p-21f;      // in units of t
+  // (in shared memory: registers are what limits the warps of an SM)
+  __shared__ __align__(16) float s_bias[32 * NPL];
+  if (warp == 0)
 #pragma unroll
-  for (int i = 0; i < NPL; ++i) bias[i] = fmaf(bias[i], a, base);
+    for (int i = 0; i < NPL; ++i) s_bias[e0 + i] = fmaf(bias[i], a, base);
+  __syncthreads();
   float* sc = reinterpret_cast<float*>(s_c[warp]);
-  for (long long t = (long long)blockIdx.x * WARPS + warp; t < p.T; t += (long long)gridDim.x * WARPS) {
+  unsigned* sk = reinterpret_cast<unsigned*>(s_c[warp]) + lane * NPL;        // (not while sc is in use)
+  const int step = gridDim.x * WARPS;
+  int t = blockIdx.x * WARPS + warp;
+  Pack<TL, NPL> ahead;                                           // the next token's logits are on their way meanwhile
+  if (t < p.T) ahead = fetch_row<TL, NPL>(reinterpret_cast<const TL*>(p.logits) + t * p.ld, e0, p.E, p.vec);
+  while (t < p.T) {
+  int waiting = 0;                                               // tokens for choose_exact, behind the loop (a call inside it costs its registers)
+  for (; t < p.T && waiting < WAIT; t += step) {
     const TL* row = reinterpret_cast<const TL*>(p.logits) + t * p.ld;
     float x[NPL];
-    load_row<TL, NPL>(row, e0, p.E, p.vec, x);
+    row_values<TL, NPL, FULL>(ahead, e0, p.E, x);
+    if (p.T - t > step) ahead = fetch_row<TL, NPL>(row + (long long)step * p.ld, e0, p.E, p.vec);
     float m = 0.f, inv = 1.f;
     if (!p.sigmoid) softmax_stats<NPL>(x, m, inv);
     unsigned key[NPL];
@@ -252,7 +302,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams 
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
         const float s = p.sigmoid ? sigmoid_fast(x[i]) : __expf(x[i] - m) * inv;
-        c[i] = fminf(fmaxf(fmaf(s, a, bias[i]), 1.f + 0x1p-23f), 2.f - 0x1p-23f);      // (NaN and -inf: the smallest)
+        c[i] = fmaf(fma_sat(s, a, s_bias[e0 + i]), 1.f - 0x1p-20f, 1.f + 0x1p-22f);      // (NaN and -inf: the smallest)
       }
     }
 #pragma unroll
@@ -260,7 +310,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams 
       const unsigned inverse = 255u - (unsigned)(e0 + i);
       // (the exponent of t leaves the word at the top: 0x3f8 << 28 is 2^31, taken off again)
       key[i] = biased ? (__float_as_uint(c[i]) << 8) - 0x80000000u + inverse : (key_of(x[i]) & 0xffffff00u) | inverse;
-      if (e0 + i >= p.E) key[i] = 0u;
+      if (!FULL && e0 + i >= p.E) key[i] = 0u;
     }
     if (grouped) {
       float gap;
@@ -269,7 +319,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams 
 #pragma unroll
         for (int i = 0; i < NPL; ++i) two.add(c[i]);
         for (int o = lanes / 2; o > 0; o >>= 1) two.join(o);
-        const bool keep = keep_group<float>(two.value(n), p.G, p.top, lanes, lane, gap);
+        const bool keep = keep_group(two.value(n), p.G, p.top, lane / lanes, gap);
 #pragma unroll
         for (int i = 0; i < NPL; ++i) key[i] = keep ? key[i] : 0u;
       } else {
@@ -287,16 +337,20 @@ __global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams 
       exact = gap < 4.f * near;
     }
     sort_down<NPL>(key);
-    // the k largest keys of the warp, and the next one for the gap to it; lane j keeps the j-th
+    // the k largest keys of the warp, and the next one for the gap to it; lane j keeps the j-th.  A lane's keys behind its first wait in
+    // shared memory (moving them up in registers took as many instructions as all else in a round).
+    unsigned head = key[0];
+    if (NPL > 1) {
+#pragma unroll
+      for (int i = 1; i < NPL; ++i) sk[i - 1] = key[i];
+      sk[NPL - 1] = 0u;
+    }
+    const unsigned* next_key = sk;
     unsigned mine = 0u, top = 0u;
     for (int j = 0; j <= p.k; ++j) {
-      top = __reduce_max_sync(ALL, key[0]);
+      top = __reduce_max_sync(ALL, head);
       if (lane == j) mine = top;
-      if (key[0] == top) {
-#pragma unroll
-        for (int i = 0; i + 1 < NPL; ++i) key[i] = key[i + 1];
-        key[NPL - 1] = 0u;
-      }
+      if (head == top) head = NPL > 1 ? *next_key++ : 0u;          // (a lane whose keys are out stays at the 0 behind them)
     }
     int at = 255 - (int)(mine & 255u);
     {
@@ -313,22 +367,25 @@ __global__ void __launch_bounds__(WARPS * 32, 3) route_kernel(const RouteParams 
       exact |= __any_sync(ALL, close);
     }
     if (exact) {
-      __syncwarp();
-      at = choose_exact<TL>(row, p, s_c[warp], lane);
-      __syncwarp();
+      if (lane == 0) s_wait[warp][waiting] = t;
+      ++waiting;
+    } else {
+      weigh<TL>(row, t, at, m, inv, p, s_hist, lane);
     }
-    // weights of the chosen
-    float s = 0.f;
-    if (lane < p.k) {
-      const float xj = to_float(row[at]);
-      s = p.sigmoid ? sigmoid(xj) : __expf(xj - m) * inv;
+  }
+  for (int i = 0; i < waiting; ++i) {
+    __syncwarp();
+    const int tt = s_wait[warp][i];
+    const TL* row = reinterpret_cast<const TL*>(p.logits) + tt * p.ld;
+    const int at = choose_exact<TL>(row, p, s_c[warp], lane);
+    float m = 0.f, inv = 1.f;
+    if (!p.sigmoid) {
+      float x[NPL];
+      row_values<TL, NPL>(fetch_row<TL, NPL>(row, e0, p.E, p.vec), e0, p.E, x);
+      softmax_stats<NPL>(x, m, inv);
     }
-    const float total = p.renorm ? warp_sum(s) + EPS : 1.f;
-    if (lane < p.k) {
-      p.idx[t * p.k + lane] = at;
-      p.w[t * p.k + lane] = p.scale * (s / total);
-      atomicAdd(&s_hist[at], 1);
-    }
+    weigh<TL>(row, tt, at, m, inv, p, s_hist, lane);
+  }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += WARPS * 32) {
@@ -361,7 +418,7 @@ __global__ void __launch_bounds__(WARPS * 32) route_bwd_kernel(const RouteBwdPar
     const TL* row = reinterpret_cast<const TL*>(p.logits) + t * p.ld;
     float x[NPL], m = 0.f, inv = 1.f;
     if (!p.sigmoid) {
-      load_row<TL, NPL>(row, e0, p.E, p.vec, x);
+      row_values<TL, NPL>(fetch_row<TL, NPL>(row, e0, p.E, p.vec), e0, p.E, x);
       softmax_stats<NPL>(x, m, inv);
     }
     const bool live = lane < p.k;
@@ -430,9 +487,11 @@ unsigned route_grid(int T) {
   return (unsigned)(blocks < most ? blocks : most);
 }
 
+template <typename TL, int NPL>
+auto route_of(const RouteParams& p) { return p.E == 32 * NPL ? route_kernel<TL, NPL, true> : route_kernel<TL, NPL, false>; }
 template <typename TL>
 void launch_route(const RouteParams& p, cudaStream_t s) {
-  auto k = p.E <= 32 ? route_kernel<TL, 1> : p.E <= 64 ? route_kernel<TL, 2> : p.E <= 128 ? route_kernel<TL, 4> : route_kernel<TL, 8>;
+  auto k = p.E <= 32 ? route_of<TL, 1>(p) : p.E <= 64 ? route_of<TL, 2>(p) : p.E <= 128 ? route_of<TL, 4>(p) : route_of<TL, 8>(p);
   b200::launch(k, route_grid(p.T), WARPS * 32, 0, s, p);
 }
 template <typename TL>

@@ -120,20 +120,18 @@ def route_fwd(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: tor
         x = logits.double()
         s = _route_scores(x, score)
         lost = float("-inf")
-        by = x
-        if bias is not None or top_groups < groups:
-            by = s if bias is None else s + bias.double()
-            by = torch.where(by.isnan(), lost, by)
+        by = x if bias is None and top_groups == groups else s if bias is None else s + bias.double()
+        by = torch.where(by.isnan(), lost, by)
         if top_groups < groups:
             pair = by.unflatten(1, (groups, E // groups)).sort(-1, descending=True)[0][..., :2].sum(-1)
             kept = torch.zeros(T, groups, dtype=torch.bool).scatter_(1, pair.sort(dim=-1, descending=True, stable=True)[1][:, :top_groups], True)
             out = ~kept.repeat_interleave(E // groups, 1)
+            by = x if bias is None else by
         else:
             out = torch.zeros_like(by, dtype=torch.bool)
-        # largest first, NaN behind -inf, experts of other groups last; ties to the lower index
-        order = torch.arange(E).expand(T, E)
-        for key in (torch.where(by.isnan(), lost, by).neg(), by.isnan().double(), out.double()):
-            order = order.gather(1, key.gather(1, order).sort(dim=-1, stable=True)[1])
+        # largest first, experts of other groups last; ties to the lower index
+        order = torch.where(by.isnan(), lost, by).sort(dim=-1, descending=True, stable=True)[1]
+        order = order.gather(1, out.gather(1, order).int().sort(dim=-1, stable=True)[1])
         idx = order[:, :k]
         sj = s.gather(1, idx)
         w = scale * sj / (sj.sum(-1, keepdim=True) + ROUTE_EPS) if renormalize else scale * sj
@@ -380,8 +378,8 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.T
     The scores are ``softmax`` over all experts or ``sigmoid``.  Experts are chosen by score + ``bias`` (fp32 ``[E]``, without a gradient: a
     balance bias, or -inf for an expert that gets nothing), largest first, ties to the lower index.  With ``groups`` the experts lie in that
     many equal groups and only the ``top_groups`` with the largest sum of their two best take part.  The weights are the scores of the chosen, without
-    the bias, divided by their sum (``renormalize``) and times ``scale``.  Comparisons hold in 64 bits; without a bias and groups it is the
-    logits that are compared.  ``idx``, ``w`` and ``counts`` go into ``moe_experts`` like those of ``router_topk``, which is
+    the bias, divided by their sum (``renormalize``) and times ``scale``.  Comparisons hold in 64 bits, NaN counts as -inf; without a bias
+    experts are compared by their logits.  ``idx``, ``w`` and ``counts`` go into ``moe_experts`` like those of ``router_topk``, which is
     ``softmax`` with ``renormalize`` for few experts chosen by their logits."""
     return _apply(RouteFn, logits, bias, k, score, groups, top_groups, renormalize, scale)
 

@@ -22,7 +22,7 @@ def route(rows, k, score, bias, groups, top_groups, renormalize, scale):
         value = [sum(sorted(c[g * n:(g + 1) * n], reverse=True)[:2]) for g in range(groups)]
         stay = sorted(range(groups), key=lambda g: (-value[g], g))[:top_groups]
         pool = [e for g in sorted(stay) for e in range(g * n, (g + 1) * n)]
-        by = x if bias is None and top_groups == groups else c
+        by = x if bias is None else c
         pick = sorted(pool, key=lambda e: (-by[e], e))[:k]
         total = sum(s[e] for e in pick) + 1e-20 if renormalize else 1.0
         idx.append(pick)

@@ -89,9 +89,9 @@ def test_infinite_and_not_a_number():
     for score in M.ROUTE_SCORES:
         idx, w, _ = M.route(torch.full((1, 4), -inf), 2, score=score)
         assert idx.tolist() == [[0, 1]] and w.tolist() == [[0.0, 0.0]]
-    # NaN is behind everything
+    # NaN counts as -inf
     idx, _, _ = M.route(torch.tensor([[nan, -inf, 1.0]]), 3, score="sigmoid")
-    assert idx.tolist() == [[2, 1, 0]]
+    assert idx.tolist() == [[2, 0, 1]]
 
 
 def test_bias_step():
