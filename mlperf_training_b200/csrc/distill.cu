@@ -10,17 +10,21 @@
 // An entry whose id is outside the vocabulary or whose value is -inf is not there.  Tokens labelled `ignore` have loss and gradient 0; so has
 // the cross-entropy of another label outside the vocabulary.
 //
-// Forward: one pass over the row for the log-sum-exp of u and of z (the same pass; one exponential where tau is 1 or a is 1) on a running
-// maximum; with `rest` the ids are marked in a bitmap and left out of the sum, which is then that of the others without cancellation, and
-// the ids' own terms join it at the end.  Backward: the row again from the saved log-sum-exps, written as it is read; the elements of
-// the ids and the label are then written once more by a thread each, from logits read before any was overwritten, so the gradient may take
-// the logits' place.  p, r and their logarithms are in fp64 (r = 1 - sum p cancels), all else in fp32.
+// Forward: one pass over the row for the log-sum-exp of u and of z on one running maximum.  Where both are wanted and tau is 2, 4 or 8, the
+// term of z is that of u squared once, twice or three times; another tau takes a second exponential (16 a clock and SM: 8192 rows of
+// 128256 in bf16 with two 626 us, FWD_US with one).  With `rest` the ids are marked in a bitmap and left out of the sum, which is then that
+// of the others without cancellation, and the ids' own terms join it at the end.  One warp forms the teacher's sums meanwhile, in fp64
+// (r = 1 - sum p cancels); what they need of the student is its log-sum-exp alone.
+// Backward: the row again from the saved log-sum-exps, written as it is read; the elements of the ids and the label are then written once
+// more by a thread each, from logits read before any was overwritten, so the gradient may take the logits' place.
+// Both are bound by memory (one read; one read and one write) with four 16-byte loads a thread under way: 8192 x 128256 bf16 FWD_US and BWD_US us.
 #include "common.cuh"
 #include "runtime.h"
 
 namespace {
 
 constexpr int NT = 512, MAX_K = 1024, SLOTS = MAX_K / NT;
+constexpr int AHEAD = 4;           // 16-byte loads of a thread under way
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 enum { F32 = 0, BF16 = 1 };
@@ -49,15 +53,6 @@ B200_DEVICE float load1(const float* p) { return *p; }
 B200_DEVICE float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 B200_DEVICE void store1(float* p, float v) { *p = v; }
 B200_DEVICE void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
-B200_DEVICE void load_vec(const float* p, float (&x)[4]) {
-  const float4 v = *reinterpret_cast<const float4*>(p);
-  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-}
-B200_DEVICE void load_vec(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-  x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y; x[4] = c.x; x[5] = c.y; x[6] = d.x; x[7] = d.y;
-}
 B200_DEVICE void store_vec(float* p, const float (&x)[4]) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
 B200_DEVICE void store_vec(__nv_bfloat16* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
@@ -82,57 +77,80 @@ B200_DEVICE Span span_of(const TL* row, int lo, int hi) {
   return s;
 }
 
-// A sum of 2^(x - m) for the largest m so far.
+// Sums of 2^(x - m) and (Z) of its tau-th power, for the largest m so far.
+template <bool Z>
 struct Lse {
-  float m, s;
-  B200_DEVICE void join(float m2, float s2) {
+  float m = -INFINITY, s = 0.f, z = 0.f;
+  B200_DEVICE void join(float m2, float s2, float z2, float tau) {
     const float n = fmax_nan(m, m2);
-    s = (m == -INFINITY ? 0.f : s * ex2_approx(m - n)) + (m2 == -INFINITY ? 0.f : s2 * ex2_approx(m2 - n));
+    const float f = m == -INFINITY ? 0.f : ex2_approx(m - n), g = m2 == -INFINITY ? 0.f : ex2_approx(m2 - n);
+    s = s * f + s2 * g;
+    if (Z) z = z * (m == -INFINITY ? 0.f : ex2_approx((m - n) * tau)) + z2 * (m2 == -INFINITY ? 0.f : ex2_approx((m2 - n) * tau));
     m = n;
   }
-  B200_DEVICE float log2() const { return m == -INFINITY ? -INFINITY : m + log2f(s); }
+  B200_DEVICE void join_lane(int o, float tau) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o), z2 = Z ? __shfl_xor_sync(0xffffffffu, z, o) : 0.f;
+    join(m2, s2, z2, tau);
+  }
+  B200_DEVICE float log2_s() const { return m == -INFINITY ? -INFINITY : m + log2f(s); }
+  B200_DEVICE float log2_z(float tau) const { return m == -INFINITY ? -INFINITY : m * tau + log2f(z); }
 };
-B200_DEVICE Lse block_join(Lse v, Lse* red) {
+template <bool Z>
+B200_DEVICE Lse<Z> block_join(Lse<Z> v, float tau, Lse<Z>* red) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v.join(__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o));
+  for (int o = 16; o > 0; o >>= 1) v.join_lane(o, tau);
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  __syncthreads();
-  if (l == 0) red[w] = v;
+  if (l == 0 && w < NT / 32) red[w] = v;
   __syncthreads();
   v = red[l % (NT / 32)];
 #pragma unroll
-  for (int o = NT / 64; o > 0; o >>= 1) v.join(__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.s, o));
+  for (int o = NT / 64; o > 0; o >>= 1) v.join_lane(o, tau);
   return v;
 }
-B200_DEVICE double block_sum(double v, double* red) {
+B200_DEVICE double warp_sum64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.;
-  for (int i = 0; i < NT / 32; ++i) v += red[i];
   return v;
 }
-B200_DEVICE double block_max(double v, double* red) {
+B200_DEVICE double warp_max64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int i = 1; i < NT / 32; ++i) v = fmax(v, red[i]);
   return v;
 }
 
-// One CTA a row.  BOTH: the log-sum-exp of z beside that of u.  REST: ids are left out of the pass.
-template <typename TL, bool BOTH, bool REST>
-__global__ void __launch_bounds__(NT) distill_fwd_kernel(const DistillParams p) {
+// What one warp finds out about a token's teacher.
+struct Teacher {
+  double log_sum = 0.;      // of t / tau (plain)
+  double mass = 0.;         // sum of p
+  double own = 0.;          // sum of p log p
+  double cross = 0.;        // sum of p u[id]
+};
+
+// The largest of N elements as floats (bf16: pairs at a time).
+B200_DEVICE float largest(const float4& v) { return fmax_nan(fmax_nan(v.x, v.y), fmax_nan(v.z, v.w)); }
+B200_DEVICE float largest(const uint4& v) {
+  auto h = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h(v.x), h(v.y)), __hmax2_nan(h(v.z), h(v.w)));
+  return fmax_nan(__low2float(m), __high2float(m));
+}
+B200_DEVICE void pairs(const float4& v, float2 (&x)[2]) { x[0] = make_float2(v.x, v.y); x[1] = make_float2(v.z, v.w); }
+B200_DEVICE void pairs(const uint4& v, float2 (&x)[4]) { x[0] = unpack_bf16x2(v.x); x[1] = unpack_bf16x2(v.y); x[2] = unpack_bf16x2(v.z); x[3] = unpack_bf16x2(v.w); }
+template <typename TL> struct Raw;
+template <> struct Raw<float> { using T = float4; };
+template <> struct Raw<__nv_bfloat16> { using T = uint4; };
+
+// One CTA a row.  POWER: -1 the log-sum-exp of u alone; 1, 2, 3 that of z too, from u's terms squared so many times; 0 from an exponential
+// of its own.  REST: ids are left out of the pass.  The last warp takes the teacher, whose chain of loads and sums is about as long as a third
+// of the row (a warp that did both held the row back: 8192 x 128256 484 us, FWD_US with a warp for each).
+template <typename TL, int POWER, bool REST>
+__global__ void __launch_bounds__(NT + 32, 2) distill_fwd_kernel(const DistillParams p) {
   b200::begin_kernel();
+  constexpr bool BOTH = POWER >= 0;
+  constexpr int N = Vec<TL>::N;
   extern __shared__ unsigned s_mark[];                 // REST: a bit for each id
-  __shared__ Lse red[NT / 32];
-  __shared__ double redd[NT / 32];
+  __shared__ Lse<BOTH> red[NT / 32];
   const long long t = blockIdx.x;
+  const int lane = threadIdx.x & 31;
   const long long label = p.labels != nullptr ? p.labels[t] : 0;
   float* st = p.stats + t * 4;
   if (p.labels != nullptr && label == p.ignore) {      // (the whole CTA)
@@ -144,156 +162,169 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const DistillParams p) 
     return;
   }
   const TL* row = reinterpret_cast<const TL*>(p.logits) + t * p.ld;
-  // this thread's entries
-  int id[SLOTS];
-  float val[SLOTS], zid[SLOTS];
-  bool own[SLOTS];                                     // the first of equal ids
+  const float cu = LOG2E / p.tau;
+  // the teacher: warp 0 (the others meanwhile begin with the row)
+  Teacher te;
+  Lse<BOTH> ids;                                       // (REST) terms of the ids, each once
+  float zlabel = 0.f;
+  unsigned first = 0u;                                 // (REST) bit i: entry lane + 32 i is the first of its id
+  const bool teaches = threadIdx.x >= NT;
+  using RawT = typename Raw<TL>::T;
+  const Span sp = span_of(row, 0, p.V);
+  const RawT* vecs = reinterpret_cast<const RawT*>(row + sp.first);
+  RawT raw[AHEAD];
+  if (!teaches) {
 #pragma unroll
-  for (int i = 0; i < SLOTS; ++i) {
-    const int j = threadIdx.x + i * NT;
-    id[i] = -1;
-    val[i] = -INFINITY;
-    zid[i] = 0.f;
-    own[i] = false;
-    if (j < p.K && p.alpha > 0.f) {
-      const long long v = id_at(p, t * p.K + j);
-      val[i] = value_at(p, t * p.K + j);
-      if (v >= 0 && v < p.V && val[i] != -INFINITY) {
-        id[i] = (int)v;
-        zid[i] = load1(row + v);
-      }
-    }
+    for (int i = 0; i < AHEAD; ++i)
+      if (i * NT + (int)threadIdx.x < sp.n) raw[i] = vecs[i * NT + (int)threadIdx.x];
   }
   if (REST) {
-    for (int i = threadIdx.x; i < (p.V + 31) / 32; i += NT) s_mark[i] = 0u;
+    for (int i = threadIdx.x; i < (p.V + 31) / 32; i += NT + 32) s_mark[i] = 0u;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i)
-      if (id[i] >= 0) own[i] = !(atomicOr(&s_mark[id[i] >> 5], 1u << (id[i] & 31)) >> (id[i] & 31) & 1u);
+    // the ids are marked before the pass begins; who marked one first has it in `first`
+    if (teaches && p.alpha > 0.f)
+      for (int j = lane; j < p.K; j += 32) {
+        const long long v = id_at(p, t * p.K + j);
+        if (v >= 0 && v < p.V && value_at(p, t * p.K + j) != -INFINITY && !(atomicOr(&s_mark[v >> 5], 1u << (v & 31)) >> (v & 31) & 1u))
+          first |= 1u << (j >> 5);
+      }
     __syncthreads();
   }
-  // the pass: u and z in units of log2
-  const float cz = LOG2E, cu = LOG2E / p.tau;
-  Lse lu = {-INFINITY, 0.f};
-  float sz = 0.f, mz = -INFINITY;                      // (BOTH) sum for z on the same element's maximum
-  constexpr int N = Vec<TL>::N;
-  auto take = [&](const auto& x, const int n, const unsigned skip) {
-    float mx = -INFINITY;
-    for (int i = 0; i < n; ++i)
-      if (!REST || !(skip >> i & 1u)) mx = fmax_nan(mx, x[i]);
-    if (!(mx * cu <= lu.m)) {                          // (a NaN goes on to the sums)
-      const float nu = mx * cu, nz = mx * cz;
-      if (lu.m > -INFINITY) {
-        lu.s *= ex2_approx(lu.m - nu);
-        if (BOTH) sz *= ex2_approx(mz - nz);
+  if (teaches) {
+    if (p.alpha < 1.f && label >= 0 && label < p.V) zlabel = load1(row + label);
+    auto entry = [&](int j, float& val) -> int {       // the id, or -1 where the entry is not there
+      const long long v = id_at(p, t * p.K + j);
+      val = value_at(p, t * p.K + j);
+      return v >= 0 && v < p.V && val != -INFINITY ? (int)v : -1;
+    };
+    if (p.alpha > 0.f) {
+      if (!p.rest) {
+        double m = -INFINITY, s = 0.;
+        float val;
+        for (int j = lane; j < p.K; j += 32)
+          if (entry(j, val) >= 0) m = fmax(m, (double)val / p.tau);
+        m = warp_max64(m);
+        for (int j = lane; j < p.K; j += 32)
+          if (entry(j, val) >= 0) s += exp((double)val / p.tau - m);
+        s = warp_sum64(s);
+        te.log_sum = s != 0. ? m + log(s) : 0.;        // (no entry: s = 0)
       }
-      lu.m = nu;
-      if (BOTH) mz = nz;
+      for (int j = lane; j < p.K; j += 32) {
+        float val;
+        const int id = entry(j, val);
+        if (id < 0) continue;
+        const float zid = load1(row + id);
+        if (REST && (first >> (j >> 5) & 1u)) ids.join(zid * cu, 1.f, 1.f, p.tau);
+        const double logp = p.rest ? (double)val : (double)val / p.tau - te.log_sum, pj = exp(logp);
+        te.mass += pj;
+        if (pj != 0.) { te.own += pj * logp; te.cross += pj * ((double)zid / p.tau); }
+      }
+      te.mass = warp_sum64(te.mass);
+      te.own = warp_sum64(te.own);
+      te.cross = warp_sum64(te.cross);
+      if (REST)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ids.join_lane(o, p.tau);
     }
-    if (lu.m == -INFINITY) return;
-    for (int i = 0; i < n; ++i) {
-      if (REST && (skip >> i & 1u)) continue;
-      lu.s += ex2_approx(fmaf(x[i], cu, -lu.m));
-      if (BOTH) sz += ex2_approx(fmaf(x[i], cz, -mz));
+  }
+
+  // the pass, in units of log2
+  Lse<BOTH> acc;
+  float2 s2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);       // sums on acc.m
+  auto raise = [&](float mx) {                         // the maximum seen so far; a NaN goes on to the sums
+    const float n = mx * cu;
+    if (!(n <= acc.m)) {
+      if (acc.m > -INFINITY) {
+        const float f = ex2_approx(acc.m - n);
+        s2 = fmul2(s2, make_float2(f, f));
+        if (BOTH) {
+          const float g = ex2_approx((acc.m - n) * p.tau);
+          z2 = fmul2(z2, make_float2(g, g));
+        }
+      }
+      acc.m = n;
     }
   };
-  const Span sp = span_of(row, 0, p.V);
-  for (int v = threadIdx.x; v < sp.n; v += NT) {
-    const int c = sp.first + v * N;
-    float x[N];
-    load_vec(row + c, x);
-    unsigned skip = 0u;
-    if (REST) {
-      // N bits from bit c on
-      const unsigned lo = s_mark[c >> 5], hi = (c & 31) + N > 32 ? s_mark[(c >> 5) + 1] : 0u;
-      skip = __funnelshift_r(lo, hi, c & 31) & ((1u << N) - 1u);
-    }
-    take(x, N, skip);
-  }
-  {
-    const int edge = (sp.first - sp.lo) + (sp.hi - sp.first - sp.n * N);        // fewer than 2 N elements
-    if ((int)threadIdx.x < edge) {
-      const int c = (int)threadIdx.x < sp.first - sp.lo ? sp.lo + (int)threadIdx.x : sp.first + sp.n * N + (int)threadIdx.x - (sp.first - sp.lo);
-      const float x[1] = {load1(row + c)};
-      take(x, 1, REST ? s_mark[c >> 5] >> (c & 31) & 1u : 0u);
-    }
-  }
-  lu = block_join(lu, red);
-  // logarithms (base 2) of the sums; with REST those of the others first, then the ids' own terms
-  const float others = lu.log2();
-  if (REST) {
-    Lse mine = {-INFINITY, 0.f};
+  auto add = [&](float2 x) {
+    const float2 a = ffma2(x, make_float2(cu, cu), make_float2(-acc.m, -acc.m));
+    float2 e = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+    s2 = fadd2(s2, e);
+    if (POWER >= 1) {
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i)
-      if (own[i]) mine.join(zid[i] * cu, 1.f);
-    mine = block_join(mine, red);
-    lu.join(mine.m, mine.s);
-  }
-  const float lse_u = lu.log2();
-  float lse_z = lse_u;
-  if (BOTH) {
-    Lse lz = {mz, sz};
-    lz = block_join(lz, red);
-    if (REST) {
-      Lse mine = {-INFINITY, 0.f};
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i)
-        if (own[i]) mine.join(zid[i] * cz, 1.f);
-      mine = block_join(mine, red);
-      lz.join(mine.m, mine.s);
+      for (int i = 1; i < POWER; ++i) e = fmul2(e, e);
+      z2 = ffma2(e, e, z2);
     }
-    lse_z = lz.log2();
+    if (POWER == 0) z2 = fadd2(z2, make_float2(ex2_approx(a.x * p.tau), ex2_approx(a.y * p.tau)));
+  };
+  auto take1 = [&](int c) {                            // one element
+    if (REST && (s_mark[c >> 5] >> (c & 31) & 1u)) return;
+    const float x = load1(row + c);
+    raise(x);
+    if (acc.m != -INFINITY) add(make_float2(x, -INFINITY));
+  };
+  if (!teaches) {
+    for (int v0 = threadIdx.x; v0 < sp.n; v0 += NT * AHEAD) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int v = v0 + i * NT, later = v + AHEAD * NT;
+        const RawT now = raw[i];
+        if (later < sp.n) raw[i] = vecs[later];
+        if (v >= sp.n) continue;
+        if (REST) {
+          // N bits from bit c on
+          const int c = sp.first + v * N;
+          const unsigned lo = s_mark[c >> 5], hi = (c & 31) + N > 32 ? s_mark[(c >> 5) + 1] : 0u;
+          if (__funnelshift_r(lo, hi, c & 31) & ((1u << N) - 1u)) {
+            for (int k = 0; k < N; ++k) take1(c + k);
+            continue;
+          }
+        }
+        raise(largest(now));
+        if (acc.m == -INFINITY) continue;
+        float2 x[N / 2];
+        pairs(now, x);
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) add(x[k]);
+      }
+    }
+    const int head = sp.first - sp.lo, edge = head + (sp.hi - sp.first - sp.n * N);        // fewer than 2 N elements
+    if ((int)threadIdx.x < edge) take1((int)threadIdx.x < head ? sp.lo + (int)threadIdx.x : sp.first + sp.n * N + (int)threadIdx.x - head);
   }
-  // the teacher
-  double kl = 0., lt = 0., c = 0., ratio = 0.;
+  acc.s = s2.x + s2.y;
+  acc.z = z2.x + z2.y;
+  acc = block_join<BOTH>(acc, p.tau, red);
+  if (threadIdx.x != NT) return;                       // (the teacher's first lane)
+  // with REST the sums are those of the others, and the ids join them
+  const float others = acc.log2_s();
+  if (REST) acc.join(ids.m, ids.s, ids.z, p.tau);
+  const float lse_u = acc.log2_s(), lse_z = BOTH ? acc.log2_z(p.tau) : lse_u;
+  double loss = 0., c = te.mass, ratio = 0.;
   if (p.alpha > 0.f) {
-    double mass = 0.;
-    if (!p.rest) {
-      double m = -INFINITY, s = 0.;
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i)
-        if (id[i] >= 0) m = fmax(m, (double)val[i] / p.tau);
-      m = block_max(m, redd);
-#pragma unroll
-      for (int i = 0; i < SLOTS; ++i)
-        if (id[i] >= 0) s += exp((double)val[i] / p.tau - m);
-      s = block_sum(s, redd);
-      lt = s > 0. ? m + log(s) : 0.;
-    }
-#pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-      if (id[i] < 0) continue;
-      const double logp = p.rest ? (double)val[i] : (double)val[i] / p.tau - lt, pj = exp(logp);
-      mass += pj;
-      if (pj != 0.) kl += pj * (logp - (double)(zid[i] * cu - lse_u) * 0.6931471805599453094);
-    }
-    kl = block_sum(kl, redd);
-    c = block_sum(mass, redd);
+    const double ln2 = 0.6931471805599453094, lse = (double)lse_u * ln2;
+    double kl = te.own - te.cross + (te.mass != 0. ? te.mass * lse : 0.);
     if (REST) {
       const double r = 1. - c;
       if (r > 0. && others > -INFINITY) {              // (no id left outside: nothing for the rest to be)
-        const double lr = (double)(others - lse_u) * 0.6931471805599453094;
+        const double lr = (double)(others - lse_u) * ln2;
         kl += r * (log(r) - lr);
         ratio = r / exp(lr);
         c += r;
       }
     }
+    loss = (double)p.alpha * p.tau * p.tau * kl;
   }
-  if (threadIdx.x == 0) {
-    double loss = p.alpha > 0.f ? (double)p.alpha * p.tau * p.tau * kl : 0.;
-    if (p.alpha < 1.f && label >= 0 && label < p.V) loss += (1. - (double)p.alpha) * (double)(lse_z * LN2 - load1(row + label));
-    p.loss[t] = (float)loss;
-    st[0] = lse_u;
-    st[1] = lse_z;
-    st[2] = (float)c;
-    st[3] = (float)ratio;
-    p.teacher[t] = lt;
-  }
+  if (p.alpha < 1.f && label >= 0 && label < p.V) loss += (1. - (double)p.alpha) * (double)(lse_z * LN2 - zlabel);
+  p.loss[t] = (float)loss;
+  st[0] = lse_u;
+  st[1] = lse_z;
+  st[2] = (float)c;
+  st[3] = (float)ratio;
+  p.teacher[t] = te.log_sum;
 }
 
 // CTA (t, part): columns [part, part + 1) * V / parts of row t.
-template <typename TL, bool BOTH>
-__global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillParams p) {
+template <typename TL, int POWER>
+__global__ void __launch_bounds__(NT, 2) distill_bwd_kernel(const DistillParams p) {
   b200::begin_kernel();
   __shared__ int s_id[MAX_K];
   __shared__ float s_p[MAX_K];
@@ -330,9 +361,23 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillParams p) 
     if (threadIdx.x == 0 && labelled && label >= lo && label < hi) zlabel = load1(row + label);
     __syncthreads();
   }
-  auto other = [&](float x) -> float {
-    if (!BOTH) return (fu + gz) * ex2_approx(fmaf(x, cu, -lse_u));
-    return fu * ex2_approx(fmaf(x, cu, -lse_u)) + gz * ex2_approx(fmaf(x, LOG2E, -lse_z));
+  // e^(z - lse_z) from e^(u - lse_u): its tau-th power times 2^(tau lse_u - lse_z)
+  const float gp = POWER >= 1 ? gz * ex2_approx(p.tau * lse_u - lse_z) : 0.f;
+  auto other = [&](float2 x) -> float2 {
+    const float2 a = ffma2(x, make_float2(cu, cu), make_float2(-lse_u, -lse_u));
+    float2 e = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+    if (POWER < 0) return fmul2(e, make_float2(fu + gz, fu + gz));
+    float2 z;
+    if (POWER >= 1) {
+      z = fmul2(e, e);
+#pragma unroll
+      for (int i = 1; i < POWER; ++i) z = fmul2(z, z);
+      z = fmul2(z, make_float2(gp, gp));
+    } else {
+      const float2 b = ffma2(x, make_float2(LOG2E, LOG2E), make_float2(-lse_z, -lse_z));
+      z = fmul2(make_float2(ex2_approx(b.x), ex2_approx(b.y)), make_float2(gz, gz));
+    }
+    return ffma2(e, make_float2(fu, fu), z);
   };
   const Span sp = span_of(out, lo, hi);
   const bool vec = (((uintptr_t)row ^ (uintptr_t)out) & 15) == 0;     // both rows are aligned at the same columns
@@ -343,19 +388,37 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const DistillParams p) 
     for (int i = threadIdx.x; i < hi - lo - body; i += NT) store1(out + (i < head ? lo + i : lo + i + body), 0.f);
     return;
   }
-  for (int v = threadIdx.x; v < sp.n; v += NT) {
-    const int col = sp.first + v * N;
-    float x[N];
-    if (vec) load_vec(row + col, x);
-    else
-      for (int i = 0; i < N; ++i) x[i] = load1(row + col + i);
+  if (vec) {
+    const typename Raw<TL>::T* src = reinterpret_cast<const typename Raw<TL>::T*>(row + sp.first);
+    for (int v0 = 0; v0 < sp.n; v0 += NT * AHEAD) {
+      typename Raw<TL>::T raw[AHEAD];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = other(x[i]);
-    store_vec(out + col, x);
+      for (int i = 0; i < AHEAD; ++i) {
+        const int v = v0 + i * NT + (int)threadIdx.x;
+        if (v < sp.n) raw[i] = src[v];
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int v = v0 + i * NT + (int)threadIdx.x;
+        if (v >= sp.n) continue;
+        float2 x[N / 2];
+        pairs(raw[i], x);
+        float y[N];
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) {
+          const float2 g = other(x[k]);
+          y[2 * k] = g.x;
+          y[2 * k + 1] = g.y;
+        }
+        store_vec(out + sp.first + v * N, y);
+      }
+    }
+  } else {
+    for (int i = sp.first + (int)threadIdx.x; i < sp.first + body; i += NT) store1(out + i, other(make_float2(load1(row + i), 0.f)).x);
   }
   for (int i = threadIdx.x; i < hi - lo - body; i += NT) {
     const int col = i < head ? lo + i : lo + i + body;
-    store1(out + col, other(load1(row + col)));
+    store1(out + col, other(make_float2(load1(row + col), 0.f)).x);
   }
   __syncthreads();
   auto special = [&](int v, float z) {
@@ -393,16 +456,39 @@ int set_smem(const void* fn, size_t bytes) {
   return 0;
 }
 
-template <typename TL>
+// How the terms of z come from those of u (see distill_fwd_kernel).
+int power_of(const DistillParams& p) {
+  if (p.alpha >= 1.f || p.tau == 1.f) return -1;
+  return p.tau == 2.f ? 1 : p.tau == 4.f ? 2 : p.tau == 8.f ? 3 : 0;
+}
+
+template <typename TL, int POWER>
 int launch_fwd(const DistillParams& p, cudaStream_t s) {
-  const bool both = p.alpha < 1.f && p.tau != 1.f;
-  auto k = p.rest ? (both ? distill_fwd_kernel<TL, true, true> : distill_fwd_kernel<TL, false, true>)
-                  : (both ? distill_fwd_kernel<TL, true, false> : distill_fwd_kernel<TL, false, false>);
+  auto k = p.rest ? distill_fwd_kernel<TL, POWER, true> : distill_fwd_kernel<TL, POWER, false>;
   const size_t smem = p.rest ? ((size_t)p.V + 31) / 32 * 4 : 0;
   if (int r = set_smem((const void*)k, smem)) return r;
-  b200::launch(k, p.T, NT, smem, s, p);
+  b200::launch(k, p.T, NT + 32, smem, s, p);
   b200::count_launch();
   return b200::check_launch("distill_fwd");
+}
+template <typename TL, int POWER>
+int launch_bwd(const DistillParams& p, cudaStream_t s) {
+  // few rows: several CTAs a row, of 4096 columns or more
+  int parts = 1;
+  while (parts < 32 && (long long)p.T * parts < 2 * b200::sm_count() && p.V / (2 * parts) >= 4096) parts *= 2;
+  b200::launch(distill_bwd_kernel<TL, POWER>, dim3((unsigned)p.T, (unsigned)parts), NT, 0, s, p);
+  b200::count_launch();
+  return b200::check_launch("distill_bwd");
+}
+template <typename TL>
+int dispatch(const DistillParams& p, bool backward, cudaStream_t s) {
+  switch (power_of(p)) {
+    case -1: return backward ? launch_bwd<TL, -1>(p, s) : launch_fwd<TL, -1>(p, s);
+    case 0: return backward ? launch_bwd<TL, 0>(p, s) : launch_fwd<TL, 0>(p, s);
+    case 1: return backward ? launch_bwd<TL, 1>(p, s) : launch_fwd<TL, 1>(p, s);
+    case 2: return backward ? launch_bwd<TL, 2>(p, s) : launch_fwd<TL, 2>(p, s);
+    default: return backward ? launch_bwd<TL, 3>(p, s) : launch_fwd<TL, 3>(p, s);
+  }
 }
 
 }  // namespace
@@ -414,7 +500,7 @@ B200_API int b200_distill_fwd(const void* logits, int is_bf16, long long ld, con
   DistillParams p = {logits, ld, labels, ids, values, ids64, values_bf16, T, K, V, rest, alpha, tau, ignore, loss, stats, teacher, nullptr, nullptr, 0};
   if (int r = check_distill("distill_fwd", p)) return r;
   if (T == 0) return 0;
-  return is_bf16 ? launch_fwd<__nv_bfloat16>(p, (cudaStream_t)stream) : launch_fwd<float>(p, (cudaStream_t)stream);
+  return is_bf16 ? dispatch<__nv_bfloat16>(p, false, (cudaStream_t)stream) : dispatch<float>(p, false, (cudaStream_t)stream);
 }
 
 // grad [T, V] (the logits' type, rows ld_grad apart; may be the logits themselves) = gy[t] * dloss[t] / dlogits
@@ -425,13 +511,5 @@ B200_API int b200_distill_bwd(const void* logits, int is_bf16, long long ld, con
                      const_cast<float*>(stats), const_cast<double*>(teacher), gy, grad, ld_grad};
   if (int r = check_distill("distill_bwd", p)) return r;
   if (T == 0) return 0;
-  const bool both = alpha < 1.f && tau != 1.f;
-  auto k = is_bf16 ? (both ? distill_bwd_kernel<__nv_bfloat16, true> : distill_bwd_kernel<__nv_bfloat16, false>)
-                   : (both ? distill_bwd_kernel<float, true> : distill_bwd_kernel<float, false>);
-  // few rows: several CTAs a row, of 4096 columns or more
-  int parts = 1;
-  while (parts < 32 && (long long)T * parts < 2 * b200::sm_count() && V / (2 * parts) >= 4096) parts *= 2;
-  b200::launch(k, dim3((unsigned)T, (unsigned)parts), NT, 0, (cudaStream_t)stream, p);
-  b200::count_launch();
-  return b200::check_launch("distill_bwd");
+  return is_bf16 ? dispatch<__nv_bfloat16>(p, true, (cudaStream_t)stream) : dispatch<float>(p, true, (cudaStream_t)stream);
 }
