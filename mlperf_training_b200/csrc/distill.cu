@@ -95,18 +95,6 @@ struct Lse {
   B200_DEVICE float log2_s() const { return m == -INFINITY ? -INFINITY : m + log2f(s); }
   B200_DEVICE float log2_z(float tau) const { return m == -INFINITY ? -INFINITY : m * tau + log2f(z); }
 };
-template <bool Z>
-B200_DEVICE Lse<Z> block_join(Lse<Z> v, float tau, Lse<Z>* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v.join_lane(o, tau);
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
-  if (l == 0 && w < NT / 32) red[w] = v;
-  __syncthreads();
-  v = red[l % (NT / 32)];
-#pragma unroll
-  for (int o = NT / 64; o > 0; o >>= 1) v.join_lane(o, tau);
-  return v;
-}
 B200_DEVICE double warp_sum64(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -134,192 +122,247 @@ B200_DEVICE float largest(const uint4& v) {
   return fmax_nan(__low2float(m), __high2float(m));
 }
 B200_DEVICE void pairs(const float4& v, float2 (&x)[2]) { x[0] = make_float2(v.x, v.y); x[1] = make_float2(v.z, v.w); }
-B200_DEVICE void pairs(const uint4& v, float2 (&x)[4]) { x[0] = unpack_bf16x2(v.x); x[1] = unpack_bf16x2(v.y); x[2] = unpack_bf16x2(v.z); x[3] = unpack_bf16x2(v.w); }
+B200_DEVICE float2 pair(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+B200_DEVICE void pairs(const uint4& v, float2 (&x)[4]) { x[0] = pair(v.x); x[1] = pair(v.y); x[2] = pair(v.z); x[3] = pair(v.w); }
 template <typename TL> struct Raw;
 template <> struct Raw<float> { using T = float4; };
 template <> struct Raw<__nv_bfloat16> { using T = uint4; };
 
-// One CTA a row.  POWER: -1 the log-sum-exp of u alone; 1, 2, 3 that of z too, from u's terms squared so many times; 0 from an exponential
-// of its own.  REST: ids are left out of the pass.  The last warp takes the teacher, whose chain of loads and sums is about as long as a third
-// of the row (a warp that did both held the row back: 8192 x 128256 484 us, FWD_US with a warp for each).
+// A CTA takes every gridDim.x-th row.  POWER: -1 the log-sum-exp of u alone; 1, 2, 3 that of z too, from u's terms squared so many times; 0
+// from an exponential of its own.  REST: ids are left out of the pass.
+// The last warp takes the teacher, whose chain of loads and sums is about as long as a third of a row (a warp that did both held the row
+// back: 8192 x 128256 484 us, 410 with a warp for each), and the end of each row, while the others are at the next one already: their
+// first loads of it are under way before they join their sums (FWD_US).  One barrier a row: sums and marks have two copies.
 template <typename TL, int POWER, bool REST>
 __global__ void __launch_bounds__(NT + 32, 2) distill_fwd_kernel(const DistillParams p) {
   b200::begin_kernel();
   constexpr bool BOTH = POWER >= 0;
   constexpr int N = Vec<TL>::N;
-  extern __shared__ unsigned s_mark[];                 // REST: a bit for each id
-  __shared__ Lse<BOTH> red[NT / 32];
-  const long long t = blockIdx.x;
-  const int lane = threadIdx.x & 31;
-  const long long label = p.labels != nullptr ? p.labels[t] : 0;
-  float* st = p.stats + t * 4;
-  if (p.labels != nullptr && label == p.ignore) {      // (the whole CTA)
-    if (threadIdx.x == 0) {
-      p.loss[t] = 0.f;
-      st[0] = st[1] = st[2] = st[3] = 0.f;
-      p.teacher[t] = 0.;
+  using RawT = typename Raw<TL>::T;
+  extern __shared__ unsigned s_mark[];                 // REST: a bit for each id, of two rows
+  __shared__ Lse<BOTH> red[2][NT / 32];
+  const int lane = threadIdx.x & 31, words = (p.V + 31) / 32, step = gridDim.x;
+  const float cu = LOG2E / p.tau;
+  const bool teaches = threadIdx.x >= NT;
+  auto row_of = [&](long long t) { return reinterpret_cast<const TL*>(p.logits) + t * p.ld; };
+  auto label_of = [&](long long t) { return p.labels != nullptr ? p.labels[t] : 0ll; };
+  auto ignored = [&](long long label) { return p.labels != nullptr && label == p.ignore; };
+  // entry j of token t: its id, or -1 where it is not there
+  auto entry = [&](long long t, int j, float& val) -> int {
+    const long long v = id_at(p, t * p.K + j);
+    val = value_at(p, t * p.K + j);
+    return v >= 0 && v < p.V && val != -INFINITY ? (int)v : -1;
+  };
+  // (REST, the teacher) marks the ids of token t; bit i of the result: entry lane + 32 i is the first of its id
+  auto mark = [&](long long t, unsigned* marks) -> unsigned {
+    unsigned first = 0u;
+    float val;
+    if (t < p.T && p.alpha > 0.f && !ignored(label_of(t)))
+      for (int j = lane; j < p.K; j += 32) {
+        const int v = entry(t, j, val);
+        if (v >= 0 && !(atomicOr(&marks[v >> 5], 1u << (v & 31)) >> (v & 31) & 1u)) first |= 1u << (j >> 5);
+      }
+    return first;
+  };
+  unsigned first = 0u;
+  if (REST) {
+    for (int i = threadIdx.x; i < 2 * words; i += NT + 32) s_mark[i] = 0u;
+    __syncthreads();
+    if (teaches) first = mark(blockIdx.x, s_mark);
+    __syncthreads();
+  }
+
+  if (teaches) {
+    for (int t = blockIdx.x, n = 0; t < p.T; t += step, ++n) {
+      const long long label = label_of(t);
+      const bool live = !ignored(label);
+      const TL* row = row_of(t);
+      unsigned* marks = s_mark + (n & 1) * words;
+      Teacher te;
+      Lse<BOTH> ids;                                   // (REST) terms of the ids, each once
+      float zlabel = 0.f;
+      if (live && p.alpha < 1.f && label >= 0 && label < p.V) zlabel = load1(row + label);
+      if (live && p.alpha > 0.f) {
+        if (!p.rest) {
+          double m = -INFINITY, s = 0.;
+          float val;
+          for (int j = lane; j < p.K; j += 32)
+            if (entry(t, j, val) >= 0) m = fmax(m, (double)val / p.tau);
+          m = warp_max64(m);
+          for (int j = lane; j < p.K; j += 32)
+            if (entry(t, j, val) >= 0) s += exp((double)val / p.tau - m);
+          s = warp_sum64(s);
+          te.log_sum = s != 0. ? m + log(s) : 0.;      // (no entry: s = 0)
+        }
+        for (int j = lane; j < p.K; j += 32) {
+          float val;
+          const int id = entry(t, j, val);
+          if (id < 0) continue;
+          const float zid = load1(row + id);
+          if (REST && (first >> (j >> 5) & 1u)) ids.join(zid * cu, 1.f, 1.f, p.tau);
+          const double logp = p.rest ? (double)val : (double)val / p.tau - te.log_sum, pj = exp(logp);
+          te.mass += pj;
+          if (pj != 0.) { te.own += pj * logp; te.cross += pj * ((double)zid / p.tau); }
+        }
+        te.mass = warp_sum64(te.mass);
+        te.own = warp_sum64(te.own);
+        te.cross = warp_sum64(te.cross);
+        if (REST)
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) ids.join_lane(o, p.tau);
+      }
+      unsigned next = 0u;
+      if (REST) next = mark((long long)t + step, s_mark + (1 - (n & 1)) * words);
+      __syncthreads();                                 // the row's sums are there, its marks are no longer read
+      if (REST && first) {
+        float val;
+        for (int j = lane; j < p.K; j += 32)
+          if (first >> (j >> 5) & 1u) marks[entry(t, j, val) >> 5] = 0u;
+      }
+      __syncwarp();
+      first = next;
+      Lse<BOTH> acc = red[n & 1][lane % (NT / 32)];
+#pragma unroll
+      for (int o = NT / 64; o > 0; o >>= 1) acc.join_lane(o, p.tau);
+      if (lane != 0) continue;
+      float* st = p.stats + (long long)t * 4;
+      if (!live) {
+        p.loss[t] = 0.f;
+        st[0] = st[1] = st[2] = st[3] = 0.f;
+        p.teacher[t] = 0.;
+        continue;
+      }
+      // with REST the sums are those of the others, and the ids join them
+      const float others = acc.log2_s();
+      if (REST) acc.join(ids.m, ids.s, ids.z, p.tau);
+      const float lse_u = acc.log2_s(), lse_z = BOTH ? acc.log2_z(p.tau) : lse_u;
+      double loss = 0., c = te.mass, ratio = 0.;
+      if (p.alpha > 0.f) {
+        const double ln2 = 0.6931471805599453094, lse = (double)lse_u * ln2;
+        double kl = te.own - te.cross + (te.mass != 0. ? te.mass * lse : 0.);
+        if (REST) {
+          const double r = 1. - c;
+          if (r > 0. && others > -INFINITY) {          // (no id left outside: nothing for the rest to be)
+            const double lr = (double)(others - lse_u) * ln2;
+            kl += r * (log(r) - lr);
+            ratio = r / exp(lr);
+            c += r;
+          }
+        }
+        loss = (double)p.alpha * p.tau * p.tau * kl;
+      }
+      if (p.alpha < 1.f && label >= 0 && label < p.V) loss += (1. - (double)p.alpha) * (double)(lse_z * LN2 - zlabel);
+      p.loss[t] = (float)loss;
+      st[0] = lse_u;
+      st[1] = lse_z;
+      st[2] = (float)c;
+      st[3] = (float)ratio;
+      p.teacher[t] = te.log_sum;
     }
     return;
   }
-  const TL* row = reinterpret_cast<const TL*>(p.logits) + t * p.ld;
-  const float cu = LOG2E / p.tau;
-  // the teacher: warp 0 (the others meanwhile begin with the row)
-  Teacher te;
-  Lse<BOTH> ids;                                       // (REST) terms of the ids, each once
-  float zlabel = 0.f;
-  unsigned first = 0u;                                 // (REST) bit i: entry lane + 32 i is the first of its id
-  const bool teaches = threadIdx.x >= NT;
-  using RawT = typename Raw<TL>::T;
-  const Span sp = span_of(row, 0, p.V);
-  const RawT* vecs = reinterpret_cast<const RawT*>(row + sp.first);
+
+  // ------------------------------ the rows ------------------------------
   RawT raw[AHEAD];
-  if (!teaches) {
+  long long label = 0;
+  auto begin = [&](int t) {                            // its label and first loads
+    if (t >= p.T) return;
+    label = label_of(t);
+    const TL* row = row_of(t);
+    const Span sp = span_of(row, 0, p.V);
+    const RawT* vecs = reinterpret_cast<const RawT*>(row + sp.first);
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
       if (i * NT + (int)threadIdx.x < sp.n) raw[i] = vecs[i * NT + (int)threadIdx.x];
-  }
-  if (REST) {
-    for (int i = threadIdx.x; i < (p.V + 31) / 32; i += NT + 32) s_mark[i] = 0u;
-    __syncthreads();
-    // the ids are marked before the pass begins; who marked one first has it in `first`
-    if (teaches && p.alpha > 0.f)
-      for (int j = lane; j < p.K; j += 32) {
-        const long long v = id_at(p, t * p.K + j);
-        if (v >= 0 && v < p.V && value_at(p, t * p.K + j) != -INFINITY && !(atomicOr(&s_mark[v >> 5], 1u << (v & 31)) >> (v & 31) & 1u))
-          first |= 1u << (j >> 5);
-      }
-    __syncthreads();
-  }
-  if (teaches) {
-    if (p.alpha < 1.f && label >= 0 && label < p.V) zlabel = load1(row + label);
-    auto entry = [&](int j, float& val) -> int {       // the id, or -1 where the entry is not there
-      const long long v = id_at(p, t * p.K + j);
-      val = value_at(p, t * p.K + j);
-      return v >= 0 && v < p.V && val != -INFINITY ? (int)v : -1;
-    };
-    if (p.alpha > 0.f) {
-      if (!p.rest) {
-        double m = -INFINITY, s = 0.;
-        float val;
-        for (int j = lane; j < p.K; j += 32)
-          if (entry(j, val) >= 0) m = fmax(m, (double)val / p.tau);
-        m = warp_max64(m);
-        for (int j = lane; j < p.K; j += 32)
-          if (entry(j, val) >= 0) s += exp((double)val / p.tau - m);
-        s = warp_sum64(s);
-        te.log_sum = s != 0. ? m + log(s) : 0.;        // (no entry: s = 0)
-      }
-      for (int j = lane; j < p.K; j += 32) {
-        float val;
-        const int id = entry(j, val);
-        if (id < 0) continue;
-        const float zid = load1(row + id);
-        if (REST && (first >> (j >> 5) & 1u)) ids.join(zid * cu, 1.f, 1.f, p.tau);
-        const double logp = p.rest ? (double)val : (double)val / p.tau - te.log_sum, pj = exp(logp);
-        te.mass += pj;
-        if (pj != 0.) { te.own += pj * logp; te.cross += pj * ((double)zid / p.tau); }
-      }
-      te.mass = warp_sum64(te.mass);
-      te.own = warp_sum64(te.own);
-      te.cross = warp_sum64(te.cross);
-      if (REST)
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ids.join_lane(o, p.tau);
-    }
-  }
-
-  // the pass, in units of log2
-  Lse<BOTH> acc;
-  float2 s2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);       // sums on acc.m
-  auto raise = [&](float mx) {                         // the maximum seen so far; a NaN goes on to the sums
-    const float n = mx * cu;
-    if (!(n <= acc.m)) {
-      if (acc.m > -INFINITY) {
-        const float f = ex2_approx(acc.m - n);
-        s2 = fmul2(s2, make_float2(f, f));
-        if (BOTH) {
-          const float g = ex2_approx((acc.m - n) * p.tau);
-          z2 = fmul2(z2, make_float2(g, g));
-        }
-      }
-      acc.m = n;
-    }
   };
-  auto add = [&](float2 x) {
-    const float2 a = ffma2(x, make_float2(cu, cu), make_float2(-acc.m, -acc.m));
-    float2 e = make_float2(ex2_approx(a.x), ex2_approx(a.y));
-    s2 = fadd2(s2, e);
-    if (POWER >= 1) {
-#pragma unroll
-      for (int i = 1; i < POWER; ++i) e = fmul2(e, e);
-      z2 = ffma2(e, e, z2);
-    }
-    if (POWER == 0) z2 = fadd2(z2, make_float2(ex2_approx(a.x * p.tau), ex2_approx(a.y * p.tau)));
-  };
-  auto take1 = [&](int c) {                            // one element
-    if (REST && (s_mark[c >> 5] >> (c & 31) & 1u)) return;
-    const float x = load1(row + c);
-    raise(x);
-    if (acc.m != -INFINITY) add(make_float2(x, -INFINITY));
-  };
-  if (!teaches) {
-    for (int v0 = threadIdx.x; v0 < sp.n; v0 += NT * AHEAD) {
-#pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        const int v = v0 + i * NT, later = v + AHEAD * NT;
-        const RawT now = raw[i];
-        if (later < sp.n) raw[i] = vecs[later];
-        if (v >= sp.n) continue;
-        if (REST) {
-          // N bits from bit c on
-          const int c = sp.first + v * N;
-          const unsigned lo = s_mark[c >> 5], hi = (c & 31) + N > 32 ? s_mark[(c >> 5) + 1] : 0u;
-          if (__funnelshift_r(lo, hi, c & 31) & ((1u << N) - 1u)) {
-            for (int k = 0; k < N; ++k) take1(c + k);
-            continue;
+  begin(blockIdx.x);
+  for (int t = blockIdx.x, n = 0; t < p.T; t += step, ++n) {
+    const TL* row = row_of(t);
+    const unsigned* marks = s_mark + (n & 1) * words;
+    Lse<BOTH> acc;                                     // in units of log2
+    if (!ignored(label)) {
+      float2 s2 = make_float2(0.f, 0.f), z2 = make_float2(0.f, 0.f);       // sums on acc.m
+      auto raise = [&](float mx) {                     // the maximum seen so far; a NaN goes on to the sums
+        const float m = mx * cu;
+        if (!(m <= acc.m)) {
+          if (acc.m > -INFINITY) {
+            const float f = ex2_approx(acc.m - m);
+            s2 = fmul2(s2, make_float2(f, f));
+            if (BOTH) {
+              const float g = ex2_approx((acc.m - m) * p.tau);
+              z2 = fmul2(z2, make_float2(g, g));
+            }
           }
+          acc.m = m;
         }
-        raise(largest(now));
-        if (acc.m == -INFINITY) continue;
-        float2 x[N / 2];
-        pairs(now, x);
+      };
+      auto add = [&](float2 x) {
+        const float2 a = ffma2(x, make_float2(cu, cu), make_float2(-acc.m, -acc.m));
+        float2 e = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+        s2 = fadd2(s2, e);
+        if (POWER >= 1) {
 #pragma unroll
-        for (int k = 0; k < N / 2; ++k) add(x[k]);
+          for (int i = 1; i < POWER; ++i) e = fmul2(e, e);
+          z2 = ffma2(e, e, z2);
+        }
+        if (POWER == 0) z2 = fadd2(z2, make_float2(ex2_approx(a.x * p.tau), ex2_approx(a.y * p.tau)));
+      };
+      auto take1 = [&](int c) {                        // one element
+        if (REST && (marks[c >> 5] >> (c & 31) & 1u)) return;
+        const float x = load1(row + c);
+        raise(x);
+        if (acc.m != -INFINITY) add(make_float2(x, -INFINITY));
+      };
+      const Span sp = span_of(row, 0, p.V);
+      const RawT* vecs = reinterpret_cast<const RawT*>(row + sp.first);
+      const int head = sp.first - sp.lo, edge = head + (sp.hi - sp.first - sp.n * N);        // fewer than 2 N elements
+      auto take_edge = [&]() {
+        if ((int)threadIdx.x < edge) take1((int)threadIdx.x < head ? sp.lo + (int)threadIdx.x : sp.first + sp.n * N + (int)threadIdx.x - head);
+      };
+      // The sums go over the largest of the thread's first elements, without a look at the others: 36 instead of 83 instructions for 8
+      // elements.  Where that was no measure (an element 2^127 above it, none at all), the thread goes over its part once more.
+      if ((int)threadIdx.x < sp.n) acc.m = fmax_nan(largest(raw[0]) * cu, -1e30f);
+      for (int v0 = threadIdx.x; v0 < sp.n; v0 += NT * AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const int v = v0 + i * NT, later = v + AHEAD * NT;
+          const RawT now = raw[i];
+          if (later < sp.n) raw[i] = vecs[later];
+          if (v >= sp.n) continue;
+          if (REST) {
+            // N bits from bit c on
+            const int c = sp.first + v * N;
+            const unsigned lo = marks[c >> 5], hi = (c & 31) + N > 32 ? marks[(c >> 5) + 1] : 0u;
+            if (__funnelshift_r(lo, hi, c & 31) & ((1u << N) - 1u)) {
+              for (int k = 0; k < N; ++k) take1(c + k);
+              continue;
+            }
+          }
+          float2 x[N / 2];
+          pairs(now, x);
+#pragma unroll
+          for (int k = 0; k < N / 2; ++k) add(x[k]);
+        }
+      }
+      take_edge();
+      acc.s = s2.x + s2.y;
+      acc.z = z2.x + z2.y;
+      if (!(acc.s > 0.f && acc.s < INFINITY) || (BOTH && !(acc.z > 0.f && acc.z < INFINITY))) {
+        acc.m = -INFINITY;
+        s2 = z2 = make_float2(0.f, 0.f);
+        for (int v = threadIdx.x; v < sp.n; v += NT)
+          for (int k = 0; k < N; ++k) take1(sp.first + v * N + k);
+        take_edge();
+        acc.s = s2.x + s2.y;
+        acc.z = z2.x + z2.y;
       }
     }
-    const int head = sp.first - sp.lo, edge = head + (sp.hi - sp.first - sp.n * N);        // fewer than 2 N elements
-    if ((int)threadIdx.x < edge) take1((int)threadIdx.x < head ? sp.lo + (int)threadIdx.x : sp.first + sp.n * N + (int)threadIdx.x - head);
+    if (p.T - t > step) begin(t + step);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc.join_lane(o, p.tau);
+    if (lane == 0) red[n & 1][threadIdx.x >> 5] = acc;
+    __syncthreads();
   }
-  acc.s = s2.x + s2.y;
-  acc.z = z2.x + z2.y;
-  acc = block_join<BOTH>(acc, p.tau, red);
-  if (threadIdx.x != NT) return;                       // (the teacher's first lane)
-  // with REST the sums are those of the others, and the ids join them
-  const float others = acc.log2_s();
-  if (REST) acc.join(ids.m, ids.s, ids.z, p.tau);
-  const float lse_u = acc.log2_s(), lse_z = BOTH ? acc.log2_z(p.tau) : lse_u;
-  double loss = 0., c = te.mass, ratio = 0.;
-  if (p.alpha > 0.f) {
-    const double ln2 = 0.6931471805599453094, lse = (double)lse_u * ln2;
-    double kl = te.own - te.cross + (te.mass != 0. ? te.mass * lse : 0.);
-    if (REST) {
-      const double r = 1. - c;
-      if (r > 0. && others > -INFINITY) {              // (no id left outside: nothing for the rest to be)
-        const double lr = (double)(others - lse_u) * ln2;
-        kl += r * (log(r) - lr);
-        ratio = r / exp(lr);
-        c += r;
-      }
-    }
-    loss = (double)p.alpha * p.tau * p.tau * kl;
-  }
-  if (p.alpha < 1.f && label >= 0 && label < p.V) loss += (1. - (double)p.alpha) * (double)(lse_z * LN2 - zlabel);
-  p.loss[t] = (float)loss;
-  st[0] = lse_u;
-  st[1] = lse_z;
-  st[2] = (float)c;
-  st[3] = (float)ratio;
-  p.teacher[t] = te.log_sum;
 }
 
 // CTA (t, part): columns [part, part + 1) * V / parts of row t.
@@ -361,10 +404,11 @@ __global__ void __launch_bounds__(NT, 2) distill_bwd_kernel(const DistillParams 
     if (threadIdx.x == 0 && labelled && label >= lo && label < hi) zlabel = load1(row + label);
     __syncthreads();
   }
-  // e^(z - lse_z) from e^(u - lse_u): its tau-th power times 2^(tau lse_u - lse_z)
-  const float gp = POWER >= 1 ? gz * ex2_approx(p.tau * lse_u - lse_z) : 0.f;
+  // (POWER above 0) q1 is the tau-th power of e^(u - lse_z / tau), which is at most 1, and q that times 2^(lse_z / tau - lse_u)
+  const float shift = POWER >= 1 ? lse_z / p.tau : lse_u;
+  const float fe = POWER >= 1 ? fu * ex2_approx(shift - lse_u) : fu;
   auto other = [&](float2 x) -> float2 {
-    const float2 a = ffma2(x, make_float2(cu, cu), make_float2(-lse_u, -lse_u));
+    const float2 a = ffma2(x, make_float2(cu, cu), make_float2(-shift, -shift));
     float2 e = make_float2(ex2_approx(a.x), ex2_approx(a.y));
     if (POWER < 0) return fmul2(e, make_float2(fu + gz, fu + gz));
     float2 z;
@@ -372,12 +416,12 @@ __global__ void __launch_bounds__(NT, 2) distill_bwd_kernel(const DistillParams 
       z = fmul2(e, e);
 #pragma unroll
       for (int i = 1; i < POWER; ++i) z = fmul2(z, z);
-      z = fmul2(z, make_float2(gp, gp));
+      z = fmul2(z, make_float2(gz, gz));
     } else {
       const float2 b = ffma2(x, make_float2(LOG2E, LOG2E), make_float2(-lse_z, -lse_z));
       z = fmul2(make_float2(ex2_approx(b.x), ex2_approx(b.y)), make_float2(gz, gz));
     }
-    return ffma2(e, make_float2(fu, fu), z);
+    return ffma2(e, make_float2(fe, fe), z);
   };
   const Span sp = span_of(out, lo, hi);
   const bool vec = (((uintptr_t)row ^ (uintptr_t)out) & 15) == 0;     // both rows are aligned at the same columns
@@ -465,9 +509,10 @@ int power_of(const DistillParams& p) {
 template <typename TL, int POWER>
 int launch_fwd(const DistillParams& p, cudaStream_t s) {
   auto k = p.rest ? distill_fwd_kernel<TL, POWER, true> : distill_fwd_kernel<TL, POWER, false>;
-  const size_t smem = p.rest ? ((size_t)p.V + 31) / 32 * 4 : 0;
+  const size_t smem = p.rest ? ((size_t)p.V + 31) / 32 * 8 : 0;
   if (int r = set_smem((const void*)k, smem)) return r;
-  b200::launch(k, p.T, NT + 32, smem, s, p);
+  const int grid = p.T < 2 * b200::sm_count() ? p.T : 2 * b200::sm_count();
+  b200::launch(k, grid, NT + 32, smem, s, p);
   b200::count_launch();
   return b200::check_launch("distill_fwd");
 }

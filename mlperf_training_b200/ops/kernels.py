@@ -494,7 +494,7 @@ def cross_entropy_(logits: torch.Tensor, labels: torch.Tensor, grad_scale: float
 # distillation from a teacher's largest logits
 # --------------------------------------------------------------------------------------
 DISTILL_MAX_K = 1024
-DISTILL_MAX_REST_V = 1 << 20       # ids are marked in shared memory, a bit each
+DISTILL_MAX_REST_V = 900_000       # ids are marked in shared memory, a bit each for two tokens at a time
 
 
 def _distill_check(logits, labels, ids, values, alpha, temperature, rest) -> None:

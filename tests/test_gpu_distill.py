@@ -113,6 +113,36 @@ def test_a_bad_token_stays_alone():
     assert loss[8].isnan() and loss[12].isnan()
 
 
+def test_logits_far_apart():
+    """Rows whose first elements say nothing about the largest: differences that overflow a sum, and rows of -inf but for a few."""
+    T, V = 12, 5003
+    z, labels, ids, val, gy = inputs(T, V, 6, False, torch.float32)
+    z[0, 4000] = 300.0
+    z[1] -= 2000.0
+    z[1, 17] = 50.0
+    z[2] = float("-inf")
+    z[2, 4999], z[2, 1] = 3.0, 2.0
+    ids[2] = torch.tensor([4999, 1, -1, -1, -1, -1])
+    labels[2] = 1
+    z[3] = torch.linspace(-500, 500, V)
+    z[6, ::2] = float("-inf")
+    labels[6], ids[6] = 1, ids[6] // 2 * 2 + 1
+    for cfg in CONFIGS:
+        v = torch.log_softmax(val, 1) - 0.5 if cfg.get("rest") else val
+        want, grad, size = exact(z, labels, ids, v, gy, cfg)
+        x = z.cuda().requires_grad_(True)
+        loss = F.distill_loss(x, labels.cuda(), ids.cuda(), v.cuda(), **cfg)
+        (dx,) = torch.autograd.grad(loss, x, gy.cuda())
+        a, tau = cfg.get("alpha", 1.0), cfg.get("temperature", 1.0)
+        # exponents up to 2000 / ln 2 in size and the losses themselves, rounded to fp32
+        d = relative(V) + 3000 / min(tau, 1.0) * 2 ** -24
+        fine = torch.isfinite(want)
+        assert torch.equal(fine, torch.isfinite(loss.cpu()))
+        assert ((loss.cpu().double() - want).abs() <= (a * tau * tau * 2 + (1 - a)) * d + 2 ** -22 * want.abs())[fine].all()
+        assert ((dx.cpu().double() - grad).abs() <= 2 ** -24 * 1.01 * grad.abs() + 3 * d * size + 1e-30)[fine].all()
+    _lib.check_status("distill")
+
+
 def test_masked_vocabulary():
     z, labels, ids, val, gy = inputs(19, 333, 4, False, torch.bfloat16)
     z[:, 300:] = float("-inf")
