@@ -37,25 +37,41 @@ struct ScoreParams {
   float scale;              // of the products
   float cap;                // c of c tanh(s / c), or 0
   const float* slopes;      // [Hq]: what a key at distance d loses is slope * d, or null
+  float into, back;         // with a cap: what takes a product into the tangent, c log2(e)
+  float limit, k[5];        // products up to `limit` in size: back * tanh(into * s) = s * (k0 + k1 s^2 + .. + k4 s^8)
+
+  // tanh(x) for |x| <= 1 is x times a polynomial in x^2, fitted to the smallest largest relative error there (7e-6: 3.5e-4 of a score capped at
+  // 50); the coefficients take the scales in.  A capped score would otherwise take an exponential and a reciprocal more, and the
+  // softmax warps are bound by the MUFU unit as it is.
+  static ScoreParams of(float scale, float cap, const float* slopes) {
+    ScoreParams p = {scale, cap, slopes, 0.f, 0.f, 0.f, {0.f, 0.f, 0.f, 0.f, 0.f}};
+    if (cap > 0.f) {
+      const double c[5] = {0.99999309, -0.33298064, 0.13036807, -0.04481748, 0.00903639}, into = (double)scale / cap, back = cap * 1.4426950408889634;
+      p.into = (float)into;
+      p.back = (float)back;
+      double w = back * into;
+      for (int i = 0; i < 5; ++i, w *= into * into) p.k[i] = (float)(c[i] * w);
+      p.limit = into > 1e-4 && into < 1e3 ? (float)(1. / into) : 0.f;      // (powers of the scales that fp32 does not hold: never)
+    }
+    return p;
+  }
 };
 
-// tanh(x) for |x| <= 1: x times a polynomial in x^2, fitted to the smallest largest relative error there (7e-6: 3.5e-4 of a score
-// capped at 50).  A capped score would otherwise take an exponential and a reciprocal more, and the softmax warps are bound by the MUFU
-// unit as it is.
-B200_DEVICE float2 tanh_small2(float2 x) {
-  const float2 q = fmul2(x, x);
-  float2 r = ffma2(q, make_float2(0.00903639f, 0.00903639f), make_float2(-0.04481748f, -0.04481748f));
-  r = ffma2(r, q, make_float2(0.13036807f, 0.13036807f));
-  r = ffma2(r, q, make_float2(-0.33298064f, -0.33298064f));
-  r = ffma2(r, q, make_float2(0.99999309f, 0.99999309f));
-  return fmul2(r, x);
+// Capped scores, in units of log2, of a pair of products: of at most `limit` in size, and of any.
+B200_DEVICE float2 capped_small2(float2 s, const ScoreParams& p) {
+  const float2 q = fmul2(s, s);
+  float2 r = ffma2(q, make_float2(p.k[4], p.k[4]), make_float2(p.k[3], p.k[3]));
+  r = ffma2(r, q, make_float2(p.k[2], p.k[2]));
+  r = ffma2(r, q, make_float2(p.k[1], p.k[1]));
+  r = ffma2(r, q, make_float2(p.k[0], p.k[0]));
+  return fmul2(r, s);
 }
-// any x: 1 - 2 / (1 + e^2x), absolute error below 3e-7
-B200_DEVICE float tanh_any(float x) {
-  const float e = ex2_approx(x * (2.f * LOG2E));
+// tanh(x) = 1 - 2 / (1 + e^2x), absolute error below 3e-7
+B200_DEVICE float capped_any(float s, const ScoreParams& p) {
+  const float e = ex2_approx(s * p.into * (2.f * LOG2E));
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return fmaf(-2.f, r, 1.f);
+  return p.back * fmaf(-2.f, r, 1.f);
 }
 
 }  // namespace b200

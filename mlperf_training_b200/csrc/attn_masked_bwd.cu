@@ -304,28 +304,27 @@ attn_masked_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       tmem_ld_32x32b_x32(tm_S + lane_base + half * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
       tc_wait_ld();
       if (SCORE & b200::SCORE_CAP) {
-        const float into = p.score.scale / p.score.cap, back = p.score.cap * b200::LOG2E;
+        const float inv2 = -1.f / (p.score.back * p.score.back);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float big = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; ++i) big = fmaxf(big, fabsf(__uint_as_float(s[c * 32 + i])));
-          if (__all_sync(0xffffffffu, big * into <= 1.f)) {
+          if (__all_sync(0xffffffffu, big <= p.score.limit)) {
 #pragma unroll
             for (int i = c * 32; i < c * 32 + 32; i += 2) {
-              const float2 t = b200::tanh_small2(fmul2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(into, into)));
-              const float2 f = ffma2(make_float2(-t.x, -t.y), t, make_float2(1.f, 1.f));
-              pr[i] = t.x * back; pr[i + 1] = t.y * back;
-              s[i] = __float_as_uint(f.x); s[i + 1] = __float_as_uint(f.y);
+              const float2 y = b200::capped_small2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), p.score);
+              pr[i] = y.x; pr[i + 1] = y.y;
             }
           } else {
 #pragma unroll
-            for (int i = c * 32; i < c * 32 + 32; ++i) {
-              const float t = b200::tanh_any(__uint_as_float(s[i]) * into);
-              pr[i] = t * back;
-              s[i] = __float_as_uint(fmaf(-t, t, 1.f));
-            }
+            for (int i = c * 32; i < c * 32 + 32; ++i) pr[i] = b200::capped_any(__uint_as_float(s[i]), p.score);
           }
+        }
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) {
+          const float2 y = make_float2(pr[i], pr[i + 1]), f = ffma2(fmul2(y, make_float2(inv2, inv2)), y, make_float2(1.f, 1.f));
+          s[i] = __float_as_uint(f.x); s[i + 1] = __float_as_uint(f.y);
         }
       } else {
 #pragma unroll
@@ -589,7 +588,7 @@ B200_API int b200_attn_masked_bwd(const void* q, const void* k, const void* v, c
   const long long tiles = (long long)B * Hkv * nk;
   BwdParams p;
   p.mask = b200::MaskView::of(mask, lay);
-  p.score = {scale, cap, slopes};
+  p.score = b200::ScoreParams::of(scale, cap, slopes);
   p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Skv = Skv;
   p.scale_log2 = scale * b200::LOG2E;
   p.lse = lse; p.delta = delta;

@@ -48,15 +48,27 @@ struct Item {
   B200_DEVICE int lo(int t) const { return t ? lo1 : lo0; }
   B200_DEVICE int hi(int t) const { return t ? hi1 : hi0; }
 };
-B200_DEVICE Item make_item(int u, const FwdParams& p) {
+// What the mask's tables say about item u.  The roles load it an item ahead: two loads in a row, more than a key tile's time.
+struct Entry {
+  int id = 0;
+  int4 a = {0, 0, 0, 0}, c = {0, 0, 0, 0};
+};
+B200_DEVICE Entry load_entry(int u, const FwdParams& p) {
+  Entry e;
+  if (u >= p.items) return e;
+  e.id = p.mask.oq[u / p.Hq];                            // b * pairs + pair: its query tiles are entries 2 id and 2 id + 1
+  e.a = p.mask.qt[2ll * e.id];
+  e.c = p.mask.qt[2ll * e.id + 1];
+  return e;
+}
+B200_DEVICE Item make_item(int u, const Entry& e, const FwdParams& p) {
   Item it;
   const int np = p.mask.Sp / 256;
-  const int id = p.mask.oq[u / p.Hq];
   it.h = u % p.Hq;
-  it.b = id / np;
-  const int pair = id - it.b * np;
+  it.b = e.id / np;
+  const int pair = e.id - it.b * np;
   it.q0 = pair * 2 * BQ;
-  const int4 a = p.mask.qt[(long long)it.b * (2 * np) + 2 * pair], c = p.mask.qt[(long long)it.b * (2 * np) + 2 * pair + 1];
+  const int4 a = e.a, c = e.c;
   const bool has0 = a.y > a.x, has1 = c.y > c.x;
   it.j_lo = has0 ? a.x : c.x;
   it.lo0 = 0;
@@ -87,7 +99,8 @@ struct Smem {
   static constexpr int TOTAL = 2 * Q_TILE + 4 * KV_BYTES + 8 * STAGE_O + 1024 + 256;
 };
 
-template <int HD, int SCORE>
+// LOW: what the output loses to bf16 is written too, and row sums go over the rounded probabilities (a backward pass follows).
+template <int HD, int SCORE, bool LOW>
 __global__ void __launch_bounds__(NTHREADS, 1)
 attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -144,10 +157,12 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
       bool ok = true;
       int kv = 0, nq = 0;                    // key tiles and items so far: stage and phase of the barriers
+      Entry next = load_entry(item_of_round(0), p);
       for (int r = 0; r < rounds && ok; ++r) {
         const int u = item_of_round(r);
         if (u >= p.items) continue;
-        const Item it = make_item(u, p);
+        const Item it = make_item(u, next, p);
+        next = load_entry(item_of_round(r + 1), p);
         if (it.n_max == 0) continue;
         const int hk = it.h / (p.Hq / p.Hkv);
         if (!mbar_wait(q_empty, (nq & 1) ^ 1, abort_flag, p.status, 39)) { ok = false; break; }
@@ -184,10 +199,12 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       bool ok = true;
       int kv = 0, nq = 0;
       int np[2] = {0, 0}, no[2] = {0, 0};    // P tiles consumed / items finished per query tile
+      Entry next = load_entry(item_of_round(0), p);
       for (int r = 0; r < rounds && ok; ++r) {
         const int u = item_of_round(r);
         if (u >= p.items) continue;
-        const Item it = make_item(u, p);
+        const Item it = make_item(u, next, p);
+        next = load_entry(item_of_round(r + 1), p);
         if (it.n_max == 0) continue;
         if (!warp_wait_spin(q_full, nq & 1, abort_flag, p.status, 50)) { ok = false; break; }
         ++nq;
@@ -281,10 +298,11 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     int ns = 0, no = 0;                    // S tiles and items so far
     int kv = 0;                            // key tiles before this item: stages and phases of V
     bool ok = true;
+    Entry next = load_entry(item_of_round(0), p);
     for (int round = 0; round < rounds && ok; ++round) {
       const int u = item_of_round(round);
       if (u >= p.items) continue;
-      const Item it = make_item(u, p);
+      const Item it = make_item(u, next, p);
       const int qt0 = it.q0 + t * BQ;
       const int q_pos = qt0 + r;
       const int kv_item = kv;
@@ -295,10 +313,11 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 #pragma unroll
           for (int i = 0; i < HD / 8; ++i) {
             *reinterpret_cast<uint4*>(p.out + at + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
-            if (p.low != nullptr) *reinterpret_cast<uint4*>(p.low + at + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
+            if (LOW) *reinterpret_cast<uint4*>(p.low + at + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
           }
           p.lse[((long long)it.b * p.Hq + it.h) * p.Sq + q_pos] = p.sink != nullptr ? p.sink[it.h] : -INFINITY;
         }
+        next = load_entry(item_of_round(round + 1), p);
         continue;
       }
       const int2 seen = p.mask.q_iv[(long long)it.b * p.mask.Sp + q_pos];            // keys [x, y) of this row
@@ -334,24 +353,21 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         tc_wait_ld();
         if (SCORE & b200::SCORE_CAP) {
           // cap * tanh(s / cap), in units of log2
-          const float into = p.score.scale / p.score.cap, back = p.score.cap * b200::LOG2E;
 #pragma unroll
           for (int c = 0; c < BKV / 32; ++c) {
             float big = 0.f;
 #pragma unroll
             for (int i = 0; i < 32; i += 2)
               big = max3(big, fabsf(__uint_as_float(v[c * 32 + i])), fabsf(__uint_as_float(v[c * 32 + i + 1])));
-            if (__all_sync(0xffffffffu, big * into <= 1.f)) {
+            if (__all_sync(0xffffffffu, big <= p.score.limit)) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                float2 x = fmul2(make_float2(__uint_as_float(v[c * 32 + i]), __uint_as_float(v[c * 32 + i + 1])), make_float2(into, into));
-                x = fmul2(b200::tanh_small2(x), make_float2(back, back));
-                v[c * 32 + i] = __float_as_uint(x.x);
-                v[c * 32 + i + 1] = __float_as_uint(x.y);
+              for (int i = c * 32; i < c * 32 + 32; i += 2) {
+                const float2 y = b200::capped_small2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), p.score);
+                v[i] = __float_as_uint(y.x); v[i + 1] = __float_as_uint(y.y);
               }
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[c * 32 + i] = __float_as_uint(back * b200::tanh_any(__uint_as_float(v[c * 32 + i]) * into));
+              for (int i = c * 32; i < c * 32 + 32; ++i) v[i] = __float_as_uint(b200::capped_any(__uint_as_float(v[i]), p.score));
             }
           }
         }
@@ -406,9 +422,9 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         const float scale2 = SCORE == b200::SCORE_PLAIN ? p.scale_log2 : 1.f;
         const float2 sc2 = make_float2(scale2, scale2);
         const float2 nm2 = make_float2(-m_use, -m_use);
+        uint32_t pk[BKV / 2];
 #pragma unroll
         for (int c = 0; c < BKV / 32; ++c) {
-          uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int e = c * 32 + 2 * i;
@@ -416,10 +432,10 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             float2 x;
             if (SCORE == b200::SCORE_PLAIN && (i & POLY) == POLY) x = ex2_poly2(a);
             else x = make_float2(ex2_approx(a.x), ex2_approx(a.y));
-            pk[i] = pack_bf16x2(x.x, x.y);
-            v[e] = pk[i] << 16; v[e + 1] = pk[i] & 0xffff0000u;      // as they are multiplied
+            pk[c * 16 + i] = pack_bf16x2(x.x, x.y);
+            if (!LOW) { v[e] = __float_as_uint(x.x); v[e + 1] = __float_as_uint(x.y); }
           }
-          tmem_st_32x32b_x16(ts + c * 16, pk);
+          tmem_st_32x32b_x16(ts + c * 16, *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
           if (c == PV_EARLY / 32 - 1 || c == BKV / 32 - 1) {
             tc_wait_st();
             tc_fence_before();
@@ -427,14 +443,16 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             if (lane == 0) mbar_arrive(c == BKV / 32 - 1 ? &p_full[t] : &p_early[t]);
           }
         }
-        // the row sum of the rounded probabilities, off the path of the MMAs
+        // the row sum, off the path of the MMAs
         float2 rs2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int i = 0; i < BKV / 2; ++i)
-          rs2[i & 1] = fadd2(rs2[i & 1], make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
+          rs2[i & 1] = fadd2(rs2[i & 1], LOW ? make_float2(__uint_as_float(pk[i] << 16), __uint_as_float(pk[i] & 0xffff0000u))
+                                             : make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
         l += (rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y);
       }
       // ------------------------------ epilogue ------------------------------
+      next = load_entry(item_of_round(round + 1), p);          // (not before: the scores take the registers)
       if (!ok || !warp_wait(&o_done[t], no & 1, abort_flag, p.status, 62)) { ok = false; break; }
       ++no;
       tc_fence_after();
@@ -464,7 +482,7 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 #pragma unroll
         for (int c = 0; c < 64; ++c) v[c] = none ? 0u : __float_as_uint(__uint_as_float(v[c]) * inv);
 #pragma unroll 1
-        for (int part = 0; part < (p.low != nullptr ? 2 : 1); ++part) {
+        for (int part = 0; part < (LOW ? 2 : 1); ++part) {
           if (lane == 0) tma_store_wait_read<0>();     // the block before has left the staging buffer
           __syncwarp();
 #pragma unroll
@@ -501,14 +519,14 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   if (warp == 9) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
-template <int HD, int SCORE>
+template <int HD, int SCORE, bool LOW>
 int launch_fwd(const CUtensorMap* m, const FwdParams& p, cudaStream_t stream) {
   using SM = Smem<HD>;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_masked_fwd_kernel<HD, SCORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
+    cudaError_t e = cudaFuncSetAttribute(attn_masked_fwd_kernel<HD, SCORE, LOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
     if (e != cudaSuccess) {
       cudaGetLastError();  // clear the sticky error before reporting
       return b200::fail(951, "attn_masked_fwd: cannot set %d bytes of shared memory: %s", SM::TOTAL, cudaGetErrorString(e));
@@ -516,9 +534,13 @@ int launch_fwd(const CUtensorMap* m, const FwdParams& p, cudaStream_t stream) {
     configured[dev & 63] = true;
   }
   const int grid = p.items < b200::sm_count() ? p.items : b200::sm_count();
-  b200::launch(attn_masked_fwd_kernel<HD, SCORE>, grid, NTHREADS, SM::TOTAL, stream, m[0], m[1], m[2], m[3], m[4], p);
+  b200::launch(attn_masked_fwd_kernel<HD, SCORE, LOW>, grid, NTHREADS, SM::TOTAL, stream, m[0], m[1], m[2], m[3], m[4], p);
   b200::count_launch();
   return b200::check_launch("attn_masked_fwd");
+}
+template <int HD, int SCORE>
+int launch_fwd(const CUtensorMap* m, const FwdParams& p, cudaStream_t s) {
+  return p.low != nullptr ? launch_fwd<HD, SCORE, true>(m, p, s) : launch_fwd<HD, SCORE, false>(m, p, s);
 }
 template <int HD>
 int launch_fwd(int score, const CUtensorMap* m, const FwdParams& p, cudaStream_t s) {
@@ -553,7 +575,7 @@ B200_API int b200_attn_masked_fwd(const void* q, const void* k, const void* v, v
   const b200::MaskLayout lay = b200::MaskLayout::of(B, Sq, Skv);
   FwdParams p;
   p.mask = b200::MaskView::of(mask, lay);
-  p.score = {scale, cap, slopes};
+  p.score = b200::ScoreParams::of(scale, cap, slopes);
   p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Skv = Skv;
   p.scale_log2 = scale * b200::LOG2E;
   p.sink = sink; p.lse = lse;

@@ -133,7 +133,6 @@ attn_masked_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   const float scale2 = p.score.scale * b200::LOG2E;
   const bool capped = p.score.cap > 0.f, biased = p.score.slopes != nullptr;
-  const float into = capped ? p.score.scale / p.score.cap : 0.f, back = p.score.cap * b200::LOG2E;
   bool ok = true;
   for (int i = 0; i < n; ++i) {
     const int key = k_lo + (t0 + warp + i * WARPS) * KT;
@@ -169,7 +168,7 @@ attn_masked_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int kk = key + t * 8 + (lane & 3) * 2 + (e & 1), w = e >> 1;
-        float x = capped ? back * b200::tanh_any(s[t][e] * into) : s[t][e] * scale2;
+        float x = capped ? b200::capped_any(s[t][e], p.score) : s[t][e] * scale2;
         if (biased) x = fmaf(-slope[w], fabsf((float)(kk - pos[w])), x);
         if (masked && (kk < iv[w].x || kk >= iv[w].y)) x = -INFINITY;
         s[t][e] = x;
@@ -368,7 +367,7 @@ B200_API int b200_attn_masked_rows(const void* q, const void* k, const void* v, 
   if ((r = b200::map_bshd(&tv, v, HD, Hkv, Skv, B, v_row, v_batch, KT))) return r;
   RowsParams p;
   p.mask = b200::MaskView::of(mask, b200::MaskLayout::of(B, Sq, Skv));
-  p.score = {scale, cap, slopes};
+  p.score = b200::ScoreParams::of(scale, cap, slopes);
   p.q = (const __nv_bfloat16*)q; p.q_row = q_row; p.q_batch = q_batch;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Skv = Skv;
   p.splits = splits_of(B, Sq, Skv, Hq, Hkv);

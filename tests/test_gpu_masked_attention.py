@@ -124,13 +124,11 @@ def check(B, Sq, Skv, Hq, Hkv, D, kind, m, score):
     assert (got[0].cpu()[empty] == 0).all() and (got[1].cpu()[empty] == 0).all()
     unseen = ~ok.any(1)
     assert (got[2].cpu()[unseen] == 0).all() and (got[3].cpu()[unseen] == 0).all()
-    # without a gradient: few rows a key head take a kernel of their own, others the same one
+    # without a gradient: few rows a key head take a kernel of their own, others sum their rows before the probabilities are rounded
     with torch.no_grad():
         y = F.masked_attention(*(t.cuda() for t in (q, k, v)), mask, **to(s))
     close(y, want[0], OUT, "out without a gradient")
     assert (y.cpu()[empty] == 0).all()
-    if Hq // Hkv * Sq > 64:
-        assert torch.equal(y, got[0])
     _lib.check_status("masked attention")
     return got
 
@@ -241,13 +239,15 @@ def test_views_of_a_packed_buffer(off):
     a, b, c = (t.unflatten(-1, (-1, D)) for t in qkv.split([Hq * D, Hkv * D, Hkv * D], -1))
     y = F.masked_attention(a, b, c, mask)
     (g,) = torch.autograd.grad(y, buf, do.transpose(1, 2).contiguous().transpose(1, 2))
-    assert torch.equal(y, ref[0])
+    assert torch.equal(y.detach(), ref[0])
     g = g[..., off:off + (Hq + 2 * Hkv) * D].split([Hq * D, Hkv * D, Hkv * D], -1)
     # (dQ is added up in another order each time; dK and dV are not)
     assert torch.equal(g[1].reshape(ref[2].shape), ref[2]) and torch.equal(g[2].reshape(ref[3].shape), ref[3])
     close(g[0].reshape(ref[1].shape), ref[1].double(), 2 ** -8, "dq")
-    heads_apart = F.masked_attention(q.transpose(1, 2).contiguous().transpose(1, 2), k.expand(B, S, Hkv, D), v, mask)
-    assert torch.equal(heads_apart, ref[0])
+    with torch.no_grad():
+        plain = F.masked_attention(q, k, v, mask)
+        assert torch.equal(F.masked_attention(q.transpose(1, 2).contiguous().transpose(1, 2), k.expand(B, S, Hkv, D), v, mask), plain)
+        assert torch.equal(F.masked_attention(a, b, c, mask), plain)
     _lib.check_status("views")
 
 
