@@ -182,7 +182,8 @@ B200_DEVICE void order_tiles(const MaskLayout& m, int* buf, bool of_q, int* bins
   const int4* t = reinterpret_cast<const int4*>(buf + (of_q ? m.qt : m.kt));
   int* out = buf + (of_q ? m.oq : m.ok);
   auto bin = [&](int i) {
-    const int cost = of_q ? t[2 * i].y - t[2 * i].x + t[2 * i + 1].y - t[2 * i + 1].x : t[i].y - t[i].x;
+    auto of = [&](int k) { return (t[k].y & ~b200::UNSEEN) - t[k].x; };
+    const int cost = of_q ? of(2 * i) + of(2 * i + 1) : of(i);
     return BINS - 1 - min(max(cost, 0), BINS - 1);
   };
   for (int i = threadIdx.x; i < BINS; i += NT) bins[i] = 0;
@@ -248,6 +249,7 @@ __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ M
     }
     __syncthreads();
   }
+  bool unseen = false;                                                // a key of this thread's
   long long front = 0;                                                // (start << 32 | end of its prefix)
   for (int c = 0; c < chunks; ++c) {
     const int i0 = c * CHUNK + (int)threadIdx.x * PER;
@@ -291,6 +293,7 @@ __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ M
         last = max(last - off, 0);
         if (first >= last) first = last = max(i - off, 0);
         k_iv[i] = make_int2(first, last);
+        unseen |= first >= last;
         tk.add(first, last);
         if (i >= off) {
           q_iv[i - off] = make_int2(lo, hi);
@@ -317,6 +320,8 @@ __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ M
     v.join();
     if (lane == 0) qt[t] = v.entry(false);
   }
+  if (__syncthreads_or(unseen))
+    for (int t = threadIdx.x; t < nq; t += NT) qt[t].y |= b200::UNSEEN;
   if (m.B == 1) {
     __syncthreads();
     order_tiles(m, p.buf, true, sh.bins, red[0]);

@@ -10,6 +10,9 @@
 
 namespace b200 {
 
+// Bit of a query tile's end tile: some key of the sequence is seen by no query.
+constexpr int UNSEEN = 1 << 30;
+
 // Offsets, in ints, of the parts of a mask's buffer.
 struct MaskLayout {
   int B, Sq, Skv, Sp, Kp;                  // Sp: rows rounded up to a pair of tiles, Kp: keys to a tile
@@ -20,7 +23,7 @@ struct MaskLayout {
     m.Sp = (Sq + 255) / 256 * 256;
     m.Kp = (Skv + 127) / 128 * 128;
     const long long b = B;
-    m.qt = 0;                              // int4 [B][Sp / 128]: first and end key tile, largest first key, smallest end of a row's keys
+    m.qt = 0;                              // int4 [B][Sp / 128]: first and end key tile (with UNSEEN), largest first key, smallest end of a row's keys
     m.kt = m.qt + b * (m.Sp / 128) * 4;    // int4 [B][Kp / 128]: the same of a key tile over its queries
     m.q_iv = m.kt + b * (m.Kp / 128) * 4;  // int2 [B][Sp]; empty behind the last query
     m.k_iv = m.q_iv + b * m.Sp * 2;        // int2 [B][Kp]; empty behind the last key

@@ -268,6 +268,10 @@ attn_masked_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     const uint32_t lane_base = uint32_t(q * 32) << 16;
     const int key = kv0 + r;
     const int2 seen = p.mask.k_iv[(long long)b * p.mask.Kp + key];      // queries [x, y) see this key
+    // of this warp's keys: queries that see all of them, and that see any
+    const bool is_seen = seen.x < seen.y;
+    const int all_lo = __reduce_max_sync(0xffffffffu, seen.x), all_hi = __reduce_min_sync(0xffffffffu, seen.y);
+    const int any_lo = __reduce_min_sync(0xffffffffu, is_seen ? seen.x : 0x7fffffff), any_hi = __reduce_max_sync(0xffffffffu, is_seen ? seen.y : 0);
     // this thread stages one value per step: the log-sum-exp (half 0) or delta (half 1) of query r of the tile
     // (loaded a step ahead as it is and turned into what the columns need only when it is stored: used at once, it cost the
     // step a global-memory latency)
@@ -341,19 +345,29 @@ attn_masked_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       {
         const float scale2 = SCORE == b200::SCORE_PLAIN ? p.scale_log2 : 1.f;
         const float2 sc2 = make_float2(scale2, scale2);
+        // 32 queries at a time: none that sees a key of the warp (no exponential then), all, or a comparison each.  (With a cap the branches
+        // cost more registers than they save: 4 x 2048 in six documents 309 us without, 345 with them.)
 #pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-          const float4 l4 = *reinterpret_cast<const float4*>(ld + i);
-          const float2 a = ffma2(make_float2(pr[i], pr[i + 1]), sc2, make_float2(-l4.x, -l4.y));
-          const float2 c = ffma2(make_float2(pr[i + 2], pr[i + 3]), sc2, make_float2(-l4.z, -l4.w));
-          pr[i] = ex2_approx(a.x); pr[i + 1] = ex2_approx(a.y); pr[i + 2] = ex2_approx(c.x); pr[i + 3] = ex2_approx(c.y);
-        }
-      }
-      if (need_mask) {
+        for (int h = 0; h < 2; ++h) {
+          const int c0 = half * 64 + h * 32, g0 = q0 + c0;
+          if (!(SCORE & b200::SCORE_CAP) && need_mask && (g0 >= any_hi || g0 + 32 <= any_lo)) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const int col = half * 64 + i;
-          if (col < c_lo || col >= c_hi) pr[i] = 0.f;
+            for (int i = 0; i < 32; ++i) pr[h * 32 + i] = 0.f;
+            continue;
+          }
+#pragma unroll
+          for (int i = h * 32; i < h * 32 + 32; i += 4) {
+            const float4 l4 = *reinterpret_cast<const float4*>(ld + i);
+            const float2 a = ffma2(make_float2(pr[i], pr[i + 1]), sc2, make_float2(-l4.x, -l4.y));
+            const float2 c = ffma2(make_float2(pr[i + 2], pr[i + 3]), sc2, make_float2(-l4.z, -l4.w));
+            pr[i] = ex2_approx(a.x); pr[i + 1] = ex2_approx(a.y); pr[i + 2] = ex2_approx(c.x); pr[i + 3] = ex2_approx(c.y);
+          }
+          if (need_mask && ((SCORE & b200::SCORE_CAP) || g0 < all_lo || g0 + 32 > all_hi)) {
+            const int from = c_lo - c0, to = c_hi - c0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < from || i >= to) pr[h * 32 + i] = 0.f;
+          }
         }
       }
       {

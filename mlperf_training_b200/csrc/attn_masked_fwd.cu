@@ -44,6 +44,7 @@ struct Item {
   int b, h, q0, j_lo;
   int lo0, lo1, hi0, hi1;   // per query tile: key tiles j_lo + [lo, hi); every tile of [0, n_max) is in one of them
   int n_max;
+  bool unseen;              // some keys are seen by no query
   int mlo0, mlo1, mhi0, mhi1;   // per query tile: keys in [mlo, mhi) are visible to all of its rows
   B200_DEVICE int lo(int t) const { return t ? lo1 : lo0; }
   B200_DEVICE int hi(int t) const { return t ? hi1 : hi0; }
@@ -68,7 +69,10 @@ B200_DEVICE Item make_item(int u, const Entry& e, const FwdParams& p) {
   it.b = e.id / np;
   const int pair = e.id - it.b * np;
   it.q0 = pair * 2 * BQ;
-  const int4 a = e.a, c = e.c;
+  int4 a = e.a, c = e.c;
+  it.unseen = (a.y & b200::UNSEEN) != 0;
+  a.y &= ~b200::UNSEEN;
+  c.y &= ~b200::UNSEEN;
   const bool has0 = a.y > a.x, has1 = c.y > c.x;
   it.j_lo = has0 ? a.x : c.x;
   it.lo0 = 0;
@@ -217,10 +221,12 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             ++k_ready;
             if (!warp_wait_spin(&k_full[(kv + k_ready) & 1], ((kv + k_ready) >> 1) & 1, abort_flag, p.status, 51)) return false;
           }
-          // the last S that reads K(n) frees its stage: S_t(n) is issued in step n - 1, tile 0 first (S_t(0) before step 0)
+          // the last S that reads K(n) frees its stage: S_t(n) is issued in step n - 1, tile 0 first; a tile's first one, of the two
+          // key tiles that are there at the start, before step 0
           const int o = 1 - t;
           const bool both = n >= it.lo(o) && n < it.hi(o);
-          const bool free_k = !both || t == 1;
+          const int mine = n == it.lo(t) && n <= 1 ? -1 : n - 1, theirs = n == it.lo(o) && n <= 1 ? -1 : n - 1;
+          const bool free_k = !both || mine > theirs || (mine == theirs && t == 1);
           const bool free_q = --s_left == 0;
           tc_fence_after();
           if (elect_one()) {
@@ -239,12 +245,12 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         };
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (ok && it.lo(t) == 0 && it.hi(t) > 0) ok = issue_s(t, 0);
+          if (ok && it.lo(t) <= 1 && it.hi(t) > it.lo(t)) ok = issue_s(t, it.lo(t));
         for (int n = 0; n < it.n_max && ok; ++n) {
           const int st = (kv + n) & 1;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (ok && n + 1 == it.lo(t) && it.hi(t) > it.lo(t)) ok = issue_s(t, n + 1);      // (K has two stages: not before)
+            if (ok && n > 0 && n + 1 == it.lo(t) && it.hi(t) > it.lo(t)) ok = issue_s(t, n + 1);      // (K has two stages: not before)
             if (!ok || n < it.lo(t) || n >= it.hi(t)) continue;
             const bool first = n == it.lo(t), last = n == it.hi(t) - 1;
             // O of the previous item has left TMEM
@@ -299,6 +305,9 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     int kv = 0;                            // key tiles before this item: stages and phases of V
     bool ok = true;
     Entry next = load_entry(item_of_round(0), p);
+    // (row r of the pair's tile t: pairs are 256 rows of the padded queries in order)
+    auto load_row = [&](const Entry& e) { return p.mask.q_iv[256ll * e.id + t * BQ + r]; };
+    int2 row_next = load_row(next);
     for (int round = 0; round < rounds && ok; ++round) {
       const int u = item_of_round(round);
       if (u >= p.items) continue;
@@ -318,9 +327,10 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           p.lse[((long long)it.b * p.Hq + it.h) * p.Sq + q_pos] = p.sink != nullptr ? p.sink[it.h] : -INFINITY;
         }
         next = load_entry(item_of_round(round + 1), p);
+        row_next = load_row(next);
         continue;
       }
-      const int2 seen = p.mask.q_iv[(long long)it.b * p.mask.Sp + q_pos];            // keys [x, y) of this row
+      const int2 seen = row_next;            // keys [x, y) of this row
       const int mlo = t ? it.mlo1 : it.mlo0, mhi = t ? it.mhi1 : it.mhi0;
       const float slope2 = (SCORE & b200::SCORE_BIAS) ? p.score.slopes[it.h] * b200::LOG2E : 0.f;
       float m_ref = -INFINITY, l = 0.f;
@@ -328,7 +338,7 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         const int kv0 = (it.j_lo + n) * BKV;
         const bool need_mask = kv0 < mlo || kv0 + BKV > mhi;
         bool unseen = false;                 // key kv0 + r, by every query (such a key lies in masked tiles alone)
-        if (need_mask) {
+        if (need_mask && it.unseen) {
           const int2 by = p.mask.k_iv[(long long)it.b * p.mask.Kp + kv0 + r];
           unseen = by.x >= by.y && kv0 + r < p.Skv;
         }
@@ -380,11 +390,10 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           }
         }
         if (need_mask) {
+          const int from = seen.x - kv0, to = seen.y - kv0;
 #pragma unroll
-          for (int i = 0; i < BKV; ++i) {
-            const int kp = kv0 + i;
-            if (kp >= seen.y || kp < seen.x) v[i] = 0xff800000u;  // -inf
-          }
+          for (int i = 0; i < BKV; ++i)
+            if (i >= to || i < from) v[i] = 0xff800000u;  // -inf
         }
         float mx4[4];
 #pragma unroll
@@ -422,9 +431,9 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         const float scale2 = SCORE == b200::SCORE_PLAIN ? p.scale_log2 : 1.f;
         const float2 sc2 = make_float2(scale2, scale2);
         const float2 nm2 = make_float2(-m_use, -m_use);
-        uint32_t pk[BKV / 2];
 #pragma unroll
         for (int c = 0; c < BKV / 32; ++c) {
+          uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int e = c * 32 + 2 * i;
@@ -432,10 +441,11 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             float2 x;
             if (SCORE == b200::SCORE_PLAIN && (i & POLY) == POLY) x = ex2_poly2(a);
             else x = make_float2(ex2_approx(a.x), ex2_approx(a.y));
-            pk[c * 16 + i] = pack_bf16x2(x.x, x.y);
-            if (!LOW) { v[e] = __float_as_uint(x.x); v[e + 1] = __float_as_uint(x.y); }
+            pk[i] = pack_bf16x2(x.x, x.y);
+            v[e] = LOW ? pk[i] << 16 : __float_as_uint(x.x);
+            v[e + 1] = LOW ? pk[i] & 0xffff0000u : __float_as_uint(x.y);
           }
-          tmem_st_32x32b_x16(ts + c * 16, *reinterpret_cast<uint32_t(*)[16]>(&pk[c * 16]));
+          tmem_st_32x32b_x16(ts + c * 16, pk);
           if (c == PV_EARLY / 32 - 1 || c == BKV / 32 - 1) {
             tc_wait_st();
             tc_fence_before();
@@ -447,8 +457,7 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         float2 rs2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int i = 0; i < BKV / 2; ++i)
-          rs2[i & 1] = fadd2(rs2[i & 1], LOW ? make_float2(__uint_as_float(pk[i] << 16), __uint_as_float(pk[i] & 0xffff0000u))
-                                             : make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
+          rs2[i & 1] = fadd2(rs2[i & 1], make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])));
         l += (rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y);
       }
       // ------------------------------ epilogue ------------------------------
@@ -456,6 +465,7 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       if (!ok || !warp_wait(&o_done[t], no & 1, abort_flag, p.status, 62)) { ok = false; break; }
       ++no;
       tc_fence_after();
+      row_next = load_row(next);
       // a row that sees nothing (its sum is not 0: the polynomial's 2^-inf is 2^-126)
       const bool none = m_ref == -INFINITY;
       if (none) l = 0.f;

@@ -37,6 +37,10 @@ def test_masks(B, Sq, Skv, kind, m):
     qt, kt = take(B * nq * 4, B, nq, 4), take(B * nk * 4, B, nk, 4)
     q_iv, k_iv = take(B * Sp * 2, B, Sp, 2), take(B * Kp * 2, B, Kp, 2)
     oq, ok = take(B * nq // 2, -1), take(B * nk, -1)
+    # (a bit of each query tile says whether some key of its sequence is seen by no query)
+    unseen = (k_iv[:, :Skv, 0] >= k_iv[:, :Skv, 1]).any(1)
+    assert torch.equal((qt[..., 1] >> 30) != 0, unseen[:, None].expand(B, nq))
+    qt = torch.stack([qt[..., 0], qt[..., 1] & ~(1 << 30), qt[..., 2], qt[..., 3]], -1)
     lo, hi = q_iv[:, :Sq, 0], q_iv[:, :Sq, 1]
     assert torch.equal(lo, ref.lo.int()) and torch.equal(hi, ref.hi.int())
     assert (lo[:, 1:] >= lo[:, :-1]).all() and (hi[:, 1:] >= hi[:, :-1]).all()       # what the tile ranges rest on
