@@ -5,6 +5,9 @@
 //                                       RuntimeError on a code other than 0
 //   gemm(...)                           ops.kernels.gemm for CUDA operands that need no copy: checks, output, split workspace, launch
 //   quant_mxfp4, dequant_mx, norm_mx, gemm_mxfp4, gated_fwd, gated_down, gated_bwd   the same for ops.mxfp4, ops.norm_mx and the gated block
+//   route, distill_loss, masked_attention   ops.moe_ops.route, ops.functional.distill_loss and masked_attention with their autograd nodes: a backward
+//                                       pass then runs in autograd's thread without Python (seven tokens' distillation and its gradient
+//                                       101 us of host time, now HOST_US; of which 42 are autograd's own)
 //
 // ctypes converts twenty arguments through as many Python objects and calls: 5 of the 20 us a launch of a small model took.  With
 // it, the native GEMM operator and no autograd nodes where no gradient is wanted: a step of a two-layer model of width 512 2020 ->
@@ -16,8 +19,12 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
+#include <mutex>
 #include <string>
 #include <unordered_map>
 
@@ -119,6 +126,31 @@ DequantFn g_dequant = nullptr;
 NormMxFn g_norm_mx = nullptr;
 Gemm4Fn g_gemm4 = nullptr;
 
+// the launchers of the operators with autograd nodes
+using RouteFn = int (*)(const void*, int, long long, const float*, int, int, int, int, int, int, int, float, int*, float*, int*, void*);
+using RouteBwdFn = int (*)(const void*, int, long long, const int*, const float*, int, int, int, int, int, float, void*, void*);
+using DistillFn = int (*)(const void*, int, long long, const long long*, const void*, int, const void*, int, int, int, int, int, float, float, long long,
+                          float*, float*, double*, void*);
+using DistillBwdFn = int (*)(const void*, int, long long, const long long*, const void*, int, const void*, int, int, int, int, int, float, float,
+                             long long, const float*, const double*, const float*, void*, long long, void*);
+using MaskedFn = int (*)(const void*, const void*, const void*, void*, void*, float*, const float*, const float*, const int*, int, int, int, int, int, int,
+                         long long, long long, long long, long long, long long, long long, float, float, void*);
+using MaskedRowsFn = int (*)(const void*, const void*, const void*, void*, float*, const float*, const float*, const int*, int, int, int, int, int, int,
+                             long long, long long, long long, long long, long long, long long, float, float, void*, long long, void*);
+using MaskedBwdFn = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, float*, void*, void*,
+                            const float*, const int*, int, int, int, int, int, int, long long, long long, long long, long long, long long, long long,
+                            long long, long long, long long, long long, float, float, void*, long long, void*);
+RouteFn g_route = nullptr;
+RouteBwdFn g_route_bwd = nullptr;
+DistillFn g_distill = nullptr;
+DistillBwdFn g_distill_bwd = nullptr;
+MaskedFn g_masked = nullptr;
+MaskedRowsFn g_masked_rows = nullptr;
+MaskedBwdFn g_masked_bwd = nullptr;
+int (*g_few_rows)(int, int, int, int) = nullptr;
+long long (*g_rows_ws)(int, int, int, int, int, int) = nullptr;
+long long (*g_masked_bwd_ws)(int, int, int, int) = nullptr;
+
 // bind({name: (address, codes)}, address of b200_last_error, fallback)
 PyObject* py_bind(PyObject*, PyObject* args) {
   PyObject *table, *fallback;
@@ -138,6 +170,16 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     PyUnicode_InternInPlace(&key);
     t[key] = Entry{reinterpret_cast<void*>(addr), codes};
     if (PyUnicode_CompareWithASCIIString(key, "b200_quant_mxfp4") == 0) g_quant4 = reinterpret_cast<Quant4Fn>(addr);
+    auto take = [&](const char* name, auto& fn) {
+      if (PyUnicode_CompareWithASCIIString(key, name) == 0) fn = reinterpret_cast<std::decay_t<decltype(fn)>>(addr);
+    };
+    take("b200_route", g_route);
+    take("b200_route_bwd", g_route_bwd);
+    take("b200_distill_fwd", g_distill);
+    take("b200_distill_bwd", g_distill_bwd);
+    take("b200_attn_masked_fwd", g_masked);
+    take("b200_attn_masked_rows", g_masked_rows);
+    take("b200_attn_masked_bwd", g_masked_bwd);
     if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_gated") == 0) g_gated = reinterpret_cast<GatedFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_gated_down") == 0) g_down = reinterpret_cast<DownFn>(addr);
     if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_gated_grad") == 0) g_gated_grad = reinterpret_cast<GatedGradFn>(addr);
@@ -553,7 +595,300 @@ PyObject* py_bind_gemm(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+// ---- operators with autograd nodes of their own: None where the general path has to look at the operands (copies, other types, errors) ----
+namespace ag = torch::autograd;
+
+void check_rc(const char* name, int rc) {
+  TORCH_CHECK(rc == 0, name, " failed with code ", rc, ": ", g_last_error ? g_last_error() : "");
+}
+cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+at::Tensor plain_grad(const at::Tensor& g, at::ScalarType type) {     // contiguous, aligned, of a type
+  at::Tensor r = g.to(type).contiguous();
+  return aligned16(r.data_ptr()) ? r : r.clone();
+}
+// A CUDA tensor of the current device; its rows (dim 2) contiguous and apart.
+bool here(const at::Tensor& t) { return t.is_cuda() && c10::cuda::current_device() == t.device().index(); }
+bool rows_ok(const at::Tensor& t) { return t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1); }
+bool float_or_bf16(const at::Tensor& t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+// None: `t` stays undefined; false where it is neither that nor a tensor
+bool optional_tensor(PyObject* o, at::Tensor& t) {
+  if (o == Py_None) return true;
+  const at::Tensor* p = tensor_of(o);
+  if (p == nullptr) return false;
+  t = *p;
+  return true;
+}
+bool float_of(PyObject* o, double& v) {
+  v = PyFloat_AsDouble(o);
+  return !(v == -1.0 && PyErr_Occurred());
+}
+template <typename N>
+void set_node(const std::shared_ptr<N>& node, at::Tensor& out, ag::edge_list&& edges) {
+  node->set_next_edges(std::move(edges));
+  ag::set_history(out, node);
+}
+
+struct RouteBackward : public ag::Node {
+  ag::SavedVariable logits, idx;
+  int sigmoid, renorm;
+  float scale;
+  std::string name() const override { return "RouteBackward"; }
+  void release_variables() override { logits.reset_data(); idx.reset_data(); }
+  ag::variable_list apply(ag::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {at::Tensor()};
+    const at::Tensor x = logits.unpack(), i = idx.unpack(), g = plain_grad(grads[0], at::kFloat);
+    at::Tensor dx = at::empty(x.sizes(), x.options().requires_grad(false));
+    check_rc("b200_route_bwd", g_route_bwd(x.data_ptr(), x.scalar_type() == at::kBFloat16, x.stride(0), i.data_ptr<int>(), g.data_ptr<float>(),
+                                           (int)x.size(0), (int)x.size(1), (int)i.size(1), sigmoid, renorm, scale, dx.data_ptr(), stream_of(x)));
+    return {dx};
+  }
+};
+
+// route(logits, k, sigmoid, bias or None, groups, top_groups, renormalize, scale): (idx, w, counts)
+PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* x;
+  at::Tensor bias;
+  long long k, sigmoid, groups, top, renorm;
+  double scale;
+  if (nargs != 8 || g_route == nullptr || g_route_bwd == nullptr || (x = tensor_of(args[0])) == nullptr || !int_of(args[1], k) ||
+      !int_of(args[2], sigmoid) || !optional_tensor(args[3], bias) || !int_of(args[4], groups) || !int_of(args[5], top) ||
+      !int_of(args[6], renorm) || !float_of(args[7], scale)) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (!here(*x) || !rows_ok(*x) || !float_or_bf16(*x)) Py_RETURN_NONE;
+  const int64_t T = x->size(0), E = x->size(1);
+  if (T < 1 || T > 0x7fffffff || E < 1 || E > 256 || k < 1 || k > 32 || k > E || groups < 1 || groups > 32 || E % groups != 0 || top < 1 ||
+      top > groups || top * (E / groups) < k)
+    Py_RETURN_NONE;
+  if (bias.defined() && (bias.device() != x->device() || bias.scalar_type() != at::kFloat || bias.dim() != 1 || bias.size(0) != E || !bias.is_contiguous()))
+    Py_RETURN_NONE;
+  at::Tensor t[3];
+  {
+    pybind11::gil_scoped_release nogil;
+    const auto o = x->options().requires_grad(false);
+    t[0] = at::empty({T, k}, o.dtype(at::kInt));
+    t[1] = at::empty({T, k}, o.dtype(at::kFloat));
+    t[2] = T <= 8 ? at::empty({E}, o.dtype(at::kInt)) : at::zeros({E}, o.dtype(at::kInt));        // (few tokens: stored whole)
+    check_rc("b200_route", g_route(x->data_ptr(), x->scalar_type() == at::kBFloat16, x->stride(0), bias.defined() ? bias.data_ptr<float>() : nullptr,
+                                   (int)T, (int)E, (int)k, (int)sigmoid, (int)groups, (int)top, (int)renorm, (float)scale, t[0].data_ptr<int>(),
+                                   t[1].data_ptr<float>(), t[2].data_ptr<int>(), stream_of(*x)));
+    if (ag::compute_requires_grad(*x)) {
+      auto node = std::shared_ptr<RouteBackward>(new RouteBackward(), ag::deleteNode);
+      node->logits = ag::SavedVariable(*x, false);
+      node->idx = ag::SavedVariable(t[0], false);
+      node->sigmoid = (int)sigmoid;
+      node->renorm = (int)renorm;
+      node->scale = (float)scale;
+      set_node(node, t[1], ag::collect_next_edges(*x));
+    }
+  }
+  return wrap_all(t, 3);
+  END_HANDLE_TH_ERRORS
+}
+
+struct DistillArgs {
+  int K, rest;
+  float alpha, tau;
+  long long ignore;
+};
+const long long* labels_of(const at::Tensor& t) { return t.defined() ? reinterpret_cast<const long long*>(t.data_ptr<int64_t>()) : nullptr; }
+
+struct DistillLossBackward : public ag::Node {
+  ag::SavedVariable logits, labels, ids, values, stats, teacher;
+  DistillArgs a;
+  std::string name() const override { return "DistillLossBackward"; }
+  void release_variables() override {
+    for (auto* v : {&logits, &labels, &ids, &values, &stats, &teacher}) v->reset_data();
+  }
+  ag::variable_list apply(ag::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {at::Tensor()};
+    const at::Tensor x = logits.unpack(), l = labels.unpack(), i = ids.unpack(), v = values.unpack(), s = stats.unpack(), te = teacher.unpack(),
+                     g = plain_grad(grads[0], at::kFloat);
+    at::Tensor dx = at::empty(x.sizes(), x.options().requires_grad(false));
+    check_rc("b200_distill_bwd",
+             g_distill_bwd(x.data_ptr(), x.scalar_type() == at::kBFloat16, x.stride(0), labels_of(l), i.data_ptr(), i.scalar_type() == at::kLong,
+                           v.data_ptr(), v.scalar_type() == at::kBFloat16, (int)x.size(0), a.K, (int)x.size(1), a.rest, a.alpha, a.tau, a.ignore,
+                           s.data_ptr<float>(), te.data_ptr<double>(), g.data_ptr<float>(), dx.data_ptr(), dx.stride(0), stream_of(x)));
+    return {dx};
+  }
+};
+
+// distill_loss(logits, labels or None, ids, values, alpha, temperature, rest, ignore_index): loss
+PyObject* py_distill_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *i, *v;
+  at::Tensor l;
+  double alpha, tau;
+  long long rest, ignore;
+  if (nargs != 8 || g_distill == nullptr || g_distill_bwd == nullptr || (x = tensor_of(args[0])) == nullptr || !optional_tensor(args[1], l) ||
+      (i = tensor_of(args[2])) == nullptr || (v = tensor_of(args[3])) == nullptr || !float_of(args[4], alpha) || !float_of(args[5], tau) ||
+      !int_of(args[6], rest) || !int_of(args[7], ignore)) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (!here(*x) || !rows_ok(*x) || !float_or_bf16(*x)) Py_RETURN_NONE;
+  const int64_t T = x->size(0), V = x->size(1);
+  if (T < 1 || T > 0x7fffffff || V < 1 || V > (rest ? 900000 : 1 << 30) || !(alpha >= 0.0 && alpha <= 1.0) || !((float)tau > 0.f && (float)tau < INFINITY) ||
+      (!l.defined() && alpha < 1.0))
+    Py_RETURN_NONE;
+  if (i->device() != x->device() || v->device() != x->device() || i->dim() != 2 || i->sizes() != v->sizes() || i->size(0) != T || i->size(1) < 1 ||
+      i->size(1) > 1024 || (i->scalar_type() != at::kLong && i->scalar_type() != at::kInt) || !float_or_bf16(*v) || !i->is_contiguous() ||
+      !v->is_contiguous())
+    Py_RETURN_NONE;
+  if (l.defined() && (l.device() != x->device() || l.scalar_type() != at::kLong || l.dim() != 1 || l.size(0) != T || !l.is_contiguous())) Py_RETURN_NONE;
+  at::Tensor loss;
+  {
+    pybind11::gil_scoped_release nogil;
+    const auto o = x->options().requires_grad(false);
+    const DistillArgs a = {(int)i->size(1), rest != 0, (float)alpha, (float)tau, ignore};
+    loss = at::empty({T}, o.dtype(at::kFloat));
+    at::Tensor stats = at::empty({T, 4}, o.dtype(at::kFloat)), teacher = at::empty({T}, o.dtype(at::kDouble));
+    check_rc("b200_distill_fwd",
+             g_distill(x->data_ptr(), x->scalar_type() == at::kBFloat16, x->stride(0), labels_of(l), i->data_ptr(), i->scalar_type() == at::kLong,
+                       v->data_ptr(), v->scalar_type() == at::kBFloat16, (int)T, a.K, (int)V, a.rest, a.alpha, a.tau, a.ignore, loss.data_ptr<float>(),
+                       stats.data_ptr<float>(), teacher.data_ptr<double>(), stream_of(*x)));
+    if (ag::compute_requires_grad(*x)) {
+      auto node = std::shared_ptr<DistillLossBackward>(new DistillLossBackward(), ag::deleteNode);
+      node->logits = ag::SavedVariable(*x, false);
+      node->labels = ag::SavedVariable(l, false);
+      node->ids = ag::SavedVariable(*i, false);
+      node->values = ag::SavedVariable(v->detach(), false);
+      node->stats = ag::SavedVariable(stats, false);
+      node->teacher = ag::SavedVariable(teacher, false);
+      node->a = a;
+      set_node(node, loss, ag::collect_next_edges(*x));
+    }
+  }
+  return THPVariable_Wrap(std::move(loss));
+  END_HANDLE_TH_ERRORS
+}
+
+// [B, S, H, D] as the kernels read it without a copy (ops.masked_attention._bshd)
+struct Pitch { long long row, batch; };
+bool bshd(const at::Tensor& t, Pitch& p) {
+  const int64_t B = t.size(0), S = t.size(1), H = t.size(2), D = t.size(3), w = H * D;
+  p.row = S > 1 ? t.stride(1) : w;
+  p.batch = B > 1 ? t.stride(0) : S * p.row;
+  return t.stride(3) == 1 && (H == 1 || t.stride(2) == D) && p.row >= w && p.batch >= w && p.row % 8 == 0 && p.batch % 8 == 0 && aligned16(t.data_ptr());
+}
+const float* floats_of(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+at::Tensor workspace(long long bytes, const at::Tensor& like) {
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
+}
+
+struct MaskedAttentionBackward : public ag::Node {
+  ag::SavedVariable q, k, v, out, low, lse, slopes, mask;
+  float softcap, scale;
+  std::string name() const override { return "MaskedAttentionBackward"; }
+  void release_variables() override {
+    for (auto* s : {&q, &k, &v, &out, &low, &lse, &slopes, &mask}) s->reset_data();
+  }
+  ag::variable_list apply(ag::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+    const at::Tensor a = q.unpack(), b = k.unpack(), c = v.unpack(), o = out.unpack(shared_from_this()), lo = low.unpack(), ls = lse.unpack(),
+                     sl = slopes.unpack(), m = mask.unpack(), g = plain_grad(grads[0], at::kBFloat16);
+    Pitch pq, pk, pv;
+    TORCH_CHECK(bshd(a, pq) && bshd(b, pk) && bshd(c, pv), "masked_attention: saved operands");
+    const int64_t B = a.size(0), Sq = a.size(1), Hq = a.size(2), D = a.size(3), Skv = b.size(1), Hkv = b.size(2);
+    const auto f32 = a.options().dtype(at::kFloat).requires_grad(false);
+    at::Tensor dq = at::zeros({B, Sq, Hq, D}, f32), dk = at::empty({B, Skv, Hkv, D}, a.options().requires_grad(false)), dv = at::empty_like(dk),
+               delta = at::empty({B, Hq, Sq}, f32);
+    const long long n = g_masked_bwd_ws((int)B, (int)Skv, (int)Hkv, (int)D), w = Hkv * D;
+    at::Tensor ws = workspace(n, a);
+    check_rc("b200_attn_masked_bwd",
+             g_masked_bwd(a.data_ptr(), b.data_ptr(), c.data_ptr(), o.data_ptr(), lo.data_ptr(), g.data_ptr(), ls.data_ptr<float>(),
+                          delta.data_ptr<float>(), dq.data_ptr<float>(), dk.data_ptr(), dv.data_ptr(), floats_of(sl), m.data_ptr<int>(), (int)B, (int)Sq,
+                          (int)Skv, (int)Hq, (int)Hkv, (int)D, pq.row, pk.row, pv.row, w, w, pq.batch, pk.batch, pv.batch, Skv * w, Skv * w, scale,
+                          softcap, n > 0 ? ws.data_ptr() : nullptr, n, stream_of(a)));
+    return {dq.to(at::kBFloat16), dk, dv};
+  }
+};
+
+// masked_attention(q, k, v, the mask's buffer, B, Sq, Skv, slopes or None, softcap, scale): out.  (Sink logits take the general path.)
+PyObject* py_masked_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const at::Tensor *q, *k, *v, *m;
+  at::Tensor sl;
+  long long mb, mq, mk;
+  double softcap, scale;
+  if (nargs != 10 || g_masked == nullptr || g_masked_rows == nullptr || g_masked_bwd == nullptr || g_few_rows == nullptr ||
+      (q = tensor_of(args[0])) == nullptr || (k = tensor_of(args[1])) == nullptr || (v = tensor_of(args[2])) == nullptr ||
+      (m = tensor_of(args[3])) == nullptr || !int_of(args[4], mb) || !int_of(args[5], mq) || !int_of(args[6], mk) || !optional_tensor(args[7], sl) ||
+      !float_of(args[8], softcap) || !float_of(args[9], scale)) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (!here(*q) || q->dim() != 4 || k->dim() != 4 || k->sizes() != v->sizes() || q->scalar_type() != at::kBFloat16 || k->scalar_type() != at::kBFloat16 ||
+      v->scalar_type() != at::kBFloat16 || k->device() != q->device() || v->device() != q->device() || m->device() != q->device())
+    Py_RETURN_NONE;
+  const int64_t B = q->size(0), Sq = q->size(1), Hq = q->size(2), D = q->size(3), Skv = k->size(1), Hkv = k->size(2);
+  Pitch pq, pk, pv;
+  if (B != mb || Sq != mq || Skv != mk || k->size(0) != B || k->size(3) != D || (D != 64 && D != 128) || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 ||
+      !bshd(*q, pq) || !bshd(*k, pk) || !bshd(*v, pv) || !((float)scale > 0.f && (float)scale < INFINITY) ||
+      !((float)softcap >= 0.f && (float)softcap < INFINITY) || m->scalar_type() != at::kInt || !m->is_contiguous())
+    Py_RETURN_NONE;
+  if (sl.defined() && (sl.device() != q->device() || sl.scalar_type() != at::kFloat || sl.dim() != 1 || sl.size(0) != Hq || !sl.is_contiguous()))
+    Py_RETURN_NONE;
+  at::Tensor out;
+  {
+    pybind11::gil_scoped_release nogil;
+    const bool grad = ag::compute_requires_grad(*q, *k, *v);
+    const auto o = q->options().requires_grad(false);
+    out = at::empty({B, Sq, Hq, D}, o);
+    at::Tensor lse = at::empty({B, Hq, Sq}, o.dtype(at::kFloat)), low;
+    if (!grad && g_few_rows((int)B, (int)Sq, (int)Hq, (int)Hkv)) {
+      const long long n = g_rows_ws((int)B, (int)Sq, (int)Skv, (int)Hq, (int)Hkv, (int)D);
+      at::Tensor ws = workspace(n, *q);
+      check_rc("b200_attn_masked_rows",
+               g_masked_rows(q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(), lse.data_ptr<float>(), nullptr, floats_of(sl), m->data_ptr<int>(),
+                             (int)B, (int)Sq, (int)Skv, (int)Hq, (int)Hkv, (int)D, pq.row, pk.row, pv.row, pq.batch, pk.batch, pv.batch, (float)scale,
+                             (float)softcap, n > 0 ? ws.data_ptr() : nullptr, n, stream_of(*q)));
+    } else {
+      if (grad) low = at::empty({B, Sq, Hq, D}, o);
+      check_rc("b200_attn_masked_fwd",
+               g_masked(q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(), grad ? low.data_ptr() : nullptr, lse.data_ptr<float>(), nullptr,
+                        floats_of(sl), m->data_ptr<int>(), (int)B, (int)Sq, (int)Skv, (int)Hq, (int)Hkv, (int)D, pq.row, pk.row, pv.row, pq.batch, pk.batch,
+                        pv.batch, (float)scale, (float)softcap, stream_of(*q)));
+    }
+    if (grad) {
+      auto node = std::shared_ptr<MaskedAttentionBackward>(new MaskedAttentionBackward(), ag::deleteNode);
+      node->softcap = (float)softcap;
+      node->scale = (float)scale;
+      set_node(node, out, ag::collect_next_edges(*q, *k, *v));
+      node->q = ag::SavedVariable(*q, false);
+      node->k = ag::SavedVariable(*k, false);
+      node->v = ag::SavedVariable(*v, false);
+      node->out = ag::SavedVariable(out, true);
+      node->low = ag::SavedVariable(low, false);
+      node->lse = ag::SavedVariable(lse, false);
+      node->slopes = ag::SavedVariable(sl.defined() ? sl.detach() : sl, false);
+      node->mask = ag::SavedVariable(*m, false);
+    }
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_masked(addresses of b200_attn_masked_few_rows, _rows_workspace, _bwd_workspace)
+PyObject* py_bind_masked(PyObject*, PyObject* args) {
+  unsigned long long a, b, c;
+  if (!PyArg_ParseTuple(args, "KKK", &a, &b, &c)) return nullptr;
+  g_few_rows = reinterpret_cast<int (*)(int, int, int, int)>(a);
+  g_rows_ws = reinterpret_cast<long long (*)(int, int, int, int, int, int)>(b);
+  g_masked_bwd_ws = reinterpret_cast<long long (*)(int, int, int, int)>(c);
+  Py_RETURN_NONE;
+}
+
 PyMethodDef methods[] = {
+    {"bind_masked", py_bind_masked, METH_VARARGS, nullptr},
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_route)), METH_FASTCALL, nullptr},
+    {"distill_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_distill_loss)), METH_FASTCALL, nullptr},
+    {"masked_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_masked_attention)), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_VARARGS, nullptr},
     {"bind_gemm", py_bind_gemm, METH_VARARGS, nullptr},
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_call)), METH_FASTCALL, nullptr},

@@ -20,6 +20,7 @@ import warnings
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 _PKG = Path(__file__).resolve().parent.parent
 # B200_KERNELS_LIB selects another build of the library (the bounds-reporting debug build)
@@ -174,6 +175,9 @@ def _declare(lib: ctypes.CDLL) -> None:
             host.bind_gemm(table["b200_gemm_bf16"][0], ctypes.cast(lib.b200_gemm_bf16_workspace, c_void_p).value)
         if hasattr(lib, "b200_gemm_mxfp4_workspace"):
             host.bind_mx(ctypes.cast(lib.b200_gemm_mxfp4_workspace, c_void_p).value)
+        if hasattr(lib, "b200_attn_masked_few_rows"):
+            host.bind_masked(*(ctypes.cast(getattr(lib, "b200_attn_masked_" + n), c_void_p).value
+                               for n in ("few_rows", "rows_workspace", "bwd_workspace")))
     lib.b200_norm_bwd_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.restype = c_ll
@@ -267,6 +271,17 @@ def use_kernels(t: torch.Tensor) -> bool:
             require()
         return True
     return False
+
+
+def native(t: torch.Tensor):
+    """The host module for operators that bring their own autograd nodes, or None: on the CPU, without the module, under function
+    transforms, forward-mode derivatives or a trace (which go by the nodes of ``torch.autograd.Function``)."""
+    if (host is None or not t.is_cuda or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
+            or torch._C._get_tracing_state() is not None):
+        return None
+    if _lib is None:
+        require()
+    return host
 
 
 def stream_ptr() -> int:

@@ -18,7 +18,7 @@ from . import kernels as K
 from . import linear as L
 from . import masked_attention as MA
 from .masked_attention import AttentionMask, attention_mask  # noqa: F401 - a mask is made once and used by masked_attention
-from ._lib import call, ptr, stream_ptr, use_kernels
+from ._lib import call, native as _native, ptr, stream_ptr, use_kernels
 
 
 class _NoGrad:
@@ -630,6 +630,12 @@ def masked_attention(q, k, v, mask, *, softcap=0.0, slopes=None, sink=None, scal
     see nothing give 0 and get no gradient.  Values of padding may be anything in the forward pass; the backward pass wants finite
     inputs everywhere."""
     MA.constant_slopes(slopes)
+    host = _native(q) if sink is None and mask.buf is not None else None
+    if host is not None:
+        out = host.masked_attention(q, k, v, mask.buf, mask.B, mask.Sq, mask.Skv, slopes, float(softcap),
+                                    1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale))
+        if out is not None:
+            return out
     return _apply(MaskedAttentionFn, q, k, v, sink, slopes, mask, softcap, scale)
 
 
@@ -825,6 +831,11 @@ def distill_loss(logits, labels, ids, values, *, alpha=1.0, temperature=1.0, res
     are logits, softmaxed over the entries at ``temperature``; or, with ``rest``, the teacher's log-probabilities over the whole vocabulary
     at that temperature, and what they leave of 1 is one further event: any other id.  Tokens whose label is ``ignore_index`` have
     loss and gradient 0; ``labels`` may be None where ``alpha`` is 1.  The gradient goes to the logits alone."""
+    host = _native(logits)
+    if host is not None:
+        out = host.distill_loss(logits, labels, ids, values, float(alpha), float(temperature), int(rest), int(ignore_index))
+        if out is not None:
+            return out
     return _apply(DistillLossFn, logits, labels, ids, values, alpha, temperature, rest, ignore_index)
 
 

@@ -381,6 +381,11 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.T
     the bias, divided by their sum (``renormalize``) and times ``scale``.  Comparisons hold in 64 bits, NaN counts as -inf; without a bias
     experts are compared by their logits.  ``idx``, ``w`` and ``counts`` go into ``moe_experts`` like those of ``router_topk``, which is
     ``softmax`` with ``renormalize`` for few experts chosen by their logits."""
+    host = _lib.native(logits)
+    if host is not None and score in ROUTE_SCORES:
+        out = host.route(logits, k, int(score == "sigmoid"), bias, groups, top_groups, int(renormalize), float(scale))
+        if out is not None:
+            return out
     return _apply(RouteFn, logits, bias, k, score, groups, top_groups, renormalize, scale)
 
 
