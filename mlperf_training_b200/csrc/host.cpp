@@ -5,9 +5,10 @@
 //                                       RuntimeError on a code other than 0
 //   gemm(...)                           ops.kernels.gemm for CUDA operands that need no copy: checks, output, split workspace, launch
 //   quant_mxfp4, dequant_mx, norm_mx, gemm_mxfp4, gated_fwd, gated_down, gated_bwd   the same for ops.mxfp4, ops.norm_mx and the gated block
+//   attention_mask                      the tables of ops.masked_attention.attention_mask
 //   route, distill_loss, masked_attention   ops.moe_ops.route, ops.functional.distill_loss and masked_attention with their autograd nodes: a backward
 //                                       pass then runs in autograd's thread without Python (seven tokens' distillation and its gradient
-//                                       101 us of host time, now HOST_US; of which 42 are autograd's own)
+//                                       101 us of host time, now 53; of which 42 are autograd's own)
 //
 // ctypes converts twenty arguments through as many Python objects and calls: 5 of the 20 us a launch of a small model took.  With
 // it, the native GEMM operator and no autograd nodes where no gradient is wanted: a step of a two-layer model of width 512 2020 ->
@@ -150,6 +151,8 @@ MaskedBwdFn g_masked_bwd = nullptr;
 int (*g_few_rows)(int, int, int, int) = nullptr;
 long long (*g_rows_ws)(int, int, int, int, int, int) = nullptr;
 long long (*g_masked_bwd_ws)(int, int, int, int) = nullptr;
+long long (*g_mask_ints)(int, int, int) = nullptr;
+int (*g_mask)(const void*, int, const uint8_t*, int, int, int, int, int, int*, void*) = nullptr;
 
 // bind({name: (address, codes)}, address of b200_last_error, fallback)
 PyObject* py_bind(PyObject*, PyObject* args) {
@@ -178,6 +181,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     take("b200_distill_fwd", g_distill);
     take("b200_distill_bwd", g_distill_bwd);
     take("b200_attn_masked_fwd", g_masked);
+    take("b200_attn_mask", g_mask);
     take("b200_attn_masked_rows", g_masked_rows);
     take("b200_attn_masked_bwd", g_masked_bwd);
     if (PyUnicode_CompareWithASCIIString(key, "b200_gemm_gated") == 0) g_gated = reinterpret_cast<GatedFn>(addr);
@@ -671,7 +675,7 @@ PyObject* py_route(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const auto o = x->options().requires_grad(false);
     t[0] = at::empty({T, k}, o.dtype(at::kInt));
     t[1] = at::empty({T, k}, o.dtype(at::kFloat));
-    t[2] = T <= 8 ? at::empty({E}, o.dtype(at::kInt)) : at::zeros({E}, o.dtype(at::kInt));        // (few tokens: stored whole)
+    t[2] = at::empty({E}, o.dtype(at::kInt));
     check_rc("b200_route", g_route(x->data_ptr(), x->scalar_type() == at::kBFloat16, x->stride(0), bias.defined() ? bias.data_ptr<float>() : nullptr,
                                    (int)T, (int)E, (int)k, (int)sigmoid, (int)groups, (int)top, (int)renorm, (float)scale, t[0].data_ptr<int>(),
                                    t[1].data_ptr<float>(), t[2].data_ptr<int>(), stream_of(*x)));
@@ -874,10 +878,42 @@ PyObject* py_masked_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
   END_HANDLE_TH_ERRORS
 }
 
-// bind_masked(addresses of b200_attn_masked_few_rows, _rows_workspace, _bwd_workspace)
+// attention_mask(documents or None, prefix or None, B, Sq, Skv, causal, window, index of the device): the mask's buffer
+PyObject* py_attention_mask(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor ids, flags;
+  long long B, Sq, Skv, causal, window, dev;
+  if (nargs != 8 || g_mask == nullptr || g_mask_ints == nullptr || !optional_tensor(args[0], ids) || !optional_tensor(args[1], flags) ||
+      !int_of(args[2], B) || !int_of(args[3], Sq) || !int_of(args[4], Skv) || !int_of(args[5], causal) || !int_of(args[6], window) ||
+      !int_of(args[7], dev)) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  if (B < 1 || Sq < 1 || Skv < Sq || Skv > (1 << 30) || B > 0x7fffffff || window < 0 || window >= (1 << 30) || dev != c10::cuda::current_device())
+    Py_RETURN_NONE;
+  for (const at::Tensor* t : {&ids, &flags})
+    if (t->defined() && (!here(*t) || t->dim() != 2 || t->size(0) != B || t->size(1) != Skv || !t->is_contiguous())) Py_RETURN_NONE;
+  if ((ids.defined() && ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) || (flags.defined() && (flags.scalar_type() != at::kBool || !causal)))
+    Py_RETURN_NONE;
+  at::Tensor buf;
+  {
+    pybind11::gil_scoped_release nogil;
+    const long long n = g_mask_ints((int)B, (int)Sq, (int)Skv);
+    TORCH_CHECK(n > 0, "attention_mask: ", B, " x ", Sq, " x ", Skv);
+    buf = at::empty({n}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)dev));
+    check_rc("b200_attn_mask", g_mask(ids.defined() ? ids.data_ptr() : nullptr, ids.defined() && ids.scalar_type() == at::kLong,
+                                      flags.defined() ? reinterpret_cast<const uint8_t*>(flags.data_ptr()) : nullptr, (int)B, (int)Sq, (int)Skv,
+                                      (int)causal, (int)window, buf.data_ptr<int>(), stream_of(buf)));
+  }
+  return THPVariable_Wrap(std::move(buf));
+  END_HANDLE_TH_ERRORS
+}
+
+// bind_masked(addresses of b200_attn_masked_few_rows, _rows_workspace, _bwd_workspace, b200_attn_mask_ints)
 PyObject* py_bind_masked(PyObject*, PyObject* args) {
-  unsigned long long a, b, c;
-  if (!PyArg_ParseTuple(args, "KKK", &a, &b, &c)) return nullptr;
+  unsigned long long a, b, c, d;
+  if (!PyArg_ParseTuple(args, "KKKK", &a, &b, &c, &d)) return nullptr;
+  g_mask_ints = reinterpret_cast<long long (*)(int, int, int)>(d);
   g_few_rows = reinterpret_cast<int (*)(int, int, int, int)>(a);
   g_rows_ws = reinterpret_cast<long long (*)(int, int, int, int, int, int)>(b);
   g_masked_bwd_ws = reinterpret_cast<long long (*)(int, int, int, int)>(c);
@@ -886,6 +922,7 @@ PyObject* py_bind_masked(PyObject*, PyObject* args) {
 
 PyMethodDef methods[] = {
     {"bind_masked", py_bind_masked, METH_VARARGS, nullptr},
+    {"attention_mask", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention_mask)), METH_FASTCALL, nullptr},
     {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_route)), METH_FASTCALL, nullptr},
     {"distill_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_distill_loss)), METH_FASTCALL, nullptr},
     {"masked_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_masked_attention)), METH_FASTCALL, nullptr},

@@ -508,15 +508,16 @@ int check_route(const char* what, int T, int E, int k) {
 
 }  // namespace
 
-// 1 if the counts of this call are stored whole (they need no clearing), else they are added to what is there
-B200_API int b200_route_stores_counts(int T) { return T > 0 && T <= WARPS ? 1 : 0; }
-
 B200_API int b200_route(const void* logits, int is_bf16, long long ld, const float* bias, int T, int E, int k, int sigmoid, int groups,
                         int top_groups, int renorm, float scale, int* idx, float* w, int* counts, void* stream) {
   if (int r = check_route("route", T, E, k)) return r;
   if (groups < 1 || groups > MAX_G || E % groups != 0 || top_groups < 1 || top_groups > groups || top_groups * (E / groups) < k)
     return b200::fail(921, "route: %d experts in %d groups (at most %d) of which %d stay, for k=%d", E, groups, MAX_G, top_groups, k);
   if (T == 0) return 0;
+  if (route_grid(T) > 1) {                 // (one block stores its counts, several add to them)
+    const cudaError_t e = cudaMemsetAsync(counts, 0, sizeof(int) * E, (cudaStream_t)stream);
+    if (e != cudaSuccess) return b200::fail(923, "route: clearing the counts: %s", cudaGetErrorString(e));
+  }
   RouteParams p = {logits, ld, bias, T, E, k, sigmoid, groups, top_groups, renorm, 0, scale, idx, w, counts};
   p.vec = is_bf16 ? packable<__nv_bfloat16>(logits, ld, E) : packable<float>(logits, ld, E);
   if (is_bf16) launch_route<__nv_bfloat16>(p, (cudaStream_t)stream);

@@ -176,8 +176,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         if hasattr(lib, "b200_gemm_mxfp4_workspace"):
             host.bind_mx(ctypes.cast(lib.b200_gemm_mxfp4_workspace, c_void_p).value)
         if hasattr(lib, "b200_attn_masked_few_rows"):
-            host.bind_masked(*(ctypes.cast(getattr(lib, "b200_attn_masked_" + n), c_void_p).value
-                               for n in ("few_rows", "rows_workspace", "bwd_workspace")))
+            host.bind_masked(*(ctypes.cast(getattr(lib, "b200_attn_mask" + n), c_void_p).value
+                               for n in ("ed_few_rows", "ed_rows_workspace", "ed_bwd_workspace", "_ints")))
     lib.b200_norm_bwd_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.restype = c_ll
@@ -192,9 +192,6 @@ def _declare(lib: ctypes.CDLL) -> None:
         lib.b200_attn_masked_rows_workspace.restype = c_ll
         lib.b200_attn_masked_bwd_workspace.argtypes = [I, I, I, I]
         lib.b200_attn_masked_bwd_workspace.restype = c_ll
-    if hasattr(lib, "b200_route_stores_counts"):
-        lib.b200_route_stores_counts.argtypes = [I]
-        lib.b200_route_stores_counts.restype = c_int
     if hasattr(lib, "b200_sort_scratch_bytes"):
         lib.b200_sort_scratch_bytes.argtypes = [L]
         lib.b200_sort_scratch_bytes.restype = c_ll

@@ -74,16 +74,21 @@ def attention_mask(B: int, Sq: int, Skv: int | None = None, *, causal: bool = Tr
     those of its document's prefix: the leading positions of the document that ``prefix [B, Skv]`` (bool) flags.  With a ``window`` it sees only keys
     less than that many positions behind it."""
     Skv = Sq if Skv is None else Skv
+    given = [t for t in (documents, prefix) if t is not None]
+    dev = torch.device(device) if device is not None else (given[0].device if given else torch.device("cpu"))
+    if dev.type == "cuda" and dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    if dev.type == "cuda" and _lib.host is not None:
+        _lib.require()
+        buf = _lib.host.attention_mask(documents, prefix, B, Sq, Skv, int(causal), window, dev.index)
+        if buf is not None:
+            return AttentionMask(B, Sq, Skv, dev, buf=buf)
     if B < 1 or Sq < 1 or Skv < Sq or Skv > 2 ** 30:
         raise ValueError(f"attention_mask: {B} sequences, {Sq} queries at the end of {Skv} positions (at least one of each)")
     if not 0 <= window < 2 ** 30:
         raise ValueError(f"attention_mask: window {window}")
     if prefix is not None and not causal:
         raise ValueError("attention_mask: a prefix is what a causal mask leaves visible")
-    given = [t for t in (documents, prefix) if t is not None]
-    dev = torch.device(device) if device is not None else (given[0].device if given else torch.device("cpu"))
-    if dev.type == "cuda" and dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
     if documents is not None and (documents.shape != (B, Skv) or documents.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"attention_mask: documents [{B}, {Skv}] in int32 or int64, not {list(documents.shape)} in {documents.dtype}")
     if prefix is not None and (prefix.shape != (B, Skv) or prefix.dtype != torch.bool):

@@ -140,7 +140,7 @@ def route_fwd(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: tor
     dev = logits.device
     idx = torch.empty((T, k), dtype=torch.int32, device=dev)
     w = torch.empty((T, k), dtype=torch.float32, device=dev)
-    counts = (torch.empty if _lib.load().b200_route_stores_counts(T) else torch.zeros)(E, dtype=torch.int32, device=dev)
+    counts = (torch.empty if T > 0 else torch.zeros)(E, dtype=torch.int32, device=dev)
     b = None if bias is None else bias.detach().float().contiguous()
     with on_device_of(logits):
         call("b200_route", ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0), ptr(b), T, E, k, int(score == "sigmoid"), groups,
