@@ -364,9 +364,15 @@ attn_masked_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           }
           if (need_mask && ((SCORE & b200::SCORE_CAP) || g0 < all_lo || g0 + 32 > all_hi)) {
             const int from = c_lo - c0, to = c_hi - c0;
+            const bool out = from >= 32 || to <= 0 || from >= to;
+            if (__all_sync(0xffffffffu, out || (from <= 0 && to >= 32))) {      // each key by all of them or by none
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < from || i >= to) pr[h * 32 + i] = 0.f;
+              for (int i = 0; i < 32; ++i) pr[h * 32 + i] = out ? 0.f : pr[h * 32 + i];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i < from || i >= to) pr[h * 32 + i] = 0.f;
+            }
           }
         }
       }

@@ -58,7 +58,10 @@ def test_masks(B, Sq, Skv, kind, m):
                 a, c = tiles[b, t, 2:].tolist()
                 if len(v) and a < c:                                # [a, c) is visible to every row of the tile
                     assert (v[:, 0] <= a).all() and (v[:, 1] >= c).all()
-    cost = (qt[..., 1] - qt[..., 0]).view(B, nq // 2, 2).sum(-1).flatten()
+    pair = qt.view(B, nq // 2, 2, 4)
+    n = (pair[..., 1] - pair[..., 0]).sum(-1)
+    shared = (pair[..., 1].amin(-1) - pair[..., 0].amax(-1)).clamp(min=0)
+    cost = (4 * (n - shared) + shared).flatten()
     assert torch.equal(oq.sort()[0], torch.arange(B * nq // 2).int()) and (cost[oq.long()].diff() <= 0).all()
     cost = (kt[..., 1] - kt[..., 0]).flatten()
     assert torch.equal(ok.sort()[0], torch.arange(B * nk).int()) and (cost[ok.long()].diff() <= 0).all()
