@@ -12,7 +12,7 @@
 // of what was compared, the token goes through the same steps in fp64 (`choose_exact`; normal logits: 0.1 % of the tokens of 256 experts with
 // sigmoid scores, 1 % with softmax).  Without a bias the order is that of the logits: their upper 24 bits are the key, exact for bf16,
 // and neighbours that agree in them but not in the rest go to `choose_exact`.
-// 65536 tokens, 256 experts in 8 groups, k 8, bf16: ROUTE_US us (33 MB in); with a scan for the maximum over unsorted fp32 values, an owner's
+// 65536 tokens, 256 experts in 8 groups, k 8, bf16: 67 us (33 MB in); with a scan for the maximum over unsorted fp32 values, an owner's
 // ballot and a shuffle a round 203.
 #include "common.cuh"
 #include "runtime.h"
@@ -207,20 +207,31 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
     }
     __syncwarp();
   }
+  // Order-preserving keys of 64 bits, of experts lane + 32 i; 0: not there, not in a group that stays, or taken.  A round is the maximum of
+  // their upper halves, of the lower halves among those, and the least index.  (Over the fp64 values in shared memory with shuffles 5 us a token.)
   const int n = p.E / p.G;
-  unsigned taken = 0;                     // of this lane's experts lane + 32 i
+  unsigned long long key[MAX_E / 32];
+#pragma unroll
+  for (int i = 0; i < MAX_E / 32; ++i) {
+    const int e = lane + 32 * i;
+    const bool in = e < p.E && (p.top == p.G || (groups >> (e / n * sub) & 1));
+    const long long u = in ? __double_as_longlong(c[e] + 0.) : 0;          // (-0 is 0)
+    key[i] = in ? (unsigned long long)(u ^ ((u >> 63) | (long long)0x8000000000000000ull)) : 0ull;
+  }
   int mine = 0;
   for (int j = 0; j < p.k; ++j) {
-    double best = -INFINITY;
-    int at = MAX_E;                       // nothing yet: -inf at an index above all
-    for (int i = 0, e = lane; e < p.E; ++i, e += 32)
-      if (!(taken >> i & 1) && (p.top == p.G || (groups >> (e / n * sub) & 1)) && (c[e] > best || at == MAX_E)) { best = c[e]; at = e; }
-    for (int o = 16; o > 0; o >>= 1) {
-      const double b = __shfl_xor_sync(ALL, best, o);
-      const int a = __shfl_xor_sync(ALL, at, o);
-      if (a != MAX_E && (at == MAX_E || b > best || (b == best && a < at))) { best = b; at = a; }
-    }
-    if (at % 32 == lane) taken |= 1u << (at / 32);
+    unsigned long long best = key[0];
+    int at = lane;
+#pragma unroll
+    for (int i = 1; i < MAX_E / 32; ++i)
+      if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+    const unsigned hi = (unsigned)(best >> 32), lo = (unsigned)best;
+    const bool first = hi == __reduce_max_sync(ALL, hi);
+    const unsigned least = __reduce_max_sync(ALL, first ? lo : 0u);
+    at = (int)__reduce_min_sync(ALL, first && lo == least && best != 0ull ? (unsigned)at : (unsigned)MAX_E - 1);
+#pragma unroll
+    for (int i = 0; i < MAX_E / 32; ++i)
+      if (at == lane + 32 * i) key[i] = 0ull;
     if (j == lane) mine = at;
   }
   return mine;
@@ -245,14 +256,14 @@ B200_DEVICE void weigh(const TL* row, int t, int at, float m, float inv, const R
 // A warp takes a token; lane l holds experts l * NPL .. + NPL - 1.
 // FULL: E is 32 * NPL.
 template <typename TL, int NPL, bool FULL>
-__global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const __grid_constant__ RouteParams p) {
   b200::begin_kernel();
   __shared__ double s_c[WARPS][MAX_E];
   __shared__ int s_hist[MAX_E];
-  __shared__ int s_wait[WARPS][WAIT];
+  __shared__ int s_wait[WARPS * WAIT], s_waiting;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e0 = lane * NPL, n = p.E / p.G;
   for (int e = threadIdx.x; e < p.E; e += WARPS * 32) s_hist[e] = 0;
-  __syncthreads();
+  if (threadIdx.x == 0) s_waiting = 0;
   const bool biased = p.bias != nullptr, grouped = p.top < p.G;
   // Groups of whole lanes, a power of two of them, are reduced in registers.
   const int lanes = n / NPL;
@@ -282,17 +293,18 @@ __global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const RouteParams 
   __syncthreads();
   float* sc = reinterpret_cast<float*>(s_c[warp]);
   unsigned* sk = reinterpret_cast<unsigned*>(s_c[warp]) + lane * NPL;        // (not while sc is in use)
-  const int step = gridDim.x * WARPS;
-  int t = blockIdx.x * WARPS + warp;
+  const unsigned T = (unsigned)p.T, step = gridDim.x * WARPS;     // (no sum below reaches 2^32)
+  unsigned t = blockIdx.x * WARPS + warp;
   Pack<TL, NPL> ahead;                                           // the next token's logits are on their way meanwhile
-  if (t < p.T) ahead = fetch_row<TL, NPL>(reinterpret_cast<const TL*>(p.logits) + t * p.ld, e0, p.E, p.vec);
-  while (t < p.T) {
-  int waiting = 0;                                               // tokens for choose_exact, behind the loop (a call inside it costs its registers)
-  for (; t < p.T && waiting < WAIT; t += step) {
+  if (t < T) ahead = fetch_row<TL, NPL>(reinterpret_cast<const TL*>(p.logits) + t * p.ld, e0, p.E, p.vec);
+  // Tokens for choose_exact wait until WAIT tokens of each warp are through and are then shared by the block's warps: a call inside the loop costs
+  // its registers, and a warp that does its own two or three is waited for by the launch (90 us at 65536 tokens instead of 75).
+  for (unsigned t0 = blockIdx.x * WARPS; t0 < T; t0 += WAIT * step) {
+  for (const unsigned end = min(T, t0 + WAIT * step); t < end; t += step) {
     const TL* row = reinterpret_cast<const TL*>(p.logits) + t * p.ld;
     float x[NPL];
     row_values<TL, NPL, FULL>(ahead, e0, p.E, x);
-    if (p.T - t > step) ahead = fetch_row<TL, NPL>(row + (long long)step * p.ld, e0, p.E, p.vec);
+    if (T - t > step) ahead = fetch_row<TL, NPL>(row + (long long)step * p.ld, e0, p.E, p.vec);
     float m = 0.f, inv = 1.f;
     if (!p.sigmoid) softmax_stats<NPL>(x, m, inv);
     unsigned key[NPL];
@@ -367,15 +379,16 @@ __global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const RouteParams 
       exact |= __any_sync(ALL, close);
     }
     if (exact) {
-      if (lane == 0) s_wait[warp][waiting] = t;
-      ++waiting;
+      if (lane == 0) s_wait[atomicAdd(&s_waiting, 1)] = t;
     } else {
       weigh<TL>(row, t, at, m, inv, p, s_hist, lane);
     }
   }
-  for (int i = 0; i < waiting; ++i) {
+  __syncthreads();
+  const int waiting = s_waiting;
+  for (int i = warp; i < waiting; i += WARPS) {
     __syncwarp();
-    const int tt = s_wait[warp][i];
+    const int tt = s_wait[i];
     const TL* row = reinterpret_cast<const TL*>(p.logits) + tt * p.ld;
     const int at = choose_exact<TL>(row, p, s_c[warp], lane);
     float m = 0.f, inv = 1.f;
@@ -386,8 +399,10 @@ __global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const RouteParams 
     }
     weigh<TL>(row, tt, at, m, inv, p, s_hist, lane);
   }
-  }
   __syncthreads();
+  if (threadIdx.x == 0) s_waiting = 0;
+  if (T - t0 > WAIT * step) __syncthreads();         // (the last time nothing is added any more)
+  }
   for (int e = threadIdx.x; e < p.E; e += WARPS * 32) {
     if (gridDim.x == 1) p.counts[e] = s_hist[e];
     else if (s_hist[e] != 0) atomicAdd(&p.counts[e], s_hist[e]);         // (whole numbers: the order does not matter)
@@ -482,22 +497,30 @@ bool packable(const void* p, long long ld, int E) {
   return ((uintptr_t)p % b) == 0 && (ld * (long long)sizeof(TL)) % b == 0;
 }
 
-unsigned route_grid(int T) {
-  const long long blocks = ((long long)T + WARPS - 1) / WARPS, most = 6ll * b200::sm_count();
-  return (unsigned)(blocks < most ? blocks : most);
+// As many blocks as run at once (a second wave, of half as many, took 15 us of 76 at 65536 tokens).
+template <auto KERNEL, typename P>
+void launch_rows(const P& p, cudaStream_t s) {
+  static const int at_once = [] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, WARPS * 32, 0) == cudaSuccess && n > 0 ? n : 1;
+  }();
+  const long long blocks = ((long long)p.T + WARPS - 1) / WARPS, most = (long long)at_once * b200::sm_count();
+  b200::launch(KERNEL, (unsigned)(blocks < most ? blocks : most), WARPS * 32, 0, s, p);
 }
 
 template <typename TL, int NPL>
-auto route_of(const RouteParams& p) { return p.E == 32 * NPL ? route_kernel<TL, NPL, true> : route_kernel<TL, NPL, false>; }
-template <typename TL>
-void launch_route(const RouteParams& p, cudaStream_t s) {
-  auto k = p.E <= 32 ? route_of<TL, 1>(p) : p.E <= 64 ? route_of<TL, 2>(p) : p.E <= 128 ? route_of<TL, 4>(p) : route_of<TL, 8>(p);
-  b200::launch(k, route_grid(p.T), WARPS * 32, 0, s, p);
+void launch_of(const RouteParams& p, cudaStream_t s) {
+  if (p.E == 32 * NPL) launch_rows<route_kernel<TL, NPL, true>>(p, s);
+  else launch_rows<route_kernel<TL, NPL, false>>(p, s);
 }
-template <typename TL>
-void launch_route_bwd(const RouteBwdParams& p, cudaStream_t s) {
-  auto k = p.E <= 32 ? route_bwd_kernel<TL, 1> : p.E <= 64 ? route_bwd_kernel<TL, 2> : p.E <= 128 ? route_bwd_kernel<TL, 4> : route_bwd_kernel<TL, 8>;
-  b200::launch(k, route_grid(p.T), WARPS * 32, 0, s, p);
+template <typename TL, int NPL>
+void launch_of(const RouteBwdParams& p, cudaStream_t s) { launch_rows<route_bwd_kernel<TL, NPL>>(p, s); }
+template <typename TL, typename P>
+void launch_route(const P& p, cudaStream_t s) {
+  if (p.E <= 32) launch_of<TL, 1>(p, s);
+  else if (p.E <= 64) launch_of<TL, 2>(p, s);
+  else if (p.E <= 128) launch_of<TL, 4>(p, s);
+  else launch_of<TL, 8>(p, s);
 }
 
 int check_route(const char* what, int T, int E, int k) {
@@ -514,7 +537,7 @@ B200_API int b200_route(const void* logits, int is_bf16, long long ld, const flo
   if (groups < 1 || groups > MAX_G || E % groups != 0 || top_groups < 1 || top_groups > groups || top_groups * (E / groups) < k)
     return b200::fail(921, "route: %d experts in %d groups (at most %d) of which %d stay, for k=%d", E, groups, MAX_G, top_groups, k);
   if (T == 0) return 0;
-  if (route_grid(T) > 1) {                 // (one block stores its counts, several add to them)
+  if (T > WARPS) {                 // (one block stores its counts, several add to them)
     const cudaError_t e = cudaMemsetAsync(counts, 0, sizeof(int) * E, (cudaStream_t)stream);
     if (e != cudaSuccess) return b200::fail(923, "route: clearing the counts: %s", cudaGetErrorString(e));
   }
@@ -533,8 +556,8 @@ B200_API int b200_route_bwd(const void* logits, int is_bf16, long long ld, const
   RouteBwdParams p = {logits, ld, idx, gw, T, E, k, sigmoid, renorm, 0, scale, dx, 0};
   p.vec = is_bf16 ? packable<__nv_bfloat16>(logits, ld, E) : packable<float>(logits, ld, E);
   p.vec_out = is_bf16 ? packable<__nv_bfloat16>(dx, E, E) : packable<float>(dx, E, E);
-  if (is_bf16) launch_route_bwd<__nv_bfloat16>(p, (cudaStream_t)stream);
-  else launch_route_bwd<float>(p, (cudaStream_t)stream);
+  if (is_bf16) launch_route<__nv_bfloat16>(p, (cudaStream_t)stream);
+  else launch_route<float>(p, (cudaStream_t)stream);
   b200::count_launch();
   return b200::check_launch("route_bwd");
 }
