@@ -333,6 +333,8 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const int2 seen = row_next;            // keys [x, y) of this row
       const int mlo = t ? it.mlo1 : it.mlo0, mhi = t ? it.mhi1 : it.mhi0;
       const float slope2 = (SCORE & b200::SCORE_BIAS) ? p.score.slopes[it.h] * b200::LOG2E : 0.f;
+      // no row of the warp sees a key behind itself: the distance needs no absolute value, and the bias is two sums a pair
+      const bool behind = (SCORE & b200::SCORE_BIAS) && __all_sync(0xffffffffu, seen.y <= q_pos + off + 1);
       float m_ref = -INFINITY, l = 0.f;
       for (int n = it.lo(t); n < it.hi(t); ++n, ++ns) {
         const int kv0 = (it.j_lo + n) * BKV;
@@ -383,10 +385,21 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         }
         if (SCORE & b200::SCORE_BIAS) {
           const float d0 = (float)(kv0 - q_pos - off);
+          if (behind) {
+            // (slope d0 + slope i: what it rounds is 2^-24 of the bias, like the score's own rounding)
+            const float base = slope2 * d0, sc = (SCORE & b200::SCORE_CAP) ? 1.f : p.scale_log2;
 #pragma unroll
-          for (int i = 0; i < BKV; ++i) {
-            const float x = (SCORE & b200::SCORE_CAP) ? __uint_as_float(v[i]) : __uint_as_float(v[i]) * p.scale_log2;
-            v[i] = __float_as_uint(fmaf(-slope2, fabsf(d0 + (float)i), x));
+            for (int i = 0; i < BKV; i += 2) {
+              const float2 y = ffma2(make_float2(slope2, slope2), make_float2((float)i, (float)(i + 1)), make_float2(base, base));
+              const float2 x = ffma2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(sc, sc), y);
+              v[i] = __float_as_uint(x.x); v[i + 1] = __float_as_uint(x.y);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < BKV; ++i) {
+              const float x = (SCORE & b200::SCORE_CAP) ? __uint_as_float(v[i]) : __uint_as_float(v[i]) * p.scale_log2;
+              v[i] = __float_as_uint(fmaf(-slope2, fabsf(d0 + (float)i), x));
+            }
           }
         }
         // Where each row of the warp sees all of the tile or nothing of it (documents that begin among its rows), the rows that see nothing
@@ -399,10 +412,12 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           by_element = !__all_sync(0xffffffffu, (out && !it.unseen) || (kv0 >= seen.x && kv0 + BKV <= seen.y));
         }
         if (by_element) {
-          const int from = seen.x - kv0, to = seen.y - kv0;
+          // visible: |i - mid| < half (one comparison; whole and half numbers, exact)
+          const float from = (float)max(seen.x - kv0, -1), to = (float)min(seen.y - kv0, BKV + 1);
+          const float mid = 0.5f * (from + to) - 0.5f, half = seen.y > seen.x ? 0.5f * (to - from) : 0.f;
 #pragma unroll
           for (int i = 0; i < BKV; ++i)
-            if (i >= to || i < from) v[i] = 0xff800000u;  // -inf
+            if (!(fabsf((float)i - mid) < half)) v[i] = 0xff800000u;  // -inf
         }
         float mx4[4];
 #pragma unroll
