@@ -6,7 +6,7 @@
 // walked once from the end before for what each such chunk has behind it.  Then the warps take tiles of 128 positions, write their
 // intervals and reduce the tables of the key tiles (and of the query tiles, where these lie on the same positions).  Then the tiles of all sequences
 // are sorted by their range, longest first, for the schedules of the attention kernels: by the same CTA for one sequence, else by a second launch.
-// 16384 positions: 32 us with a scan over 4096 positions at a time through global memory, now 9; 61 positions 5.
+// 8 x 16384 positions: 32 us with a scan over 4096 positions at a time through global memory, now 14 and 3.6 for the order; one sequence of 61: 7.
 #include "attn_mask.cuh"
 #include "runtime.h"
 
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ M
     const int top = starts ? 31 - __clz(starts) : 0;
     const long long cur = scan_front(starts ? prefix_key(t, i0, top, end, bare) : -1, front, red64);
     // positions to warps: a tile of 128 at a time, so that neighbouring lanes write neighbouring intervals (each thread its own 16 would
-    // touch 32 lines a store, which took longer than all else: 16384 positions 16 us, now 9)
+    // touch 32 lines a store, which took longer than all else: 7 us more for 16384 positions)
     s_cur[threadIdx.x] = cur;
     s_behind[threadIdx.x] = make_int2(end, bare);
     s_bits[threadIdx.x] = make_uint2((t.start & 0xffffu) | t.pad << 16, t.flag);

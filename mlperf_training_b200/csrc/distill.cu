@@ -12,12 +12,13 @@
 //
 // Forward: one pass over the row for the log-sum-exp of u and of z on one running maximum.  Where both are wanted and tau is 2, 4 or 8, the
 // term of z is that of u squared once, twice or three times; another tau takes a second exponential (16 a clock and SM: 8192 rows of
-// 128256 in bf16 with two 626 us, FWD_US with one).  With `rest` the ids are marked in a bitmap and left out of the sum, which is then that
+// 128256 in bf16 with two 626 us, 336 with one).  With `rest` the ids are marked in a bitmap and left out of the sum, which is then that
 // of the others without cancellation, and the ids' own terms join it at the end.  One warp forms the teacher's sums meanwhile, in fp64
 // (r = 1 - sum p cancels); what they need of the student is its log-sum-exp alone.
 // Backward: the row again from the saved log-sum-exps, written as it is read; the elements of the ids and the label are then written once
 // more by a thread each, from logits read before any was overwritten, so the gradient may take the logits' place.
-// Both are bound by memory (one read; one read and one write) with four 16-byte loads a thread under way: 8192 x 128256 bf16 FWD_US and BWD_US us.
+// Both are bound by memory (one read; one read and one write) with four 16-byte loads a thread under way: 8192 x 128256 bf16
+// 336 and 640 us (6.25 and 6.56 TB/s).
 #include "common.cuh"
 #include "runtime.h"
 
@@ -131,8 +132,8 @@ template <> struct Raw<__nv_bfloat16> { using T = uint4; };
 // A CTA takes every gridDim.x-th row.  POWER: -1 the log-sum-exp of u alone; 1, 2, 3 that of z too, from u's terms squared so many times; 0
 // from an exponential of its own.  REST: ids are left out of the pass.
 // The last warp takes the teacher, whose chain of loads and sums is about as long as a third of a row (a warp that did both held the row
-// back: 8192 x 128256 484 us, 410 with a warp for each), and the end of each row, while the others are at the next one already: their
-// first loads of it are under way before they join their sums (FWD_US).  One barrier a row: sums and marks have two copies.
+// back: 8192 x 128256 bf16 484 us, 410 with a warp for each), and the end of each row, while the others are at the next one already: their
+// first loads of it are under way before they join their sums (336 us).  One barrier a row: sums and marks have two copies.
 template <typename TL, int POWER, bool REST>
 __global__ void __launch_bounds__(NT + 32, 2) distill_fwd_kernel(const DistillParams p) {
   b200::begin_kernel();

@@ -208,7 +208,7 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
     __syncwarp();
   }
   // Order-preserving keys of 64 bits, of experts lane + 32 i; 0: not there, not in a group that stays, or taken.  A round is the maximum of
-  // their upper halves, of the lower halves among those, and the least index.  (Over the fp64 values in shared memory with shuffles 5 us a token.)
+  // their upper halves, of the lower halves among those, and the least index.
   const int n = p.E / p.G;
   unsigned long long key[MAX_E / 32];
 #pragma unroll
