@@ -7,7 +7,7 @@
 //     first, over the kv heads of one after the other; a worker's key row sees one interval of queries;
 //   * delta = rowsum(dO O) with the output as the forward had it: its bf16 value and what that lost;
 //   * the factor of the cap is taken after P has gone to dV.
-// 8192 tokens, 32 heads of 128 on 8, causal: 1.33 ms (1.04 PFLOP/s), 16 documents in them 0.23; delta beside it 40 us (201 MB, 5 TB/s).  Bound by the
+// 8192 tokens, 32 heads of 128 on 8, causal: 1.33 ms (1.04 PFLOP/s), 16 documents in them 0.23 (delta and a cleared dQ are 57 us of it).  Bound by the
 // chain of a step (scores, P, dP, dS, their products), of which one CTA an SM has one under way.
 #include "attn_masked.cuh"
 
@@ -514,31 +514,49 @@ attn_masked_finish_kernel(const float* __restrict__ partial, int parts, int Hkv,
   }
 }
 
-// delta[b, h, s] = sum_d (O + low)[b, s, h, d] dO[b, s, h, d]; HD / 8 lanes per (token, head), 16-byte loads.  All three are contiguous.
+// delta[b, h, s] = sum_d (O + low)[b, s, h, d] dO[b, s, h, d], and dq = 0 for the sums that follow; HD / 8 lanes per (token, head), 16-byte loads, of
+// DELTA_ROWS rows at once.  All are contiguous.  8192 x 32 x 128: 57 us (335 MB, 5.9 TB/s); one row at
+// a time 40, and 19 for a launch that clears dq.
+constexpr int DELTA_ROWS = 4;
 template <int HD>
 __global__ void __launch_bounds__(256)
 attn_masked_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ low, const __nv_bfloat16* __restrict__ dout,
-                         float* __restrict__ delta, long long rows, int S, int H) {
+                         float* __restrict__ delta, float* __restrict__ dq, long long rows, int S, int H) {
   b200::begin_kernel();
-  constexpr int LANES = HD / 8;
-  const long long w = (blockIdx.x * 256ll + threadIdx.x) / LANES;
+  constexpr int LANES = HD / 8, STEP = 256 / LANES;
+  const long long w0 = (long long)blockIdx.x * (DELTA_ROWS * STEP) + threadIdx.x / LANES;
   const int l = threadIdx.x % LANES;
-  float acc = 0.f;
-  if (w < rows) {
-    const uint4 a = reinterpret_cast<const uint4*>(o)[w * LANES + l], c = reinterpret_cast<const uint4*>(low)[w * LANES + l],
-                d = reinterpret_cast<const uint4*>(dout)[w * LANES + l];
-    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {c.x, c.y, c.z, c.w}, z[4] = {d.x, d.y, d.z, d.w};
+  uint4 a[DELTA_ROWS], c[DELTA_ROWS], d[DELTA_ROWS];
+#pragma unroll
+  for (int k = 0; k < DELTA_ROWS; ++k) {
+    const long long w = w0 + k * STEP;
+    a[k] = c[k] = d[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (w < rows) {
+      a[k] = reinterpret_cast<const uint4*>(o)[w * LANES + l];
+      c[k] = reinterpret_cast<const uint4*>(low)[w * LANES + l];
+      d[k] = reinterpret_cast<const uint4*>(dout)[w * LANES + l];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < DELTA_ROWS; ++k) {
+    const long long w = w0 + k * STEP;
+    const uint32_t x[4] = {a[k].x, a[k].y, a[k].z, a[k].w}, y[4] = {c[k].x, c[k].y, c[k].z, c[k].w}, z[4] = {d[k].x, d[k].y, d[k].z, d[k].w};
+    float acc = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 p = unpack_bf16x2(x[j]), q = unpack_bf16x2(y[j]), g = unpack_bf16x2(z[j]);
       acc += (p.x + q.x) * g.x + (p.y + q.y) * g.y;
     }
-  }
 #pragma unroll
-  for (int off = LANES / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-  if (w < rows && l == 0) {
-    const long long h = w % H, t = w / H, s = t % S, b = t / S;
-    delta[(b * H + h) * S + s] = acc;
+    for (int off = LANES / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (w < rows) {
+      float4* row = reinterpret_cast<float4*>(dq) + w * (HD / 4) + l;
+      row[0] = row[LANES] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (l == 0) {
+        const long long h = w % H, t = w / H, s = t % S, b = t / S;
+        delta[(b * H + h) * S + s] = acc;
+      }
+    }
   }
 }
 
@@ -583,7 +601,7 @@ B200_API long long b200_attn_masked_bwd_workspace(int B, int Skv, int Hkv, int H
 }
 
 // q, k, v as in b200_attn_masked_fwd; out, low, dout [B, Sq, Hq, HD] contiguous; delta: fp32 [B, Hq, Sq], written here; dq_acc: fp32
-// [B, Sq, Hq, HD] contiguous, cleared by the caller (reduce-add target); dk / dv: bf16 [B, Skv, Hkv, HD] with their own pitches.
+// [B, Sq, Hq, HD] contiguous, cleared here (reduce-add target); dk / dv: bf16 [B, Skv, Hkv, HD] with their own pitches.
 B200_API int b200_attn_masked_bwd(const void* q, const void* k, const void* v, const void* out, const void* low, const void* dout, const float* lse,
                                   float* delta, float* dq_acc, void* dk, void* dv, const float* slopes, const int* mask, int B, int Sq, int Skv,
                                   int Hq, int Hkv, int HD, long long q_row, long long k_row, long long v_row, long long dk_row, long long dv_row,
@@ -620,11 +638,11 @@ B200_API int b200_attn_masked_bwd(const void* q, const void* k, const void* v, c
   if (p.parts > 1 && (workspace == nullptr || workspace_bytes < b200_attn_masked_bwd_workspace(B, Skv, Hkv, HD)))
     return b200::fail(962, "attn_masked_bwd: a workspace of %lld bytes", workspace_bytes);
   if (tiles * p.parts > 0x7fffffff) return b200::fail(963, "attn_masked_bwd: %lld key tiles", tiles);
-  const long long rows = (long long)B * Sq * Hq, blocks = (rows * (HD / 8) + 255) / 256;
+  const long long rows = (long long)B * Sq * Hq, blocks = (rows * (HD / 8) + 256 * DELTA_ROWS - 1) / (256 * DELTA_ROWS);
   if (blocks > 0x7fffffff) return b200::fail(963, "attn_masked_bwd: %lld rows", rows);
   cudaStream_t s = (cudaStream_t)stream;
   b200::launch(HD == 128 ? attn_masked_delta_kernel<128> : attn_masked_delta_kernel<64>, (unsigned)blocks, 256, 0, s, (const __nv_bfloat16*)out,
-               (const __nv_bfloat16*)low, (const __nv_bfloat16*)dout, delta, rows, Sq, Hq);
+               (const __nv_bfloat16*)low, (const __nv_bfloat16*)dout, delta, dq_acc, rows, Sq, Hq);
   b200::count_launch();
   if ((r = b200::check_launch("attn_masked_delta"))) return r;
   const int score = (cap > 0.f ? b200::SCORE_CAP : 0) | (slopes != nullptr ? b200::SCORE_BIAS : 0);

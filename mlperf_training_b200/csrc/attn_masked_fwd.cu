@@ -12,7 +12,7 @@
 //   * for a backward pass, what the output loses to bf16, as a second bf16 tensor (delta = rowsum(dO O) is formed from both), and the log-sum-exp
 //     of the probabilities before their rounding (dQ's error at standard deviation 2.25 0.250 % with that of the rounded ones, 0.244 with it; of
 //     that 0.235 are the two roundings to bf16 that no order of the sums avoids, of dS and of dQ itself).
-// 8192 tokens, 32 heads of 128 on 8, causal: 504 us (1.09 PFLOP/s), 511 with the second tensor.  Bound by the softmax of the two tiles and its
+// 8192 tokens, 32 heads of 128 on 8, causal: 504 us (1.09 PFLOP/s), 525 for a backward pass.  Bound by the softmax of the two tiles and its
 // turns with the products (2.4 us a key tile of both, of which 1.1 are exponentials at 16 a clock and SM); with 16 documents in those tokens 100 us,
 // 14.7 an item, of which 6 are its key tiles' and the others the first products and the output of each.
 #include "attn_masked.cuh"
@@ -455,7 +455,7 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         }
         const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
         // P = exp2(S * scale - m) as bf16 pairs over the first half of the S columns; -inf gives 0.  (All by ex2.approx: with every fourth pair
-        // by a polynomial, as in attention_fwd.cu, 8192 x 32 heads took 519 us instead of 504, with `low` 541 instead of 511: the rounded
+        // by a polynomial, as in attention_fwd.cu, 8192 x 32 heads took 519 us instead of 504, with `low` 541 instead of 511 (then without the sum for the log-sum-exp): the rounded
         // sums leave the FMA pipe no room.)
         const float scale2 = SCORE == b200::SCORE_PLAIN ? p.scale_log2 : 1.f;
         const float2 sc2 = make_float2(scale2, scale2);

@@ -800,7 +800,7 @@ struct MaskedAttentionBackward : public ag::Node {
     TORCH_CHECK(bshd(a, pq) && bshd(b, pk) && bshd(c, pv), "masked_attention: saved operands");
     const int64_t B = a.size(0), Sq = a.size(1), Hq = a.size(2), D = a.size(3), Skv = b.size(1), Hkv = b.size(2);
     const auto f32 = a.options().dtype(at::kFloat).requires_grad(false);
-    at::Tensor dq = at::zeros({B, Sq, Hq, D}, f32), dk = at::empty({B, Skv, Hkv, D}, a.options().requires_grad(false)), dv = at::empty_like(dk),
+    at::Tensor dq = at::empty({B, Sq, Hq, D}, f32), dk = at::empty({B, Skv, Hkv, D}, a.options().requires_grad(false)), dv = at::empty_like(dk),
                delta = at::empty({B, Hq, Sq}, f32);
     const long long n = g_masked_bwd_ws((int)B, (int)Skv, (int)Hkv, (int)D), w = Hkv * D;
     at::Tensor ws = workspace(n, a);

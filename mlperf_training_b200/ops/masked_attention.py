@@ -222,7 +222,7 @@ def masked_attention_bwd(dout, q, k, v, out, low, lse, mask: AttentionMask, *, s
     (q, q_row, q_batch), (k, k_row, k_batch), (v, v_row, v_batch) = _bshd(q), _bshd(k), _bshd(v)
     dout = dout.to(q.dtype).contiguous()
     dout = dout if dout.data_ptr() % 16 == 0 else dout.clone()
-    dq = torch.zeros((B, Sq, Hq, D), dtype=torch.float32, device=q.device)
+    dq = torch.empty((B, Sq, Hq, D), dtype=torch.float32, device=q.device)
     dk = dk_out if dk_out is not None else torch.empty((B, Skv, Hkv, D), dtype=k.dtype, device=k.device)
     dv = dv_out if dv_out is not None else torch.empty((B, Skv, Hkv, D), dtype=v.dtype, device=v.device)
     (wk, dk_row, dk_batch), (wv, dv_row, dv_batch) = _bshd(dk), _bshd(dv)
