@@ -454,9 +454,8 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           }
         }
         const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
-        // P = exp2(S * scale - m) as bf16 pairs over the first half of the S columns; -inf gives 0.  (All by ex2.approx: with every fourth pair
-        // by a polynomial, as in attention_fwd.cu, 8192 x 32 heads took 519 us instead of 504, with `low` 541 instead of 511 (then without the sum for the log-sum-exp): the rounded
-        // sums leave the FMA pipe no room.)
+        // P = exp2(S * scale - m) as bf16 pairs over the first half of the S columns; -inf gives 0.  (All by ex2.approx: with every fourth
+        // pair by a polynomial, as in attention_fwd.cu, 8192 x 32 heads took 519 us instead of 504: the sums leave the FMA pipe no room.)
         const float scale2 = SCORE == b200::SCORE_PLAIN ? p.scale_log2 : 1.f;
         const float2 sc2 = make_float2(scale2, scale2);
         const float nm = out ? -INFINITY : -m_use;             // (a row that is out: 2^-inf throughout)

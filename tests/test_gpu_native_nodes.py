@@ -107,6 +107,50 @@ def test_another_stream_and_gradients_of_other_layouts(name):
     _lib.check_status(name)
 
 
+def captured_route():
+    b = 0.1 * randn(64)
+    return [randn(50, 64, dtype=torch.bfloat16)], randn(50, 5, seed=1), lambda x: M.route(x, 5, score="sigmoid", bias=b, groups=8, top_groups=4)[1]
+
+
+def captured_distill():
+    labels, ids, values = torch.arange(50).cuda(), (torch.arange(350).view(50, 7) * 13 % 999).cuda(), randn(50, 7)
+    return [randn(50, 999, dtype=torch.bfloat16)], randn(50, seed=1), lambda z: F.distill_loss(z, labels, ids, values, alpha=0.6, temperature=2.0)
+
+
+def captured_attention():
+    ids, slopes = documents(2, 200, "few").cuda(), 0.1 * torch.ones(4).cuda()
+    return ([randn(2, 200, h, 64, seed=h, dtype=torch.bfloat16) for h in (4, 2, 2)], randn(2, 200, 4, 64, seed=1, dtype=torch.bfloat16),
+            lambda q, k, v: F.masked_attention(q, k, v, F.attention_mask(2, 200, documents=ids), softcap=9.0, slopes=slopes))
+
+
+@pytest.mark.parametrize("make", [captured_route, captured_distill, captured_attention])
+def test_captured_and_replayed_with_its_gradient(make):
+    given, g, f = make()
+    fed = [t.clone() for t in given]
+
+    def step():
+        ins = [t.detach().requires_grad_(True) for t in fed]
+        y = f(*ins)
+        return [y.detach()] + list(torch.autograd.grad(y, ins, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in (0, 1):
+        for t, x in zip(fed, given):
+            t.copy_(x.roll(turn, -1))
+        graph.replay()
+        for a, b in zip(step(), got):                          # (dQ is added up in another order each time)
+            assert torch.isfinite(a.float()).all() and (a.float() - b.float()).norm() <= 2 ** -8 * a.float().norm()
+    _lib.check_status(make.__name__)
+
+
 def test_sink_takes_the_general_path():
     sink = torch.zeros(4, device="cuda", requires_grad=True)
     out, y, ins, g = attention(sink=sink)
