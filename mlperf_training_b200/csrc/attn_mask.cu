@@ -184,7 +184,7 @@ B200_DEVICE void order_tiles(const MaskLayout& m, int* buf, bool of_q, int* bins
   const int n = of_q ? m.B * (m.Sp / 256) : m.B * (m.Kp / 128);
   const int4* t = reinterpret_cast<const int4*>(buf + (of_q ? m.qt : m.kt));
   int* out = buf + (of_q ? m.oq : m.ok);
-  const int unit = 8 * (of_q ? m.Kp : m.Sp) / 128 / BINS + 1;            // (costs reach eight a tile of the other side)
+  const int unit = (of_q ? m.Kp : m.Sp) / 16 / BINS + 1;            // (costs reach eight a tile of the other side)
   auto bin = [&](int i) {
     if (!of_q) return BINS - 1 - (t[i].y - t[i].x) / unit;
     const int a0 = t[2 * i].x, e0 = t[2 * i].y & ~b200::UNSEEN, a1 = t[2 * i + 1].x, e1 = t[2 * i + 1].y & ~b200::UNSEEN;

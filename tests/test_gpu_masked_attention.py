@@ -310,6 +310,19 @@ def test_captured_and_replayed_beside_an_eager_call():
     _lib.check_status("graph")
 
 
+def test_mask_of_very_many_positions():
+    Skv = 2 ** 28 + 5
+    m = F.attention_mask(1, 1, Skv, window=700, device="cuda")
+    nk, Kp = -(-Skv // 128), -(-Skv // 128) * 128
+    at = 2 * 4 + nk * 4                                        # query tiles, key tiles; then keys of the queries, queries of the keys, the orders
+    assert m.buf[at:at + 2].tolist() == [Skv - 700, Skv]
+    order = m.buf[at + 2 * 256 + 2 * Kp + 1:][:nk].long()
+    assert torch.equal(order.sort()[0], torch.arange(nk, device="cuda"))
+    seen = range((Skv - 700) // 128, nk)                       # come first
+    assert set(order[:len(seen)].tolist()) == set(seen)
+    _lib.check_status("mask")
+
+
 def test_refuses_what_the_kernels_do_not_read():
     mask = F.attention_mask(1, 4, device="cuda")
     x = torch.zeros(1, 4, 2, 64, device="cuda")
