@@ -588,15 +588,21 @@ int launch_bwd(int score, const CUtensorMap* m, const BwdParams& p, long long gr
   }
 }
 
-// CTAs that share a key tile: while the key tiles alone leave SMs idle.
-int parts_of(long long tiles) { return 1; }
+// CTAs that share a key tile: two to an SM in all at most, of four steps or more each (their fill and the sums behind them cost about three).
+// Causal, us with 1 / 2 / 4 / 8: 64 tiles of up to 256 steps 615 / 326 / 180 / 197, 64 of 64 133 / 78 / 56 / 72, 128 of 64 177 / 120 / 146 / 188, 32 of
+// 16 48 / 36 / 28 / 37, 256 of 128 361 / 378 / 461 / 581.
+int parts_of(int B, int Sq, int Skv, int Hq, int Hkv) {
+  const long long tiles = (long long)B * Hkv * ((Skv + BKV - 1) / BKV), steps = (long long)(Hq / Hkv) * ((Sq + BQ - 1) / BQ);
+  const long long n = 2ll * b200::sm_count() / tiles, most = steps / 4 < 8 ? steps / 4 : 8, parts = n < most ? n : most;
+  return (int)(parts > 1 ? parts : 1);
+}
 
 }  // namespace
 
 // bytes of the sums that CTAs sharing a key tile leave (0: every tile has one)
-B200_API long long b200_attn_masked_bwd_workspace(int B, int Skv, int Hkv, int HD) {
+B200_API long long b200_attn_masked_bwd_workspace(int B, int Sq, int Skv, int Hq, int Hkv, int HD) {
   const long long tiles = (long long)B * Hkv * ((Skv + BKV - 1) / BKV);
-  const int parts = parts_of(tiles);
+  const int parts = parts_of(B, Sq, Skv, Hq, Hkv);
   return parts > 1 ? tiles * parts * 2 * BKV * HD * 4 : 0;
 }
 
@@ -633,9 +639,9 @@ B200_API int b200_attn_masked_bwd(const void* q, const void* k, const void* v, c
   p.scale_log2 = scale * b200::LOG2E;
   p.lse = lse; p.delta = delta;
   p.status = b200::status_ptr();
-  p.parts = parts_of(tiles);
+  p.parts = parts_of(B, Sq, Skv, Hq, Hkv);
   p.partial = (float*)workspace;
-  if (p.parts > 1 && (workspace == nullptr || workspace_bytes < b200_attn_masked_bwd_workspace(B, Skv, Hkv, HD)))
+  if (p.parts > 1 && (workspace == nullptr || workspace_bytes < b200_attn_masked_bwd_workspace(B, Sq, Skv, Hq, Hkv, HD)))
     return b200::fail(962, "attn_masked_bwd: a workspace of %lld bytes", workspace_bytes);
   if (tiles * p.parts > 0x7fffffff) return b200::fail(963, "attn_masked_bwd: %lld key tiles", tiles);
   const long long rows = (long long)B * Sq * Hq, blocks = (rows * (HD / 8) + 256 * DELTA_ROWS - 1) / (256 * DELTA_ROWS);

@@ -150,7 +150,7 @@ MaskedRowsFn g_masked_rows = nullptr;
 MaskedBwdFn g_masked_bwd = nullptr;
 int (*g_few_rows)(int, int, int, int) = nullptr;
 long long (*g_rows_ws)(int, int, int, int, int, int) = nullptr;
-long long (*g_masked_bwd_ws)(int, int, int, int) = nullptr;
+long long (*g_masked_bwd_ws)(int, int, int, int, int, int) = nullptr;
 long long (*g_mask_ints)(int, int, int) = nullptr;
 int (*g_mask)(const void*, int, const uint8_t*, int, int, int, int, int, int*, void*) = nullptr;
 
@@ -802,7 +802,7 @@ struct MaskedAttentionBackward : public ag::Node {
     const auto f32 = a.options().dtype(at::kFloat).requires_grad(false);
     at::Tensor dq = at::empty({B, Sq, Hq, D}, f32), dk = at::empty({B, Skv, Hkv, D}, a.options().requires_grad(false)), dv = at::empty_like(dk),
                delta = at::empty({B, Hq, Sq}, f32);
-    const long long n = g_masked_bwd_ws((int)B, (int)Skv, (int)Hkv, (int)D), w = Hkv * D;
+    const long long n = g_masked_bwd_ws((int)B, (int)Sq, (int)Skv, (int)Hq, (int)Hkv, (int)D), w = Hkv * D;
     at::Tensor ws = workspace(n, a);
     check_rc("b200_attn_masked_bwd",
              g_masked_bwd(a.data_ptr(), b.data_ptr(), c.data_ptr(), o.data_ptr(), lo.data_ptr(), g.data_ptr(), ls.data_ptr<float>(),
@@ -916,7 +916,7 @@ PyObject* py_bind_masked(PyObject*, PyObject* args) {
   g_mask_ints = reinterpret_cast<long long (*)(int, int, int)>(d);
   g_few_rows = reinterpret_cast<int (*)(int, int, int, int)>(a);
   g_rows_ws = reinterpret_cast<long long (*)(int, int, int, int, int, int)>(b);
-  g_masked_bwd_ws = reinterpret_cast<long long (*)(int, int, int, int)>(c);
+  g_masked_bwd_ws = reinterpret_cast<long long (*)(int, int, int, int, int, int)>(c);
   Py_RETURN_NONE;
 }
 

@@ -190,7 +190,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         lib.b200_attn_masked_few_rows.restype = c_int
         lib.b200_attn_masked_rows_workspace.argtypes = [I, I, I, I, I, I]
         lib.b200_attn_masked_rows_workspace.restype = c_ll
-        lib.b200_attn_masked_bwd_workspace.argtypes = [I, I, I, I]
+        lib.b200_attn_masked_bwd_workspace.argtypes = [I, I, I, I, I, I]
         lib.b200_attn_masked_bwd_workspace.restype = c_ll
     if hasattr(lib, "b200_sort_scratch_bytes"):
         lib.b200_sort_scratch_bytes.argtypes = [L]

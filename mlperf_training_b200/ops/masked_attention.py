@@ -227,7 +227,7 @@ def masked_attention_bwd(dout, q, k, v, out, low, lse, mask: AttentionMask, *, s
     dv = dv_out if dv_out is not None else torch.empty((B, Skv, Hkv, D), dtype=v.dtype, device=v.device)
     (wk, dk_row, dk_batch), (wv, dv_row, dv_batch) = _bshd(dk), _bshd(dv)
     delta = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
-    n = int(_lib.load().b200_attn_masked_bwd_workspace(B, Skv, Hkv, D))
+    n = int(_lib.load().b200_attn_masked_bwd_workspace(B, Sq, Skv, Hq, Hkv, D))
     ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
     slopes = None if slopes is None else slopes.detach().float().contiguous()
     with _lib.on_device_of(q):
