@@ -5,8 +5,9 @@
 // position without a flag; from the front, the last start with the end of its prefix.  16384 positions go at a time; longer sequences are
 // walked once from the end before for what each such chunk has behind it.  Then the warps take tiles of 128 positions, write their
 // intervals and reduce the tables of the key tiles (and of the query tiles, where these lie on the same positions).  Then the tiles of all sequences
-// are sorted by their range, longest first, for the schedules of the attention kernels: by the same CTA for one sequence, else by a second launch.
-// 8 x 16384 positions: 32 us with a scan over 4096 positions at a time through global memory, now 14 and 3.6 for the order; one sequence of 61: 7.
+// are sorted by their range, longest first, for the schedules of the attention kernels: by the same launch where a cluster holds all sequences, else
+// by a second one.  Above 4096 positions the tiles of a sequence are shared by the CTAs of a cluster, each of which makes the scans.
+// One sequence of 61 positions 6.2 us (7.8 with bins for few tiles), of 8192 9.8 (12.5 by one CTA), of 32768 21 (35); 8 of 16384 12.0 (16.7).
 #include "attn_mask.cuh"
 #include "runtime.h"
 
@@ -24,6 +25,8 @@ struct MaskParams {
   const uint8_t* flags;        // [B, Skv] or null
   int ids64, causal, window;
   int* buf;
+  int parts;                   // CTAs a sequence, neighbours in a cluster: each makes the scans and writes its share of the tiles
+  int whole;                   // the cluster holds all sequences, and sorts
 };
 
 B200_DEVICE long long id_at(const MaskParams& p, long long i) {
@@ -191,6 +194,18 @@ B200_DEVICE void order_tiles(const MaskLayout& m, int* buf, bool of_q, int* bins
     const int shared = max(min(e0, e1) - max(a0, a1), 0);
     return BINS - 1 - (4 * (e0 - a0 + e1 - a1 - shared) + shared) / unit;
   };
+  if (n <= 32) {                                               // a warp: each lane's place is the number of tiles before it
+    if (threadIdx.x < 32) {
+      const int mine = (int)threadIdx.x < n ? bin((int)threadIdx.x) : BINS;
+      int place = 0;
+      for (int i = 0; i < n; ++i) {
+        const int other = __shfl_sync(ALL, mine, i);
+        place += other < mine || (other == mine && i < (int)threadIdx.x) ? 1 : 0;
+      }
+      if ((int)threadIdx.x < n) out[place] = (int)threadIdx.x;
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < BINS; i += NT) bins[i] = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += NT) atomicAdd(&bins[bin(i)], 1);
@@ -224,6 +239,7 @@ static_assert(BINS == 2 * NT, "a thread scans two bins");
 __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ MaskParams p) {
   b200::begin_kernel();
   __shared__ int red[2][NT / 32];
+  __shared__ int s_any[8];
   __shared__ long long red64[NT / 32];
   __shared__ union {
     int bins[BINS];
@@ -233,7 +249,7 @@ __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ M
   int2* s_behind = sh.own.behind;
   uint2* s_bits = sh.own.bits;
   const MaskLayout& m = p.m;
-  const int b = blockIdx.x, S = m.Skv, off = m.Skv - m.Sq, nq = m.Sp / 128, nk = m.Kp / 128;
+  const int part = (int)blockIdx.x % p.parts, b = (int)blockIdx.x / p.parts, S = m.Skv, off = m.Skv - m.Sq, nq = m.Sp / 128, nk = m.Kp / 128;
   const long long base = (long long)b * S;
   int2* q_iv = reinterpret_cast<int2*>(p.buf + m.q_iv) + (long long)b * m.Sp;
   int2* k_iv = reinterpret_cast<int2*>(p.buf + m.k_iv) + (long long)b * m.Kp;
@@ -274,7 +290,7 @@ __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ M
     s_behind[threadIdx.x] = make_int2(end, bare);
     s_bits[threadIdx.x] = make_uint2((t.start & 0xffffu) | t.pad << 16, t.flag);
     __syncthreads();
-    for (int j = warp * 128; j < CHUNK && c * CHUNK + j < S; j += NT / 32 * 128) {
+    for (int j = (part * (NT / 32) + warp) * 128; j < CHUNK && c * CHUNK + j < S; j += p.parts * (NT / 32) * 128) {
       Tile tk, tq;
 #pragma unroll
       for (int part = 0; part < 4; ++part) {
@@ -315,22 +331,39 @@ __global__ void __launch_bounds__(NT) attn_mask_kernel(const __grid_constant__ M
     }
     __syncthreads();
   }
-  for (int i = S + (int)threadIdx.x; i < m.Kp; i += NT) k_iv[i] = make_int2(0, 0);
-  for (int i = m.Sq + (int)threadIdx.x; i < m.Sp; i += NT) q_iv[i] = make_int2(0, 0);
-  __syncthreads();
+  if (part == 0) {
+    for (int i = S + (int)threadIdx.x; i < m.Kp; i += NT) k_iv[i] = make_int2(0, 0);
+    for (int i = m.Sq + (int)threadIdx.x; i < m.Sp; i += NT) q_iv[i] = make_int2(0, 0);
+  }
+  const int any = __syncthreads_or(unseen);
+  if (p.parts > 1) {
+    cluster_sync_all();
+    const uint32_t first = cluster_ctarank() - part;           // the sequence's first CTA
+    if (threadIdx.x == 0) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(smem_u32(&s_any[part]), first)), "r"(any) : "memory");
+  }
   // query tiles on other positions than key tiles, and behind the last query
-  for (int t = (same ? (m.Sq + 127) / 128 : 0) + warp; t < nq; t += NT / 32) {
+  for (int t = (same ? (m.Sq + 127) / 128 : 0) + part * (NT / 32) + warp; t < nq; t += p.parts * (NT / 32)) {
     Tile v;
     for (int r = t * 128 + lane; r < (t + 1) * 128 && r < m.Sq; r += 32) v.add(q_iv[r].x, q_iv[r].y);
     v.join();
     if (lane == 0) qt[t] = v.entry(false);
   }
-  if (__syncthreads_or(unseen))
-    for (int t = threadIdx.x; t < nq; t += NT) qt[t].y |= b200::UNSEEN;
-  if (m.B == 1) {
+  bool some = any != 0;
+  if (p.parts > 1) {
+    cluster_sync_all();
+    if (part == 0)
+      for (int i = 0; i < p.parts; ++i) some |= s_any[i] != 0;
+  } else {
     __syncthreads();
-    order_tiles(m, p.buf, true, sh.bins, red[0]);
-    order_tiles(m, p.buf, false, sh.bins, red[0]);
+  }
+  if (part == 0 && some)
+    for (int t = threadIdx.x; t < nq; t += NT) qt[t].y |= b200::UNSEEN;
+  if (p.whole) {
+    const int ctas = m.B * p.parts;
+    if (m.B > 1) cluster_sync_all();
+    else __syncthreads();
+    if (blockIdx.x == 0) order_tiles(m, p.buf, true, sh.bins, red[0]);
+    if ((int)blockIdx.x == (ctas > 1 ? 1 : 0)) order_tiles(m, p.buf, false, sh.bins, red[0]);
   }
 }
 
@@ -353,11 +386,27 @@ B200_API long long b200_attn_mask_ints(int B, int Sq, int Skv) {
 B200_API int b200_attn_mask(const void* ids, int ids64, const uint8_t* flags, int B, int Sq, int Skv, int causal, int window, int* buf, void* stream) {
   if (B < 1 || Sq < 1 || Skv < Sq || Skv > (1 << 30)) return b200::fail(940, "attn_mask: B=%d, Sq=%d, Skv=%d", B, Sq, Skv);
   if (window < 0 || (flags != nullptr && !causal)) return b200::fail(941, "attn_mask: window %d, a prefix wants a causal mask", window);
-  MaskParams p = {MaskLayout::of(B, Sq, Skv), ids, flags, ids64, causal, window, buf};
+  MaskParams p = {MaskLayout::of(B, Sq, Skv), ids, flags, ids64, causal, window, buf, 1, 0};
   if ((long long)B * (p.m.Kp / 128) > 0x3fffffff) return b200::fail(942, "attn_mask: %d sequences of %d keys", B, Skv);
-  b200::launch(attn_mask_kernel, B, NT, 0, (cudaStream_t)stream, p);
+  // (a CTA has 32 warps, a tile each; one CTA for 16384 positions 8.9 us in its tiles)
+  if (Skv > NT / 32 * 128)
+    while (p.parts < 8 && 2ll * p.parts * B <= b200::sm_count()) p.parts *= 2;
+  p.whole = (long long)B * p.parts <= 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)B * p.parts);
+  cfg.blockDim = dim3(NT);
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.whole ? B * p.parts : p.parts;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = attr[1].val.clusterDim.x > 1 ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, attn_mask_kernel, p);               // (a failure is seen by check_launch)
   b200::count_launch();
-  if (B > 1) {
+  if (!p.whole) {
     b200::launch(attn_mask_order_kernel, 2, NT, 0, (cudaStream_t)stream, p.m, buf);
     b200::count_launch();
   }
