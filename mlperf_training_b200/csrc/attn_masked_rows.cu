@@ -3,7 +3,7 @@
 // The query rows of one key head (its group of heads x the queries, 16 at a time) share a CTA's tiles.  A CTA takes a share of the keys that
 // any of its rows sees, its four warps take its tiles of 16 keys in turn, each with a ring of its own (TMA, one lane), online softmax
 // in registers and m16n8k16 products (padded rows cost nothing that matters beside the loads: 16 keys are 8 KB and 32 instructions at head
-// dim 128); they join in shared memory, and where a head's keys are split over several CTAs a second launch joins those.
+// dim 128); they join in shared memory, and where a head's keys are split over several CTAs these join as a cluster or by a second launch.
 // Probabilities are exactly 0 where a row does not see a key, their sum is of the rounded ones that are multiplied, and value rows
 // that no row sees are cleared before the product.
 // 8 tokens over 7400 to 16384 keys each, 8 key heads of 128: 372 MB in 61 us (6.1 TB/s), the join 7.
@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int WARPS = 4, KT = 16, STAGES = 3, ROWS = 16;
+constexpr int WARPS = 4, KT = 16, STAGES = 3, ROWS = 16, CLUSTER = 8;
 
 struct RowsParams {
   b200::MaskView mask;
@@ -22,7 +22,8 @@ struct RowsParams {
   const float* sink;
   float* lse;               // [B, Hq, Sq]
   __nv_bfloat16* out;       // [B, Sq, Hq, HD]
-  float* part;              // splits > 1: [rows][splits][HD], rows = (b * Sq + q) * Hq + h
+  int cluster;              // the CTAs of a head's shares are a cluster, and join in its shared memory
+  float* part;              // else, splits > 1: [rows][splits][HD], rows = (b * Sq + q) * Hq + h
   float2* part_ml;          // [rows][splits]: maximum (log2) and sum
   int* status;
 };
@@ -46,6 +47,33 @@ B200_DEVICE void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_
 }
 // 16-byte chunk `ch` of row r of a tile of 64-column blocks, 128-byte swizzle
 B200_DEVICE uint32_t chunk(uint32_t tile, int r, int ch) { return tile + (ch >> 3) * (KT * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4); }
+
+B200_DEVICE float2 ld_cluster_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+B200_DEVICE float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// A warp's row `at` = (b * Sq + q) * Hq + h from its sum of values, maximum and sum of probabilities (mw, lw).
+template <int HD>
+B200_DEVICE void finish_row(const RowsParams& p, long long at, float (&acc)[HD / 32], float mw, float lw, int lane) {
+  const int h = (int)(at % p.Hq);
+  const long long bq = at / p.Hq;
+  const bool none = mw == -INFINITY;
+  if (p.sink != nullptr) {
+    const float sk = p.sink[h] * b200::LOG2E;
+    if (none) { mw = sk; lw = 1.f; } else lw += ex2_approx(sk - mw);
+  }
+  const float inv = none ? 0.f : 1.f / lw;
+#pragma unroll
+  for (int c = 0; c < HD / 32; ++c) p.out[at * HD + c * 32 + lane] = __float2bfloat16(none ? 0.f : acc[c] * inv);
+  if (lane == 0) p.lse[((bq / p.Sq) * p.Hq + h) * p.Sq + bq % p.Sq] = lw > 0.f ? (mw + log2f(lw)) * 0.6931471805599453f : -INFINITY;
+}
 
 template <int HD>
 __global__ void __launch_bounds__(WARPS * 32, 2)
@@ -258,21 +286,36 @@ attn_masked_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       for (int w = 0; w < WARPS; ++w)
         if (f[w] != 0.f) acc[c] += f[w] * reinterpret_cast<const float*>(smem + w * STAGES * 2 * SM::TILE)[rr * (HD + 4) + c * 32 + lane];
     }
-    if (p.splits > 1) {
+    if (p.splits == 1) {
+      finish_row<HD>(p, at, acc, mw, lw, lane);
+    } else if (p.cluster) {                                    // (in the first warp's part: the row is this warp's alone)
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) reinterpret_cast<float*>(smem)[rr * (HD + 4) + c * 32 + lane] = acc[c];
+      if (lane == 0) s_ml[rr] = make_float2(mw, lw);
+      __syncwarp();
+    } else {
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) p.part[(at * p.splits + split) * HD + c * 32 + lane] = acc[c];
       if (lane == 0) p.part_ml[at * p.splits + split] = make_float2(mw, lw);
-      continue;
     }
-    const bool none = mw == -INFINITY;
-    if (p.sink != nullptr) {
-      const float sk = p.sink[h] * b200::LOG2E;
-      if (none) { mw = sk; lw = 1.f; } else lw += ex2_approx(sk - mw);
-    }
-    const float inv = none ? 0.f : 1.f / lw;
+  }
+  if (p.splits > 1 && p.cluster) {
+    cluster_sync_all();
+    // the rows in turn to the warps of the cluster
+    for (int rr = split * WARPS + warp; rr < ROWS && row0 + rr < rows; rr += p.splits * WARPS) {
+      const int r = row0 + rr;
+      const float2 ml = lane < p.splits ? ld_cluster_f32x2(mapa_u32(smem_u32(&s_ml[rr]), lane)) : make_float2(-INFINITY, 0.f);
+      const float mw = warp_max(ml.x), f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mw), lw = warp_sum(ml.y * f);
+      float acc[HD / 32] = {};
+      for (int z = 0; z < p.splits; ++z) {
+        const float w = __shfl_sync(0xffffffffu, f, z);
+        const uint32_t from = mapa_u32(smem_u32(smem) + (rr * (HD + 4) + lane) * 4, z);
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c) p.out[at * HD + c * 32 + lane] = __float2bfloat16(none ? 0.f : acc[c] * inv);
-    if (lane == 0) p.lse[((long long)b * p.Hq + h) * p.Sq + qi] = lw > 0.f ? (mw + log2f(lw)) * 0.6931471805599453f : -INFINITY;
+        for (int c = 0; c < HD / 32; ++c) acc[c] += w * ld_cluster_f32(from + c * 128);
+      }
+      finish_row<HD>(p, ((long long)b * p.Sq + r / group) * p.Hq + hk * group + r % group, acc, mw, lw, lane);
+    }
+    cluster_sync_all();                                        // (shared memory stays until it has been read)
   }
 }
 
@@ -283,38 +326,35 @@ __global__ void __launch_bounds__(128) attn_masked_join_kernel(const __grid_cons
   const long long at = (blockIdx.x * 128ll + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (at >= (long long)p.B * p.Sq * p.Hq) return;
-  const int h = (int)(at % p.Hq);
-  const long long bq = at / p.Hq;
   // a lane a part for the weights, then all lanes over the parts' rows (empty ones are 0)
   const float2 ml = lane < p.splits ? p.part_ml[at * p.splits + lane] : make_float2(-INFINITY, 0.f);
-  float mw = warp_max(ml.x);
-  const bool none = mw == -INFINITY;
+  const float mw = warp_max(ml.x);
   const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mw);
-  float lw = warp_sum(ml.y * f), acc[HD / 32] = {};
+  const float lw = warp_sum(ml.y * f);
+  float acc[HD / 32] = {};
 #pragma unroll 8
   for (int z = 0; z < p.splits; ++z) {
     const float w = __shfl_sync(0xffffffffu, f, z);
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c) acc[c] += w * p.part[(at * p.splits + z) * HD + c * 32 + lane];
   }
-  if (p.sink != nullptr) {
-    const float sk = p.sink[h] * b200::LOG2E;
-    if (none) { mw = sk; lw = 1.f; } else lw += ex2_approx(sk - mw);
-  }
-  const float inv = none ? 0.f : 1.f / lw;
-#pragma unroll
-  for (int c = 0; c < HD / 32; ++c) p.out[at * HD + c * 32 + lane] = __float2bfloat16(none ? 0.f : acc[c] * inv);
-  if (lane == 0) p.lse[((bq / p.Sq) * p.Hq + h) * p.Sq + bq % p.Sq] = lw > 0.f ? (mw + log2f(lw)) * 0.6931471805599453f : -INFINITY;
+  finish_row<HD>(p, at, acc, mw, lw, lane);
 }
 
 // Shares of a head's keys: four CTAs an SM in all at most (two run at once; 8 sequences of 7400 to 16384 keys x 8 key heads at head dim 128: 60.8 us
 // with 9 shares, 576 CTAs, and 70 with 10, 640), of 256 keys or more each.
-int splits_of(int B, int Sq, int Skv, int Hq, int Hkv) {
-  const long long heads = (long long)B * Hkv * (((long long)Hq / Hkv * Sq + ROWS - 1) / ROWS);
-  long long n = 4ll * b200::sm_count() / heads;
-  const long long most = (Skv + 255) / 256;
-  if (n > most) n = most;
-  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);        // (a lane of the joining warp for each)
+// Where their CTAs all run at once and a head's are at most CLUSTER, these are a cluster that joins them (3000 keys of 8 heads 11.5 -> 10.8 us, and a launch
+// less for the host); with more CTAs than that clusters wait for each other's places (2000 keys of 64 heads 18.3 -> 20.2, 32768 of 128 306 -> 323).
+struct Splits { int n; bool cluster; };
+Splits splits_of(int B, int Sq, int Skv, int Hq, int Hkv) {
+  const long long heads = (long long)B * Hkv * (((long long)Hq / Hkv * Sq + ROWS - 1) / ROWS), at_once = b200::sm_count() * 3ll / 2;
+  const long long n = 4ll * b200::sm_count() / heads, most = (Skv + 255) / 256;
+  Splits s = {(int)(n < most ? n : most), false};
+  if (s.n > CLUSTER && s.n < 2 * CLUSTER && heads * CLUSTER <= at_once) s.n = CLUSTER;
+  if (s.n < 1) s.n = 1;
+  if (s.n > 32) s.n = 32;                            // (a lane of the joining warp for each)
+  s.cluster = s.n > 1 && s.n <= CLUSTER && heads * s.n <= at_once;
+  return s;
 }
 
 template <int HD>
@@ -332,10 +372,23 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const RowsParams& 
     configured[dev & 63] = true;
   }
   const int blocks = (p.Hq / p.Hkv * p.Sq + ROWS - 1) / ROWS;
-  b200::launch(attn_masked_rows_kernel<HD>, dim3((unsigned)p.splits, (unsigned)(p.Hkv * blocks), (unsigned)p.B), WARPS * 32, SM::TOTAL, stream, tk, tv, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.splits, (unsigned)(p.Hkv * blocks), (unsigned)p.B);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = SM::TOTAL;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, attn_masked_rows_kernel<HD>, tk, tv, p);      // (a failure is seen by check_launch)
   b200::count_launch();
   int r = b200::check_launch("attn_masked_rows");
-  if (r || p.splits == 1) return r;
+  if (r || p.splits == 1 || p.cluster) return r;
   const long long rows = (long long)p.B * p.Sq * p.Hq;
   b200::launch(attn_masked_join_kernel<HD>, (unsigned)((rows * 32 + 127) / 128), 128, 0, stream, p);
   b200::count_launch();
@@ -350,8 +403,8 @@ B200_API int b200_attn_masked_few_rows(int B, int Sq, int Hq, int Hkv) {
 }
 // bytes of workspace (0: none)
 B200_API long long b200_attn_masked_rows_workspace(int B, int Sq, int Skv, int Hq, int Hkv, int HD) {
-  const int n = splits_of(B, Sq, Skv, Hq, Hkv);
-  return n > 1 ? (long long)B * Sq * Hq * n * (HD * 4 + 8) : 0;
+  const Splits s = splits_of(B, Sq, Skv, Hq, Hkv);
+  return s.n > 1 && !s.cluster ? (long long)B * Sq * Hq * s.n * (HD * 4 + 8) : 0;
 }
 
 // As b200_attn_masked_fwd, for the calls that b200_attn_masked_few_rows names.
@@ -372,11 +425,13 @@ B200_API int b200_attn_masked_rows(const void* q, const void* k, const void* v, 
   p.score = b200::ScoreParams::of(scale, cap, slopes);
   p.q = (const __nv_bfloat16*)q; p.q_row = q_row; p.q_batch = q_batch;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Skv = Skv;
-  p.splits = splits_of(B, Sq, Skv, Hq, Hkv);
+  const Splits sp = splits_of(B, Sq, Skv, Hq, Hkv);
+  p.splits = sp.n;
+  p.cluster = sp.cluster;
   p.sink = sink; p.lse = lse; p.out = (__nv_bfloat16*)out;
   p.status = b200::status_ptr();
   const long long rows = (long long)B * Sq * Hq;
-  if (p.splits > 1 && (workspace == nullptr || workspace_bytes < rows * p.splits * (HD * 4 + 8)))
+  if (p.splits > 1 && !p.cluster && (workspace == nullptr || workspace_bytes < rows * p.splits * (HD * 4 + 8)))
     return b200::fail(972, "attn_masked_rows: a workspace of %lld bytes", workspace_bytes);
   p.part = (float*)workspace;
   p.part_ml = reinterpret_cast<float2*>(p.part + rows * p.splits * HD);
