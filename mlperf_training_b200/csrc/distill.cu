@@ -24,8 +24,9 @@
 
 namespace {
 
-constexpr int NT = 512, MAX_K = 1024, SLOTS = MAX_K / NT;
+constexpr int MAX_K = 1024;
 constexpr int AHEAD = 4;           // 16-byte loads of a thread under way
+constexpr int SHORT_BYTES = 100 * 1024;      // of a row, up to which it is short
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 enum { F32 = 0, BF16 = 1 };
@@ -134,8 +135,9 @@ template <> struct Raw<__nv_bfloat16> { using T = uint4; };
 // The last warp takes the teacher, whose chain of loads and sums is about as long as a third of a row (a warp that did both held the row
 // back: 8192 x 128256 bf16 484 us, 410 with a warp for each), and the end of each row, while the others are at the next one already: their
 // first loads of it are under way before they join their sums (336 us).  One barrier a row: sums and marks have two copies.
-template <typename TL, int POWER, bool REST>
-__global__ void __launch_bounds__(NT + 32, 2) distill_fwd_kernel(const DistillParams p) {
+// NT threads for a row's elements: 512, or 64 in more CTAs where rows are short (see launch_fwd).
+template <typename TL, int POWER, bool REST, int NT>
+__global__ void __launch_bounds__(NT + 32, NT == 512 ? 2 : 10) distill_fwd_kernel(const DistillParams p) {
   b200::begin_kernel();
   constexpr bool BOTH = POWER >= 0;
   constexpr int N = Vec<TL>::N;
@@ -367,12 +369,12 @@ __global__ void __launch_bounds__(NT + 32, 2) distill_fwd_kernel(const DistillPa
 }
 
 // CTA (t, part): columns [part, part + 1) * V / parts of row t.
-template <typename TL, int POWER>
-__global__ void __launch_bounds__(NT, 2) distill_bwd_kernel(const DistillParams p) {
+template <typename TL, int POWER, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const DistillParams p) {
   b200::begin_kernel();
   __shared__ int s_id[MAX_K];
   __shared__ float s_p[MAX_K];
-  constexpr int N = Vec<TL>::N;
+  constexpr int N = Vec<TL>::N, SLOTS = MAX_K / NT;
   const long long t = blockIdx.x;
   const int lo = (int)((long long)p.V * blockIdx.y / gridDim.y), hi = (int)((long long)p.V * (blockIdx.y + 1) / gridDim.y);
   const TL* row = reinterpret_cast<const TL*>(p.logits) + t * p.ld;
@@ -507,22 +509,33 @@ int power_of(const DistillParams& p) {
   return p.tau == 2.f ? 1 : p.tau == 4.f ? 2 : p.tau == 8.f ? 3 : 0;
 }
 
-template <typename TL, int POWER>
+// Many short rows: what counts is how many are under way, not how fast one is.  us, forward and backward, 512 threads against 64 and 128:
+// 16384 x 1000 fp32 213 + 261, 46 + 80; 8192 x 4096 bf16 91 + 143, 24 + 51; 4096 x 50304 bf16 91 + 172, 76 + 152; 4096 x 32000 fp32 78 + 181, 90 + 178.
+template <typename TL>
+bool short_rows(const DistillParams& p) { return p.T > 2 * b200::sm_count() && (long long)p.V * (int)sizeof(TL) <= SHORT_BYTES; }
+
+template <typename TL, int POWER, int NT>
 int launch_fwd(const DistillParams& p, cudaStream_t s) {
-  auto k = p.rest ? distill_fwd_kernel<TL, POWER, true> : distill_fwd_kernel<TL, POWER, false>;
+  auto k = p.rest ? distill_fwd_kernel<TL, POWER, true, NT> : distill_fwd_kernel<TL, POWER, false, NT>;
   const size_t smem = p.rest ? ((size_t)p.V + 31) / 32 * 8 : 0;
   if (int r = set_smem((const void*)k, smem)) return r;
-  const int grid = p.T < 2 * b200::sm_count() ? p.T : 2 * b200::sm_count();
-  b200::launch(k, grid, NT + 32, smem, s, p);
+  const int most = (NT == 512 ? 2 : 10) * b200::sm_count();
+  b200::launch(k, p.T < most ? p.T : most, NT + 32, smem, s, p);
   b200::count_launch();
   return b200::check_launch("distill_fwd");
+}
+template <typename TL, int POWER>
+int launch_fwd(const DistillParams& p, cudaStream_t s) {
+  return short_rows<TL>(p) ? launch_fwd<TL, POWER, 64>(p, s) : launch_fwd<TL, POWER, 512>(p, s);
 }
 template <typename TL, int POWER>
 int launch_bwd(const DistillParams& p, cudaStream_t s) {
   // few rows: several CTAs a row, of 4096 columns or more
   int parts = 1;
   while (parts < 32 && (long long)p.T * parts < 2 * b200::sm_count() && p.V / (2 * parts) >= 4096) parts *= 2;
-  b200::launch(distill_bwd_kernel<TL, POWER>, dim3((unsigned)p.T, (unsigned)parts), NT, 0, s, p);
+  const dim3 grid((unsigned)p.T, (unsigned)parts);
+  if (short_rows<TL>(p)) b200::launch(distill_bwd_kernel<TL, POWER, 128>, grid, 128, 0, s, p);
+  else b200::launch(distill_bwd_kernel<TL, POWER, 512>, grid, 512, 0, s, p);
   b200::count_launch();
   return b200::check_launch("distill_bwd");
 }

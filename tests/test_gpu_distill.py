@@ -31,14 +31,14 @@ def relative(V):
     return 2 ** -22 + (100 + V / 512 + 16) * 2 ** -24
 
 
-def check(z, labels, ids, val, gy, cfg, dev="cuda"):
+def check(z, labels, ids, val, gy, cfg, dev="cuda", threads=512):
     a, tau = cfg.get("alpha", 1.0), cfg.get("temperature", 1.0)
     want, grad, size = exact(z, labels, ids, val, gy, cfg)
     x = z.to(dev).requires_grad_(True)
     args = [None if labels is None else labels.to(dev), ids.to(dev), val.to(dev)]
     loss = F.distill_loss(x, *args, **cfg)
     (dx,) = torch.autograd.grad(loss, x, gy.to(dev))
-    d = relative(z.shape[1])
+    d = relative(z.shape[1] * 512 / threads)
     # (the teacher's weights sum to 1: an error of the log-sum-exp enters once for it and once for the label)
     assert ((loss.cpu().double() - want).abs() <= (a * tau * tau * 2 + (1 - a)) * d + 2 ** -23 * want.abs()).all()
     half = torch.finfo(z.dtype).eps / 2
@@ -60,6 +60,16 @@ def test_distill(T, V, Kt, dtype, cfg):
     if cfg.get("rest") and Kt > V // 2:
         val = val - 0.7                                   # (something is left for the rest)
     check(z, labels, ids, val, gy, cfg)
+
+
+@pytest.mark.parametrize("cfg", CONFIGS, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T,V,Kt", [(3100, 7, 3), (1600, 64, 8), (1000, 929, 6), (600, 4099, 128), (310, 1201, 1024), (300, 25600, 40)])
+def test_many_short_rows(T, V, Kt, dtype, cfg):
+    z, labels, ids, val, gy = inputs(T, V, Kt, cfg.get("rest", False), dtype)
+    if cfg.get("rest") and Kt > V // 2:
+        val = val - 0.7
+    check(z, labels, ids, val, gy, cfg, threads=64)            # (a thread of the forward pass sums V / 64 elements)
 
 
 @pytest.mark.parametrize("cfg", [CONFIGS[2], CONFIGS[5]], ids=str)
