@@ -4,6 +4,7 @@
 //   s = scale q k     s = cap tanh(s / cap)     s -= slope_h |p - j|     O = softmax over the visible j of s, times V
 //
 //   * the key tiles of an item, and which of them hold anything to mask, from the mask's tables; items of all sequences longest first;
+//   * few pairs of query tiles over many keys: their key tiles in parts, joined by a second launch;
 //   * rows that see nothing: output 0, log-sum-exp -inf, whatever their inputs; a value row that no query sees is cleared in shared memory before
 //     the product (its probability is 0, but 0 times NaN is not);
 //   * the sum of a row is taken over the rounded probabilities that the second product multiplies.  The output is then a mean with weights
@@ -37,36 +38,52 @@ struct FwdParams {
   __nv_bfloat16* low; // the same: what `out` has lost to bf16; or null
   int* status;
   int items;
+  int parts, per;     // SPLIT: items for a pair's key tiles, each of them for `per` tiles or more (a pair of no more than that has one)
+  float* part;        // SPLIT: [rows][parts][HD], rows = (b * Sq + q) * Hq + h: sums of values on the part's maximum
+  float4* part_ml;    // SPLIT: [rows][parts]: maximum (log2), sum of the rounded probabilities and of those before
 };
 
-// Work item u of the launch (items go by the mask's order, over the heads of one pair of query tiles after the other), and the key
-// tiles its two query tiles look at.
+// Work item u of the launch (items go by the mask's order, over the heads of one pair of query tiles after the other, SPLIT: and over the parts of its
+// key tiles), and the key tiles its two query tiles look at.
 struct Item {
   int b, h, q0, j_lo;
   int lo0, lo1, hi0, hi1;   // per query tile: key tiles j_lo + [lo, hi); every tile of [0, n_max) is in one of them
   int n_max;
   bool unseen;              // some keys are seen by no query
   int mlo0, mlo1, mhi0, mhi1;   // per query tile: keys in [mlo, mhi) are visible to all of its rows
+  int part, parts;
   B200_DEVICE int lo(int t) const { return t ? lo1 : lo0; }
   B200_DEVICE int hi(int t) const { return t ? hi1 : hi0; }
 };
 // What the mask's tables say about item u.  The roles load it an item ahead: two loads in a row, more than a key tile's time.
+// Parts of the key tiles [x, y) that either tile of a pair looks at.
+struct Union { int x, y; };
+B200_DEVICE Union union_of(int4 a, int4 c) {
+  a.y &= ~b200::UNSEEN;
+  c.y &= ~b200::UNSEEN;
+  const int x = a.y > a.x ? (c.y > c.x ? min(a.x, c.x) : a.x) : c.x;
+  return {x, max(max(a.y, c.y), x)};
+}
+B200_DEVICE int parts_of(Union u, const FwdParams& p) { return min(max((u.y - u.x + p.per - 1) / p.per, 1), p.parts); }
 struct Entry {
   int id = 0;
   int4 a = {0, 0, 0, 0}, c = {0, 0, 0, 0};
 };
+template <bool SPLIT>
 B200_DEVICE Entry load_entry(int u, const FwdParams& p) {
   Entry e;
   if (u >= p.items) return e;
-  e.id = p.mask.oq[u / p.Hq];                            // b * pairs + pair: its query tiles are entries 2 id and 2 id + 1
+  e.id = p.mask.oq[SPLIT ? u / (p.Hq * p.parts) : u / p.Hq];                            // b * pairs + pair: its query tiles are entries 2 id and 2 id + 1
   e.a = p.mask.qt[2ll * e.id];
   e.c = p.mask.qt[2ll * e.id + 1];
   return e;
 }
+template <bool SPLIT>
 B200_DEVICE Item make_item(int u, const Entry& e, const FwdParams& p) {
   Item it;
   const int np = p.mask.Sp / 256;
-  it.h = u % p.Hq;
+  it.part = SPLIT ? u % p.parts : 0;
+  it.h = (SPLIT ? u / p.parts : u) % p.Hq;
   it.b = e.id / np;
   const int pair = e.id - it.b * np;
   it.q0 = pair * 2 * BQ;
@@ -74,6 +91,14 @@ B200_DEVICE Item make_item(int u, const Entry& e, const FwdParams& p) {
   it.unseen = (a.y & b200::UNSEEN) != 0;
   a.y &= ~b200::UNSEEN;
   c.y &= ~b200::UNSEEN;
+  it.parts = 1;
+  if (SPLIT) {                                           // this part of the key tiles (none: behind the last)
+    const Union w = union_of(a, c);
+    it.parts = parts_of(w, p);
+    const int n = w.y - w.x, z = min(it.part, it.parts), j0 = w.x + n * z / it.parts, j1 = w.x + n * min(z + 1, it.parts) / it.parts;
+    a.x = max(a.x, j0); a.y = min(a.y, j1);
+    c.x = max(c.x, j0); c.y = min(c.y, j1);
+  }
   const bool has0 = a.y > a.x, has1 = c.y > c.x;
   it.j_lo = has0 ? a.x : c.x;
   it.lo0 = 0;
@@ -104,8 +129,9 @@ struct Smem {
   static constexpr int TOTAL = 2 * Q_TILE + 4 * KV_BYTES + 8 * STAGE_O + 1024 + 256;
 };
 
-// LOW: what the output loses to bf16 is written too, and row sums go over the rounded probabilities (a backward pass follows).
-template <int HD, int SCORE, bool LOW>
+// LOW: what the output loses to bf16 is written too, and row sums go over the rounded probabilities (a backward pass follows).  SPLIT (with
+// LOW's sums): items are parts of pairs, and leave their sums for attn_masked_parts_kernel.
+template <int HD, int SCORE, bool LOW, bool SPLIT>
 __global__ void __launch_bounds__(NTHREADS, 1)
 attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -162,12 +188,12 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
       bool ok = true;
       int kv = 0, nq = 0;                    // key tiles and items so far: stage and phase of the barriers
-      Entry next = load_entry(item_of_round(0), p);
+      Entry next = load_entry<SPLIT>(item_of_round(0), p);
       for (int r = 0; r < rounds && ok; ++r) {
         const int u = item_of_round(r);
         if (u >= p.items) continue;
-        const Item it = make_item(u, next, p);
-        next = load_entry(item_of_round(r + 1), p);
+        const Item it = make_item<SPLIT>(u, next, p);
+        next = load_entry<SPLIT>(item_of_round(r + 1), p);
         if (it.n_max == 0) continue;
         const int hk = it.h / (p.Hq / p.Hkv);
         if (!mbar_wait(q_empty, (nq & 1) ^ 1, abort_flag, p.status, 39)) { ok = false; break; }
@@ -204,12 +230,12 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       bool ok = true;
       int kv = 0, nq = 0;
       int np[2] = {0, 0}, no[2] = {0, 0};    // P tiles consumed / items finished per query tile
-      Entry next = load_entry(item_of_round(0), p);
+      Entry next = load_entry<SPLIT>(item_of_round(0), p);
       for (int r = 0; r < rounds && ok; ++r) {
         const int u = item_of_round(r);
         if (u >= p.items) continue;
-        const Item it = make_item(u, next, p);
-        next = load_entry(item_of_round(r + 1), p);
+        const Item it = make_item<SPLIT>(u, next, p);
+        next = load_entry<SPLIT>(item_of_round(r + 1), p);
         if (it.n_max == 0) continue;
         if (!warp_wait_spin(q_full, nq & 1, abort_flag, p.status, 50)) { ok = false; break; }
         ++nq;
@@ -305,29 +331,32 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     int ns = 0, no = 0;                    // S tiles and items so far
     int kv = 0;                            // key tiles before this item: stages and phases of V
     bool ok = true;
-    Entry next = load_entry(item_of_round(0), p);
+    Entry next = load_entry<SPLIT>(item_of_round(0), p);
     // (row r of the pair's tile t: pairs are 256 rows of the padded queries in order)
     auto load_row = [&](const Entry& e) { return p.mask.q_iv[256ll * e.id + t * BQ + r]; };
     int2 row_next = load_row(next);
     for (int round = 0; round < rounds && ok; ++round) {
       const int u = item_of_round(round);
       if (u >= p.items) continue;
-      const Item it = make_item(u, next, p);
+      const Item it = make_item<SPLIT>(u, next, p);
       const int qt0 = it.q0 + t * BQ;
       const int q_pos = qt0 + r;
       const int kv_item = kv;
       kv += it.n_max;
       if (it.hi(t) <= it.lo(t)) {            // no row of the tile sees anything
-        if (q_pos < p.Sq) {
+        if (SPLIT && (it.parts > 1 || it.part > 0)) {
+          if (it.part < it.parts && q_pos < p.Sq)
+            p.part_ml[(((long long)it.b * p.Sq + q_pos) * p.Hq + it.h) * p.parts + it.part] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        } else if (q_pos < p.Sq) {
           const long long at = (((long long)it.b * p.Sq + q_pos) * p.Hq + it.h) * HD;
 #pragma unroll
           for (int i = 0; i < HD / 8; ++i) {
             *reinterpret_cast<uint4*>(p.out + at + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
-            if (LOW) *reinterpret_cast<uint4*>(p.low + at + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
+            if (LOW && (!SPLIT || p.low != nullptr)) *reinterpret_cast<uint4*>(p.low + at + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
           }
           p.lse[((long long)it.b * p.Hq + it.h) * p.Sq + q_pos] = p.sink != nullptr ? p.sink[it.h] : -INFINITY;
         }
-        next = load_entry(item_of_round(round + 1), p);
+        next = load_entry<SPLIT>(item_of_round(round + 1), p);
         row_next = load_row(next);
         continue;
       }
@@ -491,11 +520,31 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         lx += x2.x + x2.y;
       }
       // ------------------------------ epilogue ------------------------------
-      next = load_entry(item_of_round(round + 1), p);          // (not before: the scores take the registers)
+      next = load_entry<SPLIT>(item_of_round(round + 1), p);          // (not before: the scores take the registers)
       if (!ok || !warp_wait(&o_done[t], no & 1, abort_flag, p.status, 62)) { ok = false; break; }
       ++no;
       tc_fence_after();
       row_next = load_row(next);
+      if (SPLIT && it.parts > 1) {
+        const long long at = (((long long)it.b * p.Sq + q_pos) * p.Hq + it.h) * p.parts + it.part;
+        if (q_pos < p.Sq) p.part_ml[at] = make_float4(m_ref, l, lx, 0.f);
+#pragma unroll 1
+        for (int i = 0; i < HD / 32; ++i) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(to + i * 32, v);
+          tc_wait_ld();
+          if (i == HD / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[t]);
+          }
+          if (q_pos < p.Sq)
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+              *reinterpret_cast<uint4*>(p.part + at * HD + i * 32 + g * 4) = make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        }
+        continue;
+      }
       const bool none = m_ref == -INFINITY;                   // a row that sees nothing
       if (p.sink != nullptr) {
         const float sk = p.sink[it.h] * 1.4426950408889634f;
@@ -520,7 +569,7 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 #pragma unroll
         for (int c = 0; c < 64; ++c) v[c] = none ? 0u : __float_as_uint(__uint_as_float(v[c]) * inv);
 #pragma unroll 1
-        for (int part = 0; part < (LOW ? 2 : 1); ++part) {
+        for (int part = 0; part < (LOW && (!SPLIT || p.low != nullptr) ? 2 : 1); ++part) {
           if (lane == 0) tma_store_wait_read<0>();     // the block before has left the staging buffer
           __syncwarp();
 #pragma unroll
@@ -557,14 +606,64 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   if (warp == 9) { tc_fence_after(); tmem_dealloc(tmem_base, 512); }
 }
 
-template <int HD, int SCORE, bool LOW>
+// Joins the parts of 8 rows of a pair of query tiles and a head, a warp a row; LOW as above.
+template <int HD, bool LOW>
+__global__ void __launch_bounds__(256) attn_masked_parts_kernel(const __grid_constant__ FwdParams p) {
+  b200::begin_kernel();
+  const int lane = threadIdx.x & 31, h = (int)blockIdx.x % p.Hq, id = (int)blockIdx.x / p.Hq, np = p.mask.Sp / 256, b = id / np;
+  const int parts = parts_of(union_of(p.mask.qt[2ll * id], p.mask.qt[2ll * id + 1]), p);
+  if (parts == 1) return;                                // written by the item itself
+  const int q = (id - b * np) * 256 + (int)blockIdx.y * 8 + (int)(threadIdx.x >> 5);
+  if (q >= p.Sq) return;
+  const long long at = ((long long)b * p.Sq + q) * p.Hq + h;
+  const float4 ml = lane < parts ? p.part_ml[at * p.parts + lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  float m = warp_max(ml.x);
+  const bool none = m == -INFINITY;
+  const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - m);
+  // (a part that the row sees nothing of may hold what an infinity made of its sums)
+  float l = warp_sum(f == 0.f ? 0.f : ml.y * f), lx = warp_sum(f == 0.f ? 0.f : ml.z * f), acc[HD / 32] = {};
+  for (int z = 0; z < parts; ++z) {
+    const float w = __shfl_sync(0xffffffffu, f, z);
+    if (w == 0.f) continue;
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) acc[c] += w * p.part[(at * p.parts + z) * HD + c * 32 + lane];
+  }
+  if (p.sink != nullptr) {
+    const float sk = p.sink[h] * b200::LOG2E;
+    if (none) { m = sk; l = lx = 1.f; }
+    else { l += ex2_approx(sk - m); lx += ex2_approx(sk - m); }
+  }
+  const float inv = none ? 0.f : 1.f / l;
+#pragma unroll
+  for (int c = 0; c < HD / 32; ++c) {
+    const float x = none ? 0.f : acc[c] * inv;
+    const __nv_bfloat16 o = __float2bfloat16(x);
+    p.out[at * HD + c * 32 + lane] = o;
+    if (LOW) p.low[at * HD + c * 32 + lane] = __float2bfloat16(x - __bfloat162float(o));
+  }
+  if (lane == 0) p.lse[((long long)b * p.Hq + h) * p.Sq + q] = l > 0.f ? (m + log2f(lx)) * 0.6931471805599453f : -INFINITY;
+}
+
+// Items for a pair's key tiles: two to an SM in all at most, of four key tiles or more each, where what the longest pair could save (2.4 us a tile)
+// is more than a join costs (10 us, and 3.5 TB/s for what the parts leave and it reads).  us without and with:
+// 2 x 6437 tokens of a head of 128 155 and 75, 8192 of one 132 and 47, of four 133 and 106, 300 after 16084 of 32 heads 261 and 150; 8192 of four in sixteen
+// documents 45 and 48, with a window of 512 21 and 30 (their few key tiles stay whole: what is left is the launch).
+int fwd_parts(int B, int Sq, int Skv, int Hq, int HD) {
+  const long long items = (long long)B * ((Sq + 255) / 256) * Hq, tiles = (Skv + BKV - 1) / BKV, n = 2ll * b200::sm_count() / items;
+  const long long most = tiles / 4 < 8 ? tiles / 4 : 8, parts = n < most ? n : most;
+  if (parts < 2) return 1;
+  const float saved = 2.4f * tiles * (1.f - 1.f / parts), cost = 10.f + 5.7e-7f * (float)((long long)B * Sq * Hq) * parts * (HD * 4 + 16);
+  return saved > cost ? (int)parts : 1;
+}
+
+template <int HD, int SCORE, bool LOW, bool SPLIT>
 int launch_fwd(const CUtensorMap* m, const FwdParams& p, cudaStream_t stream) {
   using SM = Smem<HD>;
   static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_masked_fwd_kernel<HD, SCORE, LOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
+    cudaError_t e = cudaFuncSetAttribute(attn_masked_fwd_kernel<HD, SCORE, LOW, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
     if (e != cudaSuccess) {
       cudaGetLastError();  // clear the sticky error before reporting
       return b200::fail(951, "attn_masked_fwd: cannot set %d bytes of shared memory: %s", SM::TOTAL, cudaGetErrorString(e));
@@ -572,13 +671,17 @@ int launch_fwd(const CUtensorMap* m, const FwdParams& p, cudaStream_t stream) {
     configured[dev & 63] = true;
   }
   const int grid = p.items < b200::sm_count() ? p.items : b200::sm_count();
-  b200::launch(attn_masked_fwd_kernel<HD, SCORE, LOW>, grid, NTHREADS, SM::TOTAL, stream, m[0], m[1], m[2], m[3], m[4], p);
+  b200::launch(attn_masked_fwd_kernel<HD, SCORE, LOW, SPLIT>, grid, NTHREADS, SM::TOTAL, stream, m[0], m[1], m[2], m[3], m[4], p);
   b200::count_launch();
   return b200::check_launch("attn_masked_fwd");
 }
 template <int HD, int SCORE>
 int launch_fwd(const CUtensorMap* m, const FwdParams& p, cudaStream_t s) {
-  return p.low != nullptr ? launch_fwd<HD, SCORE, true>(m, p, s) : launch_fwd<HD, SCORE, false>(m, p, s);
+  if (p.parts == 1) return p.low != nullptr ? launch_fwd<HD, SCORE, true, false>(m, p, s) : launch_fwd<HD, SCORE, false, false>(m, p, s);
+  if (int r = launch_fwd<HD, SCORE, true, true>(m, p, s)) return r;
+  b200::launch(p.low != nullptr ? attn_masked_parts_kernel<HD, true> : attn_masked_parts_kernel<HD, false>, dim3((unsigned)(p.items / p.parts), 32), 256, 0, s, p);
+  b200::count_launch();
+  return b200::check_launch("attn_masked_parts");
 }
 template <int HD>
 int launch_fwd(int score, const CUtensorMap* m, const FwdParams& p, cudaStream_t s) {
@@ -592,12 +695,18 @@ int launch_fwd(int score, const CUtensorMap* m, const FwdParams& p, cudaStream_t
 
 }  // namespace
 
+// bytes of the sums that parts of the key tiles leave (0: the key tiles are not parted)
+B200_API long long b200_attn_masked_fwd_workspace(int B, int Sq, int Skv, int Hq, int HD) {
+  const int parts = fwd_parts(B, Sq, Skv, Hq, HD);
+  return parts > 1 ? (long long)B * Sq * Hq * parts * (HD * 4 + 16) : 0;
+}
+
 // q: [B, Sq, Hq, HD], k/v: [B, Skv, Hkv, HD] bf16, each with its own row and batch pitch (elements), heads contiguous inside a token row;
 // out [B, Sq, Hq, HD] contiguous, `low` like it or null; mask: b200_attn_mask's buffer for (B, Sq, Skv).
 B200_API int b200_attn_masked_fwd(const void* q, const void* k, const void* v, void* out, void* low, float* lse, const float* sink,
                                   const float* slopes, const int* mask, int B, int Sq, int Skv, int Hq, int Hkv, int HD, long long q_row,
                                   long long k_row, long long v_row, long long q_batch, long long k_batch, long long v_batch, float scale,
-                                  float cap, void* stream) {
+                                  float cap, void* workspace, long long workspace_bytes, void* stream) {
   if (HD != 64 && HD != 128) return b200::fail(950, "attn_masked_fwd: head dim %d not supported (64 or 128)", HD);
   if (B < 1 || Sq < 1 || Skv < Sq || Hkv < 1 || Hq % Hkv != 0)
     return b200::fail(950, "attn_masked_fwd: B=%d, Sq=%d, Skv=%d, Hq=%d, Hkv=%d", B, Sq, Skv, Hq, Hkv);
@@ -619,7 +728,14 @@ B200_API int b200_attn_masked_fwd(const void* q, const void* k, const void* v, v
   p.sink = sink; p.lse = lse;
   p.out = (__nv_bfloat16*)out; p.low = (__nv_bfloat16*)low;
   p.status = b200::status_ptr();
-  const long long items = (long long)B * (lay.Sp / 256) * Hq;
+  p.parts = fwd_parts(B, Sq, Skv, Hq, HD);
+  p.per = ((Skv + BKV - 1) / BKV + 2 * p.parts - 1) / (2 * p.parts);
+  if (p.per < 4) p.per = 4;
+  if (p.parts > 1 && (workspace == nullptr || (uintptr_t)workspace % 16 != 0 || workspace_bytes < b200_attn_masked_fwd_workspace(B, Sq, Skv, Hq, HD)))
+    return b200::fail(952, "attn_masked_fwd: a workspace of %lld bytes", workspace_bytes);
+  p.part_ml = (float4*)workspace;
+  p.part = (float*)(p.part_ml + (long long)B * Sq * Hq * p.parts);
+  const long long items = (long long)B * (lay.Sp / 256) * Hq * p.parts;
   if (items > 0x3fffffff) return b200::fail(950, "attn_masked_fwd: %lld query tile pairs", items);
   p.items = (int)items;
   const int score = (cap > 0.f ? b200::SCORE_CAP : 0) | (slopes != nullptr ? b200::SCORE_BIAS : 0);

@@ -135,7 +135,7 @@ using DistillFn = int (*)(const void*, int, long long, const long long*, const v
 using DistillBwdFn = int (*)(const void*, int, long long, const long long*, const void*, int, const void*, int, int, int, int, int, float, float,
                              long long, const float*, const double*, const float*, void*, long long, void*);
 using MaskedFn = int (*)(const void*, const void*, const void*, void*, void*, float*, const float*, const float*, const int*, int, int, int, int, int, int,
-                         long long, long long, long long, long long, long long, long long, float, float, void*);
+                         long long, long long, long long, long long, long long, long long, float, float, void*, long long, void*);
 using MaskedRowsFn = int (*)(const void*, const void*, const void*, void*, float*, const float*, const float*, const int*, int, int, int, int, int, int,
                              long long, long long, long long, long long, long long, long long, float, float, void*, long long, void*);
 using MaskedBwdFn = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, const float*, float*, float*, void*, void*,
@@ -151,6 +151,7 @@ MaskedBwdFn g_masked_bwd = nullptr;
 int (*g_few_rows)(int, int, int, int) = nullptr;
 long long (*g_rows_ws)(int, int, int, int, int, int) = nullptr;
 long long (*g_masked_bwd_ws)(int, int, int, int, int, int) = nullptr;
+long long (*g_masked_fwd_ws)(int, int, int, int, int) = nullptr;
 long long (*g_mask_ints)(int, int, int) = nullptr;
 int (*g_mask)(const void*, int, const uint8_t*, int, int, int, int, int, int*, void*) = nullptr;
 
@@ -820,7 +821,7 @@ PyObject* py_masked_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
   at::Tensor sl;
   long long mb, mq, mk;
   double softcap, scale;
-  if (nargs != 10 || g_masked == nullptr || g_masked_rows == nullptr || g_masked_bwd == nullptr || g_few_rows == nullptr ||
+  if (nargs != 10 || g_masked == nullptr || g_masked_fwd_ws == nullptr || g_masked_rows == nullptr || g_masked_bwd == nullptr || g_few_rows == nullptr ||
       (q = tensor_of(args[0])) == nullptr || (k = tensor_of(args[1])) == nullptr || (v = tensor_of(args[2])) == nullptr ||
       (m = tensor_of(args[3])) == nullptr || !int_of(args[4], mb) || !int_of(args[5], mq) || !int_of(args[6], mk) || !optional_tensor(args[7], sl) ||
       !float_of(args[8], softcap) || !float_of(args[9], scale)) {
@@ -854,10 +855,12 @@ PyObject* py_masked_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
                              (float)softcap, n > 0 ? ws.data_ptr() : nullptr, n, stream_of(*q)));
     } else {
       if (grad) low = at::empty({B, Sq, Hq, D}, o);
+      const long long n = g_masked_fwd_ws((int)B, (int)Sq, (int)Skv, (int)Hq, (int)D);
+      at::Tensor ws = workspace(n, *q);
       check_rc("b200_attn_masked_fwd",
                g_masked(q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(), grad ? low.data_ptr() : nullptr, lse.data_ptr<float>(), nullptr,
                         floats_of(sl), m->data_ptr<int>(), (int)B, (int)Sq, (int)Skv, (int)Hq, (int)Hkv, (int)D, pq.row, pk.row, pv.row, pq.batch, pk.batch,
-                        pv.batch, (float)scale, (float)softcap, stream_of(*q)));
+                        pv.batch, (float)scale, (float)softcap, n > 0 ? ws.data_ptr() : nullptr, n, stream_of(*q)));
     }
     if (grad) {
       auto node = std::shared_ptr<MaskedAttentionBackward>(new MaskedAttentionBackward(), ag::deleteNode);
@@ -909,10 +912,11 @@ PyObject* py_attention_mask(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
   END_HANDLE_TH_ERRORS
 }
 
-// bind_masked(addresses of b200_attn_masked_few_rows, _rows_workspace, _bwd_workspace, b200_attn_mask_ints)
+// bind_masked(addresses of b200_attn_masked_few_rows, _rows_workspace, _bwd_workspace, b200_attn_mask_ints, b200_attn_masked_fwd_workspace)
 PyObject* py_bind_masked(PyObject*, PyObject* args) {
-  unsigned long long a, b, c, d;
-  if (!PyArg_ParseTuple(args, "KKKK", &a, &b, &c, &d)) return nullptr;
+  unsigned long long a, b, c, d, e;
+  if (!PyArg_ParseTuple(args, "KKKKK", &a, &b, &c, &d, &e)) return nullptr;
+  g_masked_fwd_ws = reinterpret_cast<long long (*)(int, int, int, int, int)>(e);
   g_mask_ints = reinterpret_cast<long long (*)(int, int, int)>(d);
   g_few_rows = reinterpret_cast<int (*)(int, int, int, int)>(a);
   g_rows_ws = reinterpret_cast<long long (*)(int, int, int, int, int, int)>(b);

@@ -156,7 +156,7 @@ def _declare(lib: ctypes.CDLL) -> None:
         "b200_attn_bwd": [P] * 9 + [I] * 6 + [L] * 12 + [F, I, I, I, P, L, P],
         "b200_attn_bwd_plan": [I] * 8 + [P],
         "b200_attn_mask": [P, I, P, I, I, I, I, I, P, P],
-        "b200_attn_masked_fwd": [P] * 9 + [I] * 6 + [L] * 6 + [F, F, P],
+        "b200_attn_masked_fwd": [P] * 9 + [I] * 6 + [L] * 6 + [F, F, P, L, P],
         "b200_attn_masked_rows": [P] * 8 + [I] * 6 + [L] * 6 + [F, F, P, L, P],
         "b200_attn_masked_bwd": [P] * 13 + [I] * 6 + [L] * 10 + [F, F, P, L, P],
     }
@@ -177,7 +177,7 @@ def _declare(lib: ctypes.CDLL) -> None:
             host.bind_mx(ctypes.cast(lib.b200_gemm_mxfp4_workspace, c_void_p).value)
         if hasattr(lib, "b200_attn_masked_few_rows"):
             host.bind_masked(*(ctypes.cast(getattr(lib, "b200_attn_mask" + n), c_void_p).value
-                               for n in ("ed_few_rows", "ed_rows_workspace", "ed_bwd_workspace", "_ints")))
+                               for n in ("ed_few_rows", "ed_rows_workspace", "ed_bwd_workspace", "_ints", "ed_fwd_workspace")))
     lib.b200_norm_bwd_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.argtypes = [I, I]
     lib.b200_hstu_gate_cat_scratch_elems.restype = c_ll
@@ -190,6 +190,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         lib.b200_attn_masked_few_rows.restype = c_int
         lib.b200_attn_masked_rows_workspace.argtypes = [I, I, I, I, I, I]
         lib.b200_attn_masked_rows_workspace.restype = c_ll
+        lib.b200_attn_masked_fwd_workspace.argtypes = [I, I, I, I, I]
+        lib.b200_attn_masked_fwd_workspace.restype = c_ll
         lib.b200_attn_masked_bwd_workspace.argtypes = [I, I, I, I, I, I]
         lib.b200_attn_masked_bwd_workspace.restype = c_ll
     if hasattr(lib, "b200_sort_scratch_bytes"):

@@ -196,8 +196,10 @@ def masked_attention_fwd(q, k, v, mask: AttentionMask, *, scale: float | None = 
             call("b200_attn_masked_rows", ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(sink), ptr(slopes), ptr(mask.buf), B, Sq, Skv, Hq, Hkv,
                  D, q_row, k_row, v_row, q_batch, k_batch, v_batch, float(scale), float(softcap), ptr(ws), n, stream_ptr())
             return out, lse, None
+        n = int(lib.b200_attn_masked_fwd_workspace(B, Sq, Skv, Hq, D))
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         call("b200_attn_masked_fwd", ptr(q), ptr(k), ptr(v), ptr(out), ptr(low), ptr(lse), ptr(sink), ptr(slopes), ptr(mask.buf), B, Sq, Skv, Hq,
-             Hkv, D, q_row, k_row, v_row, q_batch, k_batch, v_batch, float(scale), float(softcap), stream_ptr())
+             Hkv, D, q_row, k_row, v_row, q_batch, k_batch, v_batch, float(scale), float(softcap), ptr(ws), n, stream_ptr())
     return out, lse, low
 
 
