@@ -99,8 +99,7 @@ def close(got, want, rel, what):
 
 # Output: P rounded to bf16 (2^-9 rms at most a key, averaged over keys), O rounded once (2^-9 / sqrt 3 rms): below 2^-8 together.  dV: P and
 # dO as P's rounding, then dV's: the same.  dQ, dK: P's exponent (lse 2^-9 / sqrt 3), dS rounded (the same) and the result's rounding, where
-# dS is a difference whose terms are kept to 2^-17: below 2^-7 even for rows of few keys.  The cap's polynomial (7e-6 of a score) and a quarter of the
-# forward's exponentials (7e-4) are inside.
+# dS is a difference whose terms are kept to 2^-17: below 2^-7 even for rows of few keys.  The cap's polynomial (7e-6 of a score) is inside.
 OUT, GRAD = 2 ** -8, 2 ** -7
 
 
@@ -194,6 +193,31 @@ def test_head_layouts(Hq, Hkv):
 @pytest.mark.parametrize("score", SCORES[:4], ids=str)
 def test_long_rows(score):
     check(1, 3001, 3001, 4, 2, 128, "few", MASKS[0], score)
+
+
+@pytest.mark.parametrize("score", SCORES, ids=str)
+@pytest.mark.parametrize("kind,m", [("one", MASKS[0]), ("few", MASKS[1]), ("holes", MASKS[4]), ("left", dict(window=700)), ("few", dict(causal=False))], ids=str)
+@pytest.mark.parametrize("Sq,Skv,Hq,Hkv,D", [(2311, 2311, 2, 1, 64), (300, 5003, 4, 2, 128)])
+def test_few_tiles_over_many_keys(Sq, Skv, Hq, Hkv, D, kind, m, score):
+    """Key tiles of a pair of query tiles in parts (forward) and steps of a key tile shared (backward), beside pairs and tiles that stay whole."""
+    assert _lib.load().b200_attn_masked_fwd_workspace(1, Sq, Skv, Hq, D) > 0
+    check(1, Sq, Skv, Hq, Hkv, D, kind, m, score)
+
+
+def test_padding_may_hold_anything_beside_parts():
+    B, S = 1, 3000
+    ids = documents(B, S, "padded")
+    q, k, v, do, s = tensors(B, S, S, 2, 2, 64, {}, torch.bfloat16)
+    ok = F.attention_mask(B, S, documents=ids).visible()
+    want = oracle(q, k, v, do, ok, s)[0]
+    pad = ~ok.any(1)
+    assert pad.any()
+    q[pad], k[pad], v[pad] = float("inf"), float("nan"), float("nan")
+    with torch.no_grad():
+        y = F.masked_attention(q.cuda(), k.cuda(), v.cuda(), F.attention_mask(B, S, documents=ids.cuda()))
+    close(y, want, OUT, "out")
+    assert (y.cpu()[~ok.any(-1)] == 0).all()
+    _lib.check_status("parts")
 
 
 @pytest.mark.parametrize("cap", [0.25, 1.0, 30.0])
