@@ -289,10 +289,11 @@ __global__ void __launch_bounds__(NT + 32, NT == 512 ? 2 : 10) distill_fwd_kerne
         const float m = mx * cu;
         if (!(m <= acc.m)) {
           if (acc.m > -INFINITY) {
-            const float f = ex2_approx(acc.m - m);
+            // (sums that are too large become infinite, and stay so)
+            const float d = s2.x + s2.y + (BOTH ? z2.x + z2.y : 0.f) < 0x1p60f ? acc.m - m : INFINITY, f = ex2_approx(d);
             s2 = fmul2(s2, make_float2(f, f));
             if (BOTH) {
-              const float g = ex2_approx((acc.m - m) * p.tau);
+              const float g = ex2_approx(d * p.tau);
               z2 = fmul2(z2, make_float2(g, g));
             }
           }
@@ -323,7 +324,10 @@ __global__ void __launch_bounds__(NT + 32, NT == 512 ? 2 : 10) distill_fwd_kerne
         if ((int)threadIdx.x < edge) take1((int)threadIdx.x < head ? sp.lo + (int)threadIdx.x : sp.first + sp.n * N + (int)threadIdx.x - head);
       };
       // The sums go over the largest of the thread's first elements, without a look at the others: 36 instead of 83 instructions for 8
-      // elements.  Where that was no measure (an element 2^127 above it, none at all), the thread goes over its part once more.
+      // elements.  Where that was no measure, the thread goes over its part once more, on its largest element.  It was one where both sums
+      // lie within 2^-60 .. 2^60, here and whenever the maximum was raised: then the 512 of a row do not overflow together, what a factor of
+      // a larger maximum flushes to 0 (below 2^-126) is less than 2^-66 of what has that maximum, and so is what the exponential has
+      // flushed here (an id, which REST leaves out, may lie far above all others).
       if ((int)threadIdx.x < sp.n) acc.m = fmax_nan(largest(raw[0]) * cu, -1e30f);
       for (int v0 = threadIdx.x; v0 < sp.n; v0 += NT * AHEAD) {
 #pragma unroll
@@ -350,7 +354,8 @@ __global__ void __launch_bounds__(NT + 32, NT == 512 ? 2 : 10) distill_fwd_kerne
       take_edge();
       acc.s = s2.x + s2.y;
       acc.z = z2.x + z2.y;
-      if (!(acc.s > 0.f && acc.s < INFINITY) || (BOTH && !(acc.z > 0.f && acc.z < INFINITY))) {
+      auto measured = [](float v) { return v > 0x1p-60f && v < 0x1p60f; };
+      if (!measured(acc.s) || (BOTH && !measured(acc.z))) {
         acc.m = -INFINITY;
         s2 = z2 = make_float2(0.f, 0.f);
         for (int v = threadIdx.x; v < sp.n; v += NT)
