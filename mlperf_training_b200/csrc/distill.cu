@@ -6,6 +6,7 @@
 //          rest:  p_j = exp(t_j); what they leave, r = 1 - sum p, is one further event "any other id": r (log r - log R),
 //                 R = the student's mass outside the ids
 //   dz   = gy (a tau (c q_v - p_v - [v not among the ids] (r / R) q_v) + (1 - a) (q1_v - [v = label])),  c = sum p + r
+// q_v / R, a softmax over the ids that are left out, is formed on their own log-sum-exp: R may be far smaller than fp32 holds.
 //
 // An entry whose id is outside the vocabulary or whose value is -inf is not there.  Tokens labelled `ignore` have loss and gradient 0; so has
 // the cross-entropy of another label outside the vocabulary.
@@ -41,8 +42,8 @@ struct DistillParams {
   float alpha, tau;
   long long ignore;
   float* loss;              // [T]
-  float* stats;             // [T, 4]: log-sum-exp of u and of z (log2 units), c, r / R
-  double* teacher;          // [T]: log-sum-exp of t / tau (plain)
+  float* stats;             // [T, 4]: log-sum-exp of u and of z (log2 units), c, log-sum-exp of u outside the ids (rest)
+  double* teacher;          // [T]: log-sum-exp of t / tau (plain), r (rest; 0 where no id is left out)
   // backward
   const float* gy;          // [T]
   void* grad;               // [T, ld_grad], may be the logits
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(NT + 32, NT == 512 ? 2 : 10) distill_fwd_kerne
       const float others = acc.log2_s();
       if (REST) acc.join(ids.m, ids.s, ids.z, p.tau);
       const float lse_u = acc.log2_s(), lse_z = BOTH ? acc.log2_z(p.tau) : lse_u;
-      double loss = 0., c = te.mass, ratio = 0.;
+      double loss = 0., c = te.mass, left = 0.;
       if (p.alpha > 0.f) {
         const double ln2 = 0.6931471805599453094, lse = (double)lse_u * ln2;
         double kl = te.own - te.cross + (te.mass != 0. ? te.mass * lse : 0.);
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(NT + 32, NT == 512 ? 2 : 10) distill_fwd_kerne
           if (r > 0. && others > -INFINITY) {          // (no id left outside: nothing for the rest to be)
             const double lr = (double)(others - lse_u) * ln2;
             kl += r * (log(r) - lr);
-            ratio = r / exp(lr);
+            left = r;
             c += r;
           }
         }
@@ -259,8 +260,8 @@ __global__ void __launch_bounds__(NT + 32, NT == 512 ? 2 : 10) distill_fwd_kerne
       st[0] = lse_u;
       st[1] = lse_z;
       st[2] = (float)c;
-      st[3] = (float)ratio;
-      p.teacher[t] = te.log_sum;
+      st[3] = others;
+      p.teacher[t] = REST ? left : te.log_sum;
     }
     return;
   }
@@ -387,10 +388,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Distil
   const long long label = p.labels != nullptr ? p.labels[t] : 0;
   const bool live = p.labels == nullptr || label != p.ignore, labelled = live && p.alpha < 1.f && label >= 0 && label < p.V;
   const float gy = live ? p.gy[t] : 0.f;
-  const float lse_u = p.stats[t * 4], lse_z = p.stats[t * 4 + 1], c = p.stats[t * 4 + 2], ratio = p.stats[t * 4 + 3];
+  const float lse_u = p.stats[t * 4], lse_z = p.stats[t * 4 + 1], c = p.stats[t * 4 + 2], others = p.stats[t * 4 + 3];
+  const float left = p.rest ? (float)p.teacher[t] : 0.f;
   const float gu = gy * p.alpha * p.tau, gz = labelled ? gy * (1.f - p.alpha) : 0.f;
   const float cu = LOG2E / p.tau;
-  const float fu = gu * (c - ratio);                   // of q, outside the ids
   // the elements that a thread each writes at the end
   float zid[SLOTS], zlabel = 0.f;
   int id[SLOTS];
@@ -412,19 +413,24 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Distil
     if (threadIdx.x == 0 && labelled && label >= lo && label < hi) zlabel = load1(row + label);
     __syncthreads();
   }
-  // (POWER above 0) q1 is the tau-th power of e^(u - lse_z / tau), which is at most 1, and q that times 2^(lse_z / tau - lse_u)
-  const float shift = POWER >= 1 ? lse_z / p.tau : lse_u;
-  const float fe = POWER >= 1 ? fu * ex2_approx(shift - lse_u) : fu;
+  // One exponential e = 2^(u - shift) of an element that is not among the ids (what it is of an id does not matter: that is written again), at
+  // most 1 on each of these: the log-sum-exp of u, or of u outside the ids (rest: q = e 2^(shift - lse_u), q / R = e), or (POWER above 0)
+  // lse_z / tau, whose e is the tau-th root of q1, unless that lies so far above all others that e would flush to 0.  (q1 is then below
+  // 2^-120 of e, and `left`, which e has beside it, 2^-53 or more: q1 is not added.  A branch for it took 7 % of the pass.)
+  const float root = POWER >= 1 ? lse_z / p.tau : 0.f;
+  const bool by_root = POWER >= 1 && !(left > 0.f && root - others > 60.f);
+  const float shift = by_root ? root : left > 0.f ? others : lse_u, gr = by_root ? gz : 0.f;
+  const float fq = ex2_approx(shift - lse_u), fe = gu * (c * fq - (left > 0.f ? left * ex2_approx(shift - others) : 0.f));
   auto other = [&](float2 x) -> float2 {
     const float2 a = ffma2(x, make_float2(cu, cu), make_float2(-shift, -shift));
     float2 e = make_float2(ex2_approx(a.x), ex2_approx(a.y));
-    if (POWER < 0) return fmul2(e, make_float2(fu + gz, fu + gz));
+    if (POWER < 0) return fmul2(e, make_float2(fe + gz * fq, fe + gz * fq));
     float2 z;
     if (POWER >= 1) {
       z = fmul2(e, e);
 #pragma unroll
       for (int i = 1; i < POWER; ++i) z = fmul2(z, z);
-      z = fmul2(z, make_float2(gz, gz));
+      z = fmul2(z, make_float2(gr, gr));
     } else {
       const float2 b = ffma2(x, make_float2(LOG2E, LOG2E), make_float2(-lse_z, -lse_z));
       z = fmul2(make_float2(ex2_approx(b.x), ex2_approx(b.y)), make_float2(gz, gz));
@@ -479,7 +485,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Distil
     if (p.alpha > 0.f)
       for (int j = 0; j < p.K; ++j)
         if (s_id[j] == v) { pv += s_p[j]; among = true; }
-    float g = gu * ((among ? c : c - ratio) * ex2_approx(fmaf(z, cu, -lse_u)) - pv);
+    float g = gu * (c * ex2_approx(fmaf(z, cu, -lse_u)) - (among || !(left > 0.f) ? pv : left * ex2_approx(fmaf(z, cu, -others))));
     if (labelled) g += gz * (ex2_approx(fmaf(z, LOG2E, -lse_z)) - ((long long)v == label ? 1.f : 0.f));
     store1(out + v, g);
   };

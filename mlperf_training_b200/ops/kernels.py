@@ -554,7 +554,12 @@ def _distill_plain_grad(gy, logits, labels, ids, values, alpha, temperature, res
                                                                                             ignore_index)
     g = torch.zeros(logits.shape, dtype=torch.float64)
     if alpha > 0:
-        g = logq.exp() * (c[:, None] - torch.where(among, 0.0, ratio[:, None]))
+        g = logq.exp() * c[:, None]
+        if rest:
+            # the student's softmax over the ids that are left out, whose mass may be less than 64 bits hold
+            others = torch.logsumexp(torch.where(among, float("-inf"), logq), -1)
+            left = (1 - p.sum(-1)) * ((ratio > 0) & (others > float("-inf")))
+            g = g - torch.where(among, 0.0, left[:, None] * (logq - torch.where(left > 0, others, 0.0)[:, None]).exp())
         g.scatter_add_(1, at, torch.where(there, -p, 0.0))
         g *= alpha * temperature
     if alpha < 1:
