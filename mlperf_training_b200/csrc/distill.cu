@@ -27,6 +27,7 @@ namespace {
 
 constexpr int MAX_K = 1024;
 constexpr int AHEAD = 4;           // 16-byte loads of a thread under way
+constexpr int MAX_SMEM = 225 * 1024;         // marks of 921600 ids, two rows of them
 constexpr int SHORT_BYTES = 100 * 1024;      // of a row, up to which it is short
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
@@ -505,11 +506,13 @@ int check_distill(const char* what, const DistillParams& p) {
 }
 
 int set_smem(const void* fn, size_t bytes) {
-  if (bytes <= 48 * 1024) return 0;
-  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (bytes <= 40 * 1024) return 0;                    // (what a launch has without asking, 48 KB, is for the kernel's own variables too)
+  if (bytes > MAX_SMEM) return b200::fail(933, "distill: marks of %zu bytes, %d at most", bytes, MAX_SMEM);
+  // (always the most of all vocabularies: a call of another thread with a smaller one may come between this and the launch)
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM);
   if (e != cudaSuccess) {
     cudaGetLastError();
-    return b200::fail(933, "distill: cannot set %zu bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+    return b200::fail(933, "distill: cannot set %d bytes of shared memory: %s", MAX_SMEM, cudaGetErrorString(e));
   }
   return 0;
 }
