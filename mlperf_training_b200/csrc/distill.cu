@@ -26,6 +26,7 @@
 namespace {
 
 constexpr int MAX_K = 1024;
+constexpr int MAX_T = 0x7fff0000;  // (a row's number and the next of its block's stay in 32 bits)
 constexpr int AHEAD = 4;           // 16-byte loads of a thread under way
 constexpr int MAX_SMEM = 225 * 1024;         // marks of 921600 ids, two rows of them
 constexpr int SHORT_BYTES = 100 * 1024;      // of a row, up to which it is short
@@ -498,7 +499,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_bwd_kernel(const Distil
 }
 
 int check_distill(const char* what, const DistillParams& p) {
-  if (p.T < 0 || p.V < 1 || p.V > (1 << 30) || p.K < 1 || p.K > MAX_K)
+  if (p.T < 0 || p.T > MAX_T || p.V < 1 || p.V > (1 << 30) || p.K < 1 || p.K > MAX_K)
     return b200::fail(930, "%s: T=%d, V=%d, K=%d (1 to %d)", what, p.T, p.V, p.K, MAX_K);
   if (!(p.tau > 0.f) || !(p.alpha >= 0.f && p.alpha <= 1.f)) return b200::fail(931, "%s: temperature %g, alpha %g", what, p.tau, p.alpha);
   if (p.alpha < 1.f && p.labels == nullptr) return b200::fail(932, "%s: the cross-entropy wants labels", what);

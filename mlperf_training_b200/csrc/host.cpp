@@ -737,7 +737,7 @@ PyObject* py_distill_loss(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   }
   if (!here(*x) || !rows_ok(*x) || !float_or_bf16(*x)) Py_RETURN_NONE;
   const int64_t T = x->size(0), V = x->size(1);
-  if (T < 1 || T > 0x7fffffff || V < 1 || V > (rest ? 900000 : 1 << 30) || !(alpha >= 0.0 && alpha <= 1.0) || !((float)tau > 0.f && (float)tau < INFINITY) ||
+  if (T < 1 || T > 0x7fff0000 || V < 1 || V > (rest ? 900000 : 1 << 30) || !(alpha >= 0.0 && alpha <= 1.0) || !((float)tau > 0.f && (float)tau < INFINITY) ||
       (!l.defined() && alpha < 1.0))
     Py_RETURN_NONE;
   if (i->device() != x->device() || v->device() != x->device() || i->dim() != 2 || i->sizes() != v->sizes() || i->size(0) != T || i->size(1) < 1 ||

@@ -494,6 +494,8 @@ def cross_entropy_(logits: torch.Tensor, labels: torch.Tensor, grad_scale: float
 # distillation from a teacher's largest logits
 # --------------------------------------------------------------------------------------
 DISTILL_MAX_K = 1024
+DISTILL_MAX_T = 0x7fff0000         # rows are counted in 32 bits, a grid's worth at a time
+DISTILL_MAX_V = 2 ** 30
 DISTILL_MAX_REST_V = 900_000       # ids are marked in shared memory, a bit each for two tokens at a time
 
 
@@ -501,6 +503,8 @@ def _distill_check(logits, labels, ids, values, alpha, temperature, rest) -> Non
     if logits.dim() != 2 or logits.dtype not in (torch.float32, BF16) or logits.shape[1] < 1:
         raise ValueError(f"distill: logits [T, V] in fp32 or bf16, not {list(logits.shape)} in {logits.dtype}")
     T, V = logits.shape
+    if T > DISTILL_MAX_T or V > DISTILL_MAX_V:
+        raise ValueError(f"distill: {T} tokens of {V} logits (at most {DISTILL_MAX_T} of {DISTILL_MAX_V})")
     if ids.dim() != 2 or ids.shape != values.shape or ids.shape[0] != T or not 1 <= ids.shape[1] <= DISTILL_MAX_K:
         raise ValueError(f"distill: ids and values [{T}, K], K at most {DISTILL_MAX_K}, not {list(ids.shape)} and {list(values.shape)}")
     if ids.dtype not in (torch.int32, torch.int64) or values.dtype not in (torch.float32, BF16, torch.float16):
