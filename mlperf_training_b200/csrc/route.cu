@@ -149,8 +149,8 @@ B200_DEVICE bool keep_group(R v, int G, int top, int sub, int lane, R& gap) {
   gap = in - out;
   return g < G && rank < top;
 }
-// The same for positive fp32 values in `g` < G, by warp-wide maxima of keys that hold the group below 27 bits of its value (what they cut, 2^-19
-// of values below 4, is in the gap).
+// The same for positive fp32 values below 4 in `g` < G, by warp-wide maxima of keys that hold the group below 27 bits of its value (what they cut, 31
+// units of 2^-22, is in the gap).
 B200_DEVICE bool keep_group(float v, int G, int top, int g, float& gap) {
   unsigned key = g < G ? (__float_as_uint(v) & ~31u) | (31u - (unsigned)g) : 0u;
   unsigned last = 0u;
@@ -160,7 +160,7 @@ B200_DEVICE bool keep_group(float v, int G, int top, int g, float& gap) {
     if (key == last) { keep = true; key = 0u; }
   }
   const unsigned next = __reduce_max_sync(ALL, key);
-  gap = __uint_as_float(last & ~31u) - __uint_as_float(next & ~31u) - 0x1p-18f;
+  gap = __uint_as_float(last & ~31u) - __uint_as_float(next & ~31u) - 0x1p-17f;
   return keep;
 }
 // The same from c in shared memory, for groups that are not whole lanes: bit g * sub of the result, group g stays.
