@@ -11,7 +11,7 @@
 // experts' keys sorted.  Where neighbours in the order (the best one left out and groups included) lie closer than the error
 // of what was compared, the token goes through the same steps in fp64 (`choose_exact`; normal logits: 0.1 % of the tokens of 256 experts with
 // sigmoid scores, 1 % with softmax).  Without a bias the order is that of the logits: their upper 24 bits are the key, exact for bf16,
-// and neighbours that agree in them but not in the rest go to `choose_exact`.
+// and where neighbours (at the border of the choice: any that have its key) agree in them but not in the rest, the token goes to `choose_exact`.
 // 65536 tokens, 256 experts in 8 groups, k 8, bf16: 67 us (33 MB in); with a scan for the maximum over unsorted fp32 values, an owner's
 // ballot and a shuffle a round 203.
 #include "common.cuh"
@@ -375,6 +375,14 @@ __global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const __grid_const
         // equal in 24 bits: equal logits are in order as they are
         const float mv = to_float(row[min(at, p.E - 1)]), nv = to_float(row[min(255 - (int)(next & 255u), p.E - 1)]);
         close = close && !(mv == nv || (mv != mv && nv != nv));
+        if (sizeof(TL) == 4 && (__shfl_sync(ALL, mine, p.k - 1) ^ top) < 256u) {
+          // the last of the choice and the best one left out agree in 24 bits: so may others that are left out, and be larger
+          const float v = to_float(row[255 - (int)(top & 255u)]);
+          for (int i = 0; i < NPL && e0 + i < p.E; ++i) {
+            const float u = to_float(row[e0 + i]);
+            close |= ((key_of(u) ^ top) & 0xffffff00u) == 0u && !(u == v || (u != u && v != v));
+          }
+        }
       }
       exact |= __any_sync(ALL, close);
     }
