@@ -44,9 +44,9 @@ B200_DEVICE void from_float(__nv_bfloat16& o, float v) { o = __float2bfloat16(v)
 template <typename TL, int N>
 struct alignas(N * sizeof(TL) < 16 ? N * sizeof(TL) : 16) Pack { TL v[N]; };
 
-// Order-preserving unsigned key of a float (NaN: as -inf).
+// Order-preserving unsigned key of a float (NaN: as -inf, -0: as 0).
 B200_DEVICE unsigned key_of(float v) {
-  const int u = __float_as_int(fmaxf(v, -INFINITY));
+  const int u = __float_as_int(fmaxf(v, -INFINITY) + 0.f);
   return (unsigned)(u ^ ((u >> 31) | (int)0x80000000));          // -inf: 0x007fffff
 }
 B200_DEVICE float fma_sat(float a, float b, float c) {            // NaN: 0
