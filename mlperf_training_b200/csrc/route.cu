@@ -131,8 +131,15 @@ struct Two {
     add(a2);
     b = b < b2 ? b2 : b;
   }
-  B200_DEVICE R value(int n) const { return n > 1 ? a + b : a; }
+  B200_DEVICE R value(int n) const {       // (an expert at +inf and one at -inf: as -inf)
+    const R v = n > 1 ? a + b : a;
+    return v == v ? v : -INFINITY;
+  }
 };
+// Whether a group's two best in fixed point are what their sum does not hold: one at -inf, or the first at +inf (see route_kernel's u).
+constexpr float OFF = 1.f + 0x1p-21f, ON = 2.f - 0x1p-20f;
+B200_DEVICE bool infinite(const Two<float>& t, int n) { return n > 1 && (t.b <= OFF || t.a >= ON); }
+B200_DEVICE bool infinite(const Two<double>&, int) { return false; }       // (64 bits hold them)
 
 // Whether this lane's group stays.  Groups are `sub` lanes each, in order; `v` is the group's value in all of them.  gap: between the worst that
 // stays and the best that does not.
@@ -165,7 +172,7 @@ B200_DEVICE bool keep_group(float v, int G, int top, int g, float& gap) {
 }
 // The same from c in shared memory, for groups that are not whole lanes: bit g * sub of the result, group g stays.
 template <typename R>
-B200_DEVICE unsigned keep_groups(const R* c, int E, int G, int top, int lane, int& sub, R& gap) {
+B200_DEVICE unsigned keep_groups(const R* c, int E, int G, int top, int lane, int& sub, R& gap, bool& odd) {
   int gp = 1;
   while (gp < G) gp *= 2;
   sub = 32 / gp;
@@ -174,6 +181,7 @@ B200_DEVICE unsigned keep_groups(const R* c, int E, int G, int top, int lane, in
   if (g < G)
     for (int i = lane % sub; i < n; i += sub) t.add(c[g * n + i]);
   for (int o = sub / 2; o > 0; o >>= 1) t.join(o);
+  odd = __any_sync(ALL, g < G && infinite(t, n));
   const bool keep = keep_group<R>(t.value(n), G, top, sub, lane, gap);
   return __ballot_sync(ALL, keep && lane % sub == 0);
 }
@@ -198,7 +206,8 @@ __device__ __noinline__ int choose_exact(const TL* row, const RouteParams& p, do
   unsigned groups = ALL;
   int sub = 1;
   double gap;
-  if (p.top < p.G) groups = keep_groups<double>(c, p.E, p.G, p.top, lane, sub, gap);
+  bool odd;
+  if (p.top < p.G) groups = keep_groups<double>(c, p.E, p.G, p.top, lane, sub, gap, odd);
   if (p.bias == nullptr) {                 // the order of the experts is that of the logits
     __syncwarp();
     for (int e = lane; e < p.E; e += 32) {
@@ -268,7 +277,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const __grid_const
   // Groups of whole lanes, a power of two of them, are reduced in registers.
   const int lanes = n / NPL;
   const bool by_lanes = n % NPL == 0 && (lanes & (lanes - 1)) == 0;
-  // u = a c + b lies in (0, 1); t = 1 + 2^-22 + u (1 - 2^-20) in [1, 2): the fixed point is its mantissa
+  // u = a c + b lies in [2^-20, 1 - 2^-20], and is 0 or 1 for an infinite c; t = 1 + 2^-22 + u (1 - 2^-20) in [1, 2): the fixed point is its mantissa
   float bias[NPL];
   float least = INFINITY, most = -INFINITY, largest = 0.f;       // of the finite biases
 #pragma unroll
@@ -326,11 +335,13 @@ __global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const __grid_const
     }
     if (grouped) {
       float gap;
+      bool odd;
       if (by_lanes) {
         Two<float> two;
 #pragma unroll
         for (int i = 0; i < NPL; ++i) two.add(c[i]);
         for (int o = lanes / 2; o > 0; o >>= 1) two.join(o);
+        odd = __any_sync(ALL, lane / lanes < p.G && infinite(two, n));
         const bool keep = keep_group(two.value(n), p.G, p.top, lane / lanes, gap);
 #pragma unroll
         for (int i = 0; i < NPL; ++i) key[i] = keep ? key[i] : 0u;
@@ -340,13 +351,13 @@ __global__ void __launch_bounds__(WARPS * 32, 4) route_kernel(const __grid_const
           if (e0 + i < p.E) sc[e0 + i] = c[i];
         __syncwarp();
         int sub;
-        const unsigned groups = keep_groups<float>(sc, p.E, p.G, p.top, lane, sub, gap);
+        const unsigned groups = keep_groups<float>(sc, p.E, p.G, p.top, lane, sub, gap, odd);
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
           if (e0 + i < p.E && !(groups >> ((e0 + i) / n * sub) & 1)) key[i] = 0u;
       }
-      exact = gap < 4.f * near;
+      exact = odd || gap < 4.f * near;
     }
     sort_down<NPL>(key);
     // the k largest keys of the warp, and the next one for the gap to it; lane j keeps the j-th.  A lane's keys behind its first wait in

@@ -124,6 +124,7 @@ def route_fwd(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: tor
         by = torch.where(by.isnan(), lost, by)
         if top_groups < groups:
             pair = by.unflatten(1, (groups, E // groups)).sort(-1, descending=True)[0][..., :2].sum(-1)
+            pair = torch.where(pair.isnan(), lost, pair)            # (an expert at +inf and one at -inf)
             kept = torch.zeros(T, groups, dtype=torch.bool).scatter_(1, pair.sort(dim=-1, descending=True, stable=True)[1][:, :top_groups], True)
             out = ~kept.repeat_interleave(E // groups, 1)
             by = x if bias is None else by
@@ -377,7 +378,7 @@ def route(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.T
 
     The scores are ``softmax`` over all experts or ``sigmoid``.  Experts are chosen by score + ``bias`` (fp32 ``[E]``, without a gradient: a
     balance bias, or -inf for an expert that gets nothing), largest first, ties to the lower index.  With ``groups`` the experts lie in that
-    many equal groups and only the ``top_groups`` with the largest sum of their two best take part.  The weights are the scores of the chosen, without
+    many equal groups and only the ``top_groups`` with the largest sum of their two best take part (-inf where the second best is off).  The weights are the scores of the chosen, without
     the bias, divided by their sum (``renormalize``) and times ``scale``.  Comparisons hold in 64 bits, NaN counts as -inf; without a bias
     experts are compared by their logits.  ``idx``, ``w`` and ``counts`` go into ``moe_experts`` like those of ``router_topk``, which is
     ``softmax`` with ``renormalize`` for few experts chosen by their logits."""
