@@ -40,18 +40,25 @@ struct ScoreParams {
   float into, back;         // with a cap: what takes a product into the tangent, c log2(e)
   float limit, k[5];        // products up to `limit` in size: back * tanh(into * s) = s * (k0 + k1 s^2 + .. + k4 s^8)
 
-  // tanh(x) for |x| <= 1 is x times a polynomial in x^2, fitted to the smallest largest relative error there (7e-6: 3.5e-4 of a score capped at
-  // 50); the coefficients take the scales in.  A capped score would otherwise take an exponential and a reciprocal more, and the
-  // softmax warps are bound by the MUFU unit as it is.
+  // tanh(x) for |x| <= 1 is x times a polynomial in x^2, fitted to the smallest largest relative error there (7e-6); the coefficients take the
+  // scales in.  A capped score would otherwise take an exponential and a reciprocal more, and the softmax warps are bound by the MUFU
+  // unit as it is.  It serves scores of up to 64 (an error of 4.5e-4 there, a tenth of what P loses to bf16); larger ones, which only larger
+  // caps let through, and those of scales whose powers fp32 does not hold go through capped_any2.
   static ScoreParams of(float scale, float cap, const float* slopes) {
     ScoreParams p = {scale, cap, slopes, 0.f, 0.f, 0.f, {0.f, 0.f, 0.f, 0.f, 0.f}};
     if (cap > 0.f) {
       const double c[5] = {0.99999309, -0.33298064, 0.13036807, -0.04481748, 0.00903639}, into = (double)scale / cap, back = cap * 1.4426950408889634;
-      p.into = (float)into;
+      p.into = (float)(into < 1e38 ? into : 1e38);
       p.back = (float)back;
-      double w = back * into;
-      for (int i = 0; i < 5; ++i, w *= into * into) p.k[i] = (float)(c[i] * w);
-      p.limit = into > 1e-4 && into < 1e3 ? (float)(1. / into) : 0.f;      // (powers of the scales that fp32 does not hold: never)
+      const double x = cap < 64.f ? 1. : 64. / cap, limit = x / into;      // the largest |into * s| and |s|
+      double w = back * into, share = 1.;                                  // of term i: its scales, and what it is of the first one at most
+      bool held = limit < 1e15;                                            // (its square)
+      for (int i = 0; i < 5; ++i, w *= into * into, share *= x * x) {
+        const double k = c[i] * w, size = k < 0. ? -k : k;
+        held &= size < 1e38 && (size > 1e-37 || share < 1e-9);
+        p.k[i] = size > 1e-37 ? (float)k : 0.f;
+      }
+      p.limit = held ? (float)limit : -1.f;
     }
     return p;
   }
@@ -66,12 +73,22 @@ B200_DEVICE float2 capped_small2(float2 s, const ScoreParams& p) {
   r = ffma2(r, q, make_float2(p.k[0], p.k[0]));
   return fmul2(r, s);
 }
-// tanh(x) = 1 - 2 / (1 + e^2x), absolute error below 3e-7
-B200_DEVICE float capped_any(float s, const ScoreParams& p) {
-  const float e = ex2_approx(s * p.into * (2.f * LOG2E));
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-  return p.back * fmaf(-2.f, r, 1.f);
+// tanh(x) = 1 - 2 / (1 + e^2x) from 1/2 on, and below, where that difference cancels, x times a polynomial in x^2 (fitted like the other, 1.3e-8):
+// relative error below 5e-7, so that a cap far above the scores leaves them what they are
+B200_DEVICE float2 capped_any2(float2 s, const ScoreParams& p) {
+  auto both = [](float v) { return make_float2(v, v); };
+  const float2 x = fmul2(s, both(p.into)), q = fmul2(x, x), y = fmul2(x, both(2.f * LOG2E)), d = fadd2(make_float2(ex2_approx(y.x), ex2_approx(y.y)), both(1.f));
+  float2 r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(d.y));
+  float2 t = ffma2(q, both(0.017135007f), both(-0.052986074f));
+  t = ffma2(t, q, both(0.13324779f));
+  t = ffma2(t, q, both(-0.33333069f));
+  t = fmul2(ffma2(t, q, both(1.f)), x);
+  r = ffma2(r, both(-2.f), both(1.f));
+  return fmul2(make_float2(fabsf(x.x) < 0.5f ? t.x : r.x, fabsf(x.y) < 0.5f ? t.y : r.y), both(p.back));
 }
+// Caps that the scales above hold in fp32, with their squares (0: none)
+inline bool cap_ok(float cap) { return cap == 0.f || (cap >= 1e-12f && cap <= 1e18f); }
 
 }  // namespace b200

@@ -324,7 +324,10 @@ attn_masked_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             }
           } else {
 #pragma unroll
-            for (int i = c * 32; i < c * 32 + 32; ++i) pr[i] = b200::capped_any(__uint_as_float(s[i]), p.score);
+            for (int i = c * 32; i < c * 32 + 32; i += 2) {
+              const float2 y = b200::capped_any2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), p.score);
+              pr[i] = y.x; pr[i + 1] = y.y;
+            }
           }
         }
 #pragma unroll
@@ -616,7 +619,7 @@ B200_API int b200_attn_masked_bwd(const void* q, const void* k, const void* v, c
   if (HD != 64 && HD != 128) return b200::fail(960, "attn_masked_bwd: head dim %d not supported (64 or 128)", HD);
   if (B < 1 || Sq < 1 || Skv < Sq || Hkv < 1 || Hq % Hkv != 0)
     return b200::fail(960, "attn_masked_bwd: B=%d, Sq=%d, Skv=%d, Hq=%d, Hkv=%d", B, Sq, Skv, Hq, Hkv);
-  if (!(scale > 0.f) || !(cap >= 0.f)) return b200::fail(960, "attn_masked_bwd: scale %g, cap %g", scale, cap);
+  if (!(scale > 0.f) || !b200::cap_ok(cap)) return b200::fail(960, "attn_masked_bwd: scale %g, cap %g", scale, cap);
   CUtensorMap m[7];
   int r;
   const long long o_row = (long long)Hq * HD, o_batch = o_row * Sq;

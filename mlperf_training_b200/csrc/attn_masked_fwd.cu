@@ -410,7 +410,10 @@ attn_masked_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
               }
             } else {
 #pragma unroll
-              for (int i = c * 32; i < c * 32 + 32; ++i) v[i] = __float_as_uint(b200::capped_any(__uint_as_float(v[i]), p.score));
+              for (int i = c * 32; i < c * 32 + 32; i += 2) {
+                const float2 y = b200::capped_any2(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), p.score);
+                v[i] = __float_as_uint(y.x); v[i + 1] = __float_as_uint(y.y);
+              }
             }
           }
         }
@@ -710,7 +713,7 @@ B200_API int b200_attn_masked_fwd(const void* q, const void* k, const void* v, v
   if (HD != 64 && HD != 128) return b200::fail(950, "attn_masked_fwd: head dim %d not supported (64 or 128)", HD);
   if (B < 1 || Sq < 1 || Skv < Sq || Hkv < 1 || Hq % Hkv != 0)
     return b200::fail(950, "attn_masked_fwd: B=%d, Sq=%d, Skv=%d, Hq=%d, Hkv=%d", B, Sq, Skv, Hq, Hkv);
-  if (!(scale > 0.f) || !(cap >= 0.f)) return b200::fail(950, "attn_masked_fwd: scale %g, cap %g", scale, cap);
+  if (!(scale > 0.f) || !b200::cap_ok(cap)) return b200::fail(950, "attn_masked_fwd: scale %g, cap %g", scale, cap);
   CUtensorMap m[5];
   int r;
   if ((r = b200::map_bshd(&m[0], q, HD, Hq, Sq, B, q_row, q_batch, BQ))) return r;

@@ -192,12 +192,20 @@ attn_masked_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       mma(s[1], qf[k], kf[2], kf[3]);
     }
     float mx[2] = {-INFINITY, -INFINITY};
+    if (capped)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const float2 y = b200::capped_any2(make_float2(s[t][e], s[t][e + 1]), p.score);
+          s[t][e] = y.x; s[t][e + 1] = y.y;
+        }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int kk = key + t * 8 + (lane & 3) * 2 + (e & 1), w = e >> 1;
-        float x = capped ? b200::capped_any(s[t][e], p.score) : s[t][e] * scale2;
+        float x = capped ? s[t][e] : s[t][e] * scale2;
         if (biased) x = fmaf(-slope[w], fabsf((float)(kk - pos[w])), x);
         if (masked && (kk < iv[w].x || kk >= iv[w].y)) x = -INFINITY;
         s[t][e] = x;
@@ -415,7 +423,7 @@ B200_API int b200_attn_masked_rows(const void* q, const void* k, const void* v, 
   if (HD != 64 && HD != 128) return b200::fail(970, "attn_masked_rows: head dim %d not supported (64 or 128)", HD);
   if (B < 1 || Sq < 1 || Skv < Sq || Hkv < 1 || Hq % Hkv != 0 || !b200_attn_masked_few_rows(B, Sq, Hq, Hkv))
     return b200::fail(970, "attn_masked_rows: B=%d, Sq=%d, Skv=%d, Hq=%d, Hkv=%d", B, Sq, Skv, Hq, Hkv);
-  if (!(scale > 0.f) || !(cap >= 0.f)) return b200::fail(970, "attn_masked_rows: scale %g, cap %g", scale, cap);
+  if (!(scale > 0.f) || !b200::cap_ok(cap)) return b200::fail(970, "attn_masked_rows: scale %g, cap %g", scale, cap);
   CUtensorMap tk, tv;
   int r;
   if ((r = b200::map_bshd(&tk, k, HD, Hkv, Skv, B, k_row, k_batch, KT))) return r;

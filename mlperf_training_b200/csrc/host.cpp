@@ -835,7 +835,7 @@ PyObject* py_masked_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
   Pitch pq, pk, pv;
   if (B != mb || Sq != mq || Skv != mk || k->size(0) != B || k->size(3) != D || (D != 64 && D != 128) || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 ||
       !bshd(*q, pq) || !bshd(*k, pk) || !bshd(*v, pv) || !((float)scale > 0.f && (float)scale < INFINITY) ||
-      !((float)softcap >= 0.f && (float)softcap < INFINITY) || m->scalar_type() != at::kInt || !m->is_contiguous())
+      !(softcap == 0.0 || (softcap >= 1e-12 && softcap <= 1e18)) || m->scalar_type() != at::kInt || !m->is_contiguous())
     Py_RETURN_NONE;
   if (sl.defined() && (sl.device() != q->device() || sl.scalar_type() != at::kFloat || sl.dim() != 1 || sl.size(0) != Hq || !sl.is_contiguous()))
     Py_RETURN_NONE;

@@ -15,6 +15,7 @@ from . import _lib
 from ._lib import call, ptr, stream_ptr, use_kernels
 
 HEAD_DIMS = (64, 128)
+SOFTCAPS = (1e-12, 1e18)        # whose squares fp32 holds
 
 
 @dataclass
@@ -121,8 +122,8 @@ def _check(q, k, v, mask, scale, softcap, slopes, sink) -> None:
         raise ValueError(f"masked_attention: q, k, v of one type on one device, not {q.dtype}, {k.dtype}, {v.dtype} on {q.device}, {k.device}, {v.device}")
     if q.is_cuda and (q.dtype != torch.bfloat16 or D not in HEAD_DIMS):
         raise ValueError(f"masked_attention: bf16 with head dim 64 or 128, not {q.dtype} with {D}")
-    if not (0.0 < scale < math.inf and 0.0 <= softcap < math.inf):
-        raise ValueError(f"masked_attention: scale {scale} (above 0), softcap {softcap} (0: none)")
+    if not (0.0 < scale < math.inf and (softcap == 0.0 or SOFTCAPS[0] <= softcap <= SOFTCAPS[1])):
+        raise ValueError(f"masked_attention: scale {scale} (above 0), softcap {softcap} (0: none, else {SOFTCAPS[0]} to {SOFTCAPS[1]})")
     for name, t in (("slopes", slopes), ("sink", sink)):
         if t is not None and (t.shape != (Hq,) or t.device != q.device or not t.is_floating_point()):
             raise ValueError(f"masked_attention: {name} [{Hq}] on {q.device}, not {list(t.shape)} in {t.dtype} on {t.device}")
