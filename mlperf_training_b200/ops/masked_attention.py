@@ -243,6 +243,7 @@ def masked_attention_bwd(dout, q, k, v, out, low, lse, mask: AttentionMask, *, s
         dv.copy_(wv)
     dsink = None
     if sink is not None:
-        # of the extra column, which carries no value: -sum over rows of its probability times delta
-        dsink = -(torch.exp(sink.detach().float().view(1, Hq, 1) - lse) * delta).sum(dim=(0, 2))
+        # of the extra column, which carries no value: -sum over rows of its probability times delta (0 where the row has neither a key nor a sink)
+        at = sink.detach().float().view(1, Hq, 1)
+        dsink = -(torch.where(at == -math.inf, 0.0, torch.exp(at - lse)) * delta).sum(dim=(0, 2))
     return dq, dk, dv, dsink
