@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import json
 import re
+import warnings
 from pathlib import Path
 
 import torch
@@ -38,6 +39,7 @@ _BLOCK_MAP = {
     "mlp.w_gate_up": "mlp.linear_fc1.weight",
     "mlp.w_down": "mlp.linear_fc2.weight",
     "mlp.router": "mlp.router.weight",
+    "mlp.router_bias": "mlp.router.expert_bias",
     "mlp.w1": "mlp.experts.linear_fc1.weight",
     "mlp.w2": "mlp.experts.linear_fc2.weight",
     "lora_qkv.a": "self_attention.linear_qkv.adapter.linear_in.weight",
@@ -121,8 +123,21 @@ def global_named_parameters(model):
     if stages is None:
         yield from model.named_parameters()
         return
+    yield from _of_stages(stages, lambda stage: stage.named_parameters())
+
+
+def global_named_tensors(model):
+    """Parameters, then the routers' balance biases (buffers), as ``global_named_parameters`` names them: what a checkpoint holds."""
+    def biases(m):
+        return ((n, b) for n, b in m.named_buffers() if n.endswith(".router_bias"))
+    yield from global_named_parameters(model)
+    stages = _stages_of(model)
+    yield from biases(model) if stages is None else _of_stages(stages, biases)
+
+
+def _of_stages(stages, named):
     for _, stage in stages:
-        for name, p in stage.named_parameters():
+        for name, p in named(stage):
             parts = name.split(".")
             if parts[0] == "blocks":
                 parts[1] = str(stage.layers[int(parts[1])])
@@ -196,7 +211,7 @@ def to_megatron_state(model: GPT, tp_group=None) -> dict[str, torch.Tensor]:
     cfg = model_config_of(model)
     ep_group = _ep_group_of(model) if isinstance(model, torch.nn.Module) else None
     out = {}
-    for name, p in global_named_parameters(model):
+    for name, p in global_named_tensors(model):
         t = _full_tensor(p, cfg, tp_group, ep_group)
         if name.endswith("w_qkv") or name.endswith("lora_qkv.b"):
             t = qkv_to_megatron(t, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim)
@@ -215,7 +230,7 @@ def sharded_megatron_state(model: GPT, tp_group) -> dict:
     cfg = model_config_of(model)
     ep_group = _ep_group_of(model) if isinstance(model, torch.nn.Module) else None
     out = {}
-    for name, p in global_named_parameters(model):
+    for name, p in global_named_tensors(model):
         key = megatron_name(name, moe_pre_norm=cfg.n_experts > 0)
         shard = getattr(p, "tensor_parallel", None)
         t = p.detach()
@@ -275,6 +290,8 @@ def _load_named(named, state: dict[str, torch.Tensor], cfg: GPTConfig) -> list[s
             key = megatron_name(name, moe_pre_norm=cfg.n_experts > 0)
             if key not in state:
                 missing.append(name)
+                if name.endswith(".router_bias"):
+                    p.zero_()
                 continue
             t = state[key]
             if name.endswith("w_qkv") or name.endswith("lora_qkv.b"):
@@ -294,10 +311,20 @@ def _load_named(named, state: dict[str, torch.Tensor], cfg: GPTConfig) -> list[s
 def load_megatron_state(model: GPT, state: dict[str, torch.Tensor], strict: bool = True) -> list[str]:
     """Copy a (Megatron-named) state dict into ``model``.  Returns the model parameters that were
     not found (e.g. freshly initialised LoRA adapters when loading a base checkpoint)."""
-    missing = _load_named(list(global_named_parameters(model)), state, model_config_of(model))
-    if strict and any("lora" not in m for m in missing):
-        raise KeyError(f"checkpoint lacks parameters: {[m for m in missing if 'lora' not in m]}")
+    named = list(global_named_tensors(model))
+    missing = _load_named(named, state, model_config_of(model))
+    _check_loaded(named, missing, state, strict)
     return missing
+
+
+def _check_loaded(named, missing, present, strict: bool) -> None:
+    """Raises for parameters without an entry, but for adapters; balance biases without one start at 0.  Warns of biases that the model has no
+    place for (it routes without them)."""
+    lost = [m for m in missing if "lora" not in m and not m.endswith(".router_bias")]
+    if strict and lost:
+        raise KeyError(f"checkpoint lacks parameters: {lost}")
+    if any(k.endswith(_BLOCK_MAP["mlp.router_bias"]) for k in present) and not any(n.endswith(".router_bias") for n, _ in named):
+        warnings.warn("the checkpoint's routers have a balance bias and the model's do not (router_bias_rate): it is left out", stacklevel=3)
 
 
 def save_torch_dist(model: GPT, root: str, iteration: int = 0, extra_common: dict | None = None,
@@ -351,7 +378,7 @@ def load_torch_dist(model: GPT, root: str, iteration: int | None = None, strict:
     present = set(reader.read_metadata().state_dict_metadata.keys())
     # full-shape destinations, read and consumed a group of keys at a time (a tensor-parallel rank keeps
     # only its slice of each, so the full tensors of the whole model never sit in memory together)
-    named = list(global_named_parameters(model))
+    named = list(global_named_tensors(model))
     sharded = any(getattr(p, "tensor_parallel", None) is not None or getattr(p, "expert_shard", None) is not None for _, p in named)
     per_group = 16 if sharded else len(named)
     missing = []
@@ -365,6 +392,5 @@ def load_torch_dist(model: GPT, root: str, iteration: int | None = None, strict:
         if want:
             dcp.load(want, checkpoint_id=str(d))
         missing += _load_named(group, {k[len("model."):]: v for k, v in want.items()}, cfg)
-    if strict and any("lora" not in m for m in missing):
-        raise KeyError(f"checkpoint lacks parameters: {[m for m in missing if 'lora' not in m]}")
+    _check_loaded(named, missing, present, strict)
     return {"iteration": iteration, "missing": missing, "common": common}

@@ -38,9 +38,10 @@ class MoEMLP(nn.Module):
             self.w1.expert_shard = self.w2.expert_shard = (self.ep, self.ep_rank)
         self.dispatcher = ExpertParallelDispatcher(ep_group, E) if self.ep > 1 else None
         self.ep_comm = ep_comm
-        # a balance bias selects experts beside their scores; the load since its last step is counted while gradients are on
+        # a balance bias selects experts beside their scores (and goes where the parameters go); the load since its last step is counted while
+        # gradients are on
         balanced = cfg.router_bias_rate > 0
-        self.register_buffer("router_bias", torch.zeros(E, dtype=torch.float32, device=device) if balanced else None, persistent=False)
+        self.register_buffer("router_bias", torch.zeros(E, dtype=torch.float32, device=device) if balanced else None)
         self.register_buffer("router_load", torch.zeros(E, dtype=torch.int32, device=device) if balanced else None, persistent=False)
         self._fused = None      # built on first use: its slab size depends on the number of tokens per step
 
