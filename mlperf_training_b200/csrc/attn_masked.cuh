@@ -88,6 +88,10 @@ B200_DEVICE float2 capped_any2(float2 s, const ScoreParams& p) {
   r = ffma2(r, both(-2.f), both(1.f));
   return fmul2(make_float2(fabsf(x.x) < 0.5f ? t.x : r.x, fabsf(x.y) < 0.5f ? t.y : r.y), both(p.back));
 }
+// Sizes that a kernel can have; what is computed from others (sums to divide by) may be 0.
+inline bool sizes_ok(int B, int Sq, int Skv, int Hq, int Hkv) {
+  return B >= 1 && Sq >= 1 && Skv >= Sq && Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0;
+}
 // Caps that the scales above hold in fp32, with their squares (0: none)
 inline bool cap_ok(float cap) { return cap == 0.f || (cap >= 1e-12f && cap <= 1e18f); }
 

@@ -604,6 +604,7 @@ int parts_of(int B, int Sq, int Skv, int Hq, int Hkv) {
 
 // bytes of the sums that CTAs sharing a key tile leave (0: every tile has one)
 B200_API long long b200_attn_masked_bwd_workspace(int B, int Sq, int Skv, int Hq, int Hkv, int HD) {
+  if (!b200::sizes_ok(B, Sq, Skv, Hq, Hkv)) return 0;
   const long long tiles = (long long)B * Hkv * ((Skv + BKV - 1) / BKV);
   const int parts = parts_of(B, Sq, Skv, Hq, Hkv);
   return parts > 1 ? tiles * parts * 2 * BKV * HD * 4 : 0;
@@ -617,7 +618,7 @@ B200_API int b200_attn_masked_bwd(const void* q, const void* k, const void* v, c
                                   long long q_batch, long long k_batch, long long v_batch, long long dk_batch, long long dv_batch, float scale,
                                   float cap, void* workspace, long long workspace_bytes, void* stream) {
   if (HD != 64 && HD != 128) return b200::fail(960, "attn_masked_bwd: head dim %d not supported (64 or 128)", HD);
-  if (B < 1 || Sq < 1 || Skv < Sq || Hkv < 1 || Hq % Hkv != 0)
+  if (!b200::sizes_ok(B, Sq, Skv, Hq, Hkv))
     return b200::fail(960, "attn_masked_bwd: B=%d, Sq=%d, Skv=%d, Hq=%d, Hkv=%d", B, Sq, Skv, Hq, Hkv);
   if (!(scale > 0.f) || !b200::cap_ok(cap)) return b200::fail(960, "attn_masked_bwd: scale %g, cap %g", scale, cap);
   CUtensorMap m[7];

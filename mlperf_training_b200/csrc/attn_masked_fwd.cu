@@ -700,7 +700,7 @@ int launch_fwd(int score, const CUtensorMap* m, const FwdParams& p, cudaStream_t
 
 // bytes of the sums that parts of the key tiles leave (0: the key tiles are not parted)
 B200_API long long b200_attn_masked_fwd_workspace(int B, int Sq, int Skv, int Hq, int HD) {
-  const int parts = fwd_parts(B, Sq, Skv, Hq, HD);
+  const int parts = b200::sizes_ok(B, Sq, Skv, Hq, 1) ? fwd_parts(B, Sq, Skv, Hq, HD) : 1;
   return parts > 1 ? (long long)B * Sq * Hq * parts * (HD * 4 + 16) : 0;
 }
 
@@ -711,7 +711,7 @@ B200_API int b200_attn_masked_fwd(const void* q, const void* k, const void* v, v
                                   long long k_row, long long v_row, long long q_batch, long long k_batch, long long v_batch, float scale,
                                   float cap, void* workspace, long long workspace_bytes, void* stream) {
   if (HD != 64 && HD != 128) return b200::fail(950, "attn_masked_fwd: head dim %d not supported (64 or 128)", HD);
-  if (B < 1 || Sq < 1 || Skv < Sq || Hkv < 1 || Hq % Hkv != 0)
+  if (!b200::sizes_ok(B, Sq, Skv, Hq, Hkv))
     return b200::fail(950, "attn_masked_fwd: B=%d, Sq=%d, Skv=%d, Hq=%d, Hkv=%d", B, Sq, Skv, Hq, Hkv);
   if (!(scale > 0.f) || !b200::cap_ok(cap)) return b200::fail(950, "attn_masked_fwd: scale %g, cap %g", scale, cap);
   CUtensorMap m[5];

@@ -407,10 +407,11 @@ int launch_rows(const CUtensorMap& tk, const CUtensorMap& tv, const RowsParams& 
 
 // Whether a forward pass without a backward one takes the kernel of few rows: up to 64 of them a key head.
 B200_API int b200_attn_masked_few_rows(int B, int Sq, int Hq, int Hkv) {
-  return Hkv > 0 && B <= 65535 && (long long)(Hq / Hkv) * Sq <= 64 && (long long)Hkv * 4 <= 65535 ? 1 : 0;
+  return b200::sizes_ok(B, Sq, Sq, Hq, Hkv) && B <= 65535 && (long long)(Hq / Hkv) * Sq <= 64 && (long long)Hkv * 4 <= 65535 ? 1 : 0;
 }
 // bytes of workspace (0: none)
 B200_API long long b200_attn_masked_rows_workspace(int B, int Sq, int Skv, int Hq, int Hkv, int HD) {
+  if (!b200::sizes_ok(B, Sq, Skv, Hq, Hkv)) return 0;
   const Splits s = splits_of(B, Sq, Skv, Hq, Hkv);
   return s.n > 1 && !s.cluster ? (long long)B * Sq * Hq * s.n * (HD * 4 + 8) : 0;
 }
@@ -421,7 +422,7 @@ B200_API int b200_attn_masked_rows(const void* q, const void* k, const void* v, 
                                    long long v_row, long long q_batch, long long k_batch, long long v_batch, float scale, float cap,
                                    void* workspace, long long workspace_bytes, void* stream) {
   if (HD != 64 && HD != 128) return b200::fail(970, "attn_masked_rows: head dim %d not supported (64 or 128)", HD);
-  if (B < 1 || Sq < 1 || Skv < Sq || Hkv < 1 || Hq % Hkv != 0 || !b200_attn_masked_few_rows(B, Sq, Hq, Hkv))
+  if (!b200::sizes_ok(B, Sq, Skv, Hq, Hkv) || !b200_attn_masked_few_rows(B, Sq, Hq, Hkv))
     return b200::fail(970, "attn_masked_rows: B=%d, Sq=%d, Skv=%d, Hq=%d, Hkv=%d", B, Sq, Skv, Hq, Hkv);
   if (!(scale > 0.f) || !b200::cap_ok(cap)) return b200::fail(970, "attn_masked_rows: scale %g, cap %g", scale, cap);
   CUtensorMap tk, tv;

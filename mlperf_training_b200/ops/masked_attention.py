@@ -84,7 +84,7 @@ def attention_mask(B: int, Sq: int, Skv: int | None = None, *, causal: bool = Tr
         buf = _lib.host.attention_mask(documents, prefix, B, Sq, Skv, int(causal), window, dev.index)
         if buf is not None:
             return AttentionMask(B, Sq, Skv, dev, buf=buf)
-    if B < 1 or Sq < 1 or Skv < Sq or Skv > 2 ** 30:
+    if not 1 <= B <= 2 ** 30 or Sq < 1 or Skv < Sq or Skv > 2 ** 30:
         raise ValueError(f"attention_mask: {B} sequences, {Sq} queries at the end of {Skv} positions (at least one of each)")
     if not 0 <= window < 2 ** 30:
         raise ValueError(f"attention_mask: window {window}")
