@@ -297,6 +297,7 @@ attn_masked_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     if (p.splits == 1) {
       finish_row<HD>(p, at, acc, mw, lw, lane);
     } else if (p.cluster) {                                    // (in the first warp's part: the row is this warp's alone)
+      __syncwarp();                                            // its sums have been read by all lanes
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) reinterpret_cast<float*>(smem)[rr * (HD + 4) + c * 32 + lane] = acc[c];
       if (lane == 0) s_ml[rr] = make_float2(mw, lw);
