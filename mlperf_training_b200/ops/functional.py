@@ -625,7 +625,7 @@ class MaskedAttentionFn(Function):
 
 def masked_attention(q, k, v, mask, *, softcap=0.0, slopes=None, sink=None, scale=None):
     """Attention of ``q [B, Sq, Hq, D]`` over ``k``, ``v`` ``[B, Skv, Hkv, D]`` (bf16, D 64 or 128 on the GPU; any strides) under ``mask``, made by
-    ``attention_mask`` for (B, Sq, Skv).  A score is ``scale`` times the product; ``softcap`` makes it ``softcap * tanh(score / softcap)``;
+    ``attention_mask`` for (B, Sq, Skv).  A score is ``scale`` times the product; ``softcap`` (0: none) makes it ``softcap * tanh(score / softcap)``;
     ``slopes [Hq]`` (constants) take ``slope * |distance|`` from it; ``sink [Hq]`` adds a logit without a value to each row.  Rows that
     see nothing give 0 and get no gradient.  Values of padding may be anything in the forward pass; the backward pass wants finite
     inputs everywhere."""
